@@ -331,6 +331,59 @@ int vrwkv_qshift_mix_bwd_add(const void* x, const float* mix, const void* const*
 int vrwkv_groupnorm_gate_bwd_like(const void* y, const void* gate, const void* gn_weight, const void* gn_bias, const void* gout, void* gy, void* ggate, void* gparam, long long rows, int C, int group, float eps, int y_dtype, int io_dtype, void* workspace, size_t workspace_bytes, void* hip_stream);
 int vrwkv_biwkv_bwd_like(const float* w, const float* u, const void* k, const void* v, const void* gy, void* gw, void* gu, void* gk, void* gv, int B, int T, int C, int io_dtype, void* workspace, size_t workspace_bytes, void* hip_stream);
 
+/* ---- attention with a decay for each head: causal, with its state in and out (no counterpart in the reference) ----
+ * S_t = exp(g_t) S_{t-1} + k_t v_t^T, y_t = scale S_t^T q_t for every sequence and head.
+ * q: rows of Hq heads of Dk, k: Hk of Dk, v: Hv of Dv channels, all of dtype, channels side by side, any strides (in elements) for batch, token and
+ * head; head h of the H reads head h / (H / Hq) of q, and so on.  g: log decays of g_dtype at strides of batch, token and head (0 for a decay that all
+ * tokens share); below -200 (-inf) they count as -200, whose exponential is zero in fp32 as well; above 0 they make states grow.  Head sizes 1 to 128; each of Hq, Hk, Hv divides H.
+ * N rows of T tokens; or with offsets (N + 1 of them, 32 or 64 bits, on the device) N sequences packed in T rows, n at rows offsets[n] to offsets[n + 1],
+ * in ascending order, empty ones among them; strides of batch are not looked at.  Offsets outside 0..T are taken as 0 or T.
+ * state: the states in front of the first tokens, (N, H, Dk, Dv) contiguous fp32, or NULL: zeros.  last: those behind the last tokens, or NULL.
+ * y (batch, T, H, Dv) of dtype, contiguous; packed rows of no sequence get zeros.  States and sums are fp32.
+ * y of a token is formed with the tokens of its chunk (64 or 32 from the sequence's front on): an infinity or NaN in k or v there may reach it from
+ * behind; nothing does from other sequences or from rows outside of them. */
+typedef struct vrwkv_decay_args {
+    const void *q, *k, *v, *g, *offsets;
+    const float* state;
+    void* y;
+    float* last;
+    const void* gy;                        /* backward: gradient of y, of dtype, at gy_stride */
+    const float* glast;                    /* ... of last, or NULL: zeros */
+    void *dq, *dk, *dv, *dg;               /* contiguous: (batch, T, Hq, Dk), (.., Hk, Dk), (.., Hv, Dv) of dtype; (batch, T, H) of g_dtype, or (H) with g_per_head; NULL: not wanted */
+    float* dstate;                         /* like state, or NULL */
+    long long q_stride[3], k_stride[3], v_stride[3], g_stride[3], gy_stride[3];
+    int N, T, H, Hq, Hk, Hv, Dk, Dv, dtype, g_dtype, g_per_head, offsets64;
+    float scale;
+    void* workspace;                       /* 16-byte aligned; the sizes go by the fields above and by which pointers are NULL */
+    size_t workspace_bytes;
+} vrwkv_decay_args;
+size_t vrwkv_decay_fwd_workspace_bytes(const vrwkv_decay_args* args);
+int vrwkv_decay_fwd(const vrwkv_decay_args* args, void* hip_stream);
+size_t vrwkv_decay_bwd_workspace_bytes(const vrwkv_decay_args* args);
+int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream);
+
+/* One more token for each of N rows, whose states are pages slots[n] of a pool (P pages of H x Dk x Dv contiguous fp32 numbers, page_stride apart),
+ * updated in place; slots (32 or 64 bits, on the device; NULL: 0, 1, ..).  Rows that name the same page are tokens behind each other, in their order.
+ * A row of slot -1 (a place of the batch that is not taken) gets zeros in y, of any other slot outside the pool NaN; neither touches a page.
+ * Strides of row and head; y (N, H, Dv) of dtype, contiguous. */
+typedef struct vrwkv_decay_step_args {
+    const void *q, *k, *v, *g, *slots;
+    float* pool;
+    void* y;
+    long long q_stride[2], k_stride[2], v_stride[2], g_stride[2], page_stride;
+    int N, P, H, Hq, Hk, Hv, Dk, Dv, dtype, g_dtype, slots64;
+    float scale;
+} vrwkv_decay_step_args;
+int vrwkv_decay_step(const vrwkv_decay_step_args* args, void* hip_stream);
+
+/* ---- pages of a pool copied: page to[i] = page from[i] of the source as it was before the call, for i < M <= 4096 ----
+ * The source is the pool itself (same pointer and stride), or another that does not overlap it; strides and sizes in bytes.  from[i] = -1: zeros;
+ * to[i] = -1: nothing; an entry with another index outside the pools is left out; of several entries with the same to the last counts.  Indices of 32 or
+ * 64 bits, on the device.  workspace: vrwkv_copy_pages_workspace_bytes(M) bytes, 4-byte aligned. */
+size_t vrwkv_copy_pages_workspace_bytes(int M);
+int vrwkv_copy_pages(void* pool, long long stride, int P, const void* source, long long source_stride, int source_P, long long page_bytes,
+                     const void* from, int from64, const void* to, int to64, int M, void* workspace, size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

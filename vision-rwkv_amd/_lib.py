@@ -47,6 +47,23 @@ class Block6Params(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in POINTERS] + [("fp32_vectors", ctypes.c_int)]
 
 
+class DecayArgs(ctypes.Structure):
+    """vrwkv_decay_args of include/vrwkv_hip.h."""
+    STRIDES = ("q_stride", "k_stride", "v_stride", "g_stride", "gy_stride")
+    POINTERS = ("q", "k", "v", "g", "offsets", "state", "y", "last", "gy", "glast", "dq", "dk", "dv", "dg", "dstate")
+    INTS = ("N", "T", "H", "Hq", "Hk", "Hv", "Dk", "Dv", "dtype", "g_dtype", "g_per_head", "offsets64")
+    _fields_ = ([(n, ctypes.c_void_p) for n in POINTERS] + [(n, ctypes.c_longlong * 3) for n in STRIDES] + [(n, ctypes.c_int) for n in INTS]
+                + [("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)])
+
+
+class DecayStepArgs(ctypes.Structure):
+    """vrwkv_decay_step_args of include/vrwkv_hip.h."""
+    POINTERS = ("q", "k", "v", "g", "slots", "pool", "y")
+    INTS = ("N", "P", "H", "Hq", "Hk", "Hv", "Dk", "Dv", "dtype", "g_dtype", "slots64")
+    _fields_ = ([(n, ctypes.c_void_p) for n in POINTERS] + [(n, ctypes.c_longlong * 2) for n in ("q_stride", "k_stride", "v_stride", "g_stride")]
+                + [("page_stride", ctypes.c_longlong)] + [(n, ctypes.c_int) for n in INTS] + [("scale", ctypes.c_float)])
+
+
 class VrwkvError(RuntimeError):
     """Non-zero status from the C ABI (mirrors the RuntimeError TORCH_CHECK raises at
     classification/mmcls_custom/models/backbones/cuda_new/bi_wkv.cpp:6-8)."""
@@ -211,6 +228,16 @@ def _declare(lib):
     lib.vrwkv_wgrad_group_workspace_bytes.restype = sz
     lib.vrwkv_wgrad_group.argtypes = [pv, pv, pv, pi, pi, pi, pi, i, i, i, vp, sz, vp]
     lib.vrwkv_wgrad_group.restype = i
+    for name in ("vrwkv_decay_fwd", "vrwkv_decay_bwd"):
+        getattr(lib, name).argtypes, getattr(lib, name).restype = [c.POINTER(DecayArgs), vp], i
+        size = getattr(lib, name + "_workspace_bytes")
+        size.argtypes, size.restype = [c.POINTER(DecayArgs)], sz
+    lib.vrwkv_decay_step.argtypes = [c.POINTER(DecayStepArgs), vp]
+    lib.vrwkv_decay_step.restype = i
+    lib.vrwkv_copy_pages_workspace_bytes.argtypes = [i]
+    lib.vrwkv_copy_pages_workspace_bytes.restype = sz
+    lib.vrwkv_copy_pages.argtypes = [vp, ll, i, vp, ll, i, ll, vp, i, vp, i, i, vp, sz, vp]
+    lib.vrwkv_copy_pages.restype = i
     for name in ("rowfuse_bwd", "qshift_mix_bwd", "groupnorm_gate_bwd", "biwkv_bwd"):
         like = getattr(lib, f"vrwkv_{name}_like")
         like.argtypes, like.restype = getattr(lib, f"vrwkv_{name}").argtypes, i

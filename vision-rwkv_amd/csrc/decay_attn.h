@@ -1,0 +1,712 @@
+// Attention whose state decays head by head (gfx950): for one head, with q, k (Dk), v, y (Dv), a log decay g and the state S (Dk, Dv),
+//     S_t = exp(g_t) S_{t-1} + k_t v_t^T,      y_t = scale S_t^T q_t.
+// A sequence goes in chunks of L tokens.  With G_t = the sum of g over the chunk's tokens up to t and S0 the state in front of the chunk,
+//     y_t = scale sum_{s<=t} exp(G_t - G_s) (q_t . k_s) v_s + scale exp(G_t) S0^T q_t,      S = exp(G_end) S0 + sum_s exp(G_end - G_s) k_s v_s^T,
+// four matrix products.  With a at the place of q, b of k and c of v this one kernel computes
+//     y  from a, b, c = q, k, v                       dq from gy, v, k            (along the tokens)
+//     dv from a, b, c = k, q, gy                      dk from v, gy, q            (back along them; a token's own decay then lies behind it),
+// since R_t = scale q_t gy_t^T + exp(g_{t+1}) R_{t+1} is a state of the same kind, dq_t = scale S_t gy_t, dk_t = R_t v_t, dv_t = R_t^T k_t.
+// The gradient of g_j is what crosses from tokens in front of j to j and behind: the sum over s < j <= t of the products' terms.  Inside a chunk those
+// are summed as they are, by one more product with a triangle of ones; what enters or leaves the chunk comes from S0's part of dq and R's part of dk; what
+// passes it whole is exp(G_end) <S0, R behind the chunk>, R kept for every chunk by the pass that makes dk.  Nothing cancels: q . dq - k . dk summed over the
+// tokens from j on is the same sum, with the difference of two large ones where little crosses.
+// Sequences of few calls are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
+#pragma once
+#include "wkv6_chunk_common.h"
+
+namespace vrwkv {
+namespace decay {
+
+using wkv6_detail::bf16x4;
+using wkv6_detail::bf16x8;
+using wkv6_detail::f32x4;
+using wkv6_detail::u32x4;
+
+constexpr int TZ = 64;                                    // columns of a state that a workgroup holds
+constexpr int THREADS = 256;
+
+// A tensor (batch, token, head, channel), channels side by side; head h of the call reads head h / share.  vec: rows in 16-byte pieces.
+struct View {
+    const void* p;
+    long long sb, st, sh;
+    int share, vec;
+};
+struct OutView {
+    void* p;
+    long long sb, st, sh;
+    int f32, vec;                                         // f32: fp32 values of every head, added up and rounded by a kernel behind
+};
+struct Role {
+    View a, b, c, e;
+    OutView o;
+    const float* init;                                    // states (N, H, Dk, Dv), or null: zeros
+    float* last;                                          // where the states behind the last token go, or null
+    float *seg, *seg_decay;                               // [segment][head][tile] a segment's state (first its own, then that in front of it), [segment][head]
+    float* edge;                                          // [tile][row][head]: what a token gives to the tokens outside its chunk (written with dk, read with dq)
+    float* anchors;                                       // [chunk][head][tile]: R behind each chunk, without the decay of the token behind it
+    float* dg;                                            // [tile][row][head]
+    long long sx, sz;                                     // strides of the states' contracted and other index
+    int dx, dz, tiles, reverse;
+    float s_in, s_upd;                                    // scale where the state is read; where it is written
+};
+struct Params {
+    const void *offsets, *g;
+    long long g_sb, g_st, g_sh;
+    long long rows;                                       // batch * T
+    int off64, g_dtype, N, T, H;                          // T: tokens of a row of the batch (packed: of all sequences)
+    int seg_len, nseg, segs;                              // tokens of a segment; segments of a row (0: packed); of the call
+    int n_roles;
+    float scale;
+    Role role[3];
+};
+template <typename IO> constexpr int in_terms = std::is_same<IO, float>::value ? 3 : std::is_same<IO, __half>::value ? 2 : 1;   // bf16 numbers that hold an element
+// tokens of a chunk: 64 where their rows and the state fit the LDS twice
+template <typename IO, int DX> constexpr int chunk_len = std::is_same<IO, __hip_bfloat16>::value || (std::is_same<IO, __half>::value && DX == 64) ? 64 : 32;
+
+// y and dv; dk with what dg needs of it; dq with dg; no outputs: a segment's own state; dk or dq without dg, the same bits as with it
+enum Mode { PLAIN = 0, EDGES = 1, FLOWS = 2, STATES = 3, ALONE = 4 };
+
+struct Place {                                            // a workgroup's segment
+    int n, first, len;                                    // sequence; its first token and length
+    int s0, s1;                                           // the segment's tokens, from the first
+    int base;                                             // batch row
+    int chunk0;                                           // number of the sequence's first chunk
+    bool is_last, is_first, valid;
+};
+__device__ __forceinline__ int offset_at(const Params& p, int n) {
+    const long long v = p.off64 ? static_cast<const long long*>(p.offsets)[n] : (long long)static_cast<const int*>(p.offsets)[n];
+    return (int)(v < 0 ? 0 : v > p.T ? p.T : v);
+}
+__device__ __forceinline__ Place sequence_place(const Params& p, int n, int L) {
+    Place w;
+    w.n = n;
+    w.valid = true;
+    if (p.nseg) {
+        w.first = 0;
+        w.len = p.T;
+        w.base = n;
+        w.chunk0 = n * ((p.T + L - 1) / L);
+    } else {
+        w.first = offset_at(p, n);
+        w.len = max(0, offset_at(p, n + 1) - w.first);
+        w.base = 0;
+        w.chunk0 = w.first / L + n;
+    }
+    return w;
+}
+// Packed sequences: n's segments have the numbers from first(n) / seg_len + n on, which grow with n and leave each its room whatever its length.
+__device__ __forceinline__ int first_segment(const Params& p, int n, int first) { return p.nseg ? n * p.nseg : first / p.seg_len + n; }
+__device__ __forceinline__ int segment_count(const Params& p, int len) { return max(1, (len + p.seg_len - 1) / p.seg_len); }
+
+__device__ __forceinline__ Place find_place(const Params& p, int gid, int L) {
+    int n;
+    if (p.nseg) n = gid / p.nseg;
+    else {
+        int seen = 0;
+        for (int m = 0; m < p.N; m += THREADS) {
+            const int i = m + threadIdx.x;
+            seen += __syncthreads_count(i < p.N && offset_at(p, min(i, p.N - 1)) / p.seg_len + i <= gid);
+        }
+        n = seen - 1;
+    }
+    if (n < 0) {
+        Place w{};
+        return w;
+    }
+    Place w = sequence_place(p, n, L);
+    const int j = gid - first_segment(p, n, w.first), count = segment_count(p, w.len);
+    w.valid = j >= 0 && j < count;
+    w.s0 = j * p.seg_len;
+    w.s1 = min(w.len, w.s0 + p.seg_len);
+    w.is_first = j == 0;
+    w.is_last = j == count - 1;
+    return w;
+}
+
+__device__ __forceinline__ float log_decay(const Params& p, int base, int token, int h) {
+    const long long i = base * p.g_sb + token * p.g_st + h * p.g_sh;
+    float x;
+    if (p.g_dtype == VRWKV_F32) x = static_cast<const float*>(p.g)[i];
+    else if (p.g_dtype == VRWKV_BF16) x = to_f32(static_cast<const __hip_bfloat16*>(p.g)[i]);
+    else x = to_f32(static_cast<const __half*>(p.g)[i]);
+    return x < -200.f ? -200.f : x;                       // (exp(-200) is zero in fp32 too; sums of -inf or the lowest value would be -inf, their differences NaN)
+}
+
+// The eight channels d .. d + 7 of a row of dim, zeros behind its end.
+template <typename IO> struct Piece { unsigned w[sizeof(IO) * 2]; };
+template <typename IO>
+__device__ __forceinline__ Piece<IO> load_piece(const IO* row, int d, int dim, bool inside, int vec) {
+    Piece<IO> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(IO) * 2; ++i) r.w[i] = 0;
+    if (!inside || d >= dim) return r;
+    if (vec && d + 8 <= dim) {
+        const u32x4* s = reinterpret_cast<const u32x4*>(row + d);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(IO) / 2; ++i) {
+            const u32x4 t = s[i];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) r.w[4 * i + c] = t[c];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (d + e < dim) {
+                if constexpr (sizeof(IO) == 4) r.w[e] = reinterpret_cast<const unsigned*>(row)[d + e];
+                else r.w[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[d + e] << (16 * (e & 1));
+            }
+    }
+    return r;
+}
+// x as the sum of n bf16 numbers (two at a time): 16 bits of it with two, all 24 with three
+template <int N>
+__device__ __forceinline__ void split_pair(float x0, float x1, unsigned (&t)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        t[i] = wkv6_detail::pack_bf16(x0, x1);
+        x0 -= wkv6_detail::bf16_lo(t[i]);
+        x1 -= wkv6_detail::bf16_hi(t[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[N]) {
+    u32x4 w[N];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        unsigned o[N];
+        split_pair<N>(x[2 * p], x[2 * p + 1], o);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i][p] = o[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = __builtin_bit_cast(bf16x8, w[i]);
+}
+template <typename IO>
+__device__ __forceinline__ void piece_terms(const Piece<IO>& r, u32x4 (&t)[in_terms<IO>]) {
+    constexpr int NS = in_terms<IO>;
+    if constexpr (std::is_same<IO, __hip_bfloat16>::value) {
+        t[0] = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+    } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            unsigned o[NS];
+            if constexpr (std::is_same<IO, float>::value)
+                split_pair<NS>(__builtin_bit_cast(float, r.w[2 * p]), __builtin_bit_cast(float, r.w[2 * p + 1]), o);
+            else
+                split_pair<NS>((float)__builtin_bit_cast(_Float16, (unsigned short)r.w[p]), (float)__builtin_bit_cast(_Float16, (unsigned short)(r.w[p] >> 16)), o);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) t[i][p] = o[i];
+        }
+    }
+}
+
+// acc += a b with both operands sums of bf16 numbers; products beyond the ORDER-th correction are left out.
+template <int ORDER, int NA, int NB>
+__device__ __forceinline__ f32x4 mma(f32x4 acc, const bf16x8 (&a)[NA], const bf16x8 (&b)[NB]) {
+#pragma unroll
+    for (int o = (NA + NB - 2 < ORDER ? NA + NB - 2 : ORDER); o >= 0; --o)         // small ones first
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[o - i], acc, 0, 0, 0);
+    return acc;
+}
+
+// sum over the lanes up to this one
+__device__ __forceinline__ double wave_scan_inclusive(double x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double o = __shfl_up(x, d);
+        if (lane >= d) x += o;
+    }
+    return x;
+}
+
+template <typename IO, int DX, int MODE>
+struct Lds {
+    static constexpr int L = chunk_len<IO, DX>, NS = in_terms<IO>;
+    // terms of the products' intermediate operands: 16 bits of them for a 16-bit result, all 24 where fp32 ones depend on them: those of fp32 rows, and dg
+    static constexpr int NP = NS < 3 ? 2 : 3, NI = MODE == PLAIN ? NP : 3;
+    static constexpr int PX = DX + 8, PZ = TZ + 8;        // row pitches: 16 rows of a fragment on different banks
+    __bf16 a[MODE == STATES ? 1 : NS][MODE == STATES ? 1 : L][PX];   // channels in the order of the state's fragments
+    __bf16 b[NS][L][PX];
+    __bf16 c[NS][L][PZ];
+    __bf16 e[MODE == EDGES || MODE == FLOWS ? NS : 1][MODE == EDGES || MODE == FLOWS ? L : 1][PZ];
+    u32x4 s[MODE == STATES ? 1 : NI][4][MODE == STATES ? 1 : DX / 32][64];   // the state's terms, a lane's fragment side by side
+    float gh[64], gl[64], dt[64], dk[64];                 // G in powers of two, head and tail; exp(G); exp(G_end - G)
+    float end_decay, through_decay;                       // exp(G_end); FLOWS: with the decay of the token behind the chunk
+    float edge[2][64], inner[4][64], cross[4];            // what rows get or give across the chunk's ends, by halves of the columns; what crosses tokens inside, by waves; <S0, R>
+};
+
+// Eight channels from d on in the order that the accumulators' fragments have: inside 32 channels, 4 m .. 4 m + 3 lie at 8 (m & 3) + 4 (m >> 2).
+__device__ __forceinline__ int order_of(int d) {
+    const int m = (d >> 2) & 7;
+    return (d & ~31) + 8 * (m & 3) + 4 * (m >> 2);
+}
+
+// Packed rows in front of the first sequence and behind the last get zeros, a few from every workgroup of the head and tile.
+template <typename IO, int MODE>
+__device__ __forceinline__ void clear_outside(const Params& p, const Role& r, int gid, int z, int h) {
+    const int front = offset_at(p, 0), back = offset_at(p, p.N), rows = front + max(0, p.T - back);
+    const int d = z * TZ + (threadIdx.x & 63);
+    for (int i = gid * 4 + (threadIdx.x >> 6); i < rows; i += p.segs * 4) {
+        const long long row = i < front ? i : back + (i - front);
+        const long long at = row * r.o.st + h * r.o.sh + d;
+        if (r.o.p && d < r.dz) {
+            if (r.o.f32) static_cast<float*>(r.o.p)[at] = 0.f;
+            else static_cast<IO*>(r.o.p)[at] = from_f32<IO>(0.f);
+        }
+        if (MODE == FLOWS && (threadIdx.x & 63) == 0) r.dg[((long long)z * p.rows + row) * p.H + h] = 0.f;
+    }
+}
+
+template <typename IO, int DX, int MODE>
+__global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
+    using S = Lds<IO, DX, MODE>;
+    constexpr int L = S::L, NS = S::NS, NI = S::NI, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
+    constexpr int PA = L * DX / 8 / THREADS, PC = (L * TZ / 8 + THREADS - 1) / THREADS;
+    static_assert(PA >= 1 && L * DX % (8 * THREADS) == 0 && L * TZ % (8 * THREADS) == 0, "");
+    constexpr bool OUT = MODE != STATES, EXTRA = MODE == EDGES || MODE == FLOWS;
+    __shared__ S lds;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
+
+    // workgroup -> role, tile, head, segment (segments of a head next to each other are on different chiplets; the roles of one share its rows)
+    int id = blockIdx.x;
+    const int ri = id % p.n_roles;
+    id /= p.n_roles;
+    const Role& r = p.role[ri];
+    int tiles = 1;
+    for (int i = 0; i < p.n_roles; ++i) tiles = max(tiles, p.role[i].tiles);
+    const int z = id % tiles;
+    id /= tiles;
+    const int h = id % p.H, gid = id / p.H;
+    if (!p.nseg && OUT && z < r.tiles) clear_outside<IO, MODE>(p, r, gid, z, h);
+    const Place w = find_place(p, gid, L);
+    if (!w.valid || z >= r.tiles) return;
+    if (MODE == STATES && (r.reverse ? w.is_first : w.is_last)) return;    // nothing starts behind it
+    const int z0 = z * TZ;
+    const bool rev = r.reverse;
+
+    // ---- the state that the segment starts from: rows 16 x + 4 quarter + i, column 16 wave + col of the tile
+    f32x4 st[NX];
+    const long long page = ((long long)w.n * p.H + h) * ((long long)r.dx * r.dz);
+    const long long seg_at = (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ);
+    const int zc = z0 + 16 * wave + col;
+    bool have = MODE != STATES;
+    if (MODE == STATES) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    } else if (r.seg) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4);
+        have = r.init || !(rev ? w.is_last : w.is_first);
+    } else {
+        have = r.init != nullptr;
+#pragma unroll
+        for (int x = 0; x < NX; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int xc = 16 * x + 4 * quarter + i;
+                st[x][i] = r.init && xc < r.dx && zc < r.dz ? r.init[page + xc * r.sx + zc * r.sz] : 0.f;
+            }
+    }
+
+    const int nc = (w.s1 - w.s0 + L - 1) / L;
+    const IO* const pa = static_cast<const IO*>(r.a.p) + w.base * r.a.sb + (long long)w.first * r.a.st + (h / r.a.share) * r.a.sh;
+    const IO* const pb = static_cast<const IO*>(r.b.p) + w.base * r.b.sb + (long long)w.first * r.b.st + (h / r.b.share) * r.b.sh;
+    const IO* const pc = static_cast<const IO*>(r.c.p) + w.base * r.c.sb + (long long)w.first * r.c.st + (h / r.c.share) * r.c.sh;
+    const IO* const pe = EXTRA ? static_cast<const IO*>(r.e.p) + w.base * r.e.sb + (long long)w.first * r.e.st + (h / r.e.share) * r.e.sh : nullptr;
+
+    Piece<IO> ra[OUT ? PA : 1], rb[PA], rc[PC], re[EXTRA ? PC : 1];
+    float rg = 0.f, rg_next = 0.f;
+    // the rows of chunk c of the segment's, and their decays
+    const auto fetch = [&](int c) {
+        const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+#pragma unroll
+        for (int i = 0; i < PA; ++i) {
+            const int pi = tid + THREADS * i, row = pi / (DX / 8), d = pi % (DX / 8) * 8;
+            const long long tok = rev ? t0 + n - 1 - row : t0 + row;
+            if constexpr (OUT) ra[i] = load_piece(pa + tok * r.a.st, d, r.dx, row < n, r.a.vec);
+            rb[i] = load_piece(pb + tok * r.b.st, d, r.dx, row < n, r.b.vec);
+        }
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int pi = tid + THREADS * i, row = pi / (TZ / 8), d = z0 + pi % (TZ / 8) * 8;
+            const long long tok = rev ? t0 + n - 1 - row : t0 + row;
+            rc[i] = load_piece(pc + tok * r.c.st, d, r.dz, row < n, r.c.vec);
+            if constexpr (EXTRA) re[i] = load_piece(pe + tok * r.e.st, d, r.dz, row < n, r.e.vec);
+        }
+        if (wave == 0) {
+            // back along the tokens a row's decay is that of the token behind it, and none behind the last
+            const int tok = rev ? t0 + n - lane : t0 + lane;
+            rg = lane < n && tok < w.len ? log_decay(p, w.base, w.first + tok, h) : 0.f;
+            if constexpr (MODE == FLOWS) rg_next = t0 + n < w.len ? log_decay(p, w.base, w.first + t0 + n, h) : 0.f;
+        }
+    };
+    if (nc > 0) fetch(rev ? nc - 1 : 0);
+
+    float seg_log = 0.f;                                  // (STATES: the segment's whole decay, from wave 0)
+    for (int ci = 0; ci < nc; ++ci) {
+        const int c = rev ? nc - 1 - ci : ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+        // ---- operands to the LDS
+#pragma unroll
+        for (int i = 0; i < PA; ++i) {
+            const int pi = tid + THREADS * i, row = pi / (DX / 8), d = pi % (DX / 8) * 8;
+            const int o0 = order_of(d), o1 = order_of(d + 4);
+            u32x4 t[NS];
+            if constexpr (OUT) {
+                piece_terms<IO>(ra[i], t);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    *reinterpret_cast<uint2*>(&lds.a[s][row][o0]) = uint2{t[s][0], t[s][1]};
+                    *reinterpret_cast<uint2*>(&lds.a[s][row][o1]) = uint2{t[s][2], t[s][3]};
+                }
+            }
+            piece_terms<IO>(rb[i], t);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                *reinterpret_cast<uint2*>(&lds.b[s][row][o0]) = uint2{t[s][0], t[s][1]};
+                *reinterpret_cast<uint2*>(&lds.b[s][row][o1]) = uint2{t[s][2], t[s][3]};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int pi = tid + THREADS * i, row = pi / (TZ / 8), d = pi % (TZ / 8) * 8;
+            u32x4 t[NS];
+            piece_terms<IO>(rc[i], t);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.c[s][row][d]) = t[s];
+            if constexpr (EXTRA) {
+                piece_terms<IO>(re[i], t);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.e[s][row][d]) = t[s];
+            }
+        }
+        if constexpr (OUT) {
+            if (have) {
+#pragma unroll
+                for (int kx = 0; kx < KX; ++kx) {
+                    const float x8[8] = {st[2 * kx][0], st[2 * kx][1], st[2 * kx][2], st[2 * kx][3], st[2 * kx + 1][0], st[2 * kx + 1][1], st[2 * kx + 1][2], st[2 * kx + 1][3]};
+                    bf16x8 t[NI];
+                    split8<NI>(x8, t);
+#pragma unroll
+                    for (int s = 0; s < NI; ++s) lds.s[s][wave][kx][lane] = __builtin_bit_cast(u32x4, t[s]);
+                }
+            }
+        }
+        if (wave == 0) {
+            // sums in 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth
+            const double G = wave_scan_inclusive((double)rg * 1.4426950408889634, lane);
+            const double end = __shfl(G, 63);
+            const float gh = (float)G;
+            lds.gh[lane] = gh;
+            lds.gl[lane] = (float)(G - gh);
+            lds.dt[lane] = fast_exp2(gh);
+            lds.dk[lane] = fast_exp2((float)(end - G));
+            if (lane == 0) {
+                lds.end_decay = fast_exp2((float)end);
+                if constexpr (MODE == FLOWS) lds.through_decay = fast_exp2((float)(end + (double)rg_next * 1.4426950408889634));
+            }
+            if (MODE == STATES) seg_log += (float)end;
+        }
+        __syncthreads();
+        if (ci + 1 < nc) fetch(rev ? c - 1 : c + 1);
+
+        // ---- outputs of rows 16 tw + col, columns 16 zt + 4 quarter + i
+        if constexpr (OUT) {
+            const int tw = wave % NT, zt0 = wave / NT * NT;
+            const int t = 16 * tw + col;
+            const float gth = lds.gh[t], gtl = lds.gl[t], dec = lds.dt[t] * r.s_in;
+            bf16x8 fa[KX][NS];
+#pragma unroll
+            for (int kx = 0; kx < KX; ++kx)
+#pragma unroll
+                for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[s][t][kx * 32 + 8 * quarter]);
+            f32x4 acc[NT], far[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j] = far[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x4 flow[MODE == FLOWS ? NT : 1];            // [tile of j]: sums over s < j of the terms of row t
+#pragma unroll
+            for (int j = 0; j < (MODE == FLOWS ? NT : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (2 * ks > tw) break;
+                float pr[8], pf[8];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int st_ = 2 * ks + half;        // tile of 16 tokens s
+                    f32x4 m = {0.f, 0.f, 0.f, 0.f};
+                    if (st_ <= tw) {
+#pragma unroll
+                        for (int kx = 0; kx < KX; ++kx) {
+                            bf16x8 fb[NS];
+#pragma unroll
+                            for (int s = 0; s < NS; ++s) fb[s] = *reinterpret_cast<const bf16x8*>(&lds.b[s][16 * st_ + col][kx * 32 + 8 * quarter]);
+                            m = mma<NI - 1>(m, fb, fa[kx]);
+                        }
+                        const f32x4 sh = *reinterpret_cast<const f32x4*>(&lds.gh[16 * st_ + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&lds.gl[16 * st_ + 4 * quarter]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = m[i] * fast_exp2((gth - sh[i]) + (gtl - sl[i]));
+                            m[i] = st_ < tw || 4 * quarter + i <= col ? x : 0.f;
+                        }
+                        if constexpr (MODE == FLOWS) {
+                            f32x4 qk = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int kz = 0; kz < TZ / 32; ++kz) {
+                                bf16x8 fk[NS], fq[NS];
+#pragma unroll
+                                for (int s = 0; s < NS; ++s) {
+                                    fk[s] = *reinterpret_cast<const bf16x8*>(&lds.c[s][16 * st_ + col][kz * 32 + 8 * quarter]);
+                                    fq[s] = *reinterpret_cast<const bf16x8*>(&lds.e[s][t][kz * 32 + 8 * quarter]);
+                                }
+                                qk = mma<2>(qk, fk, fq);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) pf[4 * half + i] = m[i] * qk[i];
+                        }
+                    } else if constexpr (MODE == FLOWS) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) pf[4 * half + i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) pr[4 * half + i] = m[i];
+                }
+                if constexpr (MODE == FLOWS) {
+                    bf16x8 ff[3];
+                    split8<3>(pf, ff);
+#pragma unroll
+                    for (int j = 2 * ks; j < NT; ++j) {
+                        if (j > tw) break;
+                        // ones where s < j, row j of the tile in lane col: all of a tile in front of it, none of one behind it
+                        u32x4 ones;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const unsigned lo = 4 * quarter + 2 * e < col ? 0x3f80u : 0u, hi = 4 * quarter + 2 * e + 1 < col ? 0x3f800000u : 0u;
+                                ones[2 * half + e] = 2 * ks + half < j ? 0x3f803f80u : 2 * ks + half == j ? lo | hi : 0u;
+                            }
+                        const bf16x8 fu[1] = {__builtin_bit_cast(bf16x8, ones)};
+                        flow[j] = mma<2>(flow[j], fu, ff);
+                    }
+                }
+                bf16x8 fp[NP];
+                split8<NP>(pr, fp);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    bf16x8 fc[NS];
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) {
+                        const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * (zt0 + j) + 4 * (col & 3)];
+                        fc[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
+                    }
+                    acc[j] = mma<NP - 1>(acc[j], fc, fp);
+                }
+            }
+            if (have) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int kx = 0; kx < KX; ++kx) {
+                        bf16x8 fs[NI];
+#pragma unroll
+                        for (int s = 0; s < NI; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane]);
+                        far[j] = mma<NI - 1>(far[j], fs, fa[kx]);
+                    }
+            }
+            const long long tok = w.first + (rev ? t0 + n - 1 - t : t0 + t);
+            float edge = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int zl = 16 * (zt0 + j) + 4 * quarter;
+                f32x4 o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = dec * far[j][i];
+                    o[i] = fmaf(p.scale, acc[j][i], f);
+                    if constexpr (EXTRA) {
+                        float x = 0.f;
+#pragma unroll
+                        for (int s = NS - 1; s >= 0; --s) x += (float)lds.e[s][t][zl + i];
+                        edge = fmaf(x, f, edge);
+                    }
+                }
+                if (t < n && r.o.p) {
+                    const long long at = w.base * r.o.sb + tok * r.o.st + h * r.o.sh + z0 + zl;
+                    if (r.o.f32) {
+                        float* q = static_cast<float*>(r.o.p) + at;
+                        if (r.o.vec && z0 + zl + 4 <= r.dz) *reinterpret_cast<f32x4*>(q) = o;
+                        else
+                            for (int i = 0; i < 4; ++i)
+                                if (z0 + zl + i < r.dz) q[i] = o[i];
+                    } else {
+                        IO* q = static_cast<IO*>(r.o.p) + at;
+                        const float x4[4] = {o[0], o[1], o[2], o[3]};
+                        if (r.o.vec && z0 + zl + 4 <= r.dz) store_vec<IO, 4>(q, x4);
+                        else
+                            for (int i = 0; i < 4; ++i)
+                                if (z0 + zl + i < r.dz) q[i] = from_f32<IO>(x4[i]);
+                    }
+                }
+            }
+            if constexpr (EXTRA) {                        // over the quarters: the channels of a row
+                edge += __shfl_xor(edge, 16);
+                edge += __shfl_xor(edge, 32);
+                if (quarter == 0) lds.edge[wave / NT][t] = edge;    // (two waves share a row where the chunk has 32 tokens)
+            }
+            if constexpr (MODE == FLOWS) {
+                float crossing[16];                       // of rows t from j on
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) crossing[4 * j + i] = j < NT && (j < tw || (j == tw && 4 * quarter + i <= col)) ? flow[j < NT ? j : 0][i] : 0.f;
+                int index;
+                const float cf = wkv6_detail::row_sums16(crossing, lane, index);
+                // (the other waves of a 32-token chunk have made the same terms)
+                lds.inner[wave][16 * (index >> 2) + 4 * quarter + (index & 3)] = wave < NT ? cf * p.scale : 0.f;
+                // <S0, R>: R behind this chunk, as the pass of dk left it
+                float x = 0.f;
+                if (have) {
+                    const long long ck = (((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * r.tiles + z) * (DX * TZ);
+#pragma unroll
+                    for (int x4 = 0; x4 < NX; ++x4) {
+                        const f32x4 a4 = *reinterpret_cast<const f32x4*>(r.anchors + ck + ((x4 * 4 + wave) * 64 + lane) * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x = fmaf(st[x4][i], a4[i], x);
+                    }
+                }
+                x += __shfl_xor(x, 1);
+                x += __shfl_xor(x, 2);
+                x += __shfl_xor(x, 4);
+                x += __shfl_xor(x, 8);
+                x += __shfl_xor(x, 16);
+                x += __shfl_xor(x, 32);
+                if (lane == 0) lds.cross[wave] = x;
+            }
+        }
+
+        // ---- the state behind the chunk
+        {
+            if constexpr (MODE == EDGES) {
+                const long long ck = (((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * r.tiles + z) * (DX * TZ);
+#pragma unroll
+                for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.anchors + ck + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
+            }
+            const float ed = lds.end_decay;
+#pragma unroll
+            for (int x = 0; x < NX; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st[x][i] *= ed;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                float x8[8];
+                const f32x4 d0 = *reinterpret_cast<const f32x4*>(&lds.dk[32 * ks + 4 * quarter]), d1 = *reinterpret_cast<const f32x4*>(&lds.dk[32 * ks + 16 + 4 * quarter]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x8[i] = 0.f;
+#pragma unroll
+                for (int s = NS - 1; s >= 0; --s) {
+                    const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * wave + 4 * (col & 3)];
+                    const bf16x8 f = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x8[i] += (float)f[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x8[i] *= d0[i] * r.s_upd;
+                    x8[4 + i] *= d1[i] * r.s_upd;
+                }
+                bf16x8 fv[3];
+                split8<3>(x8, fv);
+#pragma unroll
+                for (int x = 0; x < NX; ++x) {
+                    bf16x8 fk[NS];
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) {
+                        const __bf16* q = &lds.b[s][32 * ks + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
+                        fk[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PX));
+                    }
+                    st[x] = mma<2>(st[x], fk, fv);
+                }
+            }
+            have = true;
+        }
+        __syncthreads();
+        if constexpr (MODE == EDGES) {
+            if (wave == 0 && lane < n) {
+                const long long row = (long long)w.base * p.T + w.first + t0 + n - 1 - lane;
+                r.edge[((long long)z * p.rows + row) * p.H + h] = NT == 4 ? lds.edge[0][lane] : lds.edge[0][lane] + lds.edge[1][lane];
+            }
+        }
+        if constexpr (MODE == FLOWS) {
+            if (wave == 0) {
+                const long long row = (long long)w.base * p.T + w.first + t0 + lane;
+                const long long at = ((long long)z * p.rows + row) * p.H + h;
+                // what token `lane` receives over the chunk's front and gives over its end; summed from it on, and up to it
+                double in = 0., out = 0.;
+                if (lane < n) {
+                    in = NT == 4 ? lds.edge[0][lane] : (double)lds.edge[0][lane] + lds.edge[1][lane];
+                    out = r.edge[at];
+                }
+                double before = wave_scan_inclusive(out, lane);
+                before = __shfl_up(before, 1);
+                if (lane == 0) before = 0.;
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2) {
+                    const double o = __shfl_down(in, d);
+                    if (lane + d < 64) in += o;
+                }
+                const double inner = ((double)lds.inner[0][lane] + lds.inner[1][lane]) + ((double)lds.inner[2][lane] + lds.inner[3][lane]);
+                const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * lds.through_decay;
+                if (lane < n) r.dg[at] = (float)(inner + in + before + through);
+            }
+        }
+    }
+
+    // ---- the state behind the segment
+    if constexpr (MODE == STATES) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
+        if (tid == 0 && z == 0) r.seg_decay[(long long)gid * p.H + h] = fast_exp2(seg_log);
+    } else {
+        if (r.last && (rev ? w.is_first : w.is_last)) {
+            const float d = rev && w.len > 0 ? fast_exp2(log_decay(p, w.base, w.first, h) * LOG2E) : 1.f;   // back along the tokens: the first one's decay
+#pragma unroll
+            for (int x = 0; x < NX; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int xc = 16 * x + 4 * quarter + i;
+                    if (xc < r.dx && zc < r.dz) r.last[page + xc * r.sx + zc * r.sz] = st[x][i] * d;
+                }
+        }
+    }
+}
+
+// How the host reaches the instances of each type.
+template <typename IO> int launch_decay(const Params& p, int dx, int mode, hipStream_t st);
+extern template int launch_decay<float>(const Params&, int, int, hipStream_t);
+extern template int launch_decay<__hip_bfloat16>(const Params&, int, int, hipStream_t);
+extern template int launch_decay<__half>(const Params&, int, int, hipStream_t);
+
+template <typename IO>
+int launch_decay(const Params& p, int dx, int mode, hipStream_t st) {
+    int tiles = 1;
+    for (int i = 0; i < p.n_roles; ++i) tiles = p.role[i].tiles > tiles ? p.role[i].tiles : tiles;
+    const dim3 grid((unsigned)((long long)p.segs * p.H * tiles * p.n_roles)), block(THREADS);
+    if (dx <= 64) {
+        if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, 64, PLAIN>), grid, block, 0, st, p);
+        else if (mode == EDGES) hipLaunchKernelGGL((decay_kernel<IO, 64, EDGES>), grid, block, 0, st, p);
+        else if (mode == FLOWS) hipLaunchKernelGGL((decay_kernel<IO, 64, FLOWS>), grid, block, 0, st, p);
+        else if (mode == ALONE) hipLaunchKernelGGL((decay_kernel<IO, 64, ALONE>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((decay_kernel<IO, 64, STATES>), grid, block, 0, st, p);
+    } else {
+        if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, 128, PLAIN>), grid, block, 0, st, p);
+        else if (mode == EDGES) hipLaunchKernelGGL((decay_kernel<IO, 128, EDGES>), grid, block, 0, st, p);
+        else if (mode == FLOWS) hipLaunchKernelGGL((decay_kernel<IO, 128, FLOWS>), grid, block, 0, st, p);
+        else if (mode == ALONE) hipLaunchKernelGGL((decay_kernel<IO, 128, ALONE>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((decay_kernel<IO, 128, STATES>), grid, block, 0, st, p);
+    }
+    return check_launch("decay_attention");
+}
+
+}  // namespace decay
+}  // namespace vrwkv

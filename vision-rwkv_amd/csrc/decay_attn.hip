@@ -1,0 +1,409 @@
+// Host side of the attention with a decay for each head (decay_attn.h), and the passes around its kernel: the states in front of the segments, and the
+// sums that gradients of shared heads and of the decays leave to the end.
+#include "decay_attn.h"
+#include <algorithm>
+#include <cstdint>
+
+namespace vrwkv {
+namespace decay {
+namespace {
+
+// The state in front of each segment from the segments' own ones: a lane carries four numbers along the sequence.
+// Grid (DX / 16 * N * H * tiles, 1, roles).  A segment's state is read once and written once, 32 KB for 64 channels; its loads do not wait for the sums.
+template <int DX>
+__global__ __launch_bounds__(THREADS) void segments_kernel(const Params p, int L) {
+    const Role& r = p.role[blockIdx.z];
+    int id = blockIdx.x / (DX / 16);
+    int tiles = 1;
+    for (int i = 0; i < p.n_roles; ++i) tiles = max(tiles, p.role[i].tiles);
+    const int z = id % tiles;
+    id /= tiles;
+    const int h = id % p.H, n = id / p.H;
+    if (z >= r.tiles) return;
+    const Place w = sequence_place(p, n, L);
+    const int x = blockIdx.x % (DX / 16), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int first = first_segment(p, n, w.first), count = segment_count(p, w.len);
+    f32x4 carry = {0.f, 0.f, 0.f, 0.f};
+    if (r.init) {
+        const float* page = r.init + ((long long)n * p.H + h) * ((long long)r.dx * r.dz);
+        const int zc = z * TZ + 16 * wave + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int xc = 16 * x + 4 * (lane >> 4) + i;
+            if (xc < r.dx && zc < r.dz) carry[i] = page[xc * r.sx + zc * r.sz];
+        }
+    }
+    const auto at = [&](int i) {                          // i-th on the way
+        const long long gid = first + (r.reverse ? count - 1 - i : i);
+        return gid;
+    };
+    f32x4 next = {0.f, 0.f, 0.f, 0.f};
+    float d = 1.f;
+    const long long in_tile = ((long long)x * 4 + wave) * 64 * 4 + lane * 4;
+    const auto load = [&](int i) {
+        if (i + 1 < count) {                              // (the last one on the way has not been made)
+            next = *reinterpret_cast<const f32x4*>(r.seg + ((at(i) * p.H + h) * r.tiles + z) * (DX * TZ) + in_tile);
+            d = r.seg_decay[at(i) * p.H + h];
+        }
+    };
+    load(0);
+    for (int i = 0; i < count; ++i) {
+        const f32x4 own = next;
+        const float dec = d;
+        load(i + 1);
+        *reinterpret_cast<f32x4*>(r.seg + ((at(i) * p.H + h) * r.tiles + z) * (DX * TZ) + in_tile) = carry;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) carry[c] = fmaf(carry[c], dec, own[c]);
+    }
+}
+
+// out (rows, heads, D) = the sums over the heads of part (rows, heads * share, D) that share one, rounded once
+template <typename IO>
+__global__ __launch_bounds__(THREADS) void head_sum_kernel(const float* part, IO* out, long long count, int D, int share) {
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < count; i += (long long)gridDim.x * THREADS) {
+        const long long head = i / D;
+        const int d = (int)(i % D);
+        float s = 0.f;
+        for (int j = 0; j < share; ++j) s += part[(head * share + j) * D + d];
+        out[i] = from_f32<IO>(s);
+    }
+}
+// out (rows, H) = the sums of part (tiles, rows, H)
+template <typename G>
+__global__ __launch_bounds__(THREADS) void decay_grad_kernel(const float* part, G* out, long long count, int tiles) {
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < count; i += (long long)gridDim.x * THREADS) {
+        float s = part[i];
+        for (int t = 1; t < tiles; ++t) s += part[t * count + i];
+        out[i] = from_f32<G>(s);
+    }
+}
+// The same over the rows as well, in 64 bits: slices first, then their sums.  Grid (slices, ceil(H / 64)); 4 rows of 64 heads a step.
+__global__ __launch_bounds__(THREADS) void decay_slices_kernel(const float* part, double* slices, long long rows, int H) {
+    __shared__ double red[4][64];
+    const int h = blockIdx.y * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
+    double s = 0.;
+    if (h < H)
+        for (long long r = (long long)blockIdx.x * 4 + sub; r < rows; r += (long long)gridDim.x * 4) s += part[r * H + h];
+    red[sub][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (sub == 0 && h < H) slices[(long long)blockIdx.x * H + h] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+template <typename G>
+__global__ __launch_bounds__(THREADS) void decay_total_kernel(const double* slices, G* out, int n, int H) {
+    const int h = blockIdx.x * THREADS + threadIdx.x;
+    if (h >= H) return;
+    double s = 0.;
+    for (int i = 0; i < n; ++i) s += slices[(long long)i * H + h];
+    out[h] = from_f32<G>((float)s);
+}
+
+constexpr int SLICES = 128;
+
+size_t elem(int dtype) { return dtype == VRWKV_F32 ? 4 : 2; }
+int pad_dx(int d) { return d <= 64 ? 64 : 128; }
+int tiles_of(int d) { return (d + TZ - 1) / TZ; }
+int chunk_of(int dtype, int dx) { return dtype == VRWKV_BF16 || (dtype == VRWKV_F16 && dx == 64) ? 64 : 32; }
+
+// Tokens of a segment.  A workgroup takes a chunk of 64 tokens in 1 to 2 us and two fit a compute unit: calls of fewer sequences and heads than fill
+// the chip are cut into segments of at least two chunks, which read their rows twice.
+int segment_len(const vrwkv_decay_args& a, int tiles, int roles) {
+    const long long wgs = (long long)a.H * tiles * roles, want = 3 * device_cus();
+    if (!a.offsets) {
+        const long long whole = wgs * a.N;
+        const int chunks = (a.T + 63) / 64;
+        if (whole >= want / 2 || chunks < 4) return chunks * 64;
+        const long long pieces = std::min<long long>((want + whole - 1) / whole, chunks / 2);
+        return (int)((chunks + pieces - 1) / pieces) * 64;
+    }
+    // packed: some sequence may be as long as all of them
+    const long long len = (long long)a.T * wgs / want / 64 * 64;
+    return (int)std::max<long long>(128, std::min<long long>(len, 1024));
+}
+bool cut(const vrwkv_decay_args& a, int seg_len) { return a.T > seg_len; }
+long long segment_total(const vrwkv_decay_args& a, int seg_len) {
+    return a.offsets ? (long long)a.T / seg_len + a.N : (long long)a.N * ((a.T + seg_len - 1) / seg_len);
+}
+long long chunk_total(const vrwkv_decay_args& a, int L) { return a.offsets ? (long long)a.T / L + a.N : (long long)a.N * ((a.T + L - 1) / L); }
+long long rows_of(const vrwkv_decay_args& a) { return a.offsets ? a.T : (long long)a.N * a.T; }
+
+// Workspace pieces, one behind the other on 256 bytes; with base null only their sum.
+struct Pieces {
+    char* base;
+    size_t used = 0;
+    template <typename T> T* take(size_t n) {
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used = (used + n * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
+int check_common(const vrwkv_decay_args* a, const char* who) {
+    if (!a) { set_error("%s: null args", who); return VRWKV_INVALID_ARG; }
+    if (a->N <= 0 || a->T <= 0 || a->H <= 0 || a->Hq <= 0 || a->Hk <= 0 || a->Hv <= 0) { set_error("%s: N, T and the numbers of heads must be positive", who); return VRWKV_INVALID_ARG; }
+    if (a->dtype < VRWKV_F32 || a->dtype > VRWKV_F16 || a->g_dtype < VRWKV_F32 || a->g_dtype > VRWKV_F16) { set_error("%s: dtype must be fp32, bf16 or fp16", who); return VRWKV_UNSUPPORTED_DTYPE; }
+    if (a->H % a->Hq || a->H % a->Hk || a->H % a->Hv) { set_error("%s: H (%d) must be a multiple of the heads of q, k and v (%d, %d, %d)", who, a->H, a->Hq, a->Hk, a->Hv); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (a->Dk < 1 || a->Dk > 128 || a->Dv < 1 || a->Dv > 128) { set_error("%s: head sizes (%d, %d) must be 1 to 128", who, a->Dk, a->Dv); return VRWKV_UNSUPPORTED_SHAPE; }
+    // workgroups of a launch: at most four tiles and roles, or eight pieces of two tiles, of a segment (its first chunks, or a sequence) and head
+    if (chunk_total(*a, 32) >= 1LL << 30 || (chunk_total(*a, 64) + a->N) * a->H >= 1LL << 24 || (long long)a->N * a->H * 32 >= 1LL << 24) { set_error("%s: too many tokens and heads", who); return VRWKV_UNSUPPORTED_SHAPE; }
+    return VRWKV_OK;
+}
+int check_tensors(const vrwkv_decay_args& a, const char* who) {
+    if (!a.q || !a.k || !a.v || !a.g) { set_error("%s: null q, k, v or g", who); return VRWKV_INVALID_ARG; }
+    const size_t m = elem(a.dtype) - 1;
+    for (const void* p : {a.q, a.k, a.v, (const void*)a.y, a.gy, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv})
+        if ((size_t)p & m) { set_error("%s: a tensor is not aligned to its elements", who); return VRWKV_INVALID_ARG; }
+    for (const void* p : {a.g, (const void*)a.dg})
+        if ((size_t)p & (elem(a.g_dtype) - 1)) { set_error("%s: g is not aligned to its elements", who); return VRWKV_INVALID_ARG; }
+    for (const void* p : {(const void*)a.state, (const void*)a.last, (const void*)a.glast, (const void*)a.dstate})
+        if ((size_t)p & 3) { set_error("%s: a state is not aligned to its elements", who); return VRWKV_INVALID_ARG; }
+    if (a.offsets && ((size_t)a.offsets & (a.offsets64 ? 7 : 3))) { set_error("%s: offsets are not aligned to their elements", who); return VRWKV_INVALID_ARG; }
+    return VRWKV_OK;
+}
+View view(const void* p, const long long (&s)[3], int heads, const vrwkv_decay_args& a) {
+    const long long per16 = 16 / (long long)elem(a.dtype);
+    return View{p, s[0], s[1], s[2], a.H / heads, ((size_t)p & 15) == 0 && s[0] % per16 == 0 && s[1] % per16 == 0 && s[2] % per16 == 0};
+}
+OutView out_view(void* p, int D, const vrwkv_decay_args& a, bool f32) {
+    const long long sh = D, st = (long long)a.H * D;
+    return OutView{p, st * a.T, st, sh, f32, ((size_t)p & (f32 ? 15 : 4 * elem(a.dtype) - 1)) == 0 && D % 4 == 0};
+}
+Params common(const vrwkv_decay_args& a, int seg_len) {
+    Params p{};
+    p.offsets = a.offsets;
+    p.off64 = a.offsets64;
+    p.g = a.g;
+    p.g_sb = a.g_stride[0];
+    p.g_st = a.g_stride[1];
+    p.g_sh = a.g_stride[2];
+    p.g_dtype = a.g_dtype;
+    p.rows = rows_of(a);
+    p.N = a.N;
+    p.T = a.T;
+    p.H = a.H;
+    p.seg_len = seg_len;
+    p.nseg = a.offsets ? 0 : (a.T + seg_len - 1) / seg_len;
+    p.segs = (int)segment_total(a, seg_len);
+    p.scale = a.scale;
+    return p;
+}
+int launch(const Params& p, int dtype, int dx, int mode, hipStream_t st) {
+    if (dtype == VRWKV_F32) return launch_decay<float>(p, dx, mode, st);
+    if (dtype == VRWKV_BF16) return launch_decay<__hip_bfloat16>(p, dx, mode, st);
+    return launch_decay<__half>(p, dx, mode, st);
+}
+// The segments' own states and the states in front of them, for the roles of p.
+int launch_segments(const Params& p, int dtype, int dx, hipStream_t st) {
+    const int s = launch(p, dtype, dx, STATES, st);
+    if (s != VRWKV_OK) return s;
+    int tiles = 1;
+    for (int i = 0; i < p.n_roles; ++i) tiles = std::max(tiles, p.role[i].tiles);
+    const dim3 grid((unsigned)(dx / 16 * (long long)p.N * p.H * tiles), 1, p.n_roles), block(THREADS);
+    const int L = chunk_of(dtype, dx);
+    if (dx == 64) hipLaunchKernelGGL((segments_kernel<64>), grid, block, 0, st, p, L);
+    else hipLaunchKernelGGL((segments_kernel<128>), grid, block, 0, st, p, L);
+    return check_launch("decay_attention (segments)");
+}
+void take_segments(Role& r, Pieces& ws, const vrwkv_decay_args& a, long long segs, int dx) {
+    r.seg = ws.take<float>((size_t)segs * a.H * r.tiles * dx * TZ);
+    r.seg_decay = ws.take<float>((size_t)segs * a.H);
+}
+
+struct FwdPlan {
+    int dx, seg_len;
+    Role role{};
+    FwdPlan(const vrwkv_decay_args& a, Pieces& ws) {
+        dx = pad_dx(a.Dk);
+        role.dx = a.Dk;
+        role.dz = a.Dv;
+        role.tiles = tiles_of(a.Dv);
+        seg_len = segment_len(a, role.tiles, 1);
+        if (cut(a, seg_len)) take_segments(role, ws, a, segment_total(a, seg_len), dx);
+    }
+};
+struct BwdPlan {
+    int dxk, dxv, seg_len, L;
+    Role dv{}, dk{}, dq{};
+    float *fq = nullptr, *fk = nullptr, *fv = nullptr, *fg = nullptr;   // gradients of every head, where several share one; of the decays
+    double* slices = nullptr;
+    BwdPlan(const vrwkv_decay_args& a, Pieces& ws) {
+        dxk = pad_dx(a.Dk);
+        dxv = pad_dx(a.Dv);
+        L = chunk_of(a.dtype, dxv);
+        dv.dx = dk.dz = dq.dz = a.Dk;
+        dv.dz = dk.dx = dq.dx = a.Dv;
+        dv.tiles = tiles_of(a.Dv);
+        dk.tiles = dq.tiles = tiles_of(a.Dk);
+        dv.reverse = dk.reverse = 1;
+        seg_len = segment_len(a, 1, 2);
+        const long long segs = segment_total(a, seg_len), rows = rows_of(a);
+        if (cut(a, seg_len)) {
+            take_segments(dv, ws, a, segs, dxk);
+            take_segments(dk, ws, a, segs, dxv);
+            take_segments(dq, ws, a, segs, dxv);
+        }
+        if (a.dq && a.Hq < a.H) fq = ws.take<float>((size_t)rows * a.H * a.Dk);
+        if (a.dk && a.Hk < a.H) fk = ws.take<float>((size_t)rows * a.H * a.Dk);
+        if (a.dv && a.Hv < a.H) fv = ws.take<float>((size_t)rows * a.H * a.Dv);
+        if (a.dg) {
+            dk.anchors = ws.take<float>((size_t)chunk_total(a, L) * a.H * dk.tiles * dxv * TZ);
+            dk.edge = ws.take<float>((size_t)rows * a.H * dk.tiles);
+            if (a.g_per_head || dk.tiles > 1 || a.g_dtype != VRWKV_F32) fg = ws.take<float>((size_t)rows * a.H * dk.tiles);
+            if (a.g_per_head) slices = ws.take<double>((size_t)SLICES * a.H);
+            dq.anchors = dk.anchors;
+            dq.edge = dk.edge;
+        }
+    }
+};
+int check_workspace(const vrwkv_decay_args& a, size_t need, const char* who) {
+    if (need && (!a.workspace || a.workspace_bytes < need)) { set_error("%s: workspace of %zu bytes, %zu needed", who, a.workspace ? a.workspace_bytes : 0, need); return VRWKV_WORKSPACE_TOO_SMALL; }
+    if (need && ((size_t)a.workspace & 15)) { set_error("%s: workspace must be 16-byte aligned", who); return VRWKV_INVALID_ARG; }
+    return VRWKV_OK;
+}
+template <typename IO>
+void head_sums(const float* part, void* out, const vrwkv_decay_args& a, int heads, int D, hipStream_t st) {
+    const long long count = rows_of(a) * heads * D;
+    const unsigned grid = (unsigned)std::min<long long>((count + THREADS - 1) / THREADS, 8192);
+    hipLaunchKernelGGL((head_sum_kernel<IO>), dim3(grid), dim3(THREADS), 0, st, part, static_cast<IO*>(out), count, D, a.H / heads);
+}
+template <typename G>
+void decay_sums(const BwdPlan& b, const vrwkv_decay_args& a, hipStream_t st) {
+    const long long rows = rows_of(a), count = rows * a.H;
+    if (a.g_per_head) {
+        const int n = (int)std::min<long long>(SLICES, (rows * b.dk.tiles + 3) / 4);
+        hipLaunchKernelGGL(decay_slices_kernel, dim3(n, (a.H + 63) / 64), dim3(THREADS), 0, st, b.fg, b.slices, rows * b.dk.tiles, a.H);
+        hipLaunchKernelGGL((decay_total_kernel<G>), dim3((a.H + THREADS - 1) / THREADS), dim3(THREADS), 0, st, b.slices, static_cast<G*>(a.dg), n, a.H);
+    } else {
+        const unsigned grid = (unsigned)std::min<long long>((count + THREADS - 1) / THREADS, 4096);
+        hipLaunchKernelGGL((decay_grad_kernel<G>), dim3(grid), dim3(THREADS), 0, st, b.fg, static_cast<G*>(a.dg), count, b.dk.tiles);
+    }
+}
+
+}  // namespace
+}  // namespace decay
+}  // namespace vrwkv
+
+using namespace vrwkv;
+using namespace vrwkv::decay;
+
+extern "C" size_t vrwkv_decay_fwd_workspace_bytes(const vrwkv_decay_args* args) {
+    if (check_common(args, "vrwkv_decay_fwd") != VRWKV_OK) return 0;
+    Pieces ws{nullptr};
+    FwdPlan plan(*args, ws);
+    return ws.used;
+}
+
+extern "C" int vrwkv_decay_fwd(const vrwkv_decay_args* args, void* hip_stream) {
+    const char* who = "vrwkv_decay_fwd";
+    int s = check_common(args, who);
+    if (s == VRWKV_OK) s = check_tensors(*args, who);
+    if (s != VRWKV_OK) return s;
+    const vrwkv_decay_args& a = *args;
+    if (!a.y) { set_error("%s: null y", who); return VRWKV_INVALID_ARG; }
+    Pieces size{nullptr};
+    FwdPlan sized(a, size);
+    if ((s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
+    Pieces ws{static_cast<char*>(a.workspace)};
+    FwdPlan plan(a, ws);
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    Params p = common(a, plan.seg_len);
+    p.n_roles = 1;
+    Role& r = p.role[0] = plan.role;
+    r.a = view(a.q, a.q_stride, a.Hq, a);
+    r.b = view(a.k, a.k_stride, a.Hk, a);
+    r.c = view(a.v, a.v_stride, a.Hv, a);
+    r.o = out_view(a.y, a.Dv, a, false);
+    r.init = a.state;
+    r.last = a.last;
+    r.sx = a.Dv;
+    r.sz = 1;
+    r.s_in = a.scale;
+    r.s_upd = 1.f;
+    if (r.seg && (s = launch_segments(p, a.dtype, plan.dx, st)) != VRWKV_OK) return s;
+    return launch(p, a.dtype, plan.dx, PLAIN, st);
+}
+
+extern "C" size_t vrwkv_decay_bwd_workspace_bytes(const vrwkv_decay_args* args) {
+    if (check_common(args, "vrwkv_decay_bwd") != VRWKV_OK) return 0;
+    Pieces ws{nullptr};
+    BwdPlan plan(*args, ws);
+    return ws.used;
+}
+
+extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
+    const char* who = "vrwkv_decay_bwd";
+    int s = check_common(args, who);
+    if (s == VRWKV_OK) s = check_tensors(*args, who);
+    if (s != VRWKV_OK) return s;
+    const vrwkv_decay_args& a = *args;
+    if (!a.gy) { set_error("%s: null gy", who); return VRWKV_INVALID_ARG; }
+    Pieces size{nullptr};
+    BwdPlan sized(a, size);
+    if ((s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
+    Pieces ws{static_cast<char*>(a.workspace)};
+    BwdPlan b(a, ws);
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const View q = view(a.q, a.q_stride, a.Hq, a), k = view(a.k, a.k_stride, a.Hk, a), v = view(a.v, a.v_stride, a.Hv, a), gy = view(a.gy, a.gy_stride, a.H, a);
+    // dv_t = R_t^T k_t: R from q and gy; its last state is the gradient of the first one
+    b.dv.a = k;
+    b.dv.b = q;
+    b.dv.c = gy;
+    b.dv.o = out_view(b.fv ? b.fv : a.dv, a.Dv, a, b.fv != nullptr);
+    b.dv.init = a.glast;
+    b.dv.last = a.dstate;
+    b.dv.sx = a.Dv;
+    b.dv.sz = 1;
+    b.dv.s_in = 1.f;
+    b.dv.s_upd = a.scale;
+    // dk_t = R_t v_t: R the other way round
+    b.dk.a = v;
+    b.dk.b = gy;
+    b.dk.c = q;
+    b.dk.e = k;
+    b.dk.o = out_view(b.fk ? b.fk : a.dk, a.Dk, a, b.fk != nullptr);
+    b.dk.init = a.glast;
+    b.dk.sx = 1;
+    b.dk.sz = a.Dv;
+    b.dk.s_in = 1.f;
+    b.dk.s_upd = a.scale;
+    // dq_t = scale S_t gy_t
+    b.dq.a = gy;
+    b.dq.b = v;
+    b.dq.c = k;
+    b.dq.e = q;
+    b.dq.o = out_view(b.fq ? b.fq : a.dq, a.Dk, a, b.fq != nullptr);
+    b.dq.init = a.state;
+    b.dq.sx = 1;
+    b.dq.sz = a.Dv;
+    b.dq.s_in = a.scale;
+    b.dq.s_upd = 1.f;
+    b.dq.dg = b.fg ? b.fg : static_cast<float*>(a.dg);
+    Params p = common(a, b.seg_len);
+    const auto run = [&](std::initializer_list<Role> roles, int dx, int mode) {
+        p.n_roles = 0;
+        for (const Role& r : roles) p.role[p.n_roles++] = r;
+        return mode == STATES ? launch_segments(p, a.dtype, dx, st) : launch(p, a.dtype, dx, mode, st);
+    };
+    const bool want_dv = a.dv || a.dstate, want_dk = a.dk || a.dg, want_dq = a.dq || a.dg;
+    if (b.dv.seg) {
+        if (want_dv && (s = run({b.dv}, b.dxk, STATES)) != VRWKV_OK) return s;
+        if (want_dk && want_dq) s = run({b.dk, b.dq}, b.dxv, STATES);
+        else if (want_dk || want_dq) s = run({want_dk ? b.dk : b.dq}, b.dxv, STATES);
+        if (s != VRWKV_OK) return s;
+    }
+    if (want_dv && (s = run({b.dv}, b.dxk, PLAIN)) != VRWKV_OK) return s;
+    if (want_dk && (s = run({b.dk}, b.dxv, a.dg ? EDGES : ALONE)) != VRWKV_OK) return s;
+    if (want_dq && (s = run({b.dq}, b.dxv, a.dg ? FLOWS : ALONE)) != VRWKV_OK) return s;
+    struct { const float* part; void* out; int heads, D; } sums[3] = {{b.fq, a.dq, a.Hq, a.Dk}, {b.fk, a.dk, a.Hk, a.Dk}, {b.fv, a.dv, a.Hv, a.Dv}};
+    for (const auto& t : sums)
+        if (t.part) {
+            if (a.dtype == VRWKV_F32) head_sums<float>(t.part, t.out, a, t.heads, t.D, st);
+            else if (a.dtype == VRWKV_BF16) head_sums<__hip_bfloat16>(t.part, t.out, a, t.heads, t.D, st);
+            else head_sums<__half>(t.part, t.out, a, t.heads, t.D, st);
+        }
+    if (b.fg) {
+        if (a.g_dtype == VRWKV_F32) decay_sums<float>(b, a, st);
+        else if (a.g_dtype == VRWKV_BF16) decay_sums<__hip_bfloat16>(b, a, st);
+        else decay_sums<__half>(b, a, st);
+    }
+    return check_launch(who);
+}
