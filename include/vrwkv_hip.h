@@ -333,8 +333,8 @@ int vrwkv_biwkv_bwd_like(const float* w, const float* u, const void* k, const vo
 
 /* ---- attention with a decay for each head: causal, with its state in and out (no counterpart in the reference) ----
  * S_t = exp(g_t) S_{t-1} + k_t v_t^T, y_t = scale S_t^T q_t for every sequence and head.
- * q: rows of Hq heads of Dk, k: Hk of Dk, v: Hv of Dv channels, all of dtype, channels side by side, any strides (in elements) for batch, token and
- * head; head h of the H reads head h / (H / Hq) of q, and so on.  g: log decays of g_dtype at strides of batch, token and head (0 for a decay that all
+ * q: rows of Hq heads of Dk, k: Hk of Dk, v: Hv of Dv channels, all of dtype, channels side by side, any strides (in elements) for batch, token (less
+ * than 2^22) and head; head h of the H reads head h / (H / Hq) of q, and so on.  g: log decays of g_dtype at strides of batch, token and head (0 for a decay that all
  * tokens share); below -200 (-inf) they count as -200, whose exponential is zero in fp32 as well; above 0 they make states grow.  Head sizes 1 to 128; each of Hq, Hk, Hv divides H.
  * N rows of T tokens; or with offsets (N + 1 of them, 32 or 64 bits, on the device) N sequences packed in T rows, n at rows offsets[n] to offsets[n + 1],
  * in ascending order, empty ones among them; strides of batch are not looked at.  Offsets outside 0..T are taken as 0 or T.

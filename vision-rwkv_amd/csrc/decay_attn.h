@@ -12,6 +12,7 @@
 // tokens from j on is the same sum, with the difference of two large ones where little crosses.
 // Sequences of few calls are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
 #pragma once
+#include "wave_sum.h"
 #include "wkv6_chunk_common.h"
 
 namespace vrwkv {
@@ -25,16 +26,16 @@ using wkv6_detail::u32x4;
 constexpr int TZ = 64;                                    // columns of a state that a workgroup holds
 constexpr int THREADS = 256;
 
-// A tensor (batch, token, head, channel), channels side by side; head h of the call reads head h / share.  vec: rows in 16-byte pieces.
+// A tensor (batch, token, head, channel), channels side by side; head h of the call reads head h / share.
 struct View {
     const void* p;
     long long sb, st, sh;
-    int share, vec;
+    int share;
 };
 struct OutView {
     void* p;
     long long sb, st, sh;
-    int f32, vec;                                         // f32: fp32 values of every head, added up and rounded by a kernel behind
+    int f32;                                              // fp32 values of every head, added up and rounded by a kernel behind
 };
 struct Role {
     View a, b, c, e;
@@ -107,7 +108,7 @@ __device__ __forceinline__ Place find_place(const Params& p, int gid, int L) {
             const int i = m + threadIdx.x;
             seen += __syncthreads_count(i < p.N && offset_at(p, min(i, p.N - 1)) / p.seg_len + i <= gid);
         }
-        n = seen - 1;
+        n = __builtin_amdgcn_readfirstlane(seen - 1);
     }
     if (n < 0) {
         Place w{};
@@ -132,32 +133,34 @@ __device__ __forceinline__ float log_decay(const Params& p, int base, int token,
     return x < -200.f ? -200.f : x;                       // (exp(-200) is zero in fp32 too; sums of -inf or the lowest value would be -inf, their differences NaN)
 }
 
-// The eight channels d .. d + 7 of a row of dim, zeros behind its end.
+// The eight channels d .. d + 7 of a row: at byte offset `at` of the buffer in one or two loads of 16 bytes where rows come in such pieces (VEC), element by
+// element otherwise; `count` of them exist.  What does not is asked of an offset outside the buffer and arrives as zero, without a branch: loads behind
+// branches were waited for one by one, 4.5 of the 5.5 us that a chunk took.
 template <typename IO> struct Piece { unsigned w[sizeof(IO) * 2]; };
-template <typename IO>
-__device__ __forceinline__ Piece<IO> load_piece(const IO* row, int d, int dim, bool inside, int vec) {
+template <typename IO, bool VEC>
+__device__ __forceinline__ Piece<IO> load_piece(__amdgpu_buffer_rsrc_t buf, unsigned at, int count) {
     Piece<IO> r;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(IO) * 2; ++i) r.w[i] = 0;
-    if (!inside || d >= dim) return r;
-    if (vec && d + 8 <= dim) {
-        const u32x4* s = reinterpret_cast<const u32x4*>(row + d);
+    if constexpr (VEC) {
+        const unsigned o = count > 0 ? at : OOB_OFFSET;
 #pragma unroll
         for (int i = 0; i < (int)sizeof(IO) / 2; ++i) {
-            const u32x4 t = s[i];
+            const auto t = BufRaw<16>::ld(buf, o + 16 * i, 0);
 #pragma unroll
             for (int c = 0; c < 4; ++c) r.w[4 * i + c] = t[c];
         }
-    } else {
+    } else if constexpr (sizeof(IO) == 4) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (d + e < dim) {
-                if constexpr (sizeof(IO) == 4) r.w[e] = reinterpret_cast<const unsigned*>(row)[d + e];
-                else r.w[e / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(row)[d + e] << (16 * (e & 1));
-            }
+        for (int e = 0; e < 8; ++e) r.w[e] = BufRaw<4>::ld(buf, e < count ? at + 4 * e : OOB_OFFSET, 0);
+    } else {
+        unsigned short h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = BufRaw<2>::ld(buf, e < count ? at + 2 * e : OOB_OFFSET, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.w[e] = (unsigned)h[2 * e] | (unsigned)h[2 * e + 1] << 16;
     }
     return r;
 }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) { return make_rsrc(p, 0x7fffffffu); }
 // x as the sum of n bf16 numbers (two at a time): 16 bits of it with two, all 24 with three
 template <int N>
 __device__ __forceinline__ void split_pair(float x0, float x1, unsigned (&t)[N]) {
@@ -211,14 +214,40 @@ __device__ __forceinline__ f32x4 mma(f32x4 acc, const bf16x8 (&a)[NA], const bf1
     return acc;
 }
 
-// sum over the lanes up to this one
-__device__ __forceinline__ double wave_scan_inclusive(double x, int lane) {
+// sum over the lanes up to this one: inside 16 lanes, then the rows' totals (DPP moves; lanes without a source add zero)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, ROWS, 0xf, false);
+    return x + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan_inclusive(double x) {
+    x = dpp_add<0x111, 0xf>(x);                           // row_shr:1, 2, 4, 8
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);                           // row_bcast:15 into rows 1 and 3, row_bcast:31 into 2 and 3
+    return dpp_add<0x143, 0xc>(x);
+}
+
+// Four channels of a row, `count` of them there.
+template <typename O, bool VEC>
+__device__ __forceinline__ void store_quad(__amdgpu_buffer_rsrc_t buf, unsigned at, int count, f32x4 x) {
+    O q[4];
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double o = __shfl_up(x, d);
-        if (lane >= d) x += o;
+    for (int i = 0; i < 4; ++i) q[i] = from_f32<O>(x[i]);
+    if constexpr (VEC) {
+        typename BufRaw<4 * sizeof(O)>::type d;
+        __builtin_memcpy(&d, q, sizeof(d));
+        BufRaw<4 * sizeof(O)>::st(d, buf, count > 0 ? at : OOB_OFFSET, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            typename BufRaw<sizeof(O)>::type d;
+            __builtin_memcpy(&d, &q[i], sizeof(d));
+            BufRaw<sizeof(O)>::st(d, buf, i < count ? at + i * (unsigned)sizeof(O) : OOB_OFFSET, 0);
+        }
     }
-    return x;
 }
 
 template <typename IO, int DX, int MODE>
@@ -232,8 +261,10 @@ struct Lds {
     __bf16 c[NS][L][PZ];
     __bf16 e[MODE == EDGES || MODE == FLOWS ? NS : 1][MODE == EDGES || MODE == FLOWS ? L : 1][PZ];
     u32x4 s[MODE == STATES ? 1 : NI][4][MODE == STATES ? 1 : DX / 32][64];   // the state's terms, a lane's fragment side by side
-    float gh[64], gl[64], dt[64], dk[64];                 // G in powers of two, head and tail; exp(G); exp(G_end - G)
-    float end_decay, through_decay;                       // exp(G_end); FLOWS: with the decay of the token behind the chunk
+    struct Decays {
+        float gh[64], gl[64], dt[64], dk[64];             // G in powers of two, head and tail; exp(G); exp(G_end - G)
+        float end, through;                               // exp(G_end); FLOWS: with the decay of the token behind the chunk
+    } d[2];                                               // this chunk's and the next one's
     float edge[2][64], inner[4][64], cross[4];            // what rows get or give across the chunk's ends, by halves of the columns; what crosses tokens inside, by waves; <S0, R>
 };
 
@@ -259,15 +290,17 @@ __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, in
     }
 }
 
-template <typename IO, int DX, int MODE>
-__global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
+template <typename IO, int DX, int MODE> constexpr int workgroups = sizeof(Lds<IO, DX, MODE>) <= 53 * 1024 ? 3 : sizeof(Lds<IO, DX, MODE>) <= 80 * 1024 ? 2 : 1;   // that the LDS of a compute unit holds
+
+template <typename IO, int DX, int MODE, bool VEC>
+__global__ __launch_bounds__(THREADS, (workgroups<IO, DX, MODE>)) void decay_kernel(const Params p) {
     using S = Lds<IO, DX, MODE>;
     constexpr int L = S::L, NS = S::NS, NI = S::NI, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
     constexpr int PA = L * DX / 8 / THREADS, PC = (L * TZ / 8 + THREADS - 1) / THREADS;
     static_assert(PA >= 1 && L * DX % (8 * THREADS) == 0 && L * TZ % (8 * THREADS) == 0, "");
     constexpr bool OUT = MODE != STATES, EXTRA = MODE == EDGES || MODE == FLOWS;
     __shared__ S lds;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quarter = lane >> 4, col = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
 
     // workgroup -> role, tile, head, segment (segments of a head next to each other are on different chiplets; the roles of one share its rows)
     int id = blockIdx.x;
@@ -311,47 +344,69 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
     }
 
     const int nc = (w.s1 - w.s0 + L - 1) / L;
-    const IO* const pa = static_cast<const IO*>(r.a.p) + w.base * r.a.sb + (long long)w.first * r.a.st + (h / r.a.share) * r.a.sh;
-    const IO* const pb = static_cast<const IO*>(r.b.p) + w.base * r.b.sb + (long long)w.first * r.b.st + (h / r.b.share) * r.b.sh;
-    const IO* const pc = static_cast<const IO*>(r.c.p) + w.base * r.c.sb + (long long)w.first * r.c.st + (h / r.c.share) * r.c.sh;
-    const IO* const pe = EXTRA ? static_cast<const IO*>(r.e.p) + w.base * r.e.sb + (long long)w.first * r.e.st + (h / r.e.share) * r.e.sh : nullptr;
+    const auto origin = [&](const View& v) { return static_cast<const IO*>(v.p) + w.base * v.sb + (long long)w.first * v.st + (h / v.share) * v.sh; };
+    const IO *const pa = origin(r.a), *const pb = origin(r.b), *const pc = origin(r.c), *const pe = EXTRA ? origin(r.e) : nullptr;
+    char* const po = static_cast<char*>(r.o.p) + (w.base * r.o.sb + (long long)w.first * r.o.st + h * r.o.sh) * (r.o.f32 ? 4 : (int)sizeof(IO));
 
+    // The chunk's rows in the order that the kernel takes them: row i is token t0 + i, or t0 + n - 1 - i back along the tokens, which is L - 1 - i from
+    // token t0 + n - L on; so a thread's offsets stay the same, and which rows there are is asked on top.
     Piece<IO> ra[OUT ? PA : 1], rb[PA], rc[PC], re[EXTRA ? PC : 1];
     float rg = 0.f, rg_next = 0.f;
-    // the rows of chunk c of the segment's, and their decays
+    const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, rowz = tid / (TZ / 8), dzo = z0 + tid % (TZ / 8) * 8;
+    constexpr int STEPX = THREADS / (DX / 8), STEPZ = THREADS / (TZ / 8);   // rows between a thread's pieces
+    const int countx = r.dx - dxo, countz = r.dz - dzo;
     const auto fetch = [&](int c) {
         const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+        const long long tok = rev ? t0 + n - L : t0;
+        const auto buf = [&](const IO* q, const View& v) { return buffer_at(q + tok * v.st); };
+        const auto at = [&](int row, const View& v, int d) { return (unsigned)(((rev ? L - 1 - row : row) * (int)v.st + d) * (int)sizeof(IO)); };
+        const auto ba = buf(OUT ? pa : pb, OUT ? r.a : r.b), bb = buf(pb, r.b), bc = buf(pc, r.c), be = buf(EXTRA ? pe : pc, EXTRA ? r.e : r.c);
 #pragma unroll
         for (int i = 0; i < PA; ++i) {
-            const int pi = tid + THREADS * i, row = pi / (DX / 8), d = pi % (DX / 8) * 8;
-            const long long tok = rev ? t0 + n - 1 - row : t0 + row;
-            if constexpr (OUT) ra[i] = load_piece(pa + tok * r.a.st, d, r.dx, row < n, r.a.vec);
-            rb[i] = load_piece(pb + tok * r.b.st, d, r.dx, row < n, r.b.vec);
+            const int row = rowx + STEPX * i, m = row < n ? countx : 0;
+            if constexpr (OUT) ra[i] = load_piece<IO, VEC>(ba, at(row, r.a, dxo), m);
+            rb[i] = load_piece<IO, VEC>(bb, at(row, r.b, dxo), m);
         }
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
-            const int pi = tid + THREADS * i, row = pi / (TZ / 8), d = z0 + pi % (TZ / 8) * 8;
-            const long long tok = rev ? t0 + n - 1 - row : t0 + row;
-            rc[i] = load_piece(pc + tok * r.c.st, d, r.dz, row < n, r.c.vec);
-            if constexpr (EXTRA) re[i] = load_piece(pe + tok * r.e.st, d, r.dz, row < n, r.e.vec);
+            const int row = rowz + STEPZ * i, m = row < n ? countz : 0;
+            rc[i] = load_piece<IO, VEC>(bc, at(row, r.c, dzo), m);
+            if constexpr (EXTRA) re[i] = load_piece<IO, VEC>(be, at(row, r.e, dzo), m);
         }
         if (wave == 0) {
             // back along the tokens a row's decay is that of the token behind it, and none behind the last
-            const int tok = rev ? t0 + n - lane : t0 + lane;
-            rg = lane < n && tok < w.len ? log_decay(p, w.base, w.first + tok, h) : 0.f;
+            const int g = rev ? t0 + n - lane : t0 + lane;
+            rg = lane < n && g < w.len ? log_decay(p, w.base, w.first + g, h) : 0.f;
             if constexpr (MODE == FLOWS) rg_next = t0 + n < w.len ? log_decay(p, w.base, w.first + t0 + n, h) : 0.f;
         }
     };
-    if (nc > 0) fetch(rev ? nc - 1 : 0);
-
     float seg_log = 0.f;                                  // (STATES: the segment's whole decay, from wave 0)
+    const auto put_decays = [&](typename S::Decays& d) {   // wave 0
+        // sums in 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth
+        const double G = wave_scan_inclusive((double)rg * 1.4426950408889634);
+        const unsigned long long bits = __builtin_bit_cast(unsigned long long, G);
+        const double end = __builtin_bit_cast(double, (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((int)bits, 63));
+        const float gh = (float)G;
+        d.gh[lane] = gh;
+        d.gl[lane] = (float)(G - gh);
+        d.dt[lane] = fast_exp2(gh);
+        d.dk[lane] = fast_exp2((float)(end - G));
+        if (lane == 0) {
+            d.end = fast_exp2((float)end);
+            if constexpr (MODE == FLOWS) d.through = fast_exp2((float)(end + (double)rg_next * 1.4426950408889634));
+        }
+        if (MODE == STATES) seg_log += (float)end;
+    };
+    if (nc > 0) {
+        fetch(rev ? nc - 1 : 0);
+        if (wave == 0) put_decays(lds.d[0]);
+    }
     for (int ci = 0; ci < nc; ++ci) {
         const int c = rev ? nc - 1 - ci : ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
         // ---- operands to the LDS
 #pragma unroll
         for (int i = 0; i < PA; ++i) {
-            const int pi = tid + THREADS * i, row = pi / (DX / 8), d = pi % (DX / 8) * 8;
-            const int o0 = order_of(d), o1 = order_of(d + 4);
+            const int row = rowx + STEPX * i, o0 = order_of(dxo), o1 = order_of(dxo + 4);
             u32x4 t[NS];
             if constexpr (OUT) {
                 piece_terms<IO>(ra[i], t);
@@ -370,7 +425,7 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
         }
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
-            const int pi = tid + THREADS * i, row = pi / (TZ / 8), d = pi % (TZ / 8) * 8;
+            const int row = rowz + STEPZ * i, d = dzo - z0;
             u32x4 t[NS];
             piece_terms<IO>(rc[i], t);
 #pragma unroll
@@ -393,37 +448,54 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
                 }
             }
         }
-        if (wave == 0) {
-            // sums in 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth
-            const double G = wave_scan_inclusive((double)rg * 1.4426950408889634, lane);
-            const double end = __shfl(G, 63);
-            const float gh = (float)G;
-            lds.gh[lane] = gh;
-            lds.gl[lane] = (float)(G - gh);
-            lds.dt[lane] = fast_exp2(gh);
-            lds.dk[lane] = fast_exp2((float)(end - G));
-            if (lane == 0) {
-                lds.end_decay = fast_exp2((float)end);
-                if constexpr (MODE == FLOWS) lds.through_decay = fast_exp2((float)(end + (double)rg_next * 1.4426950408889634));
-            }
-            if (MODE == STATES) seg_log += (float)end;
-        }
         __syncthreads();
         if (ci + 1 < nc) fetch(rev ? c - 1 : c + 1);
+        typename S::Decays& dec_ = lds.d[ci & 1];
 
         // ---- outputs of rows 16 tw + col, columns 16 zt + 4 quarter + i
-        if constexpr (OUT) {
-            const int tw = wave % NT, zt0 = wave / NT * NT;
-            const int t = 16 * tw + col;
-            const float gth = lds.gh[t], gtl = lds.gl[t], dec = lds.dt[t] * r.s_in;
+        f32x4 behind[MODE == FLOWS ? NX : 1];              // R behind this chunk, as the pass of dk left it
+        float given = 0.f;                                // (wave 0) what its tokens give over its end
+        if constexpr (MODE == FLOWS) {
+            const long long ck = (((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * r.tiles + z) * (DX * TZ);
+#pragma unroll
+            for (int x = 0; x < NX; ++x) behind[x] = *reinterpret_cast<const f32x4*>(r.anchors + ck + ((x * 4 + wave) * 64 + lane) * 4);
+            if (wave == 0 && lane < n) given = r.edge[((long long)z * p.rows + (long long)w.base * p.T + w.first + t0 + lane) * p.H + h];
+        }
+        const int tw = wave % NT, zt0 = wave / NT * NT, t = 16 * tw + col;
+        if (OUT && 16 * tw < n) {
+            const float gth = dec_.gh[t], gtl = dec_.gl[t], dec = dec_.dt[t] * r.s_in;
             bf16x8 fa[KX][NS];
 #pragma unroll
             for (int kx = 0; kx < KX; ++kx)
 #pragma unroll
-                for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[s][t][kx * 32 + 8 * quarter]);
-            f32x4 acc[NT], far[NT];
+                for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[OUT ? s : 0][OUT ? t : 0][kx * 32 + 8 * quarter]);
+            // what the state in front gives
+            f32x4 acc[NT];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j] = far[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            float edge = 0.f;
+            if (have) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                    for (int kx = 0; kx < KX; ++kx) {
+                        bf16x8 fs[NI];
+#pragma unroll
+                        for (int s = 0; s < NI; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[OUT ? s : 0][zt0 + j][OUT ? kx : 0][lane]);
+                        acc[j] = mma<NI - 1>(acc[j], fs, fa[kx]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[j][i] *= dec;
+                        if constexpr (EXTRA) {
+                            float x = 0.f;
+#pragma unroll
+                            for (int s = NS - 1; s >= 0; --s) x += (float)lds.e[s][t][16 * (zt0 + j) + 4 * quarter + i];
+                            edge = fmaf(x, acc[j][i], edge);
+                        }
+                    }
+                }
+            }
             f32x4 flow[MODE == FLOWS ? NT : 1];            // [tile of j]: sums over s < j of the terms of row t
 #pragma unroll
             for (int j = 0; j < (MODE == FLOWS ? NT : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -443,10 +515,10 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
                             for (int s = 0; s < NS; ++s) fb[s] = *reinterpret_cast<const bf16x8*>(&lds.b[s][16 * st_ + col][kx * 32 + 8 * quarter]);
                             m = mma<NI - 1>(m, fb, fa[kx]);
                         }
-                        const f32x4 sh = *reinterpret_cast<const f32x4*>(&lds.gh[16 * st_ + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&lds.gl[16 * st_ + 4 * quarter]);
+                        const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec_.gh[16 * st_ + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec_.gl[16 * st_ + 4 * quarter]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float x = m[i] * fast_exp2((gth - sh[i]) + (gtl - sl[i]));
+                            const float x = m[i] * (p.scale * fast_exp2((gth - sh[i]) + (gtl - sl[i])));
                             m[i] = st_ < tw || 4 * quarter + i <= col ? x : 0.f;
                         }
                         if constexpr (MODE == FLOWS) {
@@ -503,50 +575,15 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
                     acc[j] = mma<NP - 1>(acc[j], fc, fp);
                 }
             }
-            if (have) {
+            if (r.o.p) {
+                const long long tok = rev ? t0 + n - L : t0;
+                const auto bo = buffer_at(po + tok * r.o.st * (r.o.f32 ? 4 : (int)sizeof(IO)));
+                const int zl = z0 + 16 * zt0 + 4 * quarter, count = t < n ? r.dz - zl : 0;
+                const unsigned at = (unsigned)((rev ? L - 1 - t : t) * (int)r.o.st + zl);
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int kx = 0; kx < KX; ++kx) {
-                        bf16x8 fs[NI];
-#pragma unroll
-                        for (int s = 0; s < NI; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane]);
-                        far[j] = mma<NI - 1>(far[j], fs, fa[kx]);
-                    }
-            }
-            const long long tok = w.first + (rev ? t0 + n - 1 - t : t0 + t);
-            float edge = 0.f;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int zl = 16 * (zt0 + j) + 4 * quarter;
-                f32x4 o;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = dec * far[j][i];
-                    o[i] = fmaf(p.scale, acc[j][i], f);
-                    if constexpr (EXTRA) {
-                        float x = 0.f;
-#pragma unroll
-                        for (int s = NS - 1; s >= 0; --s) x += (float)lds.e[s][t][zl + i];
-                        edge = fmaf(x, f, edge);
-                    }
-                }
-                if (t < n && r.o.p) {
-                    const long long at = w.base * r.o.sb + tok * r.o.st + h * r.o.sh + z0 + zl;
-                    if (r.o.f32) {
-                        float* q = static_cast<float*>(r.o.p) + at;
-                        if (r.o.vec && z0 + zl + 4 <= r.dz) *reinterpret_cast<f32x4*>(q) = o;
-                        else
-                            for (int i = 0; i < 4; ++i)
-                                if (z0 + zl + i < r.dz) q[i] = o[i];
-                    } else {
-                        IO* q = static_cast<IO*>(r.o.p) + at;
-                        const float x4[4] = {o[0], o[1], o[2], o[3]};
-                        if (r.o.vec && z0 + zl + 4 <= r.dz) store_vec<IO, 4>(q, x4);
-                        else
-                            for (int i = 0; i < 4; ++i)
-                                if (z0 + zl + i < r.dz) q[i] = from_f32<IO>(x4[i]);
-                    }
+                for (int j = 0; j < NT; ++j) {
+                    if (r.o.f32) store_quad<float, VEC>(bo, (at + 16 * j) * 4, count - 16 * j, acc[j]);
+                    else store_quad<IO, VEC>(bo, (at + 16 * j) * (unsigned)sizeof(IO), count - 16 * j, acc[j]);
                 }
             }
             if constexpr (EXTRA) {                        // over the quarters: the channels of a row
@@ -563,26 +600,17 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
                 int index;
                 const float cf = wkv6_detail::row_sums16(crossing, lane, index);
                 // (the other waves of a 32-token chunk have made the same terms)
-                lds.inner[wave][16 * (index >> 2) + 4 * quarter + (index & 3)] = wave < NT ? cf * p.scale : 0.f;
-                // <S0, R>: R behind this chunk, as the pass of dk left it
-                float x = 0.f;
-                if (have) {
-                    const long long ck = (((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * r.tiles + z) * (DX * TZ);
-#pragma unroll
-                    for (int x4 = 0; x4 < NX; ++x4) {
-                        const f32x4 a4 = *reinterpret_cast<const f32x4*>(r.anchors + ck + ((x4 * 4 + wave) * 64 + lane) * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x = fmaf(st[x4][i], a4[i], x);
-                    }
-                }
-                x += __shfl_xor(x, 1);
-                x += __shfl_xor(x, 2);
-                x += __shfl_xor(x, 4);
-                x += __shfl_xor(x, 8);
-                x += __shfl_xor(x, 16);
-                x += __shfl_xor(x, 32);
-                if (lane == 0) lds.cross[wave] = x;
+                lds.inner[wave][16 * (index >> 2) + 4 * quarter + (index & 3)] = wave < NT ? cf : 0.f;
             }
+        } else if (MODE == FLOWS) lds.inner[wave][lane] = 0.f;
+        if constexpr (MODE == FLOWS) {
+            float x = 0.f;                                // <S0, R>
+#pragma unroll
+            for (int x4 = 0; x4 < NX; ++x4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x = fmaf(st[x4][i], behind[x4][i], x);
+            x = wave_sum(x);
+            if (lane == 0) lds.cross[wave] = x;
         }
 
         // ---- the state behind the chunk
@@ -592,15 +620,16 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
 #pragma unroll
                 for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.anchors + ck + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
             }
-            const float ed = lds.end_decay;
+            const float ed = dec_.end;
 #pragma unroll
             for (int x = 0; x < NX; ++x)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) st[x][i] *= ed;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
+                if (32 * ks >= n) break;
                 float x8[8];
-                const f32x4 d0 = *reinterpret_cast<const f32x4*>(&lds.dk[32 * ks + 4 * quarter]), d1 = *reinterpret_cast<const f32x4*>(&lds.dk[32 * ks + 16 + 4 * quarter]);
+                const f32x4 d0 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 4 * quarter]), d1 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 16 + 4 * quarter]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x8[i] = 0.f;
 #pragma unroll
@@ -630,6 +659,7 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
             }
             have = true;
         }
+        if (wave == 0 && ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
         __syncthreads();
         if constexpr (MODE == EDGES) {
             if (wave == 0 && lane < n) {
@@ -645,9 +675,9 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
                 double in = 0., out = 0.;
                 if (lane < n) {
                     in = NT == 4 ? lds.edge[0][lane] : (double)lds.edge[0][lane] + lds.edge[1][lane];
-                    out = r.edge[at];
+                    out = given;
                 }
-                double before = wave_scan_inclusive(out, lane);
+                double before = wave_scan_inclusive(out);
                 before = __shfl_up(before, 1);
                 if (lane == 0) before = 0.;
 #pragma unroll
@@ -656,7 +686,7 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
                     if (lane + d < 64) in += o;
                 }
                 const double inner = ((double)lds.inner[0][lane] + lds.inner[1][lane]) + ((double)lds.inner[2][lane] + lds.inner[3][lane]);
-                const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * lds.through_decay;
+                const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * dec_.through;
                 if (lane < n) r.dg[at] = (float)(inner + in + before + through);
             }
         }
@@ -682,29 +712,28 @@ __global__ __launch_bounds__(THREADS, 2) void decay_kernel(const Params p) {
 }
 
 // How the host reaches the instances of each type.
-template <typename IO> int launch_decay(const Params& p, int dx, int mode, hipStream_t st);
-extern template int launch_decay<float>(const Params&, int, int, hipStream_t);
-extern template int launch_decay<__hip_bfloat16>(const Params&, int, int, hipStream_t);
-extern template int launch_decay<__half>(const Params&, int, int, hipStream_t);
+template <typename IO> int launch_decay(const Params& p, int dx, int mode, bool vec, hipStream_t st);
+extern template int launch_decay<float>(const Params&, int, int, bool, hipStream_t);
+extern template int launch_decay<__hip_bfloat16>(const Params&, int, int, bool, hipStream_t);
+extern template int launch_decay<__half>(const Params&, int, int, bool, hipStream_t);
 
+template <typename IO, int DX, bool VEC>
+void launch_mode(const Params& p, int mode, dim3 grid, hipStream_t st) {
+    const dim3 block(THREADS);
+    if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, DX, PLAIN, VEC>), grid, block, 0, st, p);
+    else if (mode == EDGES) hipLaunchKernelGGL((decay_kernel<IO, DX, EDGES, VEC>), grid, block, 0, st, p);
+    else if (mode == FLOWS) hipLaunchKernelGGL((decay_kernel<IO, DX, FLOWS, VEC>), grid, block, 0, st, p);
+    else if (mode == ALONE) hipLaunchKernelGGL((decay_kernel<IO, DX, ALONE, VEC>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((decay_kernel<IO, DX, STATES, VEC>), grid, block, 0, st, p);
+}
+// vec: every row of every role in pieces of 16 bytes
 template <typename IO>
-int launch_decay(const Params& p, int dx, int mode, hipStream_t st) {
+int launch_decay(const Params& p, int dx, int mode, bool vec, hipStream_t st) {
     int tiles = 1;
     for (int i = 0; i < p.n_roles; ++i) tiles = p.role[i].tiles > tiles ? p.role[i].tiles : tiles;
-    const dim3 grid((unsigned)((long long)p.segs * p.H * tiles * p.n_roles)), block(THREADS);
-    if (dx <= 64) {
-        if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, 64, PLAIN>), grid, block, 0, st, p);
-        else if (mode == EDGES) hipLaunchKernelGGL((decay_kernel<IO, 64, EDGES>), grid, block, 0, st, p);
-        else if (mode == FLOWS) hipLaunchKernelGGL((decay_kernel<IO, 64, FLOWS>), grid, block, 0, st, p);
-        else if (mode == ALONE) hipLaunchKernelGGL((decay_kernel<IO, 64, ALONE>), grid, block, 0, st, p);
-        else hipLaunchKernelGGL((decay_kernel<IO, 64, STATES>), grid, block, 0, st, p);
-    } else {
-        if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, 128, PLAIN>), grid, block, 0, st, p);
-        else if (mode == EDGES) hipLaunchKernelGGL((decay_kernel<IO, 128, EDGES>), grid, block, 0, st, p);
-        else if (mode == FLOWS) hipLaunchKernelGGL((decay_kernel<IO, 128, FLOWS>), grid, block, 0, st, p);
-        else if (mode == ALONE) hipLaunchKernelGGL((decay_kernel<IO, 128, ALONE>), grid, block, 0, st, p);
-        else hipLaunchKernelGGL((decay_kernel<IO, 128, STATES>), grid, block, 0, st, p);
-    }
+    const dim3 grid((unsigned)((long long)p.segs * p.H * tiles * p.n_roles));
+    if (dx <= 64) vec ? launch_mode<IO, 64, true>(p, mode, grid, st) : launch_mode<IO, 64, false>(p, mode, grid, st);
+    else vec ? launch_mode<IO, 128, true>(p, mode, grid, st) : launch_mode<IO, 128, false>(p, mode, grid, st);
     return check_launch("decay_attention");
 }
 

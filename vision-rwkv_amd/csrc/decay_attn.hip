@@ -152,6 +152,9 @@ int check_tensors(const vrwkv_decay_args& a, const char* who) {
     const size_t m = elem(a.dtype) - 1;
     for (const void* p : {a.q, a.k, a.v, (const void*)a.y, a.gy, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv})
         if ((size_t)p & m) { set_error("%s: a tensor is not aligned to its elements", who); return VRWKV_INVALID_ARG; }
+    // (offsets inside a chunk's rows are 32 bits)
+    for (const long long st : {a.q_stride[1], a.k_stride[1], a.v_stride[1], a.gy ? a.gy_stride[1] : 0, (long long)a.H * std::max(a.Dk, a.Dv)})
+        if (st < 0 || st >= 1 << 22) { set_error("%s: tokens %lld elements apart, at most 2^22", who, st); return VRWKV_UNSUPPORTED_SHAPE; }
     for (const void* p : {a.g, (const void*)a.dg})
         if ((size_t)p & (elem(a.g_dtype) - 1)) { set_error("%s: g is not aligned to its elements", who); return VRWKV_INVALID_ARG; }
     for (const void* p : {(const void*)a.state, (const void*)a.last, (const void*)a.glast, (const void*)a.dstate})
@@ -159,13 +162,21 @@ int check_tensors(const vrwkv_decay_args& a, const char* who) {
     if (a.offsets && ((size_t)a.offsets & (a.offsets64 ? 7 : 3))) { set_error("%s: offsets are not aligned to their elements", who); return VRWKV_INVALID_ARG; }
     return VRWKV_OK;
 }
-View view(const void* p, const long long (&s)[3], int heads, const vrwkv_decay_args& a) {
-    const long long per16 = 16 / (long long)elem(a.dtype);
-    return View{p, s[0], s[1], s[2], a.H / heads, ((size_t)p & 15) == 0 && s[0] % per16 == 0 && s[1] % per16 == 0 && s[2] % per16 == 0};
-}
+View view(const void* p, const long long (&s)[3], int heads, const vrwkv_decay_args& a) { return View{p, s[0], s[1], s[2], a.H / heads}; }
 OutView out_view(void* p, int D, const vrwkv_decay_args& a, bool f32) {
-    const long long sh = D, st = (long long)a.H * D;
-    return OutView{p, st * a.T, st, sh, f32, ((size_t)p & (f32 ? 15 : 4 * elem(a.dtype) - 1)) == 0 && D % 4 == 0};
+    const long long st = (long long)a.H * D;
+    return OutView{p, st * a.T, st, D, f32};
+}
+// Whether a launch may read and write rows in 16-byte pieces.
+bool in_pieces(const Params& p, int dtype) {
+    const long long per16 = 16 / (long long)elem(dtype);
+    const auto fits = [&](const View& v, int d) { return !v.p || (((size_t)v.p & 15) == 0 && v.sb % per16 == 0 && v.st % per16 == 0 && v.sh % per16 == 0 && d % 8 == 0); };
+    bool vec = true;
+    for (int i = 0; i < p.n_roles; ++i) {
+        const Role& r = p.role[i];
+        vec = vec && fits(r.a, r.dx) && fits(r.b, r.dx) && fits(r.c, r.dz) && fits(r.e, r.dz) && ((size_t)r.o.p & 15) == 0;
+    }
+    return vec;
 }
 Params common(const vrwkv_decay_args& a, int seg_len) {
     Params p{};
@@ -187,9 +198,10 @@ Params common(const vrwkv_decay_args& a, int seg_len) {
     return p;
 }
 int launch(const Params& p, int dtype, int dx, int mode, hipStream_t st) {
-    if (dtype == VRWKV_F32) return launch_decay<float>(p, dx, mode, st);
-    if (dtype == VRWKV_BF16) return launch_decay<__hip_bfloat16>(p, dx, mode, st);
-    return launch_decay<__half>(p, dx, mode, st);
+    const bool vec = in_pieces(p, dtype);
+    if (dtype == VRWKV_F32) return launch_decay<float>(p, dx, mode, vec, st);
+    if (dtype == VRWKV_BF16) return launch_decay<__hip_bfloat16>(p, dx, mode, vec, st);
+    return launch_decay<__half>(p, dx, mode, vec, st);
 }
 // The segments' own states and the states in front of them, for the roles of p.
 int launch_segments(const Params& p, int dtype, int dx, hipStream_t st) {

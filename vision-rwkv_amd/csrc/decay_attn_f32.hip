@@ -3,6 +3,6 @@
 
 namespace vrwkv {
 namespace decay {
-template int launch_decay<float>(const Params&, int, int, hipStream_t);
+template int launch_decay<float>(const Params&, int, int, bool, hipStream_t);
 }
 }

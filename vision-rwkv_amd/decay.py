@@ -13,8 +13,8 @@ from .ops import _DT, _on, _stream_ptr, batched_cotangent
 
 
 def _rows(t):
-    """t as the kernels read it: any strides, but the channels of a head side by side."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t as the kernels read it: any strides, but the channels of a head side by side and tokens less than 2^22 elements apart."""
+    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() == 3 or t.stride(1) < 1 << 22) else t.contiguous()
 
 
 def _check(t, name, like=None):
