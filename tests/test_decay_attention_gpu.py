@@ -320,8 +320,9 @@ def pages_reference(pool, src, dst, source=None):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape,dtype", [((2, 8, 8), torch.float32), ((3, 5, 7), torch.float32), ((5, 7), torch.bfloat16), ((3,), torch.uint8), ((12, 64, 64), torch.float32)])
+@pytest.mark.parametrize("long", [False, True])
 @pytest.mark.parametrize("how", ["fork", "shift", "back", "cycle", "swap", "tree", "clear", "mixed", "random"])
-def test_pages(how, shape, dtype):
+def test_pages(how, shape, dtype, long):
     P = 40
     gen = np.random.default_rng(7)
     host = torch.from_numpy(gen.integers(0, 200, (P, *shape))).to(dtype)
@@ -331,6 +332,8 @@ def test_pages(how, shape, dtype):
              "clear": ([-1, -1, -1], [5, 0, 39]), "mixed": ([5, -1, 7, 50, 9, 9, -3, 2, 30], [7, 5, -1, 9, 40, 9, 11, 2, 30]),
              "random": (gen.integers(-1, P, 60).tolist(), gen.integers(-1, P, 60).tolist())}
     src, dst = lists[how]
+    if long:                                               # places that are not taken, up to a list of the length that is planned by itself
+        src, dst = src[:1] + [5] * 130 + src[1:] + [-9] * 130, dst[:1] + [-1] * 130 + dst[1:] + [3] * 130
     want = torch.from_numpy(pages_reference(host.float().numpy(), src, dst)).to(dtype)
     out = vr.copy_states(pool, torch.tensor(src, device=DEV, dtype=torch.int32), torch.tensor(dst, device=DEV))
     assert out is pool and torch.equal(pool.cpu(), want)
@@ -452,6 +455,23 @@ def test_nothing_in_it():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_serving_without_gradients(mode):
+    """Inference tensors have no version; others count the changes that are made in place."""
+    q, k, v, g, S = make(2, 6, 2, 2, 2, 2, 64, 64, "bf16", state=2)
+    with mode():
+        pool = S.clone()
+        version = None if pool.is_inference() else pool._version
+        y = torch.stack([vr.decay_attention_step(q[:, t], k[:, t], v[:, t], g[:, t], pool) for t in range(6)], 1)
+        vr.copy_states(pool, [1, 0], [0, 1])
+        vr.copy_states(pool, torch.tensor([1, 0], device=DEV), torch.tensor([0, 1], device=DEV))
+        assert version is None or pool._version == version + 8
+    want = reference(q, k, v, g, 1.0, S, [(0, 0, 6), (1, 0, 6)])
+    compare(y, want["y"], "y", "bf16", 64, 64, 6)
+    compare(pool, want["last"], "last", "fp32", 64, 64, 6)
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_gpu():
     r = lambda *s, dt=torch.float32: torch.randn(*s, device=DEV).to(dt)
     q, g = r(1, 4, 2, 8), r(1, 4, 2)
@@ -528,7 +548,7 @@ def test_the_library_refuses_before_it_launches():
     def pages(pool=1 << 20, stride=64, P=4, source=1 << 20, source_stride=64, source_P=4, size=64, src=4096, s64=0, dst=4096, d64=0, M=3, ws=4096, ws_bytes=1 << 20):
         return lib.vrwkv_copy_pages(pool, stride, P, source, source_stride, source_P, size, src, s64, dst, d64, M, ws, ws_bytes, None)
     for change, status in ((dict(pool=None), 1), (dict(src=None), 1), (dict(P=0), 1), (dict(M=0), 1), (dict(size=0), 1), (dict(M=4097), 3), (dict(stride=63), 1), (dict(source_stride=60), 1),
-                           (dict(src=4100, s64=1), 1), (dict(ws=None), 5), (dict(ws_bytes=11), 5), (dict(ws=4097), 1), (dict(source=(1 << 20) + 64), 1), (dict(source_stride=128), 1),
+                           (dict(src=4100, s64=1), 1), (dict(ws=None, M=300), 5), (dict(ws_bytes=1199, M=300), 5), (dict(ws=4097, M=300), 1), (dict(source=(1 << 20) + 64), 1), (dict(source_stride=128), 1),
                            (dict(size=1 << 30, stride=1 << 30, source_stride=1 << 30, M=4096), 3)):
         assert pages(**change) == status, change
-    assert lib.vrwkv_copy_pages_workspace_bytes(5) == 20 and lib.vrwkv_copy_pages_workspace_bytes(0) == 0
+    assert lib.vrwkv_copy_pages_workspace_bytes(300) == 1200 and lib.vrwkv_copy_pages_workspace_bytes(5) == lib.vrwkv_copy_pages_workspace_bytes(0) == 0

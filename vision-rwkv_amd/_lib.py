@@ -79,7 +79,7 @@ class _NoHost:
     def wkv(*args):
         return None
 
-    wkv6 = block_forward = wkv
+    wkv6 = block_forward = decay_attention = decay_step = copy_pages = wkv
 
     @staticmethod
     def weights_fit(*args):

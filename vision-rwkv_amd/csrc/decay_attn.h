@@ -61,11 +61,12 @@ struct Params {
     Role role[3];
 };
 template <typename IO> constexpr int in_terms = std::is_same<IO, float>::value ? 3 : std::is_same<IO, __half>::value ? 2 : 1;   // bf16 numbers that hold an element
-// tokens of a chunk: 64 where their rows and the state fit the LDS twice
-template <typename IO, int DX> constexpr int chunk_len = std::is_same<IO, __hip_bfloat16>::value || (std::is_same<IO, __half>::value && DX == 64) ? 64 : 32;
 
 // y and dv; dk with what dg needs of it; dq with dg; no outputs: a segment's own state; dk or dq without dg, the same bits as with it
 enum Mode { PLAIN = 0, EDGES = 1, FLOWS = 2, STATES = 3, ALONE = 4 };
+// tokens of a chunk: 64 where two workgroups' rows and states fit the LDS of a compute unit (fp32 rows take three times the room of bf16 ones, fp16 rows twice)
+template <typename IO, int DX, int MODE>
+constexpr int chunk_len = std::is_same<IO, __hip_bfloat16>::value || (std::is_same<IO, __half>::value && DX == 64 && (MODE == PLAIN || MODE == STATES)) ? 64 : 32;
 
 struct Place {                                            // a workgroup's segment
     int n, first, len;                                    // sequence; its first token and length
@@ -252,7 +253,7 @@ __device__ __forceinline__ void store_quad(__amdgpu_buffer_rsrc_t buf, unsigned 
 
 template <typename IO, int DX, int MODE>
 struct Lds {
-    static constexpr int L = chunk_len<IO, DX>, NS = in_terms<IO>;
+    static constexpr int L = chunk_len<IO, DX, MODE>, NS = in_terms<IO>;
     // terms of the products' intermediate operands: 16 bits of them for a 16-bit result, all 24 where fp32 ones depend on them: those of fp32 rows, and dg
     static constexpr int NP = NS < 3 ? 2 : 3, NI = MODE == PLAIN ? NP : 3;
     static constexpr int PX = DX + 8, PZ = TZ + 8;        // row pitches: 16 rows of a fragment on different banks
@@ -262,10 +263,10 @@ struct Lds {
     __bf16 e[MODE == EDGES || MODE == FLOWS ? NS : 1][MODE == EDGES || MODE == FLOWS ? L : 1][PZ];
     u32x4 s[MODE == STATES ? 1 : NI][4][MODE == STATES ? 1 : DX / 32][64];   // the state's terms, a lane's fragment side by side
     struct Decays {
-        float gh[64], gl[64], dt[64], dk[64];             // G in powers of two, head and tail; exp(G); exp(G_end - G)
+        float gh[L], gl[L], dt[L], dk[L];                 // G in powers of two, head and tail; exp(G); exp(G_end - G)
         float end, through;                               // exp(G_end); FLOWS: with the decay of the token behind the chunk
     } d[2];                                               // this chunk's and the next one's
-    float edge[2][64], inner[4][64], cross[4];            // what rows get or give across the chunk's ends, by halves of the columns; what crosses tokens inside, by waves; <S0, R>
+    float edge[2][L], inner[4][L], cross[4];            // what rows get or give across the chunk's ends, by halves of the columns; what crosses tokens inside, by waves; <S0, R>
 };
 
 // Eight channels from d on in the order that the accumulators' fragments have: inside 32 channels, 4 m .. 4 m + 3 lie at 8 (m & 3) + 4 (m >> 2).
@@ -290,10 +291,11 @@ __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, in
     }
 }
 
-template <typename IO, int DX, int MODE> constexpr int workgroups = sizeof(Lds<IO, DX, MODE>) <= 53 * 1024 ? 3 : sizeof(Lds<IO, DX, MODE>) <= 80 * 1024 ? 2 : 1;   // that the LDS of a compute unit holds
+// workgroups that a compute unit's LDS holds, up to three: more do not fit the registers
+template <size_t BYTES> constexpr int workgroups = 3 * BYTES <= 160 * 1024 ? 3 : 2 * BYTES <= 160 * 1024 ? 2 : 1;
 
 template <typename IO, int DX, int MODE, bool VEC>
-__global__ __launch_bounds__(THREADS, (workgroups<IO, DX, MODE>)) void decay_kernel(const Params p) {
+__global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) void decay_kernel(const Params p) {
     using S = Lds<IO, DX, MODE>;
     constexpr int L = S::L, NS = S::NS, NI = S::NI, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
     constexpr int PA = L * DX / 8 / THREADS, PC = (L * TZ / 8 + THREADS - 1) / THREADS;
@@ -328,10 +330,10 @@ __global__ __launch_bounds__(THREADS, (workgroups<IO, DX, MODE>)) void decay_ker
     if (MODE == STATES) {
 #pragma unroll
         for (int x = 0; x < NX; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-    } else if (r.seg) {
+    } else if (r.seg && !(rev ? w.is_last : w.is_first)) {
+        have = true;
 #pragma unroll
         for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4);
-        have = r.init || !(rev ? w.is_last : w.is_first);
     } else {
         have = r.init != nullptr;
 #pragma unroll
@@ -387,10 +389,12 @@ __global__ __launch_bounds__(THREADS, (workgroups<IO, DX, MODE>)) void decay_ker
         const unsigned long long bits = __builtin_bit_cast(unsigned long long, G);
         const double end = __builtin_bit_cast(double, (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((int)bits, 63));
         const float gh = (float)G;
-        d.gh[lane] = gh;
-        d.gl[lane] = (float)(G - gh);
-        d.dt[lane] = fast_exp2(gh);
-        d.dk[lane] = fast_exp2((float)(end - G));
+        if (lane < L) {
+            d.gh[lane] = gh;
+            d.gl[lane] = (float)(G - gh);
+            d.dt[lane] = fast_exp2(gh);
+            d.dk[lane] = fast_exp2((float)(end - G));
+        }
         if (lane == 0) {
             d.end = fast_exp2((float)end);
             if constexpr (MODE == FLOWS) d.through = fast_exp2((float)(end + (double)rg_next * 1.4426950408889634));
@@ -600,9 +604,9 @@ __global__ __launch_bounds__(THREADS, (workgroups<IO, DX, MODE>)) void decay_ker
                 int index;
                 const float cf = wkv6_detail::row_sums16(crossing, lane, index);
                 // (the other waves of a 32-token chunk have made the same terms)
-                lds.inner[wave][16 * (index >> 2) + 4 * quarter + (index & 3)] = wave < NT ? cf : 0.f;
+                if ((index >> 2) < NT) lds.inner[wave][16 * (index >> 2) + 4 * quarter + (index & 3)] = wave < NT ? cf : 0.f;
             }
-        } else if (MODE == FLOWS) lds.inner[wave][lane] = 0.f;
+        } else if (MODE == FLOWS && lane < L) lds.inner[wave][lane] = 0.f;
         if constexpr (MODE == FLOWS) {
             float x = 0.f;                                // <S0, R>
 #pragma unroll
@@ -674,7 +678,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<IO, DX, MODE>)) void decay_ker
                 // what token `lane` receives over the chunk's front and gives over its end; summed from it on, and up to it
                 double in = 0., out = 0.;
                 if (lane < n) {
-                    in = NT == 4 ? lds.edge[0][lane] : (double)lds.edge[0][lane] + lds.edge[1][lane];
+                    in = NT == 4 ? (double)lds.edge[0][lane] : (double)lds.edge[0][lane] + lds.edge[1][lane];
                     out = given;
                 }
                 double before = wave_scan_inclusive(out);
@@ -685,7 +689,8 @@ __global__ __launch_bounds__(THREADS, (workgroups<IO, DX, MODE>)) void decay_ker
                     const double o = __shfl_down(in, d);
                     if (lane + d < 64) in += o;
                 }
-                const double inner = ((double)lds.inner[0][lane] + lds.inner[1][lane]) + ((double)lds.inner[2][lane] + lds.inner[3][lane]);
+                const int at_lane = min(lane, L - 1);
+                const double inner = ((double)lds.inner[0][at_lane] + lds.inner[1][at_lane]) + ((double)lds.inner[2][at_lane] + lds.inner[3][at_lane]);
                 const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * dec_.through;
                 if (lane < n) r.dg[at] = (float)(inner + in + before + through);
             }

@@ -9,9 +9,10 @@ namespace decay {
 namespace {
 
 // The state in front of each segment from the segments' own ones: a lane carries four numbers along the sequence.
-// Grid (DX / 16 * N * H * tiles, 1, roles).  A segment's state is read once and written once, 32 KB for 64 channels; its loads do not wait for the sums.
+// Grid (DX / 16 * N * H * tiles, 1, roles).  Eight segments' states are on their way at
+// a time: one by one they were 0.35 us each.
 template <int DX>
-__global__ __launch_bounds__(THREADS) void segments_kernel(const Params p, int L) {
+__global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
     const Role& r = p.role[blockIdx.z];
     int id = blockIdx.x / (DX / 16);
     int tiles = 1;
@@ -20,7 +21,7 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p, int L
     id /= tiles;
     const int h = id % p.H, n = id / p.H;
     if (z >= r.tiles) return;
-    const Place w = sequence_place(p, n, L);
+    const Place w = sequence_place(p, n, 64);
     const int x = blockIdx.x % (DX / 16), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = first_segment(p, n, w.first), count = segment_count(p, w.len);
     f32x4 carry = {0.f, 0.f, 0.f, 0.f};
@@ -33,27 +34,27 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p, int L
             if (xc < r.dx && zc < r.dz) carry[i] = page[xc * r.sx + zc * r.sz];
         }
     }
-    const auto at = [&](int i) {                          // i-th on the way
-        const long long gid = first + (r.reverse ? count - 1 - i : i);
-        return gid;
-    };
-    f32x4 next = {0.f, 0.f, 0.f, 0.f};
-    float d = 1.f;
+    const auto at = [&](int i) { return ((long long)(first + (r.reverse ? count - 1 - i : i)) * p.H + h); };    // the i-th on the way
     const long long in_tile = ((long long)x * 4 + wave) * 64 * 4 + lane * 4;
-    const auto load = [&](int i) {
-        if (i + 1 < count) {                              // (the last one on the way has not been made)
-            next = *reinterpret_cast<const f32x4*>(r.seg + ((at(i) * p.H + h) * r.tiles + z) * (DX * TZ) + in_tile);
-            d = r.seg_decay[at(i) * p.H + h];
-        }
-    };
-    load(0);
-    for (int i = 0; i < count; ++i) {
-        const f32x4 own = next;
-        const float dec = d;
-        load(i + 1);
-        *reinterpret_cast<f32x4*>(r.seg + ((at(i) * p.H + h) * r.tiles + z) * (DX * TZ) + in_tile) = carry;
+    constexpr int U = 8;
+    if (count == 1) return;                               // (starts from what it is given)
+    for (int i0 = 0; i0 < count; i0 += U) {
+        f32x4 own[U];
+        float d[U];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) carry[c] = fmaf(carry[c], dec, own[c]);
+        for (int u = 0; u < U; ++u)
+            if (i0 + u + 1 < count) {                     // (the last one on the way has not been made)
+                own[u] = *reinterpret_cast<const f32x4*>(r.seg + (at(i0 + u) * r.tiles + z) * (DX * TZ) + in_tile);
+                d[u] = r.seg_decay[at(i0 + u)];
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u < count) {
+                if (i0 + u > 0) *reinterpret_cast<f32x4*>(r.seg + (at(i0 + u) * r.tiles + z) * (DX * TZ) + in_tile) = carry;
+                if (i0 + u + 1 < count)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) carry[c] = fmaf(carry[c], d[u], own[u][c]);
+            }
     }
 }
 
@@ -89,12 +90,13 @@ __global__ __launch_bounds__(THREADS) void decay_slices_kernel(const float* part
     if (sub == 0 && h < H) slices[(long long)blockIdx.x * H + h] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
 template <typename G>
-__global__ __launch_bounds__(THREADS) void decay_total_kernel(const double* slices, G* out, int n, int H) {
-    const int h = blockIdx.x * THREADS + threadIdx.x;
-    if (h >= H) return;
+__global__ __launch_bounds__(64) void decay_total_kernel(const double* slices, G* out, int n, int H) {
+    const int h = blockIdx.x, lane = threadIdx.x;
     double s = 0.;
-    for (int i = 0; i < n; ++i) s += slices[(long long)i * H + h];
-    out[h] = from_f32<G>((float)s);
+    for (int i = lane; i < n; i += 64) s += slices[(long long)i * H + h];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    if (lane == 0) out[h] = from_f32<G>((float)s);
 }
 
 constexpr int SLICES = 128;
@@ -102,22 +104,32 @@ constexpr int SLICES = 128;
 size_t elem(int dtype) { return dtype == VRWKV_F32 ? 4 : 2; }
 int pad_dx(int d) { return d <= 64 ? 64 : 128; }
 int tiles_of(int d) { return (d + TZ - 1) / TZ; }
-int chunk_of(int dtype, int dx) { return dtype == VRWKV_BF16 || (dtype == VRWKV_F16 && dx == 64) ? 64 : 32; }
+int chunk_of(int dtype) { return dtype == VRWKV_BF16 ? 64 : 32; }   // of dk and dq
 
-// Tokens of a segment.  A workgroup takes a chunk of 64 tokens in 1 to 2 us and two fit a compute unit: calls of fewer sequences and heads than fill
-// the chip are cut into segments of at least two chunks, which read their rows twice.
-int segment_len(const vrwkv_decay_args& a, int tiles, int roles) {
-    const long long wgs = (long long)a.H * tiles * roles, want = 3 * device_cus();
+// workgroups of a launch of outputs that the chip holds at once
+int slots(int dtype, int dx, bool backward) {
+    const int per_cu = dtype == VRWKV_BF16 ? (dx == 64 ? (backward ? 2 : 3) : (backward ? 1 : 2)) : dtype == VRWKV_F16 ? (dx == 64 || !backward ? 2 : 1) : dx == 64 ? 2 : 1;
+    return per_cu * device_cus();
+}
+// Tokens of a segment.  Calls of fewer sequences and heads than fill the chip are cut, into pieces that fill it in as few rounds as it takes: a round
+// lasts as long as its longest piece's chunks and about two more for its start; pieces cost another pass over their rows for their states,
+// half as long, and one over the states.
+int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool backward) {
+    const long long wgs = (long long)a.H * tiles * roles, room = slots(a.dtype, dx, backward);
     if (!a.offsets) {
-        const long long whole = wgs * a.N;
         const int chunks = (a.T + 63) / 64;
-        if (whole >= want / 2 || chunks < 4) return chunks * 64;
-        const long long pieces = std::min<long long>((want + whole - 1) / whole, chunks / 2);
-        return (int)((chunks + pieces - 1) / pieces) * 64;
+        int best = 1;
+        double least = 1e30;
+        for (int pieces = 1; pieces <= std::min(chunks / 2, 64) || pieces == 1; ++pieces) {
+            const int len = (chunks + pieces - 1) / pieces, n = (chunks + len - 1) / len;
+            const double rounds = (double)((wgs * a.N * n + room - 1) / room), once = rounds * (len + 2);
+            const double cost = n == 1 ? once : 1.5 * once + 3 + n / 16.0;
+            if (cost < least) { least = cost; best = len; }
+        }
+        return best * 64;
     }
     // packed: some sequence may be as long as all of them
-    const long long len = (long long)a.T * wgs / want / 64 * 64;
-    return (int)std::max<long long>(128, std::min<long long>(len, 1024));
+    return (int)std::max<long long>(256, (long long)a.T * wgs / (2 * room) / 64 * 64);
 }
 bool cut(const vrwkv_decay_args& a, int seg_len) { return a.T > seg_len; }
 long long segment_total(const vrwkv_decay_args& a, int seg_len) {
@@ -210,9 +222,8 @@ int launch_segments(const Params& p, int dtype, int dx, hipStream_t st) {
     int tiles = 1;
     for (int i = 0; i < p.n_roles; ++i) tiles = std::max(tiles, p.role[i].tiles);
     const dim3 grid((unsigned)(dx / 16 * (long long)p.N * p.H * tiles), 1, p.n_roles), block(THREADS);
-    const int L = chunk_of(dtype, dx);
-    if (dx == 64) hipLaunchKernelGGL((segments_kernel<64>), grid, block, 0, st, p, L);
-    else hipLaunchKernelGGL((segments_kernel<128>), grid, block, 0, st, p, L);
+    if (dx == 64) hipLaunchKernelGGL((segments_kernel<64>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((segments_kernel<128>), grid, block, 0, st, p);
     return check_launch("decay_attention (segments)");
 }
 void take_segments(Role& r, Pieces& ws, const vrwkv_decay_args& a, long long segs, int dx) {
@@ -228,7 +239,7 @@ struct FwdPlan {
         role.dx = a.Dk;
         role.dz = a.Dv;
         role.tiles = tiles_of(a.Dv);
-        seg_len = segment_len(a, role.tiles, 1);
+        seg_len = segment_len(a, dx, role.tiles, 1, false);
         if (cut(a, seg_len)) take_segments(role, ws, a, segment_total(a, seg_len), dx);
     }
 };
@@ -240,13 +251,13 @@ struct BwdPlan {
     BwdPlan(const vrwkv_decay_args& a, Pieces& ws) {
         dxk = pad_dx(a.Dk);
         dxv = pad_dx(a.Dv);
-        L = chunk_of(a.dtype, dxv);
+        L = chunk_of(a.dtype);
         dv.dx = dk.dz = dq.dz = a.Dk;
         dv.dz = dk.dx = dq.dx = a.Dv;
         dv.tiles = tiles_of(a.Dv);
         dk.tiles = dq.tiles = tiles_of(a.Dk);
         dv.reverse = dk.reverse = 1;
-        seg_len = segment_len(a, 1, 2);
+        seg_len = segment_len(a, dxv, dk.tiles, 1, true);
         const long long segs = segment_total(a, seg_len), rows = rows_of(a);
         if (cut(a, seg_len)) {
             take_segments(dv, ws, a, segs, dxk);
@@ -283,7 +294,7 @@ void decay_sums(const BwdPlan& b, const vrwkv_decay_args& a, hipStream_t st) {
     if (a.g_per_head) {
         const int n = (int)std::min<long long>(SLICES, (rows * b.dk.tiles + 3) / 4);
         hipLaunchKernelGGL(decay_slices_kernel, dim3(n, (a.H + 63) / 64), dim3(THREADS), 0, st, b.fg, b.slices, rows * b.dk.tiles, a.H);
-        hipLaunchKernelGGL((decay_total_kernel<G>), dim3((a.H + THREADS - 1) / THREADS), dim3(THREADS), 0, st, b.slices, static_cast<G*>(a.dg), n, a.H);
+        hipLaunchKernelGGL((decay_total_kernel<G>), dim3(a.H), dim3(64), 0, st, b.slices, static_cast<G*>(a.dg), n, a.H);
     } else {
         const unsigned grid = (unsigned)std::min<long long>((count + THREADS - 1) / THREADS, 4096);
         hipLaunchKernelGGL((decay_grad_kernel<G>), dim3(grid), dim3(THREADS), 0, st, b.fg, static_cast<G*>(a.dg), count, b.dk.tiles);

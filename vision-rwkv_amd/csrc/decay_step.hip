@@ -50,7 +50,7 @@ __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
                     if (d + c < p.Dv) S[i][c] = r[c];
         }
     }
-    // the next row behind `after` with this slot, N if none; before the first round: whether an earlier row has it
+    // the next row behind `after` with this slot, N if none
     const auto next_row = [&](int after) {
         int best = p.N;
         for (int i = after + 1 + tid; i < p.N; i += THREADS)
@@ -64,10 +64,13 @@ __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
     };
     int n = n0, next = p.N;
     if (known && p.slots) {
-        int seen = 0;
-        for (int i = tid; i < n0; i += THREADS) seen |= slot_of(p, i) == slot;
-        if (__syncthreads_or(seen)) return;
-        next = next_row(n0);
+        int others = 0;                                   // rows with the same slot, which are few if any: 1 in front of this one, 2 behind
+        for (int i = tid; i < p.N; i += THREADS)
+            if (i != n0 && slot_of(p, i) == slot) others |= i < n0 ? 1 : 2;
+        if (__syncthreads_or(others)) {
+            if (__syncthreads_or(others & 1)) return;
+            next = next_row(n0);
+        }
     }
     for (;;) {
         const IO* q = static_cast<const IO*>(p.q) + n * p.q_sn + (h / p.share_q) * p.q_sh;

@@ -8,6 +8,7 @@
 //   Bi-WKV training, 64 x 196 x 768 bf16 (kernels 56)           119.6 -> 76.1        2 x 4150 x 768 fp32 (kernels 120)   128 -> 120
 //   wkv6 training, 8 x 577 x 384 fp32 (kernels 115)             159 -> 116
 //   twelve native blocks, 1 x 196 x 192 bf16 (kernels 397)      602 -> 507
+//   decay_attention_step, 1 sequence of 12 heads (kernel 6)     @STEP@
 //
 // The operators take the plain case: exact tensors and parameters, contiguous, on the current GPU, of the types that the kernels read as
 // they lie, outside every transform, mode and trace.  To everything else they answer None, and the Python classes in ops.py go on as
@@ -18,6 +19,7 @@
 #include <torch/extension.h>
 #include <torch/version.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -296,9 +298,224 @@ py::object block_forward(py::handle x_, py::dict tensors, py::object params, py:
     if (rc != VRWKV_OK) return py::int_(rc);
     return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
 }
+
+// ---- attention with a decay for each head -----------------------------------------------------------------------------------
+// An exact Tensor or Parameter on a GPU whose memory the kernels may read at its strides, channels side by side (`t` outlives the call: the caller holds it).
+const at::Tensor* strided(py::handle o) {
+    if (!THPVariable_CheckExact(o.ptr())) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o.ptr());
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.is_conj() || t.is_neg()) return nullptr;
+    const auto keys = t.key_set();
+    if (keys.has(c10::DispatchKey::FuncTorchBatched) || keys.has(c10::DispatchKey::Batched) || keys.has(c10::DispatchKey::Python) ||
+        keys.has(c10::DispatchKey::FuncTorchGradWrapper) || keys.has(c10::DispatchKey::Functionalize))
+        return nullptr;
+    return &t;
+}
+bool rows_fit(const at::Tensor& t, int lead) { return t.dim() == lead + 2 && t.numel() > 0 && t.stride(-1) == 1 && (lead == 1 || t.stride(1) < (1 << 22)); }
+
+// q, k, v, g as decay_attention and its step take them, nothing empty, nothing to convert
+bool decay_inputs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, int lead) {
+    if (!rows_fit(q, lead) || !rows_fit(k, lead) || !rows_fit(v, lead) || code(q.scalar_type()) < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() ||
+        (g.scalar_type() != q.scalar_type() && g.scalar_type() != at::kFloat) || (g.dim() != 1 && g.dim() != lead + 1) || g.numel() == 0)
+        return false;
+    for (int i = 0; i < lead; ++i)
+        if (k.size(i) != q.size(i) || v.size(i) != q.size(i) || q.size(i) > INT_MAX || (g.dim() > 1 && g.size(i) != q.size(i))) return false;
+    const int64_t H = g.size(-1);
+    return k.size(-1) == q.size(-1) && H <= INT_MAX && H % q.size(-2) == 0 && H % k.size(-2) == 0 && H % v.size(-2) == 0 && q.size(-1) <= 128 && v.size(-1) <= 128 &&
+           k.device() == q.device() && v.device() == q.device() && g.device() == q.device() && q.get_device() == c10::hip::current_device() && !tangent(q) && !tangent(k) &&
+           !tangent(v) && !tangent(g);
+}
+bool index_fits(const at::Tensor& t, const at::Tensor& q) {
+    return t.dim() == 1 && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.is_contiguous() && t.numel() > 0 && t.device() == q.device();
+}
+
+vrwkv_decay_args decay_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, const at::Tensor& state, const at::Tensor& offsets, double scale, int N) {
+    vrwkv_decay_args a = {};
+    a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.g = g.data_ptr();
+    a.state = state.defined() ? (const float*)state.data_ptr() : nullptr;
+    a.offsets = offsets.defined() ? offsets.data_ptr() : nullptr;
+    for (int i = 0; i < 3; ++i) {
+        a.q_stride[i] = q.stride(i), a.k_stride[i] = k.stride(i), a.v_stride[i] = v.stride(i);
+        a.g_stride[i] = g.dim() == 1 ? (i == 2 ? g.stride(0) : 0) : g.stride(i);
+    }
+    a.N = N, a.T = (int)q.size(1), a.H = (int)g.size(-1), a.Hq = (int)q.size(2), a.Hk = (int)k.size(2), a.Hv = (int)v.size(2), a.Dk = (int)q.size(3), a.Dv = (int)v.size(3);
+    a.dtype = code(q.scalar_type()), a.g_dtype = code(g.scalar_type()), a.g_per_head = g.dim() == 1, a.offsets64 = offsets.defined() && offsets.scalar_type() == at::kLong;
+    a.scale = (float)scale;
+    return a;
+}
+
+struct Decay : torch::autograd::Function<Decay> {
+    struct Call {                                          // what the forward has computed, and what is not differentiated
+        at::Tensor y, last, offsets;
+        double scale;
+        int64_t N;
+    };
+    static tensor_list forward(AutogradContext* ctx, const Variable& q, const Variable& k, const Variable& v, const Variable& g, const std::optional<at::Tensor>& state, const Call* c) {
+        ctx->save_for_backward({q, k, v, g, state.value_or(at::Tensor()), c->offsets});
+        ctx->saved_data["scale"] = c->scale;
+        ctx->saved_data["N"] = c->N;
+        ctx->set_materialize_grads(false);
+        return c->last.defined() ? tensor_list{c->y, c->last} : tensor_list{c->y};
+    }
+    static at::Tensor rows(const at::Tensor& t, const at::Tensor& like) {
+        TORCH_CHECK(t.defined() && t.has_storage() && t.is_cuda() && t.device() == like.device() && t.dim() == 4 && t.scalar_type() == like.scalar_type(),
+                    "the saved tensors and the gradient must be CUDA tensors on one device");
+        return (t.stride(-1) == 1 || t.size(-1) == 1) && t.stride(1) < (1 << 22) ? t : t.contiguous();
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        const bool recorded = at::GradMode::is_enabled();
+        tensor_list out(6);
+        {
+            at::NoGradGuard no_grad;
+            const auto saved = ctx->get_saved_variables();
+            const at::Tensor q = rows(saved[0], saved[0]), k = rows(saved[1], q), v = rows(saved[2], q), &g = saved[3], &offsets = saved[5];
+            const at::Tensor state = saved[4].defined() ? saved[4].contiguous() : at::Tensor();
+            const int N = (int)ctx->saved_data["N"].toInt();
+            const int64_t H = g.size(-1);
+            at::Tensor gy = grads[0], glast = grads.size() > 1 ? grads[1] : at::Tensor();
+            if (!gy.defined() && !glast.defined()) return out;
+            Guard guard(q.device());
+            const auto plain_options = q.options().requires_grad(false);
+            gy = gy.defined() ? rows(gy.to(q.scalar_type()), q) : at::zeros({q.size(0), q.size(1), H, v.size(3)}, plain_options);
+            if (glast.defined()) glast = glast.to(at::kFloat).contiguous();
+            TORCH_CHECK(gy.size(0) == q.size(0) && gy.size(1) == q.size(1) && gy.size(2) == H && gy.size(3) == v.size(3), "the gradient must have the shape of y");
+            vrwkv_decay_args a = decay_args(q, k, v, g, state, offsets, ctx->saved_data["scale"].toDouble(), N);
+            a.gy = gy.data_ptr();
+            for (int i = 0; i < 3; ++i) a.gy_stride[i] = gy.stride(i);
+            a.glast = glast.defined() ? (const float*)glast.data_ptr() : nullptr;
+            const at::Tensor* like[5] = {&q, &k, &v, &g, &state};
+            void* ptr[5] = {};
+            for (int i = 0; i < 5; ++i)
+                if (like[i]->defined() && ctx->needs_input_grad(i)) {
+                    out[i] = at::empty(like[i]->sizes(), like[i]->options().requires_grad(false));
+                    ptr[i] = out[i].data_ptr();
+                }
+            a.dq = ptr[0], a.dk = ptr[1], a.dv = ptr[2], a.dg = ptr[3], a.dstate = (float*)ptr[4];
+            at::Tensor ws;
+            a.workspace_bytes = vrwkv_decay_bwd_workspace_bytes(&a);
+            if (a.workspace_bytes) a.workspace = (ws = bytes(a.workspace_bytes, q)).data_ptr();
+            const int rc = vrwkv_decay_bwd(&a, stream_of(q));
+            TORCH_CHECK(rc == VRWKV_OK, "vrwkv status ", rc, ": ", vrwkv_last_error());
+        }
+        if (recorded) {                                    // (create_graph: differentiating these once more raises)
+            tensor_list some;
+            for (auto& t : out)
+                if (t.defined()) some.push_back(t.detach().set_requires_grad(true));
+            const auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)some.size());
+            some = (*error)(std::move(some));
+            size_t i = 0;
+            for (auto& t : out)
+                if (t.defined()) t = some[i++];
+        }
+        return out;
+    }
+};
+
+// decay_attention of decay.py: y or (y, last); None where the Python class has to decide
+py::object decay_attention(py::handle q_, py::handle k_, py::handle v_, py::handle g_, double scale, py::handle state_, py::handle offsets_, bool keep) {
+    if (transformed()) return py::none();
+    const at::Tensor none, *qp = strided(q_), *kp = strided(k_), *vp = strided(v_), *gp = strided(g_), *sp = state_.is_none() ? &none : strided(state_),
+                           *op = offsets_.is_none() ? &none : strided(offsets_);
+    if (!qp || !kp || !vp || !gp || !sp || !op) return py::none();
+    const at::Tensor &q = *qp, &k = *kp, &v = *vp, &g = *gp, &state = *sp, &offsets = *op;
+    if (!decay_inputs(q, k, v, g, 2) || (offsets.defined() && (!index_fits(offsets, q) || q.size(0) != 1 || offsets.numel() < 2))) return py::none();
+    const int64_t N = offsets.defined() ? offsets.numel() - 1 : q.size(0), H = g.size(-1), Dk = q.size(3), Dv = v.size(3);
+    if (N > INT_MAX || (state.defined() && (state.scalar_type() != at::kFloat || !state.is_contiguous() || state.dim() != 4 || state.size(0) != N || state.size(1) != H || state.size(2) != Dk ||
+                                            state.size(3) != Dv || state.device() != q.device() || tangent(state))))
+        return py::none();
+    tensor_list out;
+    {
+        py::gil_scoped_release release;
+        Guard guard(q.device());
+        Decay::Call c;
+        c.scale = scale, c.N = N, c.offsets = offsets;
+        vrwkv_decay_args a = decay_args(q, k, v, g, state, offsets, scale, (int)N);
+        c.y = at::empty({q.size(0), q.size(1), H, Dv}, q.options().requires_grad(false));
+        a.y = c.y.data_ptr();
+        if (keep) a.last = (float*)(c.last = at::empty({N, H, Dk, Dv}, q.options().dtype(at::kFloat).requires_grad(false))).data_ptr();
+        at::Tensor ws;
+        a.workspace_bytes = vrwkv_decay_fwd_workspace_bytes(&a);
+        if (a.workspace_bytes) a.workspace = (ws = bytes(a.workspace_bytes, q)).data_ptr();
+        if (vrwkv_decay_fwd(&a, stream_of(q)) != VRWKV_OK) return py::none();
+        if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || (state.defined() && state.requires_grad())))
+            out = Decay::apply(q, k, v, g, state.defined() ? std::optional<at::Tensor>(state) : std::nullopt, &c);
+        else
+            out = {c.y, c.last};
+    }
+    py::object y = py::reinterpret_steal<py::object>(THPVariable_Wrap(out[0]));
+    if (!keep) return y;
+    return py::make_tuple(y, py::reinterpret_steal<py::object>(THPVariable_Wrap(out[1])));
+}
+
+bool pages_fit(const at::Tensor& pool) {
+    int64_t want = 1;
+    for (int64_t i = pool.dim() - 1; i > 0; --i) {
+        if (pool.size(i) != 1 && pool.stride(i) != want) return false;
+        want *= pool.size(i);
+    }
+    return pool.size(0) == 1 || pool.stride(0) >= want;
+}
+
+py::object decay_step(py::handle q_, py::handle k_, py::handle v_, py::handle g_, py::handle pool_, py::handle slots_, double scale) {
+    if (transformed()) return py::none();
+    const at::Tensor none, *qp = strided(q_), *kp = strided(k_), *vp = strided(v_), *gp = strided(g_), *pp = strided(pool_), *sp = slots_.is_none() ? &none : strided(slots_);
+    if (!qp || !kp || !vp || !gp || !pp || !sp) return py::none();
+    const at::Tensor &q = *qp, &k = *kp, &v = *vp, &g = *gp, &pool = *pp, &slots = *sp;
+    if (!decay_inputs(q, k, v, g, 1) || (slots.defined() && (!index_fits(slots, q) || slots.numel() != q.size(0)))) return py::none();
+    const int64_t N = q.size(0), H = g.size(-1), Dk = q.size(2), Dv = v.size(2);
+    if (pool.dim() != 4 || pool.size(0) == 0 || pool.size(0) > INT_MAX || pool.size(1) != H || pool.size(2) != Dk || pool.size(3) != Dv || pool.scalar_type() != at::kFloat ||
+        pool.device() != q.device() || tangent(pool) || !pages_fit(pool) ||
+        (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || pool.requires_grad())))
+        return py::none();
+    Guard guard(q.device());
+    at::Tensor y = at::empty({N, H, Dv}, q.options().requires_grad(false));
+    vrwkv_decay_step_args a = {};
+    a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.g = g.data_ptr(), a.pool = (float*)pool.data_ptr(), a.y = y.data_ptr();
+    a.slots = slots.defined() ? slots.data_ptr() : nullptr;
+    for (int i = 0; i < 2; ++i) {
+        a.q_stride[i] = q.stride(i), a.k_stride[i] = k.stride(i), a.v_stride[i] = v.stride(i);
+        a.g_stride[i] = g.dim() == 1 ? (i == 1 ? g.stride(0) : 0) : g.stride(i);
+    }
+    a.page_stride = pool.size(0) > 1 ? pool.stride(0) : H * Dk * Dv;
+    a.N = (int)N, a.P = (int)pool.size(0), a.H = (int)H, a.Hq = (int)q.size(1), a.Hk = (int)k.size(1), a.Hv = (int)v.size(1), a.Dk = (int)Dk, a.Dv = (int)Dv;
+    a.dtype = code(q.scalar_type()), a.g_dtype = code(g.scalar_type()), a.slots64 = slots.defined() && slots.scalar_type() == at::kLong, a.scale = (float)scale;
+    if (vrwkv_decay_step(&a, stream_of(q)) != VRWKV_OK) return py::none();
+    if (!pool.is_inference()) pool.unsafeGetTensorImpl()->bump_version();
+    return py::reinterpret_steal<py::object>(THPVariable_Wrap(y));
+}
+
+// copy_states of decay.py for lists on the device: whether it was done here
+bool copy_pages(py::handle pool_, py::handle src_, py::handle dst_, py::handle source_) {
+    if (transformed()) return false;
+    const at::Tensor *pp = strided(pool_), *fp = strided(src_), *tp = strided(dst_), *op = source_.is_none() ? pp : strided(source_);
+    if (!pp || !fp || !tp || !op) return false;
+    const at::Tensor &pool = *pp, &src = *fp, &dst = *tp, &source = *op;
+    if (pool.dim() < 1 || pool.numel() == 0 || source.numel() == 0 || source.dim() != pool.dim() || source.scalar_type() != pool.scalar_type() || source.device() != pool.device() ||
+        pool.get_device() != c10::hip::current_device() || pool.size(0) > INT_MAX || source.size(0) > INT_MAX || !index_fits(src, pool) || !index_fits(dst, pool) ||
+        src.numel() != dst.numel() || src.numel() > 4096 || !pages_fit(pool) || !pages_fit(source) || tangent(pool) || tangent(source) ||
+        (at::GradMode::is_enabled() && (pool.requires_grad() || source.requires_grad())))
+        return false;
+    for (int64_t i = 1; i < pool.dim(); ++i)
+        if (pool.size(i) != source.size(i)) return false;
+    const int64_t size = pool.element_size(), page = pool.numel() / pool.size(0) * size;
+    const int M = (int)src.numel();
+    Guard guard(pool.device());
+    at::Tensor ws;
+    const size_t n = vrwkv_copy_pages_workspace_bytes(M);
+    if (n) ws = bytes(n, pool);
+    const auto distance = [&](const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) * size : page; };
+    const int rc = vrwkv_copy_pages(pool.data_ptr(), distance(pool), (int)pool.size(0), source.data_ptr(), distance(source), (int)source.size(0), page, src.data_ptr(),
+                                    src.scalar_type() == at::kLong, dst.data_ptr(), dst.scalar_type() == at::kLong, M, n ? ws.data_ptr() : nullptr, n, stream_of(pool));
+    if (rc != VRWKV_OK) return false;
+    if (!pool.is_inference()) pool.unsafeGetTensorImpl()->bump_version();
+    return true;
+}
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
+    m.def("decay_attention", &decay_attention);
+    m.def("decay_step", &decay_step);
+    m.def("copy_pages", &copy_pages);
     m.attr("torch_version") = TORCH_VERSION;               // what the module's calls into torch were compiled against
     m.def("weights_fit", &weights_fit);
     m.def("block_forward", &block_forward);

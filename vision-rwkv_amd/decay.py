@@ -137,6 +137,10 @@ def decay_attention(q, k, v, g, scale=1.0, state=None, offsets=None, return_stat
     offsets (N + 1,), int32 or int64 on the device, ascending from 0 to T: N sequences packed behind each other in one row (B = 1), sequence n the tokens
     offsets[n] to offsets[n + 1] (an empty one leaves its state as it is); y of rows behind the last sequence is zero, and so are their gradients.
     Gradients for q, k, v, g and state, sums in fp32 (those of (H,) decays in 64 bits), rounded once to their inputs' types; no second ones."""
+    if not torch.compiler.is_compiling():
+        out = _lib.host().decay_attention(q, k, v, g, scale, state, offsets, return_state)
+        if out is not None:
+            return out
     H, Dk, Dv = _check_heads(q, k, v, g, 2)
     N = q.shape[0]
     if offsets is not None:
@@ -159,6 +163,10 @@ def decay_attention_step(q, k, v, g, pool, slots=None, scale=1.0):
     page, 0, 1, .. without.  Rows that name the same page are tokens behind each other, in their order.  A row of slot -1 (a place of the batch that is not
     taken) gives zeros and touches nothing, one of any other slot outside the pool NaN.  Pages may lie at any distance (pool[:, layer] of a pool for all
     layers), each contiguous.  Forward only."""
+    if not torch.compiler.is_compiling():
+        y = _lib.host().decay_step(q, k, v, g, pool, slots, scale)
+        if y is not None:
+            return y
     H, Dk, Dv = _check_heads(q, k, v, g, 1)
     N = q.shape[0]
     _check(pool, "pool", q)
@@ -188,8 +196,13 @@ def decay_attention_step(q, k, v, g, pool, slots=None, scale=1.0):
     a.N, a.P, a.H, a.Hq, a.Hk, a.Hv, a.Dk, a.Dv = N, pool.shape[0], H, q.shape[1], k.shape[1], v.shape[1], Dk, Dv
     a.dtype, a.g_dtype, a.slots64, a.scale = _DT[q.dtype], _DT[g.dtype], slots is not None and slots.dtype == torch.int64, scale
     _call("vrwkv_decay_step", a, q.device)
-    torch.autograd.graph.increment_version(pool)
+    _changed(pool)
     return y
+
+
+def _changed(pool):
+    if not pool.is_inference():                            # (those have no version)
+        torch.autograd.graph.increment_version(pool)
 
 
 def _pages_fit(pool):
@@ -223,6 +236,8 @@ def copy_states(pool, src, dst, source=None):
     from another pool or out to one.  src -1 clears the page, dst -1 is a place of the list that is not taken; of several entries with the same dst the
     last counts.  src, dst: vectors of up to 4096 int32 or int64, on the device -- where entries outside the pools are left out -- or on the host, where
     they are refused.  Pools of any type whose pages are contiguous, at any distance; a source is the pool or does not overlap it."""
+    if not torch.compiler.is_compiling() and _lib.host().copy_pages(pool, src, dst, source):
+        return pool
     _check(pool, "pool")
     source = pool if source is None else source
     _check(source, "source", pool)
@@ -250,6 +265,6 @@ def copy_states(pool, src, dst, source=None):
     with _on(pool.device):
         _lib.check(L.vrwkv_copy_pages(pool.data_ptr(), distance(pool), pool.shape[0], origin.data_ptr(), distance(origin), pages, page,
                                       src.data_ptr(), src.dtype == torch.int64, dst.data_ptr(), dst.dtype == torch.int64, M,
-                                      ws.data_ptr(), ws.numel(), _stream_ptr(pool.device)))
-    torch.autograd.graph.increment_version(pool)
+                                      ws.data_ptr() if ws.numel() else None, ws.numel(), _stream_ptr(pool.device)))
+    _changed(pool)
     return pool
