@@ -44,29 +44,32 @@ struct Role {
     float* last;                                          // where the states behind the last token go, or null
     float *seg, *seg_decay;                               // [segment][head][tile] a segment's state (first its own, then that in front of it), [segment][head]
     float* edge;                                          // [tile][row][head]: what a token gives to the tokens outside its chunk (written with dk, read with dq)
-    float* anchors;                                       // [chunk][head][tile]: R behind each chunk, without the decay of the token behind it
+    float* anchors;                                       // [chunk][head][tile]: R behind each chunk, without the decay of the token behind it; or S in front of it
     float* dg;                                            // [tile][row][head]
     long long sx, sz;                                     // strides of the states' contracted and other index
     int dx, dz, tiles, reverse;
     float s_in, s_upd;                                    // scale where the state is read; where it is written
 };
-struct Params {
+struct Call {                                             // sequences, their cut, and the decays
     const void *offsets, *g;
     long long g_sb, g_st, g_sh;
     long long rows;                                       // batch * T
     int off64, g_dtype, N, T, H;                          // T: tokens of a row of the batch (packed: of all sequences)
     int seg_len, nseg, segs;                              // tokens of a segment; segments of a row (0: packed); of the call
-    int n_roles;
     float scale;
+};
+struct Params : Call {
+    int n_roles;
     Role role[3];
 };
 template <typename IO> constexpr int in_terms = std::is_same<IO, float>::value ? 3 : std::is_same<IO, __half>::value ? 2 : 1;   // bf16 numbers that hold an element
 
-// y and dv; dk with what dg needs of it; dq with dg; no outputs: a segment's own state; dk or dq without dg, the same bits as with it
-enum Mode { PLAIN = 0, EDGES = 1, FLOWS = 2, STATES = 3, ALONE = 4 };
+// y and dv; dk with what dg needs of it; dq with dg; no outputs: a segment's own state; dk or dq without dg, the same bits as with it; no outputs: the state
+// in front of each chunk (for decay_bwd.h)
+enum Mode { PLAIN = 0, EDGES = 1, FLOWS = 2, STATES = 3, ALONE = 4, CHUNKS = 5 };
 // tokens of a chunk: 64 where two workgroups' rows and states fit the LDS of a compute unit (fp32 rows take three times the room of bf16 ones, fp16 rows twice)
 template <typename IO, int DX, int MODE>
-constexpr int chunk_len = std::is_same<IO, __hip_bfloat16>::value || (std::is_same<IO, __half>::value && DX == 64 && (MODE == PLAIN || MODE == STATES)) ? 64 : 32;
+constexpr int chunk_len = std::is_same<IO, __hip_bfloat16>::value || (std::is_same<IO, __half>::value && DX == 64 && (MODE == PLAIN || MODE == STATES || MODE == CHUNKS)) ? 64 : 32;
 
 struct Place {                                            // a workgroup's segment
     int n, first, len;                                    // sequence; its first token and length
@@ -75,11 +78,11 @@ struct Place {                                            // a workgroup's segme
     int chunk0;                                           // number of the sequence's first chunk
     bool is_last, is_first, valid;
 };
-__device__ __forceinline__ int offset_at(const Params& p, int n) {
+__device__ __forceinline__ int offset_at(const Call& p, int n) {
     const long long v = p.off64 ? static_cast<const long long*>(p.offsets)[n] : (long long)static_cast<const int*>(p.offsets)[n];
     return (int)(v < 0 ? 0 : v > p.T ? p.T : v);
 }
-__device__ __forceinline__ Place sequence_place(const Params& p, int n, int L) {
+__device__ __forceinline__ Place sequence_place(const Call& p, int n, int L) {
     Place w;
     w.n = n;
     w.valid = true;
@@ -97,15 +100,16 @@ __device__ __forceinline__ Place sequence_place(const Params& p, int n, int L) {
     return w;
 }
 // Packed sequences: n's segments have the numbers from first(n) / seg_len + n on, which grow with n and leave each its room whatever its length.
-__device__ __forceinline__ int first_segment(const Params& p, int n, int first) { return p.nseg ? n * p.nseg : first / p.seg_len + n; }
-__device__ __forceinline__ int segment_count(const Params& p, int len) { return max(1, (len + p.seg_len - 1) / p.seg_len); }
+__device__ __forceinline__ int first_segment(const Call& p, int n, int first) { return p.nseg ? n * p.nseg : first / p.seg_len + n; }
+__device__ __forceinline__ int segment_count(const Call& p, int len) { return max(1, (len + p.seg_len - 1) / p.seg_len); }
 
-__device__ __forceinline__ Place find_place(const Params& p, int gid, int L) {
+template <int THREADS_>
+__device__ __forceinline__ Place find_place(const Call& p, int gid, int L) {
     int n;
     if (p.nseg) n = gid / p.nseg;
     else {
         int seen = 0;
-        for (int m = 0; m < p.N; m += THREADS) {
+        for (int m = 0; m < p.N; m += THREADS_) {
             const int i = m + threadIdx.x;
             seen += __syncthreads_count(i < p.N && offset_at(p, min(i, p.N - 1)) / p.seg_len + i <= gid);
         }
@@ -125,7 +129,7 @@ __device__ __forceinline__ Place find_place(const Params& p, int gid, int L) {
     return w;
 }
 
-__device__ __forceinline__ float log_decay(const Params& p, int base, int token, int h) {
+__device__ __forceinline__ float log_decay(const Call& p, int base, int token, int h) {
     const long long i = base * p.g_sb + token * p.g_st + h * p.g_sh;
     float x;
     if (p.g_dtype == VRWKV_F32) x = static_cast<const float*>(p.g)[i];
@@ -231,6 +235,23 @@ __device__ __forceinline__ double wave_scan_inclusive(double x) {
     return dpp_add<0x143, 0xc>(x);
 }
 
+__device__ __forceinline__ double lane_double(double x, int lane) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+    return __builtin_bit_cast(double, (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 | (unsigned)__builtin_amdgcn_readlane((int)b, lane));
+}
+// What crosses token `lane`: terms inside the chunk, what it and the tokens behind it receive over the chunk's front, what those in front of it give over its end.
+__device__ __forceinline__ double flow_sum(double inner, double in, double out, int lane) {
+    double before = wave_scan_inclusive(out);
+    before = __shfl_up(before, 1);
+    if (lane == 0) before = 0.;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double o = __shfl_down(in, d);
+        if (lane + d < 64) in += o;
+    }
+    return inner + in + before;
+}
+
 // Four channels of a row, `count` of them there.
 template <typename O, bool VEC>
 __device__ __forceinline__ void store_quad(__amdgpu_buffer_rsrc_t buf, unsigned at, int count, f32x4 x) {
@@ -257,11 +278,12 @@ struct Lds {
     // terms of the products' intermediate operands: 16 bits of them for a 16-bit result, all 24 where fp32 ones depend on them: those of fp32 rows, and dg
     static constexpr int NP = NS < 3 ? 2 : 3, NI = MODE == PLAIN ? NP : 3;
     static constexpr int PX = DX + 8, PZ = TZ + 8;        // row pitches: 16 rows of a fragment on different banks
-    __bf16 a[MODE == STATES ? 1 : NS][MODE == STATES ? 1 : L][PX];   // channels in the order of the state's fragments
+    static constexpr bool OUT = MODE != STATES && MODE != CHUNKS;
+    __bf16 a[OUT ? NS : 1][OUT ? L : 1][PX];   // channels in the order of the state's fragments
     __bf16 b[NS][L][PX];
     __bf16 c[NS][L][PZ];
     __bf16 e[MODE == EDGES || MODE == FLOWS ? NS : 1][MODE == EDGES || MODE == FLOWS ? L : 1][PZ];
-    u32x4 s[MODE == STATES ? 1 : NI][4][MODE == STATES ? 1 : DX / 32][64];   // the state's terms, a lane's fragment side by side
+    u32x4 s[OUT ? NI : 1][4][OUT ? DX / 32 : 1][64];   // the state's terms, a lane's fragment side by side
     struct Decays {
         float gh[L], gl[L], dt[L], dk[L];                 // G in powers of two, head and tail; exp(G); exp(G_end - G)
         float end, through;                               // exp(G_end); FLOWS: with the decay of the token behind the chunk
@@ -300,7 +322,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     constexpr int L = S::L, NS = S::NS, NI = S::NI, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
     constexpr int PA = L * DX / 8 / THREADS, PC = (L * TZ / 8 + THREADS - 1) / THREADS;
     static_assert(PA >= 1 && L * DX % (8 * THREADS) == 0 && L * TZ % (8 * THREADS) == 0, "");
-    constexpr bool OUT = MODE != STATES, EXTRA = MODE == EDGES || MODE == FLOWS;
+    constexpr bool OUT = S::OUT, EXTRA = MODE == EDGES || MODE == FLOWS;
     __shared__ S lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
 
@@ -315,7 +337,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     id /= tiles;
     const int h = id % p.H, gid = id / p.H;
     if (!p.nseg && OUT && z < r.tiles) clear_outside<IO, MODE>(p, r, gid, z, h);
-    const Place w = find_place(p, gid, L);
+    const Place w = find_place<THREADS>(p, gid, L);
     if (!w.valid || z >= r.tiles) return;
     if (MODE == STATES && (r.reverse ? w.is_first : w.is_last)) return;    // nothing starts behind it
     const int z0 = z * TZ;
@@ -386,8 +408,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     const auto put_decays = [&](typename S::Decays& d) {   // wave 0
         // sums in 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth
         const double G = wave_scan_inclusive((double)rg * 1.4426950408889634);
-        const unsigned long long bits = __builtin_bit_cast(unsigned long long, G);
-        const double end = __builtin_bit_cast(double, (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((int)bits, 63));
+        const double end = lane_double(G, 63);
         const float gh = (float)G;
         if (lane < L) {
             d.gh[lane] = gh;
@@ -619,11 +640,12 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 
         // ---- the state behind the chunk
         {
-            if constexpr (MODE == EDGES) {
+            if constexpr (MODE == EDGES || MODE == CHUNKS) {
                 const long long ck = (((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * r.tiles + z) * (DX * TZ);
 #pragma unroll
                 for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.anchors + ck + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
             }
+            if (MODE == CHUNKS && ci + 1 == nc) break;     // (nothing starts behind it)
             const float ed = dec_.end;
 #pragma unroll
             for (int x = 0; x < NX; ++x)
@@ -681,18 +703,10 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                     in = NT == 4 ? (double)lds.edge[0][lane] : (double)lds.edge[0][lane] + lds.edge[1][lane];
                     out = given;
                 }
-                double before = wave_scan_inclusive(out);
-                before = __shfl_up(before, 1);
-                if (lane == 0) before = 0.;
-#pragma unroll
-                for (int d = 1; d < 64; d *= 2) {
-                    const double o = __shfl_down(in, d);
-                    if (lane + d < 64) in += o;
-                }
                 const int at_lane = min(lane, L - 1);
                 const double inner = ((double)lds.inner[0][at_lane] + lds.inner[1][at_lane]) + ((double)lds.inner[2][at_lane] + lds.inner[3][at_lane]);
                 const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * dec_.through;
-                if (lane < n) r.dg[at] = (float)(inner + in + before + through);
+                if (lane < n) r.dg[at] = (float)(flow_sum(inner, in, out, lane) + through);
             }
         }
     }
@@ -729,6 +743,9 @@ void launch_mode(const Params& p, int mode, dim3 grid, hipStream_t st) {
     else if (mode == EDGES) hipLaunchKernelGGL((decay_kernel<IO, DX, EDGES, VEC>), grid, block, 0, st, p);
     else if (mode == FLOWS) hipLaunchKernelGGL((decay_kernel<IO, DX, FLOWS, VEC>), grid, block, 0, st, p);
     else if (mode == ALONE) hipLaunchKernelGGL((decay_kernel<IO, DX, ALONE, VEC>), grid, block, 0, st, p);
+    else if (mode == CHUNKS) {
+        if constexpr (DX == 64) hipLaunchKernelGGL((decay_kernel<IO, 64, CHUNKS, VEC>), grid, block, 0, st, p);
+    }
     else hipLaunchKernelGGL((decay_kernel<IO, DX, STATES, VEC>), grid, block, 0, st, p);
 }
 // vec: every row of every role in pieces of 16 bytes

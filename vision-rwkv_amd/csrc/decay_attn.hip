@@ -1,6 +1,6 @@
 // Host side of the attention with a decay for each head (decay_attn.h), and the passes around its kernel: the states in front of the segments, and the
 // sums that gradients of shared heads and of the decays leave to the end.
-#include "decay_attn.h"
+#include "decay_bwd.h"
 #include <algorithm>
 #include <cstdint>
 
@@ -104,10 +104,11 @@ constexpr int SLICES = 128;
 size_t elem(int dtype) { return dtype == VRWKV_F32 ? 4 : 2; }
 int pad_dx(int d) { return d <= 64 ? 64 : 128; }
 int tiles_of(int d) { return (d + TZ - 1) / TZ; }
-int chunk_of(int dtype) { return dtype == VRWKV_BF16 ? 64 : 32; }   // of dk and dq
+int chunk_of(int dtype, bool together) { return dtype == VRWKV_BF16 || (together && dtype == VRWKV_F16) ? 64 : 32; }   // of the gradients' passes
 
 // workgroups of a launch of outputs that the chip holds at once
 int slots(int dtype, int dx, bool backward) {
+    if (backward && dx == 64) return device_cus();
     const int per_cu = dtype == VRWKV_BF16 ? (dx == 64 ? (backward ? 2 : 3) : (backward ? 1 : 2)) : dtype == VRWKV_F16 ? (dx == 64 || !backward ? 2 : 1) : dx == 64 ? 2 : 1;
     return per_cu * device_cus();
 }
@@ -190,8 +191,9 @@ bool in_pieces(const Params& p, int dtype) {
     }
     return vec;
 }
-Params common(const vrwkv_decay_args& a, int seg_len) {
-    Params p{};
+template <typename P>
+P common(const vrwkv_decay_args& a, int seg_len) {
+    P p{};
     p.offsets = a.offsets;
     p.off64 = a.offsets64;
     p.g = a.g;
@@ -243,15 +245,19 @@ struct FwdPlan {
         if (cut(a, seg_len)) take_segments(role, ws, a, segment_total(a, seg_len), dx);
     }
 };
+// Heads of up to 64 channels: one pass for all gradients (decay_bwd.h) behind one that keeps the states in front of the chunks.  Larger ones: dv, dk and dq one
+// after the other by the kernel of the forward pass.
 struct BwdPlan {
     int dxk, dxv, seg_len, L;
+    bool together;
     Role dv{}, dk{}, dq{};
     float *fq = nullptr, *fk = nullptr, *fv = nullptr, *fg = nullptr;   // gradients of every head, where several share one; of the decays
     double* slices = nullptr;
     BwdPlan(const vrwkv_decay_args& a, Pieces& ws) {
         dxk = pad_dx(a.Dk);
         dxv = pad_dx(a.Dv);
-        L = chunk_of(a.dtype);
+        together = dxk == 64 && dxv == 64;
+        L = chunk_of(a.dtype, together);
         dv.dx = dk.dz = dq.dz = a.Dk;
         dv.dz = dk.dx = dq.dx = a.Dv;
         dv.tiles = tiles_of(a.Dv);
@@ -260,20 +266,18 @@ struct BwdPlan {
         seg_len = segment_len(a, dxv, dk.tiles, 1, true);
         const long long segs = segment_total(a, seg_len), rows = rows_of(a);
         if (cut(a, seg_len)) {
-            take_segments(dv, ws, a, segs, dxk);
+            if (!together) take_segments(dv, ws, a, segs, dxk);
             take_segments(dk, ws, a, segs, dxv);
             take_segments(dq, ws, a, segs, dxv);
         }
         if (a.dq && a.Hq < a.H) fq = ws.take<float>((size_t)rows * a.H * a.Dk);
         if (a.dk && a.Hk < a.H) fk = ws.take<float>((size_t)rows * a.H * a.Dk);
         if (a.dv && a.Hv < a.H) fv = ws.take<float>((size_t)rows * a.H * a.Dv);
+        if (a.dg || together) dk.anchors = dq.anchors = ws.take<float>((size_t)chunk_total(a, L) * a.H * dk.tiles * dxv * TZ);
         if (a.dg) {
-            dk.anchors = ws.take<float>((size_t)chunk_total(a, L) * a.H * dk.tiles * dxv * TZ);
-            dk.edge = ws.take<float>((size_t)rows * a.H * dk.tiles);
+            if (!together) dk.edge = dq.edge = ws.take<float>((size_t)rows * a.H * dk.tiles);
             if (a.g_per_head || dk.tiles > 1 || a.g_dtype != VRWKV_F32) fg = ws.take<float>((size_t)rows * a.H * dk.tiles);
             if (a.g_per_head) slices = ws.take<double>((size_t)SLICES * a.H);
-            dq.anchors = dk.anchors;
-            dq.edge = dk.edge;
         }
     }
 };
@@ -328,7 +332,7 @@ extern "C" int vrwkv_decay_fwd(const vrwkv_decay_args* args, void* hip_stream) {
     Pieces ws{static_cast<char*>(a.workspace)};
     FwdPlan plan(a, ws);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    Params p = common(a, plan.seg_len);
+    Params p = common<Params>(a, plan.seg_len);
     p.n_roles = 1;
     Role& r = p.role[0] = plan.role;
     r.a = view(a.q, a.q_stride, a.Hq, a);
@@ -400,13 +404,37 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     b.dq.s_in = a.scale;
     b.dq.s_upd = 1.f;
     b.dq.dg = b.fg ? b.fg : static_cast<float*>(a.dg);
-    Params p = common(a, b.seg_len);
+    Params p = common<Params>(a, b.seg_len);
     const auto run = [&](std::initializer_list<Role> roles, int dx, int mode) {
         p.n_roles = 0;
         for (const Role& r : roles) p.role[p.n_roles++] = r;
         return mode == STATES ? launch_segments(p, a.dtype, dx, st) : launch(p, a.dtype, dx, mode, st);
     };
-    const bool want_dv = a.dv || a.dstate, want_dk = a.dk || a.dg, want_dq = a.dq || a.dg;
+    if (b.together) {
+        if (b.dk.seg && (s = run({b.dk, b.dq}, 64, STATES)) != VRWKV_OK) return s;
+        if ((s = run({b.dq}, 64, CHUNKS)) != VRWKV_OK) return s;
+        BwdParams t = common<BwdParams>(a, b.seg_len);
+        t.q = q;
+        t.k = k;
+        t.v = v;
+        t.gy = gy;
+        t.dq = b.dq.o;
+        t.dk = b.dk.o;
+        t.dv = b.dv.o;
+        t.dg = b.dq.dg;
+        t.chunks = b.dq.anchors;
+        t.seg = b.dk.seg;
+        t.glast = a.glast;
+        t.dstate = a.dstate;
+        t.Dk = a.Dk;
+        t.Dv = a.Dv;
+        p.n_roles = 0;
+        for (const Role& r : {b.dv, b.dk, b.dq}) p.role[p.n_roles++] = r;
+        const bool vec = in_pieces(p, a.dtype);
+        s = a.dtype == VRWKV_F32 ? launch_decay_bwd<float>(t, vec, st) : a.dtype == VRWKV_BF16 ? launch_decay_bwd<__hip_bfloat16>(t, vec, st) : launch_decay_bwd<__half>(t, vec, st);
+        if (s != VRWKV_OK) return s;
+    }
+    const bool want_dv = !b.together && (a.dv || a.dstate), want_dk = !b.together && (a.dk || a.dg), want_dq = !b.together && (a.dq || a.dg);
     if (b.dv.seg) {
         if (want_dv && (s = run({b.dv}, b.dxk, STATES)) != VRWKV_OK) return s;
         if (want_dk && want_dq) s = run({b.dk, b.dq}, b.dxv, STATES);

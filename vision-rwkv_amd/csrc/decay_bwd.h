@@ -1,0 +1,499 @@
+// Gradients of the attention with a decay for each head, heads of up to 64 channels, all in one pass back along the chunks (gfx950).
+// With S0 the state in front of a chunk (kept for every chunk by a pass of decay_attn.h), X the gradient of the state behind it, G the sums of its log
+// decays, D_ts = exp(G_t - G_s) for s <= t, P = scale D (q k^T) and dP = scale D (gy v^T):
+//     dq_t = sum_s dP_ts k_s + scale exp(G_t) S0 gy_t
+//     dv_s = sum_t P_ts gy_t + exp(G_end - G_s) X^T k_s,       dk_s = sum_t dP_ts q_t + exp(G_end - G_s) X v_s
+//     X <- exp(G_end) X + scale sum_t exp(G_t) q_t gy_t^T
+//     dg_j = what crosses from tokens in front of j to j and behind: the terms P_ts (gy_t . v_s) with s < j <= t; q . (S0's part of dq) of the tokens from j on;
+//            k . (X's part of dk) of those in front; exp(G_end) <S0, X>.  Sums of what crosses, so nothing cancels where little does.
+// Eight waves, two a SIMD: four take dq, tokens t along the lanes, and X; four take dk, dv and dg, tokens s along the lanes.  Every operand of the products is
+// read as it lies or across its rows, so the chunk's rows are staged once, where dv, dk and dq by themselves (decay_attn.h) stage ten tensors.
+// X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
+// 64 x 196 tokens of 12 heads, bf16: @BASE@.
+#pragma once
+#include "decay_attn.h"
+
+namespace vrwkv {
+namespace decay {
+
+constexpr int BWD_THREADS = 512;
+
+struct BwdParams : Call {
+    View q, k, v, gy;
+    OutView dq, dk, dv;
+    float* dg;                                            // [row][head]
+    const float *chunks;                                  // [chunk][head]: S0, rows of v's channels and columns of k's, as the accumulators lie
+    const float *seg;                                     // [segment][head]: R behind the segment, without the decay of the token behind it; null: sequences are not cut
+    const float* glast;                                   // gradients of the states behind the last tokens, or null
+    float* dstate;
+    int Dk, Dv;
+};
+
+template <typename IO>
+struct BwdLds {
+    static constexpr int L = chunk_len<IO, 64, PLAIN>, NS = in_terms<IO>, PX = 72;
+    __bf16 q[NS][L][PX], k[NS][L][PX], v[NS][L][PX], gy[NS][L][PX];   // channels in the order of the state's fragments
+    __bf16 x[3][64][PX];                                  // X [k's channel][v's, in that order]
+    u32x4 s[3][4][2][64];                                 // S0's fragments: rows of k's channels, v's side by side
+    struct Decays {
+        float gh[L], gl[L], dt[L], dk[L];
+        float end;
+    } d[2];
+    float in[2][L], out[2][L], inner[4][L], cross[4];     // what a token receives over the chunk's front, gives over its end, by halves of the columns; what crosses it inside; <S0, X>
+};
+
+template <typename IO, bool FLOW, bool VEC>
+__global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdParams p) {
+    using S = BwdLds<IO>;
+    constexpr int L = S::L, NS = S::NS, NT = L / 16, KS = L / 32, PX = S::PX, NP = NS < 3 ? 2 : 3;
+    constexpr int PIECES = L * 8 / 256;                   // of each pair of tensors, a thread's: halves of the workgroup take (q, v) and (k, gy)
+    __shared__ S lds;
+    const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2, w4 = wave & 3;
+    const int h = blockIdx.x % p.H, gid = blockIdx.x / p.H;
+
+    if (!p.nseg) {                                        // packed rows in front of the first sequence and behind the last: no gradient
+        const int front = offset_at(p, 0), back = offset_at(p, p.N), rows = front + max(0, p.T - back);
+        for (int i = gid * 8 + wave; i < rows; i += p.segs * 8) {
+            const long long row = i < front ? i : back + (i - front);
+            const OutView* const outs[3] = {&p.dq, &p.dk, &p.dv};
+#pragma unroll
+            for (int o = 0; o < 3; ++o) {
+                const OutView& v = *outs[o];
+                if (v.p && lane < (o < 2 ? p.Dk : p.Dv)) {
+                    const long long at = row * v.st + h * v.sh + lane;
+                    if (v.f32) static_cast<float*>(v.p)[at] = 0.f;
+                    else static_cast<IO*>(v.p)[at] = from_f32<IO>(0.f);
+                }
+            }
+            if (FLOW && lane == 0) p.dg[row * p.H + h] = 0.f;
+        }
+    }
+    const Place w = find_place<BWD_THREADS>(p, gid, L);
+    if (!w.valid) return;
+    const int nc = (w.s1 - w.s0 + L - 1) / L;
+
+    // ---- X behind the segment, in the waves of group 0: rows 16 x + 4 quarter + i (v's channels), column 16 w4 + col (k's)
+    f32x4 st[4];
+    const long long page = ((long long)w.n * p.H + h) * ((long long)p.Dk * p.Dv);
+    const int zc = 16 * w4 + col;
+    bool have = false;
+    {
+        const bool cut = p.seg && !w.is_last;
+        have = cut || p.glast;
+        // (R behind a segment wants the decay of the token there)
+        const float d = cut ? fast_exp2(log_decay(p, w.base, w.first + w.s1, h) * LOG2E) : 1.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (cut) st[x] = *reinterpret_cast<const f32x4*>(p.seg + ((long long)gid * p.H + h) * 4096 + ((x * 4 + w4) * 64 + lane) * 4);
+            else if (p.glast) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int xc = 16 * x + 4 * quarter + i;
+                    if (xc < p.Dv && zc < p.Dk) st[x][i] = p.glast[page + (long long)zc * p.Dv + xc];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st[x][i] *= d;
+        }
+    }
+
+    const auto origin = [&](const View& v) { return static_cast<const IO*>(v.p) + w.base * v.sb + (long long)w.first * v.st + (h / v.share) * v.sh; };
+    const int half = __builtin_amdgcn_readfirstlane(tid >> 8), row0 = (tid & 255) >> 3, d0 = (tid & 7) * 8;
+    const View &va = half ? p.k : p.q, &vb = half ? p.gy : p.v;
+    const IO *const pa = origin(va), *const pb = origin(vb);
+    const int counta = p.Dk - d0, countb = p.Dv - d0;
+    Piece<IO> ra[PIECES], rb[PIECES];
+    f32x4 s0[4];
+    float rg = 0.f;
+    const auto fetch = [&](int c) {
+        const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+        const auto ba = buffer_at(pa + (long long)t0 * va.st), bb = buffer_at(pb + (long long)t0 * vb.st);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int row = row0 + 32 * i;
+            ra[i] = load_piece<IO, VEC>(ba, (unsigned)((row * (int)va.st + d0) * (int)sizeof(IO)), row < n ? counta : 0);
+            rb[i] = load_piece<IO, VEC>(bb, (unsigned)((row * (int)vb.st + d0) * (int)sizeof(IO)), row < n ? countb : 0);
+        }
+        if (group == 0) {
+            const float* ck = p.chunks + ((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * 4096;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s0[x] = *reinterpret_cast<const f32x4*>(ck + ((x * 4 + w4) * 64 + lane) * 4);
+        }
+        if (wave == 0) rg = lane < n ? log_decay(p, w.base, w.first + t0 + lane, h) : 0.f;
+    };
+    const auto put_decays = [&](typename S::Decays& d) {   // wave 0
+        const double G = wave_scan_inclusive((double)rg * 1.4426950408889634);
+        const double end = lane_double(G, 63);
+        const float gh = (float)G;
+        if (lane < L) {
+            d.gh[lane] = gh;
+            d.gl[lane] = (float)(G - gh);
+            d.dt[lane] = fast_exp2(gh) * p.scale;
+            d.dk[lane] = fast_exp2((float)(end - G));
+        }
+        if (lane == 0) d.end = fast_exp2((float)end);
+    };
+    if (nc > 0) {
+        fetch(nc - 1);
+        if (wave == 0) put_decays(lds.d[0]);
+    }
+
+    for (int ci = 0; ci < nc; ++ci) {
+        const int c = nc - 1 - ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+        // ---- operands to the LDS
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int row = row0 + 32 * i, o0 = order_of(d0), o1 = order_of(d0 + 4);
+            u32x4 t[NS];
+            auto& qa = half ? lds.k : lds.q;
+            auto& qb = half ? lds.gy : lds.v;
+            piece_terms<IO>(ra[i], t);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                *reinterpret_cast<uint2*>(&qa[s][row][o0]) = uint2{t[s][0], t[s][1]};
+                *reinterpret_cast<uint2*>(&qa[s][row][o1]) = uint2{t[s][2], t[s][3]};
+            }
+            piece_terms<IO>(rb[i], t);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                *reinterpret_cast<uint2*>(&qb[s][row][o0]) = uint2{t[s][0], t[s][1]};
+                *reinterpret_cast<uint2*>(&qb[s][row][o1]) = uint2{t[s][2], t[s][3]};
+            }
+        }
+        if (group == 0) {
+#pragma unroll
+            for (int kx = 0; kx < 2; ++kx) {
+                const float x8[8] = {s0[2 * kx][0], s0[2 * kx][1], s0[2 * kx][2], s0[2 * kx][3], s0[2 * kx + 1][0], s0[2 * kx + 1][1], s0[2 * kx + 1][2], s0[2 * kx + 1][3]};
+                bf16x8 t[3];
+                split8<3>(x8, t);
+#pragma unroll
+                for (int s = 0; s < 3; ++s) lds.s[s][w4][kx][lane] = __builtin_bit_cast(u32x4, t[s]);
+            }
+            float cross = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                unsigned t0_[3], t1_[3];
+                split_pair<3>(st[x][0], st[x][1], t0_);
+                split_pair<3>(st[x][2], st[x][3], t1_);
+                const int at = order_of(16 * x) + 8 * quarter;
+#pragma unroll
+                for (int s = 0; s < 3; ++s) *reinterpret_cast<uint2*>(&lds.x[s][zc][at]) = uint2{t0_[s], t1_[s]};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) cross = fmaf(st[x][i], s0[x][i], cross);
+            }
+            if constexpr (FLOW) {
+                cross = wave_sum(cross);
+                if (lane == 0) lds.cross[w4] = cross;
+            }
+        }
+        __syncthreads();
+        if (ci + 1 < nc) fetch(c - 1);
+        typename S::Decays& dec = lds.d[ci & 1];
+        const int tw = w4 % NT, zt0 = w4 / NT * NT, r0 = 16 * tw + col;     // this lane's token
+        const auto rows_of = [&](const __bf16 (&a)[NS][L][PX], int row, int kx, bf16x8 (&f)[NS]) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) f[s] = *reinterpret_cast<const bf16x8*>(&a[s][row][kx * 32 + 8 * quarter]);
+        };
+        // channels 16 x + col along the lanes, tokens 32 ks + 4 quarter .. and 16 behind those side by side
+        const auto across = [&](const __bf16 (&a)[NS][L][PX], int x, int ks, bf16x8 (&f)[NS]) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const __bf16* q = &a[s][32 * ks + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
+                f[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
+            }
+        };
+        const auto widen4 = [&](const __bf16 (&a)[NS][L][PX], int row, int x, float (&o)[4]) {   // channels 16 x + 4 quarter + i
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[i] = 0.f;
+#pragma unroll
+                for (int s = NS - 1; s >= 0; --s) o[i] += (float)a[s][row][order_of(16 * x) + 8 * quarter + i];
+            }
+        };
+        const auto store = [&](const OutView& v, int D, f32x4 (&acc)[NT]) {
+            if (!v.p) return;
+            const int e = v.f32 ? 4 : (int)sizeof(IO);
+            const auto buf = buffer_at(static_cast<char*>(v.p) + (w.base * v.sb + (long long)(w.first + t0) * v.st + h * v.sh) * e);
+            const int zl = 16 * zt0 + 4 * quarter, count = r0 < n ? D - zl : 0;
+            const unsigned at = (unsigned)(r0 * (int)v.st + zl);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if (v.f32) store_quad<float, VEC>(buf, (at + 16 * j) * 4, count - 16 * j, acc[j]);
+                else store_quad<IO, VEC>(buf, (at + 16 * j) * (unsigned)sizeof(IO), count - 16 * j, acc[j]);
+            }
+        };
+        if (group == 0) {
+            if (16 * tw < n) {
+                const float gh = dec.gh[r0], gl = dec.gl[r0], dt = dec.dt[r0];
+                bf16x8 fo[2][NS];
+                rows_of(lds.gy, r0, 0, fo[0]);
+                rows_of(lds.gy, r0, 1, fo[1]);
+                f32x4 acc[NT];
+                float in = 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kx = 0; kx < 2; ++kx) {
+                        bf16x8 fs[3];
+#pragma unroll
+                        for (int s = 0; s < 3; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane]);
+                        acc[j] = mma<2>(acc[j], fs, fo[kx]);
+                    }
+                    float q4[4] = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (FLOW) widen4(lds.q, r0, zt0 + j, q4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[j][i] *= dt;
+                        if constexpr (FLOW) in = fmaf(q4[i], acc[j][i], in);
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (2 * ks > tw) break;
+                    float pr[8];
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const int ts = 2 * ks + hf;
+                        f32x4 m = {0.f, 0.f, 0.f, 0.f};
+                        if (ts <= tw) {
+#pragma unroll
+                            for (int kx = 0; kx < 2; ++kx) {
+                                bf16x8 fv[NS];
+                                rows_of(lds.v, 16 * ts + col, kx, fv);
+                                m = mma<NP - 1>(m, fv, fo[kx]);
+                            }
+                            const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec.gh[16 * ts + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * ts + 4 * quarter]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float x = m[i] * (p.scale * fast_exp2((gh - sh[i]) + (gl - sl[i])));
+                                m[i] = ts < tw || 4 * quarter + i <= col ? x : 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) pr[4 * hf + i] = m[i];
+                    }
+                    bf16x8 fp[NP];
+                    split8<NP>(pr, fp);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        bf16x8 fk[NS];
+                        across(lds.k, zt0 + j, ks, fk);
+                        acc[j] = mma<NP - 1>(acc[j], fk, fp);
+                    }
+                }
+                store(p.dq, p.Dk, acc);
+                if constexpr (FLOW) {
+                    in += __shfl_xor(in, 16);
+                    in += __shfl_xor(in, 32);
+                    if (quarter == 0) lds.in[w4 / NT][r0] = in;
+                }
+            }
+            // ---- X in front of the chunk
+            const float ed = dec.end;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st[x][i] *= ed;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (32 * ks >= n) break;
+                const f32x4 a0 = *reinterpret_cast<const f32x4*>(&dec.dt[32 * ks + 4 * quarter]), a1 = *reinterpret_cast<const f32x4*>(&dec.dt[32 * ks + 16 + 4 * quarter]);
+                bf16x8 fq[NS];
+                across(lds.q, w4, ks, fq);
+                float x8[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x8[i] = 0.f;
+#pragma unroll
+                    for (int s = NS - 1; s >= 0; --s) x8[i] += (float)fq[s][i];
+                    x8[i] *= i < 4 ? a0[i & 3] : a1[i & 3];
+                }
+                bf16x8 fd[3];
+                split8<3>(x8, fd);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    bf16x8 fo[NS];
+                    across(lds.gy, x, ks, fo);
+                    st[x] = mma<2>(st[x], fo, fd);
+                }
+            }
+            have = true;
+            if (wave == 0 && ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
+        } else if (16 * tw < n) {
+            const float gh = dec.gh[r0], gl = dec.gl[r0], dk = dec.dk[r0];
+            bf16x8 fk[2][NS], fv[2][NS];
+#pragma unroll
+            for (int kx = 0; kx < 2; ++kx) {
+                rows_of(lds.k, r0, kx, fk[kx]);
+                rows_of(lds.v, r0, kx, fv[kx]);
+            }
+            f32x4 ak[NT], av[NT], flow[FLOW ? 4 : 1];
+            float out = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) ak[j] = av[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < (FLOW ? 4 : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (have) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int x = zt0 + j;
+#pragma unroll
+                    for (int kx = 0; kx < 2; ++kx) {
+                        bf16x8 fx[3], fy[3];
+#pragma unroll
+                        for (int s = 0; s < 3; ++s) {
+                            fx[s] = *reinterpret_cast<const bf16x8*>(&lds.x[s][16 * x + col][kx * 32 + 8 * quarter]);
+                            const __bf16* q = &lds.x[s][32 * kx + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
+                            fy[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
+                        }
+                        ak[j] = mma<2>(ak[j], fx, fv[kx]);
+                        av[j] = mma<NP - 1>(av[j], fy, fk[kx]);
+                    }
+                    float k4[4] = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (FLOW) widen4(lds.k, r0, x, k4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        ak[j][i] *= dk;
+                        av[j][i] *= dk;
+                        if constexpr (FLOW) out = fmaf(k4[i], ak[j][i], out);
+                    }
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (2 * ks + 1 < tw) continue;            // tokens t in front of s
+                if (32 * ks >= n) break;
+                float pp[8], dp[8], pf[8];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int tt = 2 * ks + hf;
+                    f32x4 mq = {0.f, 0.f, 0.f, 0.f}, mo = {0.f, 0.f, 0.f, 0.f};
+                    if (tt >= tw) {
+#pragma unroll
+                        for (int kx = 0; kx < 2; ++kx) {
+                            bf16x8 f[NS];
+                            rows_of(lds.q, 16 * tt + col, kx, f);
+                            mq = mma<FLOW ? 2 : NP - 1>(mq, f, fk[kx]);
+                            rows_of(lds.gy, 16 * tt + col, kx, f);
+                            mo = mma<FLOW ? 2 : NP - 1>(mo, f, fv[kx]);
+                        }
+                        const f32x4 th = *reinterpret_cast<const f32x4*>(&dec.gh[16 * tt + 4 * quarter]), tl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * tt + 4 * quarter]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = p.scale * fast_exp2((th[i] - gh) + (tl[i] - gl));
+                            const bool seen = tt > tw || 4 * quarter + i >= col;
+                            const float y = seen ? mq[i] * x : 0.f;
+                            if constexpr (FLOW) pf[4 * hf + i] = y * mo[i];
+                            mo[i] = seen ? mo[i] * x : 0.f;
+                            mq[i] = y;
+                        }
+                    } else if constexpr (FLOW) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) pf[4 * hf + i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        pp[4 * hf + i] = mq[i];
+                        dp[4 * hf + i] = mo[i];
+                    }
+                }
+                bf16x8 fp[NP], fd[NP];
+                split8<NP>(pp, fp);
+                split8<NP>(dp, fd);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    bf16x8 f[NS];
+                    across(lds.gy, zt0 + j, ks, f);
+                    av[j] = mma<NP - 1>(av[j], f, fp);
+                    across(lds.q, zt0 + j, ks, f);
+                    ak[j] = mma<NP - 1>(ak[j], f, fd);
+                }
+                if constexpr (FLOW) {
+                    bf16x8 ff[3];
+                    split8<3>(pf, ff);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        if (j < tw || j > 2 * ks + 1) continue;
+                        // ones where j <= t, row j of the tile in lane col: all of a tile behind it, none of one in front of it
+                        u32x4 ones;
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const unsigned lo = 4 * quarter + 2 * e >= col ? 0x3f80u : 0u, hi = 4 * quarter + 2 * e + 1 >= col ? 0x3f800000u : 0u;
+                                ones[2 * hf + e] = 2 * ks + hf > j ? 0x3f803f80u : 2 * ks + hf == j ? lo | hi : 0u;
+                            }
+                        const bf16x8 fu[1] = {__builtin_bit_cast(bf16x8, ones)};
+                        flow[j] = mma<2>(flow[j], fu, ff);
+                    }
+                }
+            }
+            store(p.dk, p.Dk, ak);
+            store(p.dv, p.Dv, av);
+            if constexpr (FLOW) {
+                out += __shfl_xor(out, 16);
+                out += __shfl_xor(out, 32);
+                if (quarter == 0) lds.out[w4 / NT][r0] = out;
+                float crossing[16];                       // of rows s in front of j
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) crossing[4 * j + i] = j < NT && (j > tw || (j == tw && 4 * quarter + i > col)) ? flow[j][i] : 0.f;
+                int index;
+                const float cf = wkv6_detail::row_sums16(crossing, lane, index);
+                // (the other waves of a 32-token chunk have made the same terms)
+                if ((index >> 2) < NT) lds.inner[w4][16 * (index >> 2) + 4 * quarter + (index & 3)] = w4 < NT ? cf : 0.f;
+            }
+        } else if (FLOW && lane < L) lds.inner[w4][lane] = 0.f;
+        if (group == 1) have = true;
+        __syncthreads();
+        if constexpr (FLOW) {
+            if (wave == 0) {
+                const int at = min(lane, L - 1);
+                double in = 0., out = 0.;
+                if (lane < n) {
+                    in = NT == 4 ? (double)lds.in[0][lane] : (double)lds.in[0][lane] + lds.in[1][lane];
+                    out = NT == 4 ? (double)lds.out[0][lane] : (double)lds.out[0][lane] + lds.out[1][lane];
+                }
+                const double inner = ((double)lds.inner[0][at] + lds.inner[1][at]) + ((double)lds.inner[2][at] + lds.inner[3][at]);
+                const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * dec.end;
+                const double all = flow_sum(inner, in, out, lane) + through;
+                if (lane < n) p.dg[((long long)w.base * p.T + w.first + t0 + lane) * p.H + h] = (float)all;
+            }
+        }
+    }
+
+    if (p.dstate && w.is_first && group == 0) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int xc = 16 * x + 4 * quarter + i;
+                if (xc < p.Dv && zc < p.Dk) p.dstate[page + (long long)zc * p.Dv + xc] = st[x][i];
+            }
+    }
+}
+
+template <typename IO> int launch_decay_bwd(const BwdParams& p, bool vec, hipStream_t st);
+extern template int launch_decay_bwd<float>(const BwdParams&, bool, hipStream_t);
+extern template int launch_decay_bwd<__hip_bfloat16>(const BwdParams&, bool, hipStream_t);
+extern template int launch_decay_bwd<__half>(const BwdParams&, bool, hipStream_t);
+
+template <typename IO>
+int launch_decay_bwd(const BwdParams& p, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)((long long)p.segs * p.H)), block(BWD_THREADS);
+    if (p.dg) {
+        if (vec) hipLaunchKernelGGL((decay_bwd_kernel<IO, true, true>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((decay_bwd_kernel<IO, true, false>), grid, block, 0, st, p);
+    } else {
+        if (vec) hipLaunchKernelGGL((decay_bwd_kernel<IO, false, true>), grid, block, 0, st, p);
+        else hipLaunchKernelGGL((decay_bwd_kernel<IO, false, false>), grid, block, 0, st, p);
+    }
+    return check_launch("decay_attention (gradients)");
+}
+
+}  // namespace decay
+}  // namespace vrwkv
