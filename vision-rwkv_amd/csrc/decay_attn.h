@@ -129,43 +129,142 @@ __device__ __forceinline__ Place find_place(const Call& p, int gid, int L) {
     return w;
 }
 
-__device__ __forceinline__ float log_decay(const Call& p, int base, int token, int h) {
-    const long long i = base * p.g_sb + token * p.g_st + h * p.g_sh;
-    float x;
-    if (p.g_dtype == VRWKV_F32) x = static_cast<const float*>(p.g)[i];
-    else if (p.g_dtype == VRWKV_BF16) x = to_f32(static_cast<const __hip_bfloat16*>(p.g)[i]);
-    else x = to_f32(static_cast<const __half*>(p.g)[i]);
-    return x < -200.f ? -200.f : x;                       // (exp(-200) is zero in fp32 too; sums of -inf or the lowest value would be -inf, their differences NaN)
-}
-
 // The eight channels d .. d + 7 of a row: at byte offset `at` of the buffer in one or two loads of 16 bytes where rows come in such pieces (VEC), element by
-// element otherwise; `count` of them exist.  What does not is asked of an offset outside the buffer and arrives as zero, without a branch: loads behind
+// element otherwise; `count` of them exist; `ahead` bytes behind, the same for all lanes.  What does not is asked of an offset outside the buffer and arrives as zero, without a branch: loads behind
 // branches were waited for one by one, 4.5 of the 5.5 us that a chunk took.
 template <typename IO> struct Piece { unsigned w[sizeof(IO) * 2]; };
 template <typename IO, bool VEC>
-__device__ __forceinline__ Piece<IO> load_piece(__amdgpu_buffer_rsrc_t buf, unsigned at, int count) {
+__device__ __forceinline__ Piece<IO> load_piece(__amdgpu_buffer_rsrc_t buf, unsigned at, int count, unsigned ahead) {
     Piece<IO> r;
     if constexpr (VEC) {
-        const unsigned o = count > 0 ? at : OOB_OFFSET;
 #pragma unroll
         for (int i = 0; i < (int)sizeof(IO) / 2; ++i) {
-            const auto t = BufRaw<16>::ld(buf, o + 16 * i, 0);
+            const auto t = BufRaw<16>::ld(buf, at + 16 * i, ahead);
 #pragma unroll
             for (int c = 0; c < 4; ++c) r.w[4 * i + c] = t[c];
         }
     } else if constexpr (sizeof(IO) == 4) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r.w[e] = BufRaw<4>::ld(buf, e < count ? at + 4 * e : OOB_OFFSET, 0);
+        for (int e = 0; e < 8; ++e) r.w[e] = BufRaw<4>::ld(buf, e < count ? at + 4 * e : OOB_OFFSET, ahead);
     } else {
         unsigned short h[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = BufRaw<2>::ld(buf, e < count ? at + 2 * e : OOB_OFFSET, 0);
+        for (int e = 0; e < 8; ++e) h[e] = BufRaw<2>::ld(buf, e < count ? at + 2 * e : OOB_OFFSET, ahead);
 #pragma unroll
         for (int e = 0; e < 4; ++e) r.w[e] = (unsigned)h[2 * e] | (unsigned)h[2 * e + 1] << 16;
     }
     return r;
 }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) { return make_rsrc(p, 0x7fffffffu); }
+// The value stays in scalar registers: read again from the arguments it cost each chunk's fetch 1600 cycles and each result's address as much.
+template <typename T>
+__device__ __forceinline__ void keep(T& x) { asm volatile("" : "+s"(x)); }
+
+// Four channels of a row, `count` of them there.
+template <typename O, bool VEC>
+__device__ __forceinline__ void store_quad(__amdgpu_buffer_rsrc_t buf, unsigned at, int count, f32x4 x) {
+    O q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = from_f32<O>(x[i]);
+    if constexpr (VEC) {
+        typename BufRaw<4 * sizeof(O)>::type d;
+        __builtin_memcpy(&d, q, sizeof(d));
+        BufRaw<4 * sizeof(O)>::st(d, buf, count > 0 ? at : OOB_OFFSET, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            typename BufRaw<sizeof(O)>::type d;
+            __builtin_memcpy(&d, &q[i], sizeof(d));
+            BufRaw<sizeof(O)>::st(d, buf, i < count ? at + i * (unsigned)sizeof(O) : OOB_OFFSET, 0);
+        }
+    }
+}
+
+// A tensor's rows of one sequence and head, and a thread's pieces of a chunk: rows `row`, `row` + STEP .. in the order that the kernel takes them.  Row i is
+// token t0 + i, or back along the tokens t0 + n - 1 - i, which is L - 1 - i from token t0 + n - L on: a thread's offsets stay the same.
+template <typename IO, int PIECES, int STEP, bool VEC>
+struct Source {
+    const char* p;
+    int pitch;                                            // bytes from token to token
+    unsigned at;
+    int row, count;
+    __device__ __forceinline__ void open(const View& v, int base, int first, int head, int L, bool rev, int row_, int d, int dim) {
+        p = static_cast<const char*>(v.p) + (base * v.sb + (long long)first * v.st + (head / v.share) * v.sh) * (int)sizeof(IO);
+        pitch = (int)v.st * (int)sizeof(IO);
+        keep(p);
+        keep(pitch);
+        row = row_;
+        count = dim - d;
+        at = (unsigned)((rev ? L - 1 - row - STEP * (PIECES - 1) : row) * pitch + d * (int)sizeof(IO));
+        if (count <= 0) at = OOB_OFFSET;
+    }
+    // the first of the chunk's tokens in memory (or of the L that end with its last) and its rows
+    __device__ __forceinline__ void load(Piece<IO> (&r)[PIECES], int token, int n, bool rev) const {
+        const auto buf = buffer_at(p + (long long)token * pitch);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const bool there = row + STEP * i < n;
+            r[i] = load_piece<IO, VEC>(buf, there ? at : OOB_OFFSET, there ? count : 0, (unsigned)((rev ? PIECES - 1 - i : i) * STEP * pitch));
+        }
+    }
+};
+// Where a lane's results go: four channels of a row, and every sixteenth behind them.
+template <typename IO, bool VEC>
+struct Sink {
+    char* p;
+    int pitch, f32;
+    unsigned at;
+    int count;
+    __device__ __forceinline__ void open(const OutView& v, int base, int first, int head, int row, int d, int dim) {
+        f32 = v.f32;
+        const int e = f32 ? 4 : (int)sizeof(IO);
+        p = v.p ? static_cast<char*>(v.p) + (base * v.sb + (long long)first * v.st + head * v.sh) * e : nullptr;
+        pitch = (int)v.st * e;
+        keep(p);
+        keep(pitch);
+        keep(f32);
+        at = (unsigned)(row * pitch + d * e);
+        count = dim - d;
+    }
+    template <int N>
+    __device__ __forceinline__ void store(const f32x4 (&x)[N], int token, bool there) const {
+        if (!p) return;
+        const auto buf = buffer_at(p + (long long)token * pitch);
+        const int have = there ? count : 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (f32) store_quad<float, VEC>(buf, at + 64 * j, have - 16 * j, x[j]);
+            else store_quad<IO, VEC>(buf, at + 16 * j * (unsigned)sizeof(IO), have - 16 * j, x[j]);
+        }
+    }
+};
+// The log decays of a sequence and head.
+struct Gates {
+    const char* p;
+    int pitch, dtype;
+    __device__ __forceinline__ void open(const Call& c, int base, int first, int head) {
+        const int e = c.g_dtype == VRWKV_F32 ? 4 : 2;
+        p = static_cast<const char*>(c.g) + (base * c.g_sb + (long long)first * c.g_st + head * c.g_sh) * e;
+        pitch = (int)c.g_st * e;
+        dtype = c.g_dtype;
+        keep(p);
+        keep(pitch);
+        keep(dtype);
+    }
+    // of token `token` + i, as it lies: widened where it is used, so the fetch is ahead, with no branch on its type behind which it would be waited for
+    struct Raw {
+        unsigned word, half;
+    };
+    __device__ __forceinline__ Raw fetch(int token, int i, bool there) const {
+        const auto buf = buffer_at(p + (long long)token * pitch);
+        const unsigned at = (unsigned)(i * pitch);
+        return {BufRaw<4>::ld(buf, there && dtype == VRWKV_F32 ? at : OOB_OFFSET, 0), BufRaw<2>::ld(buf, there && dtype != VRWKV_F32 ? at : OOB_OFFSET, 0)};
+    }
+    __device__ __forceinline__ float widen(Raw r) const {
+        const float x = dtype == VRWKV_F32 ? __builtin_bit_cast(float, r.word) : dtype == VRWKV_BF16 ? __builtin_bit_cast(float, r.half << 16) : (float)__builtin_bit_cast(_Float16, (unsigned short)r.half);
+        return x < -200.f ? -200.f : x;                   // (exp(-200) is zero in fp32 too; sums of -inf or the lowest value would be -inf, their differences NaN)
+    }
+};
 // x as the sum of n bf16 numbers (two at a time): 16 bits of it with two, all 24 with three
 template <int N>
 __device__ __forceinline__ void split_pair(float x0, float x1, unsigned (&t)[N]) {
@@ -252,26 +351,6 @@ __device__ __forceinline__ double flow_sum(double inner, double in, double out, 
     return inner + in + before;
 }
 
-// Four channels of a row, `count` of them there.
-template <typename O, bool VEC>
-__device__ __forceinline__ void store_quad(__amdgpu_buffer_rsrc_t buf, unsigned at, int count, f32x4 x) {
-    O q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = from_f32<O>(x[i]);
-    if constexpr (VEC) {
-        typename BufRaw<4 * sizeof(O)>::type d;
-        __builtin_memcpy(&d, q, sizeof(d));
-        BufRaw<4 * sizeof(O)>::st(d, buf, count > 0 ? at : OOB_OFFSET, 0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            typename BufRaw<sizeof(O)>::type d;
-            __builtin_memcpy(&d, &q[i], sizeof(d));
-            BufRaw<sizeof(O)>::st(d, buf, i < count ? at + i * (unsigned)sizeof(O) : OOB_OFFSET, 0);
-        }
-    }
-}
-
 template <typename IO, int DX, int MODE>
 struct Lds {
     static constexpr int L = chunk_len<IO, DX, MODE>, NS = in_terms<IO>;
@@ -343,71 +422,73 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     const int z0 = z * TZ;
     const bool rev = r.reverse;
 
+    const int nc = (w.s1 - w.s0 + L - 1) / L;
+    const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, rowz = tid / (TZ / 8), dzo = tid % (TZ / 8) * 8;
+    constexpr int STEPX = THREADS / (DX / 8), STEPZ = THREADS / (TZ / 8);   // rows between a thread's pieces
+    Source<IO, PA, STEPX, VEC> sa, sb;
+    Source<IO, PC, STEPZ, VEC> sc, se;
+    Gates gates;
+    gates.open(p, w.base, w.first, h);
+    if constexpr (OUT) sa.open(r.a, w.base, w.first, h, L, rev, rowx, dxo, r.dx);
+    sb.open(r.b, w.base, w.first, h, L, rev, rowx, dxo, r.dx);
+    sc.open(r.c, w.base, w.first, h, L, rev, rowz, z0 + dzo, r.dz);
+    if constexpr (EXTRA) se.open(r.e, w.base, w.first, h, L, rev, rowz, z0 + dzo, r.dz);
+    Piece<IO> ra[PA], rb[PA], rc[PC], re[PC];
+    Gates::Raw rg{}, rg_next{};
+    const auto fetch = [&](int c) {
+        const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0), token = rev ? t0 + n - L : t0;
+        if constexpr (OUT) sa.load(ra, token, n, rev);
+        sb.load(rb, token, n, rev);
+        sc.load(rc, token, n, rev);
+        if constexpr (EXTRA) se.load(re, token, n, rev);
+        if (wave == 0) {
+            // back along the tokens a row's decay is that of the token behind it, and none behind the last
+            rg = rev ? gates.fetch(t0 + n - 63, 63 - lane, lane < n && t0 + n - lane < w.len) : gates.fetch(t0, lane, lane < n);
+            if constexpr (MODE == FLOWS) rg_next = gates.fetch(t0 + n, 0, t0 + n < w.len);
+        }
+    };
+    if (nc > 0) fetch(rev ? nc - 1 : 0);
+
     // ---- the state that the segment starts from: rows 16 x + 4 quarter + i, column 16 wave + col of the tile
     f32x4 st[NX];
     const long long page = ((long long)w.n * p.H + h) * ((long long)r.dx * r.dz);
     const long long seg_at = (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ);
     const int zc = z0 + 16 * wave + col;
-    bool have = MODE != STATES;
-    if (MODE == STATES) {
-#pragma unroll
-        for (int x = 0; x < NX; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-    } else if (r.seg && !(rev ? w.is_last : w.is_first)) {
-        have = true;
+    const bool first_one = rev ? w.is_last : w.is_first;
+    bool have = MODE != STATES && (first_one ? r.init != nullptr : true);
+    if (MODE != STATES && !first_one) {
 #pragma unroll
         for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4);
     } else {
-        have = r.init != nullptr;
+        const auto buf = buffer_at(r.init + page);
 #pragma unroll
         for (int x = 0; x < NX; ++x)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int xc = 16 * x + 4 * quarter + i;
-                st[x][i] = r.init && xc < r.dx && zc < r.dz ? r.init[page + xc * r.sx + zc * r.sz] : 0.f;
+                st[x][i] = __builtin_bit_cast(float, BufRaw<4>::ld(buf, have && xc < r.dx && zc < r.dz ? (unsigned)(xc * (int)r.sx + zc * (int)r.sz) * 4u : OOB_OFFSET, 0));
             }
     }
+    Sink<IO, VEC> so;
+    if constexpr (OUT) {
+        const int t = 16 * (wave % NT) + col;
+        so.open(r.o, w.base, w.first, h, rev ? L - 1 - t : t, z0 + 16 * (wave / NT * NT) + 4 * quarter, r.dz);
+    }
+    const float *anchors = nullptr, *edges = nullptr;     // of the segment's first chunk and token
+    if constexpr (MODE == EDGES || MODE == FLOWS || MODE == CHUNKS) {
+        anchors = r.anchors + (((long long)(w.chunk0 + w.s0 / L) * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4;
+        if (MODE != CHUNKS) edges = r.edge + ((long long)z * p.rows + (long long)w.base * p.T + w.first) * p.H + h;
+    }
+    const long long anchor_step = (long long)p.H * r.tiles * (DX * TZ);
+    float scale = p.scale, s_in = r.s_in, s_upd = r.s_upd;
+    keep(scale);
+    keep(s_in);
+    keep(s_upd);
 
-    const int nc = (w.s1 - w.s0 + L - 1) / L;
-    const auto origin = [&](const View& v) { return static_cast<const IO*>(v.p) + w.base * v.sb + (long long)w.first * v.st + (h / v.share) * v.sh; };
-    const IO *const pa = origin(r.a), *const pb = origin(r.b), *const pc = origin(r.c), *const pe = EXTRA ? origin(r.e) : nullptr;
-    char* const po = static_cast<char*>(r.o.p) + (w.base * r.o.sb + (long long)w.first * r.o.st + h * r.o.sh) * (r.o.f32 ? 4 : (int)sizeof(IO));
-
-    // The chunk's rows in the order that the kernel takes them: row i is token t0 + i, or t0 + n - 1 - i back along the tokens, which is L - 1 - i from
-    // token t0 + n - L on; so a thread's offsets stay the same, and which rows there are is asked on top.
-    Piece<IO> ra[OUT ? PA : 1], rb[PA], rc[PC], re[EXTRA ? PC : 1];
-    float rg = 0.f, rg_next = 0.f;
-    const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, rowz = tid / (TZ / 8), dzo = z0 + tid % (TZ / 8) * 8;
-    constexpr int STEPX = THREADS / (DX / 8), STEPZ = THREADS / (TZ / 8);   // rows between a thread's pieces
-    const int countx = r.dx - dxo, countz = r.dz - dzo;
-    const auto fetch = [&](int c) {
-        const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
-        const long long tok = rev ? t0 + n - L : t0;
-        const auto buf = [&](const IO* q, const View& v) { return buffer_at(q + tok * v.st); };
-        const auto at = [&](int row, const View& v, int d) { return (unsigned)(((rev ? L - 1 - row : row) * (int)v.st + d) * (int)sizeof(IO)); };
-        const auto ba = buf(OUT ? pa : pb, OUT ? r.a : r.b), bb = buf(pb, r.b), bc = buf(pc, r.c), be = buf(EXTRA ? pe : pc, EXTRA ? r.e : r.c);
-#pragma unroll
-        for (int i = 0; i < PA; ++i) {
-            const int row = rowx + STEPX * i, m = row < n ? countx : 0;
-            if constexpr (OUT) ra[i] = load_piece<IO, VEC>(ba, at(row, r.a, dxo), m);
-            rb[i] = load_piece<IO, VEC>(bb, at(row, r.b, dxo), m);
-        }
-#pragma unroll
-        for (int i = 0; i < PC; ++i) {
-            const int row = rowz + STEPZ * i, m = row < n ? countz : 0;
-            rc[i] = load_piece<IO, VEC>(bc, at(row, r.c, dzo), m);
-            if constexpr (EXTRA) re[i] = load_piece<IO, VEC>(be, at(row, r.e, dzo), m);
-        }
-        if (wave == 0) {
-            // back along the tokens a row's decay is that of the token behind it, and none behind the last
-            const int g = rev ? t0 + n - lane : t0 + lane;
-            rg = lane < n && g < w.len ? log_decay(p, w.base, w.first + g, h) : 0.f;
-            if constexpr (MODE == FLOWS) rg_next = t0 + n < w.len ? log_decay(p, w.base, w.first + t0 + n, h) : 0.f;
-        }
-    };
     float seg_log = 0.f;                                  // (STATES: the segment's whole decay, from wave 0)
     const auto put_decays = [&](typename S::Decays& d) {   // wave 0
         // sums in 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth
-        const double G = wave_scan_inclusive((double)rg * 1.4426950408889634);
+        const double G = wave_scan_inclusive((double)gates.widen(rg) * 1.4426950408889634);
         const double end = lane_double(G, 63);
         const float gh = (float)G;
         if (lane < L) {
@@ -418,15 +499,16 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         }
         if (lane == 0) {
             d.end = fast_exp2((float)end);
-            if constexpr (MODE == FLOWS) d.through = fast_exp2((float)(end + (double)rg_next * 1.4426950408889634));
+            if constexpr (MODE == FLOWS) d.through = fast_exp2((float)(end + (double)gates.widen(rg_next) * 1.4426950408889634));
         }
         if (MODE == STATES) seg_log += (float)end;
     };
-    if (nc > 0) {
-        fetch(rev ? nc - 1 : 0);
-        if (wave == 0) put_decays(lds.d[0]);
-    }
+    if (nc > 0 && wave == 0) put_decays(lds.d[0]);
     for (int ci = 0; ci < nc; ++ci) {
+        // (what follows from the lane is worked out anew for each chunk: kept over the loop it fills the registers, masks for every tile among it)
+        int lane_ = lane;
+        asm volatile("" : "+v"(lane_));
+        const int quarter = lane_ >> 4, col = lane_ & 15;
         const int c = rev ? nc - 1 - ci : ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
         // ---- operands to the LDS
 #pragma unroll
@@ -450,7 +532,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         }
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
-            const int row = rowz + STEPZ * i, d = dzo - z0;
+            const int row = rowz + STEPZ * i, d = dzo;
             u32x4 t[NS];
             piece_terms<IO>(rc[i], t);
 #pragma unroll
@@ -473,7 +555,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                 }
             }
         }
-        __syncthreads();
+        lds_barrier();                                    // (orders the LDS alone: the next chunk's rows and this one's results stay on their way)
         if (ci + 1 < nc) fetch(rev ? c - 1 : c + 1);
         typename S::Decays& dec_ = lds.d[ci & 1];
 
@@ -481,14 +563,13 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         f32x4 behind[MODE == FLOWS ? NX : 1];              // R behind this chunk, as the pass of dk left it
         float given = 0.f;                                // (wave 0) what its tokens give over its end
         if constexpr (MODE == FLOWS) {
-            const long long ck = (((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * r.tiles + z) * (DX * TZ);
 #pragma unroll
-            for (int x = 0; x < NX; ++x) behind[x] = *reinterpret_cast<const f32x4*>(r.anchors + ck + ((x * 4 + wave) * 64 + lane) * 4);
-            if (wave == 0 && lane < n) given = r.edge[((long long)z * p.rows + (long long)w.base * p.T + w.first + t0 + lane) * p.H + h];
+            for (int x = 0; x < NX; ++x) behind[x] = *reinterpret_cast<const f32x4*>(anchors + c * anchor_step + x * 1024);
+            if (wave == 0 && lane < n) given = edges[(long long)(t0 + lane) * p.H];
         }
         const int tw = wave % NT, zt0 = wave / NT * NT, t = 16 * tw + col;
         if (OUT && 16 * tw < n) {
-            const float gth = dec_.gh[t], gtl = dec_.gl[t], dec = dec_.dt[t] * r.s_in;
+            const float gth = dec_.gh[t], gtl = dec_.gl[t], dec = dec_.dt[t] * s_in;
             bf16x8 fa[KX][NS];
 #pragma unroll
             for (int kx = 0; kx < KX; ++kx)
@@ -543,7 +624,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                         const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec_.gh[16 * st_ + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec_.gl[16 * st_ + 4 * quarter]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float x = m[i] * (p.scale * fast_exp2((gth - sh[i]) + (gtl - sl[i])));
+                            const float x = m[i] * (scale * fast_exp2((gth - sh[i]) + (gtl - sl[i])));
                             m[i] = st_ < tw || 4 * quarter + i <= col ? x : 0.f;
                         }
                         if constexpr (MODE == FLOWS) {
@@ -600,17 +681,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                     acc[j] = mma<NP - 1>(acc[j], fc, fp);
                 }
             }
-            if (r.o.p) {
-                const long long tok = rev ? t0 + n - L : t0;
-                const auto bo = buffer_at(po + tok * r.o.st * (r.o.f32 ? 4 : (int)sizeof(IO)));
-                const int zl = z0 + 16 * zt0 + 4 * quarter, count = t < n ? r.dz - zl : 0;
-                const unsigned at = (unsigned)((rev ? L - 1 - t : t) * (int)r.o.st + zl);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if (r.o.f32) store_quad<float, VEC>(bo, (at + 16 * j) * 4, count - 16 * j, acc[j]);
-                    else store_quad<IO, VEC>(bo, (at + 16 * j) * (unsigned)sizeof(IO), count - 16 * j, acc[j]);
-                }
-            }
+            so.store(acc, rev ? t0 + n - L : t0, t < n);
             if constexpr (EXTRA) {                        // over the quarters: the channels of a row
                 edge += __shfl_xor(edge, 16);
                 edge += __shfl_xor(edge, 32);
@@ -641,9 +712,8 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         // ---- the state behind the chunk
         {
             if constexpr (MODE == EDGES || MODE == CHUNKS) {
-                const long long ck = (((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * r.tiles + z) * (DX * TZ);
 #pragma unroll
-                for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.anchors + ck + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
+                for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(const_cast<float*>(anchors) + c * anchor_step + x * 1024) = st[x];
             }
             if (MODE == CHUNKS && ci + 1 == nc) break;     // (nothing starts behind it)
             const float ed = dec_.end;
@@ -667,8 +737,8 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x8[i] *= d0[i] * r.s_upd;
-                    x8[4 + i] *= d1[i] * r.s_upd;
+                    x8[i] *= d0[i] * s_upd;
+                    x8[4 + i] *= d1[i] * s_upd;
                 }
                 bf16x8 fv[3];
                 split8<3>(x8, fv);
@@ -686,11 +756,11 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
             have = true;
         }
         if (wave == 0 && ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
-        __syncthreads();
+        lds_barrier();
         if constexpr (MODE == EDGES) {
             if (wave == 0 && lane < n) {
-                const long long row = (long long)w.base * p.T + w.first + t0 + n - 1 - lane;
-                r.edge[((long long)z * p.rows + row) * p.H + h] = NT == 4 ? lds.edge[0][lane] : lds.edge[0][lane] + lds.edge[1][lane];
+                const float x = NT == 4 ? lds.edge[0][lane] : lds.edge[0][lane] + lds.edge[1][lane];
+                const_cast<float*>(edges)[(long long)(t0 + n - 1 - lane) * p.H] = x;
             }
         }
         if constexpr (MODE == FLOWS) {
@@ -718,7 +788,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         if (tid == 0 && z == 0) r.seg_decay[(long long)gid * p.H + h] = fast_exp2(seg_log);
     } else {
         if (r.last && (rev ? w.is_first : w.is_last)) {
-            const float d = rev && w.len > 0 ? fast_exp2(log_decay(p, w.base, w.first, h) * LOG2E) : 1.f;   // back along the tokens: the first one's decay
+            const float d = rev && w.len > 0 ? fast_exp2(gates.widen(gates.fetch(0, 0, true)) * LOG2E) : 1.f;   // back along the tokens: the first one's decay
 #pragma unroll
             for (int x = 0; x < NX; ++x)
 #pragma unroll

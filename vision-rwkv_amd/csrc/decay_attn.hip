@@ -166,7 +166,7 @@ int check_tensors(const vrwkv_decay_args& a, const char* who) {
     for (const void* p : {a.q, a.k, a.v, (const void*)a.y, a.gy, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv})
         if ((size_t)p & m) { set_error("%s: a tensor is not aligned to its elements", who); return VRWKV_INVALID_ARG; }
     // (offsets inside a chunk's rows are 32 bits)
-    for (const long long st : {a.q_stride[1], a.k_stride[1], a.v_stride[1], a.gy ? a.gy_stride[1] : 0, (long long)a.H * std::max(a.Dk, a.Dv)})
+    for (const long long st : {a.q_stride[1], a.k_stride[1], a.v_stride[1], a.gy ? a.gy_stride[1] : 0, a.g_stride[1], (long long)a.H * std::max(a.Dk, a.Dv)})
         if (st < 0 || st >= 1 << 22) { set_error("%s: tokens %lld elements apart, at most 2^22", who, st); return VRWKV_UNSUPPORTED_SHAPE; }
     for (const void* p : {a.g, (const void*)a.dg})
         if ((size_t)p & (elem(a.g_dtype) - 1)) { set_error("%s: g is not aligned to its elements", who); return VRWKV_INVALID_ARG; }

@@ -6,10 +6,11 @@
 //     X <- exp(G_end) X + scale sum_t exp(G_t) q_t gy_t^T
 //     dg_j = what crosses from tokens in front of j to j and behind: the terms P_ts (gy_t . v_s) with s < j <= t; q . (S0's part of dq) of the tokens from j on;
 //            k . (X's part of dk) of those in front; exp(G_end) <S0, X>.  Sums of what crosses, so nothing cancels where little does.
-// Eight waves, two a SIMD: four take dq, tokens t along the lanes, and X; four take dk, dv and dg, tokens s along the lanes.  Every operand of the products is
-// read as it lies or across its rows, so the chunk's rows are staged once, where dv, dk and dq by themselves (decay_attn.h) stage ten tensors.
-// X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
-// 64 x 196 tokens of 12 heads, bf16: @BASE@.
+// Eight waves, two a SIMD: four take dq and dg's crossings inside the chunk, tokens t along the lanes; four take dk, dv and X, tokens s along the lanes.  (Sixteen
+// waves of four kinds: 110 us for 64 x 196 tokens of 12 heads in bf16 where eight took 90, for what the kinds form twice and the registers that they lack.)
+// Every operand of the products is read as it lies or across its rows, so the chunk's rows are staged once, where dv, dk and dq by themselves (decay_attn.h)
+// stage ten tensors.  X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
+// @BASE@
 #pragma once
 #include "decay_attn.h"
 
@@ -39,7 +40,10 @@ struct BwdLds {
         float gh[L], gl[L], dt[L], dk[L];
         float end;
     } d[2];
-    float in[2][L], out[2][L], inner[4][L], cross[4];     // what a token receives over the chunk's front, gives over its end, by halves of the columns; what crosses it inside; <S0, X>
+    struct Flows {
+        float in[2][L], out[2][L];                        // what a token receives over the chunk's front and gives over its end, by halves of the columns
+        float inner[4][L], through[4];                    // what crosses it inside, by waves; what passes the chunk
+    } f[2];                                               // this chunk's, and the last one's, which are summed beside this one's products
 };
 
 template <typename IO, bool FLOW, bool VEC>
@@ -73,82 +77,119 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
     if (!w.valid) return;
     const int nc = (w.s1 - w.s0 + L - 1) / L;
 
-    // ---- X behind the segment, in the waves of group 0: rows 16 x + 4 quarter + i (v's channels), column 16 w4 + col (k's)
-    f32x4 st[4];
+    const int row0 = (tid & 255) >> 3, d0 = (tid & 7) * 8;
+    Source<IO, PIECES, 32, VEC> sa, sb;                   // the kinds stage a pair of tensors each
+    sa.open(group ? p.k : p.q, w.base, w.first, h, L, false, row0, d0, p.Dk);
+    sb.open(group ? p.gy : p.v, w.base, w.first, h, L, false, row0, d0, p.Dv);
+    Gates gates;
+    gates.open(p, w.base, w.first, h);
+    const float* const chunks = p.chunks + ((long long)(w.chunk0 + w.s0 / L) * p.H + h) * 4096 + (w4 * 64 + lane) * 4;
+    const long long chunk_step = (long long)p.H * 4096;
+    Piece<IO> ra[PIECES], rb[PIECES];
+    Gates::Raw rg{};
+    f32x4 st[4];                                          // group 0: S0; group 1: X.  Rows 16 x + 4 quarter + i (v's channels), column 16 w4 + col (k's)
+    u32x4 held[3][2];                                     // its terms
+    const auto fetch = [&](int c) {
+        const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+        sa.load(ra, t0, n, false);
+        sb.load(rb, t0, n, false);
+        if (wave == 0) rg = gates.fetch(t0, lane, lane < n);
+    };
+    const auto fetch_state = [&](int c) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) st[x] = *reinterpret_cast<const f32x4*>(chunks + c * chunk_step + x * 1024);
+    };
+    const auto hold = [&]() {
+#pragma unroll
+        for (int kx = 0; kx < 2; ++kx) {
+            const float x8[8] = {st[2 * kx][0], st[2 * kx][1], st[2 * kx][2], st[2 * kx][3], st[2 * kx + 1][0], st[2 * kx + 1][1], st[2 * kx + 1][2], st[2 * kx + 1][3]};
+            bf16x8 t[3];
+            split8<3>(x8, t);
+#pragma unroll
+            for (int s = 0; s < 3; ++s) held[s][kx] = __builtin_bit_cast(u32x4, t[s]);
+        }
+    };
+    if (nc > 0) fetch(nc - 1);
+
+    // ---- X behind the segment
     const long long page = ((long long)w.n * p.H + h) * ((long long)p.Dk * p.Dv);
     const int zc = 16 * w4 + col;
-    bool have = false;
-    {
-        const bool cut = p.seg && !w.is_last;
-        have = cut || p.glast;
+    const bool cut = p.seg && !w.is_last;
+    bool have = cut || p.glast;
+    if (group == 0) {
+        if (nc > 0) fetch_state(nc - 1);
+    } else if (cut) {
         // (R behind a segment wants the decay of the token there)
-        const float d = cut ? fast_exp2(log_decay(p, w.base, w.first + w.s1, h) * LOG2E) : 1.f;
+        const float d = fast_exp2(gates.widen(gates.fetch(w.s1, 0, true)) * LOG2E);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (cut) st[x] = *reinterpret_cast<const f32x4*>(p.seg + ((long long)gid * p.H + h) * 4096 + ((x * 4 + w4) * 64 + lane) * 4);
-            else if (p.glast) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int xc = 16 * x + 4 * quarter + i;
-                    if (xc < p.Dv && zc < p.Dk) st[x][i] = p.glast[page + (long long)zc * p.Dv + xc];
-                }
-            }
+            st[x] = *reinterpret_cast<const f32x4*>(p.seg + ((long long)gid * p.H + h) * 4096 + ((x * 4 + w4) * 64 + lane) * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) st[x][i] *= d;
         }
+    } else {
+        const auto buf = buffer_at(p.glast + page);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int xc = 16 * x + 4 * quarter + i;
+                st[x][i] = __builtin_bit_cast(float, BufRaw<4>::ld(buf, have && xc < p.Dv && zc < p.Dk ? (unsigned)(zc * p.Dv + xc) * 4u : OOB_OFFSET, 0));
+            }
     }
+    const int tw = w4 % NT, zt0 = w4 / NT * NT;           // this wave's tile of tokens, its first tile of channels
+    Sink<IO, VEC> oa, ob;                                 // dq; dk and dv
+    oa.open(group ? p.dk : p.dq, w.base, w.first, h, 16 * tw + col, 16 * zt0 + 4 * quarter, p.Dk);
+    ob.open(p.dv, w.base, w.first, h, 16 * tw + col, 16 * zt0 + 4 * quarter, p.Dv);
+    float* dg = FLOW ? p.dg + ((long long)w.base * p.T + w.first) * p.H + h : nullptr;
+    int H = p.H;
+    float scale = p.scale;
+    keep(dg);
+    keep(H);
+    keep(scale);
 
-    const auto origin = [&](const View& v) { return static_cast<const IO*>(v.p) + w.base * v.sb + (long long)w.first * v.st + (h / v.share) * v.sh; };
-    const int half = __builtin_amdgcn_readfirstlane(tid >> 8), row0 = (tid & 255) >> 3, d0 = (tid & 7) * 8;
-    const View &va = half ? p.k : p.q, &vb = half ? p.gy : p.v;
-    const IO *const pa = origin(va), *const pb = origin(vb);
-    const int counta = p.Dk - d0, countb = p.Dv - d0;
-    Piece<IO> ra[PIECES], rb[PIECES];
-    f32x4 s0[4];
-    float rg = 0.f;
-    const auto fetch = [&](int c) {
-        const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
-        const auto ba = buffer_at(pa + (long long)t0 * va.st), bb = buffer_at(pb + (long long)t0 * vb.st);
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int row = row0 + 32 * i;
-            ra[i] = load_piece<IO, VEC>(ba, (unsigned)((row * (int)va.st + d0) * (int)sizeof(IO)), row < n ? counta : 0);
-            rb[i] = load_piece<IO, VEC>(bb, (unsigned)((row * (int)vb.st + d0) * (int)sizeof(IO)), row < n ? countb : 0);
-        }
-        if (group == 0) {
-            const float* ck = p.chunks + ((long long)(w.chunk0 + w.s0 / L + c) * p.H + h) * 4096;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) s0[x] = *reinterpret_cast<const f32x4*>(ck + ((x * 4 + w4) * 64 + lane) * 4);
-        }
-        if (wave == 0) rg = lane < n ? log_decay(p, w.base, w.first + t0 + lane, h) : 0.f;
-    };
     const auto put_decays = [&](typename S::Decays& d) {   // wave 0
-        const double G = wave_scan_inclusive((double)rg * 1.4426950408889634);
+        const double G = wave_scan_inclusive((double)gates.widen(rg) * 1.4426950408889634);
         const double end = lane_double(G, 63);
         const float gh = (float)G;
         if (lane < L) {
             d.gh[lane] = gh;
             d.gl[lane] = (float)(G - gh);
-            d.dt[lane] = fast_exp2(gh) * p.scale;
+            d.dt[lane] = fast_exp2(gh) * scale;
             d.dk[lane] = fast_exp2((float)(end - G));
         }
         if (lane == 0) d.end = fast_exp2((float)end);
     };
+    const auto put_flows = [&](const typename S::Flows& f, int t0, int n) {   // wave 0
+        const int at = min(lane, L - 1);
+        double in = 0., out = 0.;
+        if (lane < n) {
+            in = NT == 4 ? (double)f.in[0][lane] : (double)f.in[0][lane] + f.in[1][lane];
+            out = NT == 4 ? (double)f.out[0][lane] : (double)f.out[0][lane] + f.out[1][lane];
+        }
+        const double inner = ((double)f.inner[0][at] + f.inner[1][at]) + ((double)f.inner[2][at] + f.inner[3][at]);
+        const double through = ((double)f.through[0] + f.through[1]) + ((double)f.through[2] + f.through[3]);
+        const double all = flow_sum(inner, in, out, lane) + through;
+        if (lane < n) dg[(long long)(t0 + lane) * H] = (float)all;
+    };
     if (nc > 0) {
-        fetch(nc - 1);
         if (wave == 0) put_decays(lds.d[0]);
+        hold();
     }
 
     for (int ci = 0; ci < nc; ++ci) {
+        // (what follows from the lane is worked out anew for each chunk: kept over the loop it fills the registers, masks for every tile among it)
+        int lane_ = lane;
+        asm volatile("" : "+v"(lane_));
+        const int quarter = lane_ >> 4, col = lane_ & 15;
         const int c = nc - 1 - ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
         // ---- operands to the LDS
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int row = row0 + 32 * i, o0 = order_of(d0), o1 = order_of(d0 + 4);
             u32x4 t[NS];
-            auto& qa = half ? lds.k : lds.q;
-            auto& qb = half ? lds.gy : lds.v;
+            auto& qa = group ? lds.k : lds.q;
+            auto& qb = group ? lds.gy : lds.v;
             piece_terms<IO>(ra[i], t);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -162,37 +203,23 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                 *reinterpret_cast<uint2*>(&qb[s][row][o1]) = uint2{t[s][2], t[s][3]};
             }
         }
-        if (group == 0) {
+#pragma unroll
+        for (int s = 0; s < 3; ++s)
 #pragma unroll
             for (int kx = 0; kx < 2; ++kx) {
-                const float x8[8] = {s0[2 * kx][0], s0[2 * kx][1], s0[2 * kx][2], s0[2 * kx][3], s0[2 * kx + 1][0], s0[2 * kx + 1][1], s0[2 * kx + 1][2], s0[2 * kx + 1][3]};
-                bf16x8 t[3];
-                split8<3>(x8, t);
-#pragma unroll
-                for (int s = 0; s < 3; ++s) lds.s[s][w4][kx][lane] = __builtin_bit_cast(u32x4, t[s]);
+                const u32x4 t = held[s][kx];
+                if (group == 0) lds.s[s][w4][kx][lane_] = t;
+                else {
+                    *reinterpret_cast<uint2*>(&lds.x[s][16 * w4 + col][32 * kx + 8 * quarter]) = uint2{t[0], t[1]};
+                    *reinterpret_cast<uint2*>(&lds.x[s][16 * w4 + col][32 * kx + 4 + 8 * quarter]) = uint2{t[2], t[3]};
+                }
             }
-            float cross = 0.f;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                unsigned t0_[3], t1_[3];
-                split_pair<3>(st[x][0], st[x][1], t0_);
-                split_pair<3>(st[x][2], st[x][3], t1_);
-                const int at = order_of(16 * x) + 8 * quarter;
-#pragma unroll
-                for (int s = 0; s < 3; ++s) *reinterpret_cast<uint2*>(&lds.x[s][zc][at]) = uint2{t0_[s], t1_[s]};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) cross = fmaf(st[x][i], s0[x][i], cross);
-            }
-            if constexpr (FLOW) {
-                cross = wave_sum(cross);
-                if (lane == 0) lds.cross[w4] = cross;
-            }
-        }
-        __syncthreads();
+        lds_barrier();                                    // (orders the LDS alone: the next chunk's rows and this one's results stay on their way)
         if (ci + 1 < nc) fetch(c - 1);
         typename S::Decays& dec = lds.d[ci & 1];
-        const int tw = w4 % NT, zt0 = w4 / NT * NT, r0 = 16 * tw + col;     // this lane's token
-        const auto rows_of = [&](const __bf16 (&a)[NS][L][PX], int row, int kx, bf16x8 (&f)[NS]) {
+        typename S::Flows& flows = lds.f[ci & 1];
+        const int r0 = 16 * tw + col;                     // this lane's token
+        const auto row_of = [&](const __bf16 (&a)[NS][L][PX], int row, int kx, bf16x8 (&f)[NS]) {
 #pragma unroll
             for (int s = 0; s < NS; ++s) f[s] = *reinterpret_cast<const bf16x8*>(&a[s][row][kx * 32 + 8 * quarter]);
         };
@@ -206,32 +233,36 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         };
         const auto widen4 = [&](const __bf16 (&a)[NS][L][PX], int row, int x, float (&o)[4]) {   // channels 16 x + 4 quarter + i
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                o[i] = 0.f;
+            for (int s = NS - 1; s >= 0; --s) {
+                const bf16x4 t = *reinterpret_cast<const bf16x4*>(&a[s][row][order_of(16 * x) + 8 * quarter]);
 #pragma unroll
-                for (int s = NS - 1; s >= 0; --s) o[i] += (float)a[s][row][order_of(16 * x) + 8 * quarter + i];
-            }
-        };
-        const auto store = [&](const OutView& v, int D, f32x4 (&acc)[NT]) {
-            if (!v.p) return;
-            const int e = v.f32 ? 4 : (int)sizeof(IO);
-            const auto buf = buffer_at(static_cast<char*>(v.p) + (w.base * v.sb + (long long)(w.first + t0) * v.st + h * v.sh) * e);
-            const int zl = 16 * zt0 + 4 * quarter, count = r0 < n ? D - zl : 0;
-            const unsigned at = (unsigned)(r0 * (int)v.st + zl);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                if (v.f32) store_quad<float, VEC>(buf, (at + 16 * j) * 4, count - 16 * j, acc[j]);
-                else store_quad<IO, VEC>(buf, (at + 16 * j) * (unsigned)sizeof(IO), count - 16 * j, acc[j]);
+                for (int i = 0; i < 4; ++i) o[i] = s == NS - 1 ? (float)t[i] : o[i] + (float)t[i];
             }
         };
         if (group == 0) {
+            if constexpr (FLOW) {                         // <S0, X>
+                float through = 0.f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int s = 0; s < 3; ++s) {
+                        const bf16x4 t = *reinterpret_cast<const bf16x4*>(&lds.x[s][16 * w4 + col][order_of(16 * x) + 8 * quarter]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) through = fmaf((float)t[i], st[x][i], through);
+                    }
+                through = wave_sum(through);
+                if (lane_ == 0) flows.through[w4] = through * dec.end;
+            }
+            if (ci + 1 < nc) fetch_state(c - 1);
             if (16 * tw < n) {
                 const float gh = dec.gh[r0], gl = dec.gl[r0], dt = dec.dt[r0];
                 bf16x8 fo[2][NS];
-                rows_of(lds.gy, r0, 0, fo[0]);
-                rows_of(lds.gy, r0, 1, fo[1]);
-                f32x4 acc[NT];
+                row_of(lds.gy, r0, 0, fo[0]);
+                row_of(lds.gy, r0, 1, fo[1]);
+                f32x4 acc[NT], flow[FLOW ? NT : 1];       // flow [tile of j]: sums over s < j of the terms of row t
                 float in = 0.f;
+#pragma unroll
+                for (int j = 0; j < (FLOW ? NT : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -239,10 +270,10 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                     for (int kx = 0; kx < 2; ++kx) {
                         bf16x8 fs[3];
 #pragma unroll
-                        for (int s = 0; s < 3; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane]);
+                        for (int s = 0; s < 3; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane_]);
                         acc[j] = mma<2>(acc[j], fs, fo[kx]);
                     }
-                    float q4[4] = {0.f, 0.f, 0.f, 0.f};
+                    float q4[4];
                     if constexpr (FLOW) widen4(lds.q, r0, zt0 + j, q4);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -253,27 +284,36 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     if (2 * ks > tw) break;
-                    float pr[8];
+                    float pr[8], pf[8];
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
                         const int ts = 2 * ks + hf;
-                        f32x4 m = {0.f, 0.f, 0.f, 0.f};
+                        f32x4 m = {0.f, 0.f, 0.f, 0.f}, mq = {0.f, 0.f, 0.f, 0.f};
                         if (ts <= tw) {
 #pragma unroll
                             for (int kx = 0; kx < 2; ++kx) {
-                                bf16x8 fv[NS];
-                                rows_of(lds.v, 16 * ts + col, kx, fv);
-                                m = mma<NP - 1>(m, fv, fo[kx]);
+                                bf16x8 f[NS];
+                                row_of(lds.v, 16 * ts + col, kx, f);
+                                m = mma<2>(m, f, fo[kx]);
+                                if (FLOW && w4 < NT) {
+                                    bf16x8 fq[NS];
+                                    row_of(lds.k, 16 * ts + col, kx, f);
+                                    row_of(lds.q, r0, kx, fq);
+                                    mq = mma<2>(mq, f, fq);
+                                }
                             }
                             const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec.gh[16 * ts + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * ts + 4 * quarter]);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float x = m[i] * (p.scale * fast_exp2((gh - sh[i]) + (gl - sl[i])));
+                                const float x = m[i] * (scale * fast_exp2((gh - sh[i]) + (gl - sl[i])));
                                 m[i] = ts < tw || 4 * quarter + i <= col ? x : 0.f;
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) pr[4 * hf + i] = m[i];
+                        for (int i = 0; i < 4; ++i) {
+                            pr[4 * hf + i] = m[i];
+                            pf[4 * hf + i] = m[i] * mq[i];
+                        }
                     }
                     bf16x8 fp[NP];
                     split8<NP>(pr, fp);
@@ -283,12 +323,139 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                         across(lds.k, zt0 + j, ks, fk);
                         acc[j] = mma<NP - 1>(acc[j], fk, fp);
                     }
+                    if (FLOW && w4 < NT) {                // (the other waves of a 32-token chunk would make the same terms)
+                        bf16x8 ff[3];
+                        split8<3>(pf, ff);
+#pragma unroll
+                        for (int j = 2 * ks; j < NT; ++j) {
+                            if (j > tw) break;
+                            // ones where s < j, row j of the tile in lane col: all of a tile in front of it, none of one behind it
+                            u32x4 ones;
+#pragma unroll
+                            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const unsigned lo = 4 * quarter + 2 * e < col ? 0x3f80u : 0u, hi = 4 * quarter + 2 * e + 1 < col ? 0x3f800000u : 0u;
+                                    ones[2 * hf + e] = 2 * ks + hf < j ? 0x3f803f80u : 2 * ks + hf == j ? lo | hi : 0u;
+                                }
+                            const bf16x8 fu[1] = {__builtin_bit_cast(bf16x8, ones)};
+                            flow[j] = mma<2>(flow[j], fu, ff);
+                        }
+                    }
                 }
-                store(p.dq, p.Dk, acc);
+                oa.store(acc, t0, r0 < n);
                 if constexpr (FLOW) {
                     in += __shfl_xor(in, 16);
                     in += __shfl_xor(in, 32);
-                    if (quarter == 0) lds.in[w4 / NT][r0] = in;
+                    if (quarter == 0) flows.in[w4 / NT][r0] = in;
+                    float crossing[16];                   // of rows t from j on
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) crossing[4 * j + i] = j < NT && (j < tw || (j == tw && 4 * quarter + i <= col)) ? flow[j < NT ? j : 0][i] : 0.f;
+                    int index;
+                    const float cf = wkv6_detail::row_sums16(crossing, lane_, index);
+                    if ((index >> 2) < NT) flows.inner[w4][16 * (index >> 2) + 4 * quarter + (index & 3)] = cf;
+                }
+            } else if (FLOW && lane_ < L) flows.inner[w4][lane_] = 0.f;
+            if (wave == 0) {
+                if constexpr (FLOW) {
+                    if (ci > 0) put_flows(lds.f[(ci + 1) & 1], t0 + L, min(L, w.s1 - t0 - L));
+                }
+                if (ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
+            }
+            if (ci + 1 < nc) hold();
+        } else {
+            if (16 * tw < n) {
+                const float gh = dec.gh[r0], gl = dec.gl[r0], dk = dec.dk[r0];
+                bf16x8 fk[2][NS], fv[2][NS];
+#pragma unroll
+                for (int kx = 0; kx < 2; ++kx) {
+                    row_of(lds.k, r0, kx, fk[kx]);
+                    row_of(lds.v, r0, kx, fv[kx]);
+                }
+                f32x4 ak[NT], av[NT];
+                float out = 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) ak[j] = av[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (have) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const int x = zt0 + j;
+#pragma unroll
+                        for (int kx = 0; kx < 2; ++kx) {
+                            bf16x8 fx[3], fy[NP];
+#pragma unroll
+                            for (int s = 0; s < 3; ++s) fx[s] = *reinterpret_cast<const bf16x8*>(&lds.x[s][16 * x + col][kx * 32 + 8 * quarter]);
+#pragma unroll
+                            for (int s = 0; s < NP; ++s) {
+                                const __bf16* q = &lds.x[s][32 * kx + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
+                                fy[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
+                            }
+                            ak[j] = mma<2>(ak[j], fx, fv[kx]);
+                            av[j] = mma<NP - 1>(av[j], fy, fk[kx]);
+                        }
+                        float k4[4];
+                        if constexpr (FLOW) widen4(lds.k, r0, x, k4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            ak[j][i] *= dk;
+                            av[j][i] *= dk;
+                            if constexpr (FLOW) out = fmaf(k4[i], ak[j][i], out);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (2 * ks + 1 < tw) continue;        // tokens t in front of s
+                    if (32 * ks >= n) break;
+                    float pp[8], dp[8];
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const int tt = 2 * ks + hf;
+                        f32x4 mq = {0.f, 0.f, 0.f, 0.f}, mo = {0.f, 0.f, 0.f, 0.f};
+                        if (tt >= tw) {
+#pragma unroll
+                            for (int kx = 0; kx < 2; ++kx) {
+                                bf16x8 f[NS];
+                                row_of(lds.q, 16 * tt + col, kx, f);
+                                mq = mma<NP - 1>(mq, f, fk[kx]);
+                                row_of(lds.gy, 16 * tt + col, kx, f);
+                                mo = mma<NP - 1>(mo, f, fv[kx]);
+                            }
+                            const f32x4 th = *reinterpret_cast<const f32x4*>(&dec.gh[16 * tt + 4 * quarter]), tl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * tt + 4 * quarter]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float x = scale * fast_exp2((th[i] - gh) + (tl[i] - gl));
+                                const bool seen = tt > tw || 4 * quarter + i >= col;
+                                mq[i] = seen ? mq[i] * x : 0.f;
+                                mo[i] = seen ? mo[i] * x : 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            pp[4 * hf + i] = mq[i];
+                            dp[4 * hf + i] = mo[i];
+                        }
+                    }
+                    bf16x8 fp[NP], fd[NP];
+                    split8<NP>(pp, fp);
+                    split8<NP>(dp, fd);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        bf16x8 f[NS];
+                        across(lds.gy, zt0 + j, ks, f);
+                        av[j] = mma<NP - 1>(av[j], f, fp);
+                        across(lds.q, zt0 + j, ks, f);
+                        ak[j] = mma<NP - 1>(ak[j], f, fd);
+                    }
+                }
+                oa.store(ak, t0, r0 < n);
+                ob.store(av, t0, r0 < n);
+                if constexpr (FLOW) {
+                    out += __shfl_xor(out, 16);
+                    out += __shfl_xor(out, 32);
+                    if (quarter == 0) flows.out[w4 / NT][r0] = out;
                 }
             }
             // ---- X in front of the chunk
@@ -306,9 +473,9 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                 float x8[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    x8[i] = 0.f;
+                    x8[i] = (float)fq[NS - 1][i];
 #pragma unroll
-                    for (int s = NS - 1; s >= 0; --s) x8[i] += (float)fq[s][i];
+                    for (int s = NS - 2; s >= 0; --s) x8[i] += (float)fq[s][i];
                     x8[i] *= i < 4 ? a0[i & 3] : a1[i & 3];
                 }
                 bf16x8 fd[3];
@@ -321,152 +488,15 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                 }
             }
             have = true;
-            if (wave == 0 && ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
-        } else if (16 * tw < n) {
-            const float gh = dec.gh[r0], gl = dec.gl[r0], dk = dec.dk[r0];
-            bf16x8 fk[2][NS], fv[2][NS];
-#pragma unroll
-            for (int kx = 0; kx < 2; ++kx) {
-                rows_of(lds.k, r0, kx, fk[kx]);
-                rows_of(lds.v, r0, kx, fv[kx]);
-            }
-            f32x4 ak[NT], av[NT], flow[FLOW ? 4 : 1];
-            float out = 0.f;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) ak[j] = av[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < (FLOW ? 4 : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (have) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const int x = zt0 + j;
-#pragma unroll
-                    for (int kx = 0; kx < 2; ++kx) {
-                        bf16x8 fx[3], fy[3];
-#pragma unroll
-                        for (int s = 0; s < 3; ++s) {
-                            fx[s] = *reinterpret_cast<const bf16x8*>(&lds.x[s][16 * x + col][kx * 32 + 8 * quarter]);
-                            const __bf16* q = &lds.x[s][32 * kx + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
-                            fy[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
-                        }
-                        ak[j] = mma<2>(ak[j], fx, fv[kx]);
-                        av[j] = mma<NP - 1>(av[j], fy, fk[kx]);
-                    }
-                    float k4[4] = {0.f, 0.f, 0.f, 0.f};
-                    if constexpr (FLOW) widen4(lds.k, r0, x, k4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        ak[j][i] *= dk;
-                        av[j][i] *= dk;
-                        if constexpr (FLOW) out = fmaf(k4[i], ak[j][i], out);
-                    }
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (2 * ks + 1 < tw) continue;            // tokens t in front of s
-                if (32 * ks >= n) break;
-                float pp[8], dp[8], pf[8];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int tt = 2 * ks + hf;
-                    f32x4 mq = {0.f, 0.f, 0.f, 0.f}, mo = {0.f, 0.f, 0.f, 0.f};
-                    if (tt >= tw) {
-#pragma unroll
-                        for (int kx = 0; kx < 2; ++kx) {
-                            bf16x8 f[NS];
-                            rows_of(lds.q, 16 * tt + col, kx, f);
-                            mq = mma<FLOW ? 2 : NP - 1>(mq, f, fk[kx]);
-                            rows_of(lds.gy, 16 * tt + col, kx, f);
-                            mo = mma<FLOW ? 2 : NP - 1>(mo, f, fv[kx]);
-                        }
-                        const f32x4 th = *reinterpret_cast<const f32x4*>(&dec.gh[16 * tt + 4 * quarter]), tl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * tt + 4 * quarter]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = p.scale * fast_exp2((th[i] - gh) + (tl[i] - gl));
-                            const bool seen = tt > tw || 4 * quarter + i >= col;
-                            const float y = seen ? mq[i] * x : 0.f;
-                            if constexpr (FLOW) pf[4 * hf + i] = y * mo[i];
-                            mo[i] = seen ? mo[i] * x : 0.f;
-                            mq[i] = y;
-                        }
-                    } else if constexpr (FLOW) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) pf[4 * hf + i] = 0.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        pp[4 * hf + i] = mq[i];
-                        dp[4 * hf + i] = mo[i];
-                    }
-                }
-                bf16x8 fp[NP], fd[NP];
-                split8<NP>(pp, fp);
-                split8<NP>(dp, fd);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    bf16x8 f[NS];
-                    across(lds.gy, zt0 + j, ks, f);
-                    av[j] = mma<NP - 1>(av[j], f, fp);
-                    across(lds.q, zt0 + j, ks, f);
-                    ak[j] = mma<NP - 1>(ak[j], f, fd);
-                }
-                if constexpr (FLOW) {
-                    bf16x8 ff[3];
-                    split8<3>(pf, ff);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (j < tw || j > 2 * ks + 1) continue;
-                        // ones where j <= t, row j of the tile in lane col: all of a tile behind it, none of one in front of it
-                        u32x4 ones;
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const unsigned lo = 4 * quarter + 2 * e >= col ? 0x3f80u : 0u, hi = 4 * quarter + 2 * e + 1 >= col ? 0x3f800000u : 0u;
-                                ones[2 * hf + e] = 2 * ks + hf > j ? 0x3f803f80u : 2 * ks + hf == j ? lo | hi : 0u;
-                            }
-                        const bf16x8 fu[1] = {__builtin_bit_cast(bf16x8, ones)};
-                        flow[j] = mma<2>(flow[j], fu, ff);
-                    }
-                }
-            }
-            store(p.dk, p.Dk, ak);
-            store(p.dv, p.Dv, av);
-            if constexpr (FLOW) {
-                out += __shfl_xor(out, 16);
-                out += __shfl_xor(out, 32);
-                if (quarter == 0) lds.out[w4 / NT][r0] = out;
-                float crossing[16];                       // of rows s in front of j
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) crossing[4 * j + i] = j < NT && (j > tw || (j == tw && 4 * quarter + i > col)) ? flow[j][i] : 0.f;
-                int index;
-                const float cf = wkv6_detail::row_sums16(crossing, lane, index);
-                // (the other waves of a 32-token chunk have made the same terms)
-                if ((index >> 2) < NT) lds.inner[w4][16 * (index >> 2) + 4 * quarter + (index & 3)] = w4 < NT ? cf : 0.f;
-            }
-        } else if (FLOW && lane < L) lds.inner[w4][lane] = 0.f;
-        if (group == 1) have = true;
-        __syncthreads();
-        if constexpr (FLOW) {
-            if (wave == 0) {
-                const int at = min(lane, L - 1);
-                double in = 0., out = 0.;
-                if (lane < n) {
-                    in = NT == 4 ? (double)lds.in[0][lane] : (double)lds.in[0][lane] + lds.in[1][lane];
-                    out = NT == 4 ? (double)lds.out[0][lane] : (double)lds.out[0][lane] + lds.out[1][lane];
-                }
-                const double inner = ((double)lds.inner[0][at] + lds.inner[1][at]) + ((double)lds.inner[2][at] + lds.inner[3][at]);
-                const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * dec.end;
-                const double all = flow_sum(inner, in, out, lane) + through;
-                if (lane < n) p.dg[((long long)w.base * p.T + w.first + t0 + lane) * p.H + h] = (float)all;
-            }
+            if (ci + 1 < nc) hold();
         }
+        lds_barrier();
+    }
+    if constexpr (FLOW) {
+        if (wave == 0 && nc > 0) put_flows(lds.f[(nc + 1) & 1], w.s0, min(L, w.s1 - w.s0));
     }
 
-    if (p.dstate && w.is_first && group == 0) {
+    if (p.dstate && w.is_first && group == 1) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll

@@ -316,7 +316,7 @@ bool rows_fit(const at::Tensor& t, int lead) { return t.dim() == lead + 2 && t.n
 // q, k, v, g as decay_attention and its step take them, nothing empty, nothing to convert
 bool decay_inputs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, int lead) {
     if (!rows_fit(q, lead) || !rows_fit(k, lead) || !rows_fit(v, lead) || code(q.scalar_type()) < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type() ||
-        (g.scalar_type() != q.scalar_type() && g.scalar_type() != at::kFloat) || (g.dim() != 1 && g.dim() != lead + 1) || g.numel() == 0)
+        (g.scalar_type() != q.scalar_type() && g.scalar_type() != at::kFloat) || (g.dim() != 1 && g.dim() != lead + 1) || g.numel() == 0 || (g.dim() == 3 && g.stride(1) >= (1 << 22)))
         return false;
     for (int i = 0; i < lead; ++i)
         if (k.size(i) != q.size(i) || v.size(i) != q.size(i) || q.size(i) > INT_MAX || (g.dim() > 1 && g.size(i) != q.size(i))) return false;

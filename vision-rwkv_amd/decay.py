@@ -84,6 +84,7 @@ class DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, state, offsets, scale, N, H, keep_state):
         q, k, v = _rows(q), _rows(k), _rows(v)
+        g = g if g.dim() == 1 or g.stride(1) < 1 << 22 else g.contiguous()
         state = state.contiguous() if state is not None else None
         ctx.save_for_backward(q, k, v, g, state, offsets)
         ctx.meta = scale, N, H
