@@ -2,14 +2,8 @@
 //     S_t = exp(g_t) S_{t-1} + k_t v_t^T,      y_t = scale S_t^T q_t.
 // A sequence goes in chunks of L tokens.  With G_t = the sum of g over the chunk's tokens up to t and S0 the state in front of the chunk,
 //     y_t = scale sum_{s<=t} exp(G_t - G_s) (q_t . k_s) v_s + scale exp(G_t) S0^T q_t,      S = exp(G_end) S0 + sum_s exp(G_end - G_s) k_s v_s^T,
-// four matrix products.  With a at the place of q, b of k and c of v this one kernel computes
-//     y  from a, b, c = q, k, v                       dq from gy, v, k            (along the tokens)
-//     dv from a, b, c = k, q, gy                      dk from v, gy, q            (back along them; a token's own decay then lies behind it),
-// since R_t = scale q_t gy_t^T + exp(g_{t+1}) R_{t+1} is a state of the same kind, dq_t = scale S_t gy_t, dk_t = R_t v_t, dv_t = R_t^T k_t.
-// The gradient of g_j is what crosses from tokens in front of j to j and behind: the sum over s < j <= t of the products' terms.  Inside a chunk those
-// are summed as they are, by one more product with a triangle of ones; what enters or leaves the chunk comes from S0's part of dq and R's part of dk; what
-// passes it whole is exp(G_end) <S0, R behind the chunk>, R kept for every chunk by the pass that makes dk.  Nothing cancels: q . dq - k . dk summed over the
-// tokens from j on is the same sum, with the difference of two large ones where little crosses.
+// four matrix products.  The state in front of each chunk, and the same sum back along the tokens (b, c = gy, q in the places of k, v: the gradient of a
+// state), which the gradients want (decay_bwd.h), are this kernel's without its outputs.
 // Sequences of few calls are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
 #pragma once
 #include "wave_sum.h"
@@ -38,16 +32,14 @@ struct OutView {
     int f32;                                              // fp32 values of every head, added up and rounded by a kernel behind
 };
 struct Role {
-    View a, b, c, e;
+    View a, b, c;                                         // q, k, v
     OutView o;
     const float* init;                                    // states (N, H, Dk, Dv), or null: zeros
     float* last;                                          // where the states behind the last token go, or null
     float *seg, *seg_decay;                               // [segment][head][tile] a segment's state (first its own, then that in front of it), [segment][head]
-    float* edge;                                          // [tile][row][head]: what a token gives to the tokens outside its chunk (written with dk, read with dq)
-    float* anchors;                                       // [chunk][head][tile]: R behind each chunk, without the decay of the token behind it; or S in front of it
-    float* dg;                                            // [tile][row][head]
+    float* anchors;                                       // [chunk][head][tile]: the state in front of each chunk
     long long sx, sz;                                     // strides of the states' contracted and other index
-    int dx, dz, tiles, reverse;
+    int dx, dz, tiles, reverse;                           // (the roles of a launch have the same tiles)
     float s_in, s_upd;                                    // scale where the state is read; where it is written
 };
 struct Call {                                             // sequences, their cut, and the decays
@@ -60,16 +52,15 @@ struct Call {                                             // sequences, their cu
 };
 struct Params : Call {
     int n_roles;
-    Role role[3];
+    Role role[2];
 };
 template <typename IO> constexpr int in_terms = std::is_same<IO, float>::value ? 3 : std::is_same<IO, __half>::value ? 2 : 1;   // bf16 numbers that hold an element
 
-// y and dv; dk with what dg needs of it; dq with dg; no outputs: a segment's own state; dk or dq without dg, the same bits as with it; no outputs: the state
-// in front of each chunk (for decay_bwd.h)
-enum Mode { PLAIN = 0, EDGES = 1, FLOWS = 2, STATES = 3, ALONE = 4, CHUNKS = 5 };
+// outputs; no outputs: a segment's own state; no outputs: the state in front of each chunk
+enum Mode { PLAIN = 0, STATES = 1, CHUNKS = 2 };
 // tokens of a chunk: 64 where two workgroups' rows and states fit the LDS of a compute unit (fp32 rows take three times the room of bf16 ones, fp16 rows twice)
 template <typename IO, int DX, int MODE>
-constexpr int chunk_len = std::is_same<IO, __hip_bfloat16>::value || (std::is_same<IO, __half>::value && DX == 64 && (MODE == PLAIN || MODE == STATES || MODE == CHUNKS)) ? 64 : 32;
+constexpr int chunk_len = std::is_same<IO, __hip_bfloat16>::value || (std::is_same<IO, __half>::value && (DX == 64 || MODE != PLAIN)) ? 64 : 32;
 
 struct Place {                                            // a workgroup's segment
     int n, first, len;                                    // sequence; its first token and length
@@ -354,20 +345,17 @@ __device__ __forceinline__ double flow_sum(double inner, double in, double out, 
 template <typename IO, int DX, int MODE>
 struct Lds {
     static constexpr int L = chunk_len<IO, DX, MODE>, NS = in_terms<IO>;
-    // terms of the products' intermediate operands: 16 bits of them for a 16-bit result, all 24 where fp32 ones depend on them: those of fp32 rows, and dg
-    static constexpr int NP = NS < 3 ? 2 : 3, NI = MODE == PLAIN ? NP : 3;
+    static constexpr int NP = NS < 3 ? 2 : 3;             // terms of the products' intermediate operands: 16 bits of them for a 16-bit result, all 24 for an fp32 one
     static constexpr int PX = DX + 8, PZ = TZ + 8;        // row pitches: 16 rows of a fragment on different banks
-    static constexpr bool OUT = MODE != STATES && MODE != CHUNKS;
+    static constexpr bool OUT = MODE == PLAIN;
     __bf16 a[OUT ? NS : 1][OUT ? L : 1][PX];   // channels in the order of the state's fragments
     __bf16 b[NS][L][PX];
     __bf16 c[NS][L][PZ];
-    __bf16 e[MODE == EDGES || MODE == FLOWS ? NS : 1][MODE == EDGES || MODE == FLOWS ? L : 1][PZ];
-    u32x4 s[OUT ? NI : 1][4][OUT ? DX / 32 : 1][64];   // the state's terms, a lane's fragment side by side
+    u32x4 s[OUT ? NP : 1][4][OUT ? DX / 32 : 1][64];   // the state's terms, a lane's fragment side by side
     struct Decays {
         float gh[L], gl[L], dt[L], dk[L];                 // G in powers of two, head and tail; exp(G); exp(G_end - G)
-        float end, through;                               // exp(G_end); FLOWS: with the decay of the token behind the chunk
+        float end;                                        // exp(G_end)
     } d[2];                                               // this chunk's and the next one's
-    float edge[2][L], inner[4][L], cross[4];            // what rows get or give across the chunk's ends, by halves of the columns; what crosses tokens inside, by waves; <S0, R>
 };
 
 // Eight channels from d on in the order that the accumulators' fragments have: inside 32 channels, 4 m .. 4 m + 3 lie at 8 (m & 3) + 4 (m >> 2).
@@ -377,7 +365,7 @@ __device__ __forceinline__ int order_of(int d) {
 }
 
 // Packed rows in front of the first sequence and behind the last get zeros, a few from every workgroup of the head and tile.
-template <typename IO, int MODE>
+template <typename IO>
 __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, int gid, int z, int h) {
     const int front = offset_at(p, 0), back = offset_at(p, p.N), rows = front + max(0, p.T - back);
     const int d = z * TZ + (threadIdx.x & 63);
@@ -388,7 +376,6 @@ __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, in
             if (r.o.f32) static_cast<float*>(r.o.p)[at] = 0.f;
             else static_cast<IO*>(r.o.p)[at] = from_f32<IO>(0.f);
         }
-        if (MODE == FLOWS && (threadIdx.x & 63) == 0) r.dg[((long long)z * p.rows + row) * p.H + h] = 0.f;
     }
 }
 
@@ -398,10 +385,10 @@ template <size_t BYTES> constexpr int workgroups = 3 * BYTES <= 160 * 1024 ? 3 :
 template <typename IO, int DX, int MODE, bool VEC>
 __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) void decay_kernel(const Params p) {
     using S = Lds<IO, DX, MODE>;
-    constexpr int L = S::L, NS = S::NS, NI = S::NI, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
+    constexpr int L = S::L, NS = S::NS, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
     constexpr int PA = L * DX / 8 / THREADS, PC = (L * TZ / 8 + THREADS - 1) / THREADS;
     static_assert(PA >= 1 && L * DX % (8 * THREADS) == 0 && L * TZ % (8 * THREADS) == 0, "");
-    constexpr bool OUT = S::OUT, EXTRA = MODE == EDGES || MODE == FLOWS;
+    constexpr bool OUT = S::OUT;
     __shared__ S lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
 
@@ -410,41 +397,36 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     const int ri = id % p.n_roles;
     id /= p.n_roles;
     const Role& r = p.role[ri];
-    int tiles = 1;
-    for (int i = 0; i < p.n_roles; ++i) tiles = max(tiles, p.role[i].tiles);
-    const int z = id % tiles;
-    id /= tiles;
+    const int z = id % r.tiles;
+    id /= r.tiles;
     const int h = id % p.H, gid = id / p.H;
-    if (!p.nseg && OUT && z < r.tiles) clear_outside<IO, MODE>(p, r, gid, z, h);
+    if (!p.nseg && OUT) clear_outside<IO>(p, r, gid, z, h);
     const Place w = find_place<THREADS>(p, gid, L);
-    if (!w.valid || z >= r.tiles) return;
+    if (!w.valid) return;
     if (MODE == STATES && (r.reverse ? w.is_first : w.is_last)) return;    // nothing starts behind it
     const int z0 = z * TZ;
-    const bool rev = r.reverse;
+    const bool rev = MODE == STATES && r.reverse;
 
     const int nc = (w.s1 - w.s0 + L - 1) / L;
     const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, rowz = tid / (TZ / 8), dzo = tid % (TZ / 8) * 8;
     constexpr int STEPX = THREADS / (DX / 8), STEPZ = THREADS / (TZ / 8);   // rows between a thread's pieces
     Source<IO, PA, STEPX, VEC> sa, sb;
-    Source<IO, PC, STEPZ, VEC> sc, se;
+    Source<IO, PC, STEPZ, VEC> sc;
     Gates gates;
     gates.open(p, w.base, w.first, h);
     if constexpr (OUT) sa.open(r.a, w.base, w.first, h, L, rev, rowx, dxo, r.dx);
     sb.open(r.b, w.base, w.first, h, L, rev, rowx, dxo, r.dx);
     sc.open(r.c, w.base, w.first, h, L, rev, rowz, z0 + dzo, r.dz);
-    if constexpr (EXTRA) se.open(r.e, w.base, w.first, h, L, rev, rowz, z0 + dzo, r.dz);
-    Piece<IO> ra[PA], rb[PA], rc[PC], re[PC];
-    Gates::Raw rg{}, rg_next{};
+    Piece<IO> ra[PA], rb[PA], rc[PC];
+    Gates::Raw rg{};
     const auto fetch = [&](int c) {
         const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0), token = rev ? t0 + n - L : t0;
         if constexpr (OUT) sa.load(ra, token, n, rev);
         sb.load(rb, token, n, rev);
         sc.load(rc, token, n, rev);
-        if constexpr (EXTRA) se.load(re, token, n, rev);
         if (wave == 0) {
             // back along the tokens a row's decay is that of the token behind it, and none behind the last
             rg = rev ? gates.fetch(t0 + n - 63, 63 - lane, lane < n && t0 + n - lane < w.len) : gates.fetch(t0, lane, lane < n);
-            if constexpr (MODE == FLOWS) rg_next = gates.fetch(t0 + n, 0, t0 + n < w.len);
         }
     };
     if (nc > 0) fetch(rev ? nc - 1 : 0);
@@ -474,11 +456,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         const int t = 16 * (wave % NT) + col;
         so.open(r.o, w.base, w.first, h, rev ? L - 1 - t : t, z0 + 16 * (wave / NT * NT) + 4 * quarter, r.dz);
     }
-    const float *anchors = nullptr, *edges = nullptr;     // of the segment's first chunk and token
-    if constexpr (MODE == EDGES || MODE == FLOWS || MODE == CHUNKS) {
-        anchors = r.anchors + (((long long)(w.chunk0 + w.s0 / L) * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4;
-        if (MODE != CHUNKS) edges = r.edge + ((long long)z * p.rows + (long long)w.base * p.T + w.first) * p.H + h;
-    }
+    float* const anchors = MODE == CHUNKS ? r.anchors + (((long long)(w.chunk0 + w.s0 / L) * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4 : nullptr;
     const long long anchor_step = (long long)p.H * r.tiles * (DX * TZ);
     float scale = p.scale, s_in = r.s_in, s_upd = r.s_upd;
     keep(scale);
@@ -497,10 +475,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
             d.dt[lane] = fast_exp2(gh);
             d.dk[lane] = fast_exp2((float)(end - G));
         }
-        if (lane == 0) {
-            d.end = fast_exp2((float)end);
-            if constexpr (MODE == FLOWS) d.through = fast_exp2((float)(end + (double)gates.widen(rg_next) * 1.4426950408889634));
-        }
+        if (lane == 0) d.end = fast_exp2((float)end);
         if (MODE == STATES) seg_log += (float)end;
     };
     if (nc > 0 && wave == 0) put_decays(lds.d[0]);
@@ -537,21 +512,16 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
             piece_terms<IO>(rc[i], t);
 #pragma unroll
             for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.c[s][row][d]) = t[s];
-            if constexpr (EXTRA) {
-                piece_terms<IO>(re[i], t);
-#pragma unroll
-                for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.e[s][row][d]) = t[s];
-            }
         }
         if constexpr (OUT) {
             if (have) {
 #pragma unroll
                 for (int kx = 0; kx < KX; ++kx) {
                     const float x8[8] = {st[2 * kx][0], st[2 * kx][1], st[2 * kx][2], st[2 * kx][3], st[2 * kx + 1][0], st[2 * kx + 1][1], st[2 * kx + 1][2], st[2 * kx + 1][3]};
-                    bf16x8 t[NI];
-                    split8<NI>(x8, t);
+                    bf16x8 t[NP];
+                    split8<NP>(x8, t);
 #pragma unroll
-                    for (int s = 0; s < NI; ++s) lds.s[s][wave][kx][lane] = __builtin_bit_cast(u32x4, t[s]);
+                    for (int s = 0; s < NP; ++s) lds.s[s][wave][kx][lane] = __builtin_bit_cast(u32x4, t[s]);
                 }
             }
         }
@@ -560,13 +530,6 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         typename S::Decays& dec_ = lds.d[ci & 1];
 
         // ---- outputs of rows 16 tw + col, columns 16 zt + 4 quarter + i
-        f32x4 behind[MODE == FLOWS ? NX : 1];              // R behind this chunk, as the pass of dk left it
-        float given = 0.f;                                // (wave 0) what its tokens give over its end
-        if constexpr (MODE == FLOWS) {
-#pragma unroll
-            for (int x = 0; x < NX; ++x) behind[x] = *reinterpret_cast<const f32x4*>(anchors + c * anchor_step + x * 1024);
-            if (wave == 0 && lane < n) given = edges[(long long)(t0 + lane) * p.H];
-        }
         const int tw = wave % NT, zt0 = wave / NT * NT, t = 16 * tw + col;
         if (OUT && 16 * tw < n) {
             const float gth = dec_.gh[t], gtl = dec_.gl[t], dec = dec_.dt[t] * s_in;
@@ -579,36 +542,24 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
             f32x4 acc[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            float edge = 0.f;
             if (have) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
 #pragma unroll
                     for (int kx = 0; kx < KX; ++kx) {
-                        bf16x8 fs[NI];
+                        bf16x8 fs[NP];
 #pragma unroll
-                        for (int s = 0; s < NI; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[OUT ? s : 0][zt0 + j][OUT ? kx : 0][lane]);
-                        acc[j] = mma<NI - 1>(acc[j], fs, fa[kx]);
+                        for (int s = 0; s < NP; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[OUT ? s : 0][zt0 + j][OUT ? kx : 0][lane]);
+                        acc[j] = mma<NP - 1>(acc[j], fs, fa[kx]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        acc[j][i] *= dec;
-                        if constexpr (EXTRA) {
-                            float x = 0.f;
-#pragma unroll
-                            for (int s = NS - 1; s >= 0; --s) x += (float)lds.e[s][t][16 * (zt0 + j) + 4 * quarter + i];
-                            edge = fmaf(x, acc[j][i], edge);
-                        }
-                    }
+                    for (int i = 0; i < 4; ++i) acc[j][i] *= dec;
                 }
             }
-            f32x4 flow[MODE == FLOWS ? NT : 1];            // [tile of j]: sums over s < j of the terms of row t
-#pragma unroll
-            for (int j = 0; j < (MODE == FLOWS ? NT : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (2 * ks > tw) break;
-                float pr[8], pf[8];
+                float pr[8];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int st_ = 2 * ks + half;        // tile of 16 tokens s
@@ -619,7 +570,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                             bf16x8 fb[NS];
 #pragma unroll
                             for (int s = 0; s < NS; ++s) fb[s] = *reinterpret_cast<const bf16x8*>(&lds.b[s][16 * st_ + col][kx * 32 + 8 * quarter]);
-                            m = mma<NI - 1>(m, fb, fa[kx]);
+                            m = mma<NP - 1>(m, fb, fa[kx]);
                         }
                         const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec_.gh[16 * st_ + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec_.gl[16 * st_ + 4 * quarter]);
 #pragma unroll
@@ -627,46 +578,9 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                             const float x = m[i] * (scale * fast_exp2((gth - sh[i]) + (gtl - sl[i])));
                             m[i] = st_ < tw || 4 * quarter + i <= col ? x : 0.f;
                         }
-                        if constexpr (MODE == FLOWS) {
-                            f32x4 qk = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int kz = 0; kz < TZ / 32; ++kz) {
-                                bf16x8 fk[NS], fq[NS];
-#pragma unroll
-                                for (int s = 0; s < NS; ++s) {
-                                    fk[s] = *reinterpret_cast<const bf16x8*>(&lds.c[s][16 * st_ + col][kz * 32 + 8 * quarter]);
-                                    fq[s] = *reinterpret_cast<const bf16x8*>(&lds.e[s][t][kz * 32 + 8 * quarter]);
-                                }
-                                qk = mma<2>(qk, fk, fq);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) pf[4 * half + i] = m[i] * qk[i];
-                        }
-                    } else if constexpr (MODE == FLOWS) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) pf[4 * half + i] = 0.f;
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) pr[4 * half + i] = m[i];
-                }
-                if constexpr (MODE == FLOWS) {
-                    bf16x8 ff[3];
-                    split8<3>(pf, ff);
-#pragma unroll
-                    for (int j = 2 * ks; j < NT; ++j) {
-                        if (j > tw) break;
-                        // ones where s < j, row j of the tile in lane col: all of a tile in front of it, none of one behind it
-                        u32x4 ones;
-#pragma unroll
-                        for (int half = 0; half < 2; ++half)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const unsigned lo = 4 * quarter + 2 * e < col ? 0x3f80u : 0u, hi = 4 * quarter + 2 * e + 1 < col ? 0x3f800000u : 0u;
-                                ones[2 * half + e] = 2 * ks + half < j ? 0x3f803f80u : 2 * ks + half == j ? lo | hi : 0u;
-                            }
-                        const bf16x8 fu[1] = {__builtin_bit_cast(bf16x8, ones)};
-                        flow[j] = mma<2>(flow[j], fu, ff);
-                    }
                 }
                 bf16x8 fp[NP];
                 split8<NP>(pr, fp);
@@ -682,38 +596,13 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                 }
             }
             so.store(acc, rev ? t0 + n - L : t0, t < n);
-            if constexpr (EXTRA) {                        // over the quarters: the channels of a row
-                edge += __shfl_xor(edge, 16);
-                edge += __shfl_xor(edge, 32);
-                if (quarter == 0) lds.edge[wave / NT][t] = edge;    // (two waves share a row where the chunk has 32 tokens)
-            }
-            if constexpr (MODE == FLOWS) {
-                float crossing[16];                       // of rows t from j on
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) crossing[4 * j + i] = j < NT && (j < tw || (j == tw && 4 * quarter + i <= col)) ? flow[j < NT ? j : 0][i] : 0.f;
-                int index;
-                const float cf = wkv6_detail::row_sums16(crossing, lane, index);
-                // (the other waves of a 32-token chunk have made the same terms)
-                if ((index >> 2) < NT) lds.inner[wave][16 * (index >> 2) + 4 * quarter + (index & 3)] = wave < NT ? cf : 0.f;
-            }
-        } else if (MODE == FLOWS && lane < L) lds.inner[wave][lane] = 0.f;
-        if constexpr (MODE == FLOWS) {
-            float x = 0.f;                                // <S0, R>
-#pragma unroll
-            for (int x4 = 0; x4 < NX; ++x4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x = fmaf(st[x4][i], behind[x4][i], x);
-            x = wave_sum(x);
-            if (lane == 0) lds.cross[wave] = x;
         }
 
         // ---- the state behind the chunk
         {
-            if constexpr (MODE == EDGES || MODE == CHUNKS) {
+            if constexpr (MODE == CHUNKS) {
 #pragma unroll
-                for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(const_cast<float*>(anchors) + c * anchor_step + x * 1024) = st[x];
+                for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(anchors + c * anchor_step + x * 1024) = st[x];
             }
             if (MODE == CHUNKS && ci + 1 == nc) break;     // (nothing starts behind it)
             const float ed = dec_.end;
@@ -757,28 +646,6 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         }
         if (wave == 0 && ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
         lds_barrier();
-        if constexpr (MODE == EDGES) {
-            if (wave == 0 && lane < n) {
-                const float x = NT == 4 ? lds.edge[0][lane] : lds.edge[0][lane] + lds.edge[1][lane];
-                const_cast<float*>(edges)[(long long)(t0 + n - 1 - lane) * p.H] = x;
-            }
-        }
-        if constexpr (MODE == FLOWS) {
-            if (wave == 0) {
-                const long long row = (long long)w.base * p.T + w.first + t0 + lane;
-                const long long at = ((long long)z * p.rows + row) * p.H + h;
-                // what token `lane` receives over the chunk's front and gives over its end; summed from it on, and up to it
-                double in = 0., out = 0.;
-                if (lane < n) {
-                    in = NT == 4 ? (double)lds.edge[0][lane] : (double)lds.edge[0][lane] + lds.edge[1][lane];
-                    out = given;
-                }
-                const int at_lane = min(lane, L - 1);
-                const double inner = ((double)lds.inner[0][at_lane] + lds.inner[1][at_lane]) + ((double)lds.inner[2][at_lane] + lds.inner[3][at_lane]);
-                const double through = (((double)lds.cross[0] + lds.cross[1]) + ((double)lds.cross[2] + lds.cross[3])) * dec_.through;
-                if (lane < n) r.dg[at] = (float)(flow_sum(inner, in, out, lane) + through);
-            }
-        }
     }
 
     // ---- the state behind the segment
@@ -810,20 +677,13 @@ template <typename IO, int DX, bool VEC>
 void launch_mode(const Params& p, int mode, dim3 grid, hipStream_t st) {
     const dim3 block(THREADS);
     if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, DX, PLAIN, VEC>), grid, block, 0, st, p);
-    else if (mode == EDGES) hipLaunchKernelGGL((decay_kernel<IO, DX, EDGES, VEC>), grid, block, 0, st, p);
-    else if (mode == FLOWS) hipLaunchKernelGGL((decay_kernel<IO, DX, FLOWS, VEC>), grid, block, 0, st, p);
-    else if (mode == ALONE) hipLaunchKernelGGL((decay_kernel<IO, DX, ALONE, VEC>), grid, block, 0, st, p);
-    else if (mode == CHUNKS) {
-        if constexpr (DX == 64) hipLaunchKernelGGL((decay_kernel<IO, 64, CHUNKS, VEC>), grid, block, 0, st, p);
-    }
+    else if (mode == CHUNKS) hipLaunchKernelGGL((decay_kernel<IO, DX, CHUNKS, VEC>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((decay_kernel<IO, DX, STATES, VEC>), grid, block, 0, st, p);
 }
 // vec: every row of every role in pieces of 16 bytes
 template <typename IO>
 int launch_decay(const Params& p, int dx, int mode, bool vec, hipStream_t st) {
-    int tiles = 1;
-    for (int i = 0; i < p.n_roles; ++i) tiles = p.role[i].tiles > tiles ? p.role[i].tiles : tiles;
-    const dim3 grid((unsigned)((long long)p.segs * p.H * tiles * p.n_roles));
+    const dim3 grid((unsigned)((long long)p.segs * p.H * p.role[0].tiles * p.n_roles));
     if (dx <= 64) vec ? launch_mode<IO, 64, true>(p, mode, grid, st) : launch_mode<IO, 64, false>(p, mode, grid, st);
     else vec ? launch_mode<IO, 128, true>(p, mode, grid, st) : launch_mode<IO, 128, false>(p, mode, grid, st);
     return check_launch("decay_attention");

@@ -15,12 +15,9 @@ template <int DX>
 __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
     const Role& r = p.role[blockIdx.z];
     int id = blockIdx.x / (DX / 16);
-    int tiles = 1;
-    for (int i = 0; i < p.n_roles; ++i) tiles = max(tiles, p.role[i].tiles);
-    const int z = id % tiles;
-    id /= tiles;
+    const int z = id % r.tiles;
+    id /= r.tiles;
     const int h = id % p.H, n = id / p.H;
-    if (z >= r.tiles) return;
     const Place w = sequence_place(p, n, 64);
     const int x = blockIdx.x % (DX / 16), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = first_segment(p, n, w.first), count = segment_count(p, w.len);
@@ -58,15 +55,25 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
     }
 }
 
-// out (rows, heads, D) = the sums over the heads of part (rows, heads * share, D) that share one, rounded once
+// out (rows, heads, D) = the sums of part (parts, rows, heads * share, D) over the parts and the heads that share one, rounded once
+struct Sum {
+    const float* part;
+    void* out;
+    long long count, apart;                               // results; numbers from part to part
+    int D, share, parts;
+};
+struct Sums {
+    Sum s[3];
+};
 template <typename IO>
-__global__ __launch_bounds__(THREADS) void head_sum_kernel(const float* part, IO* out, long long count, int D, int share) {
-    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < count; i += (long long)gridDim.x * THREADS) {
-        const long long head = i / D;
-        const int d = (int)(i % D);
+__global__ __launch_bounds__(THREADS) void head_sum_kernel(const Sums all) {
+    const Sum t = all.s[blockIdx.y];
+    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < t.count; i += (long long)gridDim.x * THREADS) {
+        const float* q = t.part + i / t.D * t.share * t.D + i % t.D;
         float s = 0.f;
-        for (int j = 0; j < share; ++j) s += part[(head * share + j) * D + d];
-        out[i] = from_f32<IO>(s);
+        for (int p = 0; p < t.parts; ++p)
+            for (int j = 0; j < t.share; ++j) s += q[p * t.apart + j * t.D];
+        static_cast<IO*>(t.out)[i] = from_f32<IO>(s);
     }
 }
 // out (rows, H) = the sums of part (tiles, rows, H)
@@ -78,38 +85,28 @@ __global__ __launch_bounds__(THREADS) void decay_grad_kernel(const float* part, 
         out[i] = from_f32<G>(s);
     }
 }
-// The same over the rows as well, in 64 bits: slices first, then their sums.  Grid (slices, ceil(H / 64)); 4 rows of 64 heads a step.
-__global__ __launch_bounds__(THREADS) void decay_slices_kernel(const float* part, double* slices, long long rows, int H) {
-    __shared__ double red[4][64];
-    const int h = blockIdx.y * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
-    double s = 0.;
-    if (h < H)
-        for (long long r = (long long)blockIdx.x * 4 + sub; r < rows; r += (long long)gridDim.x * 4) s += part[r * H + h];
-    red[sub][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (sub == 0 && h < H) slices[(long long)blockIdx.x * H + h] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-}
+// out (H) = the sums of the segments' and tiles' totals, in 64 bits: a workgroup for each head
 template <typename G>
-__global__ __launch_bounds__(64) void decay_total_kernel(const double* slices, G* out, int n, int H) {
-    const int h = blockIdx.x, lane = threadIdx.x;
+__global__ __launch_bounds__(THREADS) void decay_total_kernel(const double* sums, G* out, long long n, int H) {
+    __shared__ double red[THREADS / 64];
+    const int h = blockIdx.x, lane = threadIdx.x & 63;
     double s = 0.;
-    for (int i = lane; i < n; i += 64) s += slices[(long long)i * H + h];
+    for (long long i = threadIdx.x; i < n; i += THREADS) s += sums[i * H + h];
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    if (lane == 0) out[h] = from_f32<G>((float)s);
+    if (lane == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) out[h] = from_f32<G>((float)((red[0] + red[1]) + (red[2] + red[3])));
 }
-
-constexpr int SLICES = 128;
 
 size_t elem(int dtype) { return dtype == VRWKV_F32 ? 4 : 2; }
 int pad_dx(int d) { return d <= 64 ? 64 : 128; }
 int tiles_of(int d) { return (d + TZ - 1) / TZ; }
-int chunk_of(int dtype, bool together) { return dtype == VRWKV_BF16 || (together && dtype == VRWKV_F16) ? 64 : 32; }   // of the gradients' passes
+int chunk_of(int dtype) { return dtype == VRWKV_F32 ? 32 : 64; }   // of the gradients' pass
 
 // workgroups of a launch of outputs that the chip holds at once
 int slots(int dtype, int dx, bool backward) {
-    if (backward && dx == 64) return device_cus();
-    const int per_cu = dtype == VRWKV_BF16 ? (dx == 64 ? (backward ? 2 : 3) : (backward ? 1 : 2)) : dtype == VRWKV_F16 ? (dx == 64 || !backward ? 2 : 1) : dx == 64 ? 2 : 1;
+    const int per_cu = backward ? 1 : dtype == VRWKV_BF16 ? (dx == 64 ? 3 : 2) : dtype == VRWKV_F16 ? 2 : dx == 64 ? 2 : 1;
     return per_cu * device_cus();
 }
 // Tokens of a segment.  Calls of fewer sequences and heads than fill the chip are cut, into pieces that fill it in as few rounds as it takes: a round
@@ -156,7 +153,6 @@ int check_common(const vrwkv_decay_args* a, const char* who) {
     if (a->dtype < VRWKV_F32 || a->dtype > VRWKV_F16 || a->g_dtype < VRWKV_F32 || a->g_dtype > VRWKV_F16) { set_error("%s: dtype must be fp32, bf16 or fp16", who); return VRWKV_UNSUPPORTED_DTYPE; }
     if (a->H % a->Hq || a->H % a->Hk || a->H % a->Hv) { set_error("%s: H (%d) must be a multiple of the heads of q, k and v (%d, %d, %d)", who, a->H, a->Hq, a->Hk, a->Hv); return VRWKV_UNSUPPORTED_SHAPE; }
     if (a->Dk < 1 || a->Dk > 128 || a->Dv < 1 || a->Dv > 128) { set_error("%s: head sizes (%d, %d) must be 1 to 128", who, a->Dk, a->Dv); return VRWKV_UNSUPPORTED_SHAPE; }
-    // workgroups of a launch: at most four tiles and roles, or eight pieces of two tiles, of a segment (its first chunks, or a sequence) and head
     if (chunk_total(*a, 32) >= 1LL << 30 || (chunk_total(*a, 64) + a->N) * a->H >= 1LL << 24 || (long long)a->N * a->H * 32 >= 1LL << 24) { set_error("%s: too many tokens and heads", who); return VRWKV_UNSUPPORTED_SHAPE; }
     return VRWKV_OK;
 }
@@ -180,17 +176,12 @@ OutView out_view(void* p, int D, const vrwkv_decay_args& a, bool f32) {
     const long long st = (long long)a.H * D;
     return OutView{p, st * a.T, st, D, f32};
 }
-// Whether a launch may read and write rows in 16-byte pieces.
-bool in_pieces(const Params& p, int dtype) {
+// Whether rows may be read, or results written, in 16-byte pieces.
+bool in_pieces(const View& v, int d, int dtype) {
     const long long per16 = 16 / (long long)elem(dtype);
-    const auto fits = [&](const View& v, int d) { return !v.p || (((size_t)v.p & 15) == 0 && v.sb % per16 == 0 && v.st % per16 == 0 && v.sh % per16 == 0 && d % 8 == 0); };
-    bool vec = true;
-    for (int i = 0; i < p.n_roles; ++i) {
-        const Role& r = p.role[i];
-        vec = vec && fits(r.a, r.dx) && fits(r.b, r.dx) && fits(r.c, r.dz) && fits(r.e, r.dz) && ((size_t)r.o.p & 15) == 0;
-    }
-    return vec;
+    return !v.p || (((size_t)v.p & 15) == 0 && v.sb % per16 == 0 && v.st % per16 == 0 && v.sh % per16 == 0 && d % 8 == 0);
 }
+bool in_pieces(const OutView& v, int d) { return ((size_t)v.p & 15) == 0 && d % 8 == 0; }
 template <typename P>
 P common(const vrwkv_decay_args& a, int seg_len) {
     P p{};
@@ -212,7 +203,11 @@ P common(const vrwkv_decay_args& a, int seg_len) {
     return p;
 }
 int launch(const Params& p, int dtype, int dx, int mode, hipStream_t st) {
-    const bool vec = in_pieces(p, dtype);
+    bool vec = true;
+    for (int i = 0; i < p.n_roles; ++i) {
+        const Role& r = p.role[i];
+        vec = vec && in_pieces(r.a, r.dx, dtype) && in_pieces(r.b, r.dx, dtype) && in_pieces(r.c, r.dz, dtype) && in_pieces(r.o, r.dz);
+    }
     if (dtype == VRWKV_F32) return launch_decay<float>(p, dx, mode, vec, st);
     if (dtype == VRWKV_BF16) return launch_decay<__hip_bfloat16>(p, dx, mode, vec, st);
     return launch_decay<__half>(p, dx, mode, vec, st);
@@ -221,9 +216,7 @@ int launch(const Params& p, int dtype, int dx, int mode, hipStream_t st) {
 int launch_segments(const Params& p, int dtype, int dx, hipStream_t st) {
     const int s = launch(p, dtype, dx, STATES, st);
     if (s != VRWKV_OK) return s;
-    int tiles = 1;
-    for (int i = 0; i < p.n_roles; ++i) tiles = std::max(tiles, p.role[i].tiles);
-    const dim3 grid((unsigned)(dx / 16 * (long long)p.N * p.H * tiles), 1, p.n_roles), block(THREADS);
+    const dim3 grid((unsigned)(dx / 16 * (long long)p.N * p.H * p.role[0].tiles), 1, p.n_roles), block(THREADS);
     if (dx == 64) hipLaunchKernelGGL((segments_kernel<64>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((segments_kernel<128>), grid, block, 0, st, p);
     return check_launch("decay_attention (segments)");
@@ -245,63 +238,54 @@ struct FwdPlan {
         if (cut(a, seg_len)) take_segments(role, ws, a, segment_total(a, seg_len), dx);
     }
 };
-// Heads of up to 64 channels: one pass for all gradients (decay_bwd.h) behind one that keeps the states in front of the chunks.  Larger ones: dv, dk and dq one
-// after the other by the kernel of the forward pass.
+// A pass that keeps the states in front of the chunks, and one for all gradients (decay_bwd.h); tiles of 64 channels of larger heads, and heads that share a row of q, k or v, leave
+// parts that are added up behind.
 struct BwdPlan {
-    int dxk, dxv, seg_len, L;
-    bool together;
-    Role dv{}, dk{}, dq{};
-    float *fq = nullptr, *fk = nullptr, *fv = nullptr, *fg = nullptr;   // gradients of every head, where several share one; of the decays
-    double* slices = nullptr;
+    int dxv, tk, tv, seg_len;
+    Role r{}, s{};                                        // R back along the tokens; S along them
+    float *fq = nullptr, *fk = nullptr, *fv = nullptr, *fg = nullptr;   // parts
+    double* sums = nullptr;                               // of decays that all tokens share
     BwdPlan(const vrwkv_decay_args& a, Pieces& ws) {
-        dxk = pad_dx(a.Dk);
         dxv = pad_dx(a.Dv);
-        together = dxk == 64 && dxv == 64;
-        L = chunk_of(a.dtype, together);
-        dv.dx = dk.dz = dq.dz = a.Dk;
-        dv.dz = dk.dx = dq.dx = a.Dv;
-        dv.tiles = tiles_of(a.Dv);
-        dk.tiles = dq.tiles = tiles_of(a.Dk);
-        dv.reverse = dk.reverse = 1;
-        seg_len = segment_len(a, dxv, dk.tiles, 1, true);
+        tk = tiles_of(a.Dk);
+        tv = tiles_of(a.Dv);
+        r.dx = s.dx = a.Dv;
+        r.dz = s.dz = a.Dk;
+        r.tiles = s.tiles = tk;
+        r.reverse = 1;
+        seg_len = segment_len(a, dxv, tk * tv, 1, true);
         const long long segs = segment_total(a, seg_len), rows = rows_of(a);
         if (cut(a, seg_len)) {
-            if (!together) take_segments(dv, ws, a, segs, dxk);
-            take_segments(dk, ws, a, segs, dxv);
-            take_segments(dq, ws, a, segs, dxv);
+            take_segments(r, ws, a, segs, dxv);
+            take_segments(s, ws, a, segs, dxv);
         }
-        if (a.dq && a.Hq < a.H) fq = ws.take<float>((size_t)rows * a.H * a.Dk);
-        if (a.dk && a.Hk < a.H) fk = ws.take<float>((size_t)rows * a.H * a.Dk);
-        if (a.dv && a.Hv < a.H) fv = ws.take<float>((size_t)rows * a.H * a.Dv);
-        if (a.dg || together) dk.anchors = dq.anchors = ws.take<float>((size_t)chunk_total(a, L) * a.H * dk.tiles * dxv * TZ);
-        if (a.dg) {
-            if (!together) dk.edge = dq.edge = ws.take<float>((size_t)rows * a.H * dk.tiles);
-            if (a.g_per_head || dk.tiles > 1 || a.g_dtype != VRWKV_F32) fg = ws.take<float>((size_t)rows * a.H * dk.tiles);
-            if (a.g_per_head) slices = ws.take<double>((size_t)SLICES * a.H);
-        }
+        if (a.dq && (a.Hq < a.H || tv > 1)) fq = ws.take<float>((size_t)rows * a.H * a.Dk * tv);
+        if (a.dk && (a.Hk < a.H || tv > 1)) fk = ws.take<float>((size_t)rows * a.H * a.Dk * tv);
+        if (a.dv && (a.Hv < a.H || tk > 1)) fv = ws.take<float>((size_t)rows * a.H * a.Dv * tk);
+        s.anchors = ws.take<float>((size_t)chunk_total(a, chunk_of(a.dtype)) * a.H * tk * dxv * TZ);
+        if (a.dg && a.g_per_head) sums = ws.take<double>((size_t)segs * tk * tv * a.H);
+        else if (a.dg && (tk * tv > 1 || a.g_dtype != VRWKV_F32)) fg = ws.take<float>((size_t)rows * a.H * tk * tv);
     }
 };
+// A launch has less than 2^32 threads.
+int check_grid(const vrwkv_decay_args& a, int seg_len, int tiles, int threads, const char* who) {
+    if (std::max(segment_total(a, seg_len) * threads, (long long)a.N * 8 * THREADS) * a.H * tiles < 1LL << 32) return VRWKV_OK;
+    set_error("%s: too many sequences and heads", who);
+    return VRWKV_UNSUPPORTED_SHAPE;
+}
 int check_workspace(const vrwkv_decay_args& a, size_t need, const char* who) {
     if (need && (!a.workspace || a.workspace_bytes < need)) { set_error("%s: workspace of %zu bytes, %zu needed", who, a.workspace ? a.workspace_bytes : 0, need); return VRWKV_WORKSPACE_TOO_SMALL; }
     if (need && ((size_t)a.workspace & 15)) { set_error("%s: workspace must be 16-byte aligned", who); return VRWKV_INVALID_ARG; }
     return VRWKV_OK;
 }
-template <typename IO>
-void head_sums(const float* part, void* out, const vrwkv_decay_args& a, int heads, int D, hipStream_t st) {
-    const long long count = rows_of(a) * heads * D;
-    const unsigned grid = (unsigned)std::min<long long>((count + THREADS - 1) / THREADS, 8192);
-    hipLaunchKernelGGL((head_sum_kernel<IO>), dim3(grid), dim3(THREADS), 0, st, part, static_cast<IO*>(out), count, D, a.H / heads);
-}
 template <typename G>
 void decay_sums(const BwdPlan& b, const vrwkv_decay_args& a, hipStream_t st) {
-    const long long rows = rows_of(a), count = rows * a.H;
-    if (a.g_per_head) {
-        const int n = (int)std::min<long long>(SLICES, (rows * b.dk.tiles + 3) / 4);
-        hipLaunchKernelGGL(decay_slices_kernel, dim3(n, (a.H + 63) / 64), dim3(THREADS), 0, st, b.fg, b.slices, rows * b.dk.tiles, a.H);
-        hipLaunchKernelGGL((decay_total_kernel<G>), dim3(a.H), dim3(64), 0, st, b.slices, static_cast<G*>(a.dg), n, a.H);
-    } else {
+    if (b.sums)
+        hipLaunchKernelGGL((decay_total_kernel<G>), dim3(a.H), dim3(THREADS), 0, st, b.sums, static_cast<G*>(a.dg), segment_total(a, b.seg_len) * b.tk * b.tv, a.H);
+    else {
+        const long long count = rows_of(a) * a.H;
         const unsigned grid = (unsigned)std::min<long long>((count + THREADS - 1) / THREADS, 4096);
-        hipLaunchKernelGGL((decay_grad_kernel<G>), dim3(grid), dim3(THREADS), 0, st, b.fg, static_cast<G*>(a.dg), count, b.dk.tiles);
+        hipLaunchKernelGGL((decay_grad_kernel<G>), dim3(grid), dim3(THREADS), 0, st, b.fg, static_cast<G*>(a.dg), count, b.tk * b.tv);
     }
 }
 
@@ -328,7 +312,7 @@ extern "C" int vrwkv_decay_fwd(const vrwkv_decay_args* args, void* hip_stream) {
     if (!a.y) { set_error("%s: null y", who); return VRWKV_INVALID_ARG; }
     Pieces size{nullptr};
     FwdPlan sized(a, size);
-    if ((s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
+    if ((s = check_grid(a, sized.seg_len, sized.role.tiles, THREADS, who)) != VRWKV_OK || (s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
     Pieces ws{static_cast<char*>(a.workspace)};
     FwdPlan plan(a, ws);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
@@ -365,93 +349,71 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     if (!a.gy) { set_error("%s: null gy", who); return VRWKV_INVALID_ARG; }
     Pieces size{nullptr};
     BwdPlan sized(a, size);
-    if ((s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
+    if ((s = check_grid(a, sized.seg_len, sized.tk * sized.tv, BWD_THREADS, who)) != VRWKV_OK || (s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
     Pieces ws{static_cast<char*>(a.workspace)};
     BwdPlan b(a, ws);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const View q = view(a.q, a.q_stride, a.Hq, a), k = view(a.k, a.k_stride, a.Hk, a), v = view(a.v, a.v_stride, a.Hv, a), gy = view(a.gy, a.gy_stride, a.H, a);
-    // dv_t = R_t^T k_t: R from q and gy; its last state is the gradient of the first one
-    b.dv.a = k;
-    b.dv.b = q;
-    b.dv.c = gy;
-    b.dv.o = out_view(b.fv ? b.fv : a.dv, a.Dv, a, b.fv != nullptr);
-    b.dv.init = a.glast;
-    b.dv.last = a.dstate;
-    b.dv.sx = a.Dv;
-    b.dv.sz = 1;
-    b.dv.s_in = 1.f;
-    b.dv.s_upd = a.scale;
-    // dk_t = R_t v_t: R the other way round
-    b.dk.a = v;
-    b.dk.b = gy;
-    b.dk.c = q;
-    b.dk.e = k;
-    b.dk.o = out_view(b.fk ? b.fk : a.dk, a.Dk, a, b.fk != nullptr);
-    b.dk.init = a.glast;
-    b.dk.sx = 1;
-    b.dk.sz = a.Dv;
-    b.dk.s_in = 1.f;
-    b.dk.s_upd = a.scale;
-    // dq_t = scale S_t gy_t
-    b.dq.a = gy;
-    b.dq.b = v;
-    b.dq.c = k;
-    b.dq.e = q;
-    b.dq.o = out_view(b.fq ? b.fq : a.dq, a.Dk, a, b.fq != nullptr);
-    b.dq.init = a.state;
-    b.dq.sx = 1;
-    b.dq.sz = a.Dv;
-    b.dq.s_in = a.scale;
-    b.dq.s_upd = 1.f;
-    b.dq.dg = b.fg ? b.fg : static_cast<float*>(a.dg);
     Params p = common<Params>(a, b.seg_len);
-    const auto run = [&](std::initializer_list<Role> roles, int dx, int mode) {
-        p.n_roles = 0;
-        for (const Role& r : roles) p.role[p.n_roles++] = r;
-        return mode == STATES ? launch_segments(p, a.dtype, dx, st) : launch(p, a.dtype, dx, mode, st);
+    for (Role* r : {&b.r, &b.s}) {
+        r->b = r == &b.r ? gy : v;
+        r->c = r == &b.r ? q : k;
+        r->init = r == &b.r ? a.glast : a.state;
+        r->sx = 1;                                        // rows of v's channels, columns of k's
+        r->sz = a.Dv;
+        r->s_in = 1.f;
+        r->s_upd = r == &b.r ? a.scale : 1.f;
+    }
+    if (b.r.seg) {
+        p.n_roles = 2;
+        p.role[0] = b.r;
+        p.role[1] = b.s;
+        if ((s = launch_segments(p, a.dtype, b.dxv, st)) != VRWKV_OK) return s;
+    }
+    p.n_roles = 1;
+    p.role[0] = b.s;
+    if ((s = launch(p, a.dtype, b.dxv, CHUNKS, st)) != VRWKV_OK) return s;
+    BwdParams t = common<BwdParams>(a, b.seg_len);
+    t.q = q;
+    t.k = k;
+    t.v = v;
+    t.gy = gy;
+    t.dq = out_view(b.fq ? b.fq : a.dq, a.Dk, a, b.fq != nullptr);
+    t.dk = out_view(b.fk ? b.fk : a.dk, a.Dk, a, b.fk != nullptr);
+    t.dv = out_view(b.fv ? b.fv : a.dv, a.Dv, a, b.fv != nullptr);
+    t.dg = b.sums ? nullptr : b.fg ? b.fg : static_cast<float*>(a.dg);
+    t.dg_sums = b.sums;
+    t.chunks = b.s.anchors;
+    t.seg = b.r.seg;
+    t.glast = a.glast;
+    t.dstate = a.dstate;
+    t.Dk = a.Dk;
+    t.Dv = a.Dv;
+    t.tk = b.tk;
+    t.tv = b.tv;
+    const bool vec = in_pieces(q, a.Dk, a.dtype) && in_pieces(k, a.Dk, a.dtype) && in_pieces(v, a.Dv, a.dtype) && in_pieces(gy, a.Dv, a.dtype) && in_pieces(t.dq, a.Dk) && in_pieces(t.dk, a.Dk) &&
+                     in_pieces(t.dv, a.Dv);
+    s = a.dtype == VRWKV_F32 ? launch_decay_bwd<float>(t, vec, st) : a.dtype == VRWKV_BF16 ? launch_decay_bwd<__hip_bfloat16>(t, vec, st) : launch_decay_bwd<__half>(t, vec, st);
+    if (s != VRWKV_OK) return s;
+    Sums sums{};
+    int n_sums = 0;
+    long long most = 0;
+    const auto add = [&](const float* part, void* out, int heads, int D, int parts) {
+        if (!part) return;
+        const long long rows = rows_of(a);
+        sums.s[n_sums++] = Sum{part, out, rows * heads * D, rows * a.H * D, D, a.H / heads, parts};
+        most = std::max(most, rows * heads * D);
     };
-    if (b.together) {
-        if (b.dk.seg && (s = run({b.dk, b.dq}, 64, STATES)) != VRWKV_OK) return s;
-        if ((s = run({b.dq}, 64, CHUNKS)) != VRWKV_OK) return s;
-        BwdParams t = common<BwdParams>(a, b.seg_len);
-        t.q = q;
-        t.k = k;
-        t.v = v;
-        t.gy = gy;
-        t.dq = b.dq.o;
-        t.dk = b.dk.o;
-        t.dv = b.dv.o;
-        t.dg = b.dq.dg;
-        t.chunks = b.dq.anchors;
-        t.seg = b.dk.seg;
-        t.glast = a.glast;
-        t.dstate = a.dstate;
-        t.Dk = a.Dk;
-        t.Dv = a.Dv;
-        p.n_roles = 0;
-        for (const Role& r : {b.dv, b.dk, b.dq}) p.role[p.n_roles++] = r;
-        const bool vec = in_pieces(p, a.dtype);
-        s = a.dtype == VRWKV_F32 ? launch_decay_bwd<float>(t, vec, st) : a.dtype == VRWKV_BF16 ? launch_decay_bwd<__hip_bfloat16>(t, vec, st) : launch_decay_bwd<__half>(t, vec, st);
-        if (s != VRWKV_OK) return s;
+    add(b.fq, a.dq, a.Hq, a.Dk, b.tv);
+    add(b.fk, a.dk, a.Hk, a.Dk, b.tv);
+    add(b.fv, a.dv, a.Hv, a.Dv, b.tk);
+    if (n_sums) {
+        const dim3 grid((unsigned)std::min<long long>((most + THREADS - 1) / THREADS, 8192), n_sums);
+        if (a.dtype == VRWKV_F32) hipLaunchKernelGGL((head_sum_kernel<float>), grid, dim3(THREADS), 0, st, sums);
+        else if (a.dtype == VRWKV_BF16) hipLaunchKernelGGL((head_sum_kernel<__hip_bfloat16>), grid, dim3(THREADS), 0, st, sums);
+        else hipLaunchKernelGGL((head_sum_kernel<__half>), grid, dim3(THREADS), 0, st, sums);
     }
-    const bool want_dv = !b.together && (a.dv || a.dstate), want_dk = !b.together && (a.dk || a.dg), want_dq = !b.together && (a.dq || a.dg);
-    if (b.dv.seg) {
-        if (want_dv && (s = run({b.dv}, b.dxk, STATES)) != VRWKV_OK) return s;
-        if (want_dk && want_dq) s = run({b.dk, b.dq}, b.dxv, STATES);
-        else if (want_dk || want_dq) s = run({want_dk ? b.dk : b.dq}, b.dxv, STATES);
-        if (s != VRWKV_OK) return s;
-    }
-    if (want_dv && (s = run({b.dv}, b.dxk, PLAIN)) != VRWKV_OK) return s;
-    if (want_dk && (s = run({b.dk}, b.dxv, a.dg ? EDGES : ALONE)) != VRWKV_OK) return s;
-    if (want_dq && (s = run({b.dq}, b.dxv, a.dg ? FLOWS : ALONE)) != VRWKV_OK) return s;
-    struct { const float* part; void* out; int heads, D; } sums[3] = {{b.fq, a.dq, a.Hq, a.Dk}, {b.fk, a.dk, a.Hk, a.Dk}, {b.fv, a.dv, a.Hv, a.Dv}};
-    for (const auto& t : sums)
-        if (t.part) {
-            if (a.dtype == VRWKV_F32) head_sums<float>(t.part, t.out, a, t.heads, t.D, st);
-            else if (a.dtype == VRWKV_BF16) head_sums<__hip_bfloat16>(t.part, t.out, a, t.heads, t.D, st);
-            else head_sums<__half>(t.part, t.out, a, t.heads, t.D, st);
-        }
-    if (b.fg) {
+    if (b.sums || b.fg) {
         if (a.g_dtype == VRWKV_F32) decay_sums<float>(b, a, st);
         else if (a.g_dtype == VRWKV_BF16) decay_sums<__hip_bfloat16>(b, a, st);
         else decay_sums<__half>(b, a, st);

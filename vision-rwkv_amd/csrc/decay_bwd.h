@@ -1,4 +1,4 @@
-// Gradients of the attention with a decay for each head, heads of up to 64 channels, all in one pass back along the chunks (gfx950).
+// Gradients of the attention with a decay for each head, all in one pass back along the chunks (gfx950).
 // With S0 the state in front of a chunk (kept for every chunk by a pass of decay_attn.h), X the gradient of the state behind it, G the sums of its log
 // decays, D_ts = exp(G_t - G_s) for s <= t, P = scale D (q k^T) and dP = scale D (gy v^T):
 //     dq_t = sum_s dP_ts k_s + scale exp(G_t) S0 gy_t
@@ -10,6 +10,8 @@
 // waves of four kinds: 110 us for 64 x 196 tokens of 12 heads in bf16 where eight took 90, for what the kinds form twice and the registers that they lack.)
 // Every operand of the products is read as it lies or across its rows, so the chunk's rows are staged once, where dv, dk and dq by themselves (decay_attn.h)
 // stage ten tensors.  X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
+// Larger heads go in tiles of 64 of k's and 64 of v's channels.  Everything is a sum over one or both kinds of tiles: dq and dk over v's, dv over k's, dg over
+// all pairs; the parts are added up in fp32 behind.
 // @BASE@
 #pragma once
 #include "decay_attn.h"
@@ -21,13 +23,14 @@ constexpr int BWD_THREADS = 512;
 
 struct BwdParams : Call {
     View q, k, v, gy;
-    OutView dq, dk, dv;
-    float* dg;                                            // [row][head]
-    const float *chunks;                                  // [chunk][head]: S0, rows of v's channels and columns of k's, as the accumulators lie
-    const float *seg;                                     // [segment][head]: R behind the segment, without the decay of the token behind it; null: sequences are not cut
+    OutView dq, dk, dv;                                   // (parts lie rows * heads * channels apart)
+    float* dg;                                            // [tiles][row][head]
+    double* dg_sums;                                      // or, for decays that all tokens share, [segment][tiles][head]
+    const float *chunks;                                  // [chunk][head][tile of k][tile of v]: S0, rows of v's channels and columns of k's, as the accumulators lie
+    const float *seg;                                     // [segment][head][..][..]: R behind the segment, without the decay of the token behind it; null: sequences are not cut
     const float* glast;                                   // gradients of the states behind the last tokens, or null
     float* dstate;
-    int Dk, Dv;
+    int Dk, Dv, tk, tv;                                   // channels; tiles of 64
 };
 
 template <typename IO>
@@ -54,37 +57,51 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
     __shared__ S lds;
     const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2, w4 = wave & 3;
-    const int h = blockIdx.x % p.H, gid = blockIdx.x / p.H;
+    // tiles of one head next to each other: they read the same rows
+    const int tile = blockIdx.x % (p.tk * p.tv), h = blockIdx.x / (p.tk * p.tv) % p.H, gid = blockIdx.x / (p.tk * p.tv) / p.H;
+    const int ik = tile % p.tk, iv = tile / p.tk, k0 = 64 * ik, v0 = 64 * iv;
+    const auto part = [&](OutView v, int i, int D) {
+        if (v.p && v.f32) v.p = static_cast<float*>(v.p) + i * p.rows * p.H * D;
+        return v;
+    };
+    const OutView out_q = part(p.dq, iv, p.Dk), out_k = part(p.dk, iv, p.Dk), out_v = part(p.dv, ik, p.Dv);
+    float* const dg_part = FLOW && p.dg ? p.dg + tile * p.rows * p.H : nullptr;
+    double* const dg_sum = FLOW && p.dg_sums ? p.dg_sums + ((long long)gid * p.tk * p.tv + tile) * p.H + h : nullptr;
 
     if (!p.nseg) {                                        // packed rows in front of the first sequence and behind the last: no gradient
         const int front = offset_at(p, 0), back = offset_at(p, p.N), rows = front + max(0, p.T - back);
         for (int i = gid * 8 + wave; i < rows; i += p.segs * 8) {
             const long long row = i < front ? i : back + (i - front);
-            const OutView* const outs[3] = {&p.dq, &p.dk, &p.dv};
+            const OutView* const outs[3] = {&out_q, &out_k, &out_v};
 #pragma unroll
             for (int o = 0; o < 3; ++o) {
                 const OutView& v = *outs[o];
-                if (v.p && lane < (o < 2 ? p.Dk : p.Dv)) {
-                    const long long at = row * v.st + h * v.sh + lane;
+                const int d = (o < 2 ? k0 : v0) + lane;
+                if (v.p && d < (o < 2 ? p.Dk : p.Dv)) {
+                    const long long at = row * v.st + h * v.sh + d;
                     if (v.f32) static_cast<float*>(v.p)[at] = 0.f;
                     else static_cast<IO*>(v.p)[at] = from_f32<IO>(0.f);
                 }
             }
-            if (FLOW && lane == 0) p.dg[row * p.H + h] = 0.f;
+            if (dg_part && lane == 0) dg_part[row * p.H + h] = 0.f;
         }
     }
     const Place w = find_place<BWD_THREADS>(p, gid, L);
-    if (!w.valid) return;
+    if (!w.valid) {
+        if (dg_sum && tid == 0) *dg_sum = 0.;
+        return;
+    }
     const int nc = (w.s1 - w.s0 + L - 1) / L;
 
     const int row0 = (tid & 255) >> 3, d0 = (tid & 7) * 8;
     Source<IO, PIECES, 32, VEC> sa, sb;                   // the kinds stage a pair of tensors each
-    sa.open(group ? p.k : p.q, w.base, w.first, h, L, false, row0, d0, p.Dk);
-    sb.open(group ? p.gy : p.v, w.base, w.first, h, L, false, row0, d0, p.Dv);
+    sa.open(group ? p.k : p.q, w.base, w.first, h, L, false, row0, k0 + d0, p.Dk);
+    sb.open(group ? p.gy : p.v, w.base, w.first, h, L, false, row0, v0 + d0, p.Dv);
     Gates gates;
     gates.open(p, w.base, w.first, h);
-    const float* const chunks = p.chunks + ((long long)(w.chunk0 + w.s0 / L) * p.H + h) * 4096 + (w4 * 64 + lane) * 4;
-    const long long chunk_step = (long long)p.H * 4096;
+    const int tiles = p.tk * p.tv * 4096, my_tile = (ik * p.tv + iv) * 4096 + (w4 * 64 + lane) * 4;
+    const float* const chunks = p.chunks + ((long long)(w.chunk0 + w.s0 / L) * p.H + h) * tiles + my_tile;
+    const long long chunk_step = (long long)p.H * tiles;
     Piece<IO> ra[PIECES], rb[PIECES];
     Gates::Raw rg{};
     f32x4 st[4];                                          // group 0: S0; group 1: X.  Rows 16 x + 4 quarter + i (v's channels), column 16 w4 + col (k's)
@@ -113,7 +130,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
 
     // ---- X behind the segment
     const long long page = ((long long)w.n * p.H + h) * ((long long)p.Dk * p.Dv);
-    const int zc = 16 * w4 + col;
+    const int zc = k0 + 16 * w4 + col;
     const bool cut = p.seg && !w.is_last;
     bool have = cut || p.glast;
     if (group == 0) {
@@ -123,7 +140,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         const float d = fast_exp2(gates.widen(gates.fetch(w.s1, 0, true)) * LOG2E);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            st[x] = *reinterpret_cast<const f32x4*>(p.seg + ((long long)gid * p.H + h) * 4096 + ((x * 4 + w4) * 64 + lane) * 4);
+            st[x] = *reinterpret_cast<const f32x4*>(p.seg + ((long long)gid * p.H + h) * tiles + my_tile + x * 1024);
 #pragma unroll
             for (int i = 0; i < 4; ++i) st[x][i] *= d;
         }
@@ -133,15 +150,16 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         for (int x = 0; x < 4; ++x)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int xc = 16 * x + 4 * quarter + i;
+                const int xc = v0 + 16 * x + 4 * quarter + i;
                 st[x][i] = __builtin_bit_cast(float, BufRaw<4>::ld(buf, have && xc < p.Dv && zc < p.Dk ? (unsigned)(zc * p.Dv + xc) * 4u : OOB_OFFSET, 0));
             }
     }
     const int tw = w4 % NT, zt0 = w4 / NT * NT;           // this wave's tile of tokens, its first tile of channels
     Sink<IO, VEC> oa, ob;                                 // dq; dk and dv
-    oa.open(group ? p.dk : p.dq, w.base, w.first, h, 16 * tw + col, 16 * zt0 + 4 * quarter, p.Dk);
-    ob.open(p.dv, w.base, w.first, h, 16 * tw + col, 16 * zt0 + 4 * quarter, p.Dv);
-    float* dg = FLOW ? p.dg + ((long long)w.base * p.T + w.first) * p.H + h : nullptr;
+    oa.open(group ? out_k : out_q, w.base, w.first, h, 16 * tw + col, k0 + 16 * zt0 + 4 * quarter, p.Dk);
+    ob.open(out_v, w.base, w.first, h, 16 * tw + col, v0 + 16 * zt0 + 4 * quarter, p.Dv);
+    float* dg = dg_part ? dg_part + ((long long)w.base * p.T + w.first) * p.H + h : nullptr;
+    double dg_total = 0.;                                 // (wave 0) of the segment's tokens
     int H = p.H;
     float scale = p.scale;
     keep(dg);
@@ -170,7 +188,10 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         const double inner = ((double)f.inner[0][at] + f.inner[1][at]) + ((double)f.inner[2][at] + f.inner[3][at]);
         const double through = ((double)f.through[0] + f.through[1]) + ((double)f.through[2] + f.through[3]);
         const double all = flow_sum(inner, in, out, lane) + through;
-        if (lane < n) dg[(long long)(t0 + lane) * H] = (float)all;
+        if (lane < n) {
+            if (dg) dg[(long long)(t0 + lane) * H] = (float)all;
+            dg_total += all;
+        }
     };
     if (nc > 0) {
         if (wave == 0) put_decays(lds.d[0]);
@@ -493,7 +514,14 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         lds_barrier();
     }
     if constexpr (FLOW) {
-        if (wave == 0 && nc > 0) put_flows(lds.f[(nc + 1) & 1], w.s0, min(L, w.s1 - w.s0));
+        if (wave == 0) {
+            if (nc > 0) put_flows(lds.f[(nc + 1) & 1], w.s0, min(L, w.s1 - w.s0));
+            if (dg_sum) {
+#pragma unroll
+                for (int d = 32; d; d >>= 1) dg_total += __shfl_xor(dg_total, d);
+                if (lane == 0) *dg_sum = dg_total;
+            }
+        }
     }
 
     if (p.dstate && w.is_first && group == 1) {
@@ -501,7 +529,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         for (int x = 0; x < 4; ++x)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int xc = 16 * x + 4 * quarter + i;
+                const int xc = v0 + 16 * x + 4 * quarter + i;
                 if (xc < p.Dv && zc < p.Dk) p.dstate[page + (long long)zc * p.Dv + xc] = st[x][i];
             }
     }
@@ -514,8 +542,8 @@ extern template int launch_decay_bwd<__half>(const BwdParams&, bool, hipStream_t
 
 template <typename IO>
 int launch_decay_bwd(const BwdParams& p, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)((long long)p.segs * p.H)), block(BWD_THREADS);
-    if (p.dg) {
+    const dim3 grid((unsigned)((long long)p.segs * p.H * p.tk * p.tv)), block(BWD_THREADS);
+    if (p.dg || p.dg_sums) {
         if (vec) hipLaunchKernelGGL((decay_bwd_kernel<IO, true, true>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((decay_bwd_kernel<IO, true, false>), grid, block, 0, st, p);
     } else {
