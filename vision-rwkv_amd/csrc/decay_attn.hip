@@ -121,7 +121,8 @@ int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool ba
         for (int pieces = 1; pieces <= std::min(chunks / 2, 64) || pieces == 1; ++pieces) {
             const int len = (chunks + pieces - 1) / pieces, n = (chunks + len - 1) / len;
             const double rounds = (double)((wgs * a.N * n + room - 1) / room), once = rounds * (len + 2);
-            const double cost = n == 1 ? once : 1.5 * once + 3 + n / 16.0;
+            // (backward: the pass over the chunks' states a third of the time beside it, the segments' states a third of its rows' again)
+            const double cost = backward ? 1.35 * once + (n == 1 ? 0. : 0.3 * once + 2 + n / 16.0) : n == 1 ? once : 1.5 * once + 3 + n / 16.0;
             if (cost < least) { least = cost; best = len; }
         }
         return best * 64;

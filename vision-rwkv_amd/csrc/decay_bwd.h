@@ -6,8 +6,9 @@
 //     X <- exp(G_end) X + scale sum_t exp(G_t) q_t gy_t^T
 //     dg_j = what crosses from tokens in front of j to j and behind: the terms P_ts (gy_t . v_s) with s < j <= t; q . (S0's part of dq) of the tokens from j on;
 //            k . (X's part of dk) of those in front; exp(G_end) <S0, X>.  Sums of what crosses, so nothing cancels where little does.
-// Eight waves, two a SIMD: four take dq and dg's crossings inside the chunk, tokens t along the lanes; four take dk, dv and X, tokens s along the lanes.  (Sixteen
-// waves of four kinds: 110 us for 64 x 196 tokens of 12 heads in bf16 where eight took 90, for what the kinds form twice and the registers that they lack.)
+// Twelve waves, three a SIMD, of three kinds: dq and dg's crossings inside the chunk (tokens t along the lanes), dk, and dv and X (tokens s along the lanes).  What
+// one kind waits for the others cover: with dk, dv and X in one kind of eight waves a chunk of 64 bf16 tokens took 12 900 cycles, 60 % of them with an instruction; with
+// sixteen waves the registers did not do.
 // Every operand of the products is read as it lies or across its rows, so the chunk's rows are staged once, where dv, dk and dq by themselves (decay_attn.h)
 // stage ten tensors.  X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
 // Larger heads go in tiles of 64 of k's and 64 of v's channels.  Everything is a sum over one or both kinds of tiles: dq and dk over v's, dv over k's, dg over
@@ -19,7 +20,8 @@
 namespace vrwkv {
 namespace decay {
 
-constexpr int BWD_THREADS = 512;
+constexpr int BWD_THREADS = 768;
+enum Kind { DQ = 0, DK = 1, DV = 2 };
 
 struct BwdParams : Call {
     View q, k, v, gy;
@@ -50,13 +52,13 @@ struct BwdLds {
 };
 
 template <typename IO, bool FLOW, bool VEC>
-__global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdParams p) {
+__global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdParams p) {
     using S = BwdLds<IO>;
     constexpr int L = S::L, NS = S::NS, NT = L / 16, KS = L / 32, PX = S::PX, NP = NS < 3 ? 2 : 3;
-    constexpr int PIECES = L * 8 / 256;                   // of each pair of tensors, a thread's: halves of the workgroup take (q, v) and (k, gy)
+    constexpr int PIECES = L * 8 / 256;                   // a thread's of the tensor that its kind stages: q, k or v; the first two kinds take half of gy besides
     __shared__ S lds;
     const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2, w4 = wave & 3;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kind = wave >> 2, w4 = wave & 3;
     // tiles of one head next to each other: they read the same rows
     const int tile = blockIdx.x % (p.tk * p.tv), h = blockIdx.x / (p.tk * p.tv) % p.H, gid = blockIdx.x / (p.tk * p.tv) / p.H;
     const int ik = tile % p.tk, iv = tile / p.tk, k0 = 64 * ik, v0 = 64 * iv;
@@ -70,7 +72,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
 
     if (!p.nseg) {                                        // packed rows in front of the first sequence and behind the last: no gradient
         const int front = offset_at(p, 0), back = offset_at(p, p.N), rows = front + max(0, p.T - back);
-        for (int i = gid * 8 + wave; i < rows; i += p.segs * 8) {
+        for (int i = gid * 12 + wave; i < rows; i += p.segs * 12) {
             const long long row = i < front ? i : back + (i - front);
             const OutView* const outs[3] = {&out_q, &out_k, &out_v};
 #pragma unroll
@@ -94,23 +96,28 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
     const int nc = (w.s1 - w.s0 + L - 1) / L;
 
     const int row0 = (tid & 255) >> 3, d0 = (tid & 7) * 8;
-    Source<IO, PIECES, 32, VEC> sa, sb;                   // the kinds stage a pair of tensors each
-    sa.open(group ? p.k : p.q, w.base, w.first, h, L, false, row0, k0 + d0, p.Dk);
-    sb.open(group ? p.gy : p.v, w.base, w.first, h, L, false, row0, v0 + d0, p.Dv);
+    // (half of gy: rows of even and odd blocks of 32 where a thread takes two of its own tensor, otherwise the workgroup's first and second 16)
+    const int gy_row = PIECES == 2 ? row0 + 32 * kind : kind * 16 + row0;
+    const bool gy_mine = kind < DV && (PIECES == 2 || row0 < 16);
+    Source<IO, PIECES, 32, VEC> sa;
+    Source<IO, 1, 32, VEC> sb;
+    sa.open(kind == DQ ? p.q : kind == DK ? p.k : p.v, w.base, w.first, h, L, false, row0, (kind == DV ? v0 : k0) + d0, kind == DV ? p.Dv : p.Dk);
+    sb.open(p.gy, w.base, w.first, h, L, false, gy_mine ? gy_row : L, v0 + d0, p.Dv);
     Gates gates;
     gates.open(p, w.base, w.first, h);
     const int tiles = p.tk * p.tv * 4096, my_tile = (ik * p.tv + iv) * 4096 + (w4 * 64 + lane) * 4;
     const float* const chunks = p.chunks + ((long long)(w.chunk0 + w.s0 / L) * p.H + h) * tiles + my_tile;
     const long long chunk_step = (long long)p.H * tiles;
-    Piece<IO> ra[PIECES], rb[PIECES];
+    Piece<IO> ra[PIECES], rb[1];
     Gates::Raw rg{};
-    f32x4 st[4];                                          // group 0: S0; group 1: X.  Rows 16 x + 4 quarter + i (v's channels), column 16 w4 + col (k's)
+    constexpr int LIGHT = 4 * DK + 3;                     // the wave with the least to do: of dk, with the last tokens
+    f32x4 st[4];                                          // dk: S0; dv: X.  Rows 16 x + 4 quarter + i (v's channels), column 16 w4 + col (k's)
     u32x4 held[3][2];                                     // its terms
     const auto fetch = [&](int c) {
         const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
         sa.load(ra, t0, n, false);
         sb.load(rb, t0, n, false);
-        if (wave == 0) rg = gates.fetch(t0, lane, lane < n);
+        if (wave == LIGHT) rg = gates.fetch(t0, lane, lane < n);
     };
     const auto fetch_state = [&](int c) {
 #pragma unroll
@@ -126,6 +133,16 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
             for (int s = 0; s < 3; ++s) held[s][kx] = __builtin_bit_cast(u32x4, t[s]);
         }
     };
+    // (a kind that has no state: its registers are free while it works)
+    const auto forget = [&]() {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 3; ++s)
+#pragma unroll
+            for (int kx = 0; kx < 2; ++kx) held[s][kx] = u32x4{0, 0, 0, 0};
+    };
+    forget();
     if (nc > 0) fetch(nc - 1);
 
     // ---- X behind the segment
@@ -133,9 +150,9 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
     const int zc = k0 + 16 * w4 + col;
     const bool cut = p.seg && !w.is_last;
     bool have = cut || p.glast;
-    if (group == 0) {
+    if (kind == DK) {
         if (nc > 0) fetch_state(nc - 1);
-    } else if (cut) {
+    } else if (kind == DV && cut) {
         // (R behind a segment wants the decay of the token there)
         const float d = fast_exp2(gates.widen(gates.fetch(w.s1, 0, true)) * LOG2E);
 #pragma unroll
@@ -144,7 +161,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
 #pragma unroll
             for (int i = 0; i < 4; ++i) st[x][i] *= d;
         }
-    } else {
+    } else if (kind == DV) {
         const auto buf = buffer_at(p.glast + page);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -155,18 +172,18 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
             }
     }
     const int tw = w4 % NT, zt0 = w4 / NT * NT;           // this wave's tile of tokens, its first tile of channels
-    Sink<IO, VEC> oa, ob;                                 // dq; dk and dv
-    oa.open(group ? out_k : out_q, w.base, w.first, h, 16 * tw + col, k0 + 16 * zt0 + 4 * quarter, p.Dk);
-    ob.open(out_v, w.base, w.first, h, 16 * tw + col, v0 + 16 * zt0 + 4 * quarter, p.Dv);
+    Sink<IO, VEC> so;
+    if (kind == DV) so.open(out_v, w.base, w.first, h, 16 * tw + col, v0 + 16 * zt0 + 4 * quarter, p.Dv);
+    else so.open(kind == DK ? out_k : out_q, w.base, w.first, h, 16 * tw + col, k0 + 16 * zt0 + 4 * quarter, p.Dk);
     float* dg = dg_part ? dg_part + ((long long)w.base * p.T + w.first) * p.H + h : nullptr;
-    double dg_total = 0.;                                 // (wave 0) of the segment's tokens
+    double dg_total = 0.;                                 // (the light wave) of the segment's tokens
     int H = p.H;
     float scale = p.scale;
     keep(dg);
     keep(H);
     keep(scale);
 
-    const auto put_decays = [&](typename S::Decays& d) {   // wave 0
+    const auto put_decays = [&](typename S::Decays& d) {   // the light wave
         const double G = wave_scan_inclusive((double)gates.widen(rg) * 1.4426950408889634);
         const double end = lane_double(G, 63);
         const float gh = (float)G;
@@ -178,7 +195,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         }
         if (lane == 0) d.end = fast_exp2((float)end);
     };
-    const auto put_flows = [&](const typename S::Flows& f, int t0, int n) {   // wave 0
+    const auto put_flows = [&](const typename S::Flows& f, int t0, int n) {   // the light wave
         const int at = min(lane, L - 1);
         double in = 0., out = 0.;
         if (lane < n) {
@@ -194,8 +211,8 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         }
     };
     if (nc > 0) {
-        if (wave == 0) put_decays(lds.d[0]);
-        hold();
+        if (wave == LIGHT) put_decays(lds.d[0]);
+        if (kind != DQ) hold();
     }
 
     for (int ci = 0; ci < nc; ++ci) {
@@ -205,38 +222,39 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         const int quarter = lane_ >> 4, col = lane_ & 15;
         const int c = nc - 1 - ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
         // ---- operands to the LDS
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int row = row0 + 32 * i, o0 = order_of(d0), o1 = order_of(d0 + 4);
+        const auto put = [&](const Piece<IO>& r, __bf16 (&a)[NS][L][PX], int row) {
+            const int o0 = order_of(d0), o1 = order_of(d0 + 4);
             u32x4 t[NS];
-            auto& qa = group ? lds.k : lds.q;
-            auto& qb = group ? lds.gy : lds.v;
-            piece_terms<IO>(ra[i], t);
+            piece_terms<IO>(r, t);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                *reinterpret_cast<uint2*>(&qa[s][row][o0]) = uint2{t[s][0], t[s][1]};
-                *reinterpret_cast<uint2*>(&qa[s][row][o1]) = uint2{t[s][2], t[s][3]};
+                *reinterpret_cast<uint2*>(&a[s][row][o0]) = uint2{t[s][0], t[s][1]};
+                *reinterpret_cast<uint2*>(&a[s][row][o1]) = uint2{t[s][2], t[s][3]};
             }
-            piece_terms<IO>(rb[i], t);
+        };
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                *reinterpret_cast<uint2*>(&qb[s][row][o0]) = uint2{t[s][0], t[s][1]};
-                *reinterpret_cast<uint2*>(&qb[s][row][o1]) = uint2{t[s][2], t[s][3]};
-            }
-        }
+        for (int i = 0; i < PIECES; ++i) put(ra[i], kind == DQ ? lds.q : kind == DK ? lds.k : lds.v, row0 + 32 * i);
+        if (gy_mine) put(rb[0], lds.gy, gy_row);
+        if (kind != DQ) {
 #pragma unroll
-        for (int s = 0; s < 3; ++s)
+            for (int s = 0; s < 3; ++s)
 #pragma unroll
-            for (int kx = 0; kx < 2; ++kx) {
-                const u32x4 t = held[s][kx];
-                if (group == 0) lds.s[s][w4][kx][lane_] = t;
-                else {
-                    *reinterpret_cast<uint2*>(&lds.x[s][16 * w4 + col][32 * kx + 8 * quarter]) = uint2{t[0], t[1]};
-                    *reinterpret_cast<uint2*>(&lds.x[s][16 * w4 + col][32 * kx + 4 + 8 * quarter]) = uint2{t[2], t[3]};
+                for (int kx = 0; kx < 2; ++kx) {
+                    const u32x4 t = held[s][kx];
+                    if (kind == DK) lds.s[s][w4][kx][lane_] = t;
+                    else {
+                        *reinterpret_cast<uint2*>(&lds.x[s][16 * w4 + col][32 * kx + 8 * quarter]) = uint2{t[0], t[1]};
+                        *reinterpret_cast<uint2*>(&lds.x[s][16 * w4 + col][32 * kx + 4 + 8 * quarter]) = uint2{t[2], t[3]};
+                    }
                 }
-            }
+        }
         lds_barrier();                                    // (orders the LDS alone: the next chunk's rows and this one's results stay on their way)
         if (ci + 1 < nc) fetch(c - 1);
+        else {                                            // (nothing of the last rows is kept)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) ra[i] = Piece<IO>{};
+            rb[0] = Piece<IO>{};
+        }
         typename S::Decays& dec = lds.d[ci & 1];
         typename S::Flows& flows = lds.f[ci & 1];
         const int r0 = 16 * tw + col;                     // this lane's token
@@ -260,21 +278,45 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                 for (int i = 0; i < 4; ++i) o[i] = s == NS - 1 ? (float)t[i] : o[i] + (float)t[i];
             }
         };
-        if (group == 0) {
-            if constexpr (FLOW) {                         // <S0, X>
-                float through = 0.f;
+        // acc += what the tokens t >= s of the chunk give: (a_t . mine) D_ts of each, times c_t
+        const auto gathered = [&](const __bf16 (&a)[NS][L][PX], const bf16x8 (&mine)[2][NS], const __bf16 (&c_)[NS][L][PX], float gh, float gl, f32x4 (&acc)[NT]) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
+            for (int ks = 0; ks < KS; ++ks) {
+                if (2 * ks + 1 < tw) continue;
+                if (32 * ks >= n) break;
+                float pr[8];
 #pragma unroll
-                    for (int s = 0; s < 3; ++s) {
-                        const bf16x4 t = *reinterpret_cast<const bf16x4*>(&lds.x[s][16 * w4 + col][order_of(16 * x) + 8 * quarter]);
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int tt = 2 * ks + hf;
+                    f32x4 m = {0.f, 0.f, 0.f, 0.f};
+                    if (tt >= tw) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) through = fmaf((float)t[i], st[x][i], through);
+                        for (int kx = 0; kx < 2; ++kx) {
+                            bf16x8 f[NS];
+                            row_of(a, 16 * tt + col, kx, f);
+                            m = mma<NP - 1>(m, f, mine[kx]);
+                        }
+                        const f32x4 th = *reinterpret_cast<const f32x4*>(&dec.gh[16 * tt + 4 * quarter]), tl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * tt + 4 * quarter]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = m[i] * (scale * fast_exp2((th[i] - gh) + (tl[i] - gl)));
+                            m[i] = tt > tw || 4 * quarter + i >= col ? x : 0.f;
+                        }
                     }
-                through = wave_sum(through);
-                if (lane_ == 0) flows.through[w4] = through * dec.end;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) pr[4 * hf + i] = m[i];
+                }
+                bf16x8 fp[NP];
+                split8<NP>(pr, fp);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    bf16x8 f[NS];
+                    across(c_, zt0 + j, ks, f);
+                    acc[j] = mma<NP - 1>(acc[j], f, fp);
+                }
             }
-            if (ci + 1 < nc) fetch_state(c - 1);
+        };
+        if (kind == DQ) {
             if (16 * tw < n) {
                 const float gh = dec.gh[r0], gl = dec.gl[r0], dt = dec.dt[r0];
                 bf16x8 fo[2][NS];
@@ -336,6 +378,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                             pf[4 * hf + i] = m[i] * mq[i];
                         }
                     }
+                    __builtin_amdgcn_sched_barrier(0);    // (what is read ahead of its use fills the registers otherwise)
                     bf16x8 fp[NP];
                     split8<NP>(pr, fp);
 #pragma unroll
@@ -344,6 +387,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                         across(lds.k, zt0 + j, ks, fk);
                         acc[j] = mma<NP - 1>(acc[j], fk, fp);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                     if (FLOW && w4 < NT) {                // (the other waves of a 32-token chunk would make the same terms)
                         bf16x8 ff[3];
                         split8<3>(pf, ff);
@@ -364,7 +408,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                         }
                     }
                 }
-                oa.store(acc, t0, r0 < n);
+                so.store(acc, t0, r0 < n);
                 if constexpr (FLOW) {
                     in += __shfl_xor(in, 16);
                     in += __shfl_xor(in, 32);
@@ -379,105 +423,95 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                     if ((index >> 2) < NT) flows.inner[w4][16 * (index >> 2) + 4 * quarter + (index & 3)] = cf;
                 }
             } else if (FLOW && lane_ < L) flows.inner[w4][lane_] = 0.f;
-            if (wave == 0) {
+            forget();
+        } else if (kind == DK) {
+            if constexpr (FLOW) {                         // <S0, X>
+                float through = 0.f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int s = 0; s < 3; ++s) {
+                        const bf16x4 t = *reinterpret_cast<const bf16x4*>(&lds.x[s][16 * w4 + col][order_of(16 * x) + 8 * quarter]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) through = fmaf((float)t[i], st[x][i], through);
+                    }
+                through = wave_sum(through);
+                if (lane_ == 0) flows.through[w4] = through * dec.end;
+            }
+            fetch_state(max(c - 1, 0));
+            if (16 * tw < n) {
+                const float gh = dec.gh[r0], gl = dec.gl[r0], dk = dec.dk[r0];
+                bf16x8 fv[2][NS];
+                row_of(lds.v, r0, 0, fv[0]);
+                row_of(lds.v, r0, 1, fv[1]);
+                f32x4 acc[NT];
+                float out = 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (have) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                        for (int kx = 0; kx < 2; ++kx) {
+                            bf16x8 fx[3];
+#pragma unroll
+                            for (int s = 0; s < 3; ++s) fx[s] = *reinterpret_cast<const bf16x8*>(&lds.x[s][16 * (zt0 + j) + col][kx * 32 + 8 * quarter]);
+                            acc[j] = mma<2>(acc[j], fx, fv[kx]);
+                        }
+                        float k4[4];
+                        if constexpr (FLOW) widen4(lds.k, r0, zt0 + j, k4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            acc[j][i] *= dk;
+                            if constexpr (FLOW) out = fmaf(k4[i], acc[j][i], out);
+                        }
+                    }
+                }
+                gathered(lds.gy, fv, lds.q, gh, gl, acc);
+                so.store(acc, t0, r0 < n);
+                if constexpr (FLOW) {
+                    out += __shfl_xor(out, 16);
+                    out += __shfl_xor(out, 32);
+                    if (quarter == 0) flows.out[w4 / NT][r0] = out;
+                }
+            }
+            have = true;
+            hold();
+            if (wave == LIGHT) {
                 if constexpr (FLOW) {
                     if (ci > 0) put_flows(lds.f[(ci + 1) & 1], t0 + L, min(L, w.s1 - t0 - L));
                 }
                 if (ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
             }
-            if (ci + 1 < nc) hold();
         } else {
             if (16 * tw < n) {
                 const float gh = dec.gh[r0], gl = dec.gl[r0], dk = dec.dk[r0];
-                bf16x8 fk[2][NS], fv[2][NS];
+                bf16x8 fk[2][NS];
+                row_of(lds.k, r0, 0, fk[0]);
+                row_of(lds.k, r0, 1, fk[1]);
+                f32x4 acc[NT];
 #pragma unroll
-                for (int kx = 0; kx < 2; ++kx) {
-                    row_of(lds.k, r0, kx, fk[kx]);
-                    row_of(lds.v, r0, kx, fv[kx]);
-                }
-                f32x4 ak[NT], av[NT];
-                float out = 0.f;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) ak[j] = av[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (have) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         const int x = zt0 + j;
 #pragma unroll
                         for (int kx = 0; kx < 2; ++kx) {
-                            bf16x8 fx[3], fy[NP];
-#pragma unroll
-                            for (int s = 0; s < 3; ++s) fx[s] = *reinterpret_cast<const bf16x8*>(&lds.x[s][16 * x + col][kx * 32 + 8 * quarter]);
+                            bf16x8 fy[NP];
 #pragma unroll
                             for (int s = 0; s < NP; ++s) {
                                 const __bf16* q = &lds.x[s][32 * kx + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
                                 fy[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
                             }
-                            ak[j] = mma<2>(ak[j], fx, fv[kx]);
-                            av[j] = mma<NP - 1>(av[j], fy, fk[kx]);
+                            acc[j] = mma<NP - 1>(acc[j], fy, fk[kx]);
                         }
-                        float k4[4];
-                        if constexpr (FLOW) widen4(lds.k, r0, x, k4);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            ak[j][i] *= dk;
-                            av[j][i] *= dk;
-                            if constexpr (FLOW) out = fmaf(k4[i], ak[j][i], out);
-                        }
+                        for (int i = 0; i < 4; ++i) acc[j][i] *= dk;
                     }
                 }
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    if (2 * ks + 1 < tw) continue;        // tokens t in front of s
-                    if (32 * ks >= n) break;
-                    float pp[8], dp[8];
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        const int tt = 2 * ks + hf;
-                        f32x4 mq = {0.f, 0.f, 0.f, 0.f}, mo = {0.f, 0.f, 0.f, 0.f};
-                        if (tt >= tw) {
-#pragma unroll
-                            for (int kx = 0; kx < 2; ++kx) {
-                                bf16x8 f[NS];
-                                row_of(lds.q, 16 * tt + col, kx, f);
-                                mq = mma<NP - 1>(mq, f, fk[kx]);
-                                row_of(lds.gy, 16 * tt + col, kx, f);
-                                mo = mma<NP - 1>(mo, f, fv[kx]);
-                            }
-                            const f32x4 th = *reinterpret_cast<const f32x4*>(&dec.gh[16 * tt + 4 * quarter]), tl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * tt + 4 * quarter]);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float x = scale * fast_exp2((th[i] - gh) + (tl[i] - gl));
-                                const bool seen = tt > tw || 4 * quarter + i >= col;
-                                mq[i] = seen ? mq[i] * x : 0.f;
-                                mo[i] = seen ? mo[i] * x : 0.f;
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            pp[4 * hf + i] = mq[i];
-                            dp[4 * hf + i] = mo[i];
-                        }
-                    }
-                    bf16x8 fp[NP], fd[NP];
-                    split8<NP>(pp, fp);
-                    split8<NP>(dp, fd);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        bf16x8 f[NS];
-                        across(lds.gy, zt0 + j, ks, f);
-                        av[j] = mma<NP - 1>(av[j], f, fp);
-                        across(lds.q, zt0 + j, ks, f);
-                        ak[j] = mma<NP - 1>(ak[j], f, fd);
-                    }
-                }
-                oa.store(ak, t0, r0 < n);
-                ob.store(av, t0, r0 < n);
-                if constexpr (FLOW) {
-                    out += __shfl_xor(out, 16);
-                    out += __shfl_xor(out, 32);
-                    if (quarter == 0) flows.out[w4 / NT][r0] = out;
-                }
+                gathered(lds.q, fk, lds.gy, gh, gl, acc);
+                so.store(acc, t0, r0 < n);
             }
             // ---- X in front of the chunk
             const float ed = dec.end;
@@ -509,12 +543,12 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
                 }
             }
             have = true;
-            if (ci + 1 < nc) hold();
+            hold();
         }
         lds_barrier();
     }
     if constexpr (FLOW) {
-        if (wave == 0) {
+        if (wave == LIGHT) {
             if (nc > 0) put_flows(lds.f[(nc + 1) & 1], w.s0, min(L, w.s1 - w.s0));
             if (dg_sum) {
 #pragma unroll
@@ -524,7 +558,7 @@ __global__ __launch_bounds__(BWD_THREADS, 2) void decay_bwd_kernel(const BwdPara
         }
     }
 
-    if (p.dstate && w.is_first && group == 1) {
+    if (p.dstate && w.is_first && kind == DV) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
