@@ -257,13 +257,26 @@ struct Gates {
     }
 };
 // x as the sum of n bf16 numbers (two at a time): 16 bits of it with two, all 24 with three
-template <int N>
+// DOT: heads are subtracted by a dot product each, x + (head0, head1) . (-1, 0), instead of two instructions.  The other product is zero but where the other
+// number is no number: for pairs that one sum takes up.
+template <int N, bool DOT = false>
 __device__ __forceinline__ void split_pair(float x0, float x1, unsigned (&t)[N]) {
+    typedef wkv6_detail::bf16x2 pair_t;
+    unsigned lo = 0x0000bf80u, hi = 0xbf800000u;          // (kept opaque: as constants they become an inline operand that stands for another pair)
+    if (DOT) asm("" : "+s"(lo), "+s"(hi));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         t[i] = wkv6_detail::pack_bf16(x0, x1);
-        x0 -= wkv6_detail::bf16_lo(t[i]);
-        x1 -= wkv6_detail::bf16_hi(t[i]);
+        if (i + 1 < N) {
+            if (DOT) {
+                const pair_t h = __builtin_bit_cast(pair_t, t[i]);
+                x0 = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(pair_t, lo), x0, false);
+                x1 = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(pair_t, hi), x1, false);
+            } else {
+                x0 -= wkv6_detail::bf16_lo(t[i]);
+                x1 -= wkv6_detail::bf16_hi(t[i]);
+            }
+        }
     }
 }
 template <int N>
@@ -272,7 +285,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[N]) {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         unsigned o[N];
-        split_pair<N>(x[2 * p], x[2 * p + 1], o);
+        split_pair<N, true>(x[2 * p], x[2 * p + 1], o);
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i][p] = o[i];
     }
