@@ -39,7 +39,7 @@ struct Role {
     float *seg, *seg_decay;                               // [segment][head][tile] a segment's state (first its own, then that in front of it), [segment][head]
     float* anchors;                                       // [chunk][head][tile]: the state in front of each chunk
     long long sx, sz;                                     // strides of the states' contracted and other index
-    int dx, dz, tiles, reverse;                           // (the roles of a launch have the same tiles)
+    int dx, dz, tiles, reverse;                           // (one or two tiles; the roles of a launch have the same)
     float s_in, s_upd;                                    // scale where the state is read; where it is written
 };
 struct Call {                                             // sequences, their cut, and the decays
@@ -67,6 +67,7 @@ struct Place {                                            // a workgroup's segme
     int s0, s1;                                           // the segment's tokens, from the first
     int base;                                             // batch row
     int chunk0;                                           // number of the sequence's first chunk
+    int front, back;                                      // packed: where the first sequence begins, and the last one ends
     bool is_last, is_first, valid;
 };
 __device__ __forceinline__ int offset_at(const Call& p, int n) {
@@ -74,7 +75,7 @@ __device__ __forceinline__ int offset_at(const Call& p, int n) {
     return (int)(v < 0 ? 0 : v > p.T ? p.T : v);
 }
 __device__ __forceinline__ Place sequence_place(const Call& p, int n, int L) {
-    Place w;
+    Place w{};
     w.n = n;
     w.valid = true;
     if (p.nseg) {
@@ -94,24 +95,38 @@ __device__ __forceinline__ Place sequence_place(const Call& p, int n, int L) {
 __device__ __forceinline__ int first_segment(const Call& p, int n, int first) { return p.nseg ? n * p.nseg : first / p.seg_len + n; }
 __device__ __forceinline__ int segment_count(const Call& p, int len) { return max(1, (len + p.seg_len - 1) / p.seg_len); }
 
+// offs: THREADS_ numbers of shared memory (packed sequences: one read of the offsets where they are fewer than the threads).
 template <int THREADS_>
-__device__ __forceinline__ Place find_place(const Call& p, int gid, int L) {
-    int n;
-    if (p.nseg) n = gid / p.nseg;
-    else {
+__device__ __forceinline__ Place find_place(const Call& p, int gid, int L, int* offs) {
+    Place w{};
+    if (p.nseg) {
+        w = sequence_place(p, p.nseg == 1 ? gid : gid / p.nseg, L);
+    } else if (p.N < THREADS_) {
+        const int i = threadIdx.x, o = offset_at(p, min(i, p.N));
+        offs[i] = o;
+        const int seen = __syncthreads_count(i < p.N && o / p.seg_len + i <= gid), n = __builtin_amdgcn_readfirstlane(seen - 1);
+        w.front = __builtin_amdgcn_readfirstlane(offs[0]);
+        w.back = __builtin_amdgcn_readfirstlane(offs[p.N]);
+        if (n >= 0) {
+            w.n = n;
+            w.first = __builtin_amdgcn_readfirstlane(offs[n]);
+            w.len = max(0, __builtin_amdgcn_readfirstlane(offs[n + 1]) - w.first);
+            w.chunk0 = w.first / L + n;
+            w.valid = true;
+        }
+    } else {
         int seen = 0;
         for (int m = 0; m < p.N; m += THREADS_) {
             const int i = m + threadIdx.x;
             seen += __syncthreads_count(i < p.N && offset_at(p, min(i, p.N - 1)) / p.seg_len + i <= gid);
         }
-        n = __builtin_amdgcn_readfirstlane(seen - 1);
+        const int n = __builtin_amdgcn_readfirstlane(seen - 1);
+        if (n >= 0) w = sequence_place(p, n, L);
+        w.front = offset_at(p, 0);
+        w.back = offset_at(p, p.N);
     }
-    if (n < 0) {
-        Place w{};
-        return w;
-    }
-    Place w = sequence_place(p, n, L);
-    const int j = gid - first_segment(p, n, w.first), count = segment_count(p, w.len);
+    if (!w.valid) return w;
+    const int j = gid - first_segment(p, w.n, w.first), count = segment_count(p, w.len);
     w.valid = j >= 0 && j < count;
     w.s0 = j * p.seg_len;
     w.s1 = min(w.len, w.s0 + p.seg_len);
@@ -119,6 +134,10 @@ __device__ __forceinline__ Place find_place(const Call& p, int gid, int L) {
     w.is_last = j == count - 1;
     return w;
 }
+// Workgroups: x: heads, and what varies within one (a power of two); y and z: segments.
+constexpr int GRID_Y = 32768;
+__device__ __forceinline__ int grid_segment() { return blockIdx.y + GRID_Y * blockIdx.z; }
+inline dim3 decay_grid(const Call& p, int within) { return dim3((unsigned)(p.H * within), (unsigned)(p.segs < GRID_Y ? p.segs : GRID_Y), (unsigned)((p.segs + GRID_Y - 1) / GRID_Y)); }
 
 // The eight channels d .. d + 7 of a row: at byte offset `at` of the buffer in one or two loads of 16 bytes where rows come in such pieces (VEC), element by
 // element otherwise; `count` of them exist; `ahead` bytes behind, the same for all lanes.  What does not is asked of an offset outside the buffer and arrives as zero, without a branch: loads behind
@@ -180,7 +199,7 @@ struct Source {
     unsigned at;
     int row, count;
     __device__ __forceinline__ void open(const View& v, int base, int first, int head, int L, bool rev, int row_, int d, int dim) {
-        p = static_cast<const char*>(v.p) + (base * v.sb + (long long)first * v.st + (head / v.share) * v.sh) * (int)sizeof(IO);
+        p = static_cast<const char*>(v.p) + (base * v.sb + (long long)first * v.st + (v.share == 1 ? head : head / v.share) * v.sh) * (int)sizeof(IO);
         pitch = (int)v.st * (int)sizeof(IO);
         keep(p);
         keep(pitch);
@@ -379,8 +398,8 @@ __device__ __forceinline__ int order_of(int d) {
 
 // Packed rows in front of the first sequence and behind the last get zeros, a few from every workgroup of the head and tile.
 template <typename IO>
-__device__ __forceinline__ void clear_outside(const Params& p, const Role& r, int gid, int z, int h) {
-    const int front = offset_at(p, 0), back = offset_at(p, p.N), rows = front + max(0, p.T - back);
+__device__ __forceinline__ void clear_outside(const Params& p, const Role& r, int front, int back, int gid, int z, int h) {
+    const int rows = front + max(0, p.T - back);
     const int d = z * TZ + (threadIdx.x & 63);
     for (int i = gid * 4 + (threadIdx.x >> 6); i < rows; i += p.segs * 4) {
         const long long row = i < front ? i : back + (i - front);
@@ -403,18 +422,17 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     static_assert(PA >= 1 && L * DX % (8 * THREADS) == 0 && L * TZ % (8 * THREADS) == 0, "");
     constexpr bool OUT = S::OUT;
     __shared__ S lds;
+    __shared__ int offs[THREADS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
 
-    // workgroup -> role, tile, head, segment (segments of a head next to each other are on different chiplets; the roles of one share its rows)
+    // a head's tiles, and the roles of a tile, next to each other: they read the same rows
     int id = blockIdx.x;
-    const int ri = id % p.n_roles;
-    id /= p.n_roles;
-    const Role& r = p.role[ri];
-    const int z = id % r.tiles;
-    id /= r.tiles;
-    const int h = id % p.H, gid = id / p.H;
-    if (!p.nseg && OUT) clear_outside<IO>(p, r, gid, z, h);
-    const Place w = find_place<THREADS>(p, gid, L);
+    const Role& r = p.role[id & (p.n_roles - 1)];
+    id >>= p.n_roles - 1;
+    const int z = id & (r.tiles - 1), h = id >> (r.tiles - 1), gid = grid_segment();
+    if (gid >= p.segs) return;
+    const Place w = find_place<THREADS>(p, gid, L, offs);
+    if (OUT && !p.nseg) clear_outside<IO>(p, r, w.front, w.back, gid, z, h);
     if (!w.valid) return;
     if (MODE == STATES && (r.reverse ? w.is_first : w.is_last)) return;    // nothing starts behind it
     const int z0 = z * TZ;
@@ -696,7 +714,7 @@ void launch_mode(const Params& p, int mode, dim3 grid, hipStream_t st) {
 // vec: every row of every role in pieces of 16 bytes
 template <typename IO>
 int launch_decay(const Params& p, int dx, int mode, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)((long long)p.segs * p.H * p.role[0].tiles * p.n_roles));
+    const dim3 grid = decay_grid(p, p.role[0].tiles * p.n_roles);
     if (dx <= 64) vec ? launch_mode<IO, 64, true>(p, mode, grid, st) : launch_mode<IO, 64, false>(p, mode, grid, st);
     else vec ? launch_mode<IO, 128, true>(p, mode, grid, st) : launch_mode<IO, 128, false>(p, mode, grid, st);
     return check_launch("decay_attention");

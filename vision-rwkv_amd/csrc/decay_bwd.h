@@ -57,11 +57,13 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     constexpr int L = S::L, NS = S::NS, NT = L / 16, KS = L / 32, PX = S::PX, NP = NS < 3 ? 2 : 3;
     constexpr int PIECES = L * 8 / 256;                   // a thread's of the tensor that its kind stages: q, k or v; the first two kinds take half of gy besides
     __shared__ S lds;
+    __shared__ int offs[BWD_THREADS];
     const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kind = wave >> 2, w4 = wave & 3;
-    // tiles of one head next to each other: they read the same rows
-    const int tile = blockIdx.x % (p.tk * p.tv), h = blockIdx.x / (p.tk * p.tv) % p.H, gid = blockIdx.x / (p.tk * p.tv) / p.H;
-    const int ik = tile % p.tk, iv = tile / p.tk, k0 = 64 * ik, v0 = 64 * iv;
+    // a head's tiles next to each other: they read the same rows
+    const int shift = (p.tk - 1) + (p.tv - 1), tile = blockIdx.x & ((1 << shift) - 1), h = blockIdx.x >> shift, gid = grid_segment();
+    if (gid >= p.segs) return;
+    const int ik = tile & (p.tk - 1), iv = tile >> (p.tk - 1), k0 = 64 * ik, v0 = 64 * iv;
     const auto part = [&](OutView v, int i, int D) {
         if (v.p && v.f32) v.p = static_cast<float*>(v.p) + i * p.rows * p.H * D;
         return v;
@@ -70,8 +72,9 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     float* const dg_part = FLOW && p.dg ? p.dg + tile * p.rows * p.H : nullptr;
     double* const dg_sum = FLOW && p.dg_sums ? p.dg_sums + ((long long)gid * p.tk * p.tv + tile) * p.H + h : nullptr;
 
+    const Place w = find_place<BWD_THREADS>(p, gid, L, offs);
     if (!p.nseg) {                                        // packed rows in front of the first sequence and behind the last: no gradient
-        const int front = offset_at(p, 0), back = offset_at(p, p.N), rows = front + max(0, p.T - back);
+        const int front = w.front, back = w.back, rows = front + max(0, p.T - back);
         for (int i = gid * 12 + wave; i < rows; i += p.segs * 12) {
             const long long row = i < front ? i : back + (i - front);
             const OutView* const outs[3] = {&out_q, &out_k, &out_v};
@@ -88,7 +91,6 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
             if (dg_part && lane == 0) dg_part[row * p.H + h] = 0.f;
         }
     }
-    const Place w = find_place<BWD_THREADS>(p, gid, L);
     if (!w.valid) {
         if (dg_sum && tid == 0) *dg_sum = 0.;
         return;
@@ -576,7 +578,7 @@ extern template int launch_decay_bwd<__half>(const BwdParams&, bool, hipStream_t
 
 template <typename IO>
 int launch_decay_bwd(const BwdParams& p, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)((long long)p.segs * p.H * p.tk * p.tv)), block(BWD_THREADS);
+    const dim3 grid = decay_grid(p, p.tk * p.tv), block(BWD_THREADS);
     if (p.dg || p.dg_sums) {
         if (vec) hipLaunchKernelGGL((decay_bwd_kernel<IO, true, true>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((decay_bwd_kernel<IO, true, false>), grid, block, 0, st, p);
