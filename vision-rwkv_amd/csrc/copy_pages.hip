@@ -2,14 +2,14 @@
 // Bound by the pages' bytes.  An entry whose source no other entry overwrites and whose target no other reads goes by itself ("free"); the others
 // ("tied") go strip by strip: a workgroup reads its strip of all their sources into registers before it writes one of their targets, so the strips need
 // nothing of each other and no page is copied twice.  Two workgroups a compute unit: one reads while the other writes.  (Strips through the LDS, one
-// workgroup: 103 us for 690 of 1024 pages of 196 KB; so @TIED@.)
+// workgroup: 103 us for 690 of 1024 pages of 196 KB; so 74.)
 #include "vrwkv_common.h"
 #include <algorithm>
 
 namespace vrwkv {
 namespace {
 
-constexpr int THREADS = 512, MAX_LIST = 4096, SMALL_LIST = 256, HELD = 16;     // HELD: units that a thread holds
+constexpr int THREADS = 512, MAX_LIST = 4096, SMALL_LIST = 256;
 enum { SKIP = 0, FREE = 1, TIED = 2 };
 
 struct PageParams {
@@ -45,9 +45,10 @@ __global__ __launch_bounds__(256) void plan_kernel(const PageParams p) {
     if (lane == 0) p.plan[i] = entry_kind(entry_good(p, from, to), flags);
 }
 
-// U: 16, 4, 2 or 1 bytes at a time
-template <typename U>
-__global__ __launch_bounds__(THREADS, 4) void copy_kernel(const PageParams p) {
+// U: 16, 4, 2 or 1 bytes at a time.  HELD: units that a thread holds: the more, the wider the strips (690 pages of 196 KB: 92 us with 16, strips of 128 bytes; 74 with 24 and
+// strips of 256; 174 with 48 and 512, one workgroup a compute unit), the fewer, the sooner a short list's few strips are begun.
+template <typename U, int HELD>
+__global__ __launch_bounds__(THREADS, HELD <= 16 ? 4 : 2) void copy_kernel(const PageParams p) {
     __shared__ int sfrom[MAX_LIST], sto[MAX_LIST];        // tied entries
     __shared__ long long lfrom[SMALL_LIST], lto[SMALL_LIST];
     __shared__ int count;
@@ -70,12 +71,12 @@ __global__ __launch_bounds__(THREADS, 4) void copy_kernel(const PageParams p) {
         U* dst = reinterpret_cast<U*>(p.pool + to * p.stride);
         const long long u0 = (long long)s * p.held * THREADS + tid;
 #pragma unroll
-        for (int k = 0; k < HELD; ++k) {
+        for (int k = 0; k < 16; ++k) {
             t[k] = U{};
             if (k < p.held && from >= 0 && u0 + k * THREADS < units) t[k] = src[u0 + k * THREADS];
         }
 #pragma unroll
-        for (int k = 0; k < HELD; ++k)
+        for (int k = 0; k < 16; ++k)
             if (k < p.held && u0 + k * THREADS < units) dst[u0 + k * THREADS] = t[k];
         return;
     }
@@ -137,12 +138,18 @@ __global__ __launch_bounds__(THREADS, 4) void copy_kernel(const PageParams p) {
 template <typename U>
 void launch_copies(PageParams p, hipStream_t st) {
     const long long units = p.bytes / (long long)sizeof(U);
-    p.held = HELD;
+    const int held = p.M > SMALL_LIST ? 24 : 16;
+    p.held = 16;
     while (p.held > 1 && p.M * ((units + (long long)p.held * THREADS - 1) / (p.held * THREADS)) < 2048) p.held /= 2;
     p.strips = (int)((units + (long long)p.held * THREADS - 1) / (p.held * THREADS));
     p.free_blocks = p.M * p.strips;
-    const int tied_blocks = p.same && p.M > 1 ? 2 * device_cus() : 0;
-    hipLaunchKernelGGL((copy_kernel<U>), dim3(p.free_blocks + tied_blocks), dim3(THREADS), 0, st, p);
+    // (as many as there are strips if every entry is tied)
+    long long width = 1;
+    while (2 * width * p.M <= held * THREADS && 2 * width * (int)sizeof(U) <= 1024) width *= 2;
+    const int tied_blocks = p.same && p.M > 1 ? (int)std::min<long long>(2 * device_cus(), (units + width - 1) / width) : 0;
+    const dim3 grid(p.free_blocks + tied_blocks), block(THREADS);
+    if (held == 24) hipLaunchKernelGGL((copy_kernel<U, 24>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((copy_kernel<U, 16>), grid, block, 0, st, p);
 }
 
 }  // namespace
