@@ -34,15 +34,14 @@ __device__ __forceinline__ int entry_flags(const PageParams& p, int i, long long
 }
 __device__ __forceinline__ int entry_kind(bool good, int flags) { return !good || (flags & 1) ? SKIP : flags & 2 ? TIED : FREE; }
 
-// A wave for each entry.
+// A workgroup for each entry.
 __global__ __launch_bounds__(256) void plan_kernel(const PageParams p) {
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= p.M) return;
+    const int i = blockIdx.x;
     const long long from = index_at(p.from, p.from64, i), to = index_at(p.to, p.to64, i);
     int flags = 0;
-    for (int j = lane; j < p.M; j += 64) flags |= entry_flags(p, i, from, to, j, index_at(p.from, p.from64, j), index_at(p.to, p.to64, j));
-    flags = (__any(flags & 1) ? 1 : 0) | (__any(flags & 2) ? 2 : 0);
-    if (lane == 0) p.plan[i] = entry_kind(entry_good(p, from, to), flags);
+    for (int j = threadIdx.x; j < p.M; j += 256) flags |= entry_flags(p, i, from, to, j, index_at(p.from, p.from64, j), index_at(p.to, p.to64, j));
+    const int f1 = __syncthreads_or(flags & 1), f2 = __syncthreads_or(flags & 2);
+    if (threadIdx.x == 0) p.plan[i] = entry_kind(entry_good(p, from, to), (f1 ? 1 : 0) | (f2 ? 2 : 0));
 }
 
 // U: 16, 4, 2 or 1 bytes at a time.  HELD: units that a thread holds: the more, the wider the strips (690 pages of 196 KB: 92 us with 16, strips of 128 bytes; 74 with 24 and
@@ -176,7 +175,7 @@ extern "C" int vrwkv_copy_pages(void* pool, long long stride, int P, const void*
     if (!same && a < b + b_end && b < a + a_end) { set_error("%s: the source overlaps the pool", who); return VRWKV_INVALID_ARG; }
     PageParams p{static_cast<char*>(pool), b, from, to, M > SMALL_LIST ? static_cast<int*>(workspace) : nullptr, stride, source_stride, page_bytes, from64, to64, M, P, source_P, same, 0, 0, 0};
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    if (p.plan) hipLaunchKernelGGL(plan_kernel, dim3((M + 3) / 4), dim3(256), 0, st, p);
+    if (p.plan) hipLaunchKernelGGL(plan_kernel, dim3(M), dim3(256), 0, st, p);
     const size_t bits = (size_t)pool | (size_t)source | (size_t)stride | (size_t)source_stride | (size_t)page_bytes;
     if (!(bits & 15)) launch_copies<uint4>(p, st);
     else if (!(bits & 3)) launch_copies<unsigned>(p, st);

@@ -24,14 +24,20 @@ __device__ __forceinline__ long long slot_of(const StepParams& p, int n) {
     return p.slots64 ? static_cast<const long long*>(p.slots)[n] : (long long)static_cast<const int*>(p.slots)[n];
 }
 
+constexpr int GRID_Y = 32768;
+__device__ __forceinline__ float gate_at(const StepParams& p, long long i) {
+    return p.g_dtype == VRWKV_F32 ? static_cast<const float*>(p.g)[i] : p.g_dtype == VRWKV_BF16 ? to_f32(static_cast<const __hip_bfloat16*>(p.g)[i]) : to_f32(static_cast<const __half*>(p.g)[i]);
+}
+
 // NX: sixteenths of the rows of a state
 template <typename IO, int NX>
 __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
     __shared__ f32x4 red[4][16];
     __shared__ int found[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cg = tid & 15, rg = tid >> 4;
-    const int tiles = (p.Dv + COLS - 1) / COLS;
-    const int z = blockIdx.x % tiles, h = blockIdx.x / tiles % p.H, n0 = blockIdx.x / tiles / p.H;
+    const int two = p.Dv > COLS ? 1 : 0;                  // tiles of a head next to each other
+    const int z = blockIdx.x & two, h = blockIdx.x >> two, n0 = blockIdx.y + GRID_Y * blockIdx.z;
+    if (n0 >= p.N) return;
     const int d = z * COLS + 4 * cg;
     const long long slot = slot_of(p, n0);
     const bool known = slot >= 0 && slot < p.P;
@@ -50,6 +56,24 @@ __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
                     if (d + c < p.Dv) S[i][c] = r[c];
         }
     }
+    // a token's numbers: fetched with the page, before anything is waited for
+    float kk[NX], qq[NX], dec;
+    f32x4 vv;
+    const auto token = [&](int n) {
+        const IO* q = static_cast<const IO*>(p.q) + n * p.q_sn + (h / p.share_q) * p.q_sh;
+        const IO* k = static_cast<const IO*>(p.k) + n * p.k_sn + (h / p.share_k) * p.k_sh;
+        const IO* v = static_cast<const IO*>(p.v) + n * p.v_sn + (h / p.share_v) * p.v_sh;
+        dec = gate_at(p, n * p.g_sn + h * p.g_sh);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vv[c] = d + c < p.Dv ? to_f32(v[d + c]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+            const int x = rg + 16 * i;
+            kk[i] = x < p.Dk ? to_f32(k[x]) : 0.f;
+            qq[i] = x < p.Dk ? to_f32(q[x]) : 0.f;
+        }
+    };
+    token(n0);
     // the next row behind `after` with this slot, N if none
     const auto next_row = [&](int after) {
         int best = p.N;
@@ -73,30 +97,16 @@ __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
         }
     }
     for (;;) {
-        const IO* q = static_cast<const IO*>(p.q) + n * p.q_sn + (h / p.share_q) * p.q_sh;
-        const IO* k = static_cast<const IO*>(p.k) + n * p.k_sn + (h / p.share_k) * p.k_sh;
-        const IO* v = static_cast<const IO*>(p.v) + n * p.v_sn + (h / p.share_v) * p.v_sh;
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        const float e = expf(dec);
         if (known) {
-            const long long gi = n * p.g_sn + h * p.g_sh;
-            const float g = p.g_dtype == VRWKV_F32 ? static_cast<const float*>(p.g)[gi]
-                          : p.g_dtype == VRWKV_BF16 ? to_f32(static_cast<const __hip_bfloat16*>(p.g)[gi]) : to_f32(static_cast<const __half*>(p.g)[gi]);
-            const float dec = expf(g);
-            f32x4 vv;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) vv[c] = d + c < p.Dv ? to_f32(v[d + c]) : 0.f;
+            for (int i = 0; i < NX; ++i)
 #pragma unroll
-            for (int i = 0; i < NX; ++i) {
-                const int x = rg + 16 * i;
-                if (x < p.Dk) {
-                    const float kk = to_f32(k[x]), qq = to_f32(q[x]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        S[i][c] = fmaf(S[i][c], dec, kk * vv[c]);
-                        y[c] = fmaf(qq, S[i][c], y[c]);
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    S[i][c] = fmaf(S[i][c], e, kk[i] * vv[c]);
+                    y[c] = fmaf(qq[i], S[i][c], y[c]);
                 }
-            }
         }
         if (next >= p.N && known) {
 #pragma unroll
@@ -127,14 +137,14 @@ __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
         if (next >= p.N) break;
         n = next;
         next = next_row(n);
+        token(n);
         __syncthreads();
     }
 }
 
 template <typename IO>
 int launch_step(const StepParams& p, hipStream_t st) {
-    const int tiles = (p.Dv + COLS - 1) / COLS;
-    const dim3 grid((unsigned)((long long)p.N * p.H * tiles)), block(THREADS);
+    const dim3 grid((unsigned)(p.H * (p.Dv > COLS ? 2 : 1)), (unsigned)std::min(p.N, GRID_Y), (unsigned)((p.N + GRID_Y - 1) / GRID_Y)), block(THREADS);
     if (p.Dk <= 64) hipLaunchKernelGGL((step_kernel<IO, 4>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((step_kernel<IO, 8>), grid, block, 0, st, p);
     return check_launch("vrwkv_decay_step");
