@@ -631,7 +631,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 
         // ---- the state behind the chunk
         {
-            if constexpr (MODE == CHUNKS) {
+            if (MODE == CHUNKS && have) {                 // (zeros in front of a first chunk are not kept)
 #pragma unroll
                 for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(anchors + c * anchor_step + x * 1024) = st[x];
             }

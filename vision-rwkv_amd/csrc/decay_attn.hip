@@ -373,7 +373,7 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     }
     p.n_roles = 1;
     p.role[0] = b.s;
-    if ((s = launch(p, a.dtype, b.dxv, CHUNKS, st)) != VRWKV_OK) return s;
+    if ((a.state || a.T > chunk_of(a.dtype)) && (s = launch(p, a.dtype, b.dxv, CHUNKS, st)) != VRWKV_OK) return s;
     BwdParams t = common<BwdParams>(a, b.seg_len);
     t.q = q;
     t.k = k;
@@ -390,6 +390,7 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     t.dstate = a.dstate;
     t.Dk = a.Dk;
     t.Dv = a.Dv;
+    t.begun = a.state != nullptr;
     t.tk = b.tk;
     t.tv = b.tv;
     const bool vec = in_pieces(q, a.Dk, a.dtype) && in_pieces(k, a.Dk, a.dtype) && in_pieces(v, a.Dv, a.dtype) && in_pieces(gy, a.Dv, a.dtype) && in_pieces(t.dq, a.Dk) && in_pieces(t.dk, a.Dk) &&

@@ -33,6 +33,7 @@ struct BwdParams : Call {
     const float* glast;                                   // gradients of the states behind the last tokens, or null
     float* dstate;
     int Dk, Dv, tk, tv;                                   // channels; tiles of 64
+    int begun;                                            // there are states in front of the first tokens
 };
 
 template <typename IO>
@@ -121,9 +122,11 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         sb.load(rb, t0, n, false);
         if (wave == LIGHT) rg = gates.fetch(t0, lane, lane < n);
     };
+    const auto begun = [&](int c) { return c > 0 || !w.is_first || p.begun; };
     const auto fetch_state = [&](int c) {
+        const bool there = begun(c);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) st[x] = *reinterpret_cast<const f32x4*>(chunks + c * chunk_step + x * 1024);
+        for (int x = 0; x < 4; ++x) st[x] = !there ? f32x4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const f32x4*>(chunks + c * chunk_step + x * 1024);
     };
     const auto hold = [&]() {
 #pragma unroll
@@ -329,21 +332,24 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
 #pragma unroll
                 for (int j = 0; j < (FLOW ? NT : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (begun(c)) {
 #pragma unroll
-                    for (int kx = 0; kx < 2; ++kx) {
-                        bf16x8 fs[3];
+                    for (int j = 0; j < NT; ++j) {
 #pragma unroll
-                        for (int s = 0; s < 3; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane_]);
-                        acc[j] = mma<2>(acc[j], fs, fo[kx]);
-                    }
-                    float q4[4];
-                    if constexpr (FLOW) widen4(lds.q, r0, zt0 + j, q4);
+                        for (int kx = 0; kx < 2; ++kx) {
+                            bf16x8 fs[3];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        acc[j][i] *= dt;
-                        if constexpr (FLOW) in = fmaf(q4[i], acc[j][i], in);
+                            for (int s = 0; s < 3; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane_]);
+                            acc[j] = mma<2>(acc[j], fs, fo[kx]);
+                        }
+                        float q4[4];
+                        if constexpr (FLOW) widen4(lds.q, r0, zt0 + j, q4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            acc[j][i] *= dt;
+                            if constexpr (FLOW) in = fmaf(q4[i], acc[j][i], in);
+                        }
                     }
                 }
 #pragma unroll
