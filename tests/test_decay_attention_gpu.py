@@ -438,6 +438,137 @@ def test_on_another_stream_and_twice_at_once():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [255, 256, 800])
+def test_many_short_sequences(N):
+    """More sequences than a workgroup reads offsets at once; most of a token or none."""
+    lens = np.random.default_rng(N).integers(0, 4, N)
+    lens[N // 2] = 70
+    offsets = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    q, k, v, g, S = make(1, offsets[-1], 2, 2, 2, 2, 8, 8, "fp32", state=N)
+    check_all(q, k, v, g, S, "fp32", offsets=offsets)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_the_same_without_the_host_module(dtype, monkeypatch):
+    """Through the Python classes: the same kernels, bit for bit."""
+    q, k, v, g, S = make(2, 150, 4, 2, 1, 4, 64, 80, dtype, state=2)
+    gen = torch.Generator(DEV).manual_seed(2)
+    gy, gl = torch.randn(2, 150, 4, 80, generator=gen, device=DEV).to(DT[dtype]), torch.randn(2, 4, 64, 80, generator=gen, device=DEV)
+    pool0 = torch.randn(5, 4, 64, 80, generator=gen, device=DEV)
+
+    def run():
+        ts = [t.clone().requires_grad_() for t in (q, k, v, g, S)]
+        y, last = vr.decay_attention(*ts[:4], scale=0.5, state=ts[4], return_state=True)
+        grads = torch.autograd.grad((y, last), ts, (gy, gl))
+        off = torch.tensor([0, 40, 150], device=DEV)
+        with torch.no_grad():
+            packed = vr.decay_attention(q[:1], k[:1], v[:1], g[:1], offsets=off)
+            pool = pool0.clone()
+            s = vr.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], pool, torch.tensor([3, 1], device=DEV))
+            vr.copy_states(pool, torch.tensor([3, 0], device=DEV), torch.tensor([0, 3], device=DEV))
+        return [y, last, *grads, packed, s, pool]
+    a = run()
+    monkeypatch.setattr(vr._lib, "_host", vr._lib._NoHost)
+    for x, y in zip(a, run()):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_hooks_on_saved_tensors_and_gradients_in_batches():
+    q, k, v, g, S = make(1, 100, 2, 2, 2, 2, 64, 64, "bf16", state=1)
+    ts = [t.clone().requires_grad_() for t in (q, k, v, g, S)]
+    y = vr.decay_attention(*ts[:4], state=ts[4])
+    want = torch.autograd.grad(y, ts, torch.ones_like(y))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(DEV)):
+        y = vr.decay_attention(*ts[:4], state=ts[4])
+    for a, b in zip(torch.autograd.grad(y, ts, torch.ones_like(y)), want):
+        assert torch.equal(a, b)
+    y = vr.decay_attention(*ts[:4], state=ts[4])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, ts, torch.ones(2, *y.shape, device=DEV, dtype=y.dtype), is_grads_batched=True)
+
+
+@pytest.mark.gpu
+def test_inside_a_compiled_program():
+    """The calls are left as they are."""
+    q, k, v, g, S = make(1, 70, 2, 2, 2, 2, 64, 64, "fp32", state=1)
+
+    def layer(q, k, v, g, S):
+        y, last = vr.decay_attention(q * 2, k, v, g, state=S, return_state=True)
+        return y + 1, last
+
+    def token(q, pool):
+        y = vr.decay_attention_step(q, q, q, g[:, 0], pool)
+        return y, vr.copy_states(pool, torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV))
+    for f, args in ((layer, (q, k, v, g, S)), (token, (q[:, 0], S))):
+        with torch.no_grad():
+            want = f(*(t.clone() for t in args))
+            got = torch.compile(f, backend="eager")(*(t.clone() for t in args))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    ts = [t.clone().requires_grad_() for t in (q, k, v, g, S)]
+    want = torch.autograd.grad(layer(*ts)[0].sum(), ts)
+    for a, b in zip(torch.autograd.grad(torch.compile(layer, backend="eager")(*ts)[0].sum(), ts), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_the_same_bits_twice():
+    for dtype, T, offsets in (("bf16", 900, None), ("fp32", 300, None), ("bf16", 900, [0, 500, 510, 900])):
+        q, k, v, g, S = make(1, T, 3, 1, 3, 3, 64, 64, dtype, g="head", state=3 if offsets else 1)
+        off = torch.tensor(offsets, device=DEV) if offsets else None
+        def run():
+            ts = [t.clone().requires_grad_() for t in (q, k, v, g, S)]
+            y, last = vr.decay_attention(*ts[:4], state=ts[4], offsets=off, return_state=True)
+            return [y, last, *torch.autograd.grad((y, last), ts, (torch.ones_like(y), torch.ones_like(last)))]
+        for a, b in zip(run(), run()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_hundred_thousand_tokens():
+    """As two halves, the second going on from the first's state.  Bound: both sides are within that of compare(), whose absolute sums are at most
+    64 max|q| max|k| max|v| (tokens that a decay of 0.03 keeps: 1 / 0.03)."""
+    T, D = 100_000, 16
+    q, k, v, _, _ = make(1, T, 2, 2, 2, 2, D, D, "fp32", seed=4)
+    g = torch.full((2,), -0.03, device=DEV)
+    y, last = vr.decay_attention(q, k, v, g, scale=0.25, return_state=True)
+    h = T // 2 + 13
+    a, mid = vr.decay_attention(q[:, :h], k[:, :h], v[:, :h], g, scale=0.25, return_state=True)
+    b, end = vr.decay_attention(q[:, h:], k[:, h:], v[:, h:], g, scale=0.25, state=mid, return_state=True)
+    bound = 2 * (D + D + 128) * 2.0 ** -24 * 0.25 * D * (1 / 0.03) * q.abs().max() * k.abs().max() * v.abs().max()
+    assert (torch.cat([a, b], 1) - y).abs().max() <= bound and (end - last).abs().max() <= bound
+
+
+@pytest.mark.gpu
+def test_strides_and_pages_beyond_32_bits():
+    """A batch whose rows, and pools whose pages, lie 2^31 and more elements apart."""
+    far = (1 << 31) + 64
+    big = torch.empty(far + 4096, dtype=torch.bfloat16, device=DEV)
+    q, k, v, g, S = make(2, 40, 1, 1, 1, 1, 64, 64, "bf16", state=2)
+    views = []
+    for t, at in ((q, 0),):
+        w = big.as_strided(t.shape, (far, 64, 64, 1), at)
+        w.copy_(t)
+        views.append(w)
+    a = vr.decay_attention(q, k, v, g, state=S, return_state=True)
+    b = vr.decay_attention(views[0], k, v, g, state=S, return_state=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    del big, views, w
+    torch.cuda.empty_cache()
+    big = torch.empty(far + 8192, device=DEV)
+    pool = big.as_strided((2, 1, 64, 64), (far, 4096, 64, 1))
+    pool.copy_(S)
+    dense = S.clone()
+    slots = torch.tensor([1, 0], device=DEV)
+    ys = [vr.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], p, slots) for p in (pool, dense)]
+    assert torch.equal(*ys) and torch.equal(pool, dense)
+    vr.copy_states(pool, torch.tensor([1, 0], device=DEV), torch.tensor([0, 1], device=DEV))
+    assert torch.equal(pool, dense.flip(0))
+
+
+@pytest.mark.gpu
 def test_nothing_in_it():
     r = lambda *s: torch.randn(*s, device=DEV, requires_grad=True)
     for B, T in ((0, 5), (2, 0)):

@@ -12,6 +12,11 @@ from . import _lib
 from .ops import _DT, _on, _stream_ptr, batched_cotangent
 
 
+def _eager(f):
+    """f as a call that a compiled program makes and does not look into: its kernels take memory, not traces."""
+    return torch.compiler.disable(f)
+
+
 def _rows(t):
     """t as the kernels read it: any strides, but the channels of a head side by side and tokens less than 2^22 elements apart."""
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() == 3 or t.stride(1) < 1 << 22) else t.contiguous()
@@ -138,10 +143,11 @@ def decay_attention(q, k, v, g, scale=1.0, state=None, offsets=None, return_stat
     offsets (N + 1,), int32 or int64 on the device, ascending from 0 to T: N sequences packed behind each other in one row (B = 1), sequence n the tokens
     offsets[n] to offsets[n + 1] (an empty one leaves its state as it is); y of rows behind the last sequence is zero, and so are their gradients.
     Gradients for q, k, v, g and state, sums in fp32 (those of (H,) decays in 64 bits), rounded once to their inputs' types; no second ones."""
-    if not torch.compiler.is_compiling():
-        out = _lib.host().decay_attention(q, k, v, g, scale, state, offsets, return_state)
-        if out is not None:
-            return out
+    if torch.compiler.is_compiling():
+        return _eager(decay_attention)(q, k, v, g, scale, state, offsets, return_state)
+    out = _lib.host().decay_attention(q, k, v, g, scale, state, offsets, return_state)
+    if out is not None:
+        return out
     H, Dk, Dv = _check_heads(q, k, v, g, 2)
     N = q.shape[0]
     if offsets is not None:
@@ -164,10 +170,11 @@ def decay_attention_step(q, k, v, g, pool, slots=None, scale=1.0):
     page, 0, 1, .. without.  Rows that name the same page are tokens behind each other, in their order.  A row of slot -1 (a place of the batch that is not
     taken) gives zeros and touches nothing, one of any other slot outside the pool NaN.  Pages may lie at any distance (pool[:, layer] of a pool for all
     layers), each contiguous.  Forward only."""
-    if not torch.compiler.is_compiling():
-        y = _lib.host().decay_step(q, k, v, g, pool, slots, scale)
-        if y is not None:
-            return y
+    if torch.compiler.is_compiling():
+        return _eager(decay_attention_step)(q, k, v, g, pool, slots, scale)
+    y = _lib.host().decay_step(q, k, v, g, pool, slots, scale)
+    if y is not None:
+        return y
     H, Dk, Dv = _check_heads(q, k, v, g, 1)
     N = q.shape[0]
     _check(pool, "pool", q)
@@ -237,7 +244,9 @@ def copy_states(pool, src, dst, source=None):
     from another pool or out to one.  src -1 clears the page, dst -1 is a place of the list that is not taken; of several entries with the same dst the
     last counts.  src, dst: vectors of up to 4096 int32 or int64, on the device -- where entries outside the pools are left out -- or on the host, where
     they are refused.  Pools of any type whose pages are contiguous, at any distance; a source is the pool or does not overlap it."""
-    if not torch.compiler.is_compiling() and _lib.host().copy_pages(pool, src, dst, source):
+    if torch.compiler.is_compiling():
+        return _eager(copy_states)(pool, src, dst, source)
+    if _lib.host().copy_pages(pool, src, dst, source):
         return pool
     _check(pool, "pool")
     source = pool if source is None else source
