@@ -298,13 +298,13 @@ __device__ __forceinline__ void split_pair(float x0, float x1, unsigned (&t)[N])
         }
     }
 }
-template <int N>
+template <int N, bool DOT = true>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[N]) {
     u32x4 w[N];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         unsigned o[N];
-        split_pair<N, true>(x[2 * p], x[2 * p + 1], o);
+        split_pair<N, DOT>(x[2 * p], x[2 * p + 1], o);
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i][p] = o[i];
     }
@@ -327,6 +327,16 @@ __device__ __forceinline__ void piece_terms(const Piece<IO>& r, u32x4 (&t)[in_te
 #pragma unroll
             for (int i = 0; i < NS; ++i) t[i][p] = o[i];
         }
+    }
+}
+
+template <typename IO>
+__device__ __forceinline__ void widen_piece(const Piece<IO>& r, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (std::is_same<IO, float>::value) x[e] = __builtin_bit_cast(float, r.w[e]);
+        else if constexpr (std::is_same<IO, __half>::value) x[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)(r.w[e / 2] >> (16 * (e & 1))));
+        else x[e] = __builtin_bit_cast(float, e & 1 ? r.w[e / 2] & 0xffff0000u : r.w[e / 2] << 16);
     }
 }
 
@@ -381,8 +391,10 @@ struct Lds {
     static constexpr int PX = DX + 8, PZ = TZ + 8;        // row pitches: 16 rows of a fragment on different banks
     static constexpr bool OUT = MODE == PLAIN;
     __bf16 a[OUT ? NS : 1][OUT ? L : 1][PX];   // channels in the order of the state's fragments
-    __bf16 b[NS][L][PX];
-    __bf16 c[NS][L][PZ];
+    __bf16 b[NS][L][PX];                                  // (as they lie where there are no outputs: read across the rows alone, with fewer bank conflicts)
+    // c with its decays to the chunk's end, where it is wanted with them alone and has more terms than one: scaled before it is split, not put together to be scaled
+    static constexpr bool SCALED = !OUT && NS > 1;
+    __bf16 c[SCALED ? 3 : NS][L][PZ];
     u32x4 s[OUT ? NP : 1][4][OUT ? DX / 32 : 1][64];   // the state's terms, a lane's fragment side by side
     struct Decays {
         float gh[L], gl[L], dt[L], dk[L];                 // G in powers of two, head and tail; exp(G); exp(G_end - G)
@@ -510,6 +522,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         if (MODE == STATES) seg_log += (float)end;
     };
     if (nc > 0 && wave == 0) put_decays(lds.d[0]);
+    if (S::SCALED) lds_barrier();                         // (c is scaled with them)
     for (int ci = 0; ci < nc; ++ci) {
         // (what follows from the lane is worked out anew for each chunk: kept over the loop it fills the registers, masks for every tile among it)
         int lane_ = lane;
@@ -532,17 +545,31 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
             piece_terms<IO>(rb[i], t);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                *reinterpret_cast<uint2*>(&lds.b[s][row][o0]) = uint2{t[s][0], t[s][1]};
-                *reinterpret_cast<uint2*>(&lds.b[s][row][o1]) = uint2{t[s][2], t[s][3]};
+                if constexpr (OUT) {
+                    *reinterpret_cast<uint2*>(&lds.b[s][row][o0]) = uint2{t[s][0], t[s][1]};
+                    *reinterpret_cast<uint2*>(&lds.b[s][row][o1]) = uint2{t[s][2], t[s][3]};
+                } else *reinterpret_cast<u32x4*>(&lds.b[s][row][dxo]) = t[s];
             }
         }
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
             const int row = rowz + STEPZ * i, d = dzo;
-            u32x4 t[NS];
-            piece_terms<IO>(rc[i], t);
+            if constexpr (S::SCALED) {
+                const float f = lds.d[ci & 1].dk[row] * s_upd;
+                float x8[8];
+                widen_piece<IO>(rc[i], x8);
 #pragma unroll
-            for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.c[s][row][d]) = t[s];
+                for (int e = 0; e < 8; ++e) x8[e] *= f;
+                bf16x8 t[3];
+                split8<3, false>(x8, t);
+#pragma unroll
+                for (int s = 0; s < 3; ++s) *reinterpret_cast<bf16x8*>(&lds.c[s][row][d]) = t[s];
+            } else {
+                u32x4 t[NS];
+                piece_terms<IO>(rc[i], t);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.c[s][row][d]) = t[s];
+            }
         }
         if constexpr (OUT) {
             if (have) {
@@ -644,30 +671,38 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (32 * ks >= n) break;
-                float x8[8];
-                const f32x4 d0 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 4 * quarter]), d1 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 16 + 4 * quarter]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x8[i] = 0.f;
-#pragma unroll
-                for (int s = NS - 1; s >= 0; --s) {
-                    const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * wave + 4 * (col & 3)];
-                    const bf16x8 f = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x8[i] += (float)f[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x8[i] *= d0[i] * s_upd;
-                    x8[4 + i] *= d1[i] * s_upd;
-                }
                 bf16x8 fv[3];
-                split8<3>(x8, fv);
+                if constexpr (S::SCALED) {
+#pragma unroll
+                    for (int s = 0; s < 3; ++s) {
+                        const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * wave + 4 * (col & 3)];
+                        fv[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
+                    }
+                } else {
+                    float x8[8];
+                    const f32x4 d0 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 4 * quarter]), d1 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 16 + 4 * quarter]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x8[i] = 0.f;
+#pragma unroll
+                    for (int s = NS - 1; s >= 0; --s) {
+                        const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * wave + 4 * (col & 3)];
+                        const bf16x8 f = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x8[i] += (float)f[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x8[i] *= d0[i] * s_upd;
+                        x8[4 + i] *= d1[i] * s_upd;
+                    }
+                    split8<3>(x8, fv);
+                }
 #pragma unroll
                 for (int x = 0; x < NX; ++x) {
                     bf16x8 fk[NS];
 #pragma unroll
                     for (int s = 0; s < NS; ++s) {
-                        const __bf16* q = &lds.b[s][32 * ks + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
+                        const __bf16* q = &lds.b[s][32 * ks + 4 * quarter + (col >> 2)][OUT ? (x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3) : 16 * x + 4 * (col & 3)];
                         fk[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PX));
                     }
                     st[x] = mma<2>(st[x], fk, fv);
