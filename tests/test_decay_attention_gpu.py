@@ -630,7 +630,57 @@ def test_refusals_on_the_gpu():
         first.sum().backward()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+def test_one_token_of_rows_that_lie_far_apart(host, monkeypatch):
+    """(T, B, H, D) with T = 1 seen as (B, T, H, D): the stride of tokens that are not there may be anything."""
+    if not host:
+        monkeypatch.setattr(vr._lib, "_host", vr._lib._NoHost)
+    q, k, v, g, S = make(3, 1, 2, 2, 2, 2, 64, 64, "bf16", state=3)
+    gy = torch.randn(3, 1, 2, 64, generator=torch.Generator(DEV).manual_seed(5), device=DEV).bfloat16()
+    results = []
+    for far in (False, True):
+        view = (lambda t: t.as_strided(t.shape, (t.stride(0), 1 << 23, *t.stride()[2:]))) if far else lambda t: t
+        ts = [t.clone().requires_grad_() for t in (q, k, v, g, S)]
+        y, last = vr.decay_attention(*(view(t) for t in ts[:4]), state=ts[4], return_state=True)
+        results.append((y, last, *torch.autograd.grad(y, ts, view(gy))))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_pages_of_one_layer_from_another():
+    layers = torch.randn(6, 3, 2, 8, 8, device=DEV)
+    before = layers.clone()
+    vr.copy_states(layers[:, 0], [5, 0, -1], [1, 5, 2], source=layers[:, 2])
+    before[1, 0], before[5, 0], before[2, 0] = before[5, 2], before[0, 2], 0
+    assert torch.equal(layers, before)
+    flat = layers.flatten(1)
+    for pool, source in ((flat[:, :256], flat[:, 128:]), (flat[:, :192], flat[:, 191:383]), (flat[:, :128], flat[::2, 128:256])):
+        with pytest.raises(RuntimeError):                  # overlapping by half, by one number; at another distance
+            vr.copy_states(pool, [0], [1], source=source)
+
+
+@pytest.mark.gpu
+def test_refusals_of_sizes_and_of_moved_tensors():
+    wide = torch.zeros(1, 1, 1, 1, device=DEV).expand(1, (1 << 31) + 5, 1, 1)
+    for call in (lambda: vr.decay_attention(wide, wide, wide, torch.zeros(1, device=DEV)),
+                 lambda: vr.decay_attention_step(wide[0], wide[0], wide[0], torch.zeros(1, device=DEV), torch.zeros(2, 1, 1, 1, device=DEV))):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            call()
+    q, k, v, g, S = make(1, 20, 2, 2, 2, 2, 64, 64, "bf16", state=1)
+    for name, t in (("g", g), ("state", S), ("q", q)):
+        x = q.clone().requires_grad_()
+        back = lambda u, like=t: u.cpu() if u.shape == like.shape and u.dtype == like.dtype else u
+        with torch.autograd.graph.saved_tensors_hooks(lambda u: u, back):
+            y = vr.decay_attention(x, k, v, g, state=S)
+        with pytest.raises(RuntimeError):
+            y.float().sum().backward()
+
+
 def test_refusals_without_a_gpu():
+    with pytest.raises(RuntimeError, match="number"):
+        vr.decay_attention(torch.randn(1, 4, 2, 8), torch.randn(1, 4, 2, 8), torch.randn(1, 4, 2, 8), torch.randn(1, 4, 2), scale=torch.ones(()))
     q, g = torch.randn(1, 4, 2, 8), torch.randn(1, 4, 2)
     with pytest.raises(RuntimeError, match="CUDA"):
         vr.decay_attention(q, q, q, g)
@@ -680,6 +730,6 @@ def test_the_library_refuses_before_it_launches():
         return lib.vrwkv_copy_pages(pool, stride, P, source, source_stride, source_P, size, src, s64, dst, d64, M, ws, ws_bytes, None)
     for change, status in ((dict(pool=None), 1), (dict(src=None), 1), (dict(P=0), 1), (dict(M=0), 1), (dict(size=0), 1), (dict(M=4097), 3), (dict(stride=63), 1), (dict(source_stride=60), 1),
                            (dict(src=4100, s64=1), 1), (dict(ws=None, M=300), 5), (dict(ws_bytes=1199, M=300), 5), (dict(ws=4097, M=300), 1), (dict(source=(1 << 20) + 64), 1), (dict(source_stride=128), 1),
-                           (dict(size=1 << 30, stride=1 << 30, source_stride=1 << 30, M=4096), 3)):
+                           (dict(size=1 << 30, stride=1 << 30, source_stride=1 << 30, M=4096), 3), (dict(size=(1 << 23) + 1, stride=1 << 24, source_stride=1 << 24, M=4096), 3)):
         assert pages(**change) == status, change
     assert lib.vrwkv_copy_pages_workspace_bytes(300) == 1200 and lib.vrwkv_copy_pages_workspace_bytes(5) == lib.vrwkv_copy_pages_workspace_bytes(0) == 0

@@ -165,21 +165,26 @@ extern "C" int vrwkv_copy_pages(void* pool, long long stride, int P, const void*
     if (M <= 0 || P <= 0 || source_P < 0 || page_bytes <= 0) { set_error("%s: sizes must be positive", who); return VRWKV_INVALID_ARG; }
     if (M > MAX_LIST) { set_error("%s: %d entries, at most %d", who, M, MAX_LIST); return VRWKV_UNSUPPORTED_SHAPE; }
     if (stride < page_bytes || source_stride < page_bytes) { set_error("%s: pages overlap", who); return VRWKV_INVALID_ARG; }
-    if (page_bytes / THREADS * M >= 1LL << 32) { set_error("%s: too many bytes", who); return VRWKV_UNSUPPORTED_SHAPE; }
     if (((size_t)from & (from64 ? 7 : 3)) || ((size_t)to & (to64 ? 7 : 3))) { set_error("%s: an index is not aligned to its elements", who); return VRWKV_INVALID_ARG; }
     if (M > SMALL_LIST && (!workspace || workspace_bytes < vrwkv_copy_pages_workspace_bytes(M))) { set_error("%s: workspace of %zu bytes, %zu needed", who, workspace ? workspace_bytes : 0, vrwkv_copy_pages_workspace_bytes(M)); return VRWKV_WORKSPACE_TOO_SMALL; }
     if (M > SMALL_LIST && ((size_t)workspace & 3)) { set_error("%s: workspace must be 4-byte aligned", who); return VRWKV_INVALID_ARG; }
     const char *a = static_cast<const char*>(pool), *b = static_cast<const char*>(source);
     const bool same = a == b && stride == source_stride;
     const long long a_end = (P - 1) * stride + page_bytes, b_end = source_P ? (source_P - 1) * source_stride + page_bytes : 0;
-    if (!same && a < b + b_end && b < a + a_end) { set_error("%s: the source overlaps the pool", who); return VRWKV_INVALID_ARG; }
+    // (pages of the same stride that lie in each other's gaps, as those of two layers in one pool, are apart as well)
+    const long long shift = ((b - a) % stride + stride) % stride;
+    const bool gaps = stride == source_stride && shift >= page_bytes && shift + page_bytes <= stride;
+    if (!same && !gaps && a < b + b_end && b < a + a_end) { set_error("%s: the source overlaps the pool", who); return VRWKV_INVALID_ARG; }
     PageParams p{static_cast<char*>(pool), b, from, to, M > SMALL_LIST ? static_cast<int*>(workspace) : nullptr, stride, source_stride, page_bytes, from64, to64, M, P, source_P, same, 0, 0, 0};
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    if (p.plan) hipLaunchKernelGGL(plan_kernel, dim3(M), dim3(256), 0, st, p);
     const size_t bits = (size_t)pool | (size_t)source | (size_t)stride | (size_t)source_stride | (size_t)page_bytes;
-    if (!(bits & 15)) launch_copies<uint4>(p, st);
-    else if (!(bits & 3)) launch_copies<unsigned>(p, st);
-    else if (!(bits & 1)) launch_copies<unsigned short>(p, st);
+    const int unit = !(bits & 15) ? 16 : !(bits & 3) ? 4 : !(bits & 1) ? 2 : 1;
+    // (a launch has less than 2^32 threads, of 16 units each)
+    if (page_bytes / unit >= 1LL << 35 || page_bytes / unit * M >= 1LL << 35) { set_error("%s: too many bytes", who); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (p.plan) hipLaunchKernelGGL(plan_kernel, dim3(M), dim3(256), 0, st, p);
+    if (unit == 16) launch_copies<uint4>(p, st);
+    else if (unit == 4) launch_copies<unsigned>(p, st);
+    else if (unit == 2) launch_copies<unsigned short>(p, st);
     else launch_copies<unsigned char>(p, st);
     return check_launch(who);
 }

@@ -4,7 +4,7 @@
 //     y_t = scale sum_{s<=t} exp(G_t - G_s) (q_t . k_s) v_s + scale exp(G_t) S0^T q_t,      S = exp(G_end) S0 + sum_s exp(G_end - G_s) k_s v_s^T,
 // four matrix products.  The state in front of each chunk, and the same sum back along the tokens (b, c = gy, q in the places of k, v: the gradient of a
 // state), which the gradients want (decay_bwd.h), are this kernel's without its outputs.
-// Sequences of few calls are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
+// Calls of few sequences are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
 #pragma once
 #include "wave_sum.h"
 #include "wkv6_chunk_common.h"
@@ -416,10 +416,7 @@ __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, in
     for (int i = gid * 4 + (threadIdx.x >> 6); i < rows; i += p.segs * 4) {
         const long long row = i < front ? i : back + (i - front);
         const long long at = row * r.o.st + h * r.o.sh + d;
-        if (r.o.p && d < r.dz) {
-            if (r.o.f32) static_cast<float*>(r.o.p)[at] = 0.f;
-            else static_cast<IO*>(r.o.p)[at] = from_f32<IO>(0.f);
-        }
+        if (d < r.dz) static_cast<IO*>(r.o.p)[at] = from_f32<IO>(0.f);
     }
 }
 
@@ -497,7 +494,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     Sink<IO, VEC> so;
     if constexpr (OUT) {
         const int t = 16 * (wave % NT) + col;
-        so.open(r.o, w.base, w.first, h, rev ? L - 1 - t : t, z0 + 16 * (wave / NT * NT) + 4 * quarter, r.dz);
+        so.open(r.o, w.base, w.first, h, t, z0 + 16 * (wave / NT * NT) + 4 * quarter, r.dz);
     }
     float* const anchors = MODE == CHUNKS ? r.anchors + (((long long)(w.chunk0 + w.s0 / L) * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4 : nullptr;
     const long long anchor_step = (long long)p.H * r.tiles * (DX * TZ);
@@ -653,7 +650,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                     acc[j] = mma<NP - 1>(acc[j], fc, fp);
                 }
             }
-            so.store(acc, rev ? t0 + n - L : t0, t < n);
+            so.store(acc, t0, t < n);
         }
 
         // ---- the state behind the chunk
@@ -719,17 +716,14 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 #pragma unroll
         for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
         if (tid == 0 && z == 0) r.seg_decay[(long long)gid * p.H + h] = fast_exp2(seg_log);
-    } else {
-        if (r.last && (rev ? w.is_first : w.is_last)) {
-            const float d = rev && w.len > 0 ? fast_exp2(gates.widen(gates.fetch(0, 0, true)) * LOG2E) : 1.f;   // back along the tokens: the first one's decay
+    } else if (OUT && r.last && w.is_last) {
 #pragma unroll
-            for (int x = 0; x < NX; ++x)
+        for (int x = 0; x < NX; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int xc = 16 * x + 4 * quarter + i;
-                    if (xc < r.dx && zc < r.dz) r.last[page + xc * r.sx + zc * r.sz] = st[x][i] * d;
-                }
-        }
+            for (int i = 0; i < 4; ++i) {
+                const int xc = 16 * x + 4 * quarter + i;
+                if (xc < r.dx && zc < r.dz) r.last[page + xc * r.sx + zc * r.sz] = st[x][i];
+            }
     }
 }
 

@@ -335,8 +335,9 @@ vrwkv_decay_args decay_args(const at::Tensor& q, const at::Tensor& k, const at::
     a.state = state.defined() ? (const float*)state.data_ptr() : nullptr;
     a.offsets = offsets.defined() ? offsets.data_ptr() : nullptr;
     for (int i = 0; i < 3; ++i) {
-        a.q_stride[i] = q.stride(i), a.k_stride[i] = k.stride(i), a.v_stride[i] = v.stride(i);
-        a.g_stride[i] = g.dim() == 1 ? (i == 2 ? g.stride(0) : 0) : g.stride(i);
+        const bool none = i == 1 && q.size(1) == 1;        // a row of one token has no stride to a next one, whatever the view says
+        a.q_stride[i] = none ? 0 : q.stride(i), a.k_stride[i] = none ? 0 : k.stride(i), a.v_stride[i] = none ? 0 : v.stride(i);
+        a.g_stride[i] = g.dim() == 1 ? (i == 2 ? g.stride(0) : 0) : none ? 0 : g.stride(i);
     }
     a.N = N, a.T = (int)q.size(1), a.H = (int)g.size(-1), a.Hq = (int)q.size(2), a.Hk = (int)k.size(2), a.Hv = (int)v.size(2), a.Dk = (int)q.size(3), a.Dv = (int)v.size(3);
     a.dtype = code(q.scalar_type()), a.g_dtype = code(g.scalar_type()), a.g_per_head = g.dim() == 1, a.offsets64 = offsets.defined() && offsets.scalar_type() == at::kLong;
@@ -369,6 +370,8 @@ struct Decay : torch::autograd::Function<Decay> {
             at::NoGradGuard no_grad;
             const auto saved = ctx->get_saved_variables();
             const at::Tensor q = rows(saved[0], saved[0]), k = rows(saved[1], q), v = rows(saved[2], q), &g = saved[3], &offsets = saved[5];
+            for (const at::Tensor* t : {&g, &saved[4], &offsets})   // (hooks on saved tensors may have moved them)
+                TORCH_CHECK(!t->defined() || (t->is_cuda() && t->device() == q.device() && t->has_storage()), "the saved tensors must be CUDA tensors on one device");
             const at::Tensor state = saved[4].defined() ? saved[4].contiguous() : at::Tensor();
             const int N = (int)ctx->saved_data["N"].toInt();
             const int64_t H = g.size(-1);
@@ -381,7 +384,7 @@ struct Decay : torch::autograd::Function<Decay> {
             TORCH_CHECK(gy.size(0) == q.size(0) && gy.size(1) == q.size(1) && gy.size(2) == H && gy.size(3) == v.size(3), "the gradient must have the shape of y");
             vrwkv_decay_args a = decay_args(q, k, v, g, state, offsets, ctx->saved_data["scale"].toDouble(), N);
             a.gy = gy.data_ptr();
-            for (int i = 0; i < 3; ++i) a.gy_stride[i] = gy.stride(i);
+            for (int i = 0; i < 3; ++i) a.gy_stride[i] = i == 1 && gy.size(1) == 1 ? 0 : gy.stride(i);
             a.glast = glast.defined() ? (const float*)glast.data_ptr() : nullptr;
             const at::Tensor* like[5] = {&q, &k, &v, &g, &state};
             void* ptr[5] = {};

@@ -26,7 +26,18 @@ def _check(t, name, like=None):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if like is not None and t.device != like.device:
-        raise RuntimeError(f"{name} must be on {like.device}, the device of q")
+        raise RuntimeError(f"{name} must be on {like.device}, as the others")
+
+
+def _check_sizes(*shapes):
+    if any(n > 0x7fffffff for shape in shapes for n in shape):
+        raise RuntimeError("a size of 2^31 or more")       # (the library's are 32 bits)
+
+
+def _check_scale(scale):
+    if isinstance(scale, torch.Tensor):                    # (it would go in without its gradient)
+        raise RuntimeError("scale must be a number")
+    return float(scale)
 
 
 def _check_heads(q, k, v, g, lead):
@@ -43,6 +54,7 @@ def _check_heads(q, k, v, g, lead):
         raise RuntimeError("g must be float32 or have the dtype of q, k, v")
     if g.dim() != 1 and (g.dim() != lead + 1 or g.shape[:lead] != q.shape[:lead]):
         raise RuntimeError(f"g must be ({'B, T' if lead == 2 else 'N'}, H), or (H,) for one decay a head")
+    _check_sizes(*(t.shape for t in (q, k, v, g)))
     H = g.shape[-1]
     if H == 0 or any(t.shape[-2] == 0 or H % t.shape[-2] for t in (q, k, v)):
         raise RuntimeError(f"the heads of q, k and v ({q.shape[-2]}, {k.shape[-2]}, {v.shape[-2]}) must each divide those of g ({H})")
@@ -57,6 +69,11 @@ def _check_index(t, name, like):
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"{name} must be a vector of int32 or int64")
     return t.contiguous()
+
+
+def _strides(t):
+    """Strides of batch, token and head; a row of one token has none to a next one, whatever the view says."""
+    return t.stride(0), 0 if t.shape[1] == 1 else t.stride(1), t.stride(2)
 
 
 def _call(name, args, device, ws_name=None):
@@ -76,8 +93,8 @@ def _decay_args(q, k, v, g, state, offsets, scale, N, H):
     a.state = state.data_ptr() if state is not None else None
     a.offsets = offsets.data_ptr() if offsets is not None else None
     for name, t in (("q_stride", q), ("k_stride", k), ("v_stride", v)):
-        setattr(a, name, (t.stride(0), t.stride(1), t.stride(2)))
-    a.g_stride = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
+        setattr(a, name, _strides(t))
+    a.g_stride = (0, 0, g.stride(0)) if g.dim() == 1 else _strides(g)
     a.N, a.T, a.H, a.Hq, a.Hk, a.Hv, a.Dk, a.Dv = N, q.shape[1], H, q.shape[2], k.shape[2], v.shape[2], q.shape[3], v.shape[3]
     a.dtype, a.g_dtype, a.g_per_head, a.offsets64, a.scale = _DT[q.dtype], _DT[g.dtype], g.dim() == 1, offsets is not None and offsets.dtype == torch.int64, scale
     return a
@@ -110,6 +127,9 @@ class DecayAttention(torch.autograd.Function):
     def backward(ctx, gy, glast):
         q, k, v, g, state, offsets = ctx.saved_tensors
         scale, N, H = ctx.meta
+        for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (state, "state"), (offsets, "offsets")):
+            if t is not None:                              # (hooks on saved tensors may have moved them)
+                _check(t, name, q)
         if batched_cotangent(*(t for t in (gy, glast) if t is not None)):
             raise RuntimeError("decay_attention's gradients take one cotangent at a time")
         q, k, v = _rows(q), _rows(k), _rows(v)
@@ -127,7 +147,7 @@ class DecayAttention(torch.autograd.Function):
         gy = torch.zeros((*q.shape[:2], H, v.shape[3]), dtype=q.dtype, device=q.device) if gy is None else _rows(gy.to(q.dtype))
         glast = glast.float().contiguous() if glast is not None else None
         a = _decay_args(q, k, v, g, state, offsets, scale, N, H)
-        a.gy, a.gy_stride = gy.data_ptr(), gy.stride()[:3]
+        a.gy, a.gy_stride = gy.data_ptr(), _strides(gy)
         for name, t in (("glast", glast), ("dq", dq), ("dk", dk), ("dv", dv), ("dg", dg), ("dstate", dstate)):
             setattr(a, name, t.data_ptr() if t is not None else None)
         _call("vrwkv_decay_bwd", a, q.device, "vrwkv_decay_bwd_workspace_bytes")
@@ -145,6 +165,7 @@ def decay_attention(q, k, v, g, scale=1.0, state=None, offsets=None, return_stat
     Gradients for q, k, v, g and state, sums in fp32 (those of (H,) decays in 64 bits), rounded once to their inputs' types; no second ones."""
     if torch.compiler.is_compiling():
         return _eager(decay_attention)(q, k, v, g, scale, state, offsets, return_state)
+    scale = _check_scale(scale)
     out = _lib.host().decay_attention(q, k, v, g, scale, state, offsets, return_state)
     if out is not None:
         return out
@@ -159,7 +180,7 @@ def decay_attention(q, k, v, g, scale=1.0, state=None, offsets=None, return_stat
         _check(state, "state", q)
         if tuple(state.shape) != (N, H, Dk, Dv) or state.dtype != torch.float32:
             raise RuntimeError(f"state must be float32 of shape {(N, H, Dk, Dv)}")
-    y, last = DecayAttention.apply(q, k, v, g, state, offsets, float(scale), N, H, bool(return_state))
+    y, last = DecayAttention.apply(q, k, v, g, state, offsets, scale, N, H, bool(return_state))
     return (y, last) if return_state else y
 
 
@@ -172,12 +193,14 @@ def decay_attention_step(q, k, v, g, pool, slots=None, scale=1.0):
     layers), each contiguous.  Forward only."""
     if torch.compiler.is_compiling():
         return _eager(decay_attention_step)(q, k, v, g, pool, slots, scale)
+    scale = _check_scale(scale)
     y = _lib.host().decay_step(q, k, v, g, pool, slots, scale)
     if y is not None:
         return y
     H, Dk, Dv = _check_heads(q, k, v, g, 1)
     N = q.shape[0]
     _check(pool, "pool", q)
+    _check_sizes(pool.shape)
     if pool.dim() != 4 or tuple(pool.shape[1:]) != (H, Dk, Dv) or pool.dtype != torch.float32 or not _pages_fit(pool):
         raise RuntimeError(f"pool must be float32 (P, {H}, {Dk}, {Dv}) with contiguous pages")
     if slots is not None:
@@ -243,7 +266,8 @@ def copy_states(pool, src, dst, source=None):
     One list forks a state (one src, several dst), moves pages together (over pages that move as well, in any order), exchanges them, copies them in
     from another pool or out to one.  src -1 clears the page, dst -1 is a place of the list that is not taken; of several entries with the same dst the
     last counts.  src, dst: vectors of up to 4096 int32 or int64, on the device -- where entries outside the pools are left out -- or on the host, where
-    they are refused.  Pools of any type whose pages are contiguous, at any distance; a source is the pool or does not overlap it."""
+    they are refused.  Pools of any type whose pages are contiguous, at any distance; a source is the pool, or its pages overlap none of
+    the pool's (pool[:, 0] and pool[:, 1] of a pool for all layers)."""
     if torch.compiler.is_compiling():
         return _eager(copy_states)(pool, src, dst, source)
     if _lib.host().copy_pages(pool, src, dst, source):
@@ -253,6 +277,7 @@ def copy_states(pool, src, dst, source=None):
     _check(source, "source", pool)
     if pool.dim() < 1 or source.shape[1:] != pool.shape[1:] or source.dtype != pool.dtype:
         raise RuntimeError("pool and source must hold pages of one shape and type")
+    _check_sizes(pool.shape[:1], source.shape[:1])
     if not _pages_fit(pool) or not _pages_fit(source):
         raise RuntimeError("the pages of pool and source must be contiguous and apart")
     if torch.is_grad_enabled() and (pool.requires_grad or source.requires_grad):
