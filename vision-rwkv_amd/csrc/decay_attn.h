@@ -248,6 +248,18 @@ struct Sink {
         }
     }
 };
+// A state (N, H, Dk, Dv)'s numbers as a lane of the accumulators has them: x, and the rows behind it, of one column.  Addresses that differ by what is the same for
+// all lanes, and no branches: element by element behind its own check, writing the last states took 8 000 of a short sequence's 28 000 cycles.
+struct StatePage {
+    __amdgpu_buffer_rsrc_t buf;
+    unsigned at;
+    int step, count;                                      // bytes from row to row; rows from x on
+    __device__ __forceinline__ StatePage(const float* p, long long sx, long long sz, int dx, int dz, int x, int z) : buf(buffer_at(p)), step((int)sx * 4), count(z < dz ? dx - x : 0) {
+        at = (unsigned)(x * step + z * (int)sz * 4);
+    }
+    __device__ __forceinline__ float load(int i) const { return __builtin_bit_cast(float, BufRaw<4>::ld(buf, i < count ? at : OOB_OFFSET, (unsigned)(i * step))); }
+    __device__ __forceinline__ void store(int i, float v) const { BufRaw<4>::st(__builtin_bit_cast(unsigned, v), buf, i < count ? at : OOB_OFFSET, (unsigned)(i * step)); }
+};
 // The log decays of a sequence and head.
 struct Gates {
     const char* p;
@@ -436,8 +448,8 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 
     // a head's tiles, and the roles of a tile, next to each other: they read the same rows
     int id = blockIdx.x;
-    const Role& r = p.role[id & (p.n_roles - 1)];
-    id >>= p.n_roles - 1;
+    const Role& r = p.role[MODE == STATES ? id & (p.n_roles - 1) : 0];
+    if (MODE == STATES) id >>= p.n_roles - 1;
     const int z = id & (r.tiles - 1), h = id >> (r.tiles - 1), gid = grid_segment();
     if (gid >= p.segs) return;
     const Place w = find_place<THREADS>(p, gid, L, offs);
@@ -481,15 +493,15 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     if (MODE != STATES && !first_one) {
 #pragma unroll
         for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4);
-    } else {
-        const auto buf = buffer_at(r.init + page);
+    } else if (have) {
+        const StatePage s(r.init + page, r.sx, r.sz, r.dx, r.dz, 4 * quarter, zc);
 #pragma unroll
         for (int x = 0; x < NX; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int xc = 16 * x + 4 * quarter + i;
-                st[x][i] = __builtin_bit_cast(float, BufRaw<4>::ld(buf, have && xc < r.dx && zc < r.dz ? (unsigned)(xc * (int)r.sx + zc * (int)r.sz) * 4u : OOB_OFFSET, 0));
-            }
+            for (int i = 0; i < 4; ++i) st[x][i] = s.load(16 * x + i);
+    } else {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     Sink<IO, VEC> so;
     if constexpr (OUT) {
@@ -717,13 +729,11 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
         if (tid == 0 && z == 0) r.seg_decay[(long long)gid * p.H + h] = fast_exp2(seg_log);
     } else if (OUT && r.last && w.is_last) {
+        const StatePage s(r.last + page, r.sx, r.sz, r.dx, r.dz, 4 * quarter, zc);
 #pragma unroll
         for (int x = 0; x < NX; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int xc = 16 * x + 4 * quarter + i;
-                if (xc < r.dx && zc < r.dz) r.last[page + xc * r.sx + zc * r.sz] = st[x][i];
-            }
+            for (int i = 0; i < 4; ++i) s.store(16 * x + i, st[x][i]);
     }
 }
 

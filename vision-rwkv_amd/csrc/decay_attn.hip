@@ -21,6 +21,7 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
     const Place w = sequence_place(p, n, 64);
     const int x = blockIdx.x % (DX / 16), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = first_segment(p, n, w.first), count = segment_count(p, w.len);
+    if (count == 1) return;                               // (starts from what it is given)
     f32x4 carry = {0.f, 0.f, 0.f, 0.f};
     if (r.init) {
         const float* page = r.init + ((long long)n * p.H + h) * ((long long)r.dx * r.dz);
@@ -34,7 +35,6 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
     const auto at = [&](int i) { return ((long long)(first + (r.reverse ? count - 1 - i : i)) * p.H + h); };    // the i-th on the way
     const long long in_tile = ((long long)x * 4 + wave) * 64 * 4 + lane * 4;
     constexpr int U = 8;
-    if (count == 1) return;                               // (starts from what it is given)
     for (int i0 = 0; i0 < count; i0 += U) {
         f32x4 own[U];
         float d[U];

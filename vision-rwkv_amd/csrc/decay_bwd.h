@@ -166,15 +166,12 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
 #pragma unroll
             for (int i = 0; i < 4; ++i) st[x][i] *= d;
         }
-    } else if (kind == DV) {
-        const auto buf = buffer_at(p.glast + page);
+    } else if (kind == DV && have) {
+        const StatePage s(p.glast + page, 1, p.Dv, p.Dv, p.Dk, v0 + 4 * quarter, zc);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int xc = v0 + 16 * x + 4 * quarter + i;
-                st[x][i] = __builtin_bit_cast(float, BufRaw<4>::ld(buf, have && xc < p.Dv && zc < p.Dk ? (unsigned)(zc * p.Dv + xc) * 4u : OOB_OFFSET, 0));
-            }
+            for (int i = 0; i < 4; ++i) st[x][i] = s.load(16 * x + i);
     }
     const int tw = w4 % NT, zt0 = w4 / NT * NT;           // this wave's tile of tokens, its first tile of channels
     Sink<IO, VEC> so;
@@ -567,13 +564,11 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     }
 
     if (p.dstate && w.is_first && kind == DV) {
+        const StatePage s(p.dstate + page, 1, p.Dv, p.Dv, p.Dk, v0 + 4 * quarter, zc);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int xc = v0 + 16 * x + 4 * quarter + i;
-                if (xc < p.Dv && zc < p.Dk) p.dstate[page + (long long)zc * p.Dv + xc] = st[x][i];
-            }
+            for (int i = 0; i < 4; ++i) s.store(16 * x + i, st[x][i]);
     }
 }
 
