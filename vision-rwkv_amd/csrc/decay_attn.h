@@ -18,7 +18,7 @@ using wkv6_detail::f32x4;
 using wkv6_detail::u32x4;
 
 constexpr int TZ = 64;                                    // columns of a state that a workgroup holds
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, OUT_THREADS = 512;           // of a workgroup for states; for outputs
 
 // A tensor (batch, token, head, channel), channels side by side; head h of the call reads head h / share.
 struct View {
@@ -40,7 +40,7 @@ struct Role {
     float* anchors;                                       // [chunk][head][tile]: the state in front of each chunk
     long long sx, sz;                                     // strides of the states' contracted and other index
     int dx, dz, tiles, reverse;                           // (one or two tiles; the roles of a launch have the same)
-    float s_in, s_upd;                                    // scale where the state is read; where it is written
+    float s_upd;                                          // scale of what the states take up
 };
 struct Call {                                             // sequences, their cut, and the decays
     const void *offsets, *g;
@@ -414,7 +414,8 @@ struct Lds {
     } d[2];                                               // this chunk's and the next one's
 };
 
-// Eight channels from d on in the order that the accumulators' fragments have: inside 32 channels, 4 m .. 4 m + 3 lie at 8 (m & 3) + 4 (m >> 2).
+// Where channel d of a row lies in the order that the accumulators' fragments have: inside 32 channels, 4 m .. 4 m + 3 lie at 8 (m & 3) + 4 (m >> 2); of eight from an eighth
+// on, the second four 8 behind the first.
 __device__ __forceinline__ int order_of(int d) {
     const int m = (d >> 2) & 7;
     return (d & ~31) + 8 * (m & 3) + 4 * (m >> 2);
@@ -425,7 +426,7 @@ template <typename IO>
 __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, int front, int back, int gid, int z, int h) {
     const int rows = front + max(0, p.T - back);
     const int d = z * TZ + (threadIdx.x & 63);
-    for (int i = gid * 4 + (threadIdx.x >> 6); i < rows; i += p.segs * 4) {
+    for (int i = gid * (OUT_THREADS / 64) + (threadIdx.x >> 6); i < rows; i += p.segs * (OUT_THREADS / 64)) {
         const long long row = i < front ? i : back + (i - front);
         const long long at = row * r.o.st + h * r.o.sh + d;
         if (d < r.dz) static_cast<IO*>(r.o.p)[at] = from_f32<IO>(0.f);
@@ -434,14 +435,54 @@ __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, in
 
 // workgroups that a compute unit's LDS holds, up to three: more do not fit the registers
 template <size_t BYTES> constexpr int workgroups = 3 * BYTES <= 160 * 1024 ? 3 : 2 * BYTES <= 160 * 1024 ? 2 : 1;
+template <size_t BYTES> constexpr int out_workgroups = 2 * BYTES <= 160 * 1024 ? 2 : 1;
 
+// A chunk's decays by one wave, from its log decays (zero behind its last token); the sum of the powers of two.
+// In 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth.
+template <int L, typename D>
+__device__ __forceinline__ float chunk_decays(D& d, float g, int lane) {
+    const double G = wave_scan_inclusive((double)g * 1.4426950408889634);
+    const double end = lane_double(G, 63);
+    const float gh = (float)G;
+    if (lane < L) {
+        d.gh[lane] = gh;
+        d.gl[lane] = (float)(G - gh);
+        d.dt[lane] = fast_exp2(gh);
+        d.dk[lane] = fast_exp2((float)(end - G));
+    }
+    if (lane == 0) d.end = fast_exp2((float)end);
+    return (float)end;
+}
+// A fragment read across rows: a lane's four of q's row and four of the row 16 behind it.
+__device__ __forceinline__ bf16x8 across8(const __bf16* q, int pitch) { return wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * pitch)); }
+// c's rows with their decays to the chunk's end, put together from the terms, scaled and split again
+template <typename IO, int L, int PZ>
+__device__ __forceinline__ void decayed_terms(const __bf16 (&c)[in_terms<IO>][L][PZ], const float* dk, float s_upd, int ks, int column, int quarter, int col, bf16x8 (&f)[3]) {
+    float x8[8];
+    const f32x4 d0 = *reinterpret_cast<const f32x4*>(&dk[32 * ks + 4 * quarter]), d1 = *reinterpret_cast<const f32x4*>(&dk[32 * ks + 16 + 4 * quarter]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x8[i] = 0.f;
+#pragma unroll
+    for (int s = in_terms<IO> - 1; s >= 0; --s) {
+        const bf16x8 t = across8(&c[s][32 * ks + 4 * quarter + (col >> 2)][column + 4 * (col & 3)], PZ);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x8[i] += (float)t[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x8[i] *= d0[i] * s_upd;
+        x8[4 + i] *= d1[i] * s_upd;
+    }
+    split8<3>(x8, f);
+}
+
+// A segment's own state, or the states in front of a segment's chunks.
 template <typename IO, int DX, int MODE, bool VEC>
-__global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) void decay_kernel(const Params p) {
+__global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) void decay_states_kernel(const Params p) {
     using S = Lds<IO, DX, MODE>;
-    constexpr int L = S::L, NS = S::NS, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
-    constexpr int PA = L * DX / 8 / THREADS, PC = (L * TZ / 8 + THREADS - 1) / THREADS;
-    static_assert(PA >= 1 && L * DX % (8 * THREADS) == 0 && L * TZ % (8 * THREADS) == 0, "");
-    constexpr bool OUT = S::OUT;
+    constexpr int L = S::L, NS = S::NS, KS = L / 32, NX = DX / 16;
+    constexpr int PB = L * DX / 8 / THREADS, PC = L * TZ / 8 / THREADS;
+    static_assert(MODE != PLAIN && PB >= 1 && PC >= 1 && L * DX % (8 * THREADS) == 0 && L * TZ % (8 * THREADS) == 0, "");
     __shared__ S lds;
     __shared__ int offs[THREADS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quarter = lane >> 4, col = lane & 15;
@@ -453,27 +494,24 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     const int z = id & (r.tiles - 1), h = id >> (r.tiles - 1), gid = grid_segment();
     if (gid >= p.segs) return;
     const Place w = find_place<THREADS>(p, gid, L, offs);
-    if (OUT && !p.nseg) clear_outside<IO>(p, r, w.front, w.back, gid, z, h);
     if (!w.valid) return;
-    if (MODE == STATES && (r.reverse ? w.is_first : w.is_last)) return;    // nothing starts behind it
-    const int z0 = z * TZ;
     const bool rev = MODE == STATES && r.reverse;
+    if (MODE == STATES && (rev ? w.is_first : w.is_last)) return;    // nothing starts behind it
+    const int z0 = z * TZ;
 
     const int nc = (w.s1 - w.s0 + L - 1) / L;
     const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, rowz = tid / (TZ / 8), dzo = tid % (TZ / 8) * 8;
     constexpr int STEPX = THREADS / (DX / 8), STEPZ = THREADS / (TZ / 8);   // rows between a thread's pieces
-    Source<IO, PA, STEPX, VEC> sa, sb;
+    Source<IO, PB, STEPX, VEC> sb;
     Source<IO, PC, STEPZ, VEC> sc;
     Gates gates;
     gates.open(p, w.base, w.first, h);
-    if constexpr (OUT) sa.open(r.a, w.base, w.first, h, L, rev, rowx, dxo, r.dx);
     sb.open(r.b, w.base, w.first, h, L, rev, rowx, dxo, r.dx);
     sc.open(r.c, w.base, w.first, h, L, rev, rowz, z0 + dzo, r.dz);
-    Piece<IO> ra[PA], rb[PA], rc[PC];
+    Piece<IO> rb[PB], rc[PC];
     Gates::Raw rg{};
     const auto fetch = [&](int c) {
         const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0), token = rev ? t0 + n - L : t0;
-        if constexpr (OUT) sa.load(ra, token, n, rev);
         sb.load(rb, token, n, rev);
         sc.load(rc, token, n, rev);
         if (wave == 0) {
@@ -485,16 +523,13 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 
     // ---- the state that the segment starts from: rows 16 x + 4 quarter + i, column 16 wave + col of the tile
     f32x4 st[NX];
-    const long long page = ((long long)w.n * p.H + h) * ((long long)r.dx * r.dz);
-    const long long seg_at = (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ);
-    const int zc = z0 + 16 * wave + col;
-    const bool first_one = rev ? w.is_last : w.is_first;
-    bool have = MODE != STATES && (first_one ? r.init != nullptr : true);
-    if (MODE != STATES && !first_one) {
+    const long long seg_at = (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4;
+    bool have = MODE == CHUNKS && (!w.is_first || r.init);
+    if (MODE == CHUNKS && !w.is_first) {
 #pragma unroll
-        for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4);
+        for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + seg_at + x * 1024);
     } else if (have) {
-        const StatePage s(r.init + page, r.sx, r.sz, r.dx, r.dz, 4 * quarter, zc);
+        const StatePage s(r.init + ((long long)w.n * p.H + h) * ((long long)r.dx * r.dz), r.sx, r.sz, r.dx, r.dz, 4 * quarter, z0 + 16 * wave + col);
 #pragma unroll
         for (int x = 0; x < NX; ++x)
 #pragma unroll
@@ -503,66 +538,35 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 #pragma unroll
         for (int x = 0; x < NX; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    Sink<IO, VEC> so;
-    if constexpr (OUT) {
-        const int t = 16 * (wave % NT) + col;
-        so.open(r.o, w.base, w.first, h, t, z0 + 16 * (wave / NT * NT) + 4 * quarter, r.dz);
-    }
     float* const anchors = MODE == CHUNKS ? r.anchors + (((long long)(w.chunk0 + w.s0 / L) * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4 : nullptr;
     const long long anchor_step = (long long)p.H * r.tiles * (DX * TZ);
-    float scale = p.scale, s_in = r.s_in, s_upd = r.s_upd;
-    keep(scale);
-    keep(s_in);
+    float s_upd = r.s_upd;
     keep(s_upd);
 
     float seg_log = 0.f;                                  // (STATES: the segment's whole decay, from wave 0)
     const auto put_decays = [&](typename S::Decays& d) {   // wave 0
-        // sums in 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth
-        const double G = wave_scan_inclusive((double)gates.widen(rg) * 1.4426950408889634);
-        const double end = lane_double(G, 63);
-        const float gh = (float)G;
-        if (lane < L) {
-            d.gh[lane] = gh;
-            d.gl[lane] = (float)(G - gh);
-            d.dt[lane] = fast_exp2(gh);
-            d.dk[lane] = fast_exp2((float)(end - G));
-        }
-        if (lane == 0) d.end = fast_exp2((float)end);
-        if (MODE == STATES) seg_log += (float)end;
+        const float end = chunk_decays<L>(d, gates.widen(rg), lane);
+        if (MODE == STATES) seg_log += end;
     };
     if (nc > 0 && wave == 0) put_decays(lds.d[0]);
     if (S::SCALED) lds_barrier();                         // (c is scaled with them)
     for (int ci = 0; ci < nc; ++ci) {
-        // (what follows from the lane is worked out anew for each chunk: kept over the loop it fills the registers, masks for every tile among it)
+        // (what follows from the lane is worked out anew for each chunk: kept over the loop it fills the registers)
         int lane_ = lane;
         asm volatile("" : "+v"(lane_));
         const int quarter = lane_ >> 4, col = lane_ & 15;
         const int c = rev ? nc - 1 - ci : ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
         // ---- operands to the LDS
 #pragma unroll
-        for (int i = 0; i < PA; ++i) {
-            const int row = rowx + STEPX * i, o0 = order_of(dxo), o1 = order_of(dxo + 4);
+        for (int i = 0; i < PB; ++i) {
             u32x4 t[NS];
-            if constexpr (OUT) {
-                piece_terms<IO>(ra[i], t);
-#pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    *reinterpret_cast<uint2*>(&lds.a[s][row][o0]) = uint2{t[s][0], t[s][1]};
-                    *reinterpret_cast<uint2*>(&lds.a[s][row][o1]) = uint2{t[s][2], t[s][3]};
-                }
-            }
             piece_terms<IO>(rb[i], t);
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                if constexpr (OUT) {
-                    *reinterpret_cast<uint2*>(&lds.b[s][row][o0]) = uint2{t[s][0], t[s][1]};
-                    *reinterpret_cast<uint2*>(&lds.b[s][row][o1]) = uint2{t[s][2], t[s][3]};
-                } else *reinterpret_cast<u32x4*>(&lds.b[s][row][dxo]) = t[s];
-            }
+            for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.b[s][rowx + STEPX * i][dxo]) = t[s];
         }
 #pragma unroll
         for (int i = 0; i < PC; ++i) {
-            const int row = rowz + STEPZ * i, d = dzo;
+            const int row = rowz + STEPZ * i;
             if constexpr (S::SCALED) {
                 const float f = lds.d[ci & 1].dk[row] * s_upd;
                 float x8[8];
@@ -572,168 +576,283 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
                 bf16x8 t[3];
                 split8<3, false>(x8, t);
 #pragma unroll
-                for (int s = 0; s < 3; ++s) *reinterpret_cast<bf16x8*>(&lds.c[s][row][d]) = t[s];
+                for (int s = 0; s < 3; ++s) *reinterpret_cast<bf16x8*>(&lds.c[s][row][dzo]) = t[s];
             } else {
                 u32x4 t[NS];
                 piece_terms<IO>(rc[i], t);
 #pragma unroll
-                for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.c[s][row][d]) = t[s];
+                for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.c[s][row][dzo]) = t[s];
             }
         }
-        if constexpr (OUT) {
-            if (have) {
-#pragma unroll
-                for (int kx = 0; kx < KX; ++kx) {
-                    const float x8[8] = {st[2 * kx][0], st[2 * kx][1], st[2 * kx][2], st[2 * kx][3], st[2 * kx + 1][0], st[2 * kx + 1][1], st[2 * kx + 1][2], st[2 * kx + 1][3]};
-                    bf16x8 t[NP];
-                    split8<NP>(x8, t);
-#pragma unroll
-                    for (int s = 0; s < NP; ++s) lds.s[s][wave][kx][lane] = __builtin_bit_cast(u32x4, t[s]);
-                }
-            }
-        }
-        lds_barrier();                                    // (orders the LDS alone: the next chunk's rows and this one's results stay on their way)
+        lds_barrier();                                    // (orders the LDS alone: the next chunk's rows and what was stored stay on their way)
         if (ci + 1 < nc) fetch(rev ? c - 1 : c + 1);
-        typename S::Decays& dec_ = lds.d[ci & 1];
-
-        // ---- outputs of rows 16 tw + col, columns 16 zt + 4 quarter + i
-        const int tw = wave % NT, zt0 = wave / NT * NT, t = 16 * tw + col;
-        if (OUT && 16 * tw < n) {
-            const float gth = dec_.gh[t], gtl = dec_.gl[t], dec = dec_.dt[t] * s_in;
-            bf16x8 fa[KX][NS];
+        typename S::Decays& dec = lds.d[ci & 1];
+        if (MODE == CHUNKS && have) {                     // (zeros in front of a first chunk are not kept)
 #pragma unroll
-            for (int kx = 0; kx < KX; ++kx)
-#pragma unroll
-                for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[OUT ? s : 0][OUT ? t : 0][kx * 32 + 8 * quarter]);
-            // what the state in front gives
-            f32x4 acc[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (have) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                    for (int kx = 0; kx < KX; ++kx) {
-                        bf16x8 fs[NP];
-#pragma unroll
-                        for (int s = 0; s < NP; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[OUT ? s : 0][zt0 + j][OUT ? kx : 0][lane]);
-                        acc[j] = mma<NP - 1>(acc[j], fs, fa[kx]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[j][i] *= dec;
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (2 * ks > tw) break;
-                float pr[8];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int st_ = 2 * ks + half;        // tile of 16 tokens s
-                    f32x4 m = {0.f, 0.f, 0.f, 0.f};
-                    if (st_ <= tw) {
-#pragma unroll
-                        for (int kx = 0; kx < KX; ++kx) {
-                            bf16x8 fb[NS];
-#pragma unroll
-                            for (int s = 0; s < NS; ++s) fb[s] = *reinterpret_cast<const bf16x8*>(&lds.b[s][16 * st_ + col][kx * 32 + 8 * quarter]);
-                            m = mma<NP - 1>(m, fb, fa[kx]);
-                        }
-                        const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec_.gh[16 * st_ + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec_.gl[16 * st_ + 4 * quarter]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = m[i] * (scale * fast_exp2((gth - sh[i]) + (gtl - sl[i])));
-                            m[i] = st_ < tw || 4 * quarter + i <= col ? x : 0.f;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) pr[4 * half + i] = m[i];
-                }
-                bf16x8 fp[NP];
-                split8<NP>(pr, fp);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    bf16x8 fc[NS];
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) {
-                        const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * (zt0 + j) + 4 * (col & 3)];
-                        fc[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
-                    }
-                    acc[j] = mma<NP - 1>(acc[j], fc, fp);
-                }
-            }
-            so.store(acc, t0, t < n);
+            for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(anchors + c * anchor_step + x * 1024) = st[x];
         }
-
+        if (MODE == CHUNKS && ci + 1 == nc) break;         // (nothing starts behind it)
         // ---- the state behind the chunk
-        {
-            if (MODE == CHUNKS && have) {                 // (zeros in front of a first chunk are not kept)
-#pragma unroll
-                for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(anchors + c * anchor_step + x * 1024) = st[x];
-            }
-            if (MODE == CHUNKS && ci + 1 == nc) break;     // (nothing starts behind it)
-            const float ed = dec_.end;
-#pragma unroll
-            for (int x = 0; x < NX; ++x)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st[x][i] *= ed;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (32 * ks >= n) break;
-                bf16x8 fv[3];
-                if constexpr (S::SCALED) {
-#pragma unroll
-                    for (int s = 0; s < 3; ++s) {
-                        const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * wave + 4 * (col & 3)];
-                        fv[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
-                    }
-                } else {
-                    float x8[8];
-                    const f32x4 d0 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 4 * quarter]), d1 = *reinterpret_cast<const f32x4*>(&dec_.dk[32 * ks + 16 + 4 * quarter]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x8[i] = 0.f;
-#pragma unroll
-                    for (int s = NS - 1; s >= 0; --s) {
-                        const __bf16* q = &lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * wave + 4 * (col & 3)];
-                        const bf16x8 f = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PZ));
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x8[i] += (float)f[i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x8[i] *= d0[i] * s_upd;
-                        x8[4 + i] *= d1[i] * s_upd;
-                    }
-                    split8<3>(x8, fv);
-                }
-#pragma unroll
-                for (int x = 0; x < NX; ++x) {
-                    bf16x8 fk[NS];
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) {
-                        const __bf16* q = &lds.b[s][32 * ks + 4 * quarter + (col >> 2)][OUT ? (x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3) : 16 * x + 4 * (col & 3)];
-                        fk[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * S::PX));
-                    }
-                    st[x] = mma<2>(st[x], fk, fv);
-                }
-            }
-            have = true;
-        }
-        if (wave == 0 && ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
-        lds_barrier();
-    }
-
-    // ---- the state behind the segment
-    if constexpr (MODE == STATES) {
-#pragma unroll
-        for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.seg + seg_at + ((x * 4 + wave) * 64 + lane) * 4) = st[x];
-        if (tid == 0 && z == 0) r.seg_decay[(long long)gid * p.H + h] = fast_exp2(seg_log);
-    } else if (OUT && r.last && w.is_last) {
-        const StatePage s(r.last + page, r.sx, r.sz, r.dx, r.dz, 4 * quarter, zc);
+        const float ed = dec.end;
 #pragma unroll
         for (int x = 0; x < NX; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s.store(16 * x + i, st[x][i]);
+            for (int i = 0; i < 4; ++i) st[x][i] *= ed;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if (32 * ks >= n) break;
+            bf16x8 fv[3];
+            if constexpr (S::SCALED) {
+#pragma unroll
+                for (int s = 0; s < 3; ++s) fv[s] = across8(&lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * wave + 4 * (col & 3)], S::PZ);
+            } else decayed_terms<IO>(lds.c, dec.dk, s_upd, ks, 16 * wave, quarter, col, fv);
+#pragma unroll
+            for (int x = 0; x < NX; ++x) {
+                bf16x8 fk[NS];
+#pragma unroll
+                for (int s = 0; s < NS; ++s) fk[s] = across8(&lds.b[s][32 * ks + 4 * quarter + (col >> 2)][16 * x + 4 * (col & 3)], S::PX);
+                st[x] = mma<2>(st[x], fk, fv);
+            }
+        }
+        have = true;
+        if (wave == 0 && ci + 1 < nc) put_decays(lds.d[(ci + 1) & 1]);
+        lds_barrier();
+    }
+    if constexpr (MODE == STATES) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.seg + seg_at + x * 1024) = st[x];
+        if (tid == 0 && z == 0) r.seg_decay[(long long)gid * p.H + h] = fast_exp2(seg_log);
+    }
+}
+
+// Outputs.  Eight waves of two kinds, which need nothing of each other between two barriers: four take the tokens' outputs (16 tokens each), four the state
+// behind the chunk (16 columns each), its terms for the next one and the decays.
+template <typename IO, int DX, bool VEC>
+__global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX, PLAIN>)>)) void decay_kernel(const Params p) {
+    using S = Lds<IO, DX, PLAIN>;
+    constexpr int L = S::L, NS = S::NS, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
+    constexpr int PA = L * DX / 8 / 256, PC = L * TZ / 8 / 256;   // pieces of a thread of its kind
+    static_assert(PA >= 1 && PC >= 1 && L * DX % 2048 == 0 && L * TZ % 2048 == 0, "");
+    __shared__ S lds;
+    __shared__ int offs[OUT_THREADS];
+    const int tid = threadIdx.x & 255, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w4 = wave & 3;
+
+    const Role& r = p.role[0];
+    const int z = blockIdx.x & (r.tiles - 1), h = blockIdx.x >> (r.tiles - 1), gid = grid_segment();   // a head's tiles next to each other: they read the same rows
+    if (gid >= p.segs) return;
+    const Place w = find_place<OUT_THREADS>(p, gid, L, offs);
+    if (!p.nseg) clear_outside<IO>(p, r, w.front, w.back, gid, z, h);
+    if (!w.valid) return;
+    const int z0 = z * TZ, nc = (w.s1 - w.s0 + L - 1) / L;
+    const bool begun = !w.is_first || r.init;             // there is a state in front
+    constexpr int STEPX = 256 / (DX / 8), STEPZ = 256 / (TZ / 8);   // rows between a thread's pieces
+    float scale = p.scale;
+    keep(scale);
+
+    if (wave < 4) {
+        const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, o0 = order_of(dxo);
+        Source<IO, PA, STEPX, VEC> sa, sb;
+        sa.open(r.a, w.base, w.first, h, L, false, rowx, dxo, r.dx);
+        sb.open(r.b, w.base, w.first, h, L, false, rowx, dxo, r.dx);
+        Piece<IO> ra[PA], rb[PA];
+        const auto fetch = [&](int c) {
+            const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+            sa.load(ra, t0, n, false);
+            sb.load(rb, t0, n, false);
+        };
+        if (nc > 0) fetch(0);
+        const int tw = w4 % NT, zt0 = w4 / NT * NT, t = 16 * tw + col;   // rows 16 tw + col, columns 16 (zt0 + j) + 4 quarter + i
+        Sink<IO, VEC> so;
+        so.open(r.o, w.base, w.first, h, t, z0 + 16 * zt0 + 4 * quarter, r.dz);
+        for (int c = 0; c < nc; ++c) {
+            // (what follows from the lane is worked out anew for each chunk: kept over the loop it fills the registers, masks for every tile among it)
+            int lane_ = lane;
+            asm volatile("" : "+v"(lane_));
+            const int quarter = lane_ >> 4, col = lane_ & 15, t = 16 * tw + col;
+            const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+            const auto put = [&](const Piece<IO>& piece, __bf16 (&a)[NS][L][S::PX], int row) {
+                u32x4 f[NS];
+                piece_terms<IO>(piece, f);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    *reinterpret_cast<uint2*>(&a[s][row][o0]) = uint2{f[s][0], f[s][1]};
+                    *reinterpret_cast<uint2*>(&a[s][row][o0 + 8]) = uint2{f[s][2], f[s][3]};
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < PA; ++i) {
+                put(ra[i], lds.a, rowx + STEPX * i);
+                put(rb[i], lds.b, rowx + STEPX * i);
+            }
+            lds_barrier();                                // (orders the LDS alone: the next chunk's rows and this one's results stay on their way)
+            if (c + 1 < nc) fetch(c + 1);
+            typename S::Decays& dec = lds.d[c & 1];
+            if (16 * tw < n) {
+                const float gth = dec.gh[t], gtl = dec.gl[t], from_state = dec.dt[t] * scale;
+                bf16x8 fa[KX][NS];
+#pragma unroll
+                for (int kx = 0; kx < KX; ++kx)
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[s][t][kx * 32 + 8 * quarter]);
+                // what the state in front gives
+                f32x4 acc[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (begun || c > 0) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                        for (int kx = 0; kx < KX; ++kx) {
+                            bf16x8 fs[NP];
+#pragma unroll
+                            for (int s = 0; s < NP; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane_]);
+                            acc[j] = mma<NP - 1>(acc[j], fs, fa[kx]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[j][i] *= from_state;
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (2 * ks > tw) break;
+                    float pr[8];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int ts = 2 * ks + half;     // tile of 16 tokens s
+                        f32x4 m = {0.f, 0.f, 0.f, 0.f};
+                        if (ts <= tw) {
+#pragma unroll
+                            for (int kx = 0; kx < KX; ++kx) {
+                                bf16x8 fb[NS];
+#pragma unroll
+                                for (int s = 0; s < NS; ++s) fb[s] = *reinterpret_cast<const bf16x8*>(&lds.b[s][16 * ts + col][kx * 32 + 8 * quarter]);
+                                m = mma<NP - 1>(m, fb, fa[kx]);
+                            }
+                            const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec.gh[16 * ts + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * ts + 4 * quarter]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float x = m[i] * (scale * fast_exp2((gth - sh[i]) + (gtl - sl[i])));
+                                m[i] = ts < tw || 4 * quarter + i <= col ? x : 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) pr[4 * half + i] = m[i];
+                    }
+                    bf16x8 fp[NP];
+                    split8<NP>(pr, fp);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        bf16x8 fc[NS];
+#pragma unroll
+                        for (int s = 0; s < NS; ++s) fc[s] = across8(&lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * (zt0 + j) + 4 * (col & 3)], S::PZ);
+                        acc[j] = mma<NP - 1>(acc[j], fc, fp);
+                    }
+                }
+                so.store(acc, t0, t < n);
+            }
+            lds_barrier();
+        }
+    } else {
+        const int rowz = tid / (TZ / 8), dzo = tid % (TZ / 8) * 8;
+        constexpr int DECAYS = 7;                         // the wave that has the decays besides
+        Source<IO, PC, STEPZ, VEC> sc;
+        sc.open(r.c, w.base, w.first, h, L, false, rowz, z0 + dzo, r.dz);
+        Gates gates;
+        gates.open(p, w.base, w.first, h);
+        Piece<IO> rc[PC];
+        Gates::Raw rg{};
+        const auto fetch = [&](int c) {
+            const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+            sc.load(rc, t0, n, false);
+            if (wave == DECAYS) rg = gates.fetch(t0, lane, lane < n);
+        };
+        if (nc > 0) fetch(0);
+        // the state: rows 16 x + 4 quarter + i, column 16 w4 + col of the tile
+        f32x4 st[NX];
+        const long long page = ((long long)w.n * p.H + h) * ((long long)r.dx * r.dz);
+        const int zc = z0 + 16 * w4 + col;
+        if (!w.is_first) {
+#pragma unroll
+            for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ) + ((x * 4 + w4) * 64 + lane) * 4);
+        } else if (begun) {
+            const StatePage s(r.init + page, r.sx, r.sz, r.dx, r.dz, 4 * quarter, zc);
+#pragma unroll
+            for (int x = 0; x < NX; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st[x][i] = s.load(16 * x + i);
+        } else {
+#pragma unroll
+            for (int x = 0; x < NX; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        u32x4 held[NP][KX];                               // its terms
+        const auto hold = [&]() {
+#pragma unroll
+            for (int kx = 0; kx < KX; ++kx) {
+                const float x8[8] = {st[2 * kx][0], st[2 * kx][1], st[2 * kx][2], st[2 * kx][3], st[2 * kx + 1][0], st[2 * kx + 1][1], st[2 * kx + 1][2], st[2 * kx + 1][3]};
+                bf16x8 f[NP];
+                split8<NP>(x8, f);
+#pragma unroll
+                for (int s = 0; s < NP; ++s) held[s][kx] = __builtin_bit_cast(u32x4, f[s]);
+            }
+        };
+        if (nc > 0) {
+            if (wave == DECAYS) chunk_decays<L>(lds.d[0], gates.widen(rg), lane);
+            hold();
+        }
+        const bool wanted = r.last && w.is_last;          // the state behind the segment
+        for (int c = 0; c < nc; ++c) {
+            int lane_ = lane;
+            asm volatile("" : "+v"(lane_));
+            const int quarter = lane_ >> 4, col = lane_ & 15;
+            const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
+#pragma unroll
+            for (int i = 0; i < PC; ++i) {
+                u32x4 f[NS];
+                piece_terms<IO>(rc[i], f);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) *reinterpret_cast<u32x4*>(&lds.c[s][rowz + STEPZ * i][dzo]) = f[s];
+            }
+#pragma unroll
+            for (int kx = 0; kx < KX; ++kx)
+#pragma unroll
+                for (int s = 0; s < NP; ++s) lds.s[s][w4][kx][lane_] = held[s][kx];
+            lds_barrier();
+            if (c + 1 < nc) fetch(c + 1);
+            typename S::Decays& dec = lds.d[c & 1];
+            if (c + 1 < nc || wanted) {
+                const float ed = dec.end;
+#pragma unroll
+                for (int x = 0; x < NX; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st[x][i] *= ed;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (32 * ks >= n) break;
+                    bf16x8 fv[3];
+                    decayed_terms<IO>(lds.c, dec.dk, 1.f, ks, 16 * w4, quarter, col, fv);
+#pragma unroll
+                    for (int x = 0; x < NX; ++x) {
+                        bf16x8 fk[NS];
+#pragma unroll
+                        for (int s = 0; s < NS; ++s) fk[s] = across8(&lds.b[s][32 * ks + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)], S::PX);
+                        st[x] = mma<2>(st[x], fk, fv);
+                    }
+                }
+                if (c + 1 < nc) {
+                    hold();
+                    if (wave == DECAYS) chunk_decays<L>(lds.d[(c + 1) & 1], gates.widen(rg), lane);
+                }
+            }
+            lds_barrier();
+        }
+        if (wanted) {
+            const StatePage s(r.last + page, r.sx, r.sz, r.dx, r.dz, 4 * quarter, zc);
+#pragma unroll
+            for (int x = 0; x < NX; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s.store(16 * x + i, st[x][i]);
+        }
     }
 }
 
@@ -745,10 +864,9 @@ extern template int launch_decay<__half>(const Params&, int, int, bool, hipStrea
 
 template <typename IO, int DX, bool VEC>
 void launch_mode(const Params& p, int mode, dim3 grid, hipStream_t st) {
-    const dim3 block(THREADS);
-    if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, DX, PLAIN, VEC>), grid, block, 0, st, p);
-    else if (mode == CHUNKS) hipLaunchKernelGGL((decay_kernel<IO, DX, CHUNKS, VEC>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((decay_kernel<IO, DX, STATES, VEC>), grid, block, 0, st, p);
+    if (mode == PLAIN) hipLaunchKernelGGL((decay_kernel<IO, DX, VEC>), grid, dim3(OUT_THREADS), 0, st, p);
+    else if (mode == CHUNKS) hipLaunchKernelGGL((decay_states_kernel<IO, DX, CHUNKS, VEC>), grid, dim3(THREADS), 0, st, p);
+    else hipLaunchKernelGGL((decay_states_kernel<IO, DX, STATES, VEC>), grid, dim3(THREADS), 0, st, p);
 }
 // vec: every row of every role in pieces of 16 bytes
 template <typename IO>

@@ -106,7 +106,7 @@ int chunk_of(int dtype) { return dtype == VRWKV_F32 ? 32 : 64; }   // of the gra
 
 // workgroups of a launch of outputs that the chip holds at once
 int slots(int dtype, int dx, bool backward) {
-    const int per_cu = backward ? 1 : dtype == VRWKV_BF16 ? (dx == 64 ? 3 : 2) : dtype == VRWKV_F16 ? 2 : dx == 64 ? 2 : 1;
+    const int per_cu = backward ? 1 : dtype == VRWKV_F32 && dx == 128 ? 1 : 2;
     return per_cu * device_cus();
 }
 // Tokens of a segment.  Calls of fewer sequences and heads than fill the chip are cut, into pieces that fill it in as few rounds as it takes: a round
@@ -313,7 +313,7 @@ extern "C" int vrwkv_decay_fwd(const vrwkv_decay_args* args, void* hip_stream) {
     if (!a.y) { set_error("%s: null y", who); return VRWKV_INVALID_ARG; }
     Pieces size{nullptr};
     FwdPlan sized(a, size);
-    if ((s = check_grid(a, sized.seg_len, sized.role.tiles, THREADS, who)) != VRWKV_OK || (s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
+    if ((s = check_grid(a, sized.seg_len, sized.role.tiles, OUT_THREADS, who)) != VRWKV_OK || (s = check_workspace(a, size.used, who)) != VRWKV_OK) return s;
     Pieces ws{static_cast<char*>(a.workspace)};
     FwdPlan plan(a, ws);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
@@ -328,7 +328,6 @@ extern "C" int vrwkv_decay_fwd(const vrwkv_decay_args* args, void* hip_stream) {
     r.last = a.last;
     r.sx = a.Dv;
     r.sz = 1;
-    r.s_in = a.scale;
     r.s_upd = 1.f;
     if (r.seg && (s = launch_segments(p, a.dtype, plan.dx, st)) != VRWKV_OK) return s;
     return launch(p, a.dtype, plan.dx, PLAIN, st);
@@ -362,7 +361,6 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
         r->init = r == &b.r ? a.glast : a.state;
         r->sx = 1;                                        // rows of v's channels, columns of k's
         r->sz = a.Dv;
-        r->s_in = 1.f;
         r->s_upd = r == &b.r ? a.scale : 1.f;
     }
     if (b.r.seg) {

@@ -225,13 +225,13 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         const int c = nc - 1 - ci, t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
         // ---- operands to the LDS
         const auto put = [&](const Piece<IO>& r, __bf16 (&a)[NS][L][PX], int row) {
-            const int o0 = order_of(d0), o1 = order_of(d0 + 4);
+            const int o0 = order_of(d0);
             u32x4 t[NS];
             piece_terms<IO>(r, t);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 *reinterpret_cast<uint2*>(&a[s][row][o0]) = uint2{t[s][0], t[s][1]};
-                *reinterpret_cast<uint2*>(&a[s][row][o1]) = uint2{t[s][2], t[s][3]};
+                *reinterpret_cast<uint2*>(&a[s][row][o0 + 8]) = uint2{t[s][2], t[s][3]};
             }
         };
 #pragma unroll
