@@ -170,6 +170,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) { ret
 template <typename T>
 __device__ __forceinline__ void keep(T& x) { asm volatile("" : "+s"(x)); }
 
+// The arguments' cache lines asked for together: met one after the other, where each is first needed, they cost the start of a workgroup some 2000 cycles.
+__device__ __forceinline__ void touch(const Call& c) { asm volatile("" : : "s"(c.offsets), "s"(c.N), "s"(c.segs)); }
+__device__ __forceinline__ void touch(const Role& r) { asm volatile("" : : "s"(r.a.p), "s"(r.b.st), "s"(r.c.sh), "s"(r.o.f32), "s"(r.anchors), "s"(r.dx), "s"(r.s_upd)); }
+
 // Four channels of a row, `count` of them there.
 template <typename O, bool VEC>
 __device__ __forceinline__ void store_quad(__amdgpu_buffer_rsrc_t buf, unsigned at, int count, f32x4 x) {
@@ -489,6 +493,9 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 
     // a head's tiles, and the roles of a tile, next to each other: they read the same rows
     int id = blockIdx.x;
+    touch(p);
+    touch(p.role[0]);
+    if (MODE == STATES) touch(p.role[1]);
     const Role& r = p.role[MODE == STATES ? id & (p.n_roles - 1) : 0];
     if (MODE == STATES) id >>= p.n_roles - 1;
     const int z = id & (r.tiles - 1), h = id >> (r.tiles - 1), gid = grid_segment();
@@ -639,6 +646,8 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w4 = wave & 3;
 
     const Role& r = p.role[0];
+    touch(p);
+    touch(r);
     const int z = blockIdx.x & (r.tiles - 1), h = blockIdx.x >> (r.tiles - 1), gid = grid_segment();   // a head's tiles next to each other: they read the same rows
     if (gid >= p.segs) return;
     const Place w = find_place<OUT_THREADS>(p, gid, L, offs);

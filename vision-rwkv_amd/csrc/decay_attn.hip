@@ -373,13 +373,13 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     p.role[0] = b.s;
     if ((a.state || a.T > chunk_of(a.dtype)) && (s = launch(p, a.dtype, b.dxv, CHUNKS, st)) != VRWKV_OK) return s;
     BwdParams t = common<BwdParams>(a, b.seg_len);
-    t.q = q;
-    t.k = k;
-    t.v = v;
+    t.in[0] = q;
+    t.in[1] = k;
+    t.in[2] = v;
     t.gy = gy;
-    t.dq = out_view(b.fq ? b.fq : a.dq, a.Dk, a, b.fq != nullptr);
-    t.dk = out_view(b.fk ? b.fk : a.dk, a.Dk, a, b.fk != nullptr);
-    t.dv = out_view(b.fv ? b.fv : a.dv, a.Dv, a, b.fv != nullptr);
+    t.out[0] = out_view(b.fq ? b.fq : a.dq, a.Dk, a, b.fq != nullptr);
+    t.out[1] = out_view(b.fk ? b.fk : a.dk, a.Dk, a, b.fk != nullptr);
+    t.out[2] = out_view(b.fv ? b.fv : a.dv, a.Dv, a, b.fv != nullptr);
     t.dg = b.sums ? nullptr : b.fg ? b.fg : static_cast<float*>(a.dg);
     t.dg_sums = b.sums;
     t.chunks = b.s.anchors;
@@ -391,8 +391,8 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     t.begun = a.state != nullptr;
     t.tk = b.tk;
     t.tv = b.tv;
-    const bool vec = in_pieces(q, a.Dk, a.dtype) && in_pieces(k, a.Dk, a.dtype) && in_pieces(v, a.Dv, a.dtype) && in_pieces(gy, a.Dv, a.dtype) && in_pieces(t.dq, a.Dk) && in_pieces(t.dk, a.Dk) &&
-                     in_pieces(t.dv, a.Dv);
+    const bool vec = in_pieces(q, a.Dk, a.dtype) && in_pieces(k, a.Dk, a.dtype) && in_pieces(v, a.Dv, a.dtype) && in_pieces(gy, a.Dv, a.dtype) && in_pieces(t.out[0], a.Dk) && in_pieces(t.out[1], a.Dk) &&
+                     in_pieces(t.out[2], a.Dv);
     s = a.dtype == VRWKV_F32 ? launch_decay_bwd<float>(t, vec, st) : a.dtype == VRWKV_BF16 ? launch_decay_bwd<__hip_bfloat16>(t, vec, st) : launch_decay_bwd<__half>(t, vec, st);
     if (s != VRWKV_OK) return s;
     Sums sums{};

@@ -24,8 +24,8 @@ constexpr int BWD_THREADS = 768;
 enum Kind { DQ = 0, DK = 1, DV = 2 };
 
 struct BwdParams : Call {
-    View q, k, v, gy;
-    OutView dq, dk, dv;                                   // (parts lie rows * heads * channels apart)
+    View in[3], gy;                                       // q, k, v: what the waves of a kind stage, and
+    OutView out[3];                                       // dq, dk, dv: what they make, next to each other: a kind reads its own with one load (parts lie rows * heads * channels apart)
     float* dg;                                            // [tiles][row][head]
     double* dg_sums;                                      // or, for decays that all tokens share, [segment][tiles][head]
     const float *chunks;                                  // [chunk][head][tile of k][tile of v]: S0, rows of v's channels and columns of k's, as the accumulators lie
@@ -61,15 +61,17 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     __shared__ int offs[BWD_THREADS];
     const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kind = wave >> 2, w4 = wave & 3;
+    touch(p);
+    asm volatile("" : : "s"(p.in[0].p), "s"(p.in[1].sb), "s"(p.in[2].st), "s"(p.gy.sh), "s"(p.out[1].p), "s"(p.out[2].p), "s"(p.dg), "s"(p.tv));
     // a head's tiles next to each other: they read the same rows
     const int shift = (p.tk - 1) + (p.tv - 1), tile = blockIdx.x & ((1 << shift) - 1), h = blockIdx.x >> shift, gid = grid_segment();
     if (gid >= p.segs) return;
     const int ik = tile & (p.tk - 1), iv = tile >> (p.tk - 1), k0 = 64 * ik, v0 = 64 * iv;
-    const auto part = [&](OutView v, int i, int D) {
-        if (v.p && v.f32) v.p = static_cast<float*>(v.p) + i * p.rows * p.H * D;
+    const auto out_of = [&](int kind) {
+        OutView v = p.out[kind];
+        if (v.p && v.f32) v.p = static_cast<float*>(v.p) + (kind == DV ? ik : iv) * p.rows * p.H * (kind == DV ? p.Dv : p.Dk);
         return v;
     };
-    const OutView out_q = part(p.dq, iv, p.Dk), out_k = part(p.dk, iv, p.Dk), out_v = part(p.dv, ik, p.Dv);
     float* const dg_part = FLOW && p.dg ? p.dg + tile * p.rows * p.H : nullptr;
     double* const dg_sum = FLOW && p.dg_sums ? p.dg_sums + ((long long)gid * p.tk * p.tv + tile) * p.H + h : nullptr;
 
@@ -78,10 +80,9 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         const int front = w.front, back = w.back, rows = front + max(0, p.T - back);
         for (int i = gid * 12 + wave; i < rows; i += p.segs * 12) {
             const long long row = i < front ? i : back + (i - front);
-            const OutView* const outs[3] = {&out_q, &out_k, &out_v};
 #pragma unroll
             for (int o = 0; o < 3; ++o) {
-                const OutView& v = *outs[o];
+                const OutView v = out_of(o);
                 const int d = (o < 2 ? k0 : v0) + lane;
                 if (v.p && d < (o < 2 ? p.Dk : p.Dv)) {
                     const long long at = row * v.st + h * v.sh + d;
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     const bool gy_mine = kind < DV && (PIECES == 2 || row0 < 16);
     Source<IO, PIECES, 32, VEC> sa;
     Source<IO, 1, 32, VEC> sb;
-    sa.open(kind == DQ ? p.q : kind == DK ? p.k : p.v, w.base, w.first, h, L, false, row0, (kind == DV ? v0 : k0) + d0, kind == DV ? p.Dv : p.Dk);
+    sa.open(p.in[kind], w.base, w.first, h, L, false, row0, (kind == DV ? v0 : k0) + d0, kind == DV ? p.Dv : p.Dk);
     sb.open(p.gy, w.base, w.first, h, L, false, gy_mine ? gy_row : L, v0 + d0, p.Dv);
     Gates gates;
     gates.open(p, w.base, w.first, h);
@@ -175,8 +176,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     }
     const int tw = w4 % NT, zt0 = w4 / NT * NT;           // this wave's tile of tokens, its first tile of channels
     Sink<IO, VEC> so;
-    if (kind == DV) so.open(out_v, w.base, w.first, h, 16 * tw + col, v0 + 16 * zt0 + 4 * quarter, p.Dv);
-    else so.open(kind == DK ? out_k : out_q, w.base, w.first, h, 16 * tw + col, k0 + 16 * zt0 + 4 * quarter, p.Dk);
+    so.open(out_of(kind), w.base, w.first, h, 16 * tw + col, (kind == DV ? v0 : k0) + 16 * zt0 + 4 * quarter, kind == DV ? p.Dv : p.Dk);
     float* dg = dg_part ? dg_part + ((long long)w.base * p.T + w.first) * p.H + h : nullptr;
     double dg_total = 0.;                                 // (the light wave) of the segment's tokens
     int H = p.H;
