@@ -59,44 +59,72 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
 struct Sum {
     const float* part;
     void* out;
-    long long count, apart;                               // results; numbers from part to part
-    int D, share, parts;
+    long long count, apart;                               // results, or fours of them; numbers from part to part
+    int D, share, parts, fours;
 };
 struct Sums {
     Sum s[3];
+    const float* decay_part;                              // dg (rows, H) = the sums of (tiles, rows, H), of which each has decay_count numbers; or
+    const double* decay_sums;                             // dg (H) = the sums of (segments and tiles, H), in 64 bits: a workgroup for each head
+    void* dg;
+    long long decay_count, decay_n;
+    int n, g_dtype, tiles, H;                             // sums of s
 };
+__device__ __forceinline__ void put_decay(const Sums& all, long long i, float x) {
+    if (all.g_dtype == VRWKV_F32) static_cast<float*>(all.dg)[i] = x;
+    else if (all.g_dtype == VRWKV_BF16) static_cast<__hip_bfloat16*>(all.dg)[i] = from_f32<__hip_bfloat16>(x);
+    else static_cast<__half*>(all.dg)[i] = from_f32<__half>(x);
+}
+// All that a call adds up, in one launch: y 0 .. n - 1 the gradients of s, y = n those of the decays.
 template <typename IO>
-__global__ __launch_bounds__(THREADS) void head_sum_kernel(const Sums all) {
-    const Sum t = all.s[blockIdx.y];
-    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < t.count; i += (long long)gridDim.x * THREADS) {
-        const float* q = t.part + i / t.D * t.share * t.D + i % t.D;
-        float s = 0.f;
-        for (int p = 0; p < t.parts; ++p)
-            for (int j = 0; j < t.share; ++j) s += q[p * t.apart + j * t.D];
-        static_cast<IO*>(t.out)[i] = from_f32<IO>(s);
-    }
-}
-// out (rows, H) = the sums of part (tiles, rows, H)
-template <typename G>
-__global__ __launch_bounds__(THREADS) void decay_grad_kernel(const float* part, G* out, long long count, int tiles) {
-    for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < count; i += (long long)gridDim.x * THREADS) {
-        float s = part[i];
-        for (int t = 1; t < tiles; ++t) s += part[t * count + i];
-        out[i] = from_f32<G>(s);
-    }
-}
-// out (H) = the sums of the segments' and tiles' totals, in 64 bits: a workgroup for each head
-template <typename G>
-__global__ __launch_bounds__(THREADS) void decay_total_kernel(const double* sums, G* out, long long n, int H) {
-    __shared__ double red[THREADS / 64];
-    const int h = blockIdx.x, lane = threadIdx.x & 63;
-    double s = 0.;
-    for (long long i = threadIdx.x; i < n; i += THREADS) s += sums[i * H + h];
+__global__ __launch_bounds__(THREADS) void sums_kernel(const Sums all) {
+    const long long first = (long long)blockIdx.x * THREADS + threadIdx.x, step = (long long)gridDim.x * THREADS;
+    if ((int)blockIdx.y < all.n) {
+        const Sum t = all.s[blockIdx.y];
+        if (t.fours) {
+            const int D4 = t.D / 4;
+            for (long long i = first; i < t.count; i += step) {
+                const float* q = t.part + i / D4 * t.share * t.D + i % D4 * 4;
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+                for (int p = 0; p < t.parts; ++p)
+                    for (int j = 0; j < t.share; ++j) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(q + p * t.apart + j * t.D);
 #pragma unroll
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    if (lane == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) out[h] = from_f32<G>((float)((red[0] + red[1]) + (red[2] + red[3])));
+                        for (int c = 0; c < 4; ++c) s[c] += x[c];
+                    }
+                IO o[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[c] = from_f32<IO>(s[c]);
+                __builtin_memcpy(static_cast<IO*>(t.out) + 4 * i, o, sizeof(o));
+            }
+            return;
+        }
+        for (long long i = first; i < t.count; i += step) {
+            const float* q = t.part + i / t.D * t.share * t.D + i % t.D;
+            float s = 0.f;
+            for (int p = 0; p < t.parts; ++p)
+                for (int j = 0; j < t.share; ++j) s += q[p * t.apart + j * t.D];
+            static_cast<IO*>(t.out)[i] = from_f32<IO>(s);
+        }
+    } else if (all.decay_part) {
+        for (long long i = first; i < all.decay_count; i += step) {
+            float s = all.decay_part[i];
+            for (int t = 1; t < all.tiles; ++t) s += all.decay_part[t * all.decay_count + i];
+            put_decay(all, i, s);
+        }
+    } else {
+        __shared__ double red[THREADS / 64];
+        for (int h = blockIdx.x; h < all.H; h += gridDim.x) {
+            double s = 0.;
+            for (long long i = threadIdx.x; i < all.decay_n; i += THREADS) s += all.decay_sums[i * all.H + h];
+#pragma unroll
+            for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+            __syncthreads();                               // (the head in front has been read)
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+            __syncthreads();
+            if (threadIdx.x == 0) put_decay(all, h, (float)((red[0] + red[1]) + (red[2] + red[3])));
+        }
+    }
 }
 
 size_t elem(int dtype) { return dtype == VRWKV_F32 ? 4 : 2; }
@@ -279,16 +307,6 @@ int check_workspace(const vrwkv_decay_args& a, size_t need, const char* who) {
     if (need && ((size_t)a.workspace & 15)) { set_error("%s: workspace must be 16-byte aligned", who); return VRWKV_INVALID_ARG; }
     return VRWKV_OK;
 }
-template <typename G>
-void decay_sums(const BwdPlan& b, const vrwkv_decay_args& a, hipStream_t st) {
-    if (b.sums)
-        hipLaunchKernelGGL((decay_total_kernel<G>), dim3(a.H), dim3(THREADS), 0, st, b.sums, static_cast<G*>(a.dg), segment_total(a, b.seg_len) * b.tk * b.tv, a.H);
-    else {
-        const long long count = rows_of(a) * a.H;
-        const unsigned grid = (unsigned)std::min<long long>((count + THREADS - 1) / THREADS, 4096);
-        hipLaunchKernelGGL((decay_grad_kernel<G>), dim3(grid), dim3(THREADS), 0, st, b.fg, static_cast<G*>(a.dg), count, b.tk * b.tv);
-    }
-}
 
 }  // namespace
 }  // namespace decay
@@ -396,27 +414,35 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     s = a.dtype == VRWKV_F32 ? launch_decay_bwd<float>(t, vec, st) : a.dtype == VRWKV_BF16 ? launch_decay_bwd<__hip_bfloat16>(t, vec, st) : launch_decay_bwd<__half>(t, vec, st);
     if (s != VRWKV_OK) return s;
     Sums sums{};
-    int n_sums = 0;
-    long long most = 0;
+    long long most = 1;
     const auto add = [&](const float* part, void* out, int heads, int D, int parts) {
         if (!part) return;
         const long long rows = rows_of(a);
-        sums.s[n_sums++] = Sum{part, out, rows * heads * D, rows * a.H * D, D, a.H / heads, parts};
-        most = std::max(most, rows * heads * D);
+        const bool fours = D % 4 == 0 && ((size_t)out & 15) == 0;
+        const long long count = rows * heads * D / (fours ? 4 : 1);
+        sums.s[sums.n++] = Sum{part, out, count, rows * a.H * D, D, a.H / heads, parts, fours};
+        most = std::max(most, count);
     };
     add(b.fq, a.dq, a.Hq, a.Dk, b.tv);
     add(b.fk, a.dk, a.Hk, a.Dk, b.tv);
     add(b.fv, a.dv, a.Hv, a.Dv, b.tk);
-    if (n_sums) {
-        const dim3 grid((unsigned)std::min<long long>((most + THREADS - 1) / THREADS, 8192), n_sums);
-        if (a.dtype == VRWKV_F32) hipLaunchKernelGGL((head_sum_kernel<float>), grid, dim3(THREADS), 0, st, sums);
-        else if (a.dtype == VRWKV_BF16) hipLaunchKernelGGL((head_sum_kernel<__hip_bfloat16>), grid, dim3(THREADS), 0, st, sums);
-        else hipLaunchKernelGGL((head_sum_kernel<__half>), grid, dim3(THREADS), 0, st, sums);
+    const bool decays = b.sums || b.fg;
+    if (decays) {
+        sums.decay_part = b.fg;
+        sums.decay_sums = b.sums;
+        sums.dg = a.dg;
+        sums.decay_count = rows_of(a) * a.H;
+        sums.decay_n = segment_total(a, b.seg_len) * b.tk * b.tv;
+        sums.g_dtype = a.g_dtype;
+        sums.tiles = b.tk * b.tv;
+        sums.H = a.H;
+        most = std::max(most, b.fg ? sums.decay_count : (long long)a.H * THREADS);
     }
-    if (b.sums || b.fg) {
-        if (a.g_dtype == VRWKV_F32) decay_sums<float>(b, a, st);
-        else if (a.g_dtype == VRWKV_BF16) decay_sums<__hip_bfloat16>(b, a, st);
-        else decay_sums<__half>(b, a, st);
+    if (sums.n || decays) {
+        const dim3 grid((unsigned)std::min<long long>((most + THREADS - 1) / THREADS, 8192), sums.n + (decays ? 1 : 0));
+        if (a.dtype == VRWKV_F32) hipLaunchKernelGGL((sums_kernel<float>), grid, dim3(THREADS), 0, st, sums);
+        else if (a.dtype == VRWKV_BF16) hipLaunchKernelGGL((sums_kernel<__hip_bfloat16>), grid, dim3(THREADS), 0, st, sums);
+        else hipLaunchKernelGGL((sums_kernel<__half>), grid, dim3(THREADS), 0, st, sums);
     }
     return check_launch(who);
 }

@@ -214,7 +214,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     };
     if (nc > 0) {
         if (wave == LIGHT) put_decays(lds.d[0]);
-        if (kind != DQ) hold();
+        if (kind == DK || (kind == DV && have)) hold();
     }
 
     for (int ci = 0; ci < nc; ++ci) {
