@@ -240,11 +240,11 @@ struct Sink {
         at = (unsigned)(row * pitch + d * e);
         count = dim - d;
     }
+    // (called on every way through a chunk, so that what was asked for before is waited for without waiting for this)
     template <int N>
     __device__ __forceinline__ void store(const f32x4 (&x)[N], int token, bool there) const {
-        if (!p) return;
         const auto buf = buffer_at(p + (long long)token * pitch);
-        const int have = there ? count : 0;
+        const int have = there && p ? count : 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             if (f32) store_quad<float, VEC>(buf, at + 64 * j, have - 16 * j, x[j]);
@@ -697,6 +697,9 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
             lds_barrier();                                // (orders the LDS alone: the next chunk's rows and this one's results stay on their way)
             if (c + 1 < nc) fetch(c + 1);
             typename S::Decays& dec = lds.d[c & 1];
+            f32x4 acc[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (16 * tw < n) {
                 const float gth = dec.gh[t], gtl = dec.gl[t], from_state = dec.dt[t] * scale;
                 bf16x8 fa[KX][NS];
@@ -705,9 +708,6 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
 #pragma unroll
                     for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[s][t][kx * 32 + 8 * quarter]);
                 // what the state in front gives
-                f32x4 acc[NT];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (begun || c > 0) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -758,8 +758,8 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
                         acc[j] = mma<NP - 1>(acc[j], fc, fp);
                     }
                 }
-                so.store(acc, t0, t < n);
             }
+            so.store(acc, t0, t < n);
             lds_barrier();
         }
     } else {

@@ -318,18 +318,19 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                 }
             }
         };
+        f32x4 acc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (kind == DQ) {
             if (16 * tw < n) {
                 const float gh = dec.gh[r0], gl = dec.gl[r0], dt = dec.dt[r0];
                 bf16x8 fo[2][NS];
                 row_of(lds.gy, r0, 0, fo[0]);
                 row_of(lds.gy, r0, 1, fo[1]);
-                f32x4 acc[NT], flow[FLOW ? NT : 1];       // flow [tile of j]: sums over s < j of the terms of row t
+                f32x4 flow[FLOW ? NT : 1];                // [tile of j]: sums over s < j of the terms of row t
                 float in = 0.f;
 #pragma unroll
                 for (int j = 0; j < (FLOW ? NT : 1); ++j) flow[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (begun(c)) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -413,7 +414,6 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                         }
                     }
                 }
-                so.store(acc, t0, r0 < n);
                 if constexpr (FLOW) {
                     in += __shfl_xor(in, 16);
                     in += __shfl_xor(in, 32);
@@ -428,6 +428,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                     if ((index >> 2) < NT) flows.inner[w4][16 * (index >> 2) + 4 * quarter + (index & 3)] = cf;
                 }
             } else if (FLOW && lane_ < L) flows.inner[w4][lane_] = 0.f;
+            so.store(acc, t0, r0 < n);
             forget();
         } else if (kind == DK) {
             if constexpr (FLOW) {                         // <S0, X>
@@ -449,10 +450,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                 bf16x8 fv[2][NS];
                 row_of(lds.v, r0, 0, fv[0]);
                 row_of(lds.v, r0, 1, fv[1]);
-                f32x4 acc[NT];
                 float out = 0.f;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (have) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -473,7 +471,6 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                     }
                 }
                 gathered(lds.gy, fv, lds.q, gh, gl, acc);
-                so.store(acc, t0, r0 < n);
                 if constexpr (FLOW) {
                     out += __shfl_xor(out, 16);
                     out += __shfl_xor(out, 32);
@@ -481,6 +478,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                 }
             }
             have = true;
+            so.store(acc, t0, r0 < n);
             hold();
             if (wave == LIGHT) {
                 if constexpr (FLOW) {
@@ -494,9 +492,6 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                 bf16x8 fk[2][NS];
                 row_of(lds.k, r0, 0, fk[0]);
                 row_of(lds.k, r0, 1, fk[1]);
-                f32x4 acc[NT];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (have) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
@@ -516,8 +511,8 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                     }
                 }
                 gathered(lds.q, fk, lds.gy, gh, gl, acc);
-                so.store(acc, t0, r0 < n);
             }
+            so.store(acc, t0, r0 < n);
             // ---- X in front of the chunk
             const float ed = dec.end;
 #pragma unroll
