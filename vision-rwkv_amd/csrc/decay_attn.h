@@ -5,6 +5,8 @@
 // four matrix products.  The state in front of each chunk, and the same sum back along the tokens (b, c = gy, q in the places of k, v: the gradient of a
 // state), which the gradients want (decay_bwd.h), are this kernel's without its outputs.
 // Calls of few sequences are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
+// 64 x 196 tokens, 12 heads of 64, bf16: 23.6 us, 90 MB at 3.8 TB/s.  4 x 16384 in fp16, where operands have two terms: 67 us for the segments' states, 6 to add them up
+// and 136 for the outputs, of which the vector units are busy 47 %, the LDS 51, the matrix units 24: bound by a chunk's chain of staging, products, exponentials and products again.
 #pragma once
 #include "wave_sum.h"
 #include "wkv6_chunk_common.h"
@@ -480,7 +482,8 @@ __device__ __forceinline__ void decayed_terms(const __bf16 (&c)[in_terms<IO>][L]
     split8<3>(x8, f);
 }
 
-// A segment's own state, or the states in front of a segment's chunks.
+// A segment's own state, or the states in front of a segment's chunks.  Four waves, 16 columns each, several workgroups a compute unit; four more that stage the next
+// chunk beside them were slower (4 x 16384 x 12 fp16: 67 us without, 87 with).
 template <typename IO, int DX, int MODE, bool VEC>
 __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) void decay_states_kernel(const Params p) {
     using S = Lds<IO, DX, MODE>;
@@ -633,7 +636,8 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 }
 
 // Outputs.  Eight waves of two kinds, which need nothing of each other between two barriers: four take the tokens' outputs (16 tokens each), four the state
-// behind the chunk (16 columns each), its terms for the next one and the decays.
+// behind the chunk (16 columns each), its terms for the next one and the decays.  (Four waves that did one after the other: one image of 196 tokens 11.9 us, so 9.8; 2 x 4150 x 12
+// fp32 59.5, so 55; 4 x 16384 x 12 fp16 197, so 190.)
 template <typename IO, int DX, bool VEC>
 __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX, PLAIN>)>)) void decay_kernel(const Params p) {
     using S = Lds<IO, DX, PLAIN>;
