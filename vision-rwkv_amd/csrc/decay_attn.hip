@@ -8,50 +8,53 @@ namespace vrwkv {
 namespace decay {
 namespace {
 
-// The state in front of each segment from the segments' own ones: a lane carries four numbers along the sequence.
-// Grid (DX / 16 * N * H * tiles, 1, roles).  Eight segments' states are on their way at
-// a time: one by one they were 0.35 us each.
-template <int DX>
+// The state in front of each segment from the segments' own ones: a lane carries four numbers, of XS rows of fragments, along the sequence.
+// Grid (DX / 16 / XS * N * H * tiles, 1, roles).  Several segments' states are on their way at a time: one by one they were 0.35 us each.
+template <int DX, int XS>
 __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
+    constexpr int XG = DX / 16 / XS, U = XS == 1 ? 8 : 4;
+    touch(p);
     const Role& r = p.role[blockIdx.z];
-    int id = blockIdx.x / (DX / 16);
+    int id = blockIdx.x / XG;
     const int z = id % r.tiles;
     id /= r.tiles;
     const int h = id % p.H, n = id / p.H;
     const Place w = sequence_place(p, n, 64);
-    const int x = blockIdx.x % (DX / 16), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int x0 = blockIdx.x % XG * XS, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int first = first_segment(p, n, w.first), count = segment_count(p, w.len);
     if (count == 1) return;                               // (starts from what it is given)
-    f32x4 carry = {0.f, 0.f, 0.f, 0.f};
-    if (r.init) {
-        const float* page = r.init + ((long long)n * p.H + h) * ((long long)r.dx * r.dz);
-        const int zc = z * TZ + 16 * wave + (lane & 15);
+    f32x4 carry[XS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int xc = 16 * x + 4 * (lane >> 4) + i;
-            if (xc < r.dx && zc < r.dz) carry[i] = page[xc * r.sx + zc * r.sz];
-        }
+    for (int x = 0; x < XS; ++x) carry[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (r.init) {
+        const StatePage s(r.init + ((long long)n * p.H + h) * ((long long)r.dx * r.dz), r.sx, r.sz, r.dx, r.dz, 16 * x0 + 4 * (lane >> 4), z * TZ + 16 * wave + (lane & 15));
+#pragma unroll
+        for (int x = 0; x < XS; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) carry[x][i] = s.load(16 * x + i);
     }
     const auto at = [&](int i) { return ((long long)(first + (r.reverse ? count - 1 - i : i)) * p.H + h); };    // the i-th on the way
-    const long long in_tile = ((long long)x * 4 + wave) * 64 * 4 + lane * 4;
-    constexpr int U = 8;
+    const long long in_tile = ((long long)x0 * 4 + wave) * 64 * 4 + lane * 4;
     for (int i0 = 0; i0 < count; i0 += U) {
-        f32x4 own[U];
+        f32x4 own[U][XS];
         float d[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i0 + u + 1 < count) {                     // (the last one on the way has not been made)
-                own[u] = *reinterpret_cast<const f32x4*>(r.seg + (at(i0 + u) * r.tiles + z) * (DX * TZ) + in_tile);
+#pragma unroll
+                for (int x = 0; x < XS; ++x) own[u][x] = *reinterpret_cast<const f32x4*>(r.seg + (at(i0 + u) * r.tiles + z) * (DX * TZ) + in_tile + x * 1024);
                 d[u] = r.seg_decay[at(i0 + u)];
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i0 + u < count) {
-                if (i0 + u > 0) *reinterpret_cast<f32x4*>(r.seg + (at(i0 + u) * r.tiles + z) * (DX * TZ) + in_tile) = carry;
-                if (i0 + u + 1 < count)
+            if (i0 + u < count)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) carry[c] = fmaf(carry[c], d[u], own[u][c]);
-            }
+                for (int x = 0; x < XS; ++x) {
+                    if (i0 + u > 0) *reinterpret_cast<f32x4*>(r.seg + (at(i0 + u) * r.tiles + z) * (DX * TZ) + in_tile + x * 1024) = carry[x];
+                    if (i0 + u + 1 < count)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) carry[x][c] = fmaf(carry[x][c], d[u], own[u][x][c]);
+                }
     }
 }
 
@@ -245,9 +248,14 @@ int launch(const Params& p, int dtype, int dx, int mode, hipStream_t st) {
 int launch_segments(const Params& p, int dtype, int dx, hipStream_t st) {
     const int s = launch(p, dtype, dx, STATES, st);
     if (s != VRWKV_OK) return s;
-    const dim3 grid((unsigned)(dx / 16 * (long long)p.N * p.H * p.role[0].tiles), 1, p.n_roles), block(THREADS);
-    if (dx == 64) hipLaunchKernelGGL((segments_kernel<64>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((segments_kernel<128>), grid, block, 0, st, p);
+    // (many sequences, most of them not cut: a quarter of the workgroups, 48 packed prompts of 16 heads 10.2 to 8.1 us; few long ones: all that there may be)
+    const long long sequences = (long long)p.N * p.H * p.role[0].tiles;
+    const int wide = sequences * (dx / 16) > 2048 ? 4 : 1;
+    const dim3 grid((unsigned)(dx / 16 / wide * sequences), 1, p.n_roles), block(THREADS);
+    if (dx == 64 && wide == 1) hipLaunchKernelGGL((segments_kernel<64, 1>), grid, block, 0, st, p);
+    else if (dx == 64) hipLaunchKernelGGL((segments_kernel<64, 4>), grid, block, 0, st, p);
+    else if (wide == 1) hipLaunchKernelGGL((segments_kernel<128, 1>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((segments_kernel<128, 4>), grid, block, 0, st, p);
     return check_launch("decay_attention (segments)");
 }
 void take_segments(Role& r, Pieces& ws, const vrwkv_decay_args& a, long long segs, int dx) {

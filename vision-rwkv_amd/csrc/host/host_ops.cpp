@@ -8,7 +8,7 @@
 //   Bi-WKV training, 64 x 196 x 768 bf16 (kernels 56)           119.6 -> 76.1        2 x 4150 x 768 fp32 (kernels 120)   128 -> 120
 //   wkv6 training, 8 x 577 x 384 fp32 (kernels 115)             159 -> 116
 //   twelve native blocks, 1 x 196 x 192 bf16 (kernels 397)      602 -> 507
-//   decay_attention_step, 1 sequence of 12 heads (kernel 6)     18.2 -> 5.4
+//   decay_attention_step, 1 sequence of 12 heads (kernel 5)     18.2 -> 5.4
 //
 // The operators take the plain case: exact tensors and parameters, contiguous, on the current GPU, of the types that the kernels read as
 // they lie, outside every transform, mode and trace.  To everything else they answer None, and the Python classes in ops.py go on as
