@@ -141,8 +141,9 @@ int slots(int dtype, int dx, bool backward) {
     return per_cu * device_cus();
 }
 // Tokens of a segment.  Calls of fewer sequences and heads than fill the chip are cut, into pieces that fill it in as few rounds as it takes: a round
-// lasts as long as its longest piece's chunks and about two more for its start; pieces cost another pass over their rows for their states,
-// half as long, and one over the states.
+// lasts as long as its longest piece's chunks and two or three more for its start; pieces cost another pass over their rows for their states,
+// half as long, and one over the states.  (Gradients of 48 sequences of 577 tokens in tiles of 64 of 80 channels, fp16: 1 piece 130 us, 2 pieces 109, 3 119, 5 105; of 24 of 4150,
+// fp32: 8 pieces 215, 10 189, 11 222, 22 202.  Outputs of the latter: 10 pieces 60, 13 63, 17 55, 22 57.)
 int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool backward) {
     const long long wgs = (long long)a.H * tiles * roles, room = slots(a.dtype, dx, backward);
     if (!a.offsets) {
@@ -151,9 +152,12 @@ int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool ba
         double least = 1e30;
         for (int pieces = 1; pieces <= std::min(chunks / 2, 64) || pieces == 1; ++pieces) {
             const int len = (chunks + pieces - 1) / pieces, n = (chunks + len - 1) / len;
-            const double rounds = (double)((wgs * a.N * n + room - 1) / room), once = rounds * (len + 2);
-            // (backward: the pass over the chunks' states a third of the time beside it, the segments' states a third of its rows' again)
-            const double cost = backward ? 1.35 * once + (n == 1 ? 0. : 0.3 * once + 2 + n / 16.0) : n == 1 ? once : 1.5 * once + 3 + n / 16.0;
+            const auto rounds = [&](long long slots) { return (double)((wgs * a.N * n + slots - 1) / slots); };
+            double cost;
+            if (backward) {                               // (the passes over states hold three workgroups a compute unit, and take 0.43 of the gradients' time; one of them without a cut)
+                const double states = 0.43 * rounds(3LL * device_cus()) * (len + 2.7);
+                cost = rounds(room) * (len + 2.7) + (n == 1 ? states : 2 * states + 0.9);
+            } else cost = n == 1 ? rounds(room) * (len + 2) : 1.5 * rounds(room) * (len + 2) + 3 + n / 16.0;
             if (cost < least) { least = cost; best = len; }
         }
         return best * 64;
