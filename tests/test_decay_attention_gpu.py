@@ -449,6 +449,31 @@ def test_many_short_sequences(N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [3000, 300000])
+def test_packed_rows_of_one_token(N):
+    """Thousands of packed sequences of one token, empty ones among them, are the rows of a batch of one token each: the same bits."""
+    gen = torch.Generator(DEV).manual_seed(N)
+    taken = torch.rand(N, generator=gen, device=DEV) < 0.8
+    offsets = torch.cat([torch.zeros(1, dtype=torch.long, device=DEV), taken.long().cumsum(0)])
+    B = int(offsets[-1])
+    q, k, v, g, S = make(B, 1, 1, 1, 1, 1, 8, 8, "fp32", state=N, seed=1)
+    gy = torch.randn(B, 1, 1, 8, generator=gen, device=DEV)
+    gl = torch.randn(N, 1, 8, 8, generator=gen, device=DEV)
+
+    def run(packed):
+        ts = [(t.transpose(0, 1) if packed else t).clone().requires_grad_() for t in (q, k, v, g)] + [(S if packed else S[taken]).clone().requires_grad_()]
+        y, last = vr.decay_attention(*ts[:4], scale=0.5, state=ts[4], offsets=offsets if packed else None, return_state=True)
+        grads = torch.autograd.grad((y, last), ts, (gy.transpose(0, 1), gl) if packed else (gy, gl[taken]))
+        return [y, *grads[:4]], last, grads[4]
+    rows, last, dstate = run(True)
+    want_rows, want_last, want_dstate = run(False)
+    for a, b in zip(rows, want_rows):
+        assert torch.equal(a.transpose(0, 1), b)
+    assert torch.equal(last[taken], want_last) and torch.equal(last[~taken], S[~taken])
+    assert torch.equal(dstate[taken], want_dstate) and torch.equal(dstate[~taken], gl[~taken])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "fp16"])
 def test_the_same_without_the_host_module(dtype, monkeypatch):
     """Through the Python classes: the same kernels, bit for bit."""

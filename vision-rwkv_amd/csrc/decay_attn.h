@@ -117,12 +117,17 @@ __device__ __forceinline__ Place find_place(const Call& p, int gid, int L, int* 
             w.valid = true;
         }
     } else {
-        int seen = 0;
-        for (int m = 0; m < p.N; m += THREADS_) {
-            const int i = m + threadIdx.x;
-            seen += __syncthreads_count(i < p.N && offset_at(p, min(i, p.N - 1)) / p.seg_len + i <= gid);
-        }
-        const int n = __builtin_amdgcn_readfirstlane(seen - 1);
+        // the last sequence that begins at this segment or in front of it: every step-th one looked at together, then those behind the last that does
+        int n = 0, size = p.N, step;
+        do {
+            step = (size + THREADS_ - 1) / THREADS_;
+            const int i = min((int)threadIdx.x * step, size), at = n + min(i, size - 1);
+            const int seen = __syncthreads_count(i < size && offset_at(p, at) / p.seg_len + at <= gid);
+            if (seen == 0) { n = -1; break; }
+            n += (seen - 1) * step;
+            size = min(step, size - (seen - 1) * step);
+        } while (step > 1);
+        n = __builtin_amdgcn_readfirstlane(n);
         if (n >= 0) w = sequence_place(p, n, L);
         w.front = offset_at(p, 0);
         w.back = offset_at(p, p.N);
