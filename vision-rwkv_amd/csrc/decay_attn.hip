@@ -143,7 +143,8 @@ int slots(int dtype, int dx, bool backward) {
 // Tokens of a segment.  Calls of fewer sequences and heads than fill the chip are cut, into pieces that fill it in as few rounds as it takes: a round
 // lasts as long as its longest piece's chunks and two or three more for its start; pieces cost another pass over their rows for their states,
 // half as long, and one over the states.  (Gradients of 48 sequences of 577 tokens in tiles of 64 of 80 channels, fp16: 1 piece 130 us, 2 pieces 109, 3 119, 5 105; of 24 of 4150,
-// fp32: 8 pieces 215, 10 189, 11 222, 22 202.  Outputs of the latter: 10 pieces 60, 13 63, 17 55, 22 57.)
+// fp32: 8 pieces 215, 10 189, 11 222, 22 202.  Outputs of the latter: 10 pieces 60, 13 63, 17 55, 22 57; of 48
+// of 16384, fp16: 8 pieces 219, 10 189, 11 206, 16 182, 20 194, 32 190.)
 int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool backward) {
     const long long wgs = (long long)a.H * tiles * roles, room = slots(a.dtype, dx, backward);
     if (!a.offsets) {
@@ -157,7 +158,11 @@ int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool ba
             if (backward) {                               // (the passes over states hold three workgroups a compute unit, and take 0.43 of the gradients' time; one of them without a cut)
                 const double states = 0.43 * rounds(3LL * device_cus()) * (len + 2.7);
                 cost = rounds(room) * (len + 2.7) + (n == 1 ? states : 2 * states + 0.9);
-            } else cost = n == 1 ? rounds(room) * (len + 2) : 1.5 * rounds(room) * (len + 2) + 3 + n / 16.0;
+            } else {                                      // (a second workgroup makes a compute unit's round 1.3 to 1.55 times as long; the rounds of more overlap)
+                const double load = (double)(wgs * a.N * n) / device_cus();
+                const double once = (room == device_cus() ? rounds(room) : load <= 1 ? 1 : load <= 2 ? 1 + 0.28 * load : 1.75 + 0.6 * (load - 2)) * (len + 2);
+                cost = n == 1 ? once : 1.5 * once + 3 + n / 16.0;
+            }
             if (cost < least) { least = cost; best = len; }
         }
         return best * 64;
