@@ -5,8 +5,8 @@
 // four matrix products.  The state in front of each chunk, and the same sum back along the tokens (b, c = gy, q in the places of k, v: the gradient of a
 // state), which the gradients want (decay_bwd.h), are this kernel's without its outputs.
 // Calls of few sequences are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
-// 64 x 196 tokens, 12 heads of 64, bf16: 23.6 us, 90 MB at 3.8 TB/s.  4 x 16384 in fp16, where operands have two terms: 67 us for the segments' states, 6 to add them up
-// and 136 for the outputs, of which the vector units are busy 47 %, the LDS 51, the matrix units 24: bound by a chunk's chain of staging, products, exponentials and products again.
+// 64 x 196 tokens, 12 heads of 64, bf16: 23.6 us, 90 MB at 3.8 TB/s.  4 x 16384 in fp16, where operands have two terms: 62 us for the segments' states, 10 to add them up
+// and 128 for the outputs, of which the vector units are busy 47 %, the LDS 51, the matrix units 24: bound by a chunk's chain of staging, products, exponentials and products again.
 #pragma once
 #include "wave_sum.h"
 #include "wkv6_chunk_common.h"
