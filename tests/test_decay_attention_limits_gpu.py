@@ -1,0 +1,86 @@
+"""decay_attention, decay_attention_step and copy_states at the edges of what they take: sums that cancel, and what is refused.
+
+The reference and the bounds of ordinary results are those of test_decay_attention_gpu.py."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import vision_rwkv_amd as vr
+from test_decay_attention_gpu import DEV, DT, reference
+
+
+def short(x, bits):
+    """x with `bits` bits of mantissa."""
+    m, e = torch.frexp(x)
+    return torch.ldexp(torch.round(m * 2.0 ** bits) / 2.0 ** bits, e)
+
+
+def pairs(x, first, second):
+    """Rows (B, n, ..) as (B, 2 n, ..): each row times `first`, and behind it times `second`."""
+    return torch.stack([first * x, second * x], 2).flatten(1, 2)
+
+
+def cancelled(got, spread, what):
+    """Bound: terms that cancel leave the rounding of their running sum, whose size is their root of squares: 2^-24 of it a step, of random sign, for the up
+    to 64 sums that a matrix instruction and the chunk's terms make: 2^-21.  A factor of 16 bits would leave 2^-19.3 (an error of up to half a step
+    of 2^-17, evenly spread, times 2^-0.8)."""
+    err = got.detach().double().cpu().norm() / spread.norm()
+    assert err <= 2.0 ** -21, f"{what}: 2^{math.log2(err):.1f}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 64), (100, 72)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_sums_that_cancel_keep_32_bits(dtype, Dk, Dv):
+    """Of 16-bit rows: tokens two by two with k and 3 v, then 3 k and -v.  Behind each second one the state is zero, and y and dq are what is left of sums that cancel; with q and
+    gy made the same way, dk and dv of each first one."""
+    B, n, H = 1, 20, 2
+    bits = {"bf16": 6, "fp16": 9}[dtype]
+    gen = torch.Generator(DEV).manual_seed(Dk)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    rows = lambda x, a, b: pairs(short(x, bits), a, b).to(DT[dtype])
+    free = lambda d: r(B, 2 * n, H, d).to(DT[dtype])
+    g = torch.zeros(H, device=DEV)
+    wide = lambda *ts: [t.detach().double().cpu().transpose(1, 2) for t in ts]          # (B, H, T, D)
+    ahead = torch.ones(2 * n, 2 * n, dtype=torch.float64).tril()
+
+    def run(q, k, v, gy):
+        ts = [t.requires_grad_() for t in (q, k, v)]
+        y = vr.decay_attention(*ts, g, scale=0.25)
+        return [y, *torch.autograd.grad(y, ts, gy)], wide(q, k, v, gy)
+
+    def spread(weights, x):
+        """Root of the summed squares of the terms weights (.., t, s) x (.., s, d), as (B, T, H, d)."""
+        return ((weights * weights) @ (x * x)).sqrt().transpose(1, 2)
+    (y, dq, _, _), (Q, K, V, GY) = run(free(Dk), rows(r(B, n, H, Dk), 1, 3), rows(r(B, n, H, Dv), 3, -1), free(Dv))
+    cancelled(y[:, 1::2], spread(0.25 * (Q @ K.mT) * ahead, V)[:, 1::2], "y")
+    cancelled(dq[:, 1::2], spread(0.25 * (GY @ V.mT) * ahead, K)[:, 1::2], "dq")
+    (_, _, dk, dv), (Q, K, V, GY) = run(rows(r(B, n, H, Dk), 1, 3), free(Dk), free(Dv), rows(r(B, n, H, Dv), 3, -1))
+    cancelled(dv[:, 0::2], spread((0.25 * (Q @ K.mT) * ahead).mT, GY)[:, 0::2], "dv")
+    cancelled(dk[:, 0::2], spread((0.25 * (GY @ V.mT) * ahead).mT, Q)[:, 0::2], "dk")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 64)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_states_that_cancel_keep_32_bits(dtype, Dk, Dv):
+    """A state whose rows lie two by two as S, -3 S, read with 3 q, q; a state's gradient the same way for dv.  What is left is the rounding of -3 S."""
+    H, T = 2, 3
+    gen = torch.Generator(DEV).manual_seed(Dv)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    bits = {"bf16": 6, "fp16": 9}[dtype]
+    two = lambda x, a, b: torch.stack([a * x, b * x], -1).flatten(-2)
+    row = two(short(r(1, T, H, Dk // 2), bits), 3, 1).to(DT[dtype])
+    S = two(r(1, H, Dv, Dk // 2), 1, -3).mT.contiguous()
+    zk, zv = torch.zeros(1, T, H, Dk, device=DEV, dtype=DT[dtype]), torch.zeros(1, T, H, Dv, device=DEV, dtype=DT[dtype])
+    g = torch.zeros(H, device=DEV)
+    f = lambda t: t.detach().double().cpu()
+    exact = torch.einsum("bthk,bhkv->bthv", f(row), f(S))
+    spread = torch.einsum("bthk,bhkv->bthv", f(row) ** 2, f(S) ** 2).sqrt()
+    y = vr.decay_attention(row, zk, zv, g, state=S)
+    cancelled(f(y) - exact, spread, "y")
+    k, v = row.clone(), zv.clone().requires_grad_()
+    _, last = vr.decay_attention(zk, k, v, g, return_state=True)
+    cancelled(f(torch.autograd.grad(last, v, S)[0]) - exact, spread, "dv")

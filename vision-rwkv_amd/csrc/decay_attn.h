@@ -229,6 +229,46 @@ struct Source {
         }
     }
 };
+// Sixteen rows as the products take them from the lanes, straight from memory: a lane's row, and of each 32 channels the four from 4 quarter on and those 16 behind.
+template <typename IO, int KX, bool VEC>
+struct Fragments {
+    const char* p;
+    int pitch;
+    unsigned at;
+    int row, count;
+    __device__ __forceinline__ void open(const View& v, int base, int first, int head, int row_, int quarter, int dim) {
+        p = static_cast<const char*>(v.p) + (base * v.sb + (long long)first * v.st + (v.share == 1 ? head : head / v.share) * v.sh) * (int)sizeof(IO);
+        pitch = (int)v.st * (int)sizeof(IO);
+        keep(p);
+        keep(pitch);
+        row = row_;
+        count = dim - 4 * quarter;
+        at = (unsigned)(row * pitch + 4 * quarter * (int)sizeof(IO));
+    }
+    __device__ __forceinline__ void load(Piece<IO> (&r)[KX], int token, int n, bool) const {
+        const auto buf = buffer_at(p + (long long)token * pitch);
+        const int have = row < n ? count : 0;
+#pragma unroll
+        for (int i = 0; i < 2 * KX; ++i) {                // fours
+            const unsigned ahead = 16 * i * (unsigned)sizeof(IO);
+            unsigned* const w = &r[i / 2].w[(i & 1) * (int)sizeof(IO)];
+            if constexpr (VEC) {
+                const auto t = BufRaw<4 * sizeof(IO)>::ld(buf, 16 * i < have ? at : OOB_OFFSET, ahead);
+#pragma unroll
+                for (int c = 0; c < (int)sizeof(IO); ++c) w[c] = t[c];
+            } else if constexpr (sizeof(IO) == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = BufRaw<4>::ld(buf, 16 * i + e < have ? at + 4 * e : OOB_OFFSET, ahead);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const unsigned lo = BufRaw<2>::ld(buf, 16 * i + 2 * e < have ? at + 4 * e : OOB_OFFSET, ahead), hi = BufRaw<2>::ld(buf, 16 * i + 2 * e + 1 < have ? at + 4 * e + 2 : OOB_OFFSET, ahead);
+                    w[e] = lo | hi << 16;
+                }
+            }
+        }
+    }
+};
 // Where a lane's results go: four channels of a row, and every sixteenth behind them.
 template <typename IO, bool VEC>
 struct Sink {
@@ -410,15 +450,17 @@ __device__ __forceinline__ double flow_sum(double inner, double in, double out, 
 template <typename IO, int DX, int MODE>
 struct Lds {
     static constexpr int L = chunk_len<IO, DX, MODE>, NS = in_terms<IO>;
-    static constexpr int NP = NS < 3 ? 2 : 3;             // terms of the products' intermediate operands: 16 bits of them for a 16-bit result, all 24 for an fp32 one
     static constexpr int PX = DX + 8, PZ = TZ + 8;        // row pitches: 16 rows of a fragment on different banks
     static constexpr bool OUT = MODE == PLAIN;
-    __bf16 a[OUT ? NS : 1][OUT ? L : 1][PX];   // channels in the order of the state's fragments
-    __bf16 b[NS][L][PX];                                  // (as they lie where there are no outputs: read across the rows alone, with fewer bank conflicts)
+    // q's rows, each read by one wave or two, come through the LDS (in wide pieces: 64 x 196 x 12 bf16 26.9 us, straight from memory 27.7; 2 x 4150 x 12 fp32 55 and 56) where they
+    // leave room for two workgroups, or for one alone either way; fp16 rows, and bf16 ones of more than 64 channels, do not (4 x 16384 x 12 fp16 204 us, with them 232)
+    static constexpr bool STAGED = OUT && (NS == 3 || (NS == 1 && DX == 64));
+    __bf16 a[STAGED ? NS : 1][STAGED ? L : 1][STAGED ? PX : 8];
+    __bf16 b[NS][L][PX];                                  // channels in the order of the state's fragments (as they lie where there are no outputs: read across the rows alone, with fewer bank conflicts)
     // c with its decays to the chunk's end, where it is wanted with them alone and has more terms than one: scaled before it is split, not put together to be scaled
     static constexpr bool SCALED = !OUT && NS > 1;
     __bf16 c[SCALED ? 3 : NS][L][PZ];
-    u32x4 s[OUT ? NP : 1][4][OUT ? DX / 32 : 1][64];   // the state's terms, a lane's fragment side by side
+    u32x4 s[OUT ? 3 : 1][4][OUT ? DX / 32 : 1][64];   // the state's terms, a lane's fragment side by side
     struct Decays {
         float gh[L], gl[L], dt[L], dk[L];                 // G in powers of two, head and tail; exp(G); exp(G_end - G)
         float end;                                        // exp(G_end)
@@ -646,9 +688,9 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 template <typename IO, int DX, bool VEC>
 __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX, PLAIN>)>)) void decay_kernel(const Params p) {
     using S = Lds<IO, DX, PLAIN>;
-    constexpr int L = S::L, NS = S::NS, NP = S::NP, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
-    constexpr int PA = L * DX / 8 / 256, PC = L * TZ / 8 / 256;   // pieces of a thread of its kind
-    static_assert(PA >= 1 && PC >= 1 && L * DX % 2048 == 0 && L * TZ % 2048 == 0, "");
+    constexpr int L = S::L, NS = S::NS, NT = L / 16, KX = DX / 32, KS = L / 32, NX = DX / 16;
+    constexpr int PB = L * DX / 8 / 256, PC = L * TZ / 8 / 256;   // pieces of a thread of its kind
+    static_assert(PB >= 1 && PC >= 1 && L * DX % 2048 == 0 && L * TZ % 2048 == 0, "");
     __shared__ S lds;
     __shared__ int offs[OUT_THREADS];
     const int tid = threadIdx.x & 255, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
@@ -670,17 +712,19 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
 
     if (wave < 4) {
         const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, o0 = order_of(dxo);
-        Source<IO, PA, STEPX, VEC> sa, sb;
-        sa.open(r.a, w.base, w.first, h, L, false, rowx, dxo, r.dx);
+        const int tw = w4 % NT, zt0 = w4 / NT * NT, t = 16 * tw + col;   // rows 16 tw + col, columns 16 (zt0 + j) + 4 quarter + i
+        std::conditional_t<S::STAGED, Source<IO, PB, STEPX, VEC>, Fragments<IO, KX, VEC>> sa;
+        Source<IO, PB, STEPX, VEC> sb;
+        if constexpr (S::STAGED) sa.open(r.a, w.base, w.first, h, L, false, rowx, dxo, r.dx);
+        else sa.open(r.a, w.base, w.first, h, t, quarter, r.dx);
         sb.open(r.b, w.base, w.first, h, L, false, rowx, dxo, r.dx);
-        Piece<IO> ra[PA], rb[PA];
+        Piece<IO> ra[S::STAGED ? PB : KX], rb[PB];
         const auto fetch = [&](int c) {
             const int t0 = w.s0 + c * L, n = min(L, w.s1 - t0);
             sa.load(ra, t0, n, false);
             sb.load(rb, t0, n, false);
         };
         if (nc > 0) fetch(0);
-        const int tw = w4 % NT, zt0 = w4 / NT * NT, t = 16 * tw + col;   // rows 16 tw + col, columns 16 (zt0 + j) + 4 quarter + i
         Sink<IO, VEC> so;
         so.open(r.o, w.base, w.first, h, t, z0 + 16 * zt0 + 4 * quarter, r.dz);
         for (int c = 0; c < nc; ++c) {
@@ -698,10 +742,20 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
                     *reinterpret_cast<uint2*>(&a[s][row][o0 + 8]) = uint2{f[s][2], f[s][3]};
                 }
             };
+            bf16x8 fa[KX][NS];
 #pragma unroll
-            for (int i = 0; i < PA; ++i) {
-                put(ra[i], lds.a, rowx + STEPX * i);
+            for (int i = 0; i < PB; ++i) {
+                if constexpr (S::STAGED) put(ra[i], lds.a, rowx + STEPX * i);
                 put(rb[i], lds.b, rowx + STEPX * i);
+            }
+            if constexpr (!S::STAGED) {
+#pragma unroll
+                for (int kx = 0; kx < KX; ++kx) {
+                    u32x4 f[NS];
+                    piece_terms<IO>(ra[kx], f);
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) fa[kx][s] = __builtin_bit_cast(bf16x8, f[s]);
+                }
             }
             lds_barrier();                                // (orders the LDS alone: the next chunk's rows and this one's results stay on their way)
             if (c + 1 < nc) fetch(c + 1);
@@ -711,21 +765,22 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
             for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (16 * tw < n) {
                 const float gth = dec.gh[t], gtl = dec.gl[t], from_state = dec.dt[t] * scale;
-                bf16x8 fa[KX][NS];
+                if constexpr (S::STAGED) {
 #pragma unroll
-                for (int kx = 0; kx < KX; ++kx)
+                    for (int kx = 0; kx < KX; ++kx)
 #pragma unroll
-                    for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[s][t][kx * 32 + 8 * quarter]);
+                        for (int s = 0; s < NS; ++s) fa[kx][s] = *reinterpret_cast<const bf16x8*>(&lds.a[s][t][kx * 32 + 8 * quarter]);
+                }
                 // what the state in front gives
                 if (begun || c > 0) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
 #pragma unroll
                         for (int kx = 0; kx < KX; ++kx) {
-                            bf16x8 fs[NP];
+                            bf16x8 fs[3];
 #pragma unroll
-                            for (int s = 0; s < NP; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane_]);
-                            acc[j] = mma<NP - 1>(acc[j], fs, fa[kx]);
+                            for (int s = 0; s < 3; ++s) fs[s] = __builtin_bit_cast(bf16x8, lds.s[s][zt0 + j][kx][lane_]);
+                            acc[j] = mma<2>(acc[j], fs, fa[kx]);
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[j][i] *= from_state;
@@ -745,7 +800,7 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
                                 bf16x8 fb[NS];
 #pragma unroll
                                 for (int s = 0; s < NS; ++s) fb[s] = *reinterpret_cast<const bf16x8*>(&lds.b[s][16 * ts + col][kx * 32 + 8 * quarter]);
-                                m = mma<NP - 1>(m, fb, fa[kx]);
+                                m = mma<2>(m, fb, fa[kx]);
                             }
                             const f32x4 sh = *reinterpret_cast<const f32x4*>(&dec.gh[16 * ts + 4 * quarter]), sl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * ts + 4 * quarter]);
 #pragma unroll
@@ -757,14 +812,14 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
 #pragma unroll
                         for (int i = 0; i < 4; ++i) pr[4 * half + i] = m[i];
                     }
-                    bf16x8 fp[NP];
-                    split8<NP>(pr, fp);
+                    bf16x8 fp[3];
+                    split8<3>(pr, fp);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         bf16x8 fc[NS];
 #pragma unroll
                         for (int s = 0; s < NS; ++s) fc[s] = across8(&lds.c[s][32 * ks + 4 * quarter + (col >> 2)][16 * (zt0 + j) + 4 * (col & 3)], S::PZ);
-                        acc[j] = mma<NP - 1>(acc[j], fc, fp);
+                        acc[j] = mma<2>(acc[j], fc, fp);
                     }
                 }
             }
@@ -803,15 +858,15 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
 #pragma unroll
             for (int x = 0; x < NX; ++x) st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        u32x4 held[NP][KX];                               // its terms
+        u32x4 held[3][KX];                               // its terms
         const auto hold = [&]() {
 #pragma unroll
             for (int kx = 0; kx < KX; ++kx) {
                 const float x8[8] = {st[2 * kx][0], st[2 * kx][1], st[2 * kx][2], st[2 * kx][3], st[2 * kx + 1][0], st[2 * kx + 1][1], st[2 * kx + 1][2], st[2 * kx + 1][3]};
-                bf16x8 f[NP];
-                split8<NP>(x8, f);
+                bf16x8 f[3];
+                split8<3>(x8, f);
 #pragma unroll
-                for (int s = 0; s < NP; ++s) held[s][kx] = __builtin_bit_cast(u32x4, f[s]);
+                for (int s = 0; s < 3; ++s) held[s][kx] = __builtin_bit_cast(u32x4, f[s]);
             }
         };
         if (nc > 0) {
@@ -834,7 +889,7 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
 #pragma unroll
             for (int kx = 0; kx < KX; ++kx)
 #pragma unroll
-                for (int s = 0; s < NP; ++s) lds.s[s][w4][kx][lane_] = held[s][kx];
+                for (int s = 0; s < 3; ++s) lds.s[s][w4][kx][lane_] = held[s][kx];
             lds_barrier();
             if (c + 1 < nc) fetch(c + 1);
             typename S::Decays& dec = lds.d[c & 1];

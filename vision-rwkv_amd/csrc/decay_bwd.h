@@ -57,7 +57,7 @@ struct BwdLds {
 template <typename IO, bool FLOW, bool VEC>
 __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdParams p) {
     using S = BwdLds<IO>;
-    constexpr int L = S::L, NS = S::NS, NT = L / 16, KS = L / 32, PX = S::PX, NP = NS < 3 ? 2 : 3;
+    constexpr int L = S::L, NS = S::NS, NT = L / 16, KS = L / 32, PX = S::PX;
     constexpr int PIECES = L * 8 / 256;                   // a thread's of the tensor that its kind stages: q, k or v; the first two kinds take half of gy besides
     __shared__ S lds;
     __shared__ int offs[BWD_THREADS];
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                         for (int kx = 0; kx < 2; ++kx) {
                             bf16x8 f[NS];
                             row_of(a, 16 * tt + col, kx, f);
-                            m = mma<NP - 1>(m, f, mine[kx]);
+                            m = mma<2>(m, f, mine[kx]);
                         }
                         const f32x4 th = *reinterpret_cast<const f32x4*>(&dec.gh[16 * tt + 4 * quarter]), tl = *reinterpret_cast<const f32x4*>(&dec.gl[16 * tt + 4 * quarter]);
 #pragma unroll
@@ -310,13 +310,13 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
 #pragma unroll
                     for (int i = 0; i < 4; ++i) pr[4 * hf + i] = m[i];
                 }
-                bf16x8 fp[NP];
-                split8<NP>(pr, fp);
+                bf16x8 fp[3];
+                split8<3>(pr, fp);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     bf16x8 f[NS];
                     across(c_, zt0 + j, ks, f);
-                    acc[j] = mma<NP - 1>(acc[j], f, fp);
+                    acc[j] = mma<2>(acc[j], f, fp);
                 }
             }
         };
@@ -387,13 +387,13 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);    // (what is read ahead of its use fills the registers otherwise)
-                    bf16x8 fp[NP];
-                    split8<NP>(pr, fp);
+                    bf16x8 fp[3];
+                    split8<3>(pr, fp);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         bf16x8 fk[NS];
                         across(lds.k, zt0 + j, ks, fk);
-                        acc[j] = mma<NP - 1>(acc[j], fk, fp);
+                        acc[j] = mma<2>(acc[j], fk, fp);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                     if (FLOW && w4 < NT) {                // (the other waves of a 32-token chunk would make the same terms)
@@ -500,13 +500,13 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                         const int x = zt0 + j;
 #pragma unroll
                         for (int kx = 0; kx < 2; ++kx) {
-                            bf16x8 fy[NP];
+                            bf16x8 fy[3];
 #pragma unroll
-                            for (int s = 0; s < NP; ++s) {
+                            for (int s = 0; s < 3; ++s) {
                                 const __bf16* q = &lds.x[s][32 * kx + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
                                 fy[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
                             }
-                            acc[j] = mma<NP - 1>(acc[j], fy, fk[kx]);
+                            acc[j] = mma<2>(acc[j], fy, fk[kx]);
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[j][i] *= dk;
