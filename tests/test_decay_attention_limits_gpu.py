@@ -3,12 +3,11 @@
 The reference and the bounds of ordinary results are those of test_decay_attention_gpu.py."""
 import math
 
-import numpy as np
 import pytest
 import torch
 
 import vision_rwkv_amd as vr
-from test_decay_attention_gpu import DEV, DT, reference
+from test_decay_attention_gpu import DEV, DT
 
 
 def short(x, bits):
@@ -84,3 +83,26 @@ def test_states_that_cancel_keep_32_bits(dtype, Dk, Dv):
     k, v = row.clone(), zv.clone().requires_grad_()
     _, last = vr.decay_attention(zk, k, v, g, return_state=True)
     cancelled(f(torch.autograd.grad(last, v, S)[0]) - exact, spread, "dv")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+def test_what_the_library_refuses_raises_its_own_error(host, monkeypatch):
+    """Calls that every check in front of the library lets through."""
+    if not host:
+        monkeypatch.setattr(vr._lib, "_host", vr._lib._NoHost)
+    z = lambda *s: torch.zeros((1,) * len(s), device=DEV).expand(*s)
+    for grads in (False, True):
+        g = torch.zeros(2, device=DEV, requires_grad=grads)
+        with pytest.raises(vr.VrwkvError, match="too many tokens and heads"):
+            vr.decay_attention(z(1 << 18, 1, 1, 1), z(1 << 18, 1, 1, 1), z(1 << 18, 1, 1, 1), g)
+        with pytest.raises(vr.VrwkvError, match="elements apart"):
+            vr.decay_attention(z(1, 1, 1, 64), z(1, 1, 1, 64), z(1, 1, 1, 64), z(1 << 16).contiguous().requires_grad_(grads))
+    x, g = z(1 << 19, 1, 1), torch.zeros(16, device=DEV)
+    with pytest.raises(vr.VrwkvError, match="too many rows and heads"):
+        vr.decay_attention_step(x, x, x, g, torch.zeros(1, 16, 1, 1, device=DEV), torch.zeros(1 << 19, dtype=torch.int32, device=DEV))
+    with pytest.raises(vr.VrwkvError, match="overlaps the pool"):
+        pool = torch.zeros(5, 8, device=DEV)
+        vr.copy_states(pool[:4], torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), source=pool[1:])
+    q = torch.ones(1, 3, 2, 8, device=DEV)                 # (and the call behind is as before)
+    assert torch.isfinite(vr.decay_attention(q, q, q, torch.zeros(2, device=DEV))).all()

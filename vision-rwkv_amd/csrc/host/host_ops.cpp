@@ -439,12 +439,13 @@ py::object decay_attention(py::handle q_, py::handle k_, py::handle v_, py::hand
         at::Tensor ws;
         a.workspace_bytes = vrwkv_decay_fwd_workspace_bytes(&a);
         if (a.workspace_bytes) a.workspace = (ws = bytes(a.workspace_bytes, q)).data_ptr();
-        if (vrwkv_decay_fwd(&a, stream_of(q)) != VRWKV_OK) return py::none();
-        if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || (state.defined() && state.requires_grad())))
+        const bool done = vrwkv_decay_fwd(&a, stream_of(q)) == VRWKV_OK;   // (None is a Python object: not to be touched in here)
+        if (done && at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || (state.defined() && state.requires_grad())))
             out = Decay::apply(q, k, v, g, state.defined() ? std::optional<at::Tensor>(state) : std::nullopt, &c);
-        else
+        else if (done)
             out = {c.y, c.last};
     }
+    if (out.empty()) return py::none();
     py::object y = py::reinterpret_steal<py::object>(THPVariable_Wrap(out[0]));
     if (!keep) return y;
     return py::make_tuple(y, py::reinterpret_steal<py::object>(THPVariable_Wrap(out[1])));
