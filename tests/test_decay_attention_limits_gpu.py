@@ -5,6 +5,8 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import vision_rwkv_amd as vr
 from test_decay_attention_gpu import DEV, DT
@@ -106,3 +108,66 @@ def test_what_the_library_refuses_raises_its_own_error(host, monkeypatch):
         vr.copy_states(pool[:4], torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), source=pool[1:])
     q = torch.ones(1, 3, 2, 8, device=DEV)                 # (and the call behind is as before)
     assert torch.isfinite(vr.decay_attention(q, q, q, torch.zeros(2, device=DEV))).all()
+
+
+def small_calls():
+    """{name: (call, its float inputs)} of the three operators."""
+    gen = torch.Generator(DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    q, g, pool = r(1, 5, 2, 8), -r(1, 5, 2).abs(), r(4, 2, 8, 8)
+    src, dst = (torch.tensor(x, device=DEV) for x in ([0, 2], [1, 3]))
+    return {"attention": (lambda q, g, S: vr.decay_attention(q, q, q, g, state=S), (q, g, pool[:1].clone())),
+            "step": (lambda q, g, pool: vr.decay_attention_step(q, q, q, g, pool, src), (q[0, :2], g[0, :2], pool)),
+            "pages": (lambda pool, source: vr.copy_states(pool, src, dst, source=source), (pool, r(4, 2, 8, 8)))}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+@pytest.mark.parametrize("name", ["attention", "step", "pages"])
+def test_tangents_are_refused(name, host, monkeypatch):
+    if not host:
+        monkeypatch.setattr(vr._lib, "_host", vr._lib._NoHost)
+    call, args = small_calls()[name]
+    for i in range(len(args)):
+        before = [a.clone() for a in args]
+        for mode in (torch.no_grad, torch.enable_grad):
+            with forward_ad.dual_level(), mode():
+                dual = [forward_ad.make_dual(a, torch.ones_like(a)) if i == j else a for j, a in enumerate(args)]
+                with pytest.raises(RuntimeError):
+                    call(*dual)
+                call(*(a.clone() for a in args))           # (a level by itself is no tangent)
+        assert all(torch.equal(a, b) for a, b in zip(args, before))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["attention", "step", "pages"])
+def test_recordings_are_refused(name):
+    """A trace would hold the outputs' allocations and nothing that fills them."""
+    call, args = small_calls()[name]
+    copies = lambda: tuple(a.clone() for a in args)
+    want = call(*copies())
+    for record in (lambda: torch.jit.trace(call, copies(), check_trace=False), lambda: make_fx(call)(*copies())):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            record()
+    assert torch.equal(call(*copies()), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["attention", "step", "pages"])
+def test_transforms_are_refused(name):
+    call, args = small_calls()[name]
+    copies = lambda: tuple(a.clone() for a in args)
+    for transform in (lambda: torch.func.vmap(call)(*(torch.stack([a, a]) for a in copies())), lambda: torch.func.grad(lambda *a: call(*a).sum())(*copies()),
+                      lambda: torch.func.jvp(call, copies(), copies()), lambda: torch.func.functionalize(call)(*copies())):
+        with pytest.raises(RuntimeError):
+            transform()
+    # lists or a state alone that a transform has wrapped: not taken for ones that are not there
+    q, g, pool = small_calls()["step"][1]
+    before = pool.clone()
+    with pytest.raises(RuntimeError):
+        torch.func.functionalize(lambda s: vr.decay_attention_step(q, q, q, g, pool, s))(torch.tensor([3, 1], device=DEV))
+    with pytest.raises(RuntimeError):
+        torch.func.functionalize(lambda s: vr.decay_attention(q[None], q[None], q[None], g[None], state=s))(pool[:1])
+    with pytest.raises(RuntimeError):
+        torch.func.functionalize(lambda s: vr.copy_states(pool, s, s))(torch.tensor([3, 1], device=DEV))
+    assert torch.equal(pool, before)

@@ -6,15 +6,30 @@ Beside wkv6, which looks both ways and returns no state, this is the form for se
 a video, rows of an image in order.  The reference has no counterpart.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DT, _on, _stream_ptr, batched_cotangent
+from .ops import _DT, _forward_mode, _on, _stream_ptr, batched_cotangent
 
 
 def _eager(f):
     """f as a call that a compiled program makes and does not look into: its kernels take memory, not traces."""
     return torch.compiler.disable(f)
+
+
+def _check_recorders(name, *tensors):
+    """Refuses what a kernel would drop without a word: recordings of tensor operations, in which it leaves no trace, tangents, and tensors whose memory is
+    elsewhere."""
+    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError(f"{name} cannot be traced")
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            continue
+        if _forward_mode() and (t.is_floating_point() or t.is_complex()) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward mode")
+        if t.is_cuda and t.numel() and not t.data_ptr():
+            raise RuntimeError(f"{name} takes tensors with memory of their own")
 
 
 def _rows(t):
@@ -162,13 +177,15 @@ def decay_attention(q, k, v, g, scale=1.0, state=None, offsets=None, return_stat
     forgets.  Head sizes 1 to 128.  state: the states in front, (N, H, Dk, Dv) float32, zeros without; N = B.
     offsets (N + 1,), int32 or int64 on the device, ascending from 0 to T: N sequences packed behind each other in one row (B = 1), sequence n the tokens
     offsets[n] to offsets[n + 1] (an empty one leaves its state as it is); y of rows behind the last sequence is zero, and so are their gradients.
-    Gradients for q, k, v, g and state, sums in fp32 (those of (H,) decays in 64 bits), rounded once to their inputs' types; no second ones."""
+    Gradients for q, k, v, g and state, sums in fp32 (those of (H,) decays in 64 bits), rounded once to their inputs' types; no second ones, no
+    forward mode, no tracing (a compiled program makes the call as it is)."""
     if torch.compiler.is_compiling():
         return _eager(decay_attention)(q, k, v, g, scale, state, offsets, return_state)
     scale = _check_scale(scale)
     out = _lib.host().decay_attention(q, k, v, g, scale, state, offsets, return_state)
     if out is not None:
         return out
+    _check_recorders("decay_attention", q, k, v, g, state, offsets)
     H, Dk, Dv = _check_heads(q, k, v, g, 2)
     N = q.shape[0]
     if offsets is not None:
@@ -190,13 +207,14 @@ def decay_attention_step(q, k, v, g, pool, slots=None, scale=1.0):
     q (N, Hq, Dk), k (N, Hk, Dk), v (N, Hv, Dv) and g (N, H) or (H,) as in decay_attention.  slots (N,), int32 or int64 on the device: row n's
     page, 0, 1, .. without.  Rows that name the same page are tokens behind each other, in their order.  A row of slot -1 (a place of the batch that is not
     taken) gives zeros and touches nothing, one of any other slot outside the pool NaN.  Pages may lie at any distance (pool[:, layer] of a pool for all
-    layers), each contiguous.  Forward only."""
+    layers), each contiguous.  Forward only: inputs that want gradients or carry tangents are refused, and so is tracing."""
     if torch.compiler.is_compiling():
         return _eager(decay_attention_step)(q, k, v, g, pool, slots, scale)
     scale = _check_scale(scale)
     y = _lib.host().decay_step(q, k, v, g, pool, slots, scale)
     if y is not None:
         return y
+    _check_recorders("decay_attention_step", q, k, v, g, pool, slots)
     H, Dk, Dv = _check_heads(q, k, v, g, 1)
     N = q.shape[0]
     _check(pool, "pool", q)
@@ -267,11 +285,12 @@ def copy_states(pool, src, dst, source=None):
     from another pool or out to one.  src -1 clears the page, dst -1 is a place of the list that is not taken; of several entries with the same dst the
     last counts.  src, dst: vectors of up to 4096 int32 or int64, on the device -- where entries outside the pools are left out -- or on the host, where
     they are refused.  Pools of any type whose pages are contiguous, at any distance; a source is the pool, or its pages overlap none of
-    the pool's (pool[:, 0] and pool[:, 1] of a pool for all layers)."""
+    the pool's (pool[:, 0] and pool[:, 1] of a pool for all layers).  No gradients, tangents or tracing, as in decay_attention_step."""
     if torch.compiler.is_compiling():
         return _eager(copy_states)(pool, src, dst, source)
     if _lib.host().copy_pages(pool, src, dst, source):
         return pool
+    _check_recorders("copy_states", pool, src, dst, source)
     _check(pool, "pool")
     source = pool if source is None else source
     _check(source, "source", pool)
