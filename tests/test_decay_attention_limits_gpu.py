@@ -171,3 +171,34 @@ def test_transforms_are_refused(name):
     with pytest.raises(RuntimeError):
         torch.func.functionalize(lambda s: vr.copy_states(pool, s, s))(torch.tensor([3, 1], device=DEV))
     assert torch.equal(pool, before)
+
+
+@pytest.mark.gpu
+def test_negated_and_conjugated_views():
+    """Tensors whose memory holds the negative or the conjugate of what they are: read as what they are, not written."""
+    gen = torch.Generator(DEV).manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    neg = torch._neg_view
+    q, k, v, g, S, gy = r(2, 5, 2, 8), r(2, 5, 2, 8), r(2, 5, 2, 8), -r(2, 5, 2).abs(), r(2, 2, 8, 8), r(2, 5, 2, 8)
+    want = None
+    for view in (lambda t: t, lambda t: neg(-t)):
+        ts = [t.clone().requires_grad_() for t in (q, k, v, g, S)]
+        y, last = vr.decay_attention(*(view(t) for t in ts[:4]), state=view(ts[4]), return_state=True)
+        results = [y, last, *torch.autograd.grad(y, ts, view(gy))]
+        want = want or results
+        assert all(torch.equal(a, b) for a, b in zip(results, want))
+    pool, step = S.clone(), [t[:, 0] for t in (q, k, v, g)]
+    y = vr.decay_attention_step(*step, S.clone())
+    assert torch.equal(vr.decay_attention_step(*(neg(-t) for t in step), pool), y)
+    slots = torch.tensor([0, 1], device=DEV)
+    with pytest.raises(RuntimeError, match="in place"):
+        vr.decay_attention_step(*step, neg(pool), slots)
+    assert torch.equal(vr.decay_attention_step(*step, S.clone(), neg(-slots)), y)
+    c = torch.complex(r(4, 3), r(4, 3))
+    pages = torch.zeros(4, 3, device=DEV, dtype=torch.complex64)
+    vr.copy_states(pages, slots, slots + 2, source=c.conj())
+    assert torch.equal(pages[2:], c[:2].conj().resolve_conj())
+    with pytest.raises(RuntimeError, match="in place"):
+        vr.copy_states(pages.conj(), slots, slots + 2)
+    vr.copy_states(pages, neg(-slots), neg(-slots), source=c)
+    assert torch.equal(pages[:2], c[:2])

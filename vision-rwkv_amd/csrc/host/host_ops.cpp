@@ -379,8 +379,8 @@ struct Decay : torch::autograd::Function<Decay> {
             if (!gy.defined() && !glast.defined()) return out;
             Guard guard(q.device());
             const auto plain_options = q.options().requires_grad(false);
-            gy = gy.defined() ? rows(gy.to(q.scalar_type()), q) : at::zeros({q.size(0), q.size(1), H, v.size(3)}, plain_options);
-            if (glast.defined()) glast = glast.to(at::kFloat).contiguous();
+            gy = gy.defined() ? rows(gy.to(q.scalar_type()).resolve_neg(), q) : at::zeros({q.size(0), q.size(1), H, v.size(3)}, plain_options);
+            if (glast.defined()) glast = glast.to(at::kFloat).resolve_neg().contiguous();
             TORCH_CHECK(gy.size(0) == q.size(0) && gy.size(1) == q.size(1) && gy.size(2) == H && gy.size(3) == v.size(3), "the gradient must have the shape of y");
             vrwkv_decay_args a = decay_args(q, k, v, g, state, offsets, ctx->saved_data["scale"].toDouble(), N);
             a.gy = gy.data_ptr();

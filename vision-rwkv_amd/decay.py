@@ -32,6 +32,16 @@ def _check_recorders(name, *tensors):
             raise RuntimeError(f"{name} takes tensors with memory of their own")
 
 
+def _resolved(t):
+    """t with the values that its memory holds (a view of another's imaginary part may be marked as negated)."""
+    return t.resolve_conj().resolve_neg() if isinstance(t, torch.Tensor) else t
+
+
+def _check_in_place(t, name):
+    if t.is_neg() or t.is_conj():
+        raise RuntimeError(f"{name} is a negated or conjugated view: it cannot be written in place")
+
+
 def _rows(t):
     """t as the kernels read it: any strides, but the channels of a head side by side and tokens less than 2^22 elements apart."""
     return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() == 3 or t.stride(1) < 1 << 22) else t.contiguous()
@@ -145,6 +155,7 @@ class DecayAttention(torch.autograd.Function):
         for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (state, "state"), (offsets, "offsets")):
             if t is not None:                              # (hooks on saved tensors may have moved them)
                 _check(t, name, q)
+        gy, glast = _resolved(gy), _resolved(glast)
         if batched_cotangent(*(t for t in (gy, glast) if t is not None)):
             raise RuntimeError("decay_attention's gradients take one cotangent at a time")
         q, k, v = _rows(q), _rows(k), _rows(v)
@@ -186,6 +197,7 @@ def decay_attention(q, k, v, g, scale=1.0, state=None, offsets=None, return_stat
     if out is not None:
         return out
     _check_recorders("decay_attention", q, k, v, g, state, offsets)
+    q, k, v, g, state, offsets = (_resolved(t) for t in (q, k, v, g, state, offsets))
     H, Dk, Dv = _check_heads(q, k, v, g, 2)
     N = q.shape[0]
     if offsets is not None:
@@ -215,9 +227,11 @@ def decay_attention_step(q, k, v, g, pool, slots=None, scale=1.0):
     if y is not None:
         return y
     _check_recorders("decay_attention_step", q, k, v, g, pool, slots)
+    q, k, v, g, slots = (_resolved(t) for t in (q, k, v, g, slots))
     H, Dk, Dv = _check_heads(q, k, v, g, 1)
     N = q.shape[0]
     _check(pool, "pool", q)
+    _check_in_place(pool, "pool")
     _check_sizes(pool.shape)
     if pool.dim() != 4 or tuple(pool.shape[1:]) != (H, Dk, Dv) or pool.dtype != torch.float32 or not _pages_fit(pool):
         raise RuntimeError(f"pool must be float32 (P, {H}, {Dk}, {Dv}) with contiguous pages")
@@ -292,8 +306,10 @@ def copy_states(pool, src, dst, source=None):
         return pool
     _check_recorders("copy_states", pool, src, dst, source)
     _check(pool, "pool")
+    _check_in_place(pool, "pool")
     source = pool if source is None else source
     _check(source, "source", pool)
+    src, dst, source = _resolved(src), _resolved(dst), _resolved(source)
     if pool.dim() < 1 or source.shape[1:] != pool.shape[1:] or source.dtype != pool.dtype:
         raise RuntimeError("pool and source must hold pages of one shape and type")
     _check_sizes(pool.shape[:1], source.shape[:1])
