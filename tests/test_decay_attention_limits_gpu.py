@@ -202,3 +202,21 @@ def test_negated_and_conjugated_views():
         vr.copy_states(pages.conj(), slots, slots + 2)
     vr.copy_states(pages, neg(-slots), neg(-slots), source=c)
     assert torch.equal(pages[:2], c[:2])
+
+
+@pytest.mark.gpu
+def test_the_class_by_itself_checks_what_it_is_given():
+    gen = torch.Generator(DEV).manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    q, g, S, off = r(2, 6, 2, 8), -r(2, 6, 2).abs(), r(2, 2, 8, 8), torch.tensor([0, 9, 2, 9, 6, 9], device=DEV)[::2]
+    good = dict(q=q, k=q, v=q, g=g, state=S, offsets=None, scale=0.5, N=2, H=2, keep=True)
+    call = lambda **change: vr.DecayAttention.apply(*{**good, **change}.values())
+    for a, b in zip(call(), vr.decay_attention(q, q, q, g, scale=0.5, state=S, return_state=True)):
+        assert torch.equal(a, b)
+    row = dict(q=q[:1], k=q[:1], v=q[:1], g=g[:1], offsets=off)
+    for a, b in zip(call(**row), vr.decay_attention(q[:1], q[:1], q[:1], g[:1], scale=0.5, state=S, offsets=off, return_state=True)):
+        assert torch.equal(a, b)
+    for change in (dict(N=3), dict(N=1), dict(H=4), dict(H=1), dict(state=S[:1]), dict(k=q[:1]), dict(v=q[:, :5]), dict(g=g[:, :3]), dict(q=q.half()), dict(offsets=off), dict(row, N=3),
+                   dict(row, offsets=off.float())):
+        with pytest.raises(RuntimeError):
+            call(**change)

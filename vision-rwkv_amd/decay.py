@@ -96,6 +96,22 @@ def _check_index(t, name, like):
     return t.contiguous()
 
 
+def _check_call(q, k, v, g, state, offsets):
+    """decay_attention's checks; the numbers of sequences and heads."""
+    H, Dk, Dv = _check_heads(q, k, v, g, 2)
+    N = q.shape[0]
+    if offsets is not None:
+        _check_index(offsets, "offsets", q)
+        if q.shape[0] != 1 or offsets.numel() < 1:
+            raise RuntimeError("packed sequences (offsets) come as one row, B = 1, with N + 1 offsets")
+        N = offsets.numel() - 1
+    if state is not None:
+        _check(state, "state", q)
+        if tuple(state.shape) != (N, H, Dk, Dv) or state.dtype != torch.float32:
+            raise RuntimeError(f"state must be float32 of shape {(N, H, Dk, Dv)}")
+    return N, H
+
+
 def _strides(t):
     """Strides of batch, token and head; a row of one token has none to a next one, whatever the view says."""
     return t.stride(0), 0 if t.shape[1] == 1 else t.stride(1), t.stride(2)
@@ -130,6 +146,10 @@ class DecayAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, g, state, offsets, scale, N, H, keep_state):
+        q, k, v, g, state, offsets = (_resolved(t) for t in (q, k, v, g, state, offsets))
+        if (N, H) != _check_call(q, k, v, g, state, offsets):
+            raise RuntimeError(f"{N} sequences and {H} heads are not those of the tensors")
+        offsets = offsets.contiguous() if offsets is not None else None
         q, k, v = _rows(q), _rows(k), _rows(v)
         g = g if g.dim() == 1 or g.stride(1) < 1 << 22 else g.contiguous()
         state = state.contiguous() if state is not None else None
@@ -197,18 +217,7 @@ def decay_attention(q, k, v, g, scale=1.0, state=None, offsets=None, return_stat
     if out is not None:
         return out
     _check_recorders("decay_attention", q, k, v, g, state, offsets)
-    q, k, v, g, state, offsets = (_resolved(t) for t in (q, k, v, g, state, offsets))
-    H, Dk, Dv = _check_heads(q, k, v, g, 2)
-    N = q.shape[0]
-    if offsets is not None:
-        offsets = _check_index(offsets, "offsets", q)
-        if q.shape[0] != 1 or offsets.numel() < 1:
-            raise RuntimeError("packed sequences (offsets) come as one row, B = 1, with N + 1 offsets")
-        N = offsets.numel() - 1
-    if state is not None:
-        _check(state, "state", q)
-        if tuple(state.shape) != (N, H, Dk, Dv) or state.dtype != torch.float32:
-            raise RuntimeError(f"state must be float32 of shape {(N, H, Dk, Dv)}")
+    N, H = _check_call(q, k, v, g, state, offsets)
     y, last = DecayAttention.apply(q, k, v, g, state, offsets, scale, N, H, bool(return_state))
     return (y, last) if return_state else y
 
