@@ -220,3 +220,34 @@ def test_the_class_by_itself_checks_what_it_is_given():
                    dict(row, offsets=off.float())):
         with pytest.raises(RuntimeError):
             call(**change)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+def test_saved_tensors_that_a_hook_has_changed(host, monkeypatch):
+    if not host:
+        monkeypatch.setattr(vr._lib, "_host", vr._lib._NoHost)
+    gen = torch.Generator(DEV).manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    ins = [r(2, 6, 2, 8), r(2, 6, 1, 8), r(2, 6, 2, 4), -r(2, 6, 2).abs(), r(2, 2, 8, 4)]
+
+    def grads(ins, unpack, offsets=None):
+        ts = [t.clone().requires_grad_() for t in ins]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+            y = vr.decay_attention(*ts[:4], state=ts[4], offsets=offsets)
+        return torch.autograd.grad(y, ts, torch.ones_like(y))
+    want = grads(ins, lambda t: t)
+    far = lambda t: torch.stack([t, t], -1)[..., 0] if t.dtype == torch.float32 else t       # (the same values at other strides)
+    for a, b in zip(grads(ins, far), want):
+        assert torch.equal(a, b)
+    for like in ins:
+        shorter = lambda t: t[:1] if t.shape == like.shape else t
+        narrower = lambda t: t[..., :-1] if t.shape == like.shape else t
+        wider = lambda t: t.double() if t.shape == like.shape else t
+        for change in (shorter, narrower, wider):
+            with pytest.raises(RuntimeError):
+                grads(ins, change)
+    row = [t.flatten(0, 1)[None] for t in ins[:4]] + ins[4:]
+    for change in (lambda t: t[:-1], lambda t: t.float()):
+        with pytest.raises(RuntimeError):
+            grads(row, lambda t: change(t) if t.dim() == 1 else t, offsets=torch.tensor([0, 4, 12], device=DEV))

@@ -322,8 +322,10 @@ bool decay_inputs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
         if (k.size(i) != q.size(i) || v.size(i) != q.size(i) || q.size(i) > INT_MAX || (g.dim() > 1 && g.size(i) != q.size(i))) return false;
     const int64_t H = g.size(-1);
     return k.size(-1) == q.size(-1) && H <= INT_MAX && H % q.size(-2) == 0 && H % k.size(-2) == 0 && H % v.size(-2) == 0 && q.size(-1) <= 128 && v.size(-1) <= 128 &&
-           k.device() == q.device() && v.device() == q.device() && g.device() == q.device() && q.get_device() == c10::hip::current_device() && !tangent(q) && !tangent(k) &&
-           !tangent(v) && !tangent(g);
+           k.device() == q.device() && v.device() == q.device() && g.device() == q.device();
+}
+bool here(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g) {
+    return q.get_device() == c10::hip::current_device() && !tangent(q) && !tangent(k) && !tangent(v) && !tangent(g);
 }
 bool index_fits(const at::Tensor& t, const at::Tensor& q) {
     return t.dim() == 1 && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.is_contiguous() && t.numel() > 0 && t.device() == q.device();
@@ -361,6 +363,7 @@ struct Decay : torch::autograd::Function<Decay> {
     static at::Tensor rows(const at::Tensor& t, const at::Tensor& like) {
         TORCH_CHECK(t.defined() && t.has_storage() && t.is_cuda() && t.device() == like.device() && t.dim() == 4 && t.scalar_type() == like.scalar_type(),
                     "the saved tensors and the gradient must be CUDA tensors on one device");
+        if (t.is_neg()) return rows(t.resolve_neg(), like);
         return (t.stride(-1) == 1 || t.size(-1) == 1) && t.stride(1) < (1 << 22) ? t : t.contiguous();
     }
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
@@ -369,12 +372,16 @@ struct Decay : torch::autograd::Function<Decay> {
         {
             at::NoGradGuard no_grad;
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor q = rows(saved[0], saved[0]), k = rows(saved[1], q), v = rows(saved[2], q), &g = saved[3], &offsets = saved[5];
-            for (const at::Tensor* t : {&g, &saved[4], &offsets})   // (hooks on saved tensors may have moved them)
-                TORCH_CHECK(!t->defined() || (t->is_cuda() && t->device() == q.device() && t->has_storage()), "the saved tensors must be CUDA tensors on one device");
-            const at::Tensor state = saved[4].defined() ? saved[4].contiguous() : at::Tensor();
+            const at::Tensor q = rows(saved[0], saved[0]), k = rows(saved[1], q), v = rows(saved[2], q);
+            for (int i = 3; i < 6; ++i)                    // (hooks on saved tensors may have moved or changed them)
+                TORCH_CHECK(!saved[i].defined() || (saved[i].is_cuda() && saved[i].device() == q.device() && saved[i].has_storage()), "the saved tensors must be CUDA tensors on one device");
+            const auto own = [](const at::Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; };
+            const at::Tensor g = saved[3].is_neg() || (saved[3].dim() == 3 && saved[3].stride(1) >= (1 << 22)) ? own(saved[3]) : saved[3], state = own(saved[4]), offsets = own(saved[5]);
             const int N = (int)ctx->saved_data["N"].toInt();
             const int64_t H = g.size(-1);
+            TORCH_CHECK(decay_inputs(q, k, v, g, 2) && (offsets.defined() ? index_fits(offsets, q) && offsets.numel() == N + 1LL && q.size(0) == 1 : q.size(0) == N) &&
+                            (!state.defined() || (state.scalar_type() == at::kFloat && state.sizes() == at::IntArrayRef({N, H, q.size(3), v.size(3)}))),
+                        "the saved tensors have other sizes or types than those of the call");
             at::Tensor gy = grads[0], glast = grads.size() > 1 ? grads[1] : at::Tensor();
             if (!gy.defined() && !glast.defined()) return out;
             Guard guard(q.device());
@@ -421,7 +428,7 @@ py::object decay_attention(py::handle q_, py::handle k_, py::handle v_, py::hand
                            *op = offsets_.is_none() ? &none : strided(offsets_);
     if (!qp || !kp || !vp || !gp || !sp || !op) return py::none();
     const at::Tensor &q = *qp, &k = *kp, &v = *vp, &g = *gp, &state = *sp, &offsets = *op;
-    if (!decay_inputs(q, k, v, g, 2) || (offsets.defined() && (!index_fits(offsets, q) || q.size(0) != 1 || offsets.numel() < 2))) return py::none();
+    if (!decay_inputs(q, k, v, g, 2) || !here(q, k, v, g) || (offsets.defined() && (!index_fits(offsets, q) || q.size(0) != 1 || offsets.numel() < 2))) return py::none();
     const int64_t N = offsets.defined() ? offsets.numel() - 1 : q.size(0), H = g.size(-1), Dk = q.size(3), Dv = v.size(3);
     if (N > INT_MAX || (state.defined() && (state.scalar_type() != at::kFloat || !state.is_contiguous() || state.dim() != 4 || state.size(0) != N || state.size(1) != H || state.size(2) != Dk ||
                                             state.size(3) != Dv || state.device() != q.device() || tangent(state))))
@@ -465,7 +472,7 @@ py::object decay_step(py::handle q_, py::handle k_, py::handle v_, py::handle g_
     const at::Tensor none, *qp = strided(q_), *kp = strided(k_), *vp = strided(v_), *gp = strided(g_), *pp = strided(pool_), *sp = slots_.is_none() ? &none : strided(slots_);
     if (!qp || !kp || !vp || !gp || !pp || !sp) return py::none();
     const at::Tensor &q = *qp, &k = *kp, &v = *vp, &g = *gp, &pool = *pp, &slots = *sp;
-    if (!decay_inputs(q, k, v, g, 1) || (slots.defined() && (!index_fits(slots, q) || slots.numel() != q.size(0)))) return py::none();
+    if (!decay_inputs(q, k, v, g, 1) || !here(q, k, v, g) || (slots.defined() && (!index_fits(slots, q) || slots.numel() != q.size(0)))) return py::none();
     const int64_t N = q.size(0), H = g.size(-1), Dk = q.size(2), Dv = v.size(2);
     if (pool.dim() != 4 || pool.size(0) == 0 || pool.size(0) > INT_MAX || pool.size(1) != H || pool.size(2) != Dk || pool.size(3) != Dv || pool.scalar_type() != at::kFloat ||
         pool.device() != q.device() || tangent(pool) || !pages_fit(pool) ||

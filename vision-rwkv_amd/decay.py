@@ -172,14 +172,14 @@ class DecayAttention(torch.autograd.Function):
     def backward(ctx, gy, glast):
         q, k, v, g, state, offsets = ctx.saved_tensors
         scale, N, H = ctx.meta
-        for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (state, "state"), (offsets, "offsets")):
-            if t is not None:                              # (hooks on saved tensors may have moved them)
-                _check(t, name, q)
-        gy, glast = _resolved(gy), _resolved(glast)
+        if (N, H) != _check_call(q, k, v, g, state, offsets):   # (hooks on saved tensors may have moved or changed them)
+            raise RuntimeError("the saved tensors have other sizes than those of the call")
+        q, k, v, g, state, offsets, gy, glast = (_resolved(t) for t in (q, k, v, g, state, offsets, gy, glast))
         if batched_cotangent(*(t for t in (gy, glast) if t is not None)):
             raise RuntimeError("decay_attention's gradients take one cotangent at a time")
         q, k, v = _rows(q), _rows(k), _rows(v)
-        state = state.contiguous() if state is not None else None
+        g = g if g.dim() == 1 or g.stride(1) < 1 << 22 else g.contiguous()
+        state, offsets = (t.contiguous() if t is not None else None for t in (state, offsets))
         new = lambda t, need: torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
         dq, dk, dv, dg, dstate = (new(t, n) for t, n in zip((q, k, v, g, state), ctx.needs_input_grad[:5]))
         out = dq, dk, dv, dg, dstate, None, None, None, None, None
