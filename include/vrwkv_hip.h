@@ -377,7 +377,7 @@ typedef struct vrwkv_decay_step_args {
 int vrwkv_decay_step(const vrwkv_decay_step_args* args, void* hip_stream);
 
 /* ---- pages of a pool copied: page to[i] = page from[i] of the source as it was before the call, for i < M <= 4096 ----
- * The source is the pool itself (same pointer and stride), or pages that overlap none of the pool's (apart, or in its gaps at the same stride); strides and sizes in bytes.  from[i] = -1: zeros;
+ * The source is the pool itself (same pointer and stride), or pages that overlap none of the pool's (apart, or in its gaps at the same stride; one page takes the other's stride); strides and sizes in bytes.  from[i] = -1: zeros;
  * to[i] = -1: nothing; an entry with another index outside the pools is left out; of several entries with the same to the last counts.  Indices of 32 or
  * 64 bits, on the device.  workspace: vrwkv_copy_pages_workspace_bytes(M) bytes, 4-byte aligned; NULL where that is 0 (short lists). */
 size_t vrwkv_copy_pages_workspace_bytes(int M);

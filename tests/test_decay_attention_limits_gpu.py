@@ -251,3 +251,31 @@ def test_saved_tensors_that_a_hook_has_changed(host, monkeypatch):
     for change in (lambda t: t[:-1], lambda t: t.float()):
         with pytest.raises(RuntimeError):
             grads(row, lambda t: change(t) if t.dim() == 1 else t, offsets=torch.tensor([0, 4, 12], device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("host", [True, False])
+def test_one_page_of_a_layer(host, monkeypatch):
+    """A pool or a source of a single page between another layer's pages: nothing overlaps, whatever distance its view says."""
+    if not host:
+        monkeypatch.setattr(vr._lib, "_host", vr._lib._NoHost)
+    at = lambda *x: torch.tensor(x, device=DEV)
+    layers = torch.randn(6, 3, 2, 8, 8, device=DEV)
+    want = layers.clone()
+    want[[0, 5], 0] = want[2, 1]
+    vr.copy_states(layers[:, 0], at(0, 0), at(0, 5), source=layers[2:3, 1])
+    assert torch.equal(layers, want)
+    want[3, 2] = want[4, 0]
+    vr.copy_states(layers[3:4, 2], at(4), at(0), source=layers[:, 0])
+    assert torch.equal(layers, want)
+    want[1, 1] = want[5, 2]
+    vr.copy_states(layers[1:2, 1], at(0), at(0), source=layers[5:6, 2])
+    assert torch.equal(layers, want)
+    want[[3, 4], 1] = torch.stack([want[0, 1], torch.zeros_like(want[0, 1])])
+    vr.copy_states(layers[:, 1], at(0, -1), at(3, 4), source=layers[:1, 1])        # the pool's own first page
+    assert torch.equal(layers, want)
+    flat = layers.flatten(1)
+    for pool, source in ((flat[:, :128], flat[2:3, 64:192]), (flat[2:3, 64:192], flat[:, :128]), (flat[:, :128], flat[5:, :128]), (flat[5:, 1:129], flat[5:, :128])):
+        with pytest.raises(RuntimeError):
+            vr.copy_states(pool, at(0), at(0), source=source)
+    assert torch.equal(layers, want)

@@ -169,6 +169,8 @@ extern "C" int vrwkv_copy_pages(void* pool, long long stride, int P, const void*
     if (M > SMALL_LIST && (!workspace || workspace_bytes < vrwkv_copy_pages_workspace_bytes(M))) { set_error("%s: workspace of %zu bytes, %zu needed", who, workspace ? workspace_bytes : 0, vrwkv_copy_pages_workspace_bytes(M)); return VRWKV_WORKSPACE_TOO_SMALL; }
     if (M > SMALL_LIST && ((size_t)workspace & 3)) { set_error("%s: workspace must be 4-byte aligned", who); return VRWKV_INVALID_ARG; }
     const char *a = static_cast<const char*>(pool), *b = static_cast<const char*>(source);
+    if (source_P == 1) source_stride = stride;            // (one page has no distance to a next one: it takes the other's)
+    else if (P == 1) stride = source_stride;
     const bool same = a == b && stride == source_stride;
     const long long a_end = (P - 1) * stride + page_bytes, b_end = source_P ? (source_P - 1) * source_stride + page_bytes : 0;
     // (pages of the same stride that lie in each other's gaps, as those of two layers in one pool, are apart as well)

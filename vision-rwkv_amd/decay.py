@@ -308,7 +308,7 @@ def copy_states(pool, src, dst, source=None):
     from another pool or out to one.  src -1 clears the page, dst -1 is a place of the list that is not taken; of several entries with the same dst the
     last counts.  src, dst: vectors of up to 4096 int32 or int64, on the device -- where entries outside the pools are left out -- or on the host, where
     they are refused.  Pools of any type whose pages are contiguous, at any distance; a source is the pool, or its pages overlap none of
-    the pool's (pool[:, 0] and pool[:, 1] of a pool for all layers).  No gradients, tangents or tracing, as in decay_attention_step."""
+    the pool's: memory of its own, or gaps between the pool's pages at the same distance (pool[:, 0] and pool[:, 1] of a pool for all layers, or one page of it).  No gradients, tangents or tracing, as in decay_attention_step."""
     if torch.compiler.is_compiling():
         return _eager(copy_states)(pool, src, dst, source)
     if _lib.host().copy_pages(pool, src, dst, source):
