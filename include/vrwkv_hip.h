@@ -340,8 +340,8 @@ int vrwkv_biwkv_bwd_like(const float* w, const float* u, const void* k, const vo
  * in ascending order, empty ones among them; strides of batch are not looked at.  Offsets outside 0..T are taken as 0 or T.
  * state: the states in front of the first tokens, (N, H, Dk, Dv) contiguous fp32, or NULL: zeros.  last: those behind the last tokens, or NULL.
  * y (batch, T, H, Dv) of dtype, contiguous; packed rows of no sequence get zeros.  States and sums are fp32.
- * y of a token is formed with the tokens of its chunk (64 or 32 from the sequence's front on): an infinity or NaN in k or v there may reach it from
- * behind; nothing does from other sequences or from rows outside of them. */
+ * Infinities and NaN go where the recurrence takes them: from a token to those behind it.  A head's segment with a result that is not finite is made
+ * again token by token. */
 typedef struct vrwkv_decay_args {
     const void *q, *k, *v, *g, *offsets;
     const float* state;

@@ -9,7 +9,7 @@ from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import vision_rwkv_amd as vr
-from test_decay_attention_gpu import DEV, DT
+from test_decay_attention_gpu import DEV, DT, HALF_STEP, make, reference
 
 
 def short(x, bits):
@@ -279,3 +279,79 @@ def test_one_page_of_a_layer(host, monkeypatch):
         with pytest.raises(RuntimeError):
             vr.copy_states(pool, at(0), at(0), source=source)
     assert torch.equal(layers, want)
+
+
+def as_defined(got, want, name, dtype, T, Dk, Dv):
+    """NaN where the recurrence in 64 bits has NaN, infinities where it has them, and what is finite within the bounds of ordinary results (compare())."""
+    x, (ref, scale) = got.detach().double().cpu(), want
+    for what, a, b in (("NaN", torch.isnan(x), torch.isnan(ref)), ("+inf", x == math.inf, ref == math.inf), ("-inf", x == -math.inf, ref == -math.inf)):
+        assert torch.equal(a, b), f"{name}: {int((a != b).sum())} of {a.numel()} {what} otherwise"
+    good = torch.isfinite(ref)
+    inner = (Dk + Dv + 128 + 3 * math.ceil(T / 32)) * 2.0 ** -24
+    # (a sum of absolute terms that is not finite belongs to a result that an infinity has reached and left again, as by a decay of -inf: none here)
+    limit = HALF_STEP[dtype] * ref.abs() + inner * scale + (2.0 ** -25 if dtype == "fp16" else 0.0) + 1e-30
+    over = ((x - ref).abs() / limit)[good & torch.isfinite(scale)]
+    assert not over.numel() or over.max() <= 1.0, f"{name}: {over.max():.3g} of the bound"
+
+
+def poison(ts, marks):
+    """Copies of q, k, v, g, S, gy, glast with numbers put where marks say: (tensor, index, value)."""
+    ts = {n: t.clone() for n, t in ts.items() if t is not None}
+    for n, at, x in marks:
+        ts[n][at] = x
+    return ts
+
+
+INF, NAN, HUGE = math.inf, math.nan, 3.4e38                # (finite in fp32; to bf16 it rounds up to infinity)
+#   what is where, in a row of 150 tokens; head 1 stays clean
+MARKS = {"k inf": [("k", (0, 70, 0, 3), INF)], "v inf": [("v", (0, 70, 0, 3), -INF)], "q inf": [("q", (0, 70, 0, 3), INF)], "v nan": [("v", (0, 40, 0, 5), NAN)], "k nan": [("k", (0, 149, 0, 0), NAN)],
+         "q nan": [("q", (0, 0, 0, 0), NAN)], "state inf": [("S", (0, 0, 2, 3), INF)], "state nan": [("S", (0, 0, 2, 3), NAN)], "last v": [("v", (0, 149, 0, 0), INF)],
+         "two": [("k", (0, 10, 0, 3), INF), ("v", (0, 130, 0, 1), -INF)], "against": [("v", (0, 20, 0, 3), INF), ("v", (0, 21, 0, 3), -INF)], "g nan": [("g", (0, 80, 0), NAN)],
+         "both rows": [("k", (0, 66, 0, 3), INF), ("k", (1, 5, 0, 3), NAN)]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 72), (20, 13)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_infinities_and_nan_go_where_the_definition_takes_them(dtype, Dk, Dv):
+    """Forwards: from a token to those behind it, and nowhere else."""
+    q, k, v, g, S = make(2, 150, 2, 2, 2, 2, Dk, Dv, dtype, state=2, seed=3)
+    for name, marks in MARKS.items():
+        ts = poison(dict(q=q, k=k, v=v, g=g, S=S), marks)
+        y, last = vr.decay_attention(*(ts[n] for n in "qkvg"), scale=0.3, state=ts["S"], return_state=True)
+        want = reference(*(ts[n] for n in "qkvg"), 0.3, ts["S"], [(0, 0, 150), (1, 0, 150)])
+        as_defined(y, want["y"], f"{name}: y", dtype, 150, Dk, Dv)
+        as_defined(last, want["last"], f"{name}: last", "fp32", 150, Dk, Dv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,Dk,Dv", [("fp32", 64, 64), ("bf16", 64, 64), ("bf16", 100, 64), ("fp16", 40, 100)])
+def test_infinities_and_nan_in_cut_and_packed_sequences(dtype, Dk, Dv):
+    """In front of a cut, in the middle of one, between sequences; the padding behind them holds what it likes."""
+    for offsets in (None, [0, 700], [5, 400, 400, 1100, 1150]):
+        T = 1160 if offsets else 700
+        N = len(offsets) - 1 if offsets else 1
+        q, k, v, g, S = make(1, T, 1, 1, 1, 1, Dk, Dv, dtype, state=N, seed=4, strong=0.1)
+        bounds = [(0, a, e) for a, e in zip(offsets[:-1], offsets[1:])] if offsets else [(0, 0, T)]
+        off = torch.tensor(offsets, device=DEV) if offsets else None
+        for name, marks in (("early", [("k", (0, 30, 0, 3), INF)]), ("late", [("v", (0, 620, 0, 3), NAN)]), ("cut", [("v", (0, 447, 0, 0), INF), ("k", (0, 448, 0, 1), INF)]),
+                            ("outside", [(n, (0, slice(1150, None)), NAN) for n in "qkvg"] if offsets and offsets[0] else [("q", (0, 5, 0, 0), INF)])):
+            ts = poison(dict(q=q, k=k, v=v, g=g, S=S), marks)
+            y, last = vr.decay_attention(*(ts[n] for n in "qkvg"), scale=0.3, state=ts["S"], offsets=off, return_state=True)
+            want = reference(*(ts[n] for n in "qkvg"), 0.3, ts["S"], bounds)
+            as_defined(y, want["y"], f"{offsets} {name}: y", dtype, T, Dk, Dv)
+            as_defined(last, want["last"], f"{offsets} {name}: last", "fp32", T, Dk, Dv)
+
+
+@pytest.mark.gpu
+def test_finite_numbers_above_those_of_bf16():
+    """fp32 rows and states near the type's largest number; products that stay in range."""
+    q, k, v, g, S = make(1, 100, 2, 2, 2, 2, 64, 64, "fp32", state=1, seed=6)
+    k, q = k * 1e-3, q * 1e-2
+    for name, marks in (("v", [("v", (0, 50, 0, 3), HUGE)]), ("state", [("S", (0, 0, 2, 3), -HUGE)]), ("small k", [("k", (0, 50, 0), 1e-30), ("v", (0, 50, 0), HUGE)])):
+        ts = poison(dict(q=q, k=k, v=v, g=g, S=S), marks)
+        y, last = vr.decay_attention(*(ts[n] for n in "qkvg"), scale=0.3, state=ts["S"], return_state=True)
+        want = reference(*(ts[n] for n in "qkvg"), 0.3, ts["S"], [(0, 0, 100)])
+        assert torch.isfinite(want["y"][0]).all() and torch.isfinite(want["last"][0]).all()
+        as_defined(y, want["y"], f"{name}: y", "fp32", 100, 64, 64)
+        as_defined(last, want["last"], f"{name}: last", "fp32", 100, 64, 64)

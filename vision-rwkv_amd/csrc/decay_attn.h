@@ -76,6 +76,7 @@ __device__ __forceinline__ int offset_at(const Call& p, int n) {
     const long long v = p.off64 ? static_cast<const long long*>(p.offsets)[n] : (long long)static_cast<const int*>(p.offsets)[n];
     return (int)(v < 0 ? 0 : v > p.T ? p.T : v);
 }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ Place sequence_place(const Call& p, int n, int L) {
     Place w{};
     w.n = n;
@@ -86,8 +87,8 @@ __device__ __forceinline__ Place sequence_place(const Call& p, int n, int L) {
         w.base = n;
         w.chunk0 = n * ((p.T + L - 1) / L);
     } else {
-        w.first = offset_at(p, n);
-        w.len = max(0, offset_at(p, n + 1) - w.first);
+        w.first = uniform(offset_at(p, n));
+        w.len = uniform(max(0, offset_at(p, n + 1) - w.first));
         w.base = 0;
         w.chunk0 = w.first / L + n;
     }
@@ -682,6 +683,12 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     }
 }
 
+}  // namespace decay
+}  // namespace vrwkv
+#include "decay_careful.h"
+namespace vrwkv {
+namespace decay {
+
 // Outputs.  Eight waves of two kinds, which need nothing of each other between two barriers: four take the tokens' outputs (16 tokens each), four the state
 // behind the chunk (16 columns each), its terms for the next one and the decays.  (Four waves that did one after the other: one image of 196 tokens 11.9 us, so 9.8; 2 x 4150 x 12
 // fp32 59.5, so 55; 4 x 16384 x 12 fp16 197, so 190.)
@@ -709,6 +716,9 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
     constexpr int STEPX = 256 / (DX / 8), STEPZ = 256 / (TZ / 8);   // rows between a thread's pieces
     float scale = p.scale;
     keep(scale);
+    __shared__ Careful careful;                           // (a result that is not finite is heard of by way of the LDS alone: a barrier that waits for the results on their way took 0.4 us)
+    careful_begin(careful);
+    float probe = 0.f;                                    // NaN once a result was not finite
 
     if (wave < 4) {
         const int rowx = tid / (DX / 8), dxo = tid % (DX / 8) * 8, o0 = order_of(dxo);
@@ -823,6 +833,10 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
                     }
                 }
             }
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) probe = fmaf(acc[j][i], 0.f, probe);
             so.store(acc, t0, t < n);
             lds_barrier();
         }
@@ -924,8 +938,19 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
 #pragma unroll
             for (int x = 0; x < NX; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s.store(16 * x + i, st[x][i]);
+                for (int i = 0; i < 4; ++i) {
+                    s.store(16 * x + i, st[x][i]);
+                    probe = fmaf(st[x][i], 0.f, probe);
+                }
         }
+    }
+    if (!(probe == 0.f)) careful.wanted = 1;
+    lds_barrier();
+    if (nc > 0 && uniform(careful.wanted)) {
+        static_assert(sizeof(CarefulLds<DX>) <= sizeof(S), "");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what has been stored arrives in front of what takes its place
+        __syncthreads();
+        careful_outputs<IO, DX, L>(careful, reinterpret_cast<CarefulLds<DX>&>(lds), offs);
     }
 }
 
