@@ -355,3 +355,60 @@ def test_finite_numbers_above_those_of_bf16():
         assert torch.isfinite(want["y"][0]).all() and torch.isfinite(want["last"][0]).all()
         as_defined(y, want["y"], f"{name}: y", "fp32", 100, 64, 64)
         as_defined(last, want["last"], f"{name}: last", "fp32", 100, 64, 64)
+
+
+def gradients_as_defined(ts, marks, dtype, what, offsets=None, scale=0.3):
+    """Of all inputs (a decay a token or a head), against the recurrence."""
+    ts = poison(ts, marks)
+    T = ts["q"].shape[1]
+    bounds = [(b, 0, T) for b in range(ts["q"].shape[0])] if offsets is None else [(0, a, e) for a, e in zip(offsets[:-1], offsets[1:])]
+    names = [n for n in "qkvgS" if n in ts]
+    leaves = [ts[n].clone().requires_grad_() for n in names]
+    y, last = vr.decay_attention(*leaves[:4], scale=scale, state=leaves[4] if "S" in ts else None, offsets=torch.tensor(offsets, device=DEV) if offsets else None, return_state=True)
+    got = torch.autograd.grad((y, last), leaves, (ts["gy"], ts["gl"]))
+    want = reference(*(ts[n] for n in "qkvg"), scale, ts.get("S"), bounds, ts["gy"], ts["gl"])
+    for n, x in zip(names, got):
+        kind = {torch.float32: "fp32", torch.bfloat16: "bf16", torch.float16: "fp16"}[x.dtype]
+        as_defined(x, want["dstate" if n == "S" else "d" + n], f"{what}: d{n}", kind, T, ts["q"].shape[-1], ts["v"].shape[-1])
+
+
+def backward_inputs(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype, N, g="fp32", seed=3, strong=1.0):
+    q, k, v, g, S = make(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype, g=g, state=N, seed=seed, strong=strong)
+    gen = torch.Generator(DEV).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    return dict(q=q, k=k, v=v, g=g, S=S, gy=r(B, T, H, Dv).to(q.dtype), gl=r(N, H, Dk, Dv))
+
+
+BACK_MARKS = {**MARKS, "gy inf": [("gy", (0, 70, 0, 3), INF)], "gy nan": [("gy", (0, 149, 0, 3), NAN)], "gl inf": [("gl", (0, 0, 2, 3), INF)], "gl nan": [("gl", (1, 0, 2, 3), NAN)]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (72, 128), (20, 13)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_gradients_of_infinities_and_nan(dtype, Dk, Dv):
+    """Backwards: into the gradients that the formulas give them to."""
+    ts = backward_inputs(2, 150, 2, 2, 2, 2, Dk, Dv, dtype, 2)
+    for name, marks in BACK_MARKS.items():
+        gradients_as_defined(ts, marks, dtype, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,Dk,Dv,g", [("fp32", 64, 64, "fp32"), ("bf16", 64, 64, "head"), ("bf16", 100, 64, "same"), ("fp16", 40, 100, "fp32")])
+def test_gradients_of_infinities_and_nan_in_cut_and_packed_sequences(dtype, Dk, Dv, g):
+    for offsets in (None, [0, 700], [5, 400, 400, 1100, 1150]):
+        T = 1160 if offsets else 700
+        ts = backward_inputs(1, T, 2, 1, 2, 1, Dk, Dv, dtype, len(offsets) - 1 if offsets else 1, g=dtype if g == "same" else g, seed=4, strong=0.1)
+        for name, marks in (("early", [("k", (0, 30, 0, 3), INF)]), ("late", [("v", (0, 620, 0, 3), NAN)]), ("cut", [("v", (0, 447, 0, 0), INF), ("gy", (0, 448, 0, 1), INF)]),
+                            ("outside", [(n, (0, slice(1150, None)), NAN) for n in ("q", "k", "v", "gy") + (("g",) if g != "head" else ())] if offsets and offsets[0] else [("q", (0, 5, 0, 0), INF)]),
+                            ("end", [("gl", (-1, 0, 0, 0), INF)])):
+            gradients_as_defined(ts, marks, dtype, f"{offsets} {name}", offsets)
+
+
+@pytest.mark.gpu
+def test_gradients_of_numbers_above_those_of_bf16():
+    ts = backward_inputs(1, 100, 2, 2, 2, 2, 64, 64, "fp32", 1, seed=6)
+    for n in "kqv":
+        ts[n] = ts[n] * 1e-3
+    ts["S"], ts["gl"] = ts["S"] * 1e-3, ts["gl"] * 1e-3
+    for name, marks in (("gy", [("gy", (0, 50, 0, 3), HUGE)]), ("gl", [("gl", (0, 0, 2, 3), HUGE)]), ("S", [("S", (0, 0, 2, 3), -HUGE)])):
+        gradients_as_defined(ts, marks, "fp32", name)

@@ -419,11 +419,11 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     t.dg_sums = b.sums;
     t.chunks = b.s.anchors;
     t.seg = b.r.seg;
+    t.state = a.state;
     t.glast = a.glast;
     t.dstate = a.dstate;
     t.Dk = a.Dk;
     t.Dv = a.Dv;
-    t.begun = a.state != nullptr;
     t.tk = b.tk;
     t.tv = b.tv;
     const bool vec = in_pieces(q, a.Dk, a.dtype) && in_pieces(k, a.Dk, a.dtype) && in_pieces(v, a.Dv, a.dtype) && in_pieces(gy, a.Dv, a.dtype) && in_pieces(t.out[0], a.Dk) && in_pieces(t.out[1], a.Dk) &&

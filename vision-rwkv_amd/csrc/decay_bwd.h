@@ -30,13 +30,18 @@ struct BwdParams : Call {
     OutView out[3];                                       // dq, dk, dv: what they make, next to each other: a kind reads its own with one load (parts lie rows * heads * channels apart)
     float* dg;                                            // [tiles][row][head]
     double* dg_sums;                                      // or, for decays that all tokens share, [segment][tiles][head]
-    const float *chunks;                                  // [chunk][head][tile of k][tile of v]: S0, rows of v's channels and columns of k's, as the accumulators lie
+    float* chunks;                                        // [chunk][head][tile of k][tile of v]: S0, rows of v's channels and columns of k's, as the accumulators lie
     const float *seg;                                     // [segment][head][..][..]: R behind the segment, without the decay of the token behind it; null: sequences are not cut
-    const float* glast;                                   // gradients of the states behind the last tokens, or null
+    const float *state, *glast;                           // the states in front of the first tokens; gradients of those behind the last; or null
     float* dstate;
     int Dk, Dv, tk, tv;                                   // channels; tiles of 64
-    int begun;                                            // there are states in front of the first tokens
 };
+
+}  // namespace decay
+}  // namespace vrwkv
+#include "decay_bwd_careful.h"
+namespace vrwkv {
+namespace decay {
 
 template <typename IO>
 struct BwdLds {
@@ -100,6 +105,9 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         return;
     }
     const int nc = (w.s1 - w.s0 + L - 1) / L;
+    __shared__ Careful careful;
+    careful_begin(careful);
+    float probe = 0.f;                                    // NaN once a result was not finite
 
     const int row0 = (tid & 255) >> 3, d0 = (tid & 7) * 8;
     // (half of gy: rows of even and odd blocks of 32 where a thread takes two of its own tensor, otherwise the workgroup's first and second 16)
@@ -125,7 +133,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         sb.load(rb, t0, n, false);
         if (wave == LIGHT) rg = gates.fetch(t0, lane, lane < n);
     };
-    const auto begun = [&](int c) { return c > 0 || !w.is_first || p.begun; };
+    const auto begun = [&](int c) { return c > 0 || !w.is_first || p.state; };
     const auto fetch_state = [&](int c) {
         const bool there = begun(c);
 #pragma unroll
@@ -210,9 +218,16 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         const double through = ((double)f.through[0] + f.through[1]) + ((double)f.through[2] + f.through[3]);
         const double all = flow_sum(inner, in, out, lane) + through;
         if (lane < n) {
+            probe = fmaf((float)all, 0.f, probe);
             if (dg) dg[(long long)(t0 + lane) * H] = (float)all;
             dg_total += all;
         }
+    };
+    const auto watch = [&](const f32x4 (&acc)[NT]) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) probe = fmaf(acc[j][i], 0.f, probe);
     };
     if (nc > 0) {
         if (wave == LIGHT) put_decays(lds.d[0]);
@@ -430,6 +445,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                     if ((index >> 2) < NT) flows.inner[w4][16 * (index >> 2) + 4 * quarter + (index & 3)] = cf;
                 }
             } else if (FLOW && lane_ < L) flows.inner[w4][lane_] = 0.f;
+            watch(acc);
             so.store(acc, t0, r0 < n);
             forget();
         } else if (kind == DK) {
@@ -480,6 +496,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                 }
             }
             have = true;
+            watch(acc);
             so.store(acc, t0, r0 < n);
             hold();
             if (wave == LIGHT) {
@@ -514,6 +531,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                 }
                 gathered(lds.q, fk, lds.gy, gh, gl, acc);
             }
+            watch(acc);
             so.store(acc, t0, r0 < n);
             // ---- X in front of the chunk
             const float ed = dec.end;
@@ -565,7 +583,18 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s.store(16 * x + i, st[x][i]);
+            for (int i = 0; i < 4; ++i) {
+                s.store(16 * x + i, st[x][i]);
+                probe = fmaf(st[x][i], 0.f, probe);
+            }
+    }
+    if (!(probe == 0.f)) careful.wanted = 1;
+    lds_barrier();
+    if (nc > 0 && uniform(careful.wanted)) {
+        static_assert(sizeof(CarefulBwdLds) <= sizeof(S), "");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // what has been stored arrives in front of what takes its place
+        __syncthreads();
+        careful_gradients<IO, FLOW, L, BWD_THREADS>(careful, reinterpret_cast<CarefulBwdLds&>(lds), offs);
     }
 }
 

@@ -45,10 +45,10 @@ __device__ __forceinline__ bool careful_finite(const float (&st)[DX][64], int ro
     return !__syncthreads_or(!(x == 0.f));
 }
 
-// st = exp(g) st + b c for the tokens from .. to - 1 of a sequence of len, or (rev) back along them with the decay of the token behind; out(token, lane, sum of a st) of
+// st = exp(g) st + b c c_scale for the tokens from .. to - 1 of a sequence of len, or (rev) back along them with the decay of the token behind; out(token, lane, sum of a a_scale st) of
 // those behind the first `skip` on the way.  Called by all threads.
 template <int DX, typename IO, typename F>
-__device__ __forceinline__ void careful_scan(CarefulLds<DX>& m, const Gates& gates, const CarefulRows<IO>& a, const CarefulRows<IO>& b, const CarefulRows<IO>& c, float c_scale, int from, int to, int len,
+__device__ __forceinline__ void careful_scan(CarefulLds<DX>& m, const Gates& gates, const CarefulRows<IO>& a, const CarefulRows<IO>& b, const CarefulRows<IO>& c, float a_scale, float c_scale, int from, int to, int len,
                                              bool rev, int skip, const F& out) {
     const int tid = threadIdx.x, wave = tid >> 6, rows = min(DX, b.count);
 #pragma unroll 1
@@ -61,7 +61,7 @@ __device__ __forceinline__ void careful_scan(CarefulLds<DX>& m, const Gates& gat
         for (int x = tid; x < CAREFUL_TOKENS * DX; x += blockDim.x) {
             const int i = x / DX, d = x % DX, t = t0 + (rev ? n - 1 - i : i);
             m.b[d][i] = b.at(t, d, i < n);
-            m.a[d][i] = a.at(t, d, wanted && i < n);
+            m.a[d][i] = a_scale * a.at(t, d, wanted && i < n);
         }
 #pragma unroll 1
         for (int x = tid; x < CAREFUL_TOKENS * 64; x += blockDim.x) {
@@ -152,9 +152,9 @@ __device__ __forceinline__ void careful_outputs(const Careful& careful, CarefulL
         });
         if (!seg || careful_finite(m.st, r.dx)) break;
     }
-    careful_scan(m, gates, q, k, v, 1.f, start, w.s1, w.len, false, w.s0 - start, [&](int token, int lane, float y) {
+    careful_scan(m, gates, q, k, v, p.scale, 1.f, start, w.s1, w.len, false, w.s0 - start, [&](int token, int lane, float y) {
         const int column = z * TZ + lane;
-        if (column < r.dz) static_cast<IO*>(r.o.p)[w.base * r.o.sb + (long long)(w.first + token) * r.o.st + h * r.o.sh + column] = from_f32<IO>(p.scale * y);
+        if (column < r.dz) static_cast<IO*>(r.o.p)[w.base * r.o.sb + (long long)(w.first + token) * r.o.st + h * r.o.sh + column] = from_f32<IO>(y);
     });
     if (r.last && w.is_last)
         careful_each<DX>(r.dx, [&](int row, int lane) {
