@@ -316,8 +316,9 @@ MARKS = {"k inf": [("k", (0, 70, 0, 3), INF)], "v inf": [("v", (0, 70, 0, 3), -I
 def test_infinities_and_nan_go_where_the_definition_takes_them(dtype, Dk, Dv):
     """Forwards: from a token to those behind it, and nowhere else."""
     q, k, v, g, S = make(2, 150, 2, 2, 2, 2, Dk, Dv, dtype, state=2, seed=3)
-    for name, marks in MARKS.items():
-        ts = poison(dict(q=q, k=k, v=v, g=g, S=S), marks)
+    positive = dict(q=q.abs(), k=k.abs(), v=v, g=g, S=S)   # (an infinity of v comes out as one)
+    for name, marks in [*MARKS.items(), ("v inf alone", MARKS["v inf"]), ("last v alone", MARKS["last v"])]:
+        ts = poison(positive if "alone" in name else dict(q=q, k=k, v=v, g=g, S=S), marks)
         y, last = vr.decay_attention(*(ts[n] for n in "qkvg"), scale=0.3, state=ts["S"], return_state=True)
         want = reference(*(ts[n] for n in "qkvg"), 0.3, ts["S"], [(0, 0, 150), (1, 0, 150)])
         as_defined(y, want["y"], f"{name}: y", dtype, 150, Dk, Dv)
@@ -390,6 +391,9 @@ def test_gradients_of_infinities_and_nan(dtype, Dk, Dv):
     ts = backward_inputs(2, 150, 2, 2, 2, 2, Dk, Dv, dtype, 2)
     for name, marks in BACK_MARKS.items():
         gradients_as_defined(ts, marks, dtype, name)
+    ts.update({n: ts[n].abs() for n in ("q", "k", "gl")})  # (an infinity of v or gy comes out as one)
+    for name in ("v inf", "gy inf", "last v"):
+        gradients_as_defined(ts, BACK_MARKS[name], dtype, name + ", positive")
 
 
 @pytest.mark.gpu
@@ -412,3 +416,26 @@ def test_gradients_of_numbers_above_those_of_bf16():
     ts["S"], ts["gl"] = ts["S"] * 1e-3, ts["gl"] * 1e-3
     for name, marks in (("gy", [("gy", (0, 50, 0, 3), HUGE)]), ("gl", [("gl", (0, 0, 2, 3), HUGE)]), ("S", [("S", (0, 0, 2, 3), -HUGE)])):
         gradients_as_defined(ts, marks, "fp32", name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (48, 80), (7, 13), (100, 66)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_steps_with_infinities_and_nan(dtype, Dk, Dv):
+    """Row by row, and as tokens of one page behind each other."""
+    N, H = 6, 2
+    q, k, v, g, S = make(N, 1, H, H, H, H, Dk, Dv, dtype, state=N, seed=8)
+    marks = [("v", (0, 0, 0, 3), INF), ("k", (1, 0, 0, 2), -INF), ("q", (2, 0, 0, 2), INF), ("S", (3, 0, 2, 3), INF), ("v", (4, 0, 0, 1), NAN), ("g", (5, 0, 0), NAN)]
+    q[0], k[0] = q[0].abs(), k[0].abs()                    # (so that an infinity of v comes out as one)
+    ts = poison(dict(q=q, k=k, v=v, g=g, S=S), marks)
+    row = [ts[n][:, 0] for n in "qkvg"]
+    pool = ts["S"].clone()
+    y = vr.decay_attention_step(*row, pool, scale=0.3)
+    want = reference(*(ts[n] for n in "qkvg"), 0.3, ts["S"], [(n, 0, 1) for n in range(N)])
+    as_defined(y[:, None], want["y"], "y", dtype, 1, Dk, Dv)
+    as_defined(pool, want["last"], "pool", "fp32", 1, Dk, Dv)
+    pool = ts["S"].clone()
+    y = vr.decay_attention_step(*row, pool, torch.zeros(N, dtype=torch.int32, device=DEV), scale=0.3)
+    want = reference(*(t[None] for t in row), 0.3, ts["S"][:1], [(0, 0, N)])
+    as_defined(y[None], want["y"], "tokens: y", dtype, N, Dk, Dv)
+    as_defined(pool[:1], want["last"], "tokens: pool", "fp32", N, Dk, Dv)

@@ -1,7 +1,7 @@
 // One more token for each of N sequences whose states are pages of a pool: S = exp(g) S + k v^T in place, y = scale S^T q (gfx950).
 // Bound by the pages, read and written once, past the caches' favour (512 sequences of 12 heads, 201 MB: 45.7 us where three pools take turns, 49.9 without; pools that the
-// last-level cache holds from step to step lose by it, 88 us for 81 with one pool of 201 MB): a workgroup holds 64 columns of one head's state in registers (sixteen rows of four columns a wave
-// instruction, 16 bytes a lane), with every load of the page on its way before the first is used.
+// last-level cache holds from step to step lose by it, 88 us for 81 with one pool of 201 MB): a workgroup holds 64 columns of one head's state in registers (four rows of sixty-four columns a wave
+// instruction, 16 bytes a lane; sixteen rows a workgroup), with every load of the page on its way before the first is used.
 // A slot that several rows name takes their tokens in the rows' order: the first row's workgroup goes through the others, which do nothing.
 #include "vrwkv_common.h"
 #include <algorithm>
@@ -102,12 +102,14 @@ __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
         const float e = expf(dec);
         if (known) {
 #pragma unroll
-            for (int i = 0; i < NX; ++i)
+            for (int i = 0; i < NX; ++i) {
+                const bool there = rg + 16 * i < p.Dk;    // (a row that is not: its zeros would be NaN beside an infinity of v)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    S[i][c] = fmaf(S[i][c], e, kk[i] * vv[c]);
+                    S[i][c] = there ? fmaf(S[i][c], e, kk[i] * vv[c]) : 0.f;
                     y[c] = fmaf(qq[i], S[i][c], y[c]);
                 }
+            }
         }
         if (next >= p.N && known) {
 #pragma unroll
