@@ -1,15 +1,17 @@
-"""decay_attention, decay_attention_step and copy_states at the edges of what they take: sums that cancel, and what is refused.
+"""decay_attention, decay_attention_step and copy_states at the edges of what they take: sums that cancel, infinities and NaN, what is refused, and the ways
+through the kernels that ordinary sizes do not take.
 
 The reference and the bounds of ordinary results are those of test_decay_attention_gpu.py."""
 import math
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import vision_rwkv_amd as vr
-from test_decay_attention_gpu import DEV, DT, HALF_STEP, make, reference
+from test_decay_attention_gpu import DEV, DT, HALF_STEP, check_all, make, reference
 
 
 def short(x, bits):
@@ -439,3 +441,41 @@ def test_steps_with_infinities_and_nan(dtype, Dk, Dv):
     want = reference(*(t[None] for t in row), 0.3, ts["S"][:1], [(0, 0, N)])
     as_defined(y[None], want["y"], "tokens: y", dtype, N, Dk, Dv)
     as_defined(pool[:1], want["last"], "tokens: pool", "fp32", N, Dk, Dv)
+
+
+# ---- instances and ways through the kernels that the sizes of test_decay_attention_gpu.py do not take -------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("Dk,Dv", [(128, 64), (100, 128), (72, 24)])
+def test_cut_sequences_of_large_heads(Dk, Dv, dtype):
+    """Outputs of more than 64 channels that start from a segment's state; gradients of cut sequences in two tiles of k and v."""
+    q, k, v, g, S = make(1, 700, 2, 2, 1, 2, Dk, Dv, dtype, state=1, strong=0.1)
+    check_all(q, k, v, g, S, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_many_pieces_of_one_sequence(dtype):
+    """More segments, forwards and back, than the scan over their states asks for at a time."""
+    q, k, v, g, S = make(1, 2100, 1, 1, 1, 1, 16, 24, dtype, state=1, strong=0.02)
+    check_all(q, k, v, g, S, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,H,D,dtype,state", [(900, 2, 8, "fp32", True), (900, 2, 8, "bf16", True), (800, 1, 128, "fp16", False)])
+def test_long_sequences_among_many_short_ones(N, H, D, dtype, state):
+    """More sequences than a workgroup has threads, most of a token or none and two that are cut: their segments' places are searched, and a scan in few
+    workgroups carries a state along them."""
+    lens = np.random.default_rng(N).integers(0, 4, N)
+    lens[[N // 3, N - 2]] = 1500, 700
+    offsets = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    q, k, v, g, S = make(1, offsets[-1], H, H, H, H, D, D, dtype, state=N if state else None, strong=0.1)
+    check_all(q, k, v, g, S, dtype, offsets=offsets)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 80)])
+def test_packed_and_cut_in_fp16(Dk, Dv):
+    q, k, v, g, S = make(1, 1200, 2, 1, 2, 2, Dk, Dv, "fp16", state=4, strong=0.1)
+    check_all(q, k, v, g, S, "fp16", offsets=[0, 700, 701, 701, 1150])
