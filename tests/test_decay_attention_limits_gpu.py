@@ -479,3 +479,37 @@ def test_long_sequences_among_many_short_ones(N, H, D, dtype, state):
 def test_packed_and_cut_in_fp16(Dk, Dv):
     q, k, v, g, S = make(1, 1200, 2, 1, 2, 2, Dk, Dv, "fp16", state=4, strong=0.1)
     check_all(q, k, v, g, S, "fp16", offsets=[0, 700, 701, 701, 1150])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("offsets", [None, [0, 900, 1000, 1700]])
+def test_an_infinite_state_under_decays_that_leave_fp32(offsets, dtype):
+    """It stays infinite through segments whose whole decay is below fp32's least number; a token that forgets makes NaN of it.  The gradient of the last states the same way."""
+    T, N = (offsets[-1], 3) if offsets else (900, 1)
+    ts = backward_inputs(1, T, 2, 2, 2, 2, 64, 64, dtype, N, seed=9)
+    ts["g"] = torch.full_like(ts["g"], -0.7)
+    for name, marks in (("kept", []), ("forgotten", [("g", (0, 500, 0), -INF)]), ("late", [("g", (0, 890, 0), -INF)])):
+        gradients_as_defined(ts, [("S", (0, 0, 2, 3), INF), ("gl", (0, 0, 5, 7), -INF), *marks], dtype, name, offsets)
+        y, last = vr.decay_attention(*(poison(ts, marks)[n] for n in "qkvg"), scale=0.3, state=poison(ts, [("S", (0, 0, 2, 3), INF)])["S"],
+                                     offsets=torch.tensor(offsets, device=DEV) if offsets else None, return_state=True)
+        want = reference(*(poison(ts, marks)[n] for n in "qkvg"), 0.3, poison(ts, [("S", (0, 0, 2, 3), INF)])["S"], [(0, a, e) for a, e in zip(offsets[:-1], offsets[1:])] if offsets else [(0, 0, T)])
+        as_defined(y, want["y"], f"{name}: y", dtype, T, 64, 64)
+        as_defined(last, want["last"], f"{name}: last", "fp32", T, 64, 64)
+
+
+@pytest.mark.gpu
+def test_a_long_sequence_that_is_nan_from_its_front_on():
+    """Its segments start from states that are NaN already, and none goes back to its front: 400 000 tokens take no second."""
+    T = 400_000
+    q, k, v, g, S = make(1, T, 1, 1, 1, 1, 64, 64, "bf16", seed=2)
+    k[0, 0] = NAN
+    off = torch.tensor([0, T], device=DEV)
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    vr.decay_attention(q[:, :300], k[:, :300], v[:, :300], g[:, :300])
+    begin.record()
+    y, last = vr.decay_attention(q, k, v, g, offsets=off, return_state=True)
+    end.record()
+    torch.cuda.synchronize()
+    assert torch.isnan(y).all() and torch.isnan(last).all()
+    assert begin.elapsed_time(end) < 200                   # (ms; each of 1 562 segments from the front on would have been 18 s of workgroups on 512 places)

@@ -530,6 +530,12 @@ __device__ __forceinline__ void decayed_terms(const __bf16 (&c)[in_terms<IO>][L]
     split8<3>(x8, f);
 }
 
+}  // namespace decay
+}  // namespace vrwkv
+#include "decay_careful.h"
+namespace vrwkv {
+namespace decay {
+
 // A segment's own state, or the states in front of a segment's chunks.  Four waves, 16 columns each, several workgroups a compute unit; four more that stage the next
 // chunk beside them were slower (4 x 16384 x 12 fp16: 67 us without, 87 with).
 template <typename IO, int DX, int MODE, bool VEC>
@@ -601,10 +607,14 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     float s_upd = r.s_upd;
     keep(s_upd);
 
-    float seg_log = 0.f;                                  // (STATES: the segment's whole decay, from wave 0)
+    float seg_log = 0.f;                                  // (STATES: the segment's whole decay, from wave 0,
+    unsigned long long forgets = 0;                       //  and whether a token of it keeps nothing)
     const auto put_decays = [&](typename S::Decays& d) {   // wave 0
-        const float end = chunk_decays<L>(d, gates.widen(rg), lane);
-        if (MODE == STATES) seg_log += end;
+        const float g = gates.widen(rg), end = chunk_decays<L>(d, g, lane);
+        if (MODE == STATES) {
+            seg_log += end;
+            forgets |= __builtin_amdgcn_ballot_w64(g < LOWEST_DECAY);
+        }
     };
     if (nc > 0 && wave == 0) put_decays(lds.d[0]);
     if (S::SCALED) lds_barrier();                         // (c is scaled with them)
@@ -679,15 +689,28 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
     if constexpr (MODE == STATES) {
 #pragma unroll
         for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.seg + seg_at + x * 1024) = st[x];
-        if (tid == 0 && z == 0) r.seg_decay[(long long)gid * p.H + h] = fast_exp2(seg_log);
+        if (tid == 0 && z == 0) {
+            const float d = fast_exp2(seg_log);
+            r.seg_decay[(long long)gid * p.H + h] = d == 0.f && forgets ? -0.f : d;    // (segments_kernel tells a product that is too small from one that is zero)
+        }
+        __shared__ int careful;
+        if (tid == 0) careful = 0;
+        float probe = 0.f;
+#pragma unroll
+        for (int x = 0; x < NX; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) probe = fmaf(st[x][i], 0.f, probe);
+        lds_barrier();
+        if (!(probe == 0.f)) careful = 1;
+        lds_barrier();
+        if (uniform(careful)) {
+            static_assert(sizeof(CarefulTokens<DX>) <= sizeof(S), "");
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            careful_segment<IO, DX>(reinterpret_cast<CarefulTokens<DX>&>(lds), p, r, w, gid, z, h);
+        }
     }
 }
-
-}  // namespace decay
-}  // namespace vrwkv
-#include "decay_careful.h"
-namespace vrwkv {
-namespace decay {
 
 // Outputs.  Eight waves of two kinds, which need nothing of each other between two barriers: four take the tokens' outputs (16 tokens each), four the state
 // behind the chunk (16 columns each), its terms for the next one and the decays.  (Four waves that did one after the other: one image of 196 tokens 11.9 us, so 9.8; 2 x 4150 x 12

@@ -53,7 +53,11 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
                     if (i0 + u > 0) *reinterpret_cast<f32x4*>(r.seg + (at(i0 + u) * r.tiles + z) * (DX * TZ) + in_tile + x * 1024) = carry[x];
                     if (i0 + u + 1 < count)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) carry[x][c] = fmaf(carry[x][c], d[u], own[u][x][c]);
+                        for (int c = 0; c < 4; ++c) {
+                            // (a decay of +0 is too small for fp32, and an infinity stays one; one of -0 forgets, and makes NaN of it)
+                            const bool stays = __builtin_bit_cast(unsigned, d[u]) == 0u && fabsf(carry[x][c]) == __builtin_inff();
+                            carry[x][c] = fmaf(carry[x][c], stays ? 1.f : d[u], own[u][x][c]);
+                        }
                 }
     }
 }
@@ -419,6 +423,7 @@ extern "C" int vrwkv_decay_bwd(const vrwkv_decay_args* args, void* hip_stream) {
     t.dg_sums = b.sums;
     t.chunks = b.s.anchors;
     t.seg = b.r.seg;
+    t.seg_front = b.s.seg;
     t.state = a.state;
     t.glast = a.glast;
     t.dstate = a.dstate;

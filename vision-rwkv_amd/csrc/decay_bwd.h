@@ -32,6 +32,7 @@ struct BwdParams : Call {
     double* dg_sums;                                      // or, for decays that all tokens share, [segment][tiles][head]
     float* chunks;                                        // [chunk][head][tile of k][tile of v]: S0, rows of v's channels and columns of k's, as the accumulators lie
     const float *seg;                                     // [segment][head][..][..]: R behind the segment, without the decay of the token behind it; null: sequences are not cut
+    const float* seg_front;                               // the same: S in front of the segment
     const float *state, *glast;                           // the states in front of the first tokens; gradients of those behind the last; or null
     float* dstate;
     int Dk, Dv, tk, tv;                                   // channels; tiles of 64

@@ -1,8 +1,7 @@
 // Gradients token by token in fp32, for the workgroups whose results are not all finite (decay_careful.h says when and why):
 //     R_t = exp(g_{t+1}) R_{t+1} + scale q_t gy_t^T,   dq_t = scale S_t gy_t,   dk_t = R_t v_t,   dv_t = R_t^T k_t,   dg_t = exp(g_t) <S_{t-1}, R_t>,   dS0 = exp(g_0) R_0
-// of one tile of 64 of k's and 64 of v's channels and the tokens of one segment: S from the sequence's front, R from its end, or from the nearer state in front of the segment or
-// gradient behind it where that is finite.  dg's states are kept at the front of every chunk, in the room of the states in front of the chunks, and made again from there.
-// 64 x 196 tokens, 12 heads of 64, bf16, with a NaN in every row: 1.9 ms for 95 us; 2 x 4150 fp32 2.3 ms for 135.
+// of one tile of 64 of k's and 64 of v's channels and the tokens of one segment, from the state in front of it and the gradient behind it.  dg's states are kept at the front of every chunk, in the room of the states in front of the chunks, and made again from there.
+// 64 x 196 tokens, 12 heads of 64, bf16, with a NaN in every row: 1.9 ms for 95 us; 2 x 4150 fp32 1.4 ms for 135.
 #pragma once
 
 namespace vrwkv {
@@ -28,6 +27,7 @@ __device__ __forceinline__ void careful_gradients(const Careful& careful, Carefu
     const long long tiles = p.tk * p.tv * 4096, mine = (ik * p.tv + iv) * 4096;
     float* const fronts = p.chunks + ((long long)(w.chunk0 + w.s0 / L) * p.H + h) * tiles + mine;   // of the segment's chunks; nobody else reads or writes them any more
     const long long front_step = p.H * tiles;
+    const float* const front = w.is_first ? nullptr : p.seg_front + ((long long)gid * p.H + h) * tiles + mine;
     const float* const behind = p.seg && !w.is_last ? p.seg + ((long long)gid * p.H + h) * tiles + mine : nullptr;
     Gates gates;
     gates.open(p, w.base, w.first, h);
@@ -43,34 +43,19 @@ __device__ __forceinline__ void careful_gradients(const Careful& careful, Carefu
     const auto state_at = [&](const float* s, int row, int lane) { return s && lane < nk ? s[page + (long long)(k0 + lane) * p.Dv + v0 + row] : 0.f; };
 
     // ---- S: dq, and the states at the chunks' fronts
-    int start = w.s0;
-    if (start > 0) {
-        careful_each<64>(nv, [&](int row, int lane) { m.st[row][lane] = fronts[careful_place(row, lane)]; });
-        if (!careful_finite(m.st, nv)) start = 0;
-    }
-    if (start == 0) careful_each<64>(nv, [&](int row, int lane) { m.st[row][lane] = state_at(p.state, row, lane); });
+    careful_each<64>(nv, [&](int row, int lane) { m.st[row][lane] = front ? front[careful_place(row, lane)] : state_at(p.state, row, lane); });
 #pragma unroll 1
-    for (int c = start < w.s0 ? -1 : 0; c < nc; ++c) {     // (-1: the tokens in front of the segment)
-        if (FLOW && c >= 0) careful_each<64>(nv, [&](int row, int lane) { fronts[c * front_step + careful_place(row, lane)] = m.st[row][lane]; });
-        const int from = c < 0 ? start : w.s0 + c * L, to = c < 0 ? w.s0 : min(w.s1, w.s0 + (c + 1) * L);
-        careful_scan(m, gates, gy, v, k, p.scale, 1.f, from, to, w.len, false, c < 0 ? to - from : 0, [&](int token, int lane, float x) { put(DQ, token, lane, x); });
+    for (int c = 0; c < nc; ++c) {
+        if (FLOW) careful_each<64>(nv, [&](int row, int lane) { fronts[c * front_step + careful_place(row, lane)] = m.st[row][lane]; });
+        const int from = w.s0 + c * L;
+        careful_scan(m, gates, gy, v, k, p.scale, 1.f, from, min(w.s1, from + L), w.len, false, [&](int token, int lane, float x) { put(DQ, token, lane, x); });
     }
-
-    // ---- R, as [v's][k's]: dk.  Where it starts: behind the segment, or at the sequence's end.
-    int end = w.s1;
-    if (behind) {
-        careful_each<64>(nv, [&](int row, int lane) { m.st[row][lane] = behind[careful_place(row, lane)]; });
-        if (!careful_finite(m.st, nv)) end = w.len;
-    }
-    const bool whole = end == w.len;                       // (of the last segment, or gone there)
-    if (whole) careful_each<64>(nv, [&](int row, int lane) { m.st[row][lane] = state_at(p.glast, row, lane); });
-    if (FLOW) {                                            // (R behind the segment's last token, and the next pass's start)
-        careful_scan(m, gates, v, gy, q, 1.f, p.scale, w.s1, end, w.len, true, end - w.s1, [](int, int, float) {});
-        careful_each<64>(nv, [&](int row, int lane) { f.r[row][lane] = m.st[row][lane]; });
-    }
+    // R behind the segment, as [v's][k's]
+    const auto behind_at = [&](int row, int lane) { return behind ? behind[careful_place(row, lane)] : state_at(p.glast, row, lane); };
     // ---- dg: R back along the tokens, S along them from the chunks' fronts
     if constexpr (FLOW) {
         double total = 0.;
+        careful_each<64>(nv, [&](int row, int lane) { f.r[row][lane] = behind_at(row, lane); });
 #pragma unroll 1
         for (int c = nc - 1; c >= 0; --c) {
             const int from = w.s0 + c * L, to = min(w.s1, from + L), blocks = (to - from + CAREFUL_TOKENS - 1) / CAREFUL_TOKENS;
@@ -145,13 +130,13 @@ __device__ __forceinline__ void careful_gradients(const Careful& careful, Carefu
         }
     }
     // ---- dk
-    careful_each<64>(nv, [&](int row, int lane) { m.st[row][lane] = whole ? state_at(p.glast, row, lane) : behind[careful_place(row, lane)]; });
-    careful_scan(m, gates, v, gy, q, 1.f, p.scale, w.s0, end, w.len, true, end - w.s1, [&](int token, int lane, float x) { put(DK, token, lane, x); });
+    careful_each<64>(nv, [&](int row, int lane) { m.st[row][lane] = behind_at(row, lane); });
+    careful_scan(m, gates, v, gy, q, 1.f, p.scale, w.s0, w.s1, w.len, true, [&](int token, int lane, float x) { put(DK, token, lane, x); });
     // ---- R the other way round, [k's][v's]: dv, and the first states' gradient
     careful_each<64>(nk, [&](int row, int lane) {
-        m.st[row][lane] = !whole ? behind[careful_place(lane, row)] : p.glast && lane < nv ? p.glast[page + (long long)(k0 + row) * p.Dv + v0 + lane] : 0.f;
+        m.st[row][lane] = behind ? behind[careful_place(lane, row)] : p.glast && lane < nv ? p.glast[page + (long long)(k0 + row) * p.Dv + v0 + lane] : 0.f;
     });
-    careful_scan(m, gates, k, q, gy, 1.f, p.scale, w.s0, end, w.len, true, end - w.s1, [&](int token, int lane, float x) { put(DV, token, lane, x); });
+    careful_scan(m, gates, k, q, gy, 1.f, p.scale, w.s0, w.s1, w.len, true, [&](int token, int lane, float x) { put(DV, token, lane, x); });
     if (p.dstate && w.is_first) {
         const float e = expf(gates.widen(gates.fetch(0, 0, true)));
         careful_each<64>(nk, [&](int row, int lane) {
