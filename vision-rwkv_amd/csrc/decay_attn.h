@@ -491,17 +491,17 @@ __device__ __forceinline__ void clear_outside(const Params& p, const Role& r, in
 template <size_t BYTES> constexpr int workgroups = 3 * BYTES <= 160 * 1024 ? 3 : 2 * BYTES <= 160 * 1024 ? 2 : 1;
 template <size_t BYTES> constexpr int out_workgroups = 2 * BYTES <= 160 * 1024 ? 2 : 1;
 
-// A chunk's decays by one wave, from its log decays (zero behind its last token); the sum of the powers of two.
+// A chunk's decays by one wave, from its log decays (zero behind its last token), those from its front times scale; the sum of the powers of two.
 // In 64 bits: a chunk's G may be thousands where a neighbour's difference is a hundredth.
 template <int L, typename D>
-__device__ __forceinline__ float chunk_decays(D& d, float g, int lane) {
+__device__ __forceinline__ float chunk_decays(D& d, float g, int lane, float scale = 1.f) {
     const double G = wave_scan_inclusive((double)g * 1.4426950408889634);
     const double end = lane_double(G, 63);
     const float gh = (float)G;
     if (lane < L) {
         d.gh[lane] = gh;
         d.gl[lane] = (float)(G - gh);
-        d.dt[lane] = fast_exp2(gh);
+        d.dt[lane] = fast_exp2(gh) * scale;
         d.dk[lane] = fast_exp2((float)(end - G));
     }
     if (lane == 0) d.end = fast_exp2((float)end);

@@ -144,9 +144,9 @@ int slots(int dtype, int dx, bool backward) {
     const int per_cu = backward ? 1 : dtype == VRWKV_F32 && dx == 128 ? 1 : 2;
     return per_cu * device_cus();
 }
-// Tokens of a segment.  Calls of fewer sequences and heads than fill the chip are cut, into pieces that fill it in as few rounds as it takes: a round
+// Tokens of a segment.  Rows of a batch: calls of fewer sequences and heads than fill the chip are cut, into that number of pieces, up to 64 a row, whose estimated time is least: a round
 // lasts as long as its longest piece's chunks and two or three more for its start; pieces cost another pass over their rows for their states,
-// half as long, and one over the states.  (Gradients of 48 sequences of 577 tokens in tiles of 64 of 80 channels, fp16: 1 piece 130 us, 2 pieces 109, 3 119, 5 105; of 24 of 4150,
+// half as long, and one over the states.  The numbers are fitted to the measurements below, on one card, and to no others.  (Gradients of 48 sequences of 577 tokens in tiles of 64 of 80 channels, fp16: 1 piece 130 us, 2 pieces 109, 3 119, 5 105; of 24 of 4150,
 // fp32: 8 pieces 215, 10 189, 11 222, 22 202.  Outputs of the latter: 10 pieces 60, 13 63, 17 55, 22 57; of 48
 // of 16384, fp16: 8 pieces 219, 10 189, 11 206, 16 182, 20 194, 32 190.)
 int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool backward) {
@@ -171,7 +171,8 @@ int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool ba
         }
         return best * 64;
     }
-    // packed: some sequence may be as long as all of them
+    // Packed: the host does not know the lengths, and some sequence may be as long as all of them together: as many pieces of all tokens as fill the chip twice, of 256 tokens
+    // at least (that is a plain quotient: no estimate can be made of lengths that are not known, and rows that would stay whole in a batch are cut here).
     return (int)std::max<long long>(256, (long long)a.T * wgs / (2 * room) / 64 * 64);
 }
 bool cut(const vrwkv_decay_args& a, int seg_len) { return a.T > seg_len; }

@@ -9,8 +9,8 @@
 // Twelve waves, three a SIMD, of three kinds: dq and dg's crossings inside the chunk (tokens t along the lanes), dk, and dv and X (tokens s along the lanes).  What
 // one kind waits for the others cover: with dk, dv and X in one kind of eight waves a chunk of 64 bf16 tokens took 12 900 cycles, 60 % of them with an instruction; with
 // sixteen waves the registers did not do.
-// Every operand of the products is read as it lies or across its rows, so the chunk's rows are staged once, where dv, dk and dq by themselves (decay_attn.h)
-// stage ten tensors.  X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
+// Every operand of the products is read as it lies or across its rows, so the chunk's rows are staged once (a pass each for dv, dk and dq would stage ten
+// tensors for these four).  X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
 // Larger heads go in tiles of 64 of k's and 64 of v's channels.  Everything is a sum over one or both kinds of tiles: dq and dk over v's, dv over k's, dg over
 // all pairs; the parts are added up in fp32 behind.
 // 64 x 196 tokens, 12 heads of 64, bf16: 76 us and 15.7 for the states in front (194 MB: 2.1 TB/s), the vector units busy 42 %, the matrix units 12, the LDS 32 (12 of it
@@ -196,18 +196,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
     keep(H);
     keep(scale);
 
-    const auto put_decays = [&](typename S::Decays& d) {   // the light wave
-        const double G = wave_scan_inclusive((double)gates.widen(rg) * 1.4426950408889634);
-        const double end = lane_double(G, 63);
-        const float gh = (float)G;
-        if (lane < L) {
-            d.gh[lane] = gh;
-            d.gl[lane] = (float)(G - gh);
-            d.dt[lane] = fast_exp2(gh) * scale;
-            d.dk[lane] = fast_exp2((float)(end - G));
-        }
-        if (lane == 0) d.end = fast_exp2((float)end);
-    };
+    const auto put_decays = [&](typename S::Decays& d) { chunk_decays<L>(d, gates.widen(rg), lane, scale); };   // the light wave
     const auto put_flows = [&](const typename S::Flows& f, int t0, int n) {   // the light wave
         const int at = min(lane, L - 1);
         double in = 0., out = 0.;
@@ -285,10 +274,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         // channels 16 x + col along the lanes, tokens 32 ks + 4 quarter .. and 16 behind those side by side
         const auto across = [&](const __bf16 (&a)[NS][L][PX], int x, int ks, bf16x8 (&f)[NS]) {
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const __bf16* q = &a[s][32 * ks + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
-                f[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
-            }
+            for (int s = 0; s < NS; ++s) f[s] = across8(&a[s][32 * ks + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)], PX);
         };
         const auto widen4 = [&](const __bf16 (&a)[NS][L][PX], int row, int x, float (&o)[4]) {   // channels 16 x + 4 quarter + i
 #pragma unroll
@@ -520,10 +506,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
                         for (int kx = 0; kx < 2; ++kx) {
                             bf16x8 fy[3];
 #pragma unroll
-                            for (int s = 0; s < 3; ++s) {
-                                const __bf16* q = &lds.x[s][32 * kx + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)];
-                                fy[s] = wkv6_detail::cat8(wkv6_detail::lds_read_tr4(q), wkv6_detail::lds_read_tr4(q + 16 * PX));
-                            }
+                            for (int s = 0; s < 3; ++s) fy[s] = across8(&lds.x[s][32 * kx + 4 * quarter + (col >> 2)][(x >> 1) * 32 + (x & 1) * 4 + 8 * (col & 3)], PX);
                             acc[j] = mma<2>(acc[j], fy, fk[kx]);
                         }
 #pragma unroll
