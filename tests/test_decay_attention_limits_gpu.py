@@ -482,6 +482,21 @@ def test_packed_and_cut_in_fp16(Dk, Dv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 7, 8, 9, 33, 64, 65])
+def test_infinities_in_short_sequences(T):
+    """Outputs and gradients; blocks of tokens that are not full, chunks that are."""
+    for dtype, g in (("fp32", "fp32"), ("bf16", "head"), ("fp16", "same")):
+        ts = backward_inputs(3, T, 2, 2, 1, 2, 24, 40, dtype, 3, g=dtype if g == "same" else g, seed=T)
+        marks = [("k", (0, 0, 0, 3), INF), ("v", (1, T - 1, 0, 3), -INF), ("gy", (2, T // 2, 1, 0), NAN)]
+        gradients_as_defined(ts, marks, dtype, f"{T}")
+        bad = poison(ts, marks)
+        y, last = vr.decay_attention(*(bad[n] for n in "qkvg"), scale=0.3, state=bad["S"], return_state=True)
+        want = reference(*(bad[n] for n in "qkvg"), 0.3, bad["S"], [(b, 0, T) for b in range(3)])
+        as_defined(y, want["y"], f"{T}: y", dtype, T, 24, 40)
+        as_defined(last, want["last"], f"{T}: last", "fp32", T, 24, 40)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("offsets", [None, [0, 900, 1000, 1700]])
 def test_an_infinite_state_under_decays_that_leave_fp32(offsets, dtype):
