@@ -5,8 +5,9 @@
 // four matrix products.  The state in front of each chunk, and the same sum back along the tokens (b, c = gy, q in the places of k, v: the gradient of a
 // state), which the gradients want (decay_bwd.h), are this kernel's without its outputs.
 // Calls of few sequences are cut into segments: a pass makes each segment's own state, a second adds them up, the third starts from them.
-// 64 x 196 tokens, 12 heads of 64, bf16: 23.6 us, 90 MB at 3.8 TB/s.  4 x 16384 in fp16, where operands have two terms: 62 us for the segments' states, 10 to add them up
-// and 128 for the outputs, of which the vector units are busy 47 %, the LDS 51, the matrix units 24: bound by a chunk's chain of staging, products, exponentials and products again.
+// What lies between operands (P, states) has 24 bits, three bf16 terms, in every type: with two, sums that cancel kept 2^-18 of their terms, and 64 x 196 x 12 heads in bf16 took 24.7 us.
+// 64 x 196 tokens, 12 heads of 64, bf16: 27 us, 90 MB at 3.3 TB/s.  4 x 16384 in fp16, where rows have two terms: 204 to 214 us, a third of them for the segments' states, 10 to add them
+// up, the rest for the outputs, of which the vector units are busy 50 %, the LDS 43, the matrix units 29: bound by a chunk's chain of staging, products, exponentials and products again.
 #pragma once
 #include "wave_sum.h"
 #include "wkv6_chunk_common.h"
@@ -713,8 +714,8 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 }
 
 // Outputs.  Eight waves of two kinds, which need nothing of each other between two barriers: four take the tokens' outputs (16 tokens each), four the state
-// behind the chunk (16 columns each), its terms for the next one and the decays.  (Four waves that did one after the other: one image of 196 tokens 11.9 us, so 9.8; 2 x 4150 x 12
-// fp32 59.5, so 55; 4 x 16384 x 12 fp16 197, so 190.)
+// behind the chunk (16 columns each), its terms for the next one and the decays.  (Four waves that did one after the other: one image of 196 tokens 22 % longer; 2 x 4150 x 12
+// fp32 8 %; 4 x 16384 x 12 fp16 4 %.)
 template <typename IO, int DX, bool VEC>
 __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX, PLAIN>)>)) void decay_kernel(const Params p) {
     using S = Lds<IO, DX, PLAIN>;

@@ -148,7 +148,7 @@ int slots(int dtype, int dx, bool backward) {
 // lasts as long as its longest piece's chunks and two or three more for its start; pieces cost another pass over their rows for their states,
 // half as long, and one over the states.  The numbers are fitted to the measurements below, on one card, and to no others.  (Gradients of 48 sequences of 577 tokens in tiles of 64 of 80 channels, fp16: 1 piece 130 us, 2 pieces 109, 3 119, 5 105; of 24 of 4150,
 // fp32: 8 pieces 215, 10 189, 11 222, 22 202.  Outputs of the latter: 10 pieces 60, 13 63, 17 55, 22 57; of 48
-// of 16384, fp16: 8 pieces 219, 10 189, 11 206, 16 182, 20 194, 32 190.)
+// of 16384, fp16: 8 pieces 219, 10 189, 11 206, 16 182, 20 194, 32 190.  Taken with intermediate operands of two terms, which made 16-bit calls some 10 % shorter.)
 int segment_len(const vrwkv_decay_args& a, int dx, int tiles, int roles, bool backward) {
     const long long wgs = (long long)a.H * tiles * roles, room = slots(a.dtype, dx, backward);
     if (!a.offsets) {

@@ -13,8 +13,8 @@
 // tensors for these four).  X lies in registers, rows of v's channels, and its terms in the LDS as [k's channel][v's], which both dk (rows) and dv (across) read.
 // Larger heads go in tiles of 64 of k's and 64 of v's channels.  Everything is a sum over one or both kinds of tiles: dq and dk over v's, dv over k's, dg over
 // all pairs; the parts are added up in fp32 behind.
-// 64 x 196 tokens, 12 heads of 64, bf16: 76 us and 15.7 for the states in front (194 MB: 2.1 TB/s), the vector units busy 42 %, the matrix units 12, the LDS 32 (12 of it
-// conflicts); 2 x 4150 fp32: 82 us.  A workgroup a compute unit, three a SIMD of its waves: bound by the latencies of a chunk's steps, 12 000 cycles of which no kind is idle more than
+// 64 x 196 tokens, 12 heads of 64, bf16: 82 us and 14.5 for the states in front (194 MB: 2.0 TB/s), the vector units busy 43 %, the matrix units 13, the LDS 31 (13 of it
+// conflicts); 2 x 4150 fp32: 83 us.  A workgroup a compute unit, three a SIMD of its waves: bound by the latencies of a chunk's steps, 12 000 cycles of which no kind is idle more than
 // 2500, and by 8600 at a sequence's start.
 #pragma once
 #include "decay_attn.h"

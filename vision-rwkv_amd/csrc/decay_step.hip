@@ -1,5 +1,5 @@
 // One more token for each of N sequences whose states are pages of a pool: S = exp(g) S + k v^T in place, y = scale S^T q (gfx950).
-// Bound by the pages, read and written once, past the caches' favour (512 sequences of 12 heads, 201 MB: 45.7 us where three pools take turns, 49.9 without; pools that the
+// Bound by the pages, read and written once, past the caches' favour (512 sequences of 12 heads, 201 MB: 43 us where three pools take turns, 4 more without; pools that the
 // last-level cache holds from step to step lose by it, 88 us for 81 with one pool of 201 MB): a workgroup holds 64 columns of one head's state in registers (four rows of sixty-four columns a wave
 // instruction, 16 bytes a lane; sixteen rows a workgroup), with every load of the page on its way before the first is used.
 // A slot that several rows name takes their tokens in the rows' order: the first row's workgroup goes through the others, which do nothing.
