@@ -528,3 +528,17 @@ def test_a_long_sequence_that_is_nan_from_its_front_on():
     torch.cuda.synchronize()
     assert torch.isnan(y).all() and torch.isnan(last).all()
     assert begin.elapsed_time(end) < 200                   # (ms; each of 1 562 segments from the front on would have been 18 s of workgroups on 512 places)
+
+
+def test_the_workspace_of_many_packed_sequences():
+    """States are kept for the segments that there can be, not for every sequence: two to each length of a segment."""
+    a, lib = vr._lib.DecayArgs(), vr.lib()
+    a.offsets = 4096
+    a.N, a.T, a.H, a.Hq, a.Hk, a.Hv, a.Dk, a.Dv = 4096, 4096 * 64, 16, 16, 16, 16, 128, 64
+    page = 16 * 128 * 64 * 4
+    many = lib.vrwkv_decay_fwd_workspace_bytes(a)
+    assert 0 < many <= 2 * (a.T // 256 + 1) * page         # (a segment has 256 tokens or more)
+    a.N = 1
+    assert 0 < lib.vrwkv_decay_fwd_workspace_bytes(a) <= many
+    a.N = 1 << 14
+    assert lib.vrwkv_decay_fwd_workspace_bytes(a) == many

@@ -39,7 +39,7 @@ struct Role {
     OutView o;
     const float* init;                                    // states (N, H, Dk, Dv), or null: zeros
     float* last;                                          // where the states behind the last token go, or null
-    float *seg, *seg_decay;                               // [segment][head][tile] a segment's state (first its own, then that in front of it), [segment][head]
+    float *seg, *seg_decay;                               // [page][head][tile] a segment's state (first its own, then that in front of it), [page][head]; segment_page()
     float* anchors;                                       // [chunk][head][tile]: the state in front of each chunk
     long long sx, sz;                                     // strides of the states' contracted and other index
     int dx, dz, tiles, reverse;                           // (one or two tiles; the roles of a launch have the same)
@@ -52,6 +52,7 @@ struct Call {                                             // sequences, their cu
     int off64, g_dtype, N, T, H;                          // T: tokens of a row of the batch (packed: of all sequences)
     int seg_len, nseg, segs;                              // tokens of a segment; segments of a row (0: packed); of the call
     float scale;
+    int by_start;                                         // packed: segments' states lie by where the segments start
 };
 struct Params : Call {
     int n_roles;
@@ -69,6 +70,7 @@ struct Place {                                            // a workgroup's segme
     int n, first, len;                                    // sequence; its first token and length
     int s0, s1;                                           // the segment's tokens, from the first
     int base;                                             // batch row
+    int page;                                             // of the segment's state
     int chunk0;                                           // number of the sequence's first chunk
     int front, back;                                      // packed: where the first sequence begins, and the last one ends
     bool is_last, is_first, valid;
@@ -97,6 +99,9 @@ __device__ __forceinline__ Place sequence_place(const Call& p, int n, int L) {
 }
 // Packed sequences: n's segments have the numbers from first(n) / seg_len + n on, which grow with n and leave each its room whatever its length.
 __device__ __forceinline__ int first_segment(const Call& p, int n, int first) { return p.nseg ? n * p.nseg : first / p.seg_len + n; }
+// The page of segment j of a sequence that is cut (others have none in use).  Of many packed sequences few can be: in any seg_len tokens at most one first segment of such a
+// sequence begins, and one that is not its first, so two pages to each of them do, where a page to each sequence was 2.1 GB for 4096 prompts of 64 tokens and 16 heads of 128 x 64.
+__device__ __forceinline__ int segment_page(const Call& p, int n, int first, int j) { return p.by_start ? 2 * (first / p.seg_len + j) + (j == 0 ? 1 : 0) : first_segment(p, n, first) + j; }
 __device__ __forceinline__ int segment_count(const Call& p, int len) { return max(1, (len + p.seg_len - 1) / p.seg_len); }
 
 // offs: THREADS_ numbers of shared memory (packed sequences: one read of the offsets where they are fewer than the threads).
@@ -137,6 +142,7 @@ __device__ __forceinline__ Place find_place(const Call& p, int gid, int L, int* 
     if (!w.valid) return w;
     const int j = gid - first_segment(p, w.n, w.first), count = segment_count(p, w.len);
     w.valid = j >= 0 && j < count;
+    w.page = segment_page(p, w.n, w.first, j);
     w.s0 = j * p.seg_len;
     w.s1 = min(w.len, w.s0 + p.seg_len);
     w.is_first = j == 0;
@@ -588,7 +594,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
 
     // ---- the state that the segment starts from: rows 16 x + 4 quarter + i, column 16 wave + col of the tile
     f32x4 st[NX];
-    const long long seg_at = (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4;
+    const long long seg_at = (((long long)w.page * p.H + h) * r.tiles + z) * (DX * TZ) + (wave * 64 + lane) * 4;
     bool have = MODE == CHUNKS && (!w.is_first || r.init);
     if (MODE == CHUNKS && !w.is_first) {
 #pragma unroll
@@ -692,7 +698,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
         for (int x = 0; x < NX; ++x) *reinterpret_cast<f32x4*>(r.seg + seg_at + x * 1024) = st[x];
         if (tid == 0 && z == 0) {
             const float d = fast_exp2(seg_log);
-            r.seg_decay[(long long)gid * p.H + h] = d == 0.f && forgets ? -0.f : d;    // (segments_kernel tells a product that is too small from one that is zero)
+            r.seg_decay[(long long)w.page * p.H + h] = d == 0.f && forgets ? -0.f : d;    // (segments_kernel tells a product that is too small from one that is zero)
         }
         __shared__ int careful;
         if (tid == 0) careful = 0;
@@ -708,7 +714,7 @@ __global__ __launch_bounds__(THREADS, (workgroups<sizeof(Lds<IO, DX, MODE>)>)) v
             static_assert(sizeof(CarefulTokens<DX>) <= sizeof(S), "");
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            careful_segment<IO, DX>(reinterpret_cast<CarefulTokens<DX>&>(lds), p, r, w, gid, z, h);
+            careful_segment<IO, DX>(reinterpret_cast<CarefulTokens<DX>&>(lds), p, r, w, z, h);
         }
     }
 }
@@ -885,7 +891,7 @@ __global__ __launch_bounds__(OUT_THREADS, (2 * out_workgroups<sizeof(Lds<IO, DX,
         const int zc = z0 + 16 * w4 + col;
         if (!w.is_first) {
 #pragma unroll
-            for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ) + ((x * 4 + w4) * 64 + lane) * 4);
+            for (int x = 0; x < NX; ++x) st[x] = *reinterpret_cast<const f32x4*>(r.seg + (((long long)w.page * p.H + h) * r.tiles + z) * (DX * TZ) + ((x * 4 + w4) * 64 + lane) * 4);
         } else if (begun) {
             const StatePage s(r.init + page, r.sx, r.sz, r.dx, r.dz, 4 * quarter, zc);
 #pragma unroll

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
     const int h = id % p.H, n = id / p.H;
     const Place w = sequence_place(p, n, 64);
     const int x0 = blockIdx.x % XG * XS, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int first = first_segment(p, n, w.first), count = segment_count(p, w.len);
+    const int count = segment_count(p, w.len);
     if (count == 1) return;                               // (starts from what it is given)
     f32x4 carry[XS];
 #pragma unroll
@@ -33,7 +33,11 @@ __global__ __launch_bounds__(THREADS) void segments_kernel(const Params p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) carry[x][i] = s.load(16 * x + i);
     }
-    const auto at = [&](int i) { return ((long long)(first + (r.reverse ? count - 1 - i : i)) * p.H + h); };    // the i-th on the way
+    const int lead = segment_page(p, n, w.first, 0), step = p.by_start ? 2 : 1, rest = segment_page(p, n, w.first, 1) - step;
+    const auto at = [&](int i) {                          // the i-th on the way
+        const int j = r.reverse ? count - 1 - i : i;
+        return (long long)(j == 0 ? lead : rest + step * j) * p.H + h;
+    };
     const long long in_tile = ((long long)x0 * 4 + wave) * 64 * 4 + lane * 4;
     for (int i0 = 0; i0 < count; i0 += U) {
         f32x4 own[U][XS];
@@ -179,6 +183,9 @@ bool cut(const vrwkv_decay_args& a, int seg_len) { return a.T > seg_len; }
 long long segment_total(const vrwkv_decay_args& a, int seg_len) {
     return a.offsets ? (long long)a.T / seg_len + a.N : (long long)a.N * ((a.T + seg_len - 1) / seg_len);
 }
+// pages of states: the segments' or, of many packed sequences, by where segments start (segment_page)
+bool by_start(const vrwkv_decay_args& a, int seg_len) { return a.offsets && a.N > a.T / seg_len + 2; }
+long long page_total(const vrwkv_decay_args& a, int seg_len) { return by_start(a, seg_len) ? 2 * ((long long)a.T / seg_len + 1) : segment_total(a, seg_len); }
 long long chunk_total(const vrwkv_decay_args& a, int L) { return a.offsets ? (long long)a.T / L + a.N : (long long)a.N * ((a.T + L - 1) / L); }
 long long rows_of(const vrwkv_decay_args& a) { return a.offsets ? a.T : (long long)a.N * a.T; }
 
@@ -245,6 +252,7 @@ P common(const vrwkv_decay_args& a, int seg_len) {
     p.seg_len = seg_len;
     p.nseg = a.offsets ? 0 : (a.T + seg_len - 1) / seg_len;
     p.segs = (int)segment_total(a, seg_len);
+    p.by_start = by_start(a, seg_len);
     p.scale = a.scale;
     return p;
 }
@@ -272,9 +280,9 @@ int launch_segments(const Params& p, int dtype, int dx, hipStream_t st) {
     else hipLaunchKernelGGL((segments_kernel<128, 4>), grid, block, 0, st, p);
     return check_launch("decay_attention (segments)");
 }
-void take_segments(Role& r, Pieces& ws, const vrwkv_decay_args& a, long long segs, int dx) {
-    r.seg = ws.take<float>((size_t)segs * a.H * r.tiles * dx * TZ);
-    r.seg_decay = ws.take<float>((size_t)segs * a.H);
+void take_segments(Role& r, Pieces& ws, const vrwkv_decay_args& a, long long pages, int dx) {
+    r.seg = ws.take<float>((size_t)pages * a.H * r.tiles * dx * TZ);
+    r.seg_decay = ws.take<float>((size_t)pages * a.H);
 }
 
 struct FwdPlan {
@@ -286,7 +294,7 @@ struct FwdPlan {
         role.dz = a.Dv;
         role.tiles = tiles_of(a.Dv);
         seg_len = segment_len(a, dx, role.tiles, 1, false);
-        if (cut(a, seg_len)) take_segments(role, ws, a, segment_total(a, seg_len), dx);
+        if (cut(a, seg_len)) take_segments(role, ws, a, page_total(a, seg_len), dx);
     }
 };
 // A pass that keeps the states in front of the chunks, and one for all gradients (decay_bwd.h); tiles of 64 channels of larger heads, and heads that share a row of q, k or v, leave
@@ -307,8 +315,8 @@ struct BwdPlan {
         seg_len = segment_len(a, dxv, tk * tv, 1, true);
         const long long segs = segment_total(a, seg_len), rows = rows_of(a);
         if (cut(a, seg_len)) {
-            take_segments(r, ws, a, segs, dxv);
-            take_segments(s, ws, a, segs, dxv);
+            take_segments(r, ws, a, page_total(a, seg_len), dxv);
+            take_segments(s, ws, a, page_total(a, seg_len), dxv);
         }
         if (a.dq && (a.Hq < a.H || tv > 1)) fq = ws.take<float>((size_t)rows * a.H * a.Dk * tv);
         if (a.dk && (a.Hk < a.H || tv > 1)) fk = ws.take<float>((size_t)rows * a.H * a.Dk * tv);

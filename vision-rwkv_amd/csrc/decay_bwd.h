@@ -31,7 +31,7 @@ struct BwdParams : Call {
     float* dg;                                            // [tiles][row][head]
     double* dg_sums;                                      // or, for decays that all tokens share, [segment][tiles][head]
     float* chunks;                                        // [chunk][head][tile of k][tile of v]: S0, rows of v's channels and columns of k's, as the accumulators lie
-    const float *seg;                                     // [segment][head][..][..]: R behind the segment, without the decay of the token behind it; null: sequences are not cut
+    const float *seg;                                     // [page][head][..][..]: R behind the segment, without the decay of the token behind it; null: sequences are not cut
     const float* seg_front;                               // the same: S in front of the segment
     const float *state, *glast;                           // the states in front of the first tokens; gradients of those behind the last; or null
     float* dstate;
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(BWD_THREADS, 3) void decay_bwd_kernel(const BwdPara
         const float d = fast_exp2(gates.widen(gates.fetch(w.s1, 0, true)) * LOG2E);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            st[x] = *reinterpret_cast<const f32x4*>(p.seg + ((long long)gid * p.H + h) * tiles + my_tile + x * 1024);
+            st[x] = *reinterpret_cast<const f32x4*>(p.seg + ((long long)w.page * p.H + h) * tiles + my_tile + x * 1024);
 #pragma unroll
             for (int i = 0; i < 4; ++i) st[x][i] *= d;
         }

@@ -27,8 +27,8 @@ __device__ __forceinline__ void careful_gradients(const Careful& careful, Carefu
     const long long tiles = p.tk * p.tv * 4096, mine = (ik * p.tv + iv) * 4096;
     float* const fronts = p.chunks + ((long long)(w.chunk0 + w.s0 / L) * p.H + h) * tiles + mine;   // of the segment's chunks; nobody else reads or writes them any more
     const long long front_step = p.H * tiles;
-    const float* const front = w.is_first ? nullptr : p.seg_front + ((long long)gid * p.H + h) * tiles + mine;
-    const float* const behind = p.seg && !w.is_last ? p.seg + ((long long)gid * p.H + h) * tiles + mine : nullptr;
+    const float* const front = w.is_first ? nullptr : p.seg_front + ((long long)w.page * p.H + h) * tiles + mine;
+    const float* const behind = p.seg && !w.is_last ? p.seg + ((long long)w.page * p.H + h) * tiles + mine : nullptr;
     Gates gates;
     gates.open(p, w.base, w.first, h);
     const CarefulRows<IO> q(p.in[0], w.base, w.first, h, k0, p.Dk), k(p.in[1], w.base, w.first, h, k0, p.Dk), v(p.in[2], w.base, w.first, h, v0, p.Dv), gy(p.gy, w.base, w.first, h, v0, p.Dv);

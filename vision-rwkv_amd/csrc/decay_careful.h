@@ -116,11 +116,11 @@ __device__ __forceinline__ void careful_scan(CarefulLds<DX>& m, const Gates& gat
 }
 // A segment's own state, in its place (four waves).  It starts from nothing: the first token's decay is that of what is in front, and only the segment's.
 template <typename IO, int DX>
-__device__ __forceinline__ void careful_segment(CarefulTokens<DX>& m, const Call& p, const Role& r, const Place& w, int gid, int z, int h) {
+__device__ __forceinline__ void careful_segment(CarefulTokens<DX>& m, const Call& p, const Role& r, const Place& w, int z, int h) {
     Gates gates;
     gates.open(p, w.base, w.first, h);
     const CarefulRows<IO> b(r.b, w.base, w.first, h, 0, r.dx), c(r.c, w.base, w.first, h, z * TZ, r.dz);
-    float* const seg = r.seg + (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ);
+    float* const seg = r.seg + (((long long)w.page * p.H + h) * r.tiles + z) * (DX * TZ);
 #pragma unroll 1
     for (int i0 = 0, n; i0 < w.s1 - w.s0; i0 += n) {
         n = min(CAREFUL_TOKENS, w.s1 - w.s0 - i0);
@@ -173,7 +173,7 @@ __device__ __forceinline__ void careful_outputs(const Careful& careful, CarefulL
     Gates gates;
     gates.open(p, w.base, w.first, h);
     const CarefulRows<IO> q(r.a, w.base, w.first, h, 0, r.dx), k(r.b, w.base, w.first, h, 0, r.dx), v(r.c, w.base, w.first, h, z * TZ, r.dz);
-    const float* const seg = w.is_first ? nullptr : r.seg + (((long long)gid * p.H + h) * r.tiles + z) * (DX * TZ);
+    const float* const seg = w.is_first ? nullptr : r.seg + (((long long)w.page * p.H + h) * r.tiles + z) * (DX * TZ);
     careful_each<DX>(r.dx, [&](int row, int lane) {
         const int column = z * TZ + lane;
         m.st[row][lane] = seg ? seg[careful_place(row, lane)] : r.init && column < r.dz ? r.init[page + row * r.sx + column * r.sz] : 0.f;
