@@ -136,7 +136,7 @@ __device__ __forceinline__ void careful_segment(CarefulTokens<DX>& m, const Call
     }
 }
 
-// Whether a workgroup has work here, and where its kernel's arguments are, to be read again: kept in registers from the kernel's start they would spill in its chunks.
+// Whether a workgroup has work here, and where its kernel's arguments (one struct) are, to be read again: kept in registers from the kernel's start they would spill in its chunks.
 struct Careful {
     int wanted;
     unsigned args[2];
