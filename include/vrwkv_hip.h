@@ -38,10 +38,10 @@ const char* vrwkv_last_error(void);      /* thread-local, never NULL */
 
 /* Tuning / testing switches, process-wide (no counterpart in the reference).  Names: "biwkv_l", "biwkv_s",
  * "biwkv_grid", "biwkv_no_stage", "biwkv_no_resident", "biwkv_bwd_serial", "wkv6_fwd_scalar", "wkv6_bwd_scalar",
- * "wkv6_bwd_unfused" (no effect: the backward is one kernel), "wkv6_segments", "linear_tile", "wgrad_splits", "linear_mix"; 0 = default behaviour.  The initial
+ * "wkv6_bwd_unfused" (no effect: the backward is one kernel), "wkv6_segments", "linear_tile", "wgrad_splits", "linear_mix", "scan_segments"; 0 = default behaviour.  The initial
  * value of <name> is that of the environment variable VRWKV_<NAME> when the library first looks at any switch; the entry points never read the environment afterwards.
  * vrwkv_set_option rejects (VRWKV_INVALID_ARG) a value the plans would ignore: biwkv_l takes 0, 4, 8, 16, 25, 28 (tokens
- * per wave), biwkv_s 0 or 2..8 (waves per workgroup), biwkv_grid 0 or a positive workgroup count, wkv6_segments 0..64 (segments a sequence
+ * per wave), biwkv_s 0 or 2..8 (waves per workgroup), biwkv_grid 0 or a positive workgroup count, wkv6_segments and scan_segments 0..64 (segments a sequence
  * is cut into), linear_tile 0, 1, 2, 4, 8 (16 to 128 results on a side), 16 (256 channels wide), wgrad_splits 0 or a positive count of token ranges,
  * linear_mix 0, 1 (norm, shift and mixes inside the projections of a block's halves, VRWKV_UNSUPPORTED_SHAPE where the default would have them in front),
  * 2 (in front), the others 0 or 1. */
@@ -383,6 +383,96 @@ int vrwkv_decay_step(const vrwkv_decay_step_args* args, void* hip_stream);
 size_t vrwkv_copy_pages_workspace_bytes(int M);
 int vrwkv_copy_pages(void* pool, long long stride, int P, const void* source, long long source_stride, int source_P, long long page_bytes,
                      const void* from, int from64, const void* to, int to64, int M, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* ---- the selective state space scan, the short causal convolution in front of it, and the root-mean-square norm (no counterpart in the reference) ----
+ * Token tensors are rows of E channels side by side at any strides (in elements) of batch and token (token: less than 2^22), of one dtype; sequences as in
+ * vrwkv_decay_args: N rows of T tokens, or with offsets (N + 1, 32 or 64 bits, on the device, ascending from 0) N sequences packed in T rows, strides of batch not looked at;
+ * outputs and gradients of packed rows that belong to no sequence are zeros, what such rows hold does not matter.  Sums and states are fp32.
+ *
+ * h_t = exp(dt_t A) h_{t-1} + dt_t u_t B_t^T, y_t = (C_t h_t + D u_t) silu(z_t) for each of the E channels, with dt = delta + delta_bias, softplus of that where `softplus`.
+ * A: (E, S) contiguous fp32, S 1 to 64; B, C: rows of G groups of S states side by side, strides of batch, token and group; channel e reads group e / (E / G).
+ * D, delta_bias: (E) of D_dtype, bias_dtype, or NULL; z or NULL.  state: (N, E, S) contiguous fp32, or NULL: zeros; last: the states behind the last tokens, or NULL.
+ * y (batch, T, E) of dtype, contiguous.  kept: vrwkv_scan_kept_bytes of memory, 16-byte aligned, that the forward fills with the states in front of every sixteenth
+ * token and the backward reads, or NULL in a forward without a backward. */
+typedef struct vrwkv_scan_args {
+    const void *u, *delta, *B, *C, *D, *z, *delta_bias, *offsets;
+    const float *A, *state;
+    void* y;
+    float *last, *kept;
+    const void* gy;                        /* backward: gradient of y, of dtype, at gy_stride */
+    const float* glast;                    /* ... of last, or NULL: zeros */
+    void *du, *ddelta, *dz, *dB, *dC;      /* contiguous: (batch, T, E), (batch, T, G, S) of dtype; all of them are written (dz with z) */
+    float *dA, *dstate;                    /* (E, S); (N, E, S) or NULL */
+    void *dD, *dbias;                      /* (E) of D_dtype, bias_dtype, or NULL */
+    long long u_stride[2], delta_stride[2], z_stride[2], gy_stride[2], B_stride[3], C_stride[3];
+    int N, T, E, S, G, dtype, D_dtype, bias_dtype, softplus, offsets64;
+    void* workspace;                       /* 16-byte aligned; its size goes by the sizes above and by whether there are offsets */
+    size_t workspace_bytes;
+} vrwkv_scan_args;
+size_t vrwkv_scan_kept_bytes(const vrwkv_scan_args* args);
+size_t vrwkv_scan_fwd_workspace_bytes(const vrwkv_scan_args* args);
+int vrwkv_scan_fwd(const vrwkv_scan_args* args, void* hip_stream);
+size_t vrwkv_scan_bwd_workspace_bytes(const vrwkv_scan_args* args);
+int vrwkv_scan_bwd(const vrwkv_scan_args* args, void* hip_stream);
+
+/* One more token for each of N rows, whose states are pages slots[n] of a pool (P pages of E x S contiguous fp32 numbers, page_stride apart), as in vrwkv_decay_step:
+ * updated in place, rows of one page in their order, slot -1 zeros, any other slot outside the pool NaN. */
+typedef struct vrwkv_scan_step_args {
+    const void *u, *delta, *B, *C, *D, *z, *delta_bias, *slots;
+    const float* A;
+    float* pool;
+    void* y;                               /* (N, E) of dtype, contiguous */
+    long long u_stride, delta_stride, z_stride, B_stride[2], C_stride[2], page_stride;
+    int N, P, E, S, G, dtype, D_dtype, bias_dtype, softplus, slots64;
+} vrwkv_scan_step_args;
+int vrwkv_scan_step(const vrwkv_scan_step_args* args, void* hip_stream);
+
+/* y_t = sum_j weight[:, j] x_{t - (K - 1) + j} + bias, silu of that where `silu`, for each of the E channels; weight (E, K) contiguous, K 2 to 8, and bias (E) or NULL of param_dtype.
+ * state: the K - 1 tokens in front of the first, (N, K - 1, E) contiguous of dtype, or NULL: zeros; last: those in front of a next token, of the same shape, or NULL.  y (batch, T, E). */
+typedef struct vrwkv_conv_args {
+    const void *x, *weight, *bias, *state, *offsets;
+    void *y, *last;
+    const void *gy, *glast;                /* backward: gradients of y (at gy_stride) and last (contiguous, or NULL: zeros), of dtype */
+    void *dx, *dweight, *dbias, *dstate;   /* (batch, T, E); (E, K) and (E) of param_dtype; (N, K - 1, E); dbias and dstate or NULL */
+    long long x_stride[2], gy_stride[2];
+    int N, T, E, K, dtype, param_dtype, silu, offsets64;
+    void* workspace;                       /* 16-byte aligned; the backward's */
+    size_t workspace_bytes;
+} vrwkv_conv_args;
+int vrwkv_conv_fwd(const vrwkv_conv_args* args, void* hip_stream);
+size_t vrwkv_conv_bwd_workspace_bytes(const vrwkv_conv_args* args);
+int vrwkv_conv_bwd(const vrwkv_conv_args* args, void* hip_stream);
+
+/* One more token for each of N rows, whose last K - 1 tokens are pages slots[n] of a pool (P pages of (K - 1) x E contiguous numbers of dtype, page_stride apart), as in vrwkv_scan_step. */
+typedef struct vrwkv_conv_step_args {
+    const void *x, *weight, *bias, *slots;
+    void *pool, *y;                        /* y (N, E) of dtype, contiguous */
+    long long x_stride, page_stride;
+    int N, P, E, K, dtype, param_dtype, silu, slots64;
+} vrwkv_conv_step_args;
+int vrwkv_conv_step(const vrwkv_conv_step_args* args, void* hip_stream);
+
+/* r = x + residual, rounded to residual_dtype (without residual: x), y = r / sqrt(mean(r^2) + eps) weight over rows of C channels, the mean in fp32.  x, y of dtype,
+ * residual and sum of residual_dtype, dtype or fp32; weight (C) of weight_dtype; rows contiguous, x_stride and residual_stride apart.  sum: r, or NULL.
+ * out_kind: VRWKV_Y_SAME: y of dtype; VRWKV_Y_E4M3, VRWKV_Y_INT8: y / scale rounded to nearest even, 8 bits each, with scale (rows) fp32 = max(max |y| / top, 2^-126), top 448 or
+ * 127; a row whose maximum is NaN has a scale of NaN, e4m3 values of NaN and int8 values of 0.
+ * Backward: r is `sum` as the forward returned it, gsum (of residual_dtype, or NULL) its gradient; dx of dtype, dresidual of residual_dtype or NULL, dweight (C) of weight_dtype or NULL. */
+enum { VRWKV_Y_SAME = 0, VRWKV_Y_E4M3 = 1, VRWKV_Y_INT8 = 2 };
+typedef struct vrwkv_rmsnorm_args {
+    const void *x, *residual, *weight;
+    void *y, *sum;
+    float* scale;
+    const void *gy, *gsum;
+    void *dx, *dresidual, *dweight;
+    long long rows, x_stride, residual_stride, gy_stride, gsum_stride;
+    int C, dtype, residual_dtype, weight_dtype, out_kind;
+    float eps;
+    void* workspace;
+    size_t workspace_bytes;
+} vrwkv_rmsnorm_args;
+int vrwkv_rmsnorm(const vrwkv_rmsnorm_args* args, void* hip_stream);
+size_t vrwkv_rmsnorm_bwd_workspace_bytes(const vrwkv_rmsnorm_args* args);
+int vrwkv_rmsnorm_bwd(const vrwkv_rmsnorm_args* args, void* hip_stream);
 
 #ifdef __cplusplus
 }

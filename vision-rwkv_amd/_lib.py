@@ -64,6 +64,47 @@ class DecayStepArgs(ctypes.Structure):
                 + [("page_stride", ctypes.c_longlong)] + [(n, ctypes.c_int) for n in INTS] + [("scale", ctypes.c_float)])
 
 
+def _fields(pointers=(), longs=(), ints=(), tail=()):
+    """Fields of an argument structure: pointers, [(long longs, how many)], ints, and what stands behind them."""
+    c = ctypes
+    return ([(n, c.c_void_p) for n in pointers] + [(n, c.c_longlong * k if k > 1 else c.c_longlong) for n, k in longs] + [(n, c.c_int) for n in ints] + list(tail))
+
+
+_WORKSPACE = [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class ScanArgs(ctypes.Structure):
+    """vrwkv_scan_args of include/vrwkv_hip.h."""
+    _fields_ = _fields(("u", "delta", "B", "C", "D", "z", "delta_bias", "offsets", "A", "state", "y", "last", "kept", "gy", "glast", "du", "ddelta", "dz", "dB", "dC", "dA", "dstate", "dD", "dbias"),
+                       (("u_stride", 2), ("delta_stride", 2), ("z_stride", 2), ("gy_stride", 2), ("B_stride", 3), ("C_stride", 3)),
+                       ("N", "T", "E", "S", "G", "dtype", "D_dtype", "bias_dtype", "softplus", "offsets64"), tail=_WORKSPACE)
+
+
+class ScanStepArgs(ctypes.Structure):
+    """vrwkv_scan_step_args of include/vrwkv_hip.h."""
+    _fields_ = _fields(("u", "delta", "B", "C", "D", "z", "delta_bias", "slots", "A", "pool", "y"),
+                       (("u_stride", 1), ("delta_stride", 1), ("z_stride", 1), ("B_stride", 2), ("C_stride", 2), ("page_stride", 1)),
+                       ("N", "P", "E", "S", "G", "dtype", "D_dtype", "bias_dtype", "softplus", "slots64"))
+
+
+class ConvArgs(ctypes.Structure):
+    """vrwkv_conv_args of include/vrwkv_hip.h."""
+    _fields_ = _fields(("x", "weight", "bias", "state", "offsets", "y", "last", "gy", "glast", "dx", "dweight", "dbias", "dstate"), (("x_stride", 2), ("gy_stride", 2)),
+                       ("N", "T", "E", "K", "dtype", "param_dtype", "silu", "offsets64"), tail=_WORKSPACE)
+
+
+class ConvStepArgs(ctypes.Structure):
+    """vrwkv_conv_step_args of include/vrwkv_hip.h."""
+    _fields_ = _fields(("x", "weight", "bias", "slots", "pool", "y"), (("x_stride", 1), ("page_stride", 1)), ("N", "P", "E", "K", "dtype", "param_dtype", "silu", "slots64"))
+
+
+class RmsnormArgs(ctypes.Structure):
+    """vrwkv_rmsnorm_args of include/vrwkv_hip.h."""
+    _fields_ = _fields(("x", "residual", "weight", "y", "sum", "scale", "gy", "gsum", "dx", "dresidual", "dweight"),
+                       (("rows", 1), ("x_stride", 1), ("residual_stride", 1), ("gy_stride", 1), ("gsum_stride", 1)), ("C", "dtype", "residual_dtype", "weight_dtype", "out_kind"),
+                       tail=[("eps", ctypes.c_float)] + _WORKSPACE)
+
+
 class VrwkvError(RuntimeError):
     """Non-zero status from the C ABI (mirrors the RuntimeError TORCH_CHECK raises at
     classification/mmcls_custom/models/backbones/cuda_new/bi_wkv.cpp:6-8)."""
@@ -238,6 +279,14 @@ def _declare(lib):
     lib.vrwkv_copy_pages_workspace_bytes.restype = sz
     lib.vrwkv_copy_pages.argtypes = [vp, ll, i, vp, ll, i, ll, vp, i, vp, i, i, vp, sz, vp]
     lib.vrwkv_copy_pages.restype = i
+    for name, args, size in (("scan_fwd", ScanArgs, True), ("scan_bwd", ScanArgs, True), ("scan_step", ScanStepArgs, False), ("conv_fwd", ConvArgs, False), ("conv_bwd", ConvArgs, True),
+                             ("conv_step", ConvStepArgs, False), ("rmsnorm", RmsnormArgs, False), ("rmsnorm_bwd", RmsnormArgs, True)):
+        call = getattr(lib, f"vrwkv_{name}")
+        call.argtypes, call.restype = [c.POINTER(args), vp], i
+        if size:
+            call = getattr(lib, f"vrwkv_{name}_workspace_bytes")
+            call.argtypes, call.restype = [c.POINTER(args)], sz
+    lib.vrwkv_scan_kept_bytes.argtypes, lib.vrwkv_scan_kept_bytes.restype = [c.POINTER(ScanArgs)], sz
     for name in ("rowfuse_bwd", "qshift_mix_bwd", "groupnorm_gate_bwd", "biwkv_bwd"):
         like = getattr(lib, f"vrwkv_{name}_like")
         like.argtypes, like.restype = getattr(lib, f"vrwkv_{name}").argtypes, i

@@ -22,7 +22,7 @@ void set_error(const char* fmt, ...) {
 namespace {
 const char* const kOptionNames[N_OPTIONS] = {
     "biwkv_l", "biwkv_s", "biwkv_grid", "biwkv_no_stage", "biwkv_no_resident", "biwkv_bwd_serial",
-    "wkv6_fwd_scalar", "wkv6_bwd_scalar", "wkv6_bwd_unfused", "wkv6_segments", "linear_tile", "wgrad_splits", "linear_mix",
+    "wkv6_fwd_scalar", "wkv6_bwd_scalar", "wkv6_bwd_unfused", "wkv6_segments", "linear_tile", "wgrad_splits", "linear_mix", "scan_segments",
 };
 std::atomic<int> g_options[N_OPTIONS];
 std::once_flag g_options_once;
@@ -80,7 +80,7 @@ extern "C" int vrwkv_set_option(const char* name, int value) {
     if (i == vrwkv::OPT_BIWKV_L) ok = value == 0 || value == 4 || value == 8 || value == 16 || value == 25 || value == 28;
     if (i == vrwkv::OPT_BIWKV_S) ok = value == 0 || (value >= 2 && value <= 8);
     if (i == vrwkv::OPT_BIWKV_GRID) ok = value >= 0;
-    if (i == vrwkv::OPT_WKV6_SEGMENTS) ok = value >= 0 && value <= 64;
+    if (i == vrwkv::OPT_WKV6_SEGMENTS || i == vrwkv::OPT_SCAN_SEGMENTS) ok = value >= 0 && value <= 64;
     if (i == vrwkv::OPT_LINEAR_TILE) ok = value == 0 || value == 1 || value == 2 || value == 4 || value == 8 || value == 16;
     if (i == vrwkv::OPT_WGRAD_SPLITS) ok = value >= 0;
     if (i == vrwkv::OPT_LINEAR_MIX) ok = value >= 0 && value <= 2;

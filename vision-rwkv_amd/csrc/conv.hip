@@ -1,0 +1,178 @@
+// The short causal convolution (conv.h): whole sequences, and one more token of each of N.
+#include "conv.h"
+#include "pages.h"
+
+namespace vrwkv {
+namespace conv {
+namespace {
+
+// What is behind the last token of each sequence: element i of (N, K - 1, E).
+template <typename IO>
+__device__ __forceinline__ void last_states(const Params& p, long long first, long long step) {
+    const long long all = (long long)p.N * (p.K - 1) * p.E;
+    for (long long i = first; i < all; i += step) {
+        const int c = (int)(i % p.E), k = (int)(i / p.E % (p.K - 1)), n = (int)(i / p.E / (p.K - 1));
+        const int begin = p.seq.offsets ? p.seq.of_lane(n) : 0, end = p.seq.offsets ? max(begin, p.seq.of_lane(n + 1)) : p.T, t = end - (p.K - 1) + k;
+        IO v = from_f32<IO>(0.f);
+        if (t >= begin) v = static_cast<const IO*>(p.x)[(p.seq.offsets ? 0 : n * p.x_b) + t * p.x_t + c];
+        else if (p.state) v = static_cast<const IO*>(p.state)[((long long)n * (p.K - 1) + t - begin + p.K - 1) * p.E + c];
+        static_cast<IO*>(p.last)[i] = v;
+    }
+}
+
+// Waves of a workgroup take runs next to each other.  The last `extra` workgroups of x write the states.
+template <typename IO, int VEC, int KT>
+__global__ __launch_bounds__(THREADS) void forward_kernel(const Params p, int run_blocks) {
+    const int lane = threadIdx.x & 63;
+    if ((int)blockIdx.x >= run_blocks) {
+        if (blockIdx.y == 0) last_states<IO>(p, (blockIdx.x - run_blocks) * THREADS + threadIdx.x, (long long)(gridDim.x - run_blocks) * THREADS);
+        return;
+    }
+    const int number = blockIdx.x * (THREADS / WAVE) + (threadIdx.x >> 6);
+    if (number >= p.rows * p.runs) return;
+    const Lane<IO, VEC, KT> my(p, blockIdx.y * WAVE + lane);
+    Run r(p, __builtin_amdgcn_readfirstlane(number), lane);
+    Packed<IO, VEC> ahead[AHEAD];
+    const auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) ahead[i] = my.packed(p.x, r.b * p.x_b + min(t + i, r.t1 - 1) * p.x_t);
+    };
+    fetch(r.t0);
+    Wide<VEC> x[KT];                                       // x[j]: token t - (KT - 1) + j
+#pragma unroll
+    for (int j = 0; j < KT - 1; ++j) x[j + 1] = r.w.begin < r.t0 && my.used(j) ? my.token(r.w.n, r.b, r.t0 - (KT - 1) + j, r.w.begin) : Wide<VEC>{};
+    for (int t = r.t0; t < r.t1; t += AHEAD) {
+        Packed<IO, VEC> now[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) now[i] = ahead[i];
+        if (t + AHEAD < r.t1) fetch(t + AHEAD);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (t + i >= r.t1) break;
+            const long long out = ((long long)r.b * p.T + t + i) * p.E;
+            if (t + i < r.from || t + i >= r.to) {
+                my.store(p.y, out, Wide<VEC>{});
+                continue;
+            }
+            if (t + i == r.w.begin) {
+#pragma unroll
+                for (int j = 0; j < KT - 1; ++j) x[j + 1] = my.used(j) ? my.token(r.w.n, r.b, r.w.begin - (KT - 1) + j, r.w.begin) : Wide<VEC>{};
+            }
+#pragma unroll
+            for (int j = 0; j < KT - 1; ++j) x[j] = x[j + 1];
+            widen_packed<IO, VEC>(now[i], x[KT - 1].v);
+            Wide<VEC> y = my.pre(x);
+            if (p.silu)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) y.v[k] = silu_of(y.v[k]);
+            my.store(p.y, out, y);
+            if (t + i == r.w.end - 1) r.w.next(p.seq);
+        }
+    }
+}
+
+constexpr int GRID_Y = 32768;
+struct StepParams {
+    Params f;
+    Slots slots;
+    void* pool;
+    long long page, x_n;
+};
+template <typename IO, int VEC, int KT>
+__global__ __launch_bounds__(THREADS) void step_kernel(const StepParams sp) {
+    const Params& p = sp.f;
+    const int n0 = blockIdx.y + GRID_Y * blockIdx.z;
+    if (n0 >= sp.slots.rows) return;
+    const long long slot = sp.slots.at(n0);
+    const bool known = sp.slots.has(slot);
+    IO* const page = static_cast<IO*>(sp.pool) + (known ? slot : 0) * sp.page;
+    const Lane<IO, VEC, KT> my(p, blockIdx.x * THREADS + threadIdx.x);
+    Wide<VEC> x[KT];
+    Wide<VEC> now = my.row(p.x, n0 * sp.x_n);
+#pragma unroll
+    for (int j = 0; j < KT - 1; ++j) x[j + 1] = known && my.used(j) && my.there ? my.row(page, (long long)(j - (KT - p.K)) * p.E) : Wide<VEC>{};
+    int next;
+    if (!sp.slots.first_of_page(n0, slot, next)) return;
+    for (int n = n0;;) {
+#pragma unroll
+        for (int j = 0; j < KT - 1; ++j) x[j] = x[j + 1];
+        x[KT - 1] = now;
+        Wide<VEC> y = my.pre(x);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            if (p.silu) y.v[k] = silu_of(y.v[k]);
+            if (!known) y.v[k] = slot == -1 ? 0.f : __builtin_nanf("");
+        }
+        my.store(p.y, (long long)n * p.E, y);
+        if (next >= sp.slots.rows) break;
+        n = next;
+        next = sp.slots.behind(n, slot);
+        now = my.row(p.x, n * sp.x_n);
+    }
+    if (!known) return;
+#pragma unroll
+    for (int j = 1; j < KT; ++j)
+        if (my.used(j - 1)) my.store(page, (long long)(j - 1 - (KT - p.K)) * p.E, x[j]);
+}
+
+}  // namespace
+}  // namespace conv
+}  // namespace vrwkv
+
+using namespace vrwkv;
+using namespace vrwkv::conv;
+
+extern "C" int vrwkv_conv_fwd(const vrwkv_conv_args* args, void* hip_stream) {
+    const char* who = "vrwkv_conv_fwd";
+    if (const int rc = check(who, args, false)) return rc;
+    const vrwkv_conv_args& a = *args;
+    const long long strides[] = {a.offsets ? 0 : a.x_stride[0], a.x_stride[1]};
+    const int vec = vec_of(a.dtype, a.E, 16, (size_t)a.x | (size_t)a.y | (size_t)a.state, strides, 2);
+    const Plan pl = plan_of(a, vec);
+    const Params p = params_of(a, pl);
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const int blocks = (int)(((long long)pl.rows * pl.runs + THREADS / WAVE - 1) / (THREADS / WAVE));
+    const int extra = a.last ? (int)std::min<long long>(4LL * device_cus(), ((long long)a.N * (a.K - 1) * a.E + THREADS - 1) / THREADS) : 0;
+    return with_types<8>(a.dtype, vec, [&](auto io, auto v) {
+        using IO = decltype(io);
+        constexpr int VEC = decltype(v)::value;
+        return with_taps(a.K, [&](auto k) {
+            constexpr int KT = decltype(k)::value;
+            hipLaunchKernelGGL((forward_kernel<IO, VEC, KT>), dim3(blocks + extra, pl.waves), dim3(THREADS), 0, st, p, blocks);
+            return check_launch(who);
+        });
+    });
+}
+
+extern "C" int vrwkv_conv_step(const vrwkv_conv_step_args* args, void* hip_stream) {
+    const char* who = "vrwkv_conv_step";
+    if (!args || !args->x || !args->weight || !args->pool || !args->y) { set_error("%s: null pointer", who); return VRWKV_INVALID_ARG; }
+    const vrwkv_conv_step_args& a = *args;
+    if (a.N <= 0 || a.P <= 0 || a.E <= 0) { set_error("%s: N, P and E must be positive", who); return VRWKV_INVALID_ARG; }
+    if (!typed(a.dtype) || !typed(a.param_dtype)) { set_error("%s: dtype must be fp32, bf16 or fp16", who); return VRWKV_UNSUPPORTED_DTYPE; }
+    if (a.K < 2 || a.K > 8 || a.E > 1 << 22) { set_error("%s: 2 to 8 taps (%d), and at most 2^22 channels", who, a.K); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (!a.slots && a.N > a.P) { set_error("%s: %d rows without slots, and %d pages", who, a.N, a.P); return VRWKV_INVALID_ARG; }
+    if (a.page_stride < (long long)(a.K - 1) * a.E) { set_error("%s: pages overlap", who); return VRWKV_INVALID_ARG; }
+    if (!aligned(a.x, a.dtype) || !aligned(a.y, a.dtype) || !aligned(a.pool, a.dtype) || !aligned(a.weight, a.param_dtype) || !aligned(a.bias, a.param_dtype) ||
+        (a.slots && ((size_t)a.slots & (a.slots64 ? 7 : 3)))) {
+        set_error("%s: a tensor is not aligned to its elements", who);
+        return VRWKV_INVALID_ARG;
+    }
+    StepParams sp{};
+    sp.f.x = a.x, sp.f.y = a.y, sp.f.w = ParamVec(a.weight, a.param_dtype, 1.f), sp.f.bias = ParamVec(a.bias, a.param_dtype, 1.f);
+    sp.f.E = a.E, sp.f.K = a.K, sp.f.silu = a.silu;
+    sp.slots = Slots{a.slots, a.slots64, a.N, a.P}, sp.pool = a.pool, sp.page = a.page_stride, sp.x_n = a.x_stride;
+    const long long strides[] = {a.x_stride, a.page_stride};
+    const int vec = vec_of(a.dtype, a.E, 16, (size_t)a.x | (size_t)a.y | (size_t)a.pool, strides, 2);
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const dim3 grid((a.E / vec + THREADS - 1) / THREADS, std::min(a.N, GRID_Y), (a.N + GRID_Y - 1) / GRID_Y);
+    return with_types<8>(a.dtype, vec, [&](auto io, auto v) {
+        using IO = decltype(io);
+        constexpr int VEC = decltype(v)::value;
+        return with_taps(a.K, [&](auto k) {
+            constexpr int KT = decltype(k)::value;
+            hipLaunchKernelGGL((step_kernel<IO, VEC, KT>), grid, dim3(THREADS), 0, st, sp);
+            return check_launch(who);
+        });
+    });
+}

@@ -1,0 +1,413 @@
+// Gradients of the selective state space scan (gfx950).  With R_t the gradient of h_t, g_t = gy_t silu(z_t) and e_t = exp(dt_t A):
+//
+//     R_t = g_t C_t + e_{t+1} R_{t+1}        dC_t = sum_channels g_t h_t        dB_t = sum_channels R_t dt_t u_t        dA = sum_t dt_t e_t R_t h_{t-1}
+//     ddt_t = sum_states (e_t R_t h_{t-1} A + R_t u_t B_t)        du_t = dt_t sum_states R_t B_t + D g_t        dz_t = gy_t (C_t h_t + D u_t) silu'(z_t)
+//
+// Sixteen tokens at a time, the last first: their states again from the one that the forward has kept in front of them, in registers, then back along them.  P lanes hold one channel,
+// four states each, as in the forward.  dB and dC add up channels, which lie in other lanes: the sums of two tokens go through the wave in halves
+// (lane swaps and additions, two instructions for a sum of 64 / P lanes), then through LDS over the waves, and over workgroups by the launch that ends the pass.
+#pragma once
+#include "scan.h"
+
+namespace vrwkv {
+namespace scan {
+
+struct BackParams {
+    Params f;
+    const void* gy;
+    const float* glast;
+    void *du, *dd, *dz;
+    float *dstate, *seg_r;                                 // seg_r: like seg_h, the gradient that a segment hands to the token in front of it
+    float *part_bc, *part_A, *part_D, *part_bias;          // (blocks, tokens, G, 2, 4 P); (parts, E, 4 P); (parts, E)
+    long long gy_b, gy_t;
+};
+
+// Sums over the lanes of a wave that differ above the channel's P: v[i] of the 64 / P channels to the lane of channel i.
+template <int P, int COUNT, int BIT = 32>
+__device__ __forceinline__ void sum_over_channels(float (&v)[COUNT], int lane) {
+    if constexpr (BIT >= P) {
+        constexpr int HALF = BIT / P;
+        static_assert(COUNT == 64 / P, "one sum for each channel of the wave");
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+            float a = v[i], b = v[i + HALF];
+            if constexpr (BIT >= 16) {
+                const auto x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
+                // (the elements are copied first: a bit cast of one as it stands takes the vector's first)
+                const auto r = [&] {
+                    if constexpr (BIT == 32) return __builtin_amdgcn_permlane32_swap(x, y, false, false);
+                    else return __builtin_amdgcn_permlane16_swap(x, y, false, false);
+                }();
+                const unsigned low = r[0], high = r[1];
+                v[i] = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
+            } else if constexpr (BIT == 8) {
+                a += dpp<0x128>(a);                        // row_ror:8
+                b += dpp<0x128>(b);
+                v[i] = lane & 8 ? b : a;
+            } else if constexpr (BIT == 4) {
+                a += dpp<0x104>(a);                        // row_shl:4: the lane four above, for the lower of the two
+                b += dpp<0x114>(b);                        // row_shr:4
+                v[i] = lane & 4 ? b : a;
+            } else {
+                a += across<BIT>(a);
+                b += across<BIT>(b);
+                v[i] = lane & BIT ? b : a;
+            }
+        }
+        sum_over_channels<P, COUNT, BIT / 2>(v, lane);
+    }
+}
+
+// The gradient that each segment behind the first hands on, from zeros behind it (or from its sequence's end), and its sum of step sizes.
+template <typename IO, int P, bool FULL>
+__global__ __launch_bounds__(THREADS) void back_segments_kernel(const BackParams bp) {
+    const Params& p = bp.f;
+    constexpr int OWN = BATCH / P;
+    __shared__ __attribute__((aligned(16))) float bc[2][BATCH * 2 * 4 * P];
+    const Place<P> at(p.E, p.G, p.blocks);
+    const int s = blockIdx.y + 1, b = blockIdx.z, r0 = s * p.L, r1 = min(p.T, r0 + p.L), e = at.e;
+    int from, to;
+    p.seq.inside(r0, r1, from, to);
+    Walk w;
+    w.find(p.seq, b, max(from, to - 1), at.lane);
+    float a2[4], R[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a2[k] = !FULL && 4 * at.p + k >= p.S ? 0.f : p.A[(long long)e * p.S + 4 * at.p + k] * LOG2E;
+    const float bias = p.bias.p ? p.bias.value(p.bias.fetch(e)) : 0.f;
+    Rows<IO, P> raw, ahead;
+    const auto fetch = [&](Rows<IO, P>& x, int row) {
+        x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row + at.p, r1, e);
+        x.fetch(x.g, bp.gy, b * bp.gy_b, bp.gy_t, row + at.p, r1, e);
+        if (p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row + at.p, r1, e);
+    };
+    Stage<IO, P, 2> stage;
+    const int last = r0 + (r1 - 1 - r0) / BATCH * BATCH;
+    fetch(raw, last);
+    stage.fetch(p, b, at.g, last, from, to);
+    stage.put(bc[0]);
+    lds_barrier();
+    float total = 0.f;
+    int buf = 0;
+    for (int row = last; row >= r0; row -= BATCH, buf ^= 1) {
+        const bool more = row > r0;
+        if (more) {
+            fetch(ahead, row - BATCH);
+            stage.fetch(p, b, at.g, row - BATCH, from, to);
+        }
+        float dt[OWN], g[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            const float d = to_f32(raw.d[i]) + bias;
+            dt[i] = p.softplus ? softplus(d) : d;
+            g[i] = to_f32(raw.g[i]);
+            if (p.z) {
+                const float z = to_f32(raw.z[i]);
+                g[i] *= z * sigmoid(z);
+            }
+            total += row + at.p + i * P < r1 ? dt[i] : 0.f;
+        }
+        const auto token = [&](auto j_) {
+            constexpr int j = BATCH - 1 - decltype(j_)::value;
+            const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(g[j / P]);
+            const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * 8 * P + 4 * P + 4 * at.p]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) R[k] = fast_exp2(d * a2[k]) * fmaf(Ct[k], v, R[k]);
+        };
+        if (row >= from && row + BATCH <= to && w.within(row, BATCH)) each(std::make_integer_sequence<int, BATCH>(), token);
+        else
+            each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
+                constexpr int j = BATCH - 1 - decltype(j_)::value;
+                if (row + j < from || row + j >= to) return;
+                if (row + j == w.end - 1) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) R[k] = bp.glast && (FULL || 4 * at.p + k < p.S) ? bp.glast[((long long)w.n * p.E + e) * p.S + 4 * at.p + k] : 0.f;
+                }
+                token(j_);
+                if (row + j == w.begin) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) R[k] = 0.f;
+                    w.previous(p.seq);
+                }
+            });
+        if (more) {
+            stage.put(bc[buf ^ 1]);
+            raw = ahead;
+            lds_barrier();
+        }
+    }
+    if (!at.there) return;
+    const long long place = (long long)b * p.nseg + s;
+    *reinterpret_cast<f32x4*>(bp.seg_r + (place * p.E + e) * 4 * P + 4 * at.p) = f32x4{R[0], R[1], R[2], R[3]};
+    float v[P];
+#pragma unroll
+    for (int q = 0; q < P; ++q) v[q] = total;
+    sum_to_lanes<P, P>(v, at.p);
+    if (at.p == 0) p.seg_dt[place * p.E + e] = v[0];
+}
+
+template <typename IO, int P, bool FULL>
+__global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
+    const Params& p = bp.f;
+    constexpr int OWN = BATCH / P, COUNT = 64 / P, ROW = 8 * P, SUMS = BATCH * ROW, BUFS = P == 16 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) float bc[2][SUMS];
+    __shared__ float red[BUFS][THREADS / WAVE][SUMS];
+    const Place<P> at(p.E, p.G, p.blocks);
+    const int s = blockIdx.y, r0 = s * p.L, r1 = min(p.T, r0 + p.L), e = at.e, wave = threadIdx.x >> 6;
+    const long long part = (long long)blockIdx.z * p.nseg + s;
+    int from, to;
+    p.seq.inside(r0, r1, from, to);
+    float a2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, dbias = 0.f;
+    bool pad[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        pad[k] = !FULL && 4 * at.p + k >= p.S;
+        a2[k] = pad[k] ? 0.f : p.A[(long long)e * p.S + 4 * at.p + k] * LOG2E;
+    }
+    const float bias = p.bias.p ? p.bias.value(p.bias.fetch(e)) : 0.f, skip = p.D.p ? p.D.value(p.D.fetch(e)) : 0.f;
+    const auto state_of = [&](const float* t, int n, float (&h)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = t && !pad[k] ? t[((long long)n * p.E + e) * p.S + 4 * at.p + k] : 0.f;
+    };
+    const auto first_gradient = [&](int n, const float (&h)[4]) {
+        if (!bp.dstate || !at.there) return;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (!pad[k]) bp.dstate[((long long)n * p.E + e) * p.S + 4 * at.p + k] = h[k];
+    };
+    const int last = r0 + (r1 - 1 - r0) / BATCH * BATCH, chunks = (p.T + BATCH - 1) / BATCH;
+    // where a lane leaves the sum that it is left with: of token lane / P / 8 of a group (all of one where P is 16), B's or C's, state 4 p + lane / P % 4
+    const int sum = at.lane / P, leave = P == 16 ? 4 * at.p + sum : sum / 8 * ROW + sum / 4 % 2 * 4 * P + 4 * at.p + sum % 4;
+
+    for (int b = blockIdx.z; b < p.rows; b += gridDim.z) {
+        if (b != (int)blockIdx.z) lds_barrier();           // (the last row's sums are read)
+        Walk w;
+        w.find(p.seq, b, max(from, to - 1), at.lane);
+        float R[4] = {0.f, 0.f, 0.f, 0.f};
+        if (w.end > r1 && w.begin < r1) {                  // on from the segment that the sequence ends in
+            int k = (w.end - 1) / p.L;
+            const float* at_r = bp.seg_r + ((long long)b * p.nseg * p.E + e) * 4 * P + 4 * at.p;
+            const float* at_dt = p.seg_dt + (long long)b * p.nseg * p.E + e;
+            const f32x4 x0 = *reinterpret_cast<const f32x4*>(at_r + (long long)k * p.E * 4 * P);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) R[i] = x0[i];
+#pragma unroll 4
+            for (--k; k > s; --k) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(at_r + (long long)k * p.E * 4 * P);
+                const float dt = at_dt[(long long)k * p.E];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) R[i] = decayed(R[i], dt, a2[i]) + x[i];
+            }
+        }
+        Rows<IO, P> raw, ahead;
+        f32x4 kept, kept_ahead;
+        const auto fetch = [&](Rows<IO, P>& x, f32x4& h, int row) {
+            x.fetch(x.u, p.u, b * p.u_b, p.u_t, row + at.p, r1, e);
+            x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row + at.p, r1, e);
+            x.fetch(x.g, bp.gy, b * bp.gy_b, bp.gy_t, row + at.p, r1, e);
+            if (p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row + at.p, r1, e);
+            h = *reinterpret_cast<const f32x4*>(p.kept + (((long long)b * chunks + row / BATCH) * p.E + e) * 4 * P + 4 * at.p);
+        };
+        Stage<IO, P, 2> stage;
+        fetch(raw, kept, last);
+        stage.fetch(p, b, at.g, last, from, to);
+        stage.put(bc[0]);
+        lds_barrier();
+        int buf = 0;
+        for (int row = last; row >= r0; row -= BATCH, buf ^= 1) {
+            const bool more = row > r0;
+            if (more) {
+                fetch(ahead, kept_ahead, row - BATCH);
+                stage.fetch(p, b, at.g, row - BATCH, from, to);
+            }
+            float dt[OWN], x[OWN], g[OWN];
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                const float d = to_f32(raw.d[i]) + bias;
+                dt[i] = p.softplus ? softplus(d) : d;
+                x[i] = dt[i] * to_f32(raw.u[i]);
+                g[i] = to_f32(raw.g[i]);
+                if (p.z) {
+                    const float z = to_f32(raw.z[i]);
+                    g[i] *= z * sigmoid(z);
+                }
+            }
+            const bool clean = row >= from && row + BATCH <= to && w.within(row, BATCH);
+            float hs[BATCH + 1][4], y[BATCH];              // hs[j]: the state in front of token j, but where a sequence begins there
+#pragma unroll
+            for (int k = 0; k < 4; ++k) hs[0][k] = kept[k];
+            const auto along = [&](auto j_, const float (&h)[4]) {
+                constexpr int j = decltype(j_)::value;
+                const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]);
+                const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * P + 4 * at.p]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    hs[j + 1][k] = fmaf(fast_exp2(d * a2[k]), h[k], v * Bt[k]);
+                    if (!FULL && pad[k]) hs[j + 1][k] = 0.f;
+                }
+                y[j] = fmaf(Ct[3], hs[j + 1][3], fmaf(Ct[2], hs[j + 1][2], fmaf(Ct[1], hs[j + 1][1], Ct[0] * hs[j + 1][0])));
+            };
+            if (clean) each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) { along(j_, hs[decltype(j_)::value]); });
+            else {
+                Walk f;
+                f.find(p.seq, b, max(row, from), at.lane);
+                each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
+                    constexpr int j = decltype(j_)::value;
+                    y[j] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) hs[j + 1][k] = hs[j][k];
+                    if (row + j < from || row + j >= to) return;
+                    float h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h[k] = hs[j][k];
+                    if (row + j == f.begin) state_of(p.state, f.n, h);
+                    along(j_, h);
+                    if (row + j == f.end - 1) f.next(p.seq);
+                });
+            }
+            if (p.z) {
+                sum_to_lanes<P, BATCH>(y, at.p);
+                IO* out = static_cast<IO*>(bp.dz) + ((long long)b * p.T + row + at.p) * p.E + e;
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) {
+                    const float z = to_f32(raw.z[i]), sg = sigmoid(z), inner = fmaf(skip, to_f32(raw.u[i]), y[i * P]);
+                    const int t = row + at.p + i * P;
+                    const float v = t >= from && t < to ? to_f32(raw.g[i]) * inner * (sg * fmaf(z, 1.f - sg, 1.f)) : 0.f;
+                    if (at.there && t < r1) out[(long long)i * P * p.E] = from_f32<IO>(v);
+                }
+            }
+            float along_B[BATCH], along_A[BATCH], sums[COUNT];
+            const auto back = [&](auto j_, const float (&before)[4], bool inside) {
+                constexpr int j = decltype(j_)::value;
+                const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]), gj = from_lane<P, j % P>(g[j / P]);
+                const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * P + 4 * at.p]);
+                float dB[4], dC[4];
+                along_A[j] = along_B[j] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (inside) {
+                        const float r = fmaf(Ct[k], gj, R[k]);
+                        dB[k] = at.there ? r * v : 0.f;
+                        dC[k] = at.there ? gj * hs[j + 1][k] : 0.f;
+                        along_B[j] = fmaf(r, Bt[k], along_B[j]);
+                        R[k] = fast_exp2(d * a2[k]) * r;
+                        const float q = R[k] * before[k];
+                        along_A[j] = fmaf(q, a2[k], along_A[j]);
+                        dA[k] = fmaf(q, d, dA[k]);
+                    } else dB[k] = dC[k] = 0.f;
+                }
+                if constexpr (P == 16) {
+                    sum_over_channels<P, COUNT>(dB, at.lane);
+                    sum_over_channels<P, COUNT>(dC, at.lane);
+                    red[buf % BUFS][wave][j * ROW + leave] = dB[0];
+                    red[buf % BUFS][wave][j * ROW + 4 * P + leave] = dC[0];
+                } else {
+                    constexpr int GROUP = COUNT / 8;       // tokens whose sums go through the wave together
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        sums[j % GROUP * 8 + k] = dB[k];
+                        sums[j % GROUP * 8 + 4 + k] = dC[k];
+                    }
+                    if constexpr (j % GROUP == 0) {
+                        sum_over_channels<P, COUNT>(sums, at.lane);
+                        red[buf % BUFS][wave][j * ROW + leave] = sums[0];
+                    }
+                }
+            };
+            if (clean)
+                each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
+                    constexpr int j = BATCH - 1 - decltype(j_)::value;
+                    back(std::integral_constant<int, j>(), hs[j], true);
+                });
+            else
+                each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
+                    constexpr int j = BATCH - 1 - decltype(j_)::value;
+                    const bool inside = row + j >= from && row + j < to;
+                    float before[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) before[k] = hs[j][k];
+                    if (inside && row + j == w.end - 1) state_of(bp.glast, w.n, R);
+                    if (inside && row + j == w.begin) state_of(p.state, w.n, before);
+                    back(std::integral_constant<int, j>(), before, inside);
+                    if (inside && row + j == w.begin) {
+                        first_gradient(w.n, R);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) R[k] = 0.f;
+                        w.previous(p.seq);
+                    }
+                });
+            sum_to_lanes<P, BATCH>(along_A, at.p);
+            sum_to_lanes<P, BATCH>(along_B, at.p);
+            IO* const du = static_cast<IO*>(bp.du) + ((long long)b * p.T + row + at.p) * p.E + e;
+            IO* const dd = static_cast<IO*>(bp.dd) + ((long long)b * p.T + row + at.p) * p.E + e;
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                const float u = to_f32(raw.u[i]);
+                const int t = row + at.p + i * P;
+                const bool inside = t >= from && t < to;
+                float a = fmaf(along_A[i * P], 1.f / LOG2E, u * along_B[i * P]);
+                if (p.softplus) a *= sigmoid(to_f32(raw.d[i]) + bias);
+                if (inside) {
+                    dD = fmaf(g[i], u, dD);
+                    dbias += a;
+                }
+                if (at.there && t < r1) {
+                    du[(long long)i * P * p.E] = from_f32<IO>(inside ? fmaf(dt[i], along_B[i * P], skip * g[i]) : 0.f);
+                    dd[(long long)i * P * p.E] = from_f32<IO>(inside ? a : 0.f);
+                }
+            }
+            if (more) {
+                stage.put(bc[buf ^ 1]);
+                raw = ahead;
+                kept = kept_ahead;
+            }
+            lds_barrier();
+#pragma unroll
+            for (int i = threadIdx.x; i < SUMS; i += THREADS) {
+                const int t = row + i / ROW;
+                float v = 0.f;
+#pragma unroll
+                for (int q = 0; q < THREADS / WAVE; ++q) v += red[buf % BUFS][q][i];
+                if (t < r1) bp.part_bc[((((long long)(blockIdx.x % p.blocks) * p.rows + b) * p.T + t) * p.G + at.g) * ROW + i % ROW] = t >= from && t < to ? v : 0.f;
+            }
+            if (BUFS == 1) lds_barrier();
+        }
+    }
+    if (p.seq.offsets && bp.dstate)                        // sequences without a token hand the last states' gradients on
+        for (int n0 = s; n0 < p.N; n0 += p.nseg * 64) {
+            const int mine = n0 + at.lane * p.nseg;
+            unsigned long long empty = __ballot(mine < p.N && p.seq.of_lane(min(mine, p.N - 1) + 1) <= p.seq.of_lane(min(mine, p.N - 1)));
+            for (; empty; empty &= empty - 1) {
+                const int m = n0 + (__ffsll((long long)empty) - 1) * p.nseg;
+                float h[4];
+                state_of(bp.glast, m, h);
+                first_gradient(m, h);
+            }
+        }
+    float v[P], x[P];
+#pragma unroll
+    for (int q = 0; q < P; ++q) v[q] = dD, x[q] = dbias;
+    sum_to_lanes<P, P>(v, at.p);
+    sum_to_lanes<P, P>(x, at.p);
+    if (!at.there) return;
+    *reinterpret_cast<f32x4*>(bp.part_A + (part * p.E + e) * 4 * P + 4 * at.p) = f32x4{dA[0], dA[1], dA[2], dA[3]};
+    if (at.p == 0) {
+        bp.part_D[part * p.E + e] = v[0];
+        bp.part_bias[part * p.E + e] = x[0];
+    }
+}
+
+template <typename IO>
+int launch_backward(const BackParams& bp, int parts, hipStream_t st) {
+    const Params& p = bp.f;
+    return with_lanes(p.S, [&](auto P_, auto full) {
+        constexpr int P = decltype(P_)::value;
+        constexpr bool FULL = decltype(full)::value;
+        const dim3 block(THREADS);
+        if (p.nseg > 1) hipLaunchKernelGGL((back_segments_kernel<IO, P, FULL>), dim3(p.G * p.blocks, p.nseg - 1, p.rows), block, 0, st, bp);
+        hipLaunchKernelGGL((back_kernel<IO, P, FULL>), dim3(p.G * p.blocks, p.nseg, parts), block, 0, st, bp);
+        return check_launch("vrwkv_scan_bwd");
+    });
+}
+
+}  // namespace scan
+}  // namespace vrwkv

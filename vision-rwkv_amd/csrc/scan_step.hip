@@ -1,0 +1,166 @@
+// One more token for each of N sequences whose states are pages of a pool: h = exp(dt A) h + dt u B, y = (C h + D u) silu(z), h written back (gfx950).
+// Bound by the pages, read and written once: P lanes hold four states each of NC channels, 16 bytes a lane and channel, all of them on their way before the first is used.
+#include "scan.h"
+#include "pages.h"
+#include <algorithm>
+
+namespace vrwkv {
+namespace scan {
+namespace {
+
+constexpr int NC = 4, GRID_Y = 32768;
+
+struct StepParams {
+    const void *u, *delta, *B, *C, *z;
+    const float* A;
+    ParamVec D, bias;
+    Slots slots;
+    float* pool;
+    void* y;
+    long long u_n, d_n, z_n, B_n, B_g, C_n, C_g, page;
+    int E, S, G, softplus, blocks;
+};
+
+// VEC: states and A are read and written 16 bytes at a time
+template <typename IO, int P, bool VEC>
+__global__ __launch_bounds__(THREADS) void step_kernel(const StepParams p) {
+    const int tid = threadIdx.x, q = tid % P, of_group = p.E / p.G, g = blockIdx.x / p.blocks, n0 = blockIdx.y + GRID_Y * blockIdx.z;
+    if (n0 >= p.slots.rows) return;
+    const long long slot = p.slots.at(n0);
+    const bool known = p.slots.has(slot);
+    float* const page = p.pool + (known ? slot : 0) * p.page;
+    int e[NC];
+    bool there[NC];
+    f32x4 h[NC], a[NC];
+    const auto row_of = [&](const float* t, f32x4& x) {
+        if (VEC) x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(t));
+        else
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = 4 * q + k < p.S ? t[k] : 0.f;
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int i = ((blockIdx.x % p.blocks) * NC + c) * (THREADS / P) + tid / P;
+        there[c] = i < of_group;
+        e[c] = g * of_group + min(i, of_group - 1);
+        h[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (known && there[c]) row_of(page + (long long)e[c] * p.S + 4 * q, h[c]);
+    }
+    float u[NC], d[NC], z[NC], Bt[4], Ct[4];
+    const auto token = [&](int n) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            u[c] = to_f32(static_cast<const IO*>(p.u)[n * p.u_n + e[c]]);
+            d[c] = to_f32(static_cast<const IO*>(p.delta)[n * p.d_n + e[c]]);
+            z[c] = p.z ? to_f32(static_cast<const IO*>(p.z)[n * p.z_n + e[c]]) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int s = min(4 * q + k, p.S - 1);
+            Bt[k] = to_f32(static_cast<const IO*>(p.B)[n * p.B_n + g * p.B_g + s]);
+            Ct[k] = to_f32(static_cast<const IO*>(p.C)[n * p.C_n + g * p.C_g + s]);
+        }
+    };
+    token(n0);
+    float bias[NC], skip[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        if (VEC) a[c] = *reinterpret_cast<const f32x4*>(p.A + (long long)e[c] * p.S + 4 * q);
+        else row_of(p.A + (long long)e[c] * p.S + 4 * q, a[c]);
+        a[c] *= LOG2E;
+        bias[c] = p.bias.p ? p.bias.value(p.bias.fetch(e[c])) : 0.f;
+        skip[c] = p.D.p ? p.D.value(p.D.fetch(e[c])) : 0.f;
+    }
+    int next;
+    if (!p.slots.first_of_page(n0, slot, next)) return;
+    for (int n = n0;;) {
+        float y[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const float raw = d[c] + bias[c], dt = p.softplus ? softplus(raw) : raw, x = dt * u[c];
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool pad = !VEC && 4 * q + k >= p.S;
+                h[c][k] = pad ? 0.f : fmaf(fast_exp2(dt * a[c][k]), h[c][k], x * Bt[k]);
+                s = pad ? s : fmaf(Ct[k], h[c][k], s);
+            }
+            if (P > 1) s += across<1>(s);
+            if (P > 2) s += across<2>(s);
+            if (P > 4) s += across<4>(s);
+            if (P > 8) s += across<8>(s);
+            y[c] = fmaf(skip[c], u[c], s);
+            if (p.z) y[c] *= z[c] * sigmoid(z[c]);
+            if (!known) y[c] = slot == -1 ? 0.f : __builtin_nanf("");
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (there[c] && q == 0) static_cast<IO*>(p.y)[(long long)n * p.E + e[c]] = from_f32<IO>(y[c]);
+        if (next >= p.slots.rows) break;
+        n = next;
+        next = p.slots.behind(n, slot);
+        token(n);
+    }
+    if (!known) return;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        if (!there[c]) continue;
+        float* to = page + (long long)e[c] * p.S + 4 * q;
+        if (VEC) __builtin_nontemporal_store(h[c], reinterpret_cast<f32x4*>(to));
+        else
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (4 * q + k < p.S) to[k] = h[c][k];
+    }
+}
+
+template <typename IO, int P>
+int launch(StepParams& p, bool vec, hipStream_t st) {
+    const int each = THREADS / P * NC;
+    p.blocks = (p.E / p.G + each - 1) / each;
+    const dim3 grid((unsigned)(p.G * p.blocks), (unsigned)std::min(p.slots.rows, GRID_Y), (unsigned)((p.slots.rows + GRID_Y - 1) / GRID_Y)), block(THREADS);
+    if (vec && p.S == 4 * P) hipLaunchKernelGGL((step_kernel<IO, P, true>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((step_kernel<IO, P, false>), grid, block, 0, st, p);
+    return check_launch("vrwkv_scan_step");
+}
+template <typename IO>
+int launch(StepParams& p, bool vec, hipStream_t st) {
+    if (p.S <= 4) return launch<IO, 1>(p, vec, st);
+    if (p.S <= 8) return launch<IO, 2>(p, vec, st);
+    if (p.S <= 16) return launch<IO, 4>(p, vec, st);
+    if (p.S <= 32) return launch<IO, 8>(p, vec, st);
+    return launch<IO, 16>(p, vec, st);
+}
+
+}  // namespace
+}  // namespace scan
+}  // namespace vrwkv
+
+using namespace vrwkv;
+
+extern "C" int vrwkv_scan_step(const vrwkv_scan_step_args* args, void* hip_stream) {
+    const char* who = "vrwkv_scan_step";
+    if (!args || !args->u || !args->delta || !args->A || !args->B || !args->C || !args->pool || !args->y) { set_error("%s: null pointer", who); return VRWKV_INVALID_ARG; }
+    const vrwkv_scan_step_args& a = *args;
+    if (a.N <= 0 || a.P <= 0 || a.E <= 0 || a.G <= 0) { set_error("%s: N, P, E and G must be positive", who); return VRWKV_INVALID_ARG; }
+    if (a.dtype < VRWKV_F32 || a.dtype > VRWKV_F16 || a.D_dtype < VRWKV_F32 || a.D_dtype > VRWKV_F16 || a.bias_dtype < VRWKV_F32 || a.bias_dtype > VRWKV_F16) {
+        set_error("%s: dtype must be fp32, bf16 or fp16", who);
+        return VRWKV_UNSUPPORTED_DTYPE;
+    }
+    if (a.S < 1 || a.S > 64 || a.E % a.G) { set_error("%s: 1 to 64 states (%d), and E (%d) a multiple of G (%d)", who, a.S, a.E, a.G); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (!a.slots && a.N > a.P) { set_error("%s: %d rows without slots, and %d pages", who, a.N, a.P); return VRWKV_INVALID_ARG; }
+    if (a.page_stride < (long long)a.E * a.S) { set_error("%s: pages overlap", who); return VRWKV_INVALID_ARG; }
+    const size_t w = a.dtype == VRWKV_F32 ? 3 : 1;
+    if ((((size_t)a.u | (size_t)a.delta | (size_t)a.B | (size_t)a.C | (size_t)a.z | (size_t)a.y) & w) || (((size_t)a.pool | (size_t)a.A) & 3) ||
+        ((size_t)a.D & (a.D_dtype == VRWKV_F32 ? 3 : 1)) || ((size_t)a.delta_bias & (a.bias_dtype == VRWKV_F32 ? 3 : 1)) || (a.slots && ((size_t)a.slots & (a.slots64 ? 7 : 3)))) {
+        set_error("%s: a tensor is not aligned to its elements", who);
+        return VRWKV_INVALID_ARG;
+    }
+    scan::StepParams p{a.u, a.delta, a.B, a.C, a.z, a.A, ParamVec(a.D, a.D_dtype, 1.f), ParamVec(a.delta_bias, a.bias_dtype, 1.f), Slots{a.slots, a.slots64, a.N, a.P}, a.pool, a.y,
+                       a.u_stride, a.delta_stride, a.z_stride, a.B_stride[0], a.B_stride[1], a.C_stride[0], a.C_stride[1], a.page_stride, a.E, a.S, a.G, a.softplus, 0};
+    const bool vec = (((size_t)a.pool | (size_t)a.A) & 15) == 0 && a.page_stride % 4 == 0;
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    if (a.dtype == VRWKV_F32) return scan::launch<float>(p, vec, st);
+    if (a.dtype == VRWKV_BF16) return scan::launch<__hip_bfloat16>(p, vec, st);
+    return scan::launch<__half>(p, vec, st);
+}

@@ -1,0 +1,70 @@
+#pragma once
+#include "vrwkv_common.h"
+
+namespace vrwkv {
+
+// The sequences of a batch of token rows: row b of the batch whole, or with offsets (N + 1 of 32 or 64 bits, ascending) N of them packed in one row of T tokens,
+// n at tokens offsets[n] to offsets[n + 1].  Offsets outside 0 .. T are taken as 0 or T, so that no token outside the rows is named whatever they hold.
+struct Sequences {
+    const void* offsets;
+    int is64, N, T;
+    __device__ __forceinline__ int of_lane(int i) const {
+        const long long v = is64 ? static_cast<const long long*>(offsets)[i] : (long long)static_cast<const int*>(offsets)[i];
+        return (int)(v < 0 ? 0 : v > T ? T : v);
+    }
+    // (the same i in all lanes)
+    __device__ __forceinline__ int at(int i) const { return __builtin_amdgcn_readfirstlane(of_lane(i)); }
+    // The first sequence that ends behind token t, N if there is none: 64 offsets at a time, by all lanes of a wave together.
+    __device__ __forceinline__ int first_ending_behind(int t, int lane) const {
+        int lo = 0, hi = N;                               // the answer is in lo .. hi
+        while (hi - lo > 0) {
+            const int step = (hi - lo + 63) / 64, i = lo + (lane + 1) * step - 1;   // the last of each piece
+            const bool before = i < hi && of_lane(i + 1) <= t;
+            const int pieces = __popcll(__ballot(before));
+            const int from = min(lo + pieces * step, hi);
+            hi = min(from + step - 1, hi);
+            lo = from;
+        }
+        return __builtin_amdgcn_readfirstlane(lo);
+    }
+    // The tokens [from, to) of [r0, r1) that belong to a sequence.
+    __device__ __forceinline__ void inside(int r0, int r1, int& from, int& to) const {
+        from = offsets ? max(r0, at(0)) : r0;
+        to = offsets ? min(r1, at(N)) : r1;
+    }
+};
+
+// The sequence that a walk along the tokens of batch row b is in: number n, tokens [begin, end).
+struct Walk {
+    int n, begin, end;
+    __device__ __forceinline__ void read(const Sequences& s) {
+        begin = n >= 0 && n < s.N ? s.at(n) : 0x7fffffff;
+        end = n >= 0 && n < s.N ? s.at(n + 1) : 0x7fffffff;
+    }
+    // the one that token t is in (none: one without tokens, perhaps)
+    __device__ __forceinline__ void find(const Sequences& s, int b, int t, int lane) {
+        if (!s.offsets) {
+            n = b, begin = 0, end = s.T;
+            return;
+        }
+        n = s.first_ending_behind(t, lane);
+        read(s);
+    }
+    __device__ __forceinline__ void next(const Sequences& s) {
+        const int done = end;
+        if (!s.offsets) n = s.N;
+        else
+            for (++n; n < s.N && s.at(n + 1) <= done; ++n) {}
+        read(s);
+    }
+    __device__ __forceinline__ void previous(const Sequences& s) {
+        if (!s.offsets) n = -1;
+        else
+            for (--n; n >= 0 && s.at(n) >= s.at(n + 1); --n) {}
+        read(s);
+    }
+    // whether none begins or ends in [row, row + count)
+    __device__ __forceinline__ bool within(int row, int count) const { return (begin < row || begin >= row + count) && (end <= row || end > row + count); }
+};
+
+}  // namespace vrwkv

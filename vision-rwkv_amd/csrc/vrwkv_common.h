@@ -32,6 +32,7 @@ enum Option {
     OPT_LINEAR_TILE,        // tile of the block entry's projections (1, 2, 4, 8: 16 to 128 results on a side; 16: 256 channels wide)
     OPT_WGRAD_SPLITS,       // token ranges of a weight gradient
     OPT_LINEAR_MIX,         // norm, shift and mixes inside a half's projections: 1 or an error, 2 never
+    OPT_SCAN_SEGMENTS,      // segments a sequence of the selective scan is cut into
     N_OPTIONS
 };
 int option(Option o);
