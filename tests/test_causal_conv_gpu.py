@@ -7,11 +7,19 @@ import pytest
 import torch
 
 import vision_rwkv_amd as vr
+from vision_rwkv_amd import _lib
 
 DEV = "cuda"
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=[True, False], ids=["compiled", "python"])
+def host(request, monkeypatch):
+    """The operators through the compiled host module, and through the Python classes alone."""
+    if not request.param:
+        monkeypatch.setattr(_lib, "host", lambda: _lib._NoHost)
 
 
 def reference(x, w, b, act, state, bounds, gy=None, glast=None):

@@ -8,12 +8,20 @@ import pytest
 import torch
 
 import vision_rwkv_amd as vr
+from vision_rwkv_amd import _lib
 
 DEV = "cuda"
 DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 EPS = 1e-6
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=[True, False], ids=["compiled", "python"])
+def host(request, monkeypatch):
+    """The operators through the compiled host module, and through the Python classes alone."""
+    if not request.param:
+        monkeypatch.setattr(_lib, "host", lambda: _lib._NoHost)
 
 
 def inputs(shape, dtype, params="fp32", residual=None, seed=0):

@@ -120,7 +120,7 @@ class _NoHost:
     def wkv(*args):
         return None
 
-    wkv6 = block_forward = decay_attention = decay_step = copy_pages = wkv
+    wkv6 = block_forward = decay_attention = decay_step = copy_pages = causal_conv = causal_conv_step = selective_scan = selective_scan_step = rms_norm = wkv
 
     @staticmethod
     def weights_fit(*args):

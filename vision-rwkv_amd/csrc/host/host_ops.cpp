@@ -16,37 +16,11 @@
 #include <cstddef>
 #include <string_view>
 #include <unordered_map>
-#include <torch/extension.h>
-#include <torch/version.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include "../../../include/vrwkv_hip.h"
+#include "host_common.h"
+
+using namespace host;
 
 namespace {
-using torch::autograd::AutogradContext;
-using torch::autograd::tensor_list;
-using torch::autograd::Variable;
-
-int code(at::ScalarType t) { return t == at::kFloat ? VRWKV_F32 : t == at::kBFloat16 ? VRWKV_BF16 : t == at::kHalf ? VRWKV_F16 : -1; }
-
-void* stream_of(const at::Tensor& t) { return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream(); }
-
-using Guard = c10::hip::HIPGuardMasqueradingAsCUDA;
-
-// Tracing, functorch levels, dispatch and function modes are to see the operators' Python classes.
-bool transformed() {
-    return torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
-           at::impl::PythonTorchFunctionTLS::stack_len() > 0;
-}
-
 // An exact Tensor or Parameter with memory of its own, dense, contiguous, on a GPU.
 bool plain(PyObject* o) {
     if (!THPVariable_CheckExact(o)) return false;
@@ -60,17 +34,12 @@ bool plain(PyObject* o) {
 // The entry points take dimensions as int, the Bi-WKV backward 65535 sequences.
 bool fits(const at::Tensor& t) { return t.size(0) <= 65535 && t.size(1) <= INT_MAX && t.size(2) <= INT_MAX; }
 
-// Forward-mode tangents are refused by the Python classes.
-bool tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
-
 // A tensor that a hook on saved tensors, or the engine, hands to a backward.
 at::Tensor dense(const at::Tensor& t, const at::Tensor& like) {
     TORCH_CHECK(t.defined() && t.has_storage() && t.is_cuda() && t.device() == like.device() && code(t.scalar_type()) >= 0,
                 "the saved tensors and the gradient must be CUDA tensors on one device");
     return t.contiguous();
 }
-
-at::Tensor bytes(size_t n, const at::Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)); }
 
 // ---- Bi-WKV --------------------------------------------------------------------------------------------------------------
 // y, or an undefined tensor where the entry point refuses the call
@@ -300,17 +269,6 @@ py::object block_forward(py::handle x_, py::dict tensors, py::object params, py:
 }
 
 // ---- attention with a decay for each head -----------------------------------------------------------------------------------
-// An exact Tensor or Parameter on a GPU whose memory the kernels may read at its strides, channels side by side (`t` outlives the call: the caller holds it).
-const at::Tensor* strided(py::handle o) {
-    if (!THPVariable_CheckExact(o.ptr())) return nullptr;
-    const at::Tensor& t = THPVariable_Unpack(o.ptr());
-    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.is_conj() || t.is_neg()) return nullptr;
-    const auto keys = t.key_set();
-    if (keys.has(c10::DispatchKey::FuncTorchBatched) || keys.has(c10::DispatchKey::Batched) || keys.has(c10::DispatchKey::Python) ||
-        keys.has(c10::DispatchKey::FuncTorchGradWrapper) || keys.has(c10::DispatchKey::Functionalize))
-        return nullptr;
-    return &t;
-}
 bool rows_fit(const at::Tensor& t, int lead) { return t.dim() == lead + 2 && t.numel() > 0 && t.stride(-1) == 1 && (lead == 1 || t.stride(1) < (1 << 22)); }
 
 // q, k, v, g as decay_attention and its step take them, nothing empty, nothing to convert
@@ -327,10 +285,6 @@ bool decay_inputs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
 bool here(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g) {
     return q.get_device() == c10::hip::current_device() && !tangent(q) && !tangent(k) && !tangent(v) && !tangent(g);
 }
-bool index_fits(const at::Tensor& t, const at::Tensor& q) {
-    return t.dim() == 1 && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.is_contiguous() && t.numel() > 0 && t.device() == q.device();
-}
-
 vrwkv_decay_args decay_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, const at::Tensor& state, const at::Tensor& offsets, double scale, int N) {
     vrwkv_decay_args a = {};
     a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.g = g.data_ptr();
@@ -407,16 +361,7 @@ struct Decay : torch::autograd::Function<Decay> {
             const int rc = vrwkv_decay_bwd(&a, stream_of(q));
             TORCH_CHECK(rc == VRWKV_OK, "vrwkv status ", rc, ": ", vrwkv_last_error());
         }
-        if (recorded) {                                    // (create_graph: differentiating these once more raises)
-            tensor_list some;
-            for (auto& t : out)
-                if (t.defined()) some.push_back(t.detach().set_requires_grad(true));
-            const auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)some.size());
-            some = (*error)(std::move(some));
-            size_t i = 0;
-            for (auto& t : out)
-                if (t.defined()) t = some[i++];
-        }
+        if (recorded) only_once(out);
         return out;
     }
 };
@@ -456,15 +401,6 @@ py::object decay_attention(py::handle q_, py::handle k_, py::handle v_, py::hand
     py::object y = py::reinterpret_steal<py::object>(THPVariable_Wrap(out[0]));
     if (!keep) return y;
     return py::make_tuple(y, py::reinterpret_steal<py::object>(THPVariable_Wrap(out[1])));
-}
-
-bool pages_fit(const at::Tensor& pool) {
-    int64_t want = 1;
-    for (int64_t i = pool.dim() - 1; i > 0; --i) {
-        if (pool.size(i) != 1 && pool.stride(i) != want) return false;
-        want *= pool.size(i);
-    }
-    return pool.size(0) == 1 || pool.stride(0) >= want;
 }
 
 py::object decay_step(py::handle q_, py::handle k_, py::handle v_, py::handle g_, py::handle pool_, py::handle slots_, double scale) {
@@ -523,7 +459,10 @@ bool copy_pages(py::handle pool_, py::handle src_, py::handle dst_, py::handle s
 }
 }  // namespace
 
+void add_scan_operators(py::module_& m);                   // scan_ops.cpp
+
 PYBIND11_MODULE(_host, m) {
+    add_scan_operators(m);
     m.def("decay_attention", &decay_attention);
     m.def("decay_step", &decay_step);
     m.def("copy_pages", &copy_pages);

@@ -136,6 +136,10 @@ def rms_norm(x, weight, residual=None, eps=1e-6, quantize=None):
         raise RuntimeError("eps must be a number")
     if quantize not in _KINDS:
         raise RuntimeError("quantize must be None, torch.float8_e4m3fn or torch.int8")
+    out = _lib.host().rms_norm(x, weight, residual, float(eps), _KINDS[quantize])
+    if out is not None:
+        y, scale, r = out
+        return ((y, scale) if r is None else (y, scale, r)) if quantize is not None else y if r is None else (y, r)
     _check_recorders("rms_norm", x, weight, residual)
     _check_norm(x, weight, residual)
     record = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual))

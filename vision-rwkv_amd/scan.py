@@ -206,6 +206,10 @@ def causal_conv(x, weight, bias=None, activation=None, state=None, offsets=None,
     program makes the call as it is)."""
     if torch.compiler.is_compiling():
         return _eager(causal_conv)(x, weight, bias, activation, state, offsets, return_state)
+    if activation in (None, "silu"):
+        out = _lib.host().causal_conv(x, weight, bias, activation is not None, state, offsets, return_state)
+        if out is not None:
+            return out
     _check_recorders("causal_conv", x, weight, bias, state, offsets)
     N = _check_conv(x, weight, bias, activation, state, offsets)
     y, last = CausalConv.apply(x, weight, bias, state, offsets, activation, N, bool(return_state))
@@ -219,6 +223,10 @@ def causal_conv_step(x, weight, pool, slots=None, bias=None, activation=None):
     behind each other; -1 gives zeros and touches nothing, any other slot outside the pool NaN.  Forward only: inputs that want gradients or carry tangents are refused, and so is tracing."""
     if torch.compiler.is_compiling():
         return _eager(causal_conv_step)(x, weight, pool, slots, bias, activation)
+    if activation in (None, "silu"):
+        y = _lib.host().causal_conv_step(x, weight, pool, slots, bias, activation is not None)
+        if y is not None:
+            return y
     _check_recorders("causal_conv_step", x, weight, bias, pool, slots)
     x, weight, bias, slots = (_resolved(t) for t in (x, weight, bias, slots))
     _check(x, "x")
@@ -381,6 +389,9 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     fp32 numbers a channel and token).  No second gradients, no forward mode, no tracing (a compiled program makes the call as it is)."""
     if torch.compiler.is_compiling():
         return _eager(selective_scan)(u, delta, A, B, C, D, z, delta_bias, softplus, state, offsets, return_state)
+    out = _lib.host().selective_scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, offsets, return_state)
+    if out is not None:
+        return out
     tensors = u, delta, A, B, C, D, z, delta_bias, state
     _check_recorders("selective_scan", *tensors, offsets)
     N, _ = _check_scan(*tensors, offsets)
@@ -397,6 +408,9 @@ def selective_scan_step(u, delta, A, B, C, pool, slots=None, D=None, z=None, del
     tangents are refused, and so is tracing."""
     if torch.compiler.is_compiling():
         return _eager(selective_scan_step)(u, delta, A, B, C, pool, slots, D, z, delta_bias, softplus)
+    y = _lib.host().selective_scan_step(u, delta, A, B, C, pool, slots, D, z, delta_bias, softplus)
+    if y is not None:
+        return y
     tensors = u, delta, A, B, C, D, z, delta_bias
     _check_recorders("selective_scan_step", *tensors, pool, slots)
     E, S, G = _check_scan_inputs(*tensors, 1)
