@@ -60,44 +60,54 @@ struct Place {
     }
 };
 
+// A tensor's row as all lanes of a wave see it, and a lane's place in it in bytes: an address in scalar registers and 32 bits of a vector register, not 64 for each of a lane's tokens.
+template <typename T>
+__device__ __forceinline__ T& at_row(const T* row, unsigned bytes) {
+    asm volatile("" : "+v"(bytes));                        // (else the compiler keeps their sums, from iteration to iteration)
+    return *const_cast<T*>(reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + bytes));
+}
+
 // What a lane has of sixteen tokens: its channel of every P-th.
 template <typename IO, int P>
 struct Rows {
     static constexpr int OWN = BATCH / P;
     IO u[OWN], d[OWN], z[OWN], g[OWN];
-    // tokens row, row + P, .. of a tensor whose batch row begins at `base`; behind `end` the last in front of it once more
-    __device__ __forceinline__ void fetch(IO (&to)[OWN], const void* t, long long base, long long stride, int row, int end, int e) const {
-        const IO* x = static_cast<const IO*>(t) + base + e;
-        if (row - row % P + BATCH <= end) {
-            x += row * stride;
+    // tokens row + q, row + q + P, .. of a tensor whose batch row begins at `base`; behind `end` the last in front of it once more
+    __device__ __forceinline__ void fetch(IO (&to)[OWN], const void* t, long long base, long long stride, int row, int end, int q, int e) const {
+        const IO* x = static_cast<const IO*>(t) + base + row * stride;
+        if (row + BATCH <= end) {
+            const unsigned place = (q * (unsigned)stride + e) * sizeof(IO);
 #pragma unroll
-            for (int i = 0; i < OWN; ++i) to[i] = x[(int)stride * (i * P)];
+            for (int i = 0; i < OWN; ++i) to[i] = at_row(x + i * P * stride, place);
         } else {
+            asm volatile("" : "+v"(q));                    // (nothing of this is kept for other rows)
 #pragma unroll
-            for (int i = 0; i < OWN; ++i) to[i] = x[min(row + i * P, end - 1) * stride];
+            for (int i = 0; i < OWN; ++i) to[i] = at_row(x, (min(q + i * P, end - 1 - row) * (unsigned)stride + e) * sizeof(IO));
         }
     }
 };
 
-// B and C of sixteen tokens on their way to LDS.
+// B and C of sixteen tokens on their way to LDS, first all of B: a wave's are of one of them.
 template <typename IO, int P, int WHICH>
 struct Stage {
-    static constexpr int VALUES = BATCH * WHICH * 4 * P, EACH = (VALUES + THREADS - 1) / THREADS;
+    static constexpr int ONE = BATCH * 4 * P, VALUES = ONE * WHICH, EACH = (VALUES + THREADS - 1) / THREADS;
     IO raw[EACH];
     __device__ __forceinline__ void fetch(const Params& p, long long b, int g, int row, int from, int to) {
+        const int first = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
 #pragma unroll
         for (int k = 0; k < EACH; ++k) {
-            const int i = threadIdx.x + k * THREADS, t = i / (WHICH * 4 * P), w = i / (4 * P) % WHICH, n = i % (4 * P);
+            const bool isC = first + k * THREADS >= ONE;
+            const int i = threadIdx.x + k * THREADS, t = i % ONE / (4 * P), n = i % (4 * P);
+            const IO* x = isC ? static_cast<const IO*>(p.C) + b * p.C_b + row * p.C_t + g * p.C_g : static_cast<const IO*>(p.B) + b * p.B_b + row * p.B_t + g * p.B_g;
             raw[k] = from_f32<IO>(0.f);
-            if (i < VALUES && row + t >= from && row + t < to && n < p.S)
-                raw[k] = w == 0 ? static_cast<const IO*>(p.B)[b * p.B_b + (row + t) * p.B_t + g * p.B_g + n] : static_cast<const IO*>(p.C)[b * p.C_b + (row + t) * p.C_t + g * p.C_g + n];
+            if (i < VALUES && row + t >= from && row + t < to && n < p.S) raw[k] = at_row(x, (t * (unsigned)(isC ? p.C_t : p.B_t) + n) * sizeof(IO));
         }
     }
     __device__ __forceinline__ void put(float* to) const {
 #pragma unroll
         for (int k = 0; k < EACH; ++k) {
             const int i = threadIdx.x + k * THREADS;
-            if (i < VALUES) to[i] = to_f32(raw[k]);
+            if (i < VALUES) to[i % ONE / (4 * P) * WHICH * 4 * P + i / ONE * 4 * P + i % (4 * P)] = to_f32(raw[k]);
         }
     }
 };
@@ -153,9 +163,9 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(const Params p) {
 
     Rows<IO, P> raw, ahead;
     const auto fetch = [&](Rows<IO, P>& x, int row) {
-        x.fetch(x.u, p.u, b * p.u_b, p.u_t, row + at.p, r1, e);
-        x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row + at.p, r1, e);
-        if (EMIT && p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row + at.p, r1, e);
+        x.fetch(x.u, p.u, b * p.u_b, p.u_t, row, r1, at.p, e);
+        x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
+        if (EMIT && p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row, r1, at.p, e);
     };
     Stage<IO, P, WHICH> stage;
     fetch(raw, r0);
@@ -171,65 +181,72 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(const Params p) {
             stage.fetch(p, b, at.g, row + BATCH, from, to);
         }
         if (EMIT && p.kept && at.there)
-            *reinterpret_cast<f32x4*>(p.kept + (((long long)b * ((p.T + BATCH - 1) / BATCH) + row / BATCH) * p.E + e) * 4 * P + 4 * at.p) = f32x4{h[0], h[1], h[2], h[3]};
-        float dt[OWN], x[OWN], y[BATCH];
+            at_row(reinterpret_cast<const f32x4*>(p.kept) + ((long long)b * ((p.T + BATCH - 1) / BATCH) + row / BATCH) * p.E * P, (unsigned)(e * P + at.p) * 16u) = f32x4{h[0], h[1], h[2], h[3]};
+        float dt[OWN], x[OWN];
 #pragma unroll
         for (int i = 0; i < OWN; ++i) {
             const float d = to_f32(raw.d[i]) + bias;
             dt[i] = p.softplus ? softplus(d) : d;
             x[i] = dt[i] * to_f32(raw.u[i]);
         }
-        const auto token = [&](auto j_) {
-            constexpr int j = decltype(j_)::value;
-            const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]);
-            const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * at.p]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                h[k] = fmaf(fast_exp2(d * a2[k]), h[k], v * Bt[k]);
-                if (!FULL && pad[k]) h[k] = 0.f;           // (an infinite v would make it NaN)
-            }
-            if (EMIT) {
-                const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * P + 4 * at.p]);
-                y[j] = fmaf(Ct[3], h[3], fmaf(Ct[2], h[2], fmaf(Ct[1], h[1], Ct[0] * h[0])));
-            }
-        };
-        if (row >= from && row + BATCH <= to && w.within(row, BATCH)) {
-            each(std::make_integer_sequence<int, BATCH>(), token);
-            if (!EMIT) {
-#pragma unroll
-                for (int i = 0; i < OWN; ++i) total += dt[i];
-            }
-        } else {
-            // (a segment's sum of step sizes is only read where one sequence goes through all of it: no token of such a one is left out)
-            if (!EMIT) {
-#pragma unroll
-                for (int i = 0; i < OWN; ++i) total += row + at.p + i * P < r1 ? dt[i] : 0.f;
-            }
+        const IO* const out = static_cast<const IO*>(p.y) + ((long long)b * p.T + row) * p.E;
+        const unsigned place = (at.p * (unsigned)p.E + e) * sizeof(IO);
+        // tokens [first, behind) of the sixteen, all of one sequence; PART: not all sixteen
+        const auto piece = [&](auto part_, int first, int behind) {
+            constexpr bool PART = decltype(part_)::value;
+            float y[BATCH];
             each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
                 constexpr int j = decltype(j_)::value;
                 y[j] = 0.f;
-                if (row + j < from || row + j >= to) return;
-                if (row + j == w.begin) first_state(w.n);
-                token(j_);
-                if (row + j == w.end - 1) {
-                    last_state(w.n);
-                    w.next(p.seq);
+                if (PART && (row + j < first || row + j >= behind)) return;
+                const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]);
+                const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * at.p]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    h[k] = fmaf(fast_exp2(d * a2[k]), h[k], v * Bt[k]);
+                    if (!FULL && pad[k]) h[k] = 0.f;       // (an infinite v would make it NaN)
+                }
+                if (EMIT) {
+                    const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * P + 4 * at.p]);
+                    y[j] = fmaf(Ct[3], h[3], fmaf(Ct[2], h[2], fmaf(Ct[1], h[1], Ct[0] * h[0])));
                 }
             });
-        }
-        if (EMIT) {
-            sum_to_lanes<P, BATCH>(y, at.p);
-            IO* out = static_cast<IO*>(p.y) + ((long long)b * p.T + row + at.p) * p.E + e;
+            if (EMIT) {
+                sum_to_lanes<P, BATCH>(y, at.p);
 #pragma unroll
-            for (int i = 0; i < OWN; ++i) {
-                float v = fmaf(skip, to_f32(raw.u[i]), y[i * P]);
-                if (p.z) {
-                    const float z = to_f32(raw.z[i]);
-                    v *= z * sigmoid(z);
+                for (int i = 0; i < OWN; ++i) {
+                    float v = fmaf(skip, to_f32(raw.u[i]), y[i * P]);
+                    if (p.z) {
+                        const float z = to_f32(raw.z[i]);
+                        v *= z * sigmoid(z);
+                    }
+                    const int t = row + at.p + i * P;
+                    if (at.there && (!PART || (t >= first && t < behind))) at_row(out + (long long)i * P * p.E, place) = from_f32<IO>(v);
                 }
-                const int t = row + at.p + i * P;
-                if (t < from || t >= to) v = 0.f;
-                if (at.there && t < r1) out[(long long)i * P * p.E] = from_f32<IO>(v);
+            }
+        };
+        if (!EMIT) {
+            // (a segment's sum of step sizes is only read where one sequence goes through all of it: no token of such a one is left out)
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) total += row + at.p + i * P < r1 ? dt[i] : 0.f;
+        }
+        if (row >= from && row + BATCH <= to && w.within(row, BATCH)) piece(std::false_type(), 0, 0);
+        else {
+            if (EMIT && (row < from || row + BATCH > to)) {
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) {
+                    const int t = row + at.p + i * P;
+                    if (at.there && t < r1 && (t < from || t >= to)) at_row(out + (long long)i * P * p.E, place) = from_f32<IO>(0.f);
+                }
+            }
+            for (;;) {                                     // one sequence after the other
+                const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
+                if (first >= behind) break;
+                if (first == w.begin) first_state(w.n);
+                piece(std::true_type(), first, behind);
+                if (behind < w.end) break;
+                last_state(w.n);
+                w.next(p.seq);
             }
         }
         if (more) {

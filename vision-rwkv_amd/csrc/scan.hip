@@ -61,7 +61,7 @@ int check(const char* who, const vrwkv_scan_args* args, bool backward) {
     }
     if (a.N <= 0 || a.T <= 0 || a.E <= 0 || a.G <= 0) { set_error("%s: N, T, E and G must be positive", who); return VRWKV_INVALID_ARG; }
     if (!typed(a.dtype) || !typed(a.D_dtype) || !typed(a.bias_dtype)) { set_error("%s: dtype must be fp32, bf16 or fp16", who); return VRWKV_UNSUPPORTED_DTYPE; }
-    if (a.S < 1 || a.S > 64 || a.E % a.G) { set_error("%s: 1 to 64 states (%d), and E (%d) a multiple of G (%d)", who, a.S, a.E, a.G); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (a.S < 1 || a.S > 64 || a.E % a.G || a.E > 1 << 22 || a.G > 1 << 16) { set_error("%s: 1 to 64 states (%d), E (%d, at most 2^22) a multiple of G (%d, at most 2^16)", who, a.S, a.E, a.G); return VRWKV_UNSUPPORTED_SHAPE; }
     const long long strides[] = {a.u_stride[1], a.delta_stride[1], a.z_stride[1], backward ? a.gy_stride[1] : 0, a.B_stride[1], a.C_stride[1]};
     for (long long s : strides)
         if (s < 0 || s >= 1LL << 22) { set_error("%s: tokens must be less than 2^22 elements apart", who); return VRWKV_UNSUPPORTED_SHAPE; }

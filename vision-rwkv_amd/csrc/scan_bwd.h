@@ -76,9 +76,9 @@ __global__ __launch_bounds__(THREADS) void back_segments_kernel(const BackParams
     const float bias = p.bias.p ? p.bias.value(p.bias.fetch(e)) : 0.f;
     Rows<IO, P> raw, ahead;
     const auto fetch = [&](Rows<IO, P>& x, int row) {
-        x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row + at.p, r1, e);
-        x.fetch(x.g, bp.gy, b * bp.gy_b, bp.gy_t, row + at.p, r1, e);
-        if (p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row + at.p, r1, e);
+        x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
+        x.fetch(x.g, bp.gy, b * bp.gy_b, bp.gy_t, row, r1, at.p, e);
+        if (p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row, r1, at.p, e);
     };
     Stage<IO, P, 2> stage;
     const int last = r0 + (r1 - 1 - r0) / BATCH * BATCH;
@@ -106,29 +106,32 @@ __global__ __launch_bounds__(THREADS) void back_segments_kernel(const BackParams
             }
             total += row + at.p + i * P < r1 ? dt[i] : 0.f;
         }
-        const auto token = [&](auto j_) {
-            constexpr int j = BATCH - 1 - decltype(j_)::value;
-            const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(g[j / P]);
-            const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * 8 * P + 4 * P + 4 * at.p]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) R[k] = fast_exp2(d * a2[k]) * fmaf(Ct[k], v, R[k]);
-        };
-        if (row >= from && row + BATCH <= to && w.within(row, BATCH)) each(std::make_integer_sequence<int, BATCH>(), token);
-        else
+        const auto piece = [&](auto part_, int first, int behind) {
+            constexpr bool PART = decltype(part_)::value;
             each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
                 constexpr int j = BATCH - 1 - decltype(j_)::value;
-                if (row + j < from || row + j >= to) return;
-                if (row + j == w.end - 1) {
+                if (PART && (row + j < first || row + j >= behind)) return;
+                const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(g[j / P]);
+                const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * 8 * P + 4 * P + 4 * at.p]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) R[k] = fast_exp2(d * a2[k]) * fmaf(Ct[k], v, R[k]);
+            });
+        };
+        if (row >= from && row + BATCH <= to && w.within(row, BATCH)) piece(std::false_type(), 0, 0);
+        else
+            for (;;) {                                     // one sequence in front of the other
+                const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
+                if (first >= behind) break;
+                if (behind == w.end) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) R[k] = bp.glast && (FULL || 4 * at.p + k < p.S) ? bp.glast[((long long)w.n * p.E + e) * p.S + 4 * at.p + k] : 0.f;
                 }
-                token(j_);
-                if (row + j == w.begin) {
+                piece(std::true_type(), first, behind);
+                if (first > w.begin) break;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) R[k] = 0.f;
-                    w.previous(p.seq);
-                }
-            });
+                for (int k = 0; k < 4; ++k) R[k] = 0.f;
+                w.previous(p.seq);
+            }
         if (more) {
             stage.put(bc[buf ^ 1]);
             raw = ahead;
@@ -201,17 +204,18 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
         Rows<IO, P> raw, ahead;
         f32x4 kept, kept_ahead;
         const auto fetch = [&](Rows<IO, P>& x, f32x4& h, int row) {
-            x.fetch(x.u, p.u, b * p.u_b, p.u_t, row + at.p, r1, e);
-            x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row + at.p, r1, e);
-            x.fetch(x.g, bp.gy, b * bp.gy_b, bp.gy_t, row + at.p, r1, e);
-            if (p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row + at.p, r1, e);
-            h = *reinterpret_cast<const f32x4*>(p.kept + (((long long)b * chunks + row / BATCH) * p.E + e) * 4 * P + 4 * at.p);
+            x.fetch(x.u, p.u, b * p.u_b, p.u_t, row, r1, at.p, e);
+            x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
+            x.fetch(x.g, bp.gy, b * bp.gy_b, bp.gy_t, row, r1, at.p, e);
+            if (p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row, r1, at.p, e);
+            h = at_row(reinterpret_cast<const f32x4*>(p.kept) + ((long long)b * chunks + row / BATCH) * p.E * P, (unsigned)(e * P + at.p) * 16u);
         };
         Stage<IO, P, 2> stage;
         fetch(raw, kept, last);
         stage.fetch(p, b, at.g, last, from, to);
         stage.put(bc[0]);
         lds_barrier();
+        const float* const part_row = bp.part_bc + (((long long)(blockIdx.x % p.blocks) * p.rows + b) * p.T * p.G + at.g) * ROW;
         int buf = 0;
         for (int row = last; row >= r0; row -= BATCH, buf ^= 1) {
             const bool more = row > r0;
@@ -224,135 +228,143 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
             for (int i = 0; i < OWN; ++i) {
                 const float d = to_f32(raw.d[i]) + bias;
                 dt[i] = p.softplus ? softplus(d) : d;
-                x[i] = dt[i] * to_f32(raw.u[i]);
-                g[i] = to_f32(raw.g[i]);
-                if (p.z) {
+                x[i] = at.there ? dt[i] * to_f32(raw.u[i]) : 0.f;   // (a channel that is not there adds nothing to dB and dC)
+                g[i] = at.there ? to_f32(raw.g[i]) : 0.f;
+                if (p.z && at.there) {
                     const float z = to_f32(raw.z[i]);
                     g[i] *= z * sigmoid(z);
                 }
             }
-            const bool clean = row >= from && row + BATCH <= to && w.within(row, BATCH);
-            float hs[BATCH + 1][4], y[BATCH];              // hs[j]: the state in front of token j, but where a sequence begins there
+            const long long out = ((long long)b * p.T + row) * p.E;
+            const unsigned place = (at.p * (unsigned)p.E + e) * sizeof(IO);
+            const auto put = [&](void* t, int token, float v) { at_row(static_cast<const IO*>(t) + out + (long long)token * p.E, place) = from_f32<IO>(v); };
+            // tokens [first, behind) of the sixteen, all of one sequence, from the state h in front of them; PART: not all sixteen
+            const auto piece = [&](auto part_, int first, int behind, const float (&h)[4]) {
+                constexpr bool PART = decltype(part_)::value;
+                const auto outside = [&](int j) { return PART && (row + j < first || row + j >= behind); };
+                float hs[BATCH + 1][4];                    // hs[j]: the state in front of token j
 #pragma unroll
-            for (int k = 0; k < 4; ++k) hs[0][k] = kept[k];
-            const auto along = [&](auto j_, const float (&h)[4]) {
-                constexpr int j = decltype(j_)::value;
-                const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]);
-                const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * P + 4 * at.p]);
+                for (int k = 0; k < 4; ++k) hs[0][k] = h[k];
+                {
+                    float y[BATCH];
+                    each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
+                        constexpr int j = decltype(j_)::value;
+                        y[j] = 0.f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    hs[j + 1][k] = fmaf(fast_exp2(d * a2[k]), h[k], v * Bt[k]);
-                    if (!FULL && pad[k]) hs[j + 1][k] = 0.f;
-                }
-                y[j] = fmaf(Ct[3], hs[j + 1][3], fmaf(Ct[2], hs[j + 1][2], fmaf(Ct[1], hs[j + 1][1], Ct[0] * hs[j + 1][0])));
-            };
-            if (clean) each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) { along(j_, hs[decltype(j_)::value]); });
-            else {
-                Walk f;
-                f.find(p.seq, b, max(row, from), at.lane);
-                each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
-                    constexpr int j = decltype(j_)::value;
-                    y[j] = 0.f;
+                        for (int k = 0; k < 4; ++k) hs[j + 1][k] = hs[j][k];
+                        if (outside(j)) return;
+                        const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]);
+                        const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * P + 4 * at.p]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) hs[j + 1][k] = hs[j][k];
-                    if (row + j < from || row + j >= to) return;
-                    float h[4];
+                        for (int k = 0; k < 4; ++k) {
+                            hs[j + 1][k] = fmaf(fast_exp2(d * a2[k]), hs[j][k], v * Bt[k]);
+                            if (!FULL && pad[k]) hs[j + 1][k] = 0.f;
+                        }
+                        y[j] = fmaf(Ct[3], hs[j + 1][3], fmaf(Ct[2], hs[j + 1][2], fmaf(Ct[1], hs[j + 1][1], Ct[0] * hs[j + 1][0])));
+                        asm volatile("" : "+v"(y[j]));     // (else it is made where z is looked at, from what had to wait in registers)
+                        if (!PART && j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    });
+                    if (p.z) {
+                        sum_to_lanes<P, BATCH>(y, at.p);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) h[k] = hs[j][k];
-                    if (row + j == f.begin) state_of(p.state, f.n, h);
-                    along(j_, h);
-                    if (row + j == f.end - 1) f.next(p.seq);
-                });
-            }
-            if (p.z) {
-                sum_to_lanes<P, BATCH>(y, at.p);
-                IO* out = static_cast<IO*>(bp.dz) + ((long long)b * p.T + row + at.p) * p.E + e;
-#pragma unroll
-                for (int i = 0; i < OWN; ++i) {
-                    const float z = to_f32(raw.z[i]), sg = sigmoid(z), inner = fmaf(skip, to_f32(raw.u[i]), y[i * P]);
-                    const int t = row + at.p + i * P;
-                    const float v = t >= from && t < to ? to_f32(raw.g[i]) * inner * (sg * fmaf(z, 1.f - sg, 1.f)) : 0.f;
-                    if (at.there && t < r1) out[(long long)i * P * p.E] = from_f32<IO>(v);
-                }
-            }
-            float along_B[BATCH], along_A[BATCH], sums[COUNT];
-            const auto back = [&](auto j_, const float (&before)[4], bool inside) {
-                constexpr int j = decltype(j_)::value;
-                const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]), gj = from_lane<P, j % P>(g[j / P]);
-                const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * P + 4 * at.p]);
-                float dB[4], dC[4];
-                along_A[j] = along_B[j] = 0.f;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (inside) {
-                        const float r = fmaf(Ct[k], gj, R[k]);
-                        dB[k] = at.there ? r * v : 0.f;
-                        dC[k] = at.there ? gj * hs[j + 1][k] : 0.f;
-                        along_B[j] = fmaf(r, Bt[k], along_B[j]);
-                        R[k] = fast_exp2(d * a2[k]) * r;
-                        const float q = R[k] * before[k];
-                        along_A[j] = fmaf(q, a2[k], along_A[j]);
-                        dA[k] = fmaf(q, d, dA[k]);
-                    } else dB[k] = dC[k] = 0.f;
-                }
-                if constexpr (P == 16) {
-                    sum_over_channels<P, COUNT>(dB, at.lane);
-                    sum_over_channels<P, COUNT>(dC, at.lane);
-                    red[buf % BUFS][wave][j * ROW + leave] = dB[0];
-                    red[buf % BUFS][wave][j * ROW + 4 * P + leave] = dC[0];
-                } else {
-                    constexpr int GROUP = COUNT / 8;       // tokens whose sums go through the wave together
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        sums[j % GROUP * 8 + k] = dB[k];
-                        sums[j % GROUP * 8 + 4 + k] = dC[k];
-                    }
-                    if constexpr (j % GROUP == 0) {
-                        sum_over_channels<P, COUNT>(sums, at.lane);
-                        red[buf % BUFS][wave][j * ROW + leave] = sums[0];
+                        for (int i = 0; i < OWN; ++i) {
+                            const float z = to_f32(raw.z[i]), sg = sigmoid(z), inner = fmaf(skip, to_f32(raw.u[i]), y[i * P]);
+                            if (at.there && !outside(at.p + i * P)) put(bp.dz, i * P, to_f32(raw.g[i]) * inner * (sg * fmaf(z, 1.f - sg, 1.f)));
+                        }
                     }
                 }
-            };
-            if (clean)
+                // (the exponentials are taken and B and C read again: kept, they would fill three times as many registers as the states)
+                int again = at.p;
+                asm volatile("" : "+v"(again));
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) asm volatile("" : "+v"(dt[i]));
+                float along_B[P], along_A[P], sums[COUNT];
                 each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
                     constexpr int j = BATCH - 1 - decltype(j_)::value;
-                    back(std::integral_constant<int, j>(), hs[j], true);
-                });
-            else
-                each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
-                    constexpr int j = BATCH - 1 - decltype(j_)::value;
-                    const bool inside = row + j >= from && row + j < to;
-                    float before[4];
+                    along_A[j % P] = along_B[j % P] = 0.f;
+                    float dB[4] = {0.f, 0.f, 0.f, 0.f}, dC[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (!outside(j)) {
+                        const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]), gj = from_lane<P, j % P>(g[j / P]);
+                        const f32x4 Bt = reinterpret_cast<const f32x4*>(bc[buf])[j * 2 * P + again], Ct = reinterpret_cast<const f32x4*>(bc[buf])[j * 2 * P + P + again];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) before[k] = hs[j][k];
-                    if (inside && row + j == w.end - 1) state_of(bp.glast, w.n, R);
-                    if (inside && row + j == w.begin) state_of(p.state, w.n, before);
-                    back(std::integral_constant<int, j>(), before, inside);
-                    if (inside && row + j == w.begin) {
-                        first_gradient(w.n, R);
+                        for (int k = 0; k < 4; ++k) {
+                            const float r = fmaf(Ct[k], gj, R[k]);
+                            dB[k] = r * v;
+                            dC[k] = gj * hs[j + 1][k];
+                            along_B[j % P] = fmaf(r, Bt[k], along_B[j % P]);
+                            R[k] = fast_exp2(d * a2[k]) * r;
+                            const float q = R[k] * hs[j][k];
+                            along_A[j % P] = fmaf(q, a2[k], along_A[j % P]);
+                            dA[k] = fmaf(q, d, dA[k]);
+                        }
+                    }
+                    if constexpr (P == 16) {
+                        sum_over_channels<P, COUNT>(dB, at.lane);
+                        sum_over_channels<P, COUNT>(dC, at.lane);
+                        if (!outside(j)) {
+                            red[buf % BUFS][wave][j * ROW + leave] = dB[0];
+                            red[buf % BUFS][wave][j * ROW + 4 * P + leave] = dC[0];
+                        }
+                    } else {
+                        constexpr int GROUP = COUNT / 8;   // tokens whose sums go through the wave together
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) R[k] = 0.f;
-                        w.previous(p.seq);
+                        for (int k = 0; k < 4; ++k) {
+                            sums[j % GROUP * 8 + k] = dB[k];
+                            sums[j % GROUP * 8 + 4 + k] = dC[k];
+                        }
+                        if constexpr (j % GROUP == 0) {
+                            sum_over_channels<P, COUNT>(sums, at.lane);
+                            if (!outside(j + sum / 8)) red[buf % BUFS][wave][j * ROW + leave] = sums[0];
+                        }
+                    }
+                    // (else the compiler puts the additions to dA off to the end of the sixteen tokens, with all that they add up)
+                    if (j % 2 == 0) asm volatile("" : "+v"(dA[0]), "+v"(dA[1]), "+v"(dA[2]), "+v"(dA[3]));
+                    if (!PART && j % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (j % P == 0) {
+                        constexpr int i = j / P;
+                        sum_to_lanes<P, P>(along_A, at.p);
+                        sum_to_lanes<P, P>(along_B, at.p);
+                        const float u = to_f32(raw.u[i]);
+                        float a = fmaf(along_A[0], 1.f / LOG2E, u * along_B[0]);
+                        if (p.softplus) a *= sigmoid(to_f32(raw.d[i]) + bias);
+                        if (!outside(at.p + j)) {
+                            dD = fmaf(g[i], u, dD);
+                            dbias += a;
+                            if (at.there) {
+                                put(bp.du, j, fmaf(dt[i], along_B[0], skip * g[i]));
+                                put(bp.dd, j, a);
+                            }
+                        }
                     }
                 });
-            sum_to_lanes<P, BATCH>(along_A, at.p);
-            sum_to_lanes<P, BATCH>(along_B, at.p);
-            IO* const du = static_cast<IO*>(bp.du) + ((long long)b * p.T + row + at.p) * p.E + e;
-            IO* const dd = static_cast<IO*>(bp.dd) + ((long long)b * p.T + row + at.p) * p.E + e;
+            };
+            if (row >= from && row + BATCH <= to && w.within(row, BATCH)) {
+                const float h[4] = {kept[0], kept[1], kept[2], kept[3]};
+                piece(std::false_type(), 0, 0, h);
+            } else {
+                if (row < from || row + BATCH > to) {
 #pragma unroll
-            for (int i = 0; i < OWN; ++i) {
-                const float u = to_f32(raw.u[i]);
-                const int t = row + at.p + i * P;
-                const bool inside = t >= from && t < to;
-                float a = fmaf(along_A[i * P], 1.f / LOG2E, u * along_B[i * P]);
-                if (p.softplus) a *= sigmoid(to_f32(raw.d[i]) + bias);
-                if (inside) {
-                    dD = fmaf(g[i], u, dD);
-                    dbias += a;
+                    for (int i = 0; i < OWN; ++i) {
+                        const int t = row + at.p + i * P;
+                        if (at.there && t < r1 && (t < from || t >= to)) {
+                            put(bp.du, i * P, 0.f);
+                            put(bp.dd, i * P, 0.f);
+                            if (p.z) put(bp.dz, i * P, 0.f);
+                        }
+                    }
                 }
-                if (at.there && t < r1) {
-                    du[(long long)i * P * p.E] = from_f32<IO>(inside ? fmaf(dt[i], along_B[i * P], skip * g[i]) : 0.f);
-                    dd[(long long)i * P * p.E] = from_f32<IO>(inside ? a : 0.f);
+                for (;;) {                                 // one sequence in front of the other
+                    const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
+                    if (first >= behind) break;
+                    float h[4] = {kept[0], kept[1], kept[2], kept[3]};
+                    if (behind == w.end) state_of(bp.glast, w.n, R);
+                    if (first == w.begin) state_of(p.state, w.n, h);
+                    piece(std::true_type(), first, behind, h);
+                    if (first > w.begin) break;
+                    first_gradient(w.n, R);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) R[k] = 0.f;
+                    w.previous(p.seq);
                 }
             }
             if (more) {
@@ -361,13 +373,12 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                 kept = kept_ahead;
             }
             lds_barrier();
-#pragma unroll
             for (int i = threadIdx.x; i < SUMS; i += THREADS) {
                 const int t = row + i / ROW;
                 float v = 0.f;
 #pragma unroll
                 for (int q = 0; q < THREADS / WAVE; ++q) v += red[buf % BUFS][q][i];
-                if (t < r1) bp.part_bc[((((long long)(blockIdx.x % p.blocks) * p.rows + b) * p.T + t) * p.G + at.g) * ROW + i % ROW] = t >= from && t < to ? v : 0.f;
+                if (t < r1) at_row(part_row + (long long)row * p.G * ROW, (i / ROW * (unsigned)p.G * ROW + i % ROW) * 4u) = t >= from && t < to ? v : 0.f;
             }
             if (BUFS == 1) lds_barrier();
         }
