@@ -77,8 +77,10 @@ struct Rows {
         const IO* x = static_cast<const IO*>(t) + base + row * stride;
         if (row + BATCH <= end) {
             const unsigned place = (q * (unsigned)stride + e) * sizeof(IO);
+            int step = P * (int)stride;                    // (its multiples are not kept either: scalar registers run out)
+            asm volatile("" : "+s"(step));
 #pragma unroll
-            for (int i = 0; i < OWN; ++i) to[i] = at_row(x + i * P * stride, place);
+            for (int i = 0; i < OWN; ++i, x += step) to[i] = at_row(x, place);
         } else {
             asm volatile("" : "+v"(q));                    // (nothing of this is kept for other rows)
 #pragma unroll
@@ -118,7 +120,7 @@ __device__ __forceinline__ void each(std::integer_sequence<int, I...>, F&& f) { 
 // EMIT: the outputs of a segment from the states in front of it; without, its last states from zeros (or from its sequence's first states) and its sum of step sizes.
 // FULL: S is 4 P, so that no state is there to fill up.
 template <typename IO, int P, bool FULL, bool EMIT>
-__global__ __launch_bounds__(THREADS) void scan_kernel(const Params p) {
+__global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Params p) {
     constexpr int OWN = BATCH / P, WHICH = EMIT ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float bc[2][BATCH * WHICH * 4 * P];
     const Place<P> at(p.E, p.G, p.blocks);
@@ -182,54 +184,52 @@ __global__ __launch_bounds__(THREADS) void scan_kernel(const Params p) {
         }
         if (EMIT && p.kept && at.there)
             at_row(reinterpret_cast<const f32x4*>(p.kept) + ((long long)b * ((p.T + BATCH - 1) / BATCH) + row / BATCH) * p.E * P, (unsigned)(e * P + at.p) * 16u) = f32x4{h[0], h[1], h[2], h[3]};
-        float dt[OWN], x[OWN];
-#pragma unroll
-        for (int i = 0; i < OWN; ++i) {
-            const float d = to_f32(raw.d[i]) + bias;
-            dt[i] = p.softplus ? softplus(d) : d;
-            x[i] = dt[i] * to_f32(raw.u[i]);
-        }
         const IO* const out = static_cast<const IO*>(p.y) + ((long long)b * p.T + row) * p.E;
         const unsigned place = (at.p * (unsigned)p.E + e) * sizeof(IO);
-        // tokens [first, behind) of the sixteen, all of one sequence; PART: not all sixteen
+        int width = p.E;
+        asm volatile("" : "+s"(width));
+        // tokens [first, behind) of the sixteen, all of one sequence; PART: not all sixteen.  P at a time: each lane's own, then the states of all, then each lane's own again
         const auto piece = [&](auto part_, int first, int behind) {
             constexpr bool PART = decltype(part_)::value;
-            float y[BATCH];
-            each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
-                constexpr int j = decltype(j_)::value;
-                y[j] = 0.f;
-                if (PART && (row + j < first || row + j >= behind)) return;
-                const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]);
-                const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * at.p]);
+            each(std::make_integer_sequence<int, OWN>(), [&](auto i_) {
+                constexpr int i = decltype(i_)::value;
+                const float raw_d = to_f32(raw.d[i]) + bias, u = to_f32(raw.u[i]), dt = p.softplus ? softplus(raw_d) : raw_d, x = dt * u;
+                const int mine = row + at.p + i * P;
+                float y[P];
+                each(std::make_integer_sequence<int, P>(), [&](auto q_) {
+                    constexpr int q = decltype(q_)::value, j = i * P + q;
+                    y[q] = 0.f;
+                    if (PART && (row + j < first || row + j >= behind)) return;
+                    const float d = from_lane<P, q>(dt), v = from_lane<P, q>(x);
+                    const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * at.p]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    h[k] = fmaf(fast_exp2(d * a2[k]), h[k], v * Bt[k]);
-                    if (!FULL && pad[k]) h[k] = 0.f;       // (an infinite v would make it NaN)
-                }
+                    for (int k = 0; k < 4; ++k) {
+                        h[k] = fmaf(fast_exp2(d * a2[k]), h[k], v * Bt[k]);
+                        if (!FULL && pad[k]) h[k] = 0.f;   // (an infinite v would make it NaN)
+                    }
+                    if (EMIT) {
+                        const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * P + 4 * at.p]);
+                        y[q] = fmaf(Ct[3], h[3], fmaf(Ct[2], h[2], fmaf(Ct[1], h[1], Ct[0] * h[0])));
+                    }
+                });
+                // (a segment's sum of step sizes is only read where one sequence goes through all of it: no token of such a one is left out)
+                if (!EMIT) total += !PART || mine < r1 ? dt : 0.f;
                 if (EMIT) {
-                    const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * P + 4 * at.p]);
-                    y[j] = fmaf(Ct[3], h[3], fmaf(Ct[2], h[2], fmaf(Ct[1], h[1], Ct[0] * h[0])));
-                }
-            });
-            if (EMIT) {
-                sum_to_lanes<P, BATCH>(y, at.p);
-#pragma unroll
-                for (int i = 0; i < OWN; ++i) {
-                    float v = fmaf(skip, to_f32(raw.u[i]), y[i * P]);
+                    sum_to_lanes<P, P>(y, at.p);
+                    float v = fmaf(skip, u, y[0]);
                     if (p.z) {
                         const float z = to_f32(raw.z[i]);
                         v *= z * sigmoid(z);
                     }
-                    const int t = row + at.p + i * P;
-                    if (at.there && (!PART || (t >= first && t < behind))) at_row(out + (long long)i * P * p.E, place) = from_f32<IO>(v);
+                    if (at.there && (!PART || (mine >= first && mine < behind))) at_row(out + (long long)i * P * width, place) = from_f32<IO>(v);
                 }
-            }
+                // (else B and C of all sixteen are read ahead, or the states put off, in registers that other waves could have)
+                if ((i + 1) * P % 4 == 0) {
+                    if (!EMIT) asm volatile("" : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            });
         };
-        if (!EMIT) {
-            // (a segment's sum of step sizes is only read where one sequence goes through all of it: no token of such a one is left out)
-#pragma unroll
-            for (int i = 0; i < OWN; ++i) total += row + at.p + i * P < r1 ? dt[i] : 0.f;
-        }
         if (row >= from && row + BATCH <= to && w.within(row, BATCH)) piece(std::false_type(), 0, 0);
         else {
             if (EMIT && (row < from || row + BATCH > to)) {

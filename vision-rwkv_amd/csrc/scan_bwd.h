@@ -5,7 +5,7 @@
 //
 // Sixteen tokens at a time, the last first: their states again from the one that the forward has kept in front of them, in registers, then back along them.  P lanes hold one channel,
 // four states each, as in the forward.  dB and dC add up channels, which lie in other lanes: the sums of two tokens go through the wave in halves
-// (lane swaps and additions, two instructions for a sum of 64 / P lanes), then through LDS over the waves, and over workgroups by the launch that ends the pass.
+// (two instructions for a sum of 64 / P lanes), then through LDS over the waves, and over workgroups by the launch that ends the pass.
 #pragma once
 #include "scan.h"
 
@@ -22,40 +22,84 @@ struct BackParams {
     long long gy_b, gy_t;
 };
 
-// Sums over the lanes of a wave that differ above the channel's P: v[i] of the 64 / P channels to the lane of channel i.
-template <int P, int COUNT, int BIT = 32>
-__device__ __forceinline__ void sum_over_channels(float (&v)[COUNT], int lane) {
-    if constexpr (BIT >= P) {
-        constexpr int HALF = BIT / P;
-        static_assert(COUNT == 64 / P, "one sum for each channel of the wave");
+// Sums over the lanes of a wave that differ above the channel's P: of v[0 .. 64 / P) of all channels, one is left in each lane of v[0], the one that sum_of_lane says.  At each step
+// a lane keeps one half of its sums and gets the other lanes' parts of it.  Lanes of a row of sixteen first, in additions that read one lane and write another (4.4 cycles each,
+// measured; two make a pair of sums), then rows, whose swap takes 10.
+template <int HALF>
+__device__ __forceinline__ void fold8(float* v) {          // (written out: the instruction's bank mask picks the half; two wait states in front of and behind reads across lanes)
+    if constexpr (HALF == 8)
+        asm("s_nop 1\n"
+#define FOLD(a, b) "v_add_f32_dpp %" #a ", %" #a ", %" #a " row_ror:8 row_mask:0xf bank_mask:0x3\n v_add_f32_dpp %" #a ", %" #b ", %" #b " row_ror:8 row_mask:0xf bank_mask:0xc\n"
+            FOLD(0, 8) FOLD(1, 9) FOLD(2, 10) FOLD(3, 11) FOLD(4, 12) FOLD(5, 13) FOLD(6, 14) FOLD(7, 15) "s_nop 1"
+            : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7])
+            : "v"(v[8]), "v"(v[9]), "v"(v[10]), "v"(v[11]), "v"(v[12]), "v"(v[13]), "v"(v[14]), "v"(v[15]));
+    else
 #pragma unroll
-        for (int i = 0; i < HALF; ++i) {
-            float a = v[i], b = v[i + HALF];
-            if constexpr (BIT >= 16) {
-                const auto x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
-                // (the elements are copied first: a bit cast of one as it stands takes the vector's first)
-                const auto r = [&] {
-                    if constexpr (BIT == 32) return __builtin_amdgcn_permlane32_swap(x, y, false, false);
-                    else return __builtin_amdgcn_permlane16_swap(x, y, false, false);
-                }();
-                const unsigned low = r[0], high = r[1];
-                v[i] = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
-            } else if constexpr (BIT == 8) {
-                a += dpp<0x128>(a);                        // row_ror:8
-                b += dpp<0x128>(b);
-                v[i] = lane & 8 ? b : a;
-            } else if constexpr (BIT == 4) {
-                a += dpp<0x104>(a);                        // row_shl:4: the lane four above, for the lower of the two
-                b += dpp<0x114>(b);                        // row_shr:4
-                v[i] = lane & 4 ? b : a;
-            } else {
-                a += across<BIT>(a);
-                b += across<BIT>(b);
-                v[i] = lane & BIT ? b : a;
+        for (int i = 0; i < HALF; i += 4)
+            asm("s_nop 1\n" FOLD(0, 4) FOLD(1, 5) FOLD(2, 6) FOLD(3, 7) "s_nop 1"
+#undef FOLD
+                : "+v"(v[i]), "+v"(v[i + 1]), "+v"(v[i + 2]), "+v"(v[i + 3])
+                : "v"(v[i + HALF]), "v"(v[i + HALF + 1]), "v"(v[i + HALF + 2]), "v"(v[i + HALF + 3]));
+}
+template <int HALF>
+__device__ __forceinline__ void fold4(float* v) {
+#pragma unroll
+    for (int i = 0; i < HALF; i += 4)
+        asm("s_nop 1\n"
+#define FOLD(a, b) "v_add_f32_dpp %" #a ", %" #a ", %" #a " row_shl:4 row_mask:0xf bank_mask:0x5\n v_add_f32_dpp %" #a ", %" #b ", %" #b " row_shr:4 row_mask:0xf bank_mask:0xa\n"
+            FOLD(0, 4) FOLD(1, 5) FOLD(2, 6) FOLD(3, 7) "s_nop 1"
+#undef FOLD
+            : "+v"(v[i]), "+v"(v[i + 1]), "+v"(v[i + 2]), "+v"(v[i + 3])
+            : "v"(v[i + HALF]), "v"(v[i + HALF + 1]), "v"(v[i + HALF + 2]), "v"(v[i + HALF + 3]));
+}
+template <int HALF, bool ROWS>
+__device__ __forceinline__ void fold_rows(float* v) {
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) {
+        const auto x = __builtin_bit_cast(unsigned, v[i]), y = __builtin_bit_cast(unsigned, v[i + HALF]);
+        // (the elements are copied first: a bit cast of one as it stands takes the vector's first)
+        const auto r = [&] {
+            if constexpr (ROWS) return __builtin_amdgcn_permlane32_swap(x, y, false, false);
+            else return __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        }();
+        const unsigned low = r[0], high = r[1];
+        v[i] = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
+    }
+}
+template <int P>
+__device__ __forceinline__ void sum_over_channels(float (&v)[64 / P], int lane) {
+    constexpr int N = 64 / P;
+    if constexpr (P <= 4) {
+        fold8<N / 2>(v);
+        fold4<N / 4>(v);
+        fold_rows<N / 8, true>(v);
+        fold_rows<N / 16, false>(v);
+        if constexpr (P <= 2) {
+#pragma unroll
+            for (int i = 0; i < N / 32; ++i) {
+                const float a = v[i] + across<2>(v[i]), b = v[i + N / 32] + across<2>(v[i + N / 32]);
+                v[i] = lane & 2 ? b : a;
             }
         }
-        sum_over_channels<P, COUNT, BIT / 2>(v, lane);
+        if constexpr (P == 1) {
+            const float a = v[0] + across<1>(v[0]), b = v[1] + across<1>(v[1]);
+            v[0] = lane & 1 ? b : a;
+        }
+    } else if constexpr (P == 8) {
+        fold8<4>(v);
+        fold_rows<2, true>(v);
+        fold_rows<1, false>(v);
+    } else {
+        fold_rows<2, true>(v);
+        fold_rows<1, false>(v);
     }
+}
+template <int P>
+__device__ __forceinline__ int sum_of_lane(int lane) {
+    const int rows = (lane >> 5 & 1) * 2 + (lane >> 4 & 1);  // the lanes' bits in the order of the steps
+    if constexpr (P == 16) return rows;
+    else if constexpr (P == 8) return (lane >> 3 & 1) * 4 + rows;
+    else return ((lane >> 3 & 1) * 8 + (lane >> 2 & 1) * 4 + rows) * (4 / P) + (P == 4 ? 0 : P == 2 ? lane >> 1 & 1 : (lane >> 1 & 1) * 2 + (lane & 1));
 }
 
 // The gradient that each segment behind the first hands on, from zeros behind it (or from its sequence's end), and its sum of step sizes.
@@ -151,9 +195,9 @@ __global__ __launch_bounds__(THREADS) void back_segments_kernel(const BackParams
 template <typename IO, int P, bool FULL>
 __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
     const Params& p = bp.f;
-    constexpr int OWN = BATCH / P, COUNT = 64 / P, ROW = 8 * P, SUMS = BATCH * ROW, BUFS = P == 16 ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) float bc[2][SUMS];
-    __shared__ float red[BUFS][THREADS / WAVE][SUMS];
+    constexpr int OWN = BATCH / P, COUNT = 64 / P, ROW = 8 * P, SUMS = BATCH * ROW, WAVES = THREADS / WAVE;
+    __shared__ __attribute__((aligned(16))) float bc[SUMS];
+    __shared__ float red[WAVES][SUMS];
     const Place<P> at(p.E, p.G, p.blocks);
     const int s = blockIdx.y, r0 = s * p.L, r1 = min(p.T, r0 + p.L), e = at.e, wave = threadIdx.x >> 6;
     const long long part = (long long)blockIdx.z * p.nseg + s;
@@ -178,11 +222,10 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
             if (!pad[k]) bp.dstate[((long long)n * p.E + e) * p.S + 4 * at.p + k] = h[k];
     };
     const int last = r0 + (r1 - 1 - r0) / BATCH * BATCH, chunks = (p.T + BATCH - 1) / BATCH;
-    // where a lane leaves the sum that it is left with: of token lane / P / 8 of a group (all of one where P is 16), B's or C's, state 4 p + lane / P % 4
-    const int sum = at.lane / P, leave = P == 16 ? 4 * at.p + sum : sum / 8 * ROW + sum / 4 % 2 * 4 * P + 4 * at.p + sum % 4;
+    // where a lane leaves the sum that it is left with: of token sum / 8 of a group (all of one where P is 16), B's or C's, state 4 p + sum % 4
+    const int sum = sum_of_lane<P>(at.lane), leave = P == 16 ? 4 * at.p + sum : sum / 8 * ROW + sum / 4 % 2 * 4 * P + 4 * at.p + sum % 4;
 
     for (int b = blockIdx.z; b < p.rows; b += gridDim.z) {
-        if (b != (int)blockIdx.z) lds_barrier();           // (the last row's sums are read)
         Walk w;
         w.find(p.seq, b, max(from, to - 1), at.lane);
         float R[4] = {0.f, 0.f, 0.f, 0.f};
@@ -201,43 +244,44 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                 for (int i = 0; i < 4; ++i) R[i] = decayed(R[i], dt, a2[i]) + x[i];
             }
         }
-        Rows<IO, P> raw, ahead;
-        f32x4 kept, kept_ahead;
-        const auto fetch = [&](Rows<IO, P>& x, f32x4& h, int row) {
-            x.fetch(x.u, p.u, b * p.u_b, p.u_t, row, r1, at.p, e);
-            x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
-            x.fetch(x.g, bp.gy, b * bp.gy_b, bp.gy_t, row, r1, at.p, e);
-            if (p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row, r1, at.p, e);
-            h = at_row(reinterpret_cast<const f32x4*>(p.kept) + ((long long)b * chunks + row / BATCH) * p.E * P, (unsigned)(e * P + at.p) * 16u);
-        };
+        // sixteen tokens' rows and their first state: asked for while the sums of those behind them are added up
+        Rows<IO, P> raw;
+        f32x4 kept;
         Stage<IO, P, 2> stage;
-        fetch(raw, kept, last);
-        stage.fetch(p, b, at.g, last, from, to);
-        stage.put(bc[0]);
+        const auto fetch = [&](int row) {
+            raw.fetch(raw.u, p.u, b * p.u_b, p.u_t, row, r1, at.p, e);
+            raw.fetch(raw.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
+            raw.fetch(raw.g, bp.gy, b * bp.gy_b, bp.gy_t, row, r1, at.p, e);
+            if (p.z) raw.fetch(raw.z, p.z, b * p.z_b, p.z_t, row, r1, at.p, e);
+            kept = at_row(reinterpret_cast<const f32x4*>(p.kept) + ((long long)b * chunks + row / BATCH) * p.E * P, (unsigned)(e * P + at.p) * 16u);
+            stage.fetch(p, b, at.g, row, from, to);
+        };
+        fetch(last);
+        stage.put(bc);
         lds_barrier();
         const float* const part_row = bp.part_bc + (((long long)(blockIdx.x % p.blocks) * p.rows + b) * p.T * p.G + at.g) * ROW;
-        int buf = 0;
-        for (int row = last; row >= r0; row -= BATCH, buf ^= 1) {
+        for (int row = last; row >= r0; row -= BATCH) {
             const bool more = row > r0;
-            if (more) {
-                fetch(ahead, kept_ahead, row - BATCH);
-                stage.fetch(p, b, at.g, row - BATCH, from, to);
-            }
-            float dt[OWN], x[OWN], g[OWN];
+            // a lane's own tokens: step size and its slope, u, g, and gy silu'(z)
+            float dt[OWN], bend[OWN], u[OWN], g[OWN], gz[OWN];
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
                 const float d = to_f32(raw.d[i]) + bias;
                 dt[i] = p.softplus ? softplus(d) : d;
-                x[i] = at.there ? dt[i] * to_f32(raw.u[i]) : 0.f;   // (a channel that is not there adds nothing to dB and dC)
+                bend[i] = p.softplus ? sigmoid(d) : 1.f;
+                u[i] = at.there ? to_f32(raw.u[i]) : 0.f;  // (a channel that is not there adds nothing to dB and dC)
                 g[i] = at.there ? to_f32(raw.g[i]) : 0.f;
-                if (p.z && at.there) {
-                    const float z = to_f32(raw.z[i]);
-                    g[i] *= z * sigmoid(z);
+                if (p.z) {
+                    const float z = to_f32(raw.z[i]), sg = sigmoid(z);
+                    gz[i] = g[i] * (sg * fmaf(z, 1.f - sg, 1.f));
+                    if (at.there) g[i] *= z * sg;
                 }
             }
             const long long out = ((long long)b * p.T + row) * p.E;
             const unsigned place = (at.p * (unsigned)p.E + e) * sizeof(IO);
-            const auto put = [&](void* t, int token, float v) { at_row(static_cast<const IO*>(t) + out + (long long)token * p.E, place) = from_f32<IO>(v); };
+            int width = p.E;
+            asm volatile("" : "+s"(width));
+            const auto put = [&](void* t, int token, float v) { at_row(static_cast<const IO*>(t) + out + (long long)token * width, place) = from_f32<IO>(v); };
             // tokens [first, behind) of the sixteen, all of one sequence, from the state h in front of them; PART: not all sixteen
             const auto piece = [&](auto part_, int first, int behind, const float (&h)[4]) {
                 constexpr bool PART = decltype(part_)::value;
@@ -245,34 +289,30 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                 float hs[BATCH + 1][4];                    // hs[j]: the state in front of token j
 #pragma unroll
                 for (int k = 0; k < 4; ++k) hs[0][k] = h[k];
-                {
-                    float y[BATCH];
-                    each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
-                        constexpr int j = decltype(j_)::value;
-                        y[j] = 0.f;
+                each(std::make_integer_sequence<int, OWN>(), [&](auto i_) {
+                    constexpr int i = decltype(i_)::value;
+                    float y[P];
+                    each(std::make_integer_sequence<int, P>(), [&](auto q_) {
+                        constexpr int q = decltype(q_)::value, j = i * P + q;
+                        y[q] = 0.f;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) hs[j + 1][k] = hs[j][k];
                         if (outside(j)) return;
-                        const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]);
-                        const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * ROW + 4 * P + 4 * at.p]);
+                        const float d = from_lane<P, q>(dt[i]), v = from_lane<P, q>(dt[i] * u[i]);
+                        const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[j * ROW + 4 * P + 4 * at.p]);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             hs[j + 1][k] = fmaf(fast_exp2(d * a2[k]), hs[j][k], v * Bt[k]);
                             if (!FULL && pad[k]) hs[j + 1][k] = 0.f;
                         }
-                        y[j] = fmaf(Ct[3], hs[j + 1][3], fmaf(Ct[2], hs[j + 1][2], fmaf(Ct[1], hs[j + 1][1], Ct[0] * hs[j + 1][0])));
-                        asm volatile("" : "+v"(y[j]));     // (else it is made where z is looked at, from what had to wait in registers)
-                        if (!PART && j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                        y[q] = fmaf(Ct[3], hs[j + 1][3], fmaf(Ct[2], hs[j + 1][2], fmaf(Ct[1], hs[j + 1][1], Ct[0] * hs[j + 1][0])));
+                        asm volatile("" : "+v"(y[q]));     // (else it is made where z is looked at, from what had to wait in registers)
                     });
                     if (p.z) {
-                        sum_to_lanes<P, BATCH>(y, at.p);
-#pragma unroll
-                        for (int i = 0; i < OWN; ++i) {
-                            const float z = to_f32(raw.z[i]), sg = sigmoid(z), inner = fmaf(skip, to_f32(raw.u[i]), y[i * P]);
-                            if (at.there && !outside(at.p + i * P)) put(bp.dz, i * P, to_f32(raw.g[i]) * inner * (sg * fmaf(z, 1.f - sg, 1.f)));
-                        }
+                        sum_to_lanes<P, P>(y, at.p);
+                        if (at.there && !outside(at.p + i * P)) put(bp.dz, i * P, gz[i] * fmaf(skip, u[i], y[0]));
                     }
-                }
+                });
                 // (the exponentials are taken and B and C read again: kept, they would fill three times as many registers as the states)
                 int again = at.p;
                 asm volatile("" : "+v"(again));
@@ -284,8 +324,8 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                     along_A[j % P] = along_B[j % P] = 0.f;
                     float dB[4] = {0.f, 0.f, 0.f, 0.f}, dC[4] = {0.f, 0.f, 0.f, 0.f};
                     if (!outside(j)) {
-                        const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(x[j / P]), gj = from_lane<P, j % P>(g[j / P]);
-                        const f32x4 Bt = reinterpret_cast<const f32x4*>(bc[buf])[j * 2 * P + again], Ct = reinterpret_cast<const f32x4*>(bc[buf])[j * 2 * P + P + again];
+                        const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(dt[j / P] * u[j / P]), gj = from_lane<P, j % P>(g[j / P]);
+                        const f32x4 Bt = reinterpret_cast<const f32x4*>(bc)[j * 2 * P + again], Ct = reinterpret_cast<const f32x4*>(bc)[j * 2 * P + P + again];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const float r = fmaf(Ct[k], gj, R[k]);
@@ -299,11 +339,11 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                         }
                     }
                     if constexpr (P == 16) {
-                        sum_over_channels<P, COUNT>(dB, at.lane);
-                        sum_over_channels<P, COUNT>(dC, at.lane);
+                        sum_over_channels<P>(dB, at.lane);
+                        sum_over_channels<P>(dC, at.lane);
                         if (!outside(j)) {
-                            red[buf % BUFS][wave][j * ROW + leave] = dB[0];
-                            red[buf % BUFS][wave][j * ROW + 4 * P + leave] = dC[0];
+                            red[wave][j * ROW + leave] = dB[0];
+                            red[wave][j * ROW + 4 * P + leave] = dC[0];
                         }
                     } else {
                         constexpr int GROUP = COUNT / 8;   // tokens whose sums go through the wave together
@@ -313,22 +353,19 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                             sums[j % GROUP * 8 + 4 + k] = dC[k];
                         }
                         if constexpr (j % GROUP == 0) {
-                            sum_over_channels<P, COUNT>(sums, at.lane);
-                            if (!outside(j + sum / 8)) red[buf % BUFS][wave][j * ROW + leave] = sums[0];
+                            sum_over_channels<P>(sums, at.lane);
+                            if (!outside(j + sum / 8)) red[wave][j * ROW + leave] = sums[0];
                         }
                     }
                     // (else the compiler puts the additions to dA off to the end of the sixteen tokens, with all that they add up)
                     if (j % 2 == 0) asm volatile("" : "+v"(dA[0]), "+v"(dA[1]), "+v"(dA[2]), "+v"(dA[3]));
-                    if (!PART && j % 2 == 0) __builtin_amdgcn_sched_barrier(0);
                     if constexpr (j % P == 0) {
                         constexpr int i = j / P;
                         sum_to_lanes<P, P>(along_A, at.p);
                         sum_to_lanes<P, P>(along_B, at.p);
-                        const float u = to_f32(raw.u[i]);
-                        float a = fmaf(along_A[0], 1.f / LOG2E, u * along_B[0]);
-                        if (p.softplus) a *= sigmoid(to_f32(raw.d[i]) + bias);
+                        const float a = fmaf(along_A[0], 1.f / LOG2E, u[i] * along_B[0]) * bend[i];
                         if (!outside(at.p + j)) {
-                            dD = fmaf(g[i], u, dD);
+                            dD = fmaf(g[i], u[i], dD);
                             dbias += a;
                             if (at.there) {
                                 put(bp.du, j, fmaf(dt[i], along_B[0], skip * g[i]));
@@ -338,49 +375,42 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                     }
                 });
             };
-            if (row >= from && row + BATCH <= to && w.within(row, BATCH)) {
-                const float h[4] = {kept[0], kept[1], kept[2], kept[3]};
-                piece(std::false_type(), 0, 0, h);
-            } else {
-                if (row < from || row + BATCH > to) {
+            if (row < from || row + BATCH > to) {
 #pragma unroll
-                    for (int i = 0; i < OWN; ++i) {
-                        const int t = row + at.p + i * P;
-                        if (at.there && t < r1 && (t < from || t >= to)) {
-                            put(bp.du, i * P, 0.f);
-                            put(bp.dd, i * P, 0.f);
-                            if (p.z) put(bp.dz, i * P, 0.f);
-                        }
+                for (int i = 0; i < OWN; ++i) {
+                    const int t = row + at.p + i * P;
+                    if (at.there && t < r1 && (t < from || t >= to)) {
+                        put(bp.du, i * P, 0.f);
+                        put(bp.dd, i * P, 0.f);
+                        if (p.z) put(bp.dz, i * P, 0.f);
                     }
                 }
-                for (;;) {                                 // one sequence in front of the other
-                    const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
-                    if (first >= behind) break;
-                    float h[4] = {kept[0], kept[1], kept[2], kept[3]};
-                    if (behind == w.end) state_of(bp.glast, w.n, R);
-                    if (first == w.begin) state_of(p.state, w.n, h);
-                    piece(std::true_type(), first, behind, h);
-                    if (first > w.begin) break;
-                    first_gradient(w.n, R);
+            }
+            for (;;) {                                     // one sequence in front of the other
+                const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
+                if (first >= behind) break;
+                float h[4] = {kept[0], kept[1], kept[2], kept[3]};
+                if (behind == w.end) state_of(bp.glast, w.n, R);
+                if (first == w.begin) state_of(p.state, w.n, h);
+                if (behind - first == BATCH) piece(std::false_type(), first, behind, h);
+                else piece(std::true_type(), first, behind, h);
+                if (first > w.begin) break;
+                first_gradient(w.n, R);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) R[k] = 0.f;
-                    w.previous(p.seq);
-                }
+                for (int k = 0; k < 4; ++k) R[k] = 0.f;
+                w.previous(p.seq);
             }
-            if (more) {
-                stage.put(bc[buf ^ 1]);
-                raw = ahead;
-                kept = kept_ahead;
-            }
+            if (more) fetch(row - BATCH);
             lds_barrier();
             for (int i = threadIdx.x; i < SUMS; i += THREADS) {
                 const int t = row + i / ROW;
                 float v = 0.f;
 #pragma unroll
-                for (int q = 0; q < THREADS / WAVE; ++q) v += red[buf % BUFS][q][i];
+                for (int q = 0; q < WAVES; ++q) v += red[q][i];
                 if (t < r1) at_row(part_row + (long long)row * p.G * ROW, (i / ROW * (unsigned)p.G * ROW + i % ROW) * 4u) = t >= from && t < to ? v : 0.f;
             }
-            if (BUFS == 1) lds_barrier();
+            if (more) stage.put(bc);
+            lds_barrier();
         }
     }
     if (p.seq.offsets && bp.dstate)                        // sequences without a token hand the last states' gradients on
