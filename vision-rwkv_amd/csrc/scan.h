@@ -76,13 +76,14 @@ struct Rows {
     __device__ __forceinline__ void fetch(IO (&to)[OWN], const void* t, long long base, long long stride, int row, int end, int q, int e) const {
         const IO* x = static_cast<const IO*>(t) + base + row * stride;
         if (row + BATCH <= end) {
+            asm volatile("" : "+v"(q));                    // (nothing of this is kept for other rows)
             const unsigned place = (q * (unsigned)stride + e) * sizeof(IO);
             int step = P * (int)stride;                    // (its multiples are not kept either: scalar registers run out)
             asm volatile("" : "+s"(step));
 #pragma unroll
             for (int i = 0; i < OWN; ++i, x += step) to[i] = at_row(x, place);
         } else {
-            asm volatile("" : "+v"(q));                    // (nothing of this is kept for other rows)
+            asm volatile("" : "+v"(q));
 #pragma unroll
             for (int i = 0; i < OWN; ++i) to[i] = at_row(x, (min(q + i * P, end - 1 - row) * (unsigned)stride + e) * sizeof(IO));
         }
@@ -111,6 +112,31 @@ struct Stage {
             const int i = threadIdx.x + k * THREADS;
             if (i < VALUES) to[i % ONE / (4 * P) * WHICH * 4 * P + i / ONE * 4 * P + i % (4 * P)] = to_f32(raw[k]);
         }
+    }
+};
+
+// B and C of two tokens after the other two.  NEXT: read from LDS while the two in front are worked on (with two to five waves a vector unit nothing else hides the way from there).
+template <int P, int WHICH, bool NEXT>
+struct Pairs {
+    f32x4 B[2], C[2], B_next[2], C_next[2];
+    __device__ __forceinline__ void read(const float* bc, int pair, int p) {
+        const f32x4* x = reinterpret_cast<const f32x4*>(bc);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            B_next[t] = x[(2 * pair + t) * WHICH * P + p];
+            if (WHICH == 2) C_next[t] = x[(2 * pair + t) * WHICH * P + P + p];
+        }
+    }
+    // `pair` is worked on now; `then` (if there is one) is the next
+    __device__ __forceinline__ void start(const float* bc, int pair, int p) {
+        if (NEXT) read(bc, pair, p);
+    }
+    __device__ __forceinline__ void advance(const float* bc, int pair, int then, int p) {
+        if (!NEXT) read(bc, pair, p);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) B[t] = B_next[t], C[t] = C_next[t];
+        if (NEXT && then >= 0 && then < BATCH / 2) read(bc, then, p);
+        if (NEXT) __builtin_amdgcn_sched_barrier(0);
     }
 };
 
@@ -163,7 +189,7 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
         }
     }
 
-    Rows<IO, P> raw, ahead;
+    Rows<IO, P> raw;
     const auto fetch = [&](Rows<IO, P>& x, int row) {
         x.fetch(x.u, p.u, b * p.u_b, p.u_t, row, r1, at.p, e);
         x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
@@ -179,7 +205,6 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
     for (int row = r0; row < r1; row += BATCH, buf ^= 1) {
         const bool more = row + BATCH < r1;
         if (more) {
-            fetch(ahead, row + BATCH);
             stage.fetch(p, b, at.g, row + BATCH, from, to);
         }
         if (EMIT && p.kept && at.there)
@@ -191,6 +216,8 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
         // tokens [first, behind) of the sixteen, all of one sequence; PART: not all sixteen.  P at a time: each lane's own, then the states of all, then each lane's own again
         const auto piece = [&](auto part_, int first, int behind) {
             constexpr bool PART = decltype(part_)::value;
+            Pairs<P, WHICH, false> pairs;
+            pairs.start(bc[buf], 0, at.p);
             each(std::make_integer_sequence<int, OWN>(), [&](auto i_) {
                 constexpr int i = decltype(i_)::value;
                 const float raw_d = to_f32(raw.d[i]) + bias, u = to_f32(raw.u[i]), dt = p.softplus ? softplus(raw_d) : raw_d, x = dt * u;
@@ -199,16 +226,16 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
                 each(std::make_integer_sequence<int, P>(), [&](auto q_) {
                     constexpr int q = decltype(q_)::value, j = i * P + q;
                     y[q] = 0.f;
+                    if (j % 2 == 0) pairs.advance(bc[buf], j / 2, j / 2 + 1, at.p);
                     if (PART && (row + j < first || row + j >= behind)) return;
                     const float d = from_lane<P, q>(dt), v = from_lane<P, q>(x);
-                    const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * at.p]);
+                    const f32x4 Bt = pairs.B[j % 2], Ct = pairs.C[j % 2];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         h[k] = fmaf(fast_exp2(d * a2[k]), h[k], v * Bt[k]);
                         if (!FULL && pad[k]) h[k] = 0.f;   // (an infinite v would make it NaN)
                     }
                     if (EMIT) {
-                        const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * WHICH * 4 * P + 4 * P + 4 * at.p]);
                         y[q] = fmaf(Ct[3], h[3], fmaf(Ct[2], h[2], fmaf(Ct[1], h[1], Ct[0] * h[0])));
                     }
                 });
@@ -223,35 +250,29 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
                     }
                     if (at.there && (!PART || (mine >= first && mine < behind))) at_row(out + (long long)i * P * width, place) = from_f32<IO>(v);
                 }
-                // (else B and C of all sixteen are read ahead, or the states put off, in registers that other waves could have)
-                if ((i + 1) * P % 4 == 0) {
-                    if (!EMIT) asm volatile("" : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                if (!EMIT) asm volatile("" : "+v"(h[0]), "+v"(h[1]), "+v"(h[2]), "+v"(h[3]));   // (else the compiler puts the states off)
             });
         };
-        if (row >= from && row + BATCH <= to && w.within(row, BATCH)) piece(std::false_type(), 0, 0);
-        else {
-            if (EMIT && (row < from || row + BATCH > to)) {
+        if (EMIT && (row < from || row + BATCH > to)) {
 #pragma unroll
-                for (int i = 0; i < OWN; ++i) {
-                    const int t = row + at.p + i * P;
-                    if (at.there && t < r1 && (t < from || t >= to)) at_row(out + (long long)i * P * p.E, place) = from_f32<IO>(0.f);
-                }
-            }
-            for (;;) {                                     // one sequence after the other
-                const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
-                if (first >= behind) break;
-                if (first == w.begin) first_state(w.n);
-                piece(std::true_type(), first, behind);
-                if (behind < w.end) break;
-                last_state(w.n);
-                w.next(p.seq);
+            for (int i = 0; i < OWN; ++i) {
+                const int t = row + at.p + i * P;
+                if (at.there && t < r1 && (t < from || t >= to)) at_row(out + (long long)i * P * width, place) = from_f32<IO>(0.f);
             }
         }
+        for (;;) {                                         // one sequence after the other
+            const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
+            if (first >= behind) break;
+            if (first == w.begin) first_state(w.n);
+            if (behind - first == BATCH) piece(std::false_type(), first, behind);
+            else piece(std::true_type(), first, behind);
+            if (behind < w.end) break;
+            last_state(w.n);
+            w.next(p.seq);
+        }
         if (more) {
+            fetch(raw, row + BATCH);
             stage.put(bc[buf ^ 1]);
-            raw = ahead;
             lds_barrier();
         }
     }

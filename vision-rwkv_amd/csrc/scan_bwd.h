@@ -212,11 +212,15 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
     }
     const float bias = p.bias.p ? p.bias.value(p.bias.fetch(e)) : 0.f, skip = p.D.p ? p.D.value(p.D.fetch(e)) : 0.f;
     const auto state_of = [&](const float* t, int n, float (&h)[4]) {
+        int e = at.e;
+        asm volatile("" : "+v"(e));                        // (no address of this is kept)
 #pragma unroll
         for (int k = 0; k < 4; ++k) h[k] = t && !pad[k] ? t[((long long)n * p.E + e) * p.S + 4 * at.p + k] : 0.f;
     };
     const auto first_gradient = [&](int n, const float (&h)[4]) {
         if (!bp.dstate || !at.there) return;
+        int e = at.e;
+        asm volatile("" : "+v"(e));
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (!pad[k]) bp.dstate[((long long)n * p.E + e) * p.S + 4 * at.p + k] = h[k];
@@ -285,21 +289,27 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
             // tokens [first, behind) of the sixteen, all of one sequence, from the state h in front of them; PART: not all sixteen
             const auto piece = [&](auto part_, int first, int behind, const float (&h)[4]) {
                 constexpr bool PART = decltype(part_)::value;
-                const auto outside = [&](int j) { return PART && (row + j < first || row + j >= behind); };
+                const int low = first - row, count = behind - first;
+                const auto outside = [&](int j) { return PART && (unsigned)(j - low) >= (unsigned)count; };
+                int lane_token = at.p, lane_sum = sum;
+                if (PART) asm volatile("" : "+v"(lane_token), "+v"(lane_sum));   // (nothing of this is kept for other rows)
                 float hs[BATCH + 1][4];                    // hs[j]: the state in front of token j
 #pragma unroll
                 for (int k = 0; k < 4; ++k) hs[0][k] = h[k];
+                Pairs<P, 2, !PART> pairs;
+                pairs.start(bc, 0, at.p);
                 each(std::make_integer_sequence<int, OWN>(), [&](auto i_) {
                     constexpr int i = decltype(i_)::value;
                     float y[P];
                     each(std::make_integer_sequence<int, P>(), [&](auto q_) {
                         constexpr int q = decltype(q_)::value, j = i * P + q;
                         y[q] = 0.f;
+                        if (j % 2 == 0) pairs.advance(bc, j / 2, j / 2 + 1, at.p);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) hs[j + 1][k] = hs[j][k];
                         if (outside(j)) return;
                         const float d = from_lane<P, q>(dt[i]), v = from_lane<P, q>(dt[i] * u[i]);
-                        const f32x4 Bt = *reinterpret_cast<const f32x4*>(&bc[j * ROW + 4 * at.p]), Ct = *reinterpret_cast<const f32x4*>(&bc[j * ROW + 4 * P + 4 * at.p]);
+                        const f32x4 Bt = pairs.B[j % 2], Ct = pairs.C[j % 2];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             hs[j + 1][k] = fmaf(fast_exp2(d * a2[k]), hs[j][k], v * Bt[k]);
@@ -310,7 +320,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                     });
                     if (p.z) {
                         sum_to_lanes<P, P>(y, at.p);
-                        if (at.there && !outside(at.p + i * P)) put(bp.dz, i * P, gz[i] * fmaf(skip, u[i], y[0]));
+                        if (at.there && !outside(lane_token + i * P)) put(bp.dz, i * P, gz[i] * fmaf(skip, u[i], y[0]));
                     }
                 });
                 // (the exponentials are taken and B and C read again: kept, they would fill three times as many registers as the states)
@@ -318,14 +328,16 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                 asm volatile("" : "+v"(again));
 #pragma unroll
                 for (int i = 0; i < OWN; ++i) asm volatile("" : "+v"(dt[i]));
+                pairs.start(bc, BATCH / 2 - 1, again);
                 float along_B[P], along_A[P], sums[COUNT];
                 each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
                     constexpr int j = BATCH - 1 - decltype(j_)::value;
                     along_A[j % P] = along_B[j % P] = 0.f;
+                    if (j % 2 == 1) pairs.advance(bc, j / 2, j / 2 - 1, again);
                     float dB[4] = {0.f, 0.f, 0.f, 0.f}, dC[4] = {0.f, 0.f, 0.f, 0.f};
                     if (!outside(j)) {
                         const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(dt[j / P] * u[j / P]), gj = from_lane<P, j % P>(g[j / P]);
-                        const f32x4 Bt = reinterpret_cast<const f32x4*>(bc)[j * 2 * P + again], Ct = reinterpret_cast<const f32x4*>(bc)[j * 2 * P + P + again];
+                        const f32x4 Bt = pairs.B[j % 2], Ct = pairs.C[j % 2];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const float r = fmaf(Ct[k], gj, R[k]);
@@ -354,7 +366,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                         }
                         if constexpr (j % GROUP == 0) {
                             sum_over_channels<P>(sums, at.lane);
-                            if (!outside(j + sum / 8)) red[wave][j * ROW + leave] = sums[0];
+                            if (!outside(j + lane_sum / 8)) red[wave][j * ROW + leave] = sums[0];
                         }
                     }
                     // (else the compiler puts the additions to dA off to the end of the sixteen tokens, with all that they add up)
@@ -364,7 +376,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                         sum_to_lanes<P, P>(along_A, at.p);
                         sum_to_lanes<P, P>(along_B, at.p);
                         const float a = fmaf(along_A[0], 1.f / LOG2E, u[i] * along_B[0]) * bend[i];
-                        if (!outside(at.p + j)) {
+                        if (!outside(lane_token + j)) {
                             dD = fmaf(g[i], u[i], dD);
                             dbias += a;
                             if (at.there) {
