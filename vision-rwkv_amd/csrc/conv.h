@@ -23,6 +23,7 @@ struct Params {
     float* part;                                           // (parts, K + 1, E): sums of dw and db
     long long x_b, x_t, g_b, g_t;
     int N, rows, T, E, K, silu, run, runs;                 // run: tokens of a run; runs: of a batch row
+    bool weights_aligned;                                  // a lane's weights and biases at multiples of theirs in size
 };
 
 __device__ __forceinline__ float silu_of(float p) { return p * fast_rcp(1.f + fast_exp2(-LOG2E * p)); }
@@ -45,12 +46,43 @@ struct Lane {
     __device__ __forceinline__ Lane(const Params& p_, int vec) : p(p_) {
         there = vec * VEC < p.E;
         c = there ? vec * VEC : 0;
+        if (KT < 8 && p.weights_aligned) {
+            if (p.w.dtype == VRWKV_F32) read_params<float>();
+            else if (p.w.dtype == VRWKV_BF16) read_params<__hip_bfloat16>();
+            else read_params<__half>();
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
 #pragma unroll
             for (int j = 0; j < KT; ++j) w[j].v[i] = used(j) ? p.w.value(p.w.fetch((c + i) * p.K + j - (KT - p.K))) : 0.f;
             bias.v[i] = p.bias.p ? p.bias.value(p.bias.fetch(c + i)) : 0.f;
         }
+    }
+    // VEC numbers of a parameter next to each other
+    template <typename T>
+    static __device__ __forceinline__ void read_vec(const void* t, int at, float* v) {
+        constexpr int ONE = sizeof(T) * VEC > 16 ? VEC / 2 : VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; i += ONE) {
+            float x[ONE];
+            load_vec<T, ONE>(static_cast<const T*>(t) + at + i, x);
+#pragma unroll
+            for (int k = 0; k < ONE; ++k) v[i + k] = x[k];
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void read_params() {        // the weights of VEC channels lie next to each other
+        float all[VEC * KT];
+#pragma unroll
+        for (int j = 0; j < KT; ++j) read_vec<T>(p.w.p, c * KT + j * VEC, all + j * VEC);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            bias.v[i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < KT; ++j) w[j].v[i] = all[i * KT + j];
+        }
+        if (p.bias.p) read_vec<T>(p.bias.p, c, bias.v);
     }
     __device__ __forceinline__ bool used(int j) const { return KT < 8 || j >= KT - p.K; }   // (a weight of zero would make an infinite row NaN)
     __device__ __forceinline__ Packed<IO, VEC> packed(const void* t, long long at) const { return load_packed<IO, VEC>(static_cast<const IO*>(t) + at + c); }
@@ -112,6 +144,11 @@ int vec_of(int dtype, int E, int most, size_t bits, const long long* strides, in
     return bits % most == 0 ? most / e : e == 2 && bits % 4 == 0 ? 2 : 1;
 }
 
+bool weights_fit(const void* w, const void* b, int dtype, int vec) {
+    const size_t n = std::min(16, vec * (dtype == VRWKV_F32 ? 4 : 2));
+    return (((size_t)w | (size_t)b) & (n - 1)) == 0;
+}
+
 template <typename F>
 int with_taps(int K, F&& f) {
     if (K == 2) return f(std::integral_constant<int, 2>());
@@ -154,8 +191,9 @@ int check(const char* who, const vrwkv_conv_args* args, bool backward) {
     return VRWKV_OK;
 }
 
-Params params_of(const vrwkv_conv_args& a, const Plan& pl) {
+Params params_of(const vrwkv_conv_args& a, const Plan& pl, int vec) {
     Params p{};
+    p.weights_aligned = weights_fit(a.weight, a.bias, a.param_dtype, vec);
     p.x = a.x, p.state = a.state, p.gy = a.gy, p.glast = a.glast;
     p.w = ParamVec(a.weight, a.param_dtype, 1.f), p.bias = ParamVec(a.bias, a.param_dtype, 1.f);
     p.seq = Sequences{a.offsets, a.offsets64, a.N, a.T};

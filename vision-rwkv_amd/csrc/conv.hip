@@ -129,7 +129,7 @@ extern "C" int vrwkv_conv_fwd(const vrwkv_conv_args* args, void* hip_stream) {
     const long long strides[] = {a.offsets ? 0 : a.x_stride[0], a.x_stride[1]};
     const int vec = vec_of(a.dtype, a.E, 16, (size_t)a.x | (size_t)a.y | (size_t)a.state, strides, 2);
     const Plan pl = plan_of(a, vec);
-    const Params p = params_of(a, pl);
+    const Params p = params_of(a, pl, vec);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const int blocks = (int)(((long long)pl.rows * pl.runs + THREADS / WAVE - 1) / (THREADS / WAVE));
     const int extra = a.last ? (int)std::min<long long>(4LL * device_cus(), ((long long)a.N * (a.K - 1) * a.E + THREADS - 1) / THREADS) : 0;
@@ -164,6 +164,7 @@ extern "C" int vrwkv_conv_step(const vrwkv_conv_step_args* args, void* hip_strea
     sp.slots = Slots{a.slots, a.slots64, a.N, a.P}, sp.pool = a.pool, sp.page = a.page_stride, sp.x_n = a.x_stride;
     const long long strides[] = {a.x_stride, a.page_stride};
     const int vec = vec_of(a.dtype, a.E, 16, (size_t)a.x | (size_t)a.y | (size_t)a.pool, strides, 2);
+    sp.f.weights_aligned = weights_fit(a.weight, a.bias, a.param_dtype, vec);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const dim3 grid((a.E / vec + THREADS - 1) / THREADS, std::min(a.N, GRID_Y), (a.N + GRID_Y - 1) / GRID_Y);
     return with_types<8>(a.dtype, vec, [&](auto io, auto v) {

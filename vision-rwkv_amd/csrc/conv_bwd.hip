@@ -182,7 +182,7 @@ extern "C" int vrwkv_conv_bwd(const vrwkv_conv_args* args, void* hip_stream) {
     const int parts = parts_of(pl);
     const size_t need = (size_t)parts * (a.K + 1) * a.E * 4;
     if (!a.workspace || a.workspace_bytes < need) { set_error("%s: workspace of %zu bytes, %zu needed", who, a.workspace ? a.workspace_bytes : (size_t)0, need); return VRWKV_WORKSPACE_TOO_SMALL; }
-    Params p = params_of(a, pl);
+    Params p = params_of(a, pl, vec);
     p.part = static_cast<float*>(a.workspace);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const int extra = a.offsets && a.dstate ? std::min(a.N, 64) : 0;

@@ -22,6 +22,7 @@ struct Params {
     long long rows, x_r, res_r, gy_r, gsum_r;
     int C, out_kind;
     float eps;
+    bool weights_aligned;                                  // at a multiple of a vector's size
 };
 
 // The value that the four waves of a workgroup, or one wave, agree on.
@@ -104,6 +105,17 @@ __device__ __forceinline__ void write(void* t, long long at, const float (&v)[VE
         store_vec<T, ONE>(static_cast<T*>(t) + at + i, x);
     }
 }
+// the weights of VEC channels
+template <int VEC>
+__device__ __forceinline__ void weights(const Params& p, int c, float (&w)[VEC]) {
+    if (VEC > 1 && p.weights_aligned) {
+        if (p.w.dtype == VRWKV_F32) read<float, VEC>(p.w.p, c, w);
+        else if (p.w.dtype == VRWKV_BF16) read<__hip_bfloat16, VEC>(p.w.p, c, w);
+        else read<__half, VEC>(p.w.p, c, w);
+    } else
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) w[k] = p.w.value(p.w.fetch(c + k));
+}
 // VEC elements of a row of x and residual, added and rounded
 template <typename IO, typename RES, int VEC>
 __device__ __forceinline__ void sum_of(const Params& p, long long row, int c, float (&r)[VEC]) {
@@ -138,13 +150,14 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(const Params p) {
     const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
     const long long row = WAVES == 1 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= p.rows) return;
-    float r[NV][VEC], s = 0.f;
+    float r[NV][VEC], w[NV][VEC], s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * 64 * WAVES + lane) * VEC;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) r[i][k] = 0.f;
+        for (int k = 0; k < VEC; ++k) r[i][k] = w[i][k] = 0.f;
         if (c < p.C) {
+            weights<VEC>(p, c, w[i]);
             sum_of<IO, RES, VEC>(p, row, c, r[i]);
             if (p.sum) write<RES, VEC>(p.sum, row * p.C + c, r[i]);
         }
@@ -158,12 +171,11 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * 64 * WAVES + lane) * VEC;
-        if (c < p.C)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                r[i][k] = r[i][k] * s * p.w.value(p.w.fetch(c + k));
-                most = larger(most, r[i][k]);
-            }
+        for (int k = 0; k < VEC; ++k) {
+            r[i][k] = r[i][k] * s * w[i][k];
+            most = larger(most, r[i][k]);
+        }
     }
     if (p.out_kind != VRWKV_Y_SAME) {
         const float v = scale_of(agreed<WAVES, true>(most, red), top_of(p.out_kind), inverse);
@@ -229,13 +241,12 @@ __global__ __launch_bounds__(THREADS) void backward_kernel(const Params p) {
     const long long first = WAVES == 1 ? (long long)blockIdx.x * 4 + wave : blockIdx.x, step = WAVES == 1 ? gridDim.x * 4LL : gridDim.x;
     float dw[NV][VEC], w[NV][VEC];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 64 * WAVES + lane) * VEC;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            const int c = (i * 64 * WAVES + lane) * VEC;
-            dw[i][k] = 0.f;
-            w[i][k] = c < p.C ? p.w.value(p.w.fetch(c + k)) : 0.f;
-        }
+        for (int k = 0; k < VEC; ++k) dw[i][k] = w[i][k] = 0.f;
+        if (c < p.C) weights<VEC>(p, c, w[i]);
+    }
     for (long long row = first; row < p.rows; row += step) {
         float r[NV][VEC], g[NV][VEC], s = 0.f, m = 0.f;
 #pragma unroll
@@ -356,6 +367,7 @@ Plan plan_of(const vrwkv_rmsnorm_args& a, bool backward) {
     p.parts = (int)std::min<long long>(groups, p.nv ? 4LL * device_cus() : 256);
     return p;
 }
+bool weights_fit(const vrwkv_rmsnorm_args& a) { return ((size_t)a.weight & (std::min<size_t>(16, (a.dtype == VRWKV_F32 ? 4 : 8) * size_of(a.weight_dtype)) - 1)) == 0; }
 size_t backward_bytes(const vrwkv_rmsnorm_args& a, const Plan& p) { return ((size_t)p.parts * a.C * 4 + 15) / 16 * 16 + (p.nv ? 0 : (size_t)a.rows * 4); }
 
 template <typename F>
@@ -412,6 +424,7 @@ extern "C" int vrwkv_rmsnorm(const vrwkv_rmsnorm_args* args, void* hip_stream) {
     Params p{};
     p.x = a.x, p.residual = a.residual, p.w = ParamVec(a.weight, a.weight_dtype, 1.f), p.y = a.y, p.sum = a.sum, p.scale = a.scale;
     p.rows = a.rows, p.x_r = a.x_stride, p.res_r = a.residual_stride, p.C = a.C, p.out_kind = a.out_kind, p.eps = a.eps;
+    p.weights_aligned = weights_fit(a);
     const Plan pl = plan_of(a, false);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     return with_types(a.dtype, a.residual_dtype, [&](auto io, auto res) {
@@ -442,6 +455,7 @@ extern "C" int vrwkv_rmsnorm_bwd(const vrwkv_rmsnorm_args* args, void* hip_strea
     Params p{};
     p.sum = a.sum, p.w = ParamVec(a.weight, a.weight_dtype, 1.f), p.gy = a.gy, p.gsum = a.gsum, p.dx = a.dx, p.dresidual = a.dresidual;
     p.rows = a.rows, p.x_r = a.x_stride, p.gy_r = a.gy_stride, p.gsum_r = a.gsum_stride, p.C = a.C, p.eps = a.eps;
+    p.weights_aligned = weights_fit(a);
     p.part = a.dweight ? static_cast<float*>(a.workspace) : nullptr;
     p.stat = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + ((size_t)pl.parts * a.C * 4 + 15) / 16 * 16);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
