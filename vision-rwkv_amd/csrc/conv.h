@@ -3,8 +3,8 @@
 //     p_t = sum_j w_j x_{t - (K-1) + j} + b        y_t = silu(p_t) or p_t        g_t = gy_t silu'(p_t)
 //     dx_t = sum_j w_j g_{t + (K-1) - j}           dw_j = sum_t g_t x_{t - (K-1) + j}          db = sum_t g_t
 //
-// Bound by the memory: each row is read once and written once.  A lane holds VEC channels and goes along a run of tokens with the last K - 1 rows in registers, eight rows on their
-// way ahead; the K - 1 rows in front of a run are read again (from L2).  A sequence's first state stands for K - 1 tokens in front of it, in both directions.
+// Bound by the memory: each row is read once and written once.  A lane holds VEC channels and goes along a run of tokens with the last K - 1 rows in registers, the next rows on their
+// way; the K - 1 rows in front of a run are read again (from L2).  A sequence's first state stands for K - 1 tokens in front of it, in both directions.
 #pragma once
 #include "sequences.h"
 #include <algorithm>
@@ -13,7 +13,7 @@ namespace vrwkv {
 namespace conv {
 namespace {
 
-constexpr int THREADS = 256, AHEAD = 8;
+constexpr int THREADS = 256;
 
 struct Params {
     const void *x, *state, *gy, *glast;
@@ -126,16 +126,7 @@ struct Run {
 // ---- launches --------------------------------------------------------------------------------------------------------
 
 struct Plan { int run, runs, rows, waves; };              // waves: of a row's channels
-// Runs as long as they leave four waves for each of the chip's vector units, of 8 to 64 tokens.
-Plan plan_of(const vrwkv_conv_args& a, int vec) {
-    Plan p;
-    p.rows = a.offsets ? 1 : a.N;
-    p.waves = (a.E + WAVE * vec - 1) / (WAVE * vec);
-    const long long run = (long long)p.rows * a.T * p.waves / (16LL * device_cus());
-    p.run = (int)std::max(8LL, std::min(64LL, run / AHEAD * AHEAD));
-    p.runs = (a.T + p.run - 1) / p.run;
-    return p;
-}
+
 // Channels that a lane takes: of `most` bytes where all rows of all tensors lie at multiples of it, pairs of 16-bit ones at multiples of 4, else one.
 int vec_of(int dtype, int E, int most, size_t bits, const long long* strides, int n) {
     const int e = dtype == VRWKV_F32 ? 4 : 2;

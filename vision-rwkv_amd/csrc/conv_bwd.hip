@@ -5,6 +5,7 @@ namespace vrwkv {
 namespace conv {
 namespace {
 
+constexpr int AHEAD = 4;                                  // (eight rows of two tensors ahead: 49 us for 37 at 64 x 196 x 1536 bf16, for want of registers)
 // Runs parts apart, one after the other: their sums for dw and db stay in registers until the end.
 template <typename IO, int VEC, int KT>
 __global__ __launch_bounds__(THREADS) void backward_kernel(const Params p, int run_blocks) {
@@ -156,8 +157,19 @@ int backward_vec(const vrwkv_conv_args& a) {
     return vec_of(a.dtype, a.E, a.dtype == VRWKV_F32 ? 16 : 2 * BACKWARD_VEC, (size_t)a.x | (size_t)a.gy | (size_t)a.dx | (size_t)a.state | (size_t)a.dstate | (size_t)a.glast, strides, 4);
 }
 
-constexpr int MOST_PARTS = 512;
-int parts_of(const Plan& p) { return (int)std::min<long long>(MOST_PARTS, ((long long)p.rows * p.runs + THREADS / WAVE - 1) / (THREADS / WAVE)); }
+// As many runs as there are waves at once, three for each of the chip's vector units, of 8 tokens at least; a wave takes several where there are more rows than that.
+// 64 x 196 and 8 x 2048 tokens of 1536 channels in bf16: 37 and 45 us; with a third more waves than fit 44 and 53, with twice as many 46 and 53.
+int waves_at_once(const Plan& p) { return std::max(1, 12 * device_cus() / p.waves); }
+Plan plan_of(const vrwkv_conv_args& a, int vec) {
+    Plan p;
+    p.rows = a.offsets ? 1 : a.N;
+    p.waves = (a.E + WAVE * vec - 1) / (WAVE * vec);
+    const int pieces = std::max(1, std::min(waves_at_once(p) / p.rows, a.T / 8));
+    p.run = (a.T + pieces - 1) / pieces;
+    p.runs = (a.T + p.run - 1) / p.run;
+    return p;
+}
+int parts_of(const Plan& p) { return (int)((std::min<long long>(waves_at_once(p), (long long)p.rows * p.runs) + THREADS / WAVE - 1) / (THREADS / WAVE)); }
 
 
 }  // namespace
