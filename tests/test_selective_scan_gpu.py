@@ -150,6 +150,24 @@ def test_cut_sequences(segments, dtype, S, force):
     run_and_compare(x, normal, [(0, 0, 403), (1, 0, 403)])
 
 
+@pytest.mark.parametrize("segments", [0, 1])
+@pytest.mark.parametrize("N,T,E,S,G,dtype", [(1, 1024, 8, 16, 1, "bf16"), (2, 513, 10, 3, 2, "fp32"), (1, 512, 9, 64, 1, "fp32"), (1, 300, 21, 29, 3, "fp16"), (3, 129, 14, 50, 1, "bf16"), (2, 257, 34, 8, 2, "fp16")])
+def test_few_channels_with_and_without_rounds(N, T, E, S, G, dtype, segments, force):
+    force("scan_segments", segments)
+    x, normal = inputs(N, T, E, S, G, dtype, state=N)
+    run_and_compare(x, normal, [(n, 0, T) for n in range(N)])
+
+
+def test_long_packed_rows_of_few_channels():
+    lengths = [3, 0, 250, 16, 1, 1, 240, 0, 300, 45]
+    first = [5]
+    for n in lengths:
+        first.append(first[-1] + n)
+    x, normal = inputs(1, first[-1] + 9, 6, 16, 1, "fp32", state=len(lengths))
+    offsets = torch.tensor(first, dtype=torch.int32, device="cuda")
+    run_and_compare(x, normal, [(0, a, b) for a, b in zip(first, first[1:])], offsets=offsets)
+
+
 @pytest.mark.parametrize("z,D,bias,softplus,state,glast,params", [(False, False, False, False, 0, False, "fp32"), (True, False, True, False, 2, False, "same"), (False, True, False, True, 0, True, "same"),
                                                                   (True, True, True, True, 0, False, "same"), (False, False, True, True, 2, True, "fp32")])
 def test_what_may_be_left_out(z, D, bias, softplus, state, glast, params):

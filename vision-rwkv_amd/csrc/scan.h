@@ -150,11 +150,20 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
     constexpr int OWN = BATCH / P, WHICH = EMIT ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float bc[2][BATCH * WHICH * 4 * P];
     const Place<P> at(p.E, p.G, p.blocks);
-    const int s = blockIdx.y, b = blockIdx.z, r0 = s * p.L, r1 = min(p.T, r0 + p.L), e = at.e;
+    const int s = blockIdx.y, b = blockIdx.z, e = at.e;
+    int r0 = s * p.L;
+    const int r1 = min(p.T, r0 + p.L);
     int from, to;                                          // the tokens that belong to a sequence
     p.seq.inside(r0, r1, from, to);
     Walk w;
-    w.find(p.seq, b, from, at.lane);
+    if (!EMIT) {                                           // only of the sequence that goes on behind the segment
+        w.find(p.seq, b, max(from, r1 - 1), at.lane);
+        if (w.begin >= r1 || w.end <= r1) return;
+        if (w.begin >= r0) {
+            r0 += (w.begin - r0) / BATCH * BATCH;
+            from = w.begin;
+        }
+    } else w.find(p.seq, b, from, at.lane);
     float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
     bool pad[4];
 #pragma unroll

@@ -1,5 +1,6 @@
-// vrwkv_scan_fwd and vrwkv_scan_bwd: checks, cuts and the sums that end a backward pass (the kernels: scan.h, scan_bwd.h).
+// vrwkv_scan_fwd and vrwkv_scan_bwd: checks, cuts and the sums that end a backward pass (the kernels: scan.h, scan_short.h, scan_bwd.h).
 #include "scan_bwd.h"
+#include "scan_short.h"
 #include <algorithm>
 #include <cstdint>
 
@@ -10,8 +11,11 @@ namespace scan {
 extern template int launch_forward<float>(const Params&, hipStream_t);
 extern template int launch_forward<__hip_bfloat16>(const Params&, hipStream_t);
 extern template int launch_forward<__half>(const Params&, hipStream_t);
+extern template int launch_short<float>(const Params&, int, hipStream_t);
 extern template int launch_backward<float>(const BackParams&, int, hipStream_t);
+extern template int launch_short<__hip_bfloat16>(const Params&, int, hipStream_t);
 extern template int launch_backward<__hip_bfloat16>(const BackParams&, int, hipStream_t);
+extern template int launch_short<__half>(const Params&, int, hipStream_t);
 extern template int launch_backward<__half>(const BackParams&, int, hipStream_t);
 
 namespace {
@@ -40,9 +44,17 @@ Plan plan_of(const vrwkv_scan_args& a) {
     return p;
 }
 
+// Whether a forward goes through scan_short.h: one workgroup a compute unit, and four rounds of its waves over the tokens.  bf16, 16 states, that kernel against the segments': 196 tokens of
+// 384 channels 8.0 us for 16.3, 1024 of 384 22 for 27; beyond it 196 of 1536 (384 workgroups) 15.2 for 15.7, 4 x 196 of 1536 45 for 24, 4150 of 384 80 for 51.
+bool is_short(const vrwkv_scan_args& a) {
+    const long long groups = (long long)(a.offsets ? 1 : a.N) * a.G * ((a.E / a.G + SHORT_CHANNELS - 1) / SHORT_CHANNELS);
+    return !option(OPT_SCAN_SEGMENTS) && groups <= device_cus() && a.T <= 4 * BATCH * short_waves(a.S);
+}
+
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 size_t chunks_of(const vrwkv_scan_args& a) { return ((size_t)a.T + BATCH - 1) / BATCH; }
 size_t segment_bytes(const vrwkv_scan_args& a, const Plan& p) { return p.nseg > 1 ? up16((size_t)p.rows * p.nseg * p.states * 4) + up16((size_t)p.rows * p.nseg * a.E * 4) : 0; }
+size_t forward_bytes(const vrwkv_scan_args& a, const Plan& p) { return is_short(a) ? 0 : segment_bytes(a, p); }
 size_t part_bc_floats(const vrwkv_scan_args& a, const Plan& p) { return (size_t)p.blocks * p.rows * a.T * a.G * 8 * p.P; }
 size_t backward_bytes(const vrwkv_scan_args& a, const Plan& p) {
     const size_t parts = (size_t)p.parts * p.nseg;
@@ -75,7 +87,7 @@ int check(const char* who, const vrwkv_scan_args* args, bool backward) {
         fits = fits && aligned(a.gy, a.dtype) && aligned(a.du, a.dtype) && aligned(a.ddelta, a.dtype) && aligned(a.dz, a.dtype) && aligned(a.dB, a.dtype) && aligned(a.dC, a.dtype) &&
                aligned(a.dD, a.D_dtype) && aligned(a.dbias, a.bias_dtype) && (((size_t)a.dA | (size_t)a.dstate | (size_t)a.glast) & 3) == 0;
     if (!fits) { set_error("%s: a tensor is not aligned to its elements, kept or the workspace to 16 bytes", who); return VRWKV_INVALID_ARG; }
-    const size_t need = backward ? backward_bytes(a, p) : segment_bytes(a, p);
+    const size_t need = backward ? backward_bytes(a, p) : forward_bytes(a, p);
     if (need && (!a.workspace || a.workspace_bytes < need)) { set_error("%s: workspace of %zu bytes, %zu needed", who, a.workspace ? a.workspace_bytes : (size_t)0, need); return VRWKV_WORKSPACE_TOO_SMALL; }
     return VRWKV_OK;
 }
@@ -159,13 +171,20 @@ extern "C" size_t vrwkv_scan_kept_bytes(const vrwkv_scan_args* args) {
     const Plan p = plan_of(*args);
     return (size_t)p.rows * chunks_of(*args) * p.states * 4;
 }
-extern "C" size_t vrwkv_scan_fwd_workspace_bytes(const vrwkv_scan_args* args) { return scan_sizes(args) ? segment_bytes(*args, plan_of(*args)) : 0; }
+extern "C" size_t vrwkv_scan_fwd_workspace_bytes(const vrwkv_scan_args* args) { return scan_sizes(args) ? forward_bytes(*args, plan_of(*args)) : 0; }
 extern "C" size_t vrwkv_scan_bwd_workspace_bytes(const vrwkv_scan_args* args) { return scan_sizes(args) ? backward_bytes(*args, plan_of(*args)) : 0; }
 
 extern "C" int vrwkv_scan_fwd(const vrwkv_scan_args* args, void* hip_stream) {
     if (const int rc = check("vrwkv_scan_fwd", args, false)) return rc;
-    const Params p = params_of(*args, plan_of(*args));
+    const Plan pl = plan_of(*args);
+    Params p = params_of(*args, pl);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    if (is_short(*args)) {
+        p.blocks = (args->E / args->G + SHORT_CHANNELS - 1) / SHORT_CHANNELS;
+        if (args->dtype == VRWKV_F32) return launch_short<float>(p, 4 * pl.P, st);
+        if (args->dtype == VRWKV_BF16) return launch_short<__hip_bfloat16>(p, 4 * pl.P, st);
+        return launch_short<__half>(p, 4 * pl.P, st);
+    }
     if (args->dtype == VRWKV_F32) return launch_forward<float>(p, st);
     if (args->dtype == VRWKV_BF16) return launch_forward<__hip_bfloat16>(p, st);
     return launch_forward<__half>(p, st);
