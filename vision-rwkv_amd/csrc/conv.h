@@ -46,6 +46,8 @@ struct Lane {
     __device__ __forceinline__ Lane(const Params& p_, int vec) : p(p_) {
         there = vec * VEC < p.E;
         c = there ? vec * VEC : 0;
+    }
+    __device__ __forceinline__ void read_weights() {
         if (KT < 8 && p.weights_aligned) {
             if (p.w.dtype == VRWKV_F32) read_params<float>();
             else if (p.w.dtype == VRWKV_BF16) read_params<__hip_bfloat16>();
@@ -114,10 +116,12 @@ struct Lane {
 struct Run {
     int b, t0, t1, from, to;
     Walk w;
-    __device__ __forceinline__ Run(const Params& p, int run, int lane) {
+    __device__ __forceinline__ Run(const Params& p, int run) {
         b = run / p.runs;
         t0 = run % p.runs * p.run;
         t1 = min(p.T, t0 + p.run);
+    }
+    __device__ __forceinline__ void find(const Params& p, int lane) {
         p.seq.inside(t0, t1, from, to);
         w.find(p.seq, b, from, lane);
     }

@@ -7,7 +7,7 @@ namespace conv {
 namespace {
 
 constexpr int AHEAD = 8;
-// Runs of 8 tokens, longer ones (up to 64) once there are four waves for each of the chip's vector units.  64 x 196 x 1536 bf16: 20.4 us with 8, 21.8 with 16, 30 with 32.
+// Runs of 8 tokens, longer ones (up to 64) once there are four waves for each of the chip's vector units.  64 x 196 x 1536 bf16: 19.6 us with 8, 21.8 with 16, 30 with 32.
 Plan plan_of(const vrwkv_conv_args& a, int vec) {
     Plan p;
     p.rows = a.offsets ? 1 : a.N;
@@ -42,17 +42,29 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(const Params p, int ru
     }
     const int number = blockIdx.x * (THREADS / WAVE) + (threadIdx.x >> 6);
     if (number >= p.rows * p.runs) return;
-    const Lane<IO, VEC, KT> my(p, blockIdx.y * WAVE + lane);
-    Run r(p, __builtin_amdgcn_readfirstlane(number), lane);
-    Packed<IO, VEC> ahead[AHEAD];
+    Run r(p, __builtin_amdgcn_readfirstlane(number));
+    Lane<IO, VEC, KT> my(p, blockIdx.y * WAVE + lane);
+    Packed<IO, VEC> ahead[AHEAD], front[KT - 1];
     const auto fetch = [&](int t) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) ahead[i] = my.packed(p.x, r.b * p.x_b + min(t + i, r.t1 - 1) * p.x_t);
     };
+    // all rows, and the weights, before it is known what sequences there are
+#pragma unroll
+    for (int j = 0; j < KT - 1; ++j)
+        if (my.used(j)) front[j] = my.packed(p.x, r.b * p.x_b + max(r.t0 - (KT - 1) + j, 0) * p.x_t);
     fetch(r.t0);
+    my.read_weights();
+    r.find(p, lane);
     Wide<VEC> x[KT];                                       // x[j]: token t - (KT - 1) + j
 #pragma unroll
-    for (int j = 0; j < KT - 1; ++j) x[j + 1] = r.w.begin < r.t0 && my.used(j) ? my.token(r.w.n, r.b, r.t0 - (KT - 1) + j, r.w.begin) : Wide<VEC>{};
+    for (int j = 0; j < KT - 1; ++j) {
+        x[j + 1] = Wide<VEC>{};
+        const int t = r.t0 - (KT - 1) + j;
+        if (!my.used(j) || r.w.begin >= r.t0) continue;
+        if (t >= r.w.begin) widen_packed<IO, VEC>(front[j], x[j + 1].v);
+        else x[j + 1] = my.token(r.w.n, r.b, t, r.w.begin);
+    }
     for (int t = r.t0; t < r.t1; t += AHEAD) {
         Packed<IO, VEC> now[AHEAD];
 #pragma unroll
@@ -98,7 +110,8 @@ __global__ __launch_bounds__(THREADS) void step_kernel(const StepParams sp) {
     const long long slot = sp.slots.at(n0);
     const bool known = sp.slots.has(slot);
     IO* const page = static_cast<IO*>(sp.pool) + (known ? slot : 0) * sp.page;
-    const Lane<IO, VEC, KT> my(p, blockIdx.x * THREADS + threadIdx.x);
+    Lane<IO, VEC, KT> my(p, blockIdx.x * THREADS + threadIdx.x);
+    my.read_weights();
     Wide<VEC> x[KT];
     Wide<VEC> now = my.row(p.x, n0 * sp.x_n);
 #pragma unroll

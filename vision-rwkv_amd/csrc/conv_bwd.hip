@@ -19,14 +19,14 @@ __global__ __launch_bounds__(THREADS) void backward_kernel(const Params p, int r
                 for (long long i = threadIdx.x; i < page; i += THREADS) static_cast<IO*>(p.dstate)[n * page + i] = p.glast ? static_cast<const IO*>(p.glast)[n * page + i] : from_f32<IO>(0.f);
         return;
     }
-    const Lane<IO, VEC, KT> my(p, blockIdx.y * WAVE + lane);
+    Lane<IO, VEC, KT> my(p, blockIdx.y * WAVE + lane);
+    my.read_weights();
     Wide<VEC> dw[KT], db{};
 #pragma unroll
     for (int j = 0; j < KT; ++j) dw[j] = Wide<VEC>{};
     for (int number = blockIdx.x * (THREADS / WAVE) + wave; number < p.rows * p.runs; number += run_blocks * (THREADS / WAVE)) {
-        Run r(p, __builtin_amdgcn_readfirstlane(number), lane);
-        // the gradients of a run's tokens come from up to K - 1 tokens behind it
-        const int stop = min(p.T, r.t1 + p.K - 1), to = p.seq.offsets ? min(stop, p.seq.at(p.N)) : stop;
+        Run r(p, __builtin_amdgcn_readfirstlane(number));
+        const int stop = min(p.T, r.t1 + p.K - 1);         // the gradients of a run's tokens come from up to K - 1 tokens behind it
         Packed<IO, VEC> ahead_x[AHEAD], ahead_g[AHEAD];
         const auto fetch = [&](int t) {
 #pragma unroll
@@ -37,6 +37,8 @@ __global__ __launch_bounds__(THREADS) void backward_kernel(const Params p, int r
             }
         };
         fetch(r.t0);
+        r.find(p, lane);
+        const int to = p.seq.offsets ? min(stop, p.seq.at(p.N)) : stop;
         Wide<VEC> x[KT], acc[KT];                          // acc[d]: what has come to token t - d
 #pragma unroll
         for (int j = 0; j < KT; ++j) acc[j] = x[j] = Wide<VEC>{};

@@ -14,18 +14,22 @@ struct Sequences {
     }
     // (the same i in all lanes)
     __device__ __forceinline__ int at(int i) const { return __builtin_amdgcn_readfirstlane(of_lane(i)); }
-    // The first sequence that ends behind token t, N if there is none: 64 offsets at a time, by all lanes of a wave together.
-    __device__ __forceinline__ int first_ending_behind(int t, int lane) const {
+    // The first sequence that ends behind token t, N if there is none, and its tokens [begin, end): 64 offsets at a time, by all lanes of a wave together.
+    __device__ __forceinline__ int first_ending_behind(int t, int lane, int& begin, int& end) const {
         int lo = 0, hi = N;                               // the answer is in lo .. hi
-        while (hi - lo > 0) {
-            const int step = (hi - lo + 63) / 64, i = lo + (lane + 1) * step - 1;   // the last of each piece
+        while (hi - lo > WAVE) {
+            const int step = (hi - lo + WAVE - 1) / WAVE, i = lo + (lane + 1) * step - 1;   // the last of each piece
             const bool before = i < hi && of_lane(i + 1) <= t;
             const int pieces = __popcll(__ballot(before));
-            const int from = min(lo + pieces * step, hi);
-            hi = min(from + step - 1, hi);
-            lo = from;
+            lo = min(lo + pieces * step, hi);
+            hi = min(lo + step - 1, hi);
         }
-        return __builtin_amdgcn_readfirstlane(lo);
+        lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+        const int i = min(lo + lane, N - 1), from = of_lane(i), to = of_lane(i + 1);   // (the answer's offsets with those that it is found by)
+        const int passed = __popcll(__ballot(lo + lane < hi && to <= t)), n = lo + passed;
+        begin = n < N ? passed < WAVE ? __builtin_amdgcn_readlane(from, passed) : at(n) : 0x7fffffff;
+        end = n < N ? passed < WAVE ? __builtin_amdgcn_readlane(to, passed) : at(n + 1) : 0x7fffffff;
+        return n;
     }
     // The tokens [from, to) of [r0, r1) that belong to a sequence.
     __device__ __forceinline__ void inside(int r0, int r1, int& from, int& to) const {
@@ -47,8 +51,7 @@ struct Walk {
             n = b, begin = 0, end = s.T;
             return;
         }
-        n = s.first_ending_behind(t, lane);
-        read(s);
+        n = s.first_ending_behind(t, lane, begin, end);
     }
     __device__ __forceinline__ void next(const Sequences& s) {
         const int done = end;
