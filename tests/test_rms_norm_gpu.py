@@ -198,3 +198,20 @@ def test_other_streams_and_graphs():
         torch.cuda.synchronize()
         for p, q in zip(recorded, call()):
             assert torch.equal(p, q), k
+
+
+@pytest.mark.parametrize("rows,C", [((1 << 24) + 5, 4), ((1 << 22) + 3, 3)])
+def test_more_rows_than_a_launch_has_in_one_dimension(rows, C):
+    x = torch.arange(rows * C, device=DEV, dtype=torch.float32).view(rows, C).remainder_(1021).sub_(500.25)
+    w = torch.linspace(0.5, 2, C, device=DEV).requires_grad_()
+    leaf = x.requires_grad_()
+    y = vr.rms_norm(leaf, w, eps=EPS)
+    gy = torch.ones_like(x)
+    gx, gw = torch.autograd.grad(y, [leaf, w], gy)
+    v, W = x.detach().double(), w.detach().double()
+    s = 1 / torch.sqrt((v * v).mean(-1, keepdim=True) + EPS)
+    n = v * s
+    near(y.detach(), n * W, (n * W).abs(), steps(C), "y")
+    mean = (W * n).mean(-1, keepdim=True)
+    near(gx, s * (W - n * mean), s * (W + n.abs() * (W * n.abs()).mean(-1, keepdim=True)), 2 * steps(C), "dx")
+    near(gw, n.sum(0), n.abs().sum(0), 2 * steps(C) + rows / 256 + 512, "dweight")

@@ -49,9 +49,12 @@ def test_scan_sizes():
     # the states in front of every sixteenth token, whatever the cuts
     assert L.vrwkv_scan_kept_bytes(a) == 2 * 19 * 96 * 16 * 4
     assert L.vrwkv_scan_kept_bytes(scan_args(S=5)) == 2 * 19 * 96 * 8 * 4
-    need = L.vrwkv_scan_fwd_workspace_bytes(a)
-    assert need > 0                                        # two sequences are cut
-    assert L.vrwkv_scan_fwd(scan_args(workspace_bytes=need - 1), None) == WORKSPACE and L.vrwkv_scan_fwd(scan_args(workspace=None), None) == WORKSPACE
+    assert L.vrwkv_scan_fwd_workspace_bytes(a) == 0        # few tokens of few channels: one launch
+    with vr.option("scan_segments", 3):
+        need = L.vrwkv_scan_fwd_workspace_bytes(a)
+        assert need > 0                                    # two sequences are cut
+        assert L.vrwkv_scan_fwd(scan_args(workspace_bytes=need - 1), None) == WORKSPACE and L.vrwkv_scan_fwd(scan_args(workspace=None), None) == WORKSPACE
+    assert L.vrwkv_scan_fwd_workspace_bytes(scan_args(E=9600)) > 0
     need = L.vrwkv_scan_bwd_workspace_bytes(a)
     assert L.vrwkv_scan_bwd(scan_args(workspace_bytes=need - 1), None) == WORKSPACE
     for gone in ("gy", "kept", "du", "ddelta", "dA", "dB", "dC"):
@@ -115,6 +118,23 @@ def test_bad_convolutions():
         return L.vrwkv_conv_step(a, None)
 
     assert [step(pool=None), step(N=0), step(K=1), step(dtype=3), step(N=5), step(page_stride=287), step(x=65), step(slots=66)] == [INVALID, INVALID, SHAPE, DTYPE, INVALID, INVALID, INVALID, INVALID]
+
+
+def test_more_channels_than_a_launch_takes():
+    L = _lib.lib()
+    assert L.vrwkv_scan_fwd(scan_args(E=(1 << 22) + 2), None) == SHAPE and L.vrwkv_scan_bwd(scan_args(G=(1 << 16) + 1, E=(1 << 16) + 1), None) == SHAPE
+    for f in (L.vrwkv_conv_fwd, L.vrwkv_conv_bwd):
+        assert f(conv_args(E=(1 << 22) - 63), None) == SHAPE
+    a = _lib.ScanStepArgs()
+    for n in ("u", "delta", "A", "B", "C", "pool", "y"):
+        setattr(a, n, 64)
+    a.N, a.P, a.E, a.S, a.G, a.page_stride = 1, 1, (1 << 22) + 1, 1, 1, 1 << 23
+    assert L.vrwkv_scan_step(a, None) == SHAPE
+    b = _lib.ConvStepArgs()
+    for n in ("x", "weight", "pool", "y"):
+        setattr(b, n, 64)
+    b.N, b.P, b.E, b.K, b.page_stride = 1, 1, (1 << 22) + 1, 2, 1 << 23
+    assert L.vrwkv_conv_step(b, None) == SHAPE
 
 
 def test_bad_norms():

@@ -356,6 +356,32 @@ def test_step_slots():
     assert not y[page == -1].any() and torch.isnan(y[page >= 4]).all()
 
 
+@pytest.mark.parametrize("E,S,G,dtype,shift", [(1100, 16, 2, "bf16", 0), (1090, 16, 1, "fp32", 1), (2200, 5, 2, "fp16", 0)])
+def test_steps_of_many_rows(E, S, G, dtype, shift):
+    """Pages named once, several times next to each other and far apart, and none, in a batch that fills the chip; a pool that does not lie at a multiple of 16 bytes."""
+    N, P = 530, 300
+    x, normal = inputs(1, N, E, S, G, dtype)
+    gen = torch.Generator().manual_seed(E)
+    page = torch.cat([torch.arange(200), torch.randint(180, P, (N - 220,), generator=gen), torch.tensor([5, 5, 5, 7, 7, 299, 299, 299, 299, 299, 5, 9, -1, -1, P, 9, 9, -7, 0, 0])])
+    page = page.view(-1, 2).flip(1).reshape(-1)
+    pool = torch.empty(P * E * S + shift, device=DEV)[shift:].view(P, E, S).copy_(normal(P, E, S))
+    before = pool.clone()
+    y = vr.selective_scan_step(x["u"][0], x["delta"][0], x["A"], x["B"][0], x["C"][0], pool, page.to(DEV), D=x["D"], z=x["z"][0], delta_bias=x["delta_bias"], softplus=True)
+    known = (page >= 0) & (page < P)
+    order = torch.arange(N)[known]
+    order = order[page[order].argsort(stable=True)]        # the rows of each page one after the other
+    pages, counts = page[order].unique_consecutive(return_counts=True)
+    ends = counts.cumsum(0).tolist()
+    rows = {n: x[n][:, order.to(DEV)] for n in ("u", "delta", "B", "C", "z")}
+    want = reference({**x, **rows, "state": before[pages.to(DEV)]}, [(0, j - n, j) for j, n in zip(ends, counts.tolist())], True)
+    compare(y[order.to(DEV)][None], want["y"], "y", int(counts.max()))
+    compare(pool[pages.to(DEV)], want["last"], "last", int(counts.max()))
+    rest = torch.ones(P, dtype=torch.bool)
+    rest[pages] = False
+    assert torch.equal(pool[rest.to(DEV)], before[rest.to(DEV)])
+    assert not y[(page == -1).to(DEV)].any() and torch.isnan(y[((page < -1) | (page >= P)).to(DEV)]).all()
+
+
 def test_step_pools():
     """Pages at a distance (one layer of a pool for all), without slots, pools without pages."""
     E, S = 24, 16

@@ -27,7 +27,8 @@ struct Plan {
 int lanes_of(int S) { return S <= 4 ? 1 : S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
 
 // Few sequences are cut into segments, which costs a pass over them in front of the one with the results: enough pieces for four waves on each of the chip's vector units, none
-// shorter than 32 tokens, no more than 64 (a segment goes through those in front of it).
+// shorter than 32 tokens, no more than 64 (a segment goes through those in front of it).  2 x 4150 tokens of 768 channels, bf16 forward: 690 us whole, 157 in 8, 84 in 43; 8 x 196 of
+// 1536, which have half as many waves without it, 36.8 whole and 35.9 in 7.
 Plan plan_of(const vrwkv_scan_args& a) {
     Plan p;
     p.P = lanes_of(a.S);
@@ -148,13 +149,14 @@ __global__ __launch_bounds__(THREADS) void finish_kernel(const Finish f) {
         } else if (f.dbias) put(f.dbias, i - A - f.E, f.bias_dtype, v);
         return;
     }
-    const long long i = (long long)(blockIdx.x - f.column_blocks) * THREADS + tid, all = f.tokens * f.G * 2 * f.W;
-    if (i >= all) return;
-    float v = 0.f;
+    const long long all = f.tokens * f.G * 2 * f.W;
+    for (long long i = (long long)(blockIdx.x - f.column_blocks) * THREADS + tid; i < all; i += (long long)(gridDim.x - f.column_blocks) * THREADS) {
+        float v = 0.f;
 #pragma unroll 8
-    for (int k = 0; k < f.blocks; ++k) v += f.part_bc[k * all + i];
-    const int n = (int)(i % f.W), which = (int)(i / f.W % 2);
-    if (n < f.S) put(which ? f.dC : f.dB, i / (2 * f.W) * f.S + n, f.dtype, v);
+        for (int k = 0; k < f.blocks; ++k) v += f.part_bc[k * all + i];
+        const int n = (int)(i % f.W), which = (int)(i / f.W % 2);
+        if (n < f.S) put(which ? f.dC : f.dB, i / (2 * f.W) * f.S + n, f.dtype, v);
+    }
 }
 
 }  // namespace
@@ -215,6 +217,6 @@ extern "C" int vrwkv_scan_bwd(const vrwkv_scan_args* args, void* hip_stream) {
     Finish f{bp.part_bc, bp.part_A, bp.part_D, bp.part_bias, a.dB, a.dC, a.dD, a.dbias, a.dA, (long long)pl.rows * a.T, (int)parts, pl.blocks, a.E, a.S, a.G, 4 * pl.P, a.dtype, a.D_dtype, a.bias_dtype, 0};
     const long long columns = (long long)a.E * (4 * pl.P + 2), sums = f.tokens * a.G * 8 * pl.P;
     f.column_blocks = (int)((columns + 63) / 64);
-    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)(f.column_blocks + (sums + THREADS - 1) / THREADS)), dim3(THREADS), 0, st, f);
+    hipLaunchKernelGGL(finish_kernel, dim3((unsigned)(f.column_blocks + std::min<long long>((sums + THREADS - 1) / THREADS, 1 << 20))), dim3(THREADS), 0, st, f);
     return check_launch("vrwkv_scan_bwd");
 }
