@@ -288,6 +288,33 @@ def test_infinities_and_nan_stay_with_their_tokens(dtype, segments, force):
         assert torch.equal(torch.isfinite(y.cpu()), torch.isfinite(want["y"][0]))
 
 
+@pytest.mark.parametrize("S", [10, 16, 35])
+@pytest.mark.parametrize("segments", [0, 1, 6])
+def test_infinite_step_sizes(segments, S, force):
+    """A step of any length forgets what is in front of it: no gradient comes to that, and nothing else knows of it."""
+    force("scan_segments", segments)
+    x, normal = inputs(2, 300, 12, S, 1, "fp32", state=2)
+    x["delta"][0, 40, 3] = x["u"][1, 290, 5] = float("inf")
+    leaves = {n: t.clone().requires_grad_() for n, t in x.items()}
+    y, last = vr.selective_scan(**leaves, softplus=True, return_state=True)
+    gy = normal(*y.shape)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), gy)))
+    want = reference(x, [(0, 0, 300), (1, 0, 300)], True, gy)
+    assert torch.equal(torch.isfinite(y.cpu()), torch.isfinite(want["y"][0])) and torch.equal(torch.isfinite(last.cpu()), torch.isfinite(want["last"][0]))
+    others = torch.ones(2, 300, 12, dtype=torch.bool)
+    others[0, 40:, 3] = others[1, 290:, 5] = False
+    for n in ("u", "delta", "z"):
+        ref, scale = want[NAMES[n]]
+        compare(grads[n].cpu()[others], (ref[others], scale[others]), NAMES[n], 300)
+    rows = others.all(2)
+    for n in ("B", "C"):
+        ref, scale = want[NAMES[n]]
+        compare(grads[n].cpu()[rows], (ref[rows], scale[rows]), NAMES[n], 300)
+    compare(grads["state"], want["dstate"], "dstate", 300)
+    clean = torch.tensor([e not in (3, 5) for e in range(12)])
+    compare(grads["A"].cpu()[clean], tuple(t[clean] for t in want["dA"]), "dA", 300, tokens=600)
+
+
 def test_states_far_from_one():
     """Decays that leave fp32 over a segment meet states of any size: nothing becomes NaN that the recurrence leaves finite."""
     x, _ = inputs(1, 640, 8, 16, 1, "fp32", state=1, softplus=False, bias=False)

@@ -199,6 +199,8 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
 #pragma unroll
             for (int i = 0; i < 4; ++i) h[i] = decayed(h[i], dt, a2[i]) + x[i];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = pad[i] ? 0.f : h[i];   // (an infinite step size makes what is not there NaN)
     }
 
     Rows<IO, P> raw;

@@ -161,7 +161,7 @@ __global__ __launch_bounds__(THREADS) void back_segments_kernel(const BackParams
                 const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(g[j / P]);
                 const f32x4 Ct = *reinterpret_cast<const f32x4*>(&bc[buf][j * 8 * P + 4 * P + 4 * at.p]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) R[k] = fast_exp2(d * a2[k]) * fmaf(Ct[k], v, R[k]);
+                for (int k = 0; k < 4; ++k) R[k] = !FULL && 4 * at.p + k >= p.S ? 0.f : fast_exp2(d * a2[k]) * fmaf(Ct[k], v, R[k]);
             });
         };
         if (row >= from && row + BATCH <= to && w.within(row, BATCH)) piece(std::false_type(), 0, 0);
@@ -250,6 +250,8 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) R[i] = decayed(R[i], dt, a2[i]) + x[i];
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) R[i] = pad[i] ? 0.f : R[i];   // (an infinite step size makes what is not there NaN)
         }
         // sixteen tokens' rows and their first state: asked for while the sums of those behind them are added up
         Rows<IO, P> raw;
@@ -348,6 +350,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                             dC[k] = gj * hs[j + 1][k];
                             along_B[j % P] = fmaf(r, Bt[k], along_B[j % P]);
                             R[k] = fast_exp2(d * a2[k]) * r;
+                            if (!FULL && pad[k]) R[k] = 0.f;
                             const float q = R[k] * hs[j][k];
                             along_A[j % P] = fmaf(q, a2[k], along_A[j % P]);
                             dA[k] = fmaf(q, d, dA[k]);

@@ -128,6 +128,8 @@ __global__ __launch_bounds__(W * WAVE) void short_kernel(const Params p, const i
 #pragma unroll
             for (int k = 0; k < NS; ++k) add(k, carry[buf][k][lane]);
         }
+#pragma unroll
+        for (int k = 0; k < NS; ++k) h[k] = pad[k] ? 0.f : h[k];   // (an infinite step size makes what is not there NaN)
         float y[P];
 #pragma unroll
         for (int j = 0; j < P; ++j) y[j] = 0.f;
