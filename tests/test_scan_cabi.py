@@ -130,10 +130,14 @@ def test_more_channels_than_a_launch_takes():
         setattr(a, n, 64)
     a.N, a.P, a.E, a.S, a.G, a.page_stride = 1, 1, (1 << 22) + 1, 1, 1, 1 << 23
     assert L.vrwkv_scan_step(a, None) == SHAPE
+    a.N, a.E = 1 << 30, 1
+    assert L.vrwkv_scan_step(a, None) == SHAPE
     b = _lib.ConvStepArgs()
     for n in ("x", "weight", "pool", "y"):
         setattr(b, n, 64)
     b.N, b.P, b.E, b.K, b.page_stride = 1, 1, (1 << 22) + 1, 2, 1 << 23
+    assert L.vrwkv_conv_step(b, None) == SHAPE
+    b.N, b.E = 1 << 30, 1
     assert L.vrwkv_conv_step(b, None) == SHAPE
 
 

@@ -179,6 +179,7 @@ extern "C" int vrwkv_conv_step(const vrwkv_conv_step_args* args, void* hip_strea
     if (a.N <= 0 || a.P <= 0 || a.E <= 0) { set_error("%s: N, P and E must be positive", who); return VRWKV_INVALID_ARG; }
     if (!typed(a.dtype) || !typed(a.param_dtype)) { set_error("%s: dtype must be fp32, bf16 or fp16", who); return VRWKV_UNSUPPORTED_DTYPE; }
     if (a.K < 2 || a.K > 8 || a.E > 1 << 22) { set_error("%s: 2 to 8 taps (%d), and at most 2^22 channels", who, a.K); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (a.N >= 1 << 30) { set_error("%s: 2^30 rows or more", who); return VRWKV_UNSUPPORTED_SHAPE; }
     if (!a.slots && a.N > a.P) { set_error("%s: %d rows without slots, and %d pages", who, a.N, a.P); return VRWKV_INVALID_ARG; }
     if (a.page_stride < (long long)(a.K - 1) * a.E) { set_error("%s: pages overlap", who); return VRWKV_INVALID_ARG; }
     if (!aligned(a.x, a.dtype) || !aligned(a.y, a.dtype) || !aligned(a.pool, a.dtype) || !aligned(a.weight, a.param_dtype) || !aligned(a.bias, a.param_dtype) ||

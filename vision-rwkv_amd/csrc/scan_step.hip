@@ -185,6 +185,7 @@ extern "C" int vrwkv_scan_step(const vrwkv_scan_step_args* args, void* hip_strea
         return VRWKV_UNSUPPORTED_DTYPE;
     }
     if (a.S < 1 || a.S > 64 || a.E % a.G || a.E > 1 << 22) { set_error("%s: 1 to 64 states (%d), E (%d, at most 2^22) a multiple of G (%d)", who, a.S, a.E, a.G); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (a.N >= 1 << 30) { set_error("%s: 2^30 rows or more", who); return VRWKV_UNSUPPORTED_SHAPE; }
     if (!a.slots && a.N > a.P) { set_error("%s: %d rows without slots, and %d pages", who, a.N, a.P); return VRWKV_INVALID_ARG; }
     if (a.page_stride < (long long)a.E * a.S) { set_error("%s: pages overlap", who); return VRWKV_INVALID_ARG; }
     const size_t w = a.dtype == VRWKV_F32 ? 3 : 1;
