@@ -30,6 +30,16 @@ struct Params {
     int N, rows, T, E, S, G, softplus, L, nseg, blocks;    // rows: of the batch; L: tokens of a segment; blocks: workgroups of a group's channels
 };
 
+// A kernel's arguments, read where they are asked for: kept in scalar registers they run over into lanes of vector registers, and come back from there one instruction a word.
+#define SCAN_CONSTANT __attribute__((opencl_constant))
+template <typename T>
+__device__ __forceinline__ const SCAN_CONSTANT T& arguments() {
+    unsigned none = 0;
+    asm volatile("" : "+s"(none));                         // (else all that is read through it is kept after all)
+    return *reinterpret_cast<const SCAN_CONSTANT T*>(reinterpret_cast<unsigned long long>(__builtin_amdgcn_kernarg_segment_ptr()) + none);
+}
+__device__ __forceinline__ Sequences sequences_of(const SCAN_CONSTANT Sequences& s) { return Sequences{s.offsets, s.is64, s.N, s.T}; }
+
 // log(1 + q) for q in 0 .. 1 as 2 atanh(q / (2 + q)): an odd series in s = q / (2 + q) <= 1/3, cut to five terms by a Chebyshev fit (8e-9 relative).  (1 + q rounded first
 // would cost 6e-8 / q: step sizes of a thousandth would be off by 6e-5.)
 __device__ __forceinline__ float log1p_unit(float q) {
@@ -98,7 +108,8 @@ template <typename IO, int P, int WHICH>
 struct Stage {
     static constexpr int ONE = BATCH * 4 * P, VALUES = ONE * WHICH, EACH = (VALUES + THREADS - 1) / THREADS;
     IO raw[EACH];
-    __device__ __forceinline__ void fetch(const Params& p, long long b, int g, int row, int from, int to) {
+    template <typename Args>
+    __device__ __forceinline__ void fetch(const Args& p, long long b, int g, int row, int from, int to) {
         const int first = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
 #pragma unroll
         for (int k = 0; k < EACH; ++k) {
@@ -205,6 +216,7 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
 
     Rows<IO, P> raw;
     const auto fetch = [&](Rows<IO, P>& x, int row) {
+        const auto& p = arguments<Params>();
         x.fetch(x.u, p.u, b * p.u_b, p.u_t, row, r1, at.p, e);
         x.fetch(x.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
         if (EMIT && p.z) x.fetch(x.z, p.z, b * p.z_b, p.z_t, row, r1, at.p, e);
@@ -218,15 +230,13 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
     int buf = 0;
     for (int row = r0; row < r1; row += BATCH, buf ^= 1) {
         const bool more = row + BATCH < r1;
-        if (more) {
-            stage.fetch(p, b, at.g, row + BATCH, from, to);
-        }
+        const auto& p = arguments<Params>();
+        if (more) stage.fetch(p, b, at.g, row + BATCH, from, to);
         if (EMIT && p.kept && at.there)
             at_row(reinterpret_cast<const f32x4*>(p.kept) + ((long long)b * ((p.T + BATCH - 1) / BATCH) + row / BATCH) * p.E * P, (unsigned)(e * P + at.p) * 16u) = f32x4{h[0], h[1], h[2], h[3]};
         const IO* const out = static_cast<const IO*>(p.y) + ((long long)b * p.T + row) * p.E;
         const unsigned place = (at.p * (unsigned)p.E + e) * sizeof(IO);
-        int width = p.E;
-        asm volatile("" : "+s"(width));
+        const int width = p.E;
         // tokens [first, behind) of the sixteen, all of one sequence; PART: not all sixteen.  P at a time: each lane's own, then the states of all, then each lane's own again
         const auto piece = [&](auto part_, int first, int behind) {
             constexpr bool PART = decltype(part_)::value;
@@ -282,7 +292,7 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Par
             else piece(std::true_type(), first, behind);
             if (behind < w.end) break;
             last_state(w.n);
-            w.next(p.seq);
+            w.next(sequences_of(p.seq));
         }
         if (more) {
             fetch(raw, row + BATCH);

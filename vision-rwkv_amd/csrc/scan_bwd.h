@@ -199,8 +199,10 @@ template <typename IO, int P, bool FULL>
 __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
     const Params& p = bp.f;
     constexpr int OWN = BATCH / P, COUNT = 64 / P, ROW = 8 * P, SUMS = BATCH * ROW, WAVES = THREADS / WAVE;
+    constexpr bool KEEP = P <= 4;                          // (two workgroups a compute unit with 75 KB each; more lanes a channel have more sums in LDS: no room)
     __shared__ __attribute__((aligned(16))) float bc[SUMS];
     __shared__ float red[WAVES][SUMS];
+    __shared__ f32x4 decays[KEEP ? BATCH : 1][THREADS];    // of the sixteen tokens, from the way along them for the way back
     const Place<P> at(p.E, p.G, p.blocks);
     const int s = blockIdx.y, r0 = s * p.L, r1 = min(p.T, r0 + p.L), e = at.e, wave = threadIdx.x >> 6;
     const long long part = (long long)blockIdx.z * p.nseg + s;
@@ -215,12 +217,15 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
     }
     const float bias = p.bias.p ? p.bias.value(p.bias.fetch(e)) : 0.f, skip = p.D.p ? p.D.value(p.D.fetch(e)) : 0.f;
     const auto state_of = [&](const float* t, int n, float (&h)[4]) {
+        const auto& p = arguments<BackParams>().f;
         int e = at.e;
         asm volatile("" : "+v"(e));                        // (no address of this is kept)
 #pragma unroll
         for (int k = 0; k < 4; ++k) h[k] = t && !pad[k] ? t[((long long)n * p.E + e) * p.S + 4 * at.p + k] : 0.f;
     };
     const auto first_gradient = [&](int n, const float (&h)[4]) {
+        const auto& bp = arguments<BackParams>();
+        const auto& p = bp.f;
         if (!bp.dstate || !at.there) return;
         int e = at.e;
         asm volatile("" : "+v"(e));
@@ -258,6 +263,8 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
         f32x4 kept;
         Stage<IO, P, 2> stage;
         const auto fetch = [&](int row) {
+            const auto& bp = arguments<BackParams>();
+            const auto& p = bp.f;
             raw.fetch(raw.u, p.u, b * p.u_b, p.u_t, row, r1, at.p, e);
             raw.fetch(raw.d, p.delta, b * p.d_b, p.d_t, row, r1, at.p, e);
             raw.fetch(raw.g, bp.gy, b * bp.gy_b, bp.gy_t, row, r1, at.p, e);
@@ -271,6 +278,8 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
         const float* const part_row = bp.part_bc + (((long long)(blockIdx.x % p.blocks) * p.rows + b) * p.T * p.G + at.g) * ROW;
         for (int row = last; row >= r0; row -= BATCH) {
             const bool more = row > r0;
+            const auto& bp = arguments<BackParams>();
+            const auto& p = bp.f;
             // a lane's own tokens: step size and its slope, u, g, and gy silu'(z)
             float dt[OWN], bend[OWN], u[OWN], g[OWN], gz[OWN];
 #pragma unroll
@@ -288,8 +297,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
             }
             const long long out = ((long long)b * p.T + row) * p.E;
             const unsigned place = (at.p * (unsigned)p.E + e) * sizeof(IO);
-            int width = p.E;
-            asm volatile("" : "+s"(width));
+            const int width = p.E;
             const auto put = [&](void* t, int token, float v) { at_row(static_cast<const IO*>(t) + out + (long long)token * width, place) = from_f32<IO>(v); };
             // tokens [first, behind) of the sixteen, all of one sequence, from the state h in front of them; PART: not all sixteen
             const auto piece = [&](auto part_, int first, int behind, const float (&h)[4]) {
@@ -315,11 +323,14 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                         if (outside(j)) return;
                         const float d = from_lane<P, q>(dt[i]), v = from_lane<P, q>(dt[i] * u[i]);
                         const f32x4 Bt = pairs.B[j % 2], Ct = pairs.C[j % 2];
+                        f32x4 decay;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            hs[j + 1][k] = fmaf(fast_exp2(d * a2[k]), hs[j][k], v * Bt[k]);
+                            decay[k] = fast_exp2(d * a2[k]);
+                            hs[j + 1][k] = fmaf(decay[k], hs[j][k], v * Bt[k]);
                             if (!FULL && pad[k]) hs[j + 1][k] = 0.f;
                         }
+                        if (KEEP) decays[j][threadIdx.x] = decay;
                         y[q] = fmaf(Ct[3], hs[j + 1][3], fmaf(Ct[2], hs[j + 1][2], fmaf(Ct[1], hs[j + 1][1], Ct[0] * hs[j + 1][0])));
                         asm volatile("" : "+v"(y[q]));     // (else it is made where z is looked at, from what had to wait in registers)
                     });
@@ -328,17 +339,25 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                         if (at.there && !outside(lane_token + i * P)) put(bp.dz, i * P, gz[i] * fmaf(skip, u[i], y[0]));
                     }
                 });
-                // (the exponentials are taken and B and C read again: kept, they would fill three times as many registers as the states)
+                // (B and C are read again, and the exponentials come from LDS: kept, they would fill three times as many registers as the states)
                 int again = at.p;
                 asm volatile("" : "+v"(again));
 #pragma unroll
                 for (int i = 0; i < OWN; ++i) asm volatile("" : "+v"(dt[i]));
                 pairs.start(bc, BATCH / 2 - 1, again);
                 float along_B[P], along_A[P], sums[COUNT];
+                f32x4 decay[2], decay_next[2];             // of two tokens, as B and C
+                if (KEEP) decay_next[0] = decays[BATCH - 2][threadIdx.x], decay_next[1] = decays[BATCH - 1][threadIdx.x];
                 each(std::make_integer_sequence<int, BATCH>(), [&](auto j_) {
                     constexpr int j = BATCH - 1 - decltype(j_)::value;
                     along_A[j % P] = along_B[j % P] = 0.f;
-                    if (j % 2 == 1) pairs.advance(bc, j / 2, j / 2 - 1, again);
+                    if (j % 2 == 1) {
+                        if (KEEP) {
+                            decay[0] = decay_next[0], decay[1] = decay_next[1];
+                            if (j > 1) decay_next[0] = decays[j > 1 ? j - 3 : 0][threadIdx.x], decay_next[1] = decays[j > 1 ? j - 2 : 0][threadIdx.x];
+                        }
+                        pairs.advance(bc, j / 2, j / 2 - 1, again);
+                    }
                     float dB[4] = {0.f, 0.f, 0.f, 0.f}, dC[4] = {0.f, 0.f, 0.f, 0.f};
                     if (!outside(j)) {
                         const float d = from_lane<P, j % P>(dt[j / P]), v = from_lane<P, j % P>(dt[j / P] * u[j / P]), gj = from_lane<P, j % P>(g[j / P]);
@@ -349,7 +368,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                             dB[k] = r * v;
                             dC[k] = gj * hs[j + 1][k];
                             along_B[j % P] = fmaf(r, Bt[k], along_B[j % P]);
-                            R[k] = fast_exp2(d * a2[k]) * r;
+                            R[k] = (KEEP ? decay[j % 2][k] : fast_exp2(d * a2[k])) * r;
                             if (!FULL && pad[k]) R[k] = 0.f;
                             const float q = R[k] * hs[j][k];
                             along_A[j % P] = fmaf(q, a2[k], along_A[j % P]);
@@ -416,7 +435,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                 first_gradient(w.n, R);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) R[k] = 0.f;
-                w.previous(p.seq);
+                w.previous(sequences_of(p.seq));
             }
             if (more) fetch(row - BATCH);
             lds_barrier();
