@@ -5,7 +5,7 @@
 // belongs to a token and channel alone (step size, softplus, gate, rounding) is computed by one lane of the P for every P-th token, and handed to
 // the others in registers; sums over states go the same way back.  B and C of sixteen tokens lie in LDS in fp32, for the 256 / P channels of a workgroup.
 //
-// 64 x 196 tokens of 1536 channels with 16 states, bf16: 117 us, 196 cycles a token and wave, which is what its instructions take (a vector operation between exponentials 4.5 cycles, an
+// 64 x 196 tokens of 1536 channels with 16 states, bf16: 108 us, 220 cycles a token and wave, of which its 36 instructions take 196 (a vector operation between exponentials 4.5 cycles, an
 // exponential 8.3); the bytes alone 30.
 #pragma once
 #include "lanes.h"

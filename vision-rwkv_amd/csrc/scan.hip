@@ -46,7 +46,7 @@ Plan plan_of(const vrwkv_scan_args& a) {
 }
 
 // Whether a forward goes through scan_short.h: one workgroup a compute unit, and four rounds of its waves over the tokens.  bf16, 16 states, that kernel against the segments': 196 tokens of
-// 384 channels 8.0 us for 16.3, 1024 of 384 22 for 27; beyond it 196 of 1536 (384 workgroups) 15.2 for 15.7, 4 x 196 of 1536 45 for 24, 4150 of 384 80 for 51.
+// 384 channels 7.9 us for 16.3, 1024 of 384 23 for 27; beyond it 196 of 1536 (384 workgroups) 13.6 for 15.2, 1024 of 1536 45 for 32, 4 x 196 of 1536 39 for 24, 4150 of 384 80 for 51.
 bool is_short(const vrwkv_scan_args& a) {
     const long long groups = (long long)(a.offsets ? 1 : a.N) * a.G * ((a.E / a.G + SHORT_CHANNELS - 1) / SHORT_CHANNELS);
     return !option(OPT_SCAN_SEGMENTS) && groups <= device_cus() && a.T <= 4 * BATCH * short_waves(a.S);

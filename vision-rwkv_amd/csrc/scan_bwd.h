@@ -7,8 +7,8 @@
 // four states each, as in the forward.  dB and dC add up channels, which lie in other lanes: the sums of two tokens go through the wave in halves
 // (two instructions for a sum of 64 / P lanes), then through LDS over the waves, and over workgroups by the launch that ends the pass.
 //
-// 64 x 196 tokens of 1536 channels with 16 states, bf16: 360 us, bound by the instructions (110 a token and wave) with the registers of two waves a vector unit.  Three waves, with states kept of
-// eight tokens at a time and the eight in front of them gone through twice, take as long (366), four 465.
+// 64 x 196 tokens of 1536 channels with 16 states, bf16: 340 us, bound by the instructions (110 a token and wave) with the registers of two waves a vector unit.  Three waves, with states held of
+// eight tokens at a time and the eight in front of them gone through twice, took as long as two (366 and 370 before the decays were kept in LDS), four 465.
 #pragma once
 #include "scan.h"
 

@@ -3,7 +3,7 @@
 // What bounds such a call is the way from one token to the next and the launches, not the chip: time is cut inside a workgroup, a wave has sixteen tokens of four channels and the waves
 // beside it the tokens behind.  Sixteen lanes hold one channel: lane p has token p of the sixteen for what belongs to a token alone, and states p, p + 16, .. for the rest.  A wave goes through
 // its tokens from zeros, with every decay and product kept in registers; then the waves exchange their last states and sums of step sizes, each works out the states in front of its own
-// tokens, and goes through them once more with what it kept: no exponential is made twice.  196 tokens of 384 channels with 16 states in bf16: 8.0 us (an empty launch: about 4).
+// tokens, and goes through them once more with what it kept: no exponential is made twice.  196 tokens of 384 channels with 16 states in bf16: 7.9 us (a launch of a few instructions: about 4).
 #pragma once
 #include "scan.h"
 
@@ -36,6 +36,7 @@ __global__ __launch_bounds__(W * WAVE) void short_kernel(const Params p, const i
     const auto first_state = [&](int n, int k) { return p.state && !pad[k] ? p.state[((long long)n * p.E + e) * p.S + q + P * k] : 0.f; };
     int buf = 0;
     for (int row0 = 0; row0 < p.T; row0 += waves * BATCH, buf ^= 1) {
+        const auto& p = arguments<Params>();
         const int row = row0 + wave * BATCH, read = min(row, p.T - 1), behind_read = p.T - 1 - read;
         // everything that is read, before the first of it is needed
         const auto own = [&](const void* x, long long base, long long stride) {
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(W * WAVE) void short_kernel(const Params p, const i
                 raw_C[i * NS + k] = at_row(C, (j * (unsigned)p.C_t + n) * sizeof(IO));
             }
         Walk w;
-        w.find(p.seq, b, max(read, from), lane);
+        w.find(sequences_of(p.seq), b, max(read, from), lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(W * WAVE) void short_kernel(const Params p, const i
                 else f(std::true_type(), first, behind);
                 if (behind < at.end) break;
                 ends(at.n);
-                at.next(p.seq);
+                at.next(sequences_of(p.seq));
             }
         };
         const float dt = p.softplus ? softplus(raw) : raw, x = dt * u;
