@@ -160,7 +160,7 @@ __device__ __forceinline__ void each(std::integer_sequence<int, I...>, F&& f) { 
 // EMIT: the outputs of a segment from the states in front of it; without, its last states from zeros (or from its sequence's first states) and its sum of step sizes.
 // FULL: S is 4 P, so that no state is there to fill up.
 template <typename IO, int P, bool FULL, bool EMIT>
-__global__ __launch_bounds__(THREADS, P >= 4 ? 5 : 2) void scan_kernel(const Params p) {
+__global__ __launch_bounds__(THREADS, P >= 4 ? 4 : 2) void scan_kernel(const Params p) {
     constexpr int OWN = BATCH / P, WHICH = EMIT ? 2 : 1;
     __shared__ __attribute__((aligned(16))) float bc[2][BATCH * WHICH * 4 * P];
     const Place<P> at(p.E, p.G, p.blocks);
