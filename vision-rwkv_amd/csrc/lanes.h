@@ -3,7 +3,7 @@
 
 namespace vrwkv {
 
-// Values exchanged between the lanes of a group of P = 1, 2, 4, 8 or 16 neighbours, in registers.
+// Values exchanged between the lanes of a group of P = 2, 4, 8 or 16 neighbours, in registers.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
@@ -13,8 +13,7 @@ constexpr int DPP_ROW_BROADCAST = 0x150;                  // + a lane of the row
 // x of lane Q of the group
 template <int P, int Q>
 __device__ __forceinline__ float from_lane(float x) {
-    if constexpr (P == 1) return x;
-    else if constexpr (P == 2) return dpp<Q | Q << 2 | (2 + Q) << 4 | (2 + Q) << 6>(x);
+    if constexpr (P == 2) return dpp<Q | Q << 2 | (2 + Q) << 4 | (2 + Q) << 6>(x);
     else if constexpr (P == 4) return dpp<Q * 0x55>(x);
     else if constexpr (P == 8) {
         const int low = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), DPP_ROW_BROADCAST + Q, 0xf, 0xf, true);

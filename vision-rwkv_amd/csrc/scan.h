@@ -326,7 +326,6 @@ __global__ __launch_bounds__(THREADS, P >= 4 ? 4 : 2) void scan_kernel(const Par
 template <typename F>
 int with_lanes(int S, F&& f) {
     const auto full = [&](auto P) { return S == 4 * decltype(P)::value ? f(P, std::true_type()) : f(P, std::false_type()); };
-    if (S <= 4) return full(std::integral_constant<int, 1>());
     if (S <= 8) return full(std::integral_constant<int, 2>());
     if (S <= 16) return full(std::integral_constant<int, 4>());
     if (S <= 32) return full(std::integral_constant<int, 8>());

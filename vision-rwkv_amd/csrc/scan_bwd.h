@@ -77,16 +77,9 @@ __device__ __forceinline__ void sum_over_channels(float (&v)[64 / P], int lane) 
         fold4<N / 4>(v);
         fold_rows<N / 8, true>(v);
         fold_rows<N / 16, false>(v);
-        if constexpr (P <= 2) {
-#pragma unroll
-            for (int i = 0; i < N / 32; ++i) {
-                const float a = v[i] + across<2>(v[i]), b = v[i + N / 32] + across<2>(v[i + N / 32]);
-                v[i] = lane & 2 ? b : a;
-            }
-        }
-        if constexpr (P == 1) {
-            const float a = v[0] + across<1>(v[0]), b = v[1] + across<1>(v[1]);
-            v[0] = lane & 1 ? b : a;
+        if constexpr (P == 2) {
+            const float a = v[0] + across<2>(v[0]), b = v[1] + across<2>(v[1]);
+            v[0] = lane & 2 ? b : a;
         }
     } else if constexpr (P == 8) {
         fold8<4>(v);
@@ -102,7 +95,7 @@ __device__ __forceinline__ int sum_of_lane(int lane) {
     const int rows = (lane >> 5 & 1) * 2 + (lane >> 4 & 1);  // the lanes' bits in the order of the steps
     if constexpr (P == 16) return rows;
     else if constexpr (P == 8) return (lane >> 3 & 1) * 4 + rows;
-    else return ((lane >> 3 & 1) * 8 + (lane >> 2 & 1) * 4 + rows) * (4 / P) + (P == 4 ? 0 : P == 2 ? lane >> 1 & 1 : (lane >> 1 & 1) * 2 + (lane & 1));
+    else return ((lane >> 3 & 1) * 8 + (lane >> 2 & 1) * 4 + rows) * (4 / P) + (P == 4 ? 0 : lane >> 1 & 1);
 }
 
 // The gradient that each segment behind the first hands on, from zeros behind it (or from its sequence's end), and its sum of step sizes.
