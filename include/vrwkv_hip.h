@@ -455,7 +455,7 @@ int vrwkv_conv_step(const vrwkv_conv_step_args* args, void* hip_stream);
 
 /* r = x + residual, rounded to residual_dtype (without residual: x), y = r / sqrt(mean(r^2) + eps) weight over rows of C channels, the mean in fp32.  x, y of dtype,
  * residual and sum of residual_dtype, dtype or fp32; weight (C) of weight_dtype; rows contiguous, x_stride and residual_stride apart.  sum: r, or NULL.
- * out_kind: VRWKV_Y_SAME: y of dtype; VRWKV_Y_E4M3, VRWKV_Y_INT8: y / scale rounded to nearest even, 8 bits each, with scale (rows) fp32 = max(max |y| / top, 2^-126), top 448 or
+ * out_kind: VRWKV_Y_SAME: y of dtype; VRWKV_Y_E4M3, VRWKV_Y_INT8: the quotient y / scale in fp32, rounded to nearest even in 8 bits, with scale (rows) fp32 = max(max |y| / top, 2^-126), top 448 or
  * 127; a row whose maximum is NaN has a scale of NaN, e4m3 values of NaN and int8 values of 0.
  * Backward: r is `sum` as the forward returned it, gsum (of residual_dtype, or NULL) its gradient; dx of dtype, dresidual of residual_dtype or NULL, dweight (C) of weight_dtype or NULL. */
 enum { VRWKV_Y_SAME = 0, VRWKV_Y_E4M3 = 1, VRWKV_Y_INT8 = 2 };

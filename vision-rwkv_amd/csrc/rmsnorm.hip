@@ -58,12 +58,16 @@ __device__ __forceinline__ float inverse_root(float v) {
 }
 
 __device__ __forceinline__ float top_of(int kind) { return kind == VRWKV_Y_INT8 ? 127.f : 448.f; }
-// four results of a row in 8 bits
-__device__ __forceinline__ unsigned packed8(const float* v, float inverse, float top, int kind) {
+// What a row's results are divided by: 1 / scale and -scale (0 where the scale is infinite: nothing is left over from a product with that).
+struct Divisor { float inverse, minus; };
+// four results of a row in 8 bits.  The quotient by the scale is rounded once: the product with the rounded 1 / scale is off by up to one and a half units, which puts a quotient on the border of two
+// numbers (of a bf16 row and weight one in three thousand is) on the wrong side of it; what is left of v after the product, times 1 / scale, is what it lacks.
+__device__ __forceinline__ unsigned packed8(const float* v, Divisor by, float top, int kind) {
     float q[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        q[k] = v[k] * inverse;
+        q[k] = v[k] * by.inverse;
+        q[k] = fmaf(fmaf(q[k], by.minus, v[k]), by.inverse, q[k]);
         q[k] = q[k] > top ? top : q[k] < -top ? -top : q[k];   // (a NaN stays one)
     }
     if (kind == VRWKV_Y_E4M3) {
@@ -75,11 +79,12 @@ __device__ __forceinline__ unsigned packed8(const float* v, float inverse, float
     for (int k = 0; k < 4; ++k) r |= ((unsigned)(int)(q[k] == q[k] ? rintf(q[k]) : 0.f) & 0xffu) << (8 * k);
     return r;
 }
-// the row's scale and what its results are multiplied by
-__device__ __forceinline__ float scale_of(float most, float top, float& inverse) {
+// the row's scale and what its results are divided by
+__device__ __forceinline__ float scale_of(float most, float top, Divisor& by) {
     float s = most / top;
     s = s < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : s;
-    inverse = 1.f / s;
+    by.inverse = 1.f / s;
+    by.minus = fabsf(s) < __builtin_inff() ? -s : 0.f;
     return s;
 }
 
@@ -129,7 +134,7 @@ __device__ __forceinline__ void sum_of(const Params& p, long long row, int c, fl
     }
 }
 template <typename IO, int VEC>
-__device__ __forceinline__ void put_row(const Params& p, long long row, int c, const float (&y)[VEC], float inverse) {
+__device__ __forceinline__ void put_row(const Params& p, long long row, int c, const float (&y)[VEC], Divisor by) {
     if (p.out_kind == VRWKV_Y_SAME) {
         write<IO, VEC>(p.y, row * p.C + c, y);
         return;
@@ -137,10 +142,10 @@ __device__ __forceinline__ void put_row(const Params& p, long long row, int c, c
     unsigned char* to = static_cast<unsigned char*>(p.y) + row * p.C + c;
     if constexpr (VEC % 4 == 0) {
 #pragma unroll
-        for (int k = 0; k < VEC; k += 4) reinterpret_cast<unsigned*>(to)[k / 4] = packed8(&y[k], inverse, top_of(p.out_kind), p.out_kind);
+        for (int k = 0; k < VEC; k += 4) reinterpret_cast<unsigned*>(to)[k / 4] = packed8(&y[k], by, top_of(p.out_kind), p.out_kind);
     } else {
         const float v[4] = {y[0], 0.f, 0.f, 0.f};
-        *to = (unsigned char)packed8(v, inverse, top_of(p.out_kind), p.out_kind);
+        *to = (unsigned char)packed8(v, by, top_of(p.out_kind), p.out_kind);
     }
 }
 
@@ -173,7 +178,8 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(const Params p) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) s = fmaf(r[i][k], r[i][k], s);
     s = inverse_root(agreed<WAVES, false>(s, red) / (float)p.C + p.eps);
-    float most = 0.f, inverse = 0.f;
+    float most = 0.f;
+    Divisor by{};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * 64 * WAVES + lane) * VEC;
@@ -184,13 +190,13 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(const Params p) {
         }
     }
     if (p.out_kind != VRWKV_Y_SAME) {
-        const float v = scale_of(agreed<WAVES, true>(most, red), top_of(p.out_kind), inverse);
+        const float v = scale_of(agreed<WAVES, true>(most, red), top_of(p.out_kind), by);
         if (lane == 0) p.scale[row] = v;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * 64 * WAVES + lane) * VEC;
-        if (c < p.C) put_row<IO, VEC>(p, row, c, r[i], inverse);
+        if (c < p.C) put_row<IO, VEC>(p, row, c, r[i], by);
     }
 }
 
@@ -207,19 +213,20 @@ __global__ __launch_bounds__(THREADS) void forward_any_kernel(const Params p) {
         s = fmaf(r[0], r[0], s);
     }
     s = inverse_root(agreed<4, false>(s, red) / (float)p.C + p.eps);
-    float most = 0.f, inverse = 0.f;
+    float most = 0.f;
+    Divisor by{};
     const auto value = [&](int c) {
         sum_of<IO, RES, 1>(p, row, c, r);
         return r[0] * s * p.w.value(p.w.fetch(c));
     };
     if (p.out_kind != VRWKV_Y_SAME) {
         for (int c = threadIdx.x; c < p.C; c += THREADS) most = larger(most, value(c));
-        const float v = scale_of(agreed<4, true>(most, red), top_of(p.out_kind), inverse);
+        const float v = scale_of(agreed<4, true>(most, red), top_of(p.out_kind), by);
         if (threadIdx.x == 0) p.scale[row] = v;
     }
     for (int c = threadIdx.x; c < p.C; c += THREADS) {
         const float y[1] = {value(c)};
-        put_row<IO, 1>(p, row, c, y, inverse);
+        put_row<IO, 1>(p, row, c, y, by);
     }
 }
 

@@ -129,7 +129,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, quantize=None):
     x (..., C) float32, bfloat16 or float16, weight (C,) of x's dtype or float32, residual of x's shape and of its dtype or float32.  The mean and everything behind it is
     fp32, rounded once.  Gradients for all three; no second ones, no forward mode, no tracing (a compiled program makes the call as it is).
     quantize: torch.float8_e4m3fn or torch.int8: (q, scale) or (q, scale, r) instead, y = q scale with scale (...) in float32, the row's largest |y| over 448 or 127 (2^-126 at least) and
-    q = y / scale rounded to the nearest; y is not rounded before.  A row with a NaN has a scale of NaN.  Forward only."""
+    q = y / scale, a quotient of fp32 numbers, rounded to the nearest (even) of 8 bits; y is not rounded to x's type before.  A row with a NaN has a scale of NaN.  Forward only."""
     if torch.compiler.is_compiling():
         return _eager(rms_norm)(x, weight, residual, eps, quantize)
     if isinstance(eps, torch.Tensor):                      # (it would go in without its gradient)
