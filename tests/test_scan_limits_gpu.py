@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import vision_rwkv_amd as vr
+from vision_rwkv_amd import _lib
 
 DEV = "cuda"
 pytestmark = pytest.mark.gpu
@@ -48,3 +49,80 @@ def test_eight_bits_beside_an_infinity(C):
         others = torch.arange(C) != 3
         assert torch.isinf(scale).all() and not q.float().cpu()[:, others].any()
         assert torch.isnan(q[:, 3].float()).all() if kind != torch.int8 else not q[:, 3].any()
+
+
+# ---- offsets that do not ascend ------------------------------------------------------------------------------------------
+
+class _Guarded:
+    """Outputs inside one buffer, with room around each that nothing may write."""
+
+    def __init__(self):
+        self.parts = []
+
+    def __call__(self, dtype, *shape):
+        n, room = 1, 4096
+        for k in shape:
+            n *= k
+        whole = torch.full((n + 2 * room,), 77.0, dtype=dtype, device=DEV)
+        self.parts.append((whole, room, n))
+        return whole[room:room + n]
+
+    def untouched(self):
+        return all((w[:r] == 77).all() and (w[r + n:] == 77).all() for w, r, n in self.parts)
+
+
+def _disordered(count, seed):
+    """Offsets out of order, outside the rows, and the ones that made the convolution's gradients write in front of the states': (T, offsets)."""
+    g = torch.Generator().manual_seed(seed)
+    yield 40, [0, 30, 10, 40]
+    for k in range(count):
+        T, N = int(torch.randint(1, 300, (1,), generator=g)), (1, 2, 5, 20, 150)[k % 5]
+        yield T, torch.randint(-9, T + 9, (N + 1,), generator=g).tolist()
+
+
+@pytest.mark.parametrize("K", [2, 4, 7])
+@pytest.mark.parametrize("E", [24, 7])
+def test_convolution_of_disordered_offsets_stays_in_its_tensors(K, E):
+    L = _lib.lib()
+    for T, first in _disordered(40, K):
+        N, x = len(first) - 1, torch.randn(T, E, device=DEV)
+        gy, w, state, glast = torch.randn(T, E, device=DEV), torch.randn(E, K, device=DEV), torch.randn(N, K - 1, E, device=DEV), torch.randn(N, K - 1, E, device=DEV)
+        offsets, new = torch.tensor(first, device=DEV), _Guarded()
+        a = _lib.ConvArgs()
+        a.N, a.T, a.E, a.K, a.silu, a.offsets64 = N, T, E, K, 1, 1
+        a.x_stride = a.gy_stride = (0, E)
+        out = dict(y=new(torch.float32, T, E), last=new(torch.float32, N, K - 1, E), dx=new(torch.float32, T, E), dweight=new(torch.float32, E, K), dstate=new(torch.float32, N, K - 1, E))
+        for n, t in dict(x=x, weight=w, state=state, offsets=offsets, gy=gy, glast=glast, **out).items():
+            setattr(a, n, t.data_ptr())
+        assert L.vrwkv_conv_fwd(a, None) == 0
+        a.workspace_bytes = L.vrwkv_conv_bwd_workspace_bytes(a)
+        workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=DEV)
+        a.workspace = workspace.data_ptr()
+        assert L.vrwkv_conv_bwd(a, None) == 0
+        torch.cuda.synchronize()
+        assert new.untouched(), first
+
+
+@pytest.mark.parametrize("segments", [0, 1, 5])
+@pytest.mark.parametrize("E,S", [(24, 16), (7, 5)])
+def test_scan_of_disordered_offsets_stays_in_its_tensors(E, S, segments, force):
+    force("scan_segments", segments)
+    L = _lib.lib()
+    for T, first in _disordered(25, S):
+        N, normal, new, f = len(first) - 1, lambda *s: torch.randn(*s, device=DEV), _Guarded(), torch.float32
+        offsets = torch.tensor(first, device=DEV)
+        a = _lib.ScanArgs()
+        a.N, a.T, a.E, a.S, a.G, a.softplus, a.offsets64 = N, T, E, S, 1, 1, 1
+        a.u_stride = a.delta_stride = a.z_stride = a.gy_stride = (0, E)
+        a.B_stride = a.C_stride = (0, S, S)
+        inputs = dict(u=normal(T, E), delta=normal(T, E), z=normal(T, E), gy=normal(T, E), B=normal(T, S), C=normal(T, S), A=-normal(E, S).abs(), state=normal(N, E, S), glast=normal(N, E, S), offsets=offsets)
+        kept = L.vrwkv_scan_kept_bytes(a) // 4
+        out = dict(y=new(f, T, E), last=new(f, N, E, S), kept=new(f, kept), du=new(f, T, E), ddelta=new(f, T, E), dz=new(f, T, E), dB=new(f, T, S), dC=new(f, T, S), dA=new(f, E, S), dstate=new(f, N, E, S))
+        for n, t in {**inputs, **out}.items():
+            setattr(a, n, t.data_ptr())
+        for call, size in ((L.vrwkv_scan_fwd, L.vrwkv_scan_fwd_workspace_bytes), (L.vrwkv_scan_bwd, L.vrwkv_scan_bwd_workspace_bytes)):
+            room = new(torch.uint8, max(16, size(a)))
+            a.workspace, a.workspace_bytes = room.data_ptr(), size(a)
+            assert call(a, None) == 0
+        torch.cuda.synchronize()
+        assert new.untouched(), first

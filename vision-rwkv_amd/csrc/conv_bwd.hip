@@ -45,7 +45,7 @@ __global__ __launch_bounds__(THREADS) void backward_kernel(const Params p, int r
 #pragma unroll
         for (int j = 0; j < KT - 1; ++j)
             if (r.w.begin < r.t0 && my.used(j)) x[j + 1] = my.token(r.w.n, r.b, r.t0 - (KT - 1) + j, r.w.begin);
-        // token t of the sequence, or of its first state, is complete
+        // token t of the sequence, or of its first state, is complete (of offsets that do not ascend a sequence may begin behind the token it is looked up for: nothing in front of its state is written)
         const auto done = [&](int t, Wide<VEC> v, int tail) {
             if (tail >= 0 && p.glast) {
                 const Wide<VEC> g = my.row(p.glast, ((long long)r.w.n * (p.K - 1) + tail) * p.E);
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(THREADS) void backward_kernel(const Params p, int r
             }
             if (t >= r.w.begin) {
                 if (t >= r.t0 && t < r.t1) my.store(p.dx, ((long long)r.b * p.T + t) * p.E, v);
-            } else if (p.dstate && r.w.begin >= r.t0 && r.w.begin < r.t1) my.store(p.dstate, ((long long)r.w.n * (p.K - 1) + t - r.w.begin + p.K - 1) * p.E, v);
+            } else if (p.dstate && t >= r.w.begin - (p.K - 1) && r.w.begin >= r.t0 && r.w.begin < r.t1) my.store(p.dstate, ((long long)r.w.n * (p.K - 1) + t - r.w.begin + p.K - 1) * p.E, v);
         };
         bool over = false;
         for (int t = r.t0; t < stop && !over; t += AHEAD) {

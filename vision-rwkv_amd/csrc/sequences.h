@@ -4,7 +4,8 @@
 namespace vrwkv {
 
 // The sequences of a batch of token rows: row b of the batch whole, or with offsets (N + 1 of 32 or 64 bits, ascending) N of them packed in one row of T tokens,
-// n at tokens offsets[n] to offsets[n + 1].  Offsets outside 0 .. T are taken as 0 or T, so that no token outside the rows is named whatever they hold.
+// n at tokens offsets[n] to offsets[n + 1].  Offsets outside 0 .. T are taken as 0 or T, so that no token outside the rows is named whatever they hold, and a Walk's n is one of the N where begin and end
+// are tokens.  Where they do not ascend, begin may lie behind the token that a sequence was found for, or end in front of begin: who counts from one of them into a page of states checks that.
 struct Sequences {
     const void* offsets;
     int is64, N, T;
