@@ -10,6 +10,13 @@ DEV = "cuda"
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(params=[True, False], ids=["compiled", "python"])
+def host(request, monkeypatch):
+    """The operators through the compiled host module, and through the Python classes alone."""
+    if not request.param:
+        monkeypatch.setattr(_lib, "host", lambda: _lib._NoHost)
+
+
 # ---- the norm ------------------------------------------------------------------------------------------------------------
 
 def _borders(kind, C, unit):
@@ -49,6 +56,28 @@ def test_eight_bits_beside_an_infinity(C):
         others = torch.arange(C) != 3
         assert torch.isinf(scale).all() and not q.float().cpu()[:, others].any()
         assert torch.isnan(q[:, 3].float()).all() if kind != torch.int8 else not q[:, 3].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("contiguous", [True, False])
+def test_saved_rows_of_another_type_are_refused(host, contiguous, dtype):
+    """A hook on saved tensors that hands fp32 rows back where the forward kept 16 bits: refused without a residual; with one (whose sum may be either) the same gradients."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(6, 96, generator=g).to(DEV, dtype)
+    x = (x if contiguous else torch.cat([x, x], -1)[:, :96]).detach().requires_grad_()
+    w = (1 + 0.3 * torch.randn(96, generator=g)).to(DEV, dtype).requires_grad_()
+    res = torch.randn(6, 96, generator=g).to(DEV, dtype).requires_grad_()
+    gy = torch.randn(6, 96, generator=g).to(DEV, dtype)
+    hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t.float(), lambda t: t)
+    with hooks:
+        y = vr.rms_norm(x, w)
+    with pytest.raises(RuntimeError, match="saved tensors"):
+        torch.autograd.grad(y, [x, w], gy)
+    with hooks:
+        y, r = vr.rms_norm(x, w, res)
+    got = torch.autograd.grad([y, r], [x, w, res], [gy, gy])
+    want = torch.autograd.grad(vr.rms_norm(x, w, res), [x, w, res], [gy, gy])
+    assert all(a.dtype == dtype and torch.equal(a, b) for a, b in zip(got, want))
 
 
 # ---- offsets that do not ascend ------------------------------------------------------------------------------------------

@@ -90,7 +90,7 @@ class RMSNormFunction(torch.autograd.Function):
         shape, dtype, eps, has_residual = ctx.meta
         _check(r, "the saved sum")
         _check(weight, "weight", r)
-        if r.shape != shape or r.dtype not in (dtype, torch.float32) or tuple(weight.shape) != shape[-1:] or weight.dtype not in _DT:   # (hooks on saved tensors may have changed them)
+        if r.shape != shape or (r.dtype != dtype and not (has_residual and r.dtype == torch.float32)) or tuple(weight.shape) != shape[-1:] or weight.dtype not in _DT:   # (hooks on saved tensors may have changed them)
             raise RuntimeError("the saved tensors have other sizes or types than those of the call")
         if batched_cotangent(*(t for t in (gy, gr) if t is not None)):
             raise RuntimeError("rms_norm's gradients take one cotangent at a time")
