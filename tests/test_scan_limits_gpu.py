@@ -80,6 +80,21 @@ def test_saved_rows_of_another_type_are_refused(host, contiguous, dtype):
     assert all(a.dtype == dtype and torch.equal(a, b) for a, b in zip(got, want))
 
 
+# ---- the convolution -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("N", [(1 << 24) + 3, (1 << 26) + 5])
+def test_more_runs_than_a_launch_has_in_one_dimension(N):
+    """Sequences of one token, as many as there are waves: 2^22 workgroups and 2^24, which a launch's first dimension has no room for, and some more."""
+    x, state = (torch.arange(N, device=DEV, dtype=torch.int32).remainder_(k).sub_(k // 2).to(torch.bfloat16) for k in (251, 127))
+    w = torch.tensor([[0.5, 2.0]], device=DEV)
+    leaves = [t.requires_grad_() for t in (x.view(N, 1, 1), w, state.view(N, 1, 1))]
+    y, last = vr.causal_conv(leaves[0], leaves[1], state=leaves[2], return_state=True)
+    # (products and sums are exact in fp32: what is left is the one rounding)
+    assert torch.equal(y.view(N), (2 * x.float() + 0.5 * state.float()).bfloat16()) and torch.equal(last, leaves[0])
+    dx, dstate = torch.autograd.grad([y, last], [leaves[0], leaves[2]], [torch.ones_like(y), 3 * torch.ones_like(last)])
+    assert (dx == 5).all() and (dstate == 0.5).all()
+
+
 # ---- offsets that do not ascend ------------------------------------------------------------------------------------------
 
 class _Guarded:

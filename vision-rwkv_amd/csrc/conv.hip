@@ -32,15 +32,16 @@ __device__ __forceinline__ void last_states(const Params& p, long long first, lo
     }
 }
 
-// Waves of a workgroup take runs next to each other.  The last `extra` workgroups of x write the states.
+// Waves of a workgroup take runs next to each other.  The last `extra` workgroups write the states.  Workgroups go on in z where x ends: a launch's dimension has room for 2^24 of 256 threads.
+constexpr int GRID_X = 1 << 22;
 template <typename IO, int VEC, int KT>
-__global__ __launch_bounds__(THREADS) void forward_kernel(const Params p, int run_blocks) {
-    const int lane = threadIdx.x & 63;
-    if ((int)blockIdx.x >= run_blocks) {
-        if (blockIdx.y == 0) last_states<IO>(p, (blockIdx.x - run_blocks) * THREADS + threadIdx.x, (long long)(gridDim.x - run_blocks) * THREADS);
+__global__ __launch_bounds__(THREADS) void forward_kernel(const Params p, int run_blocks, int extra) {
+    const int lane = threadIdx.x & 63, block = blockIdx.z * GRID_X + blockIdx.x;
+    if (block >= run_blocks) {
+        if (blockIdx.y == 0 && block < run_blocks + extra) last_states<IO>(p, (long long)(block - run_blocks) * THREADS + threadIdx.x, (long long)extra * THREADS);
         return;
     }
-    const int number = blockIdx.x * (THREADS / WAVE) + (threadIdx.x >> 6);
+    const int number = block * (THREADS / WAVE) + (threadIdx.x >> 6);
     if (number >= p.rows * p.runs) return;
     Run r(p, __builtin_amdgcn_readfirstlane(number));
     Lane<IO, VEC, KT> my(p, blockIdx.y * WAVE + lane);
@@ -166,7 +167,7 @@ extern "C" int vrwkv_conv_fwd(const vrwkv_conv_args* args, void* hip_stream) {
         constexpr int VEC = decltype(v)::value;
         return with_taps(a.K, [&](auto k) {
             constexpr int KT = decltype(k)::value;
-            hipLaunchKernelGGL((forward_kernel<IO, VEC, KT>), dim3(blocks + extra, pl.waves), dim3(THREADS), 0, st, p, blocks);
+            hipLaunchKernelGGL((forward_kernel<IO, VEC, KT>), dim3(std::min(blocks + extra, GRID_X), pl.waves, (blocks + extra + GRID_X - 1) / GRID_X), dim3(THREADS), 0, st, p, blocks, extra);
             return check_launch(who);
         });
     });
