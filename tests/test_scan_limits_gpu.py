@@ -5,6 +5,7 @@ import torch
 
 import vision_rwkv_amd as vr
 from vision_rwkv_amd import _lib
+import test_selective_scan_gpu as scans
 
 DEV = "cuda"
 pytestmark = pytest.mark.gpu
@@ -93,6 +94,41 @@ def test_more_runs_than_a_launch_has_in_one_dimension(N):
     assert torch.equal(y.view(N), (2 * x.float() + 0.5 * state.float()).bfloat16()) and torch.equal(last, leaves[0])
     dx, dstate = torch.autograd.grad([y, last], [leaves[0], leaves[2]], [torch.ones_like(y), 3 * torch.ones_like(last)])
     assert (dx == 5).all() and (dstate == 0.5).all()
+
+
+# ---- the scan ------------------------------------------------------------------------------------------------------------
+
+def _same_kinds(x, gy, glast, segments):
+    """All results and gradients of a call have infinities and NaN where the recurrence in 64 bits has them, of the same sign, and the other numbers are its own."""
+    N, T, _ = x["u"].shape
+    leaves = {n: t.clone().requires_grad_() for n, t in x.items() if t is not None}
+    with vr.option("scan_segments", segments):
+        y, last = vr.selective_scan(**leaves, softplus=True, return_state=True)
+        grads = torch.autograd.grad([y, last], list(leaves.values()), [gy, glast])
+    want = scans.reference(x, [(n, 0, T) for n in range(N)], True, gy, glast)
+    for name, got in (("y", y), ("last", last), *((scans.NAMES[n], g) for n, g in zip(leaves, grads))):
+        v, (ref, scale) = got.detach().cpu().double(), want[name]
+        assert torch.equal(torch.isnan(v), torch.isnan(ref)), (name, torch.isnan(v).sum(), torch.isnan(ref).sum())
+        assert torch.equal(torch.isinf(v), torch.isinf(ref)) and torch.equal(torch.sign(v)[torch.isinf(v)], torch.sign(ref)[torch.isinf(v)]), name
+        fine = torch.isfinite(ref)
+        if fine.any():
+            scans.compare(got.detach().cpu()[fine], (ref[fine], scale[fine]), name, T, tokens=N * T)
+
+
+@pytest.mark.parametrize("segments", [1, 6])
+@pytest.mark.parametrize("S", [1, 3, 10, 20, 40])
+def test_an_infinite_gradient_beside_states_that_are_not_there(S, segments):
+    """A lane's states are filled up to four and a channel's to a power of two: what fills them up hands no NaN on.  All terms of a sum over states have one sign here, so that only
+    the definition's own infinities meet."""
+    x, normal = scans.inputs(2, 100, 20, S, 1, "fp32", state=2)
+    for n in ("u", "B", "C", "state", "z"):
+        x[n].abs_()
+    gy, glast = normal(2, 100, 20), normal(2, 20, S)
+    gy[0, 40, 3] = float("inf")
+    _same_kinds(x, gy, glast, segments)
+    gy[0, 40, 3] = 1
+    glast[1, 7] = float("inf")
+    _same_kinds(x, gy, glast, segments)
 
 
 # ---- offsets that do not ascend ------------------------------------------------------------------------------------------

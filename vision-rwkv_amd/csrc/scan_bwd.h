@@ -357,7 +357,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                         const f32x4 Bt = pairs.B[j % 2], Ct = pairs.C[j % 2];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const float r = fmaf(Ct[k], gj, R[k]);
+                            const float r = !FULL && pad[k] ? 0.f : fmaf(Ct[k], gj, R[k]);   // (an infinite gj would make it NaN, and with it what is summed over states)
                             dB[k] = r * v;
                             dC[k] = gj * hs[j + 1][k];
                             along_B[j % P] = fmaf(r, Bt[k], along_B[j % P]);
