@@ -131,6 +131,23 @@ def test_an_infinite_gradient_beside_states_that_are_not_there(S, segments):
     _same_kinds(x, gy, glast, segments)
 
 
+@pytest.mark.parametrize("segments", [1, 6])
+@pytest.mark.parametrize("E,S,G", [(20, 16, 1), (70, 16, 1), (40, 8, 2), (20, 32, 1), (20, 5, 1)])
+def test_an_infinity_in_the_channel_beside_those_that_are_not_there(E, S, G, segments):
+    """A workgroup's lanes behind its last channel read that channel once more: whatever it holds, they add nothing to the sums over channels."""
+    x, normal = scans.inputs(2, 100, E, S, G, "fp32", state=2)
+    for n in ("u", "B", "C", "state", "z"):
+        x[n].abs_()
+    x["D"].abs_()
+    gy, glast = normal(2, 100, E).abs(), normal(2, E, S).abs()
+    inf = float("inf")
+    for name, place in (("u", (0, 40, E - 1)), ("state", (1, E - 1)), ("glast", (1, E - 1)), ("delta", (0, 40, E // G - 1)), ("B", (0, 40)), ("C", (1, 50))):
+        changed = {n: t.clone() if t is not None else None for n, t in x.items()}
+        ends = glast.clone()
+        (ends if name == "glast" else changed[name])[place] = inf
+        _same_kinds(changed, gy, ends, segments)
+
+
 # ---- offsets that do not ascend ------------------------------------------------------------------------------------------
 
 class _Guarded:

@@ -192,8 +192,8 @@ template <typename IO, int P, bool FULL>
 __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
     const Params& p = bp.f;
     constexpr int OWN = BATCH / P, COUNT = 64 / P, ROW = 8 * P, SUMS = BATCH * ROW, WAVES = THREADS / WAVE;
-    constexpr bool KEEP = P <= 4;                          // (two workgroups a compute unit with 75 KB each; more lanes a channel have more sums in LDS: no room)
-    __shared__ __attribute__((aligned(16))) float bc[SUMS];
+    constexpr bool KEEP = P <= 4;                          // (two workgroups a compute unit with 76 KB each; more lanes a channel have more sums in LDS: no room)
+    __shared__ __attribute__((aligned(16))) float bc[2 * SUMS];   // the second half: zeros
     __shared__ float red[WAVES][SUMS];
     __shared__ f32x4 decays[KEEP ? BATCH : 1][THREADS];    // of the sixteen tokens, from the way along them for the way back
     const Place<P> at(p.E, p.G, p.blocks);
@@ -206,15 +206,18 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         pad[k] = !FULL && 4 * at.p + k >= p.S;
-        a2[k] = pad[k] ? 0.f : p.A[(long long)e * p.S + 4 * at.p + k] * LOG2E;
+        a2[k] = pad[k] || !at.there ? 0.f : p.A[(long long)e * p.S + 4 * at.p + k] * LOG2E;
     }
+    // A lane whose channel is not there adds exact zeros to dB and dC, whatever the channel holds that it reads in place of its own: no step, no states, B and C from the zeros.
+    for (int i = threadIdx.x; i < SUMS; i += THREADS) bc[SUMS + i] = 0.f;
+    const int row_bc = at.p + (at.there ? 0 : SUMS / 4);
     const float bias = p.bias.p ? p.bias.value(p.bias.fetch(e)) : 0.f, skip = p.D.p ? p.D.value(p.D.fetch(e)) : 0.f;
     const auto state_of = [&](const float* t, int n, float (&h)[4]) {
         const auto& p = arguments<BackParams>().f;
         int e = at.e;
         asm volatile("" : "+v"(e));                        // (no address of this is kept)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = t && !pad[k] ? t[((long long)n * p.E + e) * p.S + 4 * at.p + k] : 0.f;
+        for (int k = 0; k < 4; ++k) h[k] = t && !pad[k] && at.there ? t[((long long)n * p.E + e) * p.S + 4 * at.p + k] : 0.f;
     };
     const auto first_gradient = [&](int n, const float (&h)[4]) {
         const auto& bp = arguments<BackParams>();
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                 for (int i = 0; i < 4; ++i) R[i] = decayed(R[i], dt, a2[i]) + x[i];
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) R[i] = pad[i] ? 0.f : R[i];   // (an infinite step size makes what is not there NaN)
+            for (int i = 0; i < 4; ++i) R[i] = pad[i] || !at.there ? 0.f : R[i];   // (an infinite step size makes what is not there NaN)
         }
         // sixteen tokens' rows and their first state: asked for while the sums of those behind them are added up
         Rows<IO, P> raw;
@@ -278,9 +281,9 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
                 const float d = to_f32(raw.d[i]) + bias;
-                dt[i] = p.softplus ? softplus(d) : d;
+                dt[i] = !at.there ? 0.f : p.softplus ? softplus(d) : d;
                 bend[i] = p.softplus ? sigmoid(d) : 1.f;
-                u[i] = at.there ? to_f32(raw.u[i]) : 0.f;  // (a channel that is not there adds nothing to dB and dC)
+                u[i] = at.there ? to_f32(raw.u[i]) : 0.f;
                 g[i] = at.there ? to_f32(raw.g[i]) : 0.f;
                 if (p.z) {
                     const float z = to_f32(raw.z[i]), sg = sigmoid(z);
@@ -303,14 +306,14 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) hs[0][k] = h[k];
                 Pairs<P, 2, !PART> pairs;
-                pairs.start(bc, 0, at.p);
+                pairs.start(bc, 0, row_bc);
                 each(std::make_integer_sequence<int, OWN>(), [&](auto i_) {
                     constexpr int i = decltype(i_)::value;
                     float y[P];
                     each(std::make_integer_sequence<int, P>(), [&](auto q_) {
                         constexpr int q = decltype(q_)::value, j = i * P + q;
                         y[q] = 0.f;
-                        if (j % 2 == 0) pairs.advance(bc, j / 2, j / 2 + 1, at.p);
+                        if (j % 2 == 0) pairs.advance(bc, j / 2, j / 2 + 1, row_bc);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) hs[j + 1][k] = hs[j][k];
                         if (outside(j)) return;
@@ -333,7 +336,7 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
                     }
                 });
                 // (B and C are read again, and the exponentials come from LDS: kept, they would fill three times as many registers as the states)
-                int again = at.p;
+                int again = row_bc;
                 asm volatile("" : "+v"(again));
 #pragma unroll
                 for (int i = 0; i < OWN; ++i) asm volatile("" : "+v"(dt[i]));
@@ -419,7 +422,9 @@ __global__ __launch_bounds__(THREADS, 2) void back_kernel(const BackParams bp) {
             for (;;) {                                     // one sequence in front of the other
                 const int first = max(max(row, from), w.begin), behind = min(min(row + BATCH, to), w.end);
                 if (first >= behind) break;
-                float h[4] = {kept[0], kept[1], kept[2], kept[3]};
+                float h[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h[k] = at.there ? kept[k] : 0.f;
                 if (behind == w.end) state_of(bp.glast, w.n, R);
                 if (first == w.begin) state_of(p.state, w.n, h);
                 if (behind - first == BATCH) piece(std::false_type(), first, behind, h);
