@@ -28,20 +28,22 @@ struct BackParams {
 // Sums over the lanes of a wave that differ above the channel's P: of v[0 .. 64 / P) of all channels, one is left in each lane of v[0], the one that sum_of_lane says.  At each step
 // a lane keeps one half of its sums and gets the other lanes' parts of it.  Lanes of a row of sixteen first, in additions that read one lane and write another (4.4 cycles each,
 // measured; two make a pair of sums), then rows, whose swap takes 10.
+// Written out: the instruction's bank mask picks the half.  Two wait states in front of and behind reads across lanes; a sum is written before the last of the other operands is read, so that none of
+// them may share a register with it, whatever values are known to be equal.
 template <int HALF>
-__device__ __forceinline__ void fold8(float* v) {          // (written out: the instruction's bank mask picks the half; two wait states in front of and behind reads across lanes)
+__device__ __forceinline__ void fold8(float* v) {
     if constexpr (HALF == 8)
         asm("s_nop 1\n"
 #define FOLD(a, b) "v_add_f32_dpp %" #a ", %" #a ", %" #a " row_ror:8 row_mask:0xf bank_mask:0x3\n v_add_f32_dpp %" #a ", %" #b ", %" #b " row_ror:8 row_mask:0xf bank_mask:0xc\n"
             FOLD(0, 8) FOLD(1, 9) FOLD(2, 10) FOLD(3, 11) FOLD(4, 12) FOLD(5, 13) FOLD(6, 14) FOLD(7, 15) "s_nop 1"
-            : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7])
+            : "+&v"(v[0]), "+&v"(v[1]), "+&v"(v[2]), "+&v"(v[3]), "+&v"(v[4]), "+&v"(v[5]), "+&v"(v[6]), "+&v"(v[7])
             : "v"(v[8]), "v"(v[9]), "v"(v[10]), "v"(v[11]), "v"(v[12]), "v"(v[13]), "v"(v[14]), "v"(v[15]));
     else
 #pragma unroll
         for (int i = 0; i < HALF; i += 4)
             asm("s_nop 1\n" FOLD(0, 4) FOLD(1, 5) FOLD(2, 6) FOLD(3, 7) "s_nop 1"
 #undef FOLD
-                : "+v"(v[i]), "+v"(v[i + 1]), "+v"(v[i + 2]), "+v"(v[i + 3])
+                : "+&v"(v[i]), "+&v"(v[i + 1]), "+&v"(v[i + 2]), "+&v"(v[i + 3])
                 : "v"(v[i + HALF]), "v"(v[i + HALF + 1]), "v"(v[i + HALF + 2]), "v"(v[i + HALF + 3]));
 }
 template <int HALF>
@@ -52,7 +54,7 @@ __device__ __forceinline__ void fold4(float* v) {
 #define FOLD(a, b) "v_add_f32_dpp %" #a ", %" #a ", %" #a " row_shl:4 row_mask:0xf bank_mask:0x5\n v_add_f32_dpp %" #a ", %" #b ", %" #b " row_shr:4 row_mask:0xf bank_mask:0xa\n"
             FOLD(0, 4) FOLD(1, 5) FOLD(2, 6) FOLD(3, 7) "s_nop 1"
 #undef FOLD
-            : "+v"(v[i]), "+v"(v[i + 1]), "+v"(v[i + 2]), "+v"(v[i + 3])
+            : "+&v"(v[i]), "+&v"(v[i + 1]), "+&v"(v[i + 2]), "+&v"(v[i + 3])
             : "v"(v[i + HALF]), "v"(v[i + HALF + 1]), "v"(v[i + HALF + 2]), "v"(v[i + HALF + 3]));
 }
 template <int HALF, bool ROWS>
