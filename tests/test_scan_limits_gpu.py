@@ -81,6 +81,21 @@ def test_saved_rows_of_another_type_are_refused(host, contiguous, dtype):
     assert all(a.dtype == dtype and torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("C", [64, 2048, 70])
+def test_rows_whose_mean_square_is_subnormal(host, C):
+    """eps may be zero: a mean of squares below 2^-126 still has its root.  2e-20 squared is 4e-40, 285 000 steps of 2^-149: each square is off by 2^-19 of itself at most, the root by half of
+    that (2^-20), C / 64 + 24 half steps of fp32 beside it."""
+    x = torch.where(torch.arange(4 * C).view(4, C) % 3 == 1, -2e-20, 2e-20).to(DEV)
+    w = torch.linspace(0.5, 2, C, device=DEV)
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    y = vr.rms_norm(*leaves, eps=0.0)
+    bound = 2.0 ** -20 + (C / 64 + 24) * 2.0 ** -24
+    want = torch.sign(x.detach()).double() * w.detach().double()
+    assert ((y.detach().double() - want).abs() <= bound * want.abs()).all()
+    dw = torch.autograd.grad(y, w, torch.sign(x.detach()))[0]
+    assert ((dw.double() - 4).abs() <= 4 * bound).all()
+
+
 # ---- the convolution -----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("N", [(1 << 24) + 3, (1 << 26) + 5])

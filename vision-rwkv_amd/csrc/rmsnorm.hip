@@ -51,10 +51,12 @@ __device__ __forceinline__ float larger(float m, float v) {
     const float a = fabsf(v);
     return a != a || a > m ? a : m;
 }
-// 1 / sqrt to one unit in the last place: the approximation and one Newton step (an infinite or zero argument stays what the approximation makes of it)
+// 1 / sqrt to one unit in the last place: the approximation, which takes subnormal numbers for zeros (hence the powers of two), and one Newton step (an infinite or zero argument stays what the
+// approximation makes of it)
 __device__ __forceinline__ float inverse_root(float v) {
-    const float s = __builtin_amdgcn_rsqf(v), t = s * fmaf(-0.5f * v, s * s, 1.5f);
-    return fabsf(t) < 1e38f && v >= 1e-30f ? t : s;
+    const bool small = v < 0x1p-100f;
+    const float x = small ? v * 0x1p96f : v, s = __builtin_amdgcn_rsqf(x), t = s * fmaf(-0.5f * x, s * s, 1.5f);
+    return (fabsf(t) < 1e38f ? t : s) * (small ? 0x1p48f : 1.f);
 }
 
 __device__ __forceinline__ float top_of(int kind) { return kind == VRWKV_Y_INT8 ? 127.f : 448.f; }
