@@ -388,7 +388,8 @@ int vrwkv_copy_pages(void* pool, long long stride, int P, const void* source, lo
  * Token tensors are rows of E channels side by side at any strides (in elements) of batch and token (token: less than 2^22), of one dtype; sequences as in
  * vrwkv_decay_args: N rows of T tokens, or with offsets (N + 1, 32 or 64 bits, on the device, ascending from 0) N sequences packed in T rows, strides of batch not looked at;
  * outputs and gradients of packed rows that belong to no sequence are zeros, what such rows hold does not matter.  Sums and states are fp32.  At most 2^22 - 64 channels, 2^16 groups,
- * rows of less than 2^30 tokens, 65535 of them (the convolution: less than 2^30 times eight tokens in all); less than 2^30 rows of a step, 2^31 of the norm.
+ * rows of less than 2^30 tokens, 65535 of them (the convolution: rows of less than 2^30 times eight tokens in all, each row's tokens rounded up to eight), less than 2^30 sequences packed; less than
+ * 2^30 rows of a step; of the norm less than 2^31 rows of at most 2^31 - 256 channels, 2^27 - 32 where dweight is asked for.
  *
  * h_t = exp(dt_t A) h_{t-1} + dt_t u_t B_t^T, y_t = (C_t h_t + D u_t) silu(z_t) for each of the E channels, with dt = delta + delta_bias, softplus of that where `softplus`.
  * A: (E, S) contiguous fp32, S 1 to 64; B, C: rows of G groups of S states side by side, strides of batch, token and group; channel e reads group e / (E / G).

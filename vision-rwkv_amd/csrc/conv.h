@@ -176,7 +176,7 @@ int check(const char* who, const vrwkv_conv_args* args, bool backward) {
         set_error("%s: tokens must be less than 2^22 elements apart", who);
         return VRWKV_UNSUPPORTED_SHAPE;
     }
-    if (a.T >= 1 << 30 || a.E > (1 << 22) - WAVE || (!a.offsets && (long long)a.N * ((a.T + 7) / 8) >= 1LL << 30)) { set_error("%s: too many tokens or channels", who); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (a.T >= 1 << 30 || a.N >= 1 << 30 || a.E > (1 << 22) - WAVE || (!a.offsets && (long long)a.N * ((a.T + 7) / 8) >= 1LL << 30)) { set_error("%s: too many tokens, sequences or channels", who); return VRWKV_UNSUPPORTED_SHAPE; }
     bool fits = aligned(a.x, a.dtype) && aligned(a.state, a.dtype) && aligned(a.y, a.dtype) && aligned(a.last, a.dtype) && aligned(a.weight, a.param_dtype) && aligned(a.bias, a.param_dtype) &&
                 (!a.offsets || ((size_t)a.offsets & (a.offsets64 ? 7 : 3)) == 0);
     if (backward)

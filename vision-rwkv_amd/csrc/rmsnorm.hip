@@ -419,6 +419,9 @@ int check(const char* who, const vrwkv_rmsnorm_args* args, bool backward) {
     }
     if (a.out_kind < VRWKV_Y_SAME || a.out_kind > VRWKV_Y_INT8) { set_error("%s: unknown kind of output %d", who, a.out_kind); return VRWKV_INVALID_ARG; }
     if (a.rows >= 1LL << 31) { set_error("%s: 2^31 rows or more", who); return VRWKV_UNSUPPORTED_SHAPE; }
+    // (a thread's next channel has to stay within an int; the launch that ends the sums of dweight has room for 2^27 columns)
+    const int most = backward && a.dweight ? (1 << 27) - 32 : 0x7fffffff - 255;
+    if (a.C > most) { set_error("%s: more than %d channels", who, most); return VRWKV_UNSUPPORTED_SHAPE; }
     const size_t e = size_of(a.dtype) - 1, re = size_of(a.residual_dtype) - 1, we = size_of(a.weight_dtype) - 1;
     if ((((size_t)a.x | (size_t)a.gy | (size_t)a.dx) & e) || (((size_t)a.residual | (size_t)a.sum | (size_t)a.gsum | (size_t)a.dresidual) & re) || (((size_t)a.weight | (size_t)a.dweight) & we) ||
         (a.out_kind == VRWKV_Y_SAME && ((size_t)a.y & e)) || ((size_t)a.scale & 3) || ((size_t)a.workspace & 15)) {

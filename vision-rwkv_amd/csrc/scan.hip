@@ -80,7 +80,7 @@ int check(const char* who, const vrwkv_scan_args* args, bool backward) {
     for (long long s : strides)
         if (s < 0 || s >= 1LL << 22) { set_error("%s: tokens must be less than 2^22 elements apart", who); return VRWKV_UNSUPPORTED_SHAPE; }
     const Plan p = plan_of(a);
-    if (a.T >= 1 << 30 || p.rows > 65535 || (long long)a.G * p.blocks >= 1 << 24) { set_error("%s: at most 65535 rows of less than 2^30 tokens", who); return VRWKV_UNSUPPORTED_SHAPE; }
+    if (a.T >= 1 << 30 || a.N >= 1 << 30 || p.rows > 65535 || (long long)a.G * p.blocks >= 1 << 24) { set_error("%s: at most 65535 rows of less than 2^30 tokens, less than 2^30 sequences", who); return VRWKV_UNSUPPORTED_SHAPE; }
     bool fits = aligned(a.u, a.dtype) && aligned(a.delta, a.dtype) && aligned(a.B, a.dtype) && aligned(a.C, a.dtype) && aligned(a.z, a.dtype) && aligned(a.D, a.D_dtype) &&
                 aligned(a.delta_bias, a.bias_dtype) && (((size_t)a.A | (size_t)a.state | (size_t)a.last) & 3) == 0 && (((size_t)a.kept | (size_t)a.workspace) & 15) == 0 &&
                 (!a.offsets || ((size_t)a.offsets & (a.offsets64 ? 7 : 3)) == 0);
