@@ -119,7 +119,6 @@ __global__ __launch_bounds__(W * WAVE) void short_kernel(const Params p, const i
 #pragma unroll
         for (int k = 0; k < NS; ++k) h[k] = 0.f;
         const int back = anew ? 63 - __builtin_clzll(anew) : 0;
-#pragma unroll 2
         for (int i = wave - 1; i >= back; --i) {
 #pragma unroll
             for (int k = 0; k < NS; ++k) add(k, ends[buf][i][k][lane]);
