@@ -4,7 +4,8 @@
 //     dx_t = sum_j w_j g_{t + (K-1) - j}           dw_j = sum_t g_t x_{t - (K-1) + j}          db = sum_t g_t
 //
 // Bound by the memory: each row is read once and written once.  A lane holds VEC channels and goes along a run of tokens with the last K - 1 rows in registers, the next rows on their
-// way; the K - 1 rows in front of a run are read again (from L2).  64 x 196 tokens of 1536 channels in bf16: forward 19.6 us (3.9 TB/s), gradients 37 (3.1).  A sequence's first state stands for K - 1 tokens in front of it, in both directions.
+// way; the K - 1 rows in front of a run are read again (from L2).  64 x 196 tokens of 1536 channels in bf16: forward 19.6 us (3.9 TB/s), gradients 37 (3.1); from
+// five taps on, whose weights are read one at a time, 43 (5), 56 (6) and 65 (8), and a call of the gradients 79 to 93 for 53.  A sequence's first state stands for K - 1 tokens in front of it, in both directions.
 #pragma once
 #include "sequences.h"
 #include <algorithm>

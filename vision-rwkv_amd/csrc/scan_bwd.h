@@ -7,8 +7,10 @@
 // four states each, as in the forward.  dB and dC add up channels, which lie in other lanes: the sums of two tokens go through the wave in halves
 // (two instructions for a sum of 64 / P lanes), then through LDS over the waves, and over workgroups by the launch that ends the pass.
 //
-// 64 x 196 tokens of 1536 channels with 16 states, bf16: 340 us, bound by the instructions (110 a token and wave) with the registers of two waves a vector unit.  Three waves, with states held of
-// eight tokens at a time and the eight in front of them gone through twice, took as long as two (366 and 370 before the decays were kept in LDS), four 465.
+// 64 x 196 tokens of 1536 channels with 16 states, bf16: 323 us with the sums that end the pass (9 of them), 640 cycles a token and wave.  Its 110 instructions account for about 510 of these; what is
+// left is waiting that the two waves a vector unit, for which there are registers, do not hide.  Three waves, with states held of eight tokens at a time and the eight in front of them gone through twice,
+// took as long as two (366 and 370 before the decays were kept in LDS), four 465.  4, 8, 32 and 64 states: 245, 238, 643 and 1382 (up to 8 states the registers overflow by nine; from 17 on the sums over
+// channels that go through memory grow with the square of the states).
 #pragma once
 #include "scan.h"
 

@@ -1,7 +1,7 @@
 // One more token for each of N sequences whose states are pages of a pool: h = exp(dt A) h + dt u B, y = (C h + D u) silu(z), h written back (gfx950).
 // Bound by the pages, read and written once: P lanes hold four states each of NC channels, 16 bytes a lane and channel.  A workgroup takes its channels of R rows, one after the other, with the
 // next row's page on its way: A, as large as a page, comes from L2 once for the R.  Two channels and four rows where that leaves four workgroups a compute unit, else one and one.
-// 512 rows of 1536 x 16 states, 101 MB: 23.5 us (4.5 TB/s) where the last-level cache holds the pools (three of 63 MB in turn), 34.6 where it does not (eight); with loads and stores past the
+// 512 rows of 1536 x 16 states, 101 MB: 23.5 us (4.5 TB/s) where the last-level cache holds the pools (three of 63 MB in turn), 31 to 35 where it does not (eight); with loads and stores past the
 // caches 32 in both.  One channel and one row: 42.  One row alone: 3.9.
 #include "scan.h"
 #include "pages.h"

@@ -386,7 +386,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     offsets (N + 1,), int32 or int64 on the device, ascending from 0 to T: N sequences packed behind each other in one row (B = 1), sequence n the tokens
     offsets[n] to offsets[n + 1] (an empty one leaves its state as it is); y of rows behind the last sequence is zero, and so are their gradients.
     Gradients for all of them, sums in fp32, rounded once to their inputs' types; a call that records keeps the states in front of every sixteenth token for them (S / 16
-    fp32 numbers a channel and token).  No second gradients, no forward mode, no tracing (a compiled program makes the call as it is)."""
+    fp32 numbers a channel and token, S rounded up to 8, 16, 32 or 64).  No second gradients, no forward mode, no tracing (a compiled program makes the call as it is)."""
     if torch.compiler.is_compiling():
         return _eager(selective_scan)(u, delta, A, B, C, D, z, delta_bias, softplus, state, offsets, return_state)
     out = _lib.host().selective_scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, offsets, return_state)
