@@ -238,3 +238,36 @@ def test_scan_of_disordered_offsets_stays_in_its_tensors(E, S, segments, force):
             assert call(a, None) == 0
         torch.cuda.synchronize()
         assert new.untouched(), first
+
+
+@pytest.mark.parametrize("segments", [0, 1, 6])
+def test_other_lengths_on_each_replay(segments, force):
+    """Packed sequences in a graph, forward and back, whose offsets change from replay to replay: what eager calls give, to the bit."""
+    force("scan_segments", segments)
+    T, E, S, K, N = 420, 72, 16, 4, 5
+    x, normal = scans.inputs(1, T, E, S, 1, "bf16", state=N)
+    taps, w = normal(N, K - 1, E).bfloat16(), normal(E, K)
+    leaves = [t.requires_grad_() for t in (*x.values(), taps, w)]
+    offsets = torch.tensor([0, 100, 130, 130, 300, 420], device=DEV)
+    grads = normal(1, T, E).bfloat16(), normal(N, E, S), normal(N, K - 1, E).bfloat16()
+
+    def call():
+        c, tail = vr.causal_conv(x["u"], w, None, "silu", state=taps, offsets=offsets, return_state=True)
+        y, last = vr.selective_scan(**{**x, "u": c}, softplus=True, offsets=offsets, return_state=True)
+        return [c.detach(), tail.detach(), y.detach(), last.detach(), *torch.autograd.grad([y, last, tail], leaves, list(grads))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = call()
+    for first in ([0, 100, 130, 130, 300, 420], [0, 0, 0, 0, 0, 420], [5, 21, 37, 53, 54, 60], [0, 400, 401, 402, 403, 404], [420] * 6, [1, 2, 3, 4, 5, 6]):
+        offsets.copy_(torch.tensor(first))
+        graph.replay()
+        torch.cuda.synchronize()
+        for n, (p, q) in enumerate(zip(recorded, call())):
+            assert torch.equal(p, q), (first, n)
