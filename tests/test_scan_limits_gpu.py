@@ -271,3 +271,37 @@ def test_other_lengths_on_each_replay(segments, force):
         torch.cuda.synchronize()
         for n, (p, q) in enumerate(zip(recorded, call())):
             assert torch.equal(p, q), (first, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pages_and_rows_further_apart_than_32_bits(dtype):
+    """Pages and batch rows more than 2^31 elements from each other: the same as of tensors next to each other, in place and out, gradients too."""
+    g, far, E, S, K, T = torch.Generator().manual_seed(3), (1 << 31) + 40, 24, 16, 4, 9
+    normal = lambda *s: torch.randn(*s, generator=g).to(DEV)
+    space = torch.empty(2 * far + 4096, dtype=torch.float32, device=DEV)
+
+    def apart(t, offset=0):
+        """t (n, ..) with its rows `far` elements apart."""
+        v = space.view(torch.uint8)[:(space.numel() // 4 * 4) * t.element_size()].view(t.dtype)
+        v = v.as_strided(t.shape, (far, *t[0].contiguous().stride()), offset)
+        return v.copy_(t)
+
+    u, delta, z, B, C = normal(2, T, E).to(dtype), normal(2, T, E).to(dtype), normal(2, T, E).to(dtype), normal(2, T, S).to(dtype), normal(2, T, S).to(dtype)
+    A, w = -normal(E, S).abs(), normal(E, K).to(dtype)
+    near = [u, delta, z, B, C]
+    split = [apart(t, 512 * i) for i, t in enumerate(near)]
+    results = []
+    for u_, delta_, z_, B_, C_ in (near, split):
+        leaves = [t.detach().requires_grad_() for t in (u_, delta_, z_, B_, C_)]
+        y, last = vr.selective_scan(leaves[0], leaves[1], A, leaves[3], leaves[4], z=leaves[2], softplus=True, return_state=True)
+        c, tail = vr.causal_conv(leaves[0], w, None, "silu", return_state=True)
+        results.append([y, last, c, tail, *torch.autograd.grad([y, last, c, tail], leaves, [torch.ones_like(v) for v in (y, last, c, tail)])])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    states, taps = normal(3, E, S), normal(3, K - 1, E).to(dtype)
+    slots = torch.tensor([2, 0], device=DEV)
+    for pool, other, f in ((states, apart(states), lambda p: vr.selective_scan_step(u[:, 0], delta[:, 0], A, B[:, 0], C[:, 0], p, slots, z=z[:, 0], softplus=True)),
+                           (taps, apart(taps), lambda p: vr.causal_conv_step(u[:, 0], w, p, slots, activation="silu"))):
+        other.copy_(pool)
+        assert torch.equal(f(pool), f(other)) and torch.equal(pool, other)
+    x = normal(3, 768).to(dtype)
+    assert torch.equal(vr.rms_norm(x, torch.ones(768, device=DEV)), vr.rms_norm(apart(x), torch.ones(768, device=DEV)))
